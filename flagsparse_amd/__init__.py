@@ -1,11 +1,12 @@
 """flagsparse_amd - MI355X (gfx950) CSR/COO SpMV, CSR/COO SpMM and CSR SDDMM behind FlagSparse's
-API.
+API, and attention over sequences that are rows of a CSR pattern.
 
 Drop-in for the hot path of the reference package ``flagsparse`` (src/flagsparse/__init__.py):
 the names below keep the reference's signatures, defaults, return values and exceptions.
 Names of the reference that lie outside this path (gather/scatter, SpSV, SpGEMM and the
 CuPy-backed format containers) are listed in ``__all__`` as in the reference; calling them
-raises NotImplementedError.
+raises NotImplementedError.  The names of ATTENTION_EXPORTS are this package's own: the reference
+has no counterpart, so they are not in ``__all__``, which is the reference's.
 
     import flagsparse_amd as flagsparse
     p = flagsparse.prepare_spmv_csr(data, indices, indptr, shape)
@@ -15,6 +16,16 @@ raises NotImplementedError.
 __version__ = "1.0.0"
 
 from ._common import SUPPORTED_INDEX_DTYPES, SUPPORTED_VALUE_DTYPES  # noqa: F401
+from .attention import (
+    PreparedAttention,
+    PreparedPagedKV,
+    flagsparse_attention_packed,
+    flagsparse_attention_packed_backward,
+    flagsparse_attention_paged,
+    flagsparse_paged_append,
+    prepare_attention_packed,
+    prepare_paged_kv,
+)
 from .benchmarks import benchmark_spmv_case
 from .spmm_csr import (
     PreparedCsrSpmmOpt,
@@ -58,6 +69,18 @@ HOT_PATH_EXPORTS = (
     "benchmark_spmm_opt_case",
     "comprehensive_spmm_test",
     "benchmark_spmv_case",
+)
+
+# Attention over packed sequences and a paged cache (no reference counterpart).
+ATTENTION_EXPORTS = (
+    "PreparedAttention",
+    "PreparedPagedKV",
+    "prepare_attention_packed",
+    "prepare_paged_kv",
+    "flagsparse_attention_packed",
+    "flagsparse_attention_packed_backward",
+    "flagsparse_attention_paged",
+    "flagsparse_paged_append",
 )
 
 # Reference exports outside the SpMV / SpMM path (src/flagsparse/__init__.py:5-63).

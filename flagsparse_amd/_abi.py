@@ -15,8 +15,10 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "lib
 
 FSP_F32 = 0
 FSP_F64 = 1
+FSP_BF16 = 2
+FSP_F16 = 3
 FSP_CUT_PIECES = 2
-ABI_VERSION = 19
+ABI_VERSION = 20
 
 _lib = None
 
@@ -116,6 +118,13 @@ SIGNATURES = {
     "fsp_bind_spmm_sliced": (_i32, [_p, _i32, _i32, _p, _p, _p, _i32, _i64, _i64, _i64, _p, _p,
                                     _i64, _i64, _p, _i32, _i32, _i32, _i32]),
     "fsp_run": (_i32, [_p, _p, _p, _p]),
+    "fsp_attention_dim_cap": (_i64, []),
+    "fsp_paged_append": (_i32, [_p, _p]),
+    "fsp_attention_paged_workspace": (_i64, [_p]),
+    "fsp_attention_paged": (_i32, [_p, _p]),
+    "fsp_attention_packed_tile": (_i64, []),
+    "fsp_attention_packed": (_i32, [_p, _p]),
+    "fsp_attention_packed_backward": (_i32, [_p, _p]),
 }
 
 

@@ -1,0 +1,620 @@
+"""Attention over packed sequences and over a paged cache on gfx950.
+
+Sequences of different lengths are rows of a CSR pattern: ``indptr`` over the tokens of a packed
+batch, or over the pages that a cache holds of each sequence (``indices``: the pages).
+
+* ``flagsparse_paged_append``: new keys and values, rotated by their positions, into the cache;
+* ``flagsparse_attention_paged``: one new query per sequence over all that the cache holds of it;
+* ``flagsparse_attention_packed`` and ``..._backward``: whole sequences, packed one after the other,
+  causal, with a sliding window, or between two batches of sequences; with its gradient.
+
+Queries, keys and values are [tokens, heads, dim] in bfloat16 or float16, ``dim`` a multiple of 8 up
+to 128; the query heads are shared out evenly over the key heads.  Where query i sees the keys j,
+S_ij = scale * q_i . k_j, lse_i = log(sum_j exp(S_ij)) and out_i = sum_j exp(S_ij - lse_i) v_j; a query that
+sees no key has an output of zeros and an lse of minus infinity.  Everything is summed in 32 bits and
+every sum has a fixed order: equal calls give equal results, bit for bit.
+
+As with the sparse products, ``prepare_*`` checks index arrays once (the host waits for them) and
+the calls with ``prepared=`` neither check them again nor wait: they can be captured in a graph.
+"""
+
+import struct
+
+import numpy as np
+import torch
+
+from . import _abi
+from ._common import SUPPORTED_INDEX_DTYPES, _aligned
+from ._csr_check import _capturing, csr_check
+
+SUPPORTED_ATTENTION_DTYPES = (torch.bfloat16, torch.float16)
+
+_CODES = {torch.bfloat16: _abi.FSP_BF16, torch.float16: _abi.FSP_F16}
+_DIM_CAP = 128
+_TOKENS_CAP = 2**31 - 1
+
+# The argument structs of include/flagsparse_hip.h: 8-byte fields, "d" the scale.
+_CACHE = struct.Struct("7q 4q 4q 2q")
+_APPEND = struct.Struct("5q 3q 3q 3q 3q 4q")
+_PAGED = struct.Struct("2qd 3q 3q 3q")
+_PACKED = struct.Struct("8qd 4q 3q 3q 3q 3q q 3q 3q 3q 3q q")
+
+
+class _Streams:
+    """The streams that a prepared object's arrays are marked as used on (see mark); a copy's arrays
+    are other arrays, marked nowhere."""
+
+    __slots__ = ("seen",)
+
+    def __init__(self):
+        self.seen = set()
+
+    def __reduce__(self):
+        return _Streams, ()
+
+    def mark(self, stream, device, arrays):
+        """Marks the arrays as used on ``stream``, the current one, once: calls do not wait, so
+        without the mark the caching allocator could hand their memory out while a kernel of this
+        stream still reads it.  Not while a graph is captured: nothing runs then, and keeping the
+        prepared object for the replays is the caller's."""
+        if torch.cuda.is_current_stream_capturing():
+            return
+        current = torch.cuda.current_stream(device)
+        for t in arrays:
+            t.record_stream(current)
+        self.seen.add(stream)
+
+
+def _check_tensor(t, name, dtype=None, device=None, heads=None, dim=None):
+    if not torch.is_tensor(t):
+        raise TypeError(f"{name} must be a tensor")
+    if t.ndim != 3:
+        raise ValueError(f"{name} must be a 3D tensor [tokens, heads, dim]")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if t.dtype not in SUPPORTED_ATTENTION_DTYPES:
+        raise TypeError(f"{name} dtype must be torch.bfloat16 or torch.float16")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name} dtype must be {dtype}, got {t.dtype}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    if heads is not None and t.shape[1] != heads:
+        raise ValueError(f"{name} must have {heads} heads, got {t.shape[1]}")
+    if dim is not None and t.shape[2] != dim:
+        raise ValueError(f"{name} must have dim {dim}, got {t.shape[2]}")
+    if t.shape[0] > _TOKENS_CAP:
+        raise ValueError(f"{name} must have fewer than 2^31 tokens")
+
+
+def _check_dim(dim):
+    if dim < 8 or dim % 8 or dim > _DIM_CAP:
+        raise NotImplementedError(
+            f"dim {dim} has no gfx950 kernel in flagsparse_amd (multiples of 8 up to {_DIM_CAP})")
+
+
+def _check_heads(heads, kv_heads):
+    if kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise ValueError(f"query heads ({heads}) must be a multiple of key heads ({kv_heads})")
+
+
+def _rows(t):
+    """``t`` itself where the kernels can read it (contiguous last axis, 16-byte rows), else a
+    copy."""
+    s = t.stride()
+    if s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t
+    return _aligned(t.contiguous())
+
+
+def _scale_of(scale, dim):
+    return dim ** -0.5 if scale is None else float(scale)
+
+
+def _window_of(window):
+    if window is None:
+        return 0
+    window = int(window)
+    if window < 1:
+        raise ValueError("window must be a positive number of tokens, or None")
+    return min(window, _TOKENS_CAP)
+
+
+def _check_out(out, name, shape, dtype, device):
+    if not torch.is_tensor(out) or tuple(out.shape) != tuple(shape):
+        raise ValueError(f"{name} must be a tensor of shape {tuple(shape)}")
+    if not out.is_cuda or out.device != device:
+        raise ValueError(f"{name} must be a CUDA tensor on {device}")
+    if out.dtype != dtype:
+        raise TypeError(f"{name} dtype must be {dtype}")
+
+
+def _result(out, name, shape, dtype, device):
+    """(the array the kernel writes, whether ``out`` is to be copied from it)."""
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device), False
+    _check_out(out, name, shape, dtype, device)
+    s = out.stride()
+    if s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and out.data_ptr() % 16 == 0 and \
+            (s[0] or shape[0] < 2) and (s[1] or shape[1] < 2):
+        return out, False
+    return torch.empty(shape, dtype=dtype, device=device), True
+
+
+def _int32(t, name, length, device):
+    """A contiguous int32 device array of ``length``."""
+    if not torch.is_tensor(t) or t.ndim != 1 or t.numel() != length:
+        raise ValueError(f"{name} must be a 1D tensor of length {length}")
+    if not t.is_cuda or t.device != device:
+        raise ValueError(f"{name} must be a CUDA tensor on {device}")
+    if t.dtype not in SUPPORTED_INDEX_DTYPES:
+        raise TypeError(f"{name} dtype must be torch.int32 or torch.int64")
+    if t.dtype == torch.int64:
+        t = t.clamp(-1, _TOKENS_CAP).to(torch.int32)
+    return t.contiguous()
+
+
+# ---- the paged cache ----
+
+
+class PreparedPagedKV:
+    """A paged cache and its page table, checked once.
+
+    ``k_pages`` / ``v_pages`` are the caller's own arrays, read and written in place.  The page table
+    is a copy: a table that changes (another batch, more pages) is prepared anew.  ``room`` is the
+    most tokens that the pages of one sequence hold."""
+
+    __slots__ = ("k_pages", "v_pages", "indptr", "indices", "batch", "n_pages", "page_size",
+                 "kv_heads", "dim", "room", "_streams", "_bytes")
+
+    def __init__(self, k_pages, v_pages, indptr, indices, longest):
+        self.k_pages = k_pages
+        self.v_pages = v_pages
+        self.indptr = indptr
+        self.indices = indices
+        self.batch = indptr.numel() - 1
+        self.n_pages, self.page_size, self.kv_heads, self.dim = (int(n) for n in k_pages.shape)
+        self.room = int(longest) * self.page_size
+        self._streams = _Streams()
+        self._bytes = {}  # workspace of a decoding call, by number of heads
+
+    @property
+    def dtype(self):
+        return self.k_pages.dtype
+
+    @property
+    def device(self):
+        return self.k_pages.device
+
+    def _packed(self):
+        k, v = self.k_pages, self.v_pages
+        ks, vs = k.stride(), v.stride()
+        return _CACHE.pack(_CODES[k.dtype], self.kv_heads, self.dim, self.page_size, self.n_pages,
+                           self.batch, self.indices.numel(), k.data_ptr(), ks[0], ks[1], ks[2],
+                           v.data_ptr(), vs[0], vs[1], vs[2], self.indptr.data_ptr(),
+                           self.indices.data_ptr())
+
+    def _on(self, stream):
+        if stream not in self._streams.seen:
+            self._streams.mark(stream, self.device, (self.indptr, self.indices))
+
+
+def _check_pages(t, name):
+    if not torch.is_tensor(t):
+        raise TypeError(f"{name} must be a tensor")
+    if t.ndim != 4:
+        raise ValueError(f"{name} must be a 4D tensor [pages, page_size, heads, dim]")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if t.dtype not in SUPPORTED_ATTENTION_DTYPES:
+        raise TypeError(f"{name} dtype must be torch.bfloat16 or torch.float16")
+    if t.numel() and (t.stride(3) != 1 or any(n % 8 for n in t.stride()[:3]) or
+                      t.data_ptr() % 16):
+        raise ValueError(f"{name} must have a contiguous last axis and 16-byte aligned rows")
+
+
+def prepare_paged_kv(k_pages, v_pages, indptr, indices):
+    """Check a paged cache and its page table.
+
+    ``k_pages``, ``v_pages``: [pages, page_size, kv_heads, dim], any order of the first three axes
+    in memory.  Sequence b's tokens lie in pages ``indices[indptr[b]:indptr[b + 1]]``, in order; a
+    sequence may own more pages than it fills yet, and sequences may share pages that they only
+    read.  Returns a PreparedPagedKV for flagsparse_paged_append and flagsparse_attention_paged."""
+    _check_pages(k_pages, "k_pages")
+    _check_pages(v_pages, "v_pages")
+    if k_pages.shape != v_pages.shape:
+        raise ValueError("k_pages and v_pages must have the same shape")
+    if k_pages.dtype != v_pages.dtype:
+        raise TypeError("v_pages dtype must match k_pages dtype")
+    if k_pages.device != v_pages.device:
+        raise ValueError("k_pages and v_pages must be on the same CUDA device")
+    n_pages, page_size, kv_heads, dim = k_pages.shape
+    _check_dim(dim)
+    if page_size < 1 or kv_heads < 1:
+        raise ValueError("pages must hold at least one token and one head")
+    if n_pages * page_size > _TOKENS_CAP:
+        raise ValueError("the cache must hold fewer than 2^31 tokens")
+    for t, name in ((indptr, "indptr"), (indices, "indices")):
+        if not torch.is_tensor(t) or t.ndim != 1:
+            raise ValueError(f"{name} must be a 1D tensor")
+        if not t.is_cuda or t.device != k_pages.device:
+            raise ValueError(f"{name} must be a CUDA tensor on {k_pages.device}")
+        if t.dtype not in SUPPORTED_INDEX_DTYPES:
+            raise TypeError(f"{name} dtype must be torch.int32 or torch.int64")
+    if indptr.numel() < 1:
+        raise ValueError("indptr must have at least one entry")
+    if indices.numel() * page_size > _TOKENS_CAP:
+        raise ValueError("the page table must hold fewer than 2^31 tokens")
+    (first, last, decreases, longest, least, most), idx, ptr = csr_check(
+        indices.contiguous(), indptr.contiguous(), 32)
+    if first != 0:
+        raise ValueError("indptr[0] must be 0")
+    if last != indices.numel():
+        raise ValueError(f"indptr[-1] must equal the number of indices {indices.numel()}")
+    if decreases:
+        raise ValueError("indptr must be nondecreasing")
+    if indices.numel() and (least < 0 or most >= n_pages):
+        raise IndexError("indices out of range for the cache's pages")
+    # the prepared object's own: what the checks said of them stays true
+    if idx.data_ptr() == indices.data_ptr():
+        idx = idx.clone()
+    if ptr.data_ptr() == indptr.data_ptr():
+        ptr = ptr.clone()
+    torch.cuda.current_stream(k_pages.device).synchronize()  # calls may come from other streams
+    return PreparedPagedKV(k_pages, v_pages, ptr, idx, longest if indices.numel() else 0)
+
+
+def _paged_of(prepared, k_pages, v_pages, indptr, indices, lengths):
+    """The prepared cache of a call; one that is made for the call has its lengths checked too."""
+    if prepared is not None:
+        if not isinstance(prepared, PreparedPagedKV):
+            raise TypeError("prepared must be a PreparedPagedKV instance")
+        return prepared, _int32(lengths, "lengths", prepared.batch, prepared.device)
+    if any(t is None for t in (k_pages, v_pages, indptr, indices)):
+        raise ValueError("k_pages, v_pages, indptr and indices are required when prepared is not "
+                         "provided")
+    kv = prepare_paged_kv(k_pages, v_pages, indptr, indices)
+    n = _int32(lengths, "lengths", kv.batch, kv.device)
+    if kv.batch:
+        room = (kv.indptr[1:] - kv.indptr[:-1]) * kv.page_size
+        if bool(((n < 0) | (n > room)).any()):
+            raise ValueError("lengths must lie between 0 and what the sequences' pages hold")
+    return kv, n
+
+
+def flagsparse_paged_append(k, v, lengths, token_indptr=None, *, prepared=None, k_pages=None,
+                            v_pages=None, indptr=None, indices=None, q=None, cos=None, sin=None,
+                            interleaved=False, out=None):
+    """Write new keys and values into a paged cache, rotated by their positions on the way.
+
+    ``k``, ``v``: [tokens, kv_heads, dim], the new tokens of each sequence one after the other:
+    sequence b's are ``token_indptr[b]`` to ``token_indptr[b + 1]`` (None: one token per sequence).
+    ``lengths[b]`` is what sequence b holds with them, so its last token has position
+    ``lengths[b] - 1``.  ``cos``, ``sin``: float32 [positions, half]; the first 2 * half elements of
+    every head of ``k`` and ``q`` are rotated by pairs, (a, b) -> (a cos - b sin, a sin + b cos):
+    elements half apart, or neighbours with ``interleaved``.  Without them nothing is rotated.
+
+    Returns the rotated ``q`` [tokens, heads, dim] (written to ``out`` where given), or None
+    without ``q``.  The pages that new tokens go to belong to one sequence each.  With
+    ``prepared`` nothing is waited for, so lengths are not checked: a token whose position is
+    negative or past its sequence's pages is not stored and its row of ``q`` comes back as NaN."""
+    kv, n = _paged_of(prepared, k_pages, v_pages, indptr, indices, lengths)
+    dev, dt = kv.device, kv.dtype
+    _check_tensor(k, "k", dt, dev, kv.kv_heads, kv.dim)
+    _check_tensor(v, "v", dt, dev, kv.kv_heads, kv.dim)
+    tokens = k.shape[0]
+    if v.shape[0] != tokens:
+        raise ValueError(f"v must have {tokens} tokens, got {v.shape[0]}")
+    if token_indptr is None:
+        if tokens != kv.batch:
+            raise ValueError(f"k must have one token for each of {kv.batch} sequences, got "
+                             f"{tokens}; other numbers need token_indptr")
+    else:
+        token_indptr = _int32(token_indptr, "token_indptr", kv.batch + 1, dev)
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin come together")
+    half = rows = 0
+    if cos is not None:
+        for t, name in ((cos, "cos"), (sin, "sin")):
+            if not torch.is_tensor(t) or t.ndim != 2:
+                raise ValueError(f"{name} must be a 2D tensor [positions, half]")
+            if not t.is_cuda or t.device != dev:
+                raise ValueError(f"{name} must be a CUDA tensor on {dev}")
+            if t.dtype != torch.float32:
+                raise TypeError(f"{name} dtype must be torch.float32")
+        if cos.shape != sin.shape:
+            raise ValueError("cos and sin must have the same shape")
+        rows, half = (int(x) for x in cos.shape)
+        if 2 * half > kv.dim:
+            raise ValueError(f"cos and sin must have at most dim / 2 = {kv.dim // 2} columns")
+        cos, sin = cos.contiguous(), sin.contiguous()
+    heads, res, copied, rq = 0, None, False, None
+    if q is not None:
+        _check_tensor(q, "q", dt, dev, None, kv.dim)
+        if q.shape[0] != tokens:
+            raise ValueError(f"q must have {tokens} tokens, got {q.shape[0]}")
+        heads = q.shape[1]
+        res, copied = _result(out, "out", q.shape, dt, dev)
+        rq = _rows(q)
+    elif out is not None:
+        raise ValueError("out is for the rotated q")
+    if tokens and kv.batch:
+        k, v = _rows(k), _rows(v)
+        stream = _abi.raw_stream(dev)
+        kv._on(stream)
+        qa = (rq.data_ptr(), rq.stride(0), rq.stride(1), res.data_ptr(), res.stride(0),
+              res.stride(1)) if heads else (0, 0, 0, 0, 0, 0)
+        args = kv._packed() + _APPEND.pack(
+            tokens, heads, half, rows, bool(interleaved), k.data_ptr(), k.stride(0), k.stride(1),
+            v.data_ptr(), v.stride(0), v.stride(1), *qa, cos.data_ptr() if half else 0,
+            sin.data_ptr() if half else 0, 0 if token_indptr is None else token_indptr.data_ptr(),
+            n.data_ptr())
+        _abi.check(_abi.lib().fsp_paged_append(args, stream), "fsp_paged_append")
+    if copied:
+        out.copy_(res)
+        res = out
+    return res
+
+
+def flagsparse_attention_paged(q, lengths, *, prepared=None, k_pages=None, v_pages=None,
+                               indptr=None, indices=None, scale=None, window=None, out=None,
+                               return_lse=False):
+    """Attention of one query per sequence over what a paged cache holds of it.
+
+    ``q``: [sequences, heads, dim]; ``lengths[b]``: the tokens that sequence b holds, the query's
+    own among them (0: the sequence is empty, and its output is zeros).  ``window``: only the last
+    ``window`` tokens are seen.  ``scale``: dim ** -0.5 by default.  Returns [sequences, heads, dim],
+    with the float32 log-sum-exp [sequences, heads] if ``return_lse``.  With ``prepared`` nothing is
+    waited for, so lengths are not checked: one that its sequence's pages cannot hold gives NaN."""
+    kv, n = _paged_of(prepared, k_pages, v_pages, indptr, indices, lengths)
+    dev, dt = kv.device, kv.dtype
+    _check_tensor(q, "q", dt, dev, None, kv.dim)
+    if q.shape[0] != kv.batch:
+        raise ValueError(f"q must have one token for each of {kv.batch} sequences, got "
+                         f"{q.shape[0]}")
+    heads = q.shape[1]
+    _check_heads(heads, kv.kv_heads)
+    scale, window = _scale_of(scale, kv.dim), _window_of(window)
+    res, copied = _result(out, "out", q.shape, dt, dev)
+    lse = torch.empty((kv.batch, heads), dtype=torch.float32, device=dev) if return_lse else None
+    if kv.batch:
+        q = _rows(q)
+        stream = _abi.raw_stream(dev)
+        kv._on(stream)
+        L = _abi.lib()
+        cache = kv._packed()
+
+        def pack(workspace):
+            return cache + _PAGED.pack(
+                heads, window, scale, q.data_ptr(), q.stride(0), q.stride(1), res.data_ptr(),
+                res.stride(0), res.stride(1), 0 if lse is None else lse.data_ptr(), n.data_ptr(),
+                workspace)
+
+        need = kv._bytes.get(heads)
+        if need is None:
+            need = kv._bytes[heads] = int(L.fsp_attention_paged_workspace(pack(0)))
+        work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        _abi.check(L.fsp_attention_paged(pack(0 if work is None else work.data_ptr()), stream),
+                   "fsp_attention_paged")
+    if copied:
+        out.copy_(res)
+        res = out
+    return (res, lse) if return_lse else res
+
+
+# ---- packed sequences ----
+
+
+class PreparedAttention:
+    """The sequences of a packed batch, checked once, and the kernels' work lists over them: tiles of
+    one sequence's rows, those with the most to do first, so that the last ones to finish are
+    short."""
+
+    __slots__ = ("batch", "q_tokens", "k_tokens", "device", "_tiles", "_streams")
+
+    def __init__(self, q_len, k_len, device):
+        self.batch = len(q_len)
+        self.q_tokens = int(q_len.sum())
+        self.k_tokens = int(k_len.sum())
+        self.device = device
+        tile = int(_abi.lib().fsp_attention_packed_tile())
+        lists = [_tiles(q_len, k_len, tile, causal, keys)
+                 for keys in (False, True) for causal in (False, True)]
+        flat = torch.from_numpy(np.concatenate(lists)).to(device)
+        ends = np.cumsum([0] + [len(t) for t in lists])
+        # (over keys, causal) -> the list
+        self._tiles = {(keys, causal): flat[ends[2 * keys + causal]:ends[2 * keys + causal + 1]]
+                       for keys in (False, True) for causal in (False, True)}
+        self._streams = _Streams()
+
+    def _on(self, stream):
+        if stream not in self._streams.seen:
+            self._streams.mark(stream, self.device, self._tiles.values())
+
+
+def _tiles(q_len, k_len, tile, causal, keys):
+    """The tiles of ``tile`` query rows (or key rows) as the kernels read them, by falling work."""
+    q_begin, k_begin = np.cumsum(q_len) - q_len, np.cumsum(k_len) - k_len
+    length, begin = (k_len, k_begin) if keys else (q_len, q_begin)
+    n = -(-length // tile)
+    seq = np.repeat(np.arange(len(length)), n)
+    at = (np.arange(len(seq)) - np.repeat(np.cumsum(n) - n, n)) * tile  # place in the sequence
+    nq, nk = q_len[seq], k_len[seq]
+    rows = np.minimum(tile, length[seq] - at)
+    if not causal:
+        work = nq if keys else nk
+    elif keys:  # query i sees key j from i = j - nk + nq on
+        work = np.clip(nq - np.clip(at - nk + nq, 0, None), 0, None)
+    else:
+        work = np.clip(at + rows + nk - nq, 0, nk)
+    order = np.argsort(-work, kind="stable")
+    table = np.stack([begin[seq] + at, rows, at, q_begin[seq], nq, k_begin[seq], nk,
+                      np.zeros_like(at)], axis=1)
+    return np.ascontiguousarray(table[order], dtype=np.int32)
+
+
+def _host_lengths(indptr, name):
+    if not torch.is_tensor(indptr) or indptr.ndim != 1 or indptr.numel() < 1:
+        raise ValueError(f"{name} must be a 1D tensor with at least one entry")
+    if not indptr.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if indptr.dtype not in SUPPORTED_INDEX_DTYPES:
+        raise TypeError(f"{name} dtype must be torch.int32 or torch.int64")
+    _capturing()
+    p = indptr.cpu().numpy().astype(np.int64)
+    if p[0] != 0:
+        raise ValueError(f"{name}[0] must be 0")
+    if (np.diff(p) < 0).any():
+        raise ValueError(f"{name} must be nondecreasing")
+    if p[-1] > _TOKENS_CAP:
+        raise ValueError(f"{name} must count fewer than 2^31 tokens")
+    return np.diff(p)
+
+
+def prepare_attention_packed(indptr, k_indptr=None):
+    """Check the sequences of a packed batch: sequence b's queries are the tokens ``indptr[b]`` to
+    ``indptr[b + 1]``, its keys ``k_indptr[b]`` to ``k_indptr[b + 1]`` (None: the same).  Returns a
+    PreparedAttention for every call over these sequences: all layers, forward and backward."""
+    q_len = _host_lengths(indptr, "indptr")
+    k_len = q_len
+    if k_indptr is not None:
+        k_len = _host_lengths(k_indptr, "k_indptr")
+        if len(k_len) != len(q_len):
+            raise ValueError("indptr and k_indptr must have the same length")
+        if k_indptr.device != indptr.device:
+            raise ValueError("indptr and k_indptr must be on the same CUDA device")
+    prepared = PreparedAttention(q_len, k_len, indptr.device)
+    torch.cuda.current_stream(indptr.device).synchronize()  # calls may come from other streams
+    return prepared
+
+
+def _packed_inputs(q, k, v, indptr, k_indptr, prepared, causal, window):
+    """(prepared, causal, window) of a call whose arrays are checked against each other."""
+    _check_tensor(q, "q")
+    _check_tensor(k, "k", q.dtype, q.device, None, q.shape[2])
+    _check_tensor(v, "v", q.dtype, q.device, k.shape[1], q.shape[2])
+    _check_heads(q.shape[1], k.shape[1])
+    _check_dim(q.shape[2])
+    window = _window_of(window)
+    if window and not causal:
+        raise ValueError("window needs causal=True")
+    if prepared is None:
+        if indptr is None:
+            raise ValueError("indptr is required when prepared is not provided")
+        prepared = prepare_attention_packed(indptr, k_indptr)
+    elif not isinstance(prepared, PreparedAttention):
+        raise TypeError("prepared must be a PreparedAttention instance")
+    if prepared.device != q.device:
+        raise ValueError("q, k, v and the sequences must be on the same CUDA device")
+    if q.shape[0] != prepared.q_tokens:
+        raise ValueError(f"q must have {prepared.q_tokens} tokens, got {q.shape[0]}")
+    if k.shape[0] != prepared.k_tokens or v.shape[0] != prepared.k_tokens:
+        raise ValueError(f"k and v must have {prepared.k_tokens} tokens, got {k.shape[0]} and "
+                         f"{v.shape[0]}")
+    return prepared, bool(causal), window
+
+
+_NONE3 = (0, 0, 0)
+
+
+def _place(t):
+    return (t.data_ptr(), t.stride(0), t.stride(1))
+
+
+def _pack(prepared, q, k, v, causal, window, scale, out, lse, grads=None):
+    q_tiles = prepared._tiles[False, causal]
+    if grads is None:
+        tail = (*_NONE3, *_NONE3, *_NONE3, *_NONE3, 0)
+        k_list = (0, 0)
+    else:
+        k_tiles = prepared._tiles[True, causal]
+        k_list = (k_tiles.data_ptr(), k_tiles.shape[0])
+        tail = (*_place(grads[0]), *_place(grads[1]), *_place(grads[2]), *_place(grads[3]),
+                grads[4].data_ptr())
+    return _PACKED.pack(_CODES[q.dtype], q.shape[1], k.shape[1], q.shape[2], q.shape[0],
+                        k.shape[0], causal, window, scale, q_tiles.data_ptr(), q_tiles.shape[0],
+                        *k_list, *_place(q), *_place(k), *_place(v), *_place(out), lse.data_ptr(),
+                        *tail)
+
+
+def _forward(prepared, q, k, v, causal, window, scale, out):
+    res, copied = _result(out, "out", q.shape, q.dtype, q.device)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+    if q.shape[0]:
+        q, k, v = _rows(q), _rows(k), _rows(v)
+        stream = _abi.raw_stream(q.device)
+        prepared._on(stream)
+        _abi.check(_abi.lib().fsp_attention_packed(
+            _pack(prepared, q, k, v, causal, window, scale, res, lse), stream),
+            "fsp_attention_packed")
+    if copied:
+        out.copy_(res)
+        res = out
+    return res, lse
+
+
+class _Differentiable(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, prepared, causal, window, scale):
+        out, lse = _forward(prepared, q, k, v, causal, window, scale, None)
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.rest = (prepared, causal, window, scale)
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, _):
+        q, k, v, out, lse = ctx.saved_tensors
+        prepared, causal, window, scale = ctx.rest
+        grads = _backward(prepared, grad, q, k, v, out, lse, causal, window, scale)
+        return *grads, None, None, None, None
+
+
+def flagsparse_attention_packed(q, k, v, indptr=None, k_indptr=None, *, prepared=None, causal=True,
+                                window=None, scale=None, out=None, return_lse=False):
+    """Attention over packed sequences.
+
+    ``q``: [tokens, heads, dim]; ``k``, ``v``: [key tokens, kv_heads, dim]; the sequences are given
+    by ``indptr`` / ``k_indptr`` (checked by this call, which waits for them) or by ``prepared``
+    (prepare_attention_packed).  With ``causal`` query i of nq sees key j of nk if
+    j <= i + nk - nq, the last query all of them; ``window``: only the last ``window`` of those.
+    ``scale``: dim ** -0.5 by default.  Returns [tokens, heads, dim], with the float32 log-sum-exp
+    [tokens, heads] if ``return_lse``.  The output is differentiable with respect to q, k and v where
+    they require a gradient (the log-sum-exp is not)."""
+    prepared, causal, window = _packed_inputs(q, k, v, indptr, k_indptr, prepared, causal, window)
+    scale = _scale_of(scale, q.shape[2])
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        if out is not None:
+            raise RuntimeError("out cannot be given where q, k or v require a gradient")
+        res, lse = _Differentiable.apply(q, k, v, prepared, causal, window, scale)
+    else:
+        res, lse = _forward(prepared, q, k, v, causal, window, scale, out)
+    return (res, lse) if return_lse else res
+
+
+def _backward(prepared, grad_out, q, k, v, out, lse, causal, window, scale):
+    dev, dt = q.device, q.dtype
+    dq, dk, dv = (torch.empty(t.shape, dtype=dt, device=dev) for t in (q, k, v))
+    if q.shape[0] or k.shape[0]:
+        grad_out, q, k, v, out = (_rows(t) for t in (grad_out, q, k, v, out))
+        work = torch.empty(lse.shape, dtype=torch.float32, device=dev)
+        stream = _abi.raw_stream(dev)
+        prepared._on(stream)
+        _abi.check(_abi.lib().fsp_attention_packed_backward(
+            _pack(prepared, q, k, v, causal, window, scale, out, lse.contiguous(),
+                  (grad_out, dq, dk, dv, work)), stream), "fsp_attention_packed_backward")
+    return dq, dk, dv
+
+
+def flagsparse_attention_packed_backward(grad_out, q, k, v, out, lse, indptr=None, k_indptr=None, *,
+                                         prepared=None, causal=True, window=None, scale=None):
+    """(grad_q, grad_k, grad_v) of flagsparse_attention_packed: ``grad_out`` is the gradient of its
+    output, ``out`` and ``lse`` what it returned, the other arguments its own."""
+    prepared, causal, window = _packed_inputs(q, k, v, indptr, k_indptr, prepared, causal, window)
+    for t, name in ((grad_out, "grad_out"), (out, "out")):
+        _check_tensor(t, name, q.dtype, q.device, q.shape[1], q.shape[2])
+        if t.shape[0] != q.shape[0]:
+            raise ValueError(f"{name} must have {q.shape[0]} tokens, got {t.shape[0]}")
+    _check_out(lse, "lse", q.shape[:2], torch.float32, q.device)
+    return _backward(prepared, grad_out, q, k, v, out, lse, causal, window,
+                     _scale_of(scale, q.shape[2]))

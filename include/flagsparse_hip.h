@@ -1,6 +1,7 @@
 /*
  * flagsparse_hip.h - C ABI of the MI355X (gfx950) sparse-product library: CSR/COO SpMV,
- * CSR/COO SpMM, CSR SDDMM, and a Matrix Market reader.
+ * CSR/COO SpMM, CSR SDDMM, attention over packed sequences and a paged cache, and a Matrix
+ * Market reader.
  *
  * Every entry point takes plain device pointers, sizes and a hipStream_t passed as void*.
  * Nothing here allocates device memory: workspaces (partial sums, descriptor tables) are
@@ -68,8 +69,8 @@
 extern "C" {
 #endif
 
-/* Value type of data / x / y / B / C. */
-enum fsp_dtype { FSP_F32 = 0, FSP_F64 = 1 };
+/* Value type of data / x / y / B / C (F32, F64); of queries, keys and values (BF16, F16). */
+enum fsp_dtype { FSP_F32 = 0, FSP_F64 = 1, FSP_BF16 = 2, FSP_F16 = 3 };
 
 /* Value of fsp_spmm_sliced's cut_rows (see there). */
 #define FSP_CUT_PIECES 2
@@ -664,6 +665,130 @@ int fsp_bind_spmm_sliced(void* call, int dtype, int acc_f64, const void* vals,
                          const int32_t* order, int64_t items, int64_t keep, void* sums,
                          int cut_rows, int lanes_per_row, int vec, int xcd_remap);
 int fsp_run(const void* call, const void* in, void* out, void* stream);
+
+/*
+ * Attention.  Queries, keys and values are [tokens, heads, dim] arrays of BF16 or F16 whose last
+ * axis is contiguous; a token's and a head's step are given in elements (any sign of sharing: a
+ * slice of one fused projection, or a step of 0 for a broadcast axis of an input).  dim is a
+ * multiple of 8 up to fsp_attention_dim_cap(), steps are multiples of 8 and bases 16-byte
+ * aligned.  heads is a multiple of kv_heads; query head a reads key head a / (heads / kv_heads).
+ * Sums, softmax statistics and gradients are held in 32 bits and rounded once at the end; the
+ * weights are rounded to the inputs' type before their product with the values (the matrix
+ * instructions' operand type).  The arguments come as a struct of 8-byte fields.
+ *
+ * With S_ij = scale * q_i . k_j over the keys j that query i sees, lse_i = log sum_j exp(S_ij),
+ * P_ij = exp(S_ij - lse_i): out_i = sum_j P_ij v_j.  A query that sees no key has out 0 and lse
+ * minus infinity.
+ */
+int64_t fsp_attention_dim_cap(void);
+
+/*
+ * A paged cache: pages of page_size tokens, k_pages / v_pages [n_pages, page_size, kv_heads, dim]
+ * by their steps, and a page table in CSR form: sequence b's tokens lie in pages
+ * page_indices[page_indptr[b] .. page_indptr[b + 1]), in order, each within [0, n_pages).
+ * lengths[b]: the tokens that sequence b holds (the ones appended in this step included), at most
+ * its pages' room.
+ */
+struct fsp_paged_cache {
+  int64_t dtype, kv_heads, dim, page_size, n_pages, batch, table_len;
+  void* k_pages;
+  int64_t k_page, k_slot, k_head; /* steps */
+  void* v_pages;
+  int64_t v_page, v_slot, v_head;
+  const int32_t* page_indptr;  /* [batch + 1] */
+  const int32_t* page_indices; /* [table_len] */
+};
+
+/*
+ * Appends k and v (and rotates q): token t of sequence b, the tokens of which are
+ * [token_indptr[b], token_indptr[b + 1]) (NULL: one token each), is at position
+ * p = lengths[b] - token_indptr[b + 1] + t.  The first 2 * half elements of every head of k and
+ * q are rotated by pairs with row p of cos / sin ([table_rows, half], float32; half 0: none),
+ * pairs of neighbours with interleaved != 0, else of elements half apart.  q may be NULL.
+ * A token whose position is negative, past its sequence's pages or past the table is not
+ * stored, and its row of q_out is NaN.
+ */
+struct fsp_paged_append_args {
+  struct fsp_paged_cache cache;
+  int64_t n_tokens, heads, half, table_rows, interleaved;
+  const void* k;
+  int64_t k_token, k_head;
+  const void* v;
+  int64_t v_token, v_head;
+  const void* q;
+  int64_t q_token, q_head;
+  void* q_out;
+  int64_t q_out_token, q_out_head;
+  const float* cos;
+  const float* sin;
+  const int32_t* token_indptr;
+  const int32_t* lengths;
+};
+int fsp_paged_append(const struct fsp_paged_append_args* args, void* stream);
+
+/*
+ * Attention of one query per sequence over the cache: q, out [batch, heads, dim], lse
+ * [batch, heads] float32 or NULL.  Key j of sequence b is seen if j >= lengths[b] - window
+ * (window 0: every key).  A length that is negative or more than the sequence's pages hold gives
+ * NaN.  workspace: fsp_attention_paged_workspace() bytes (0: NULL will do).
+ */
+struct fsp_attention_paged_args {
+  struct fsp_paged_cache cache;
+  int64_t heads, window;
+  double scale;
+  const void* q;
+  int64_t q_token, q_head;
+  void* out;
+  int64_t out_token, out_head;
+  float* lse;
+  const int32_t* lengths;
+  void* workspace;
+};
+int64_t fsp_attention_paged_workspace(const struct fsp_attention_paged_args* args);
+int fsp_attention_paged(const struct fsp_attention_paged_args* args, void* stream);
+
+/*
+ * Attention over packed sequences: sequence b's queries are tokens
+ * [q_indptr[b], q_indptr[b + 1]), its keys [k_indptr[b], k_indptr[b + 1]).  With causal != 0 query
+ * i of nq sees key j of nk if j <= i + nk - nq; a window > 0 (causal only) hides the keys
+ * j <= i + nk - nq - window.  lse [q_tokens, heads] float32.
+ *
+ * Work lists (fsp_attention_packed_tile()'s rows to a tile, any order): a tile is 8 int32,
+ * {first row, rows, first row's place in its sequence, sequence's q begin, q count, k begin,
+ * k count, 0}; q_tiles cover the queries, k_tiles (backward only) the keys.
+ *
+ * Backward: grad_out by its steps, out and lse of the forward pass; grad_q, grad_k, grad_v are
+ * written whole.  workspace: float32 [q_tokens, heads].
+ */
+struct fsp_attention_packed_args {
+  int64_t dtype, heads, kv_heads, dim, q_tokens, k_tokens, causal, window;
+  double scale;
+  const int32_t* q_tiles;
+  int64_t n_q_tiles;
+  const int32_t* k_tiles;
+  int64_t n_k_tiles;
+  const void* q;
+  int64_t q_token, q_head;
+  const void* k;
+  int64_t k_token, k_head;
+  const void* v;
+  int64_t v_token, v_head;
+  void* out;
+  int64_t out_token, out_head;
+  float* lse;
+  const void* grad_out;
+  int64_t grad_out_token, grad_out_head;
+  void* grad_q;
+  int64_t grad_q_token, grad_q_head;
+  void* grad_k;
+  int64_t grad_k_token, grad_k_head;
+  void* grad_v;
+  int64_t grad_v_token, grad_v_head;
+  void* workspace;
+};
+int64_t fsp_attention_packed_tile(void);
+int fsp_attention_packed(const struct fsp_attention_packed_args* args, void* stream);
+int fsp_attention_packed_backward(const struct fsp_attention_packed_args* args, void* stream);
 
 #ifdef __cplusplus
 }

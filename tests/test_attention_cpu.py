@@ -1,0 +1,167 @@
+"""Attention without a GPU: the work lists, the argument structs, the refusals that need no device, and
+the 64-bit reference against autograd."""
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import flagsparse_amd as fs
+from flagsparse_amd import _abi, attention
+from oracle import attention as ref
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("keys", [False, True])
+@pytest.mark.parametrize("lengths", [([], []), ([5], [5]), ([0, 300, 64, 65], [7, 0, 64, 1000]),
+                                     ([1] * 50, [3] * 50)])
+def test_tiles_cover_every_row_once(lengths, keys, causal):
+    q_len, k_len = (np.array(x, dtype=np.int64) for x in lengths)
+    t = attention._tiles(q_len, k_len, 64, causal, keys)
+    assert t.shape[1] == 8 and t.dtype == np.int32
+    rows = k_len if keys else q_len
+    seen = np.zeros(rows.sum(), dtype=int)
+    begin = {False: np.cumsum(q_len) - q_len, True: np.cumsum(k_len) - k_len}
+    work = []
+    for first, n, at, q_begin, nq, k_begin, nk, zero in t.tolist():
+        assert 1 <= n <= 64 and zero == 0
+        seen[first:first + n] += 1
+        b = [b for b in range(len(rows)) if rows[b] and
+             begin[keys][b] <= first < begin[keys][b] + rows[b]][0]
+        assert (q_begin, nq, k_begin, nk) == (begin[False][b], q_len[b], begin[True][b], k_len[b])
+        assert first == begin[keys][b] + at and at + n <= rows[b]
+        mask = ref.seen(nq, nk, causal, None)
+        mask = mask[:, at:at + n] if keys else mask[at:at + n]
+        work.append(int(mask.any(0 if not keys else 1).sum()))
+    assert (seen == 1).all()
+    assert work == sorted(work, reverse=True)
+
+
+def test_exports_have_a_name_in_the_package():
+    import flagsparse
+
+    for name in fs.ATTENTION_EXPORTS:
+        assert getattr(flagsparse, name) is getattr(fs, name)
+        assert name not in fs.__all__  # the reference's list
+
+
+def test_struct_sizes():
+    # 8-byte fields, as in the header
+    assert attention._CACHE.size == 8 * 17
+    assert attention._APPEND.size == 8 * 21
+    assert attention._PAGED.size == 8 * 12
+    assert attention._PACKED.size == 8 * (9 + 4 + 12 + 1 + 12 + 1)
+    assert _abi.lib().fsp_attention_dim_cap() == attention._DIM_CAP
+
+
+def _packed(**kw):
+    a = dict(dtype=2, heads=4, kv_heads=2, dim=64, q_tokens=8, k_tokens=8, causal=1, window=0,
+             scale=0.125, q_tiles=16, n_q_tiles=1, k_tiles=16, n_k_tiles=1)
+    for n in ("q", "k", "v", "out", "go", "gq", "gk", "gv"):
+        a |= {n: 64, n + "_token": 256, n + "_head": 64}
+    a |= {"lse": 16, "work": 16} | kw
+    order = ["dtype", "heads", "kv_heads", "dim", "q_tokens", "k_tokens", "causal", "window", "scale",
+             "q_tiles", "n_q_tiles", "k_tiles", "n_k_tiles"]
+    order += [n + e for n in ("q", "k", "v", "out") for e in ("", "_token", "_head")] + ["lse"]
+    order += [n + e for n in ("go", "gq", "gk", "gv") for e in ("", "_token", "_head")] + ["work"]
+    return attention._PACKED.pack(*(a[n] for n in order))
+
+
+@pytest.mark.parametrize("status,kw", [
+    (-3, {"dtype": 0}), (-3, {"dim": 132}), (-3, {"dim": 12}), (-3, {"dim": 0}),
+    (-1, {"heads": 3}), (-1, {"kv_heads": 0}), (-1, {"heads": 0}), (-1, {"q_tokens": -1}),
+    (-1, {"n_q_tiles": 1 << 40}), (-1, {"window": -1}), (-1, {"window": 5, "causal": 0}),
+    (-1, {"q": 0}), (-1, {"k": 0}), (-1, {"lse": 0}), (-1, {"q": 72}), (-1, {"k_token": 12}),
+    (-1, {"v_head": 4}), (-1, {"out": 8}), (-1, {"q_tiles": 0})])
+def test_packed_refusals_of_the_library(status, kw):
+    L = _abi.lib()
+    assert L.fsp_attention_packed(_packed(**kw), None) == status
+    assert L.fsp_last_error()
+    assert L.fsp_attention_packed_backward(_packed(**kw), None) == status
+    assert L.fsp_attention_packed(None, None) == -1
+    assert L.fsp_attention_packed_backward(None, None) == -1
+
+
+@pytest.mark.parametrize("kw", [{"go": 0}, {"gq": 0}, {"gk": 0}, {"gv": 0}, {"work": 0}, {"go": 4},
+                                {"gk_token": 3}, {"k_tiles": 0}])
+def test_backward_refusals_of_the_library(kw):
+    assert _abi.lib().fsp_attention_packed_backward(_packed(**kw), None) == -1
+
+
+def _cache(**kw):
+    a = dict(dtype=2, kv_heads=2, dim=64, page_size=16, n_pages=4, batch=2, table_len=3, k=64, kp=2048,
+             ks=128, kh=64, v=64, vp=2048, vs=128, vh=64, indptr=16, indices=16) | kw
+    return attention._CACHE.pack(*a.values())
+
+
+_PAGED_ARGS = dict(heads=4, window=0, scale=0.125, q=64, qt=256, qh=64, out=64, ot=256, oh=64, lse=0,
+                   lengths=16, work=16)
+_APPEND_ARGS = dict(n_tokens=2, heads=4, half=32, rows=64, interleaved=0, k=64, kt=128, kh=64, v=64,
+                    vt=128, vh=64, q=64, qt=256, qh=64, qo=64, qot=256, qoh=64, cos=16, sin=16,
+                    tokens=0, lengths=16)
+
+
+@pytest.mark.parametrize("status,kw", [
+    (-3, {"dtype": 1}), (-3, {"dim": 130}), (-1, {"page_size": 0}), (-1, {"batch": -1}),
+    (-1, {"n_pages": 1 << 31}), (-1, {"table_len": 1 << 28}), (-1, {"k": 0}), (-1, {"v": 8}),
+    (-1, {"kp": 4}), (-1, {"indptr": 0}), (-1, {"indices": 0})])
+def test_cache_refusals_of_the_library(status, kw):
+    L = _abi.lib()
+    c = _cache(**kw)
+    assert L.fsp_attention_paged(c + attention._PAGED.pack(*_PAGED_ARGS.values()), None) == status
+    assert L.fsp_paged_append(c + attention._APPEND.pack(*_APPEND_ARGS.values()), None) == status
+    assert L.fsp_attention_paged(None, None) == -1 and L.fsp_paged_append(None, None) == -1
+
+
+@pytest.mark.parametrize("kw", [{"heads": 3}, {"heads": 0}, {"window": -1}, {"q": 0}, {"out": 0},
+                                {"lengths": 0}, {"q": 72}, {"oh": 2}])
+def test_paged_refusals_of_the_library(kw):
+    L = _abi.lib()
+    args = _cache() + attention._PAGED.pack(*(_PAGED_ARGS | kw).values())
+    assert L.fsp_attention_paged(args, None) == -1
+
+
+@pytest.mark.parametrize("kw", [{"half": 33}, {"half": -1}, {"n_tokens": 3}, {"n_tokens": -1},
+                                {"k": 0}, {"cos": 0}, {"qo": 0}, {"lengths": 0}, {"kt": 4},
+                                {"rows": 1 << 32}])
+def test_append_refusals_of_the_library(kw):
+    L = _abi.lib()
+    args = _cache() + attention._APPEND.pack(*(_APPEND_ARGS | kw).values())
+    assert L.fsp_paged_append(args, None) == -1
+
+
+def test_refusals_that_need_no_device():
+    q = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
+    ip = torch.tensor([0, 4])
+    with pytest.raises(ValueError):
+        fs.flagsparse_attention_packed(q, q, q, ip)
+    with pytest.raises(ValueError):
+        fs.prepare_attention_packed(ip)
+    with pytest.raises(ValueError):
+        fs.prepare_paged_kv(q[None], q[None], ip, ip)
+    with pytest.raises(TypeError):
+        fs.flagsparse_attention_paged(q, ip, prepared=q)
+    with pytest.raises(ValueError):
+        fs.flagsparse_paged_append(q, q, ip)
+
+
+@pytest.mark.parametrize("causal,window", [(True, None), (False, None), (True, 3)])
+def test_reference_is_the_gradient(causal, window):
+    gen = torch.Generator().manual_seed(1)
+    q, k, v, g = (torch.randn(9, 8, generator=gen).double() for _ in range(4))
+    mask = ref.seen(9, 9, causal, window)
+    r = ref.one(q, k, v, mask, 0.3, g)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    s = (leaves[0] @ leaves[1].T * 0.3).masked_fill(~mask, float("-inf"))
+    out = torch.softmax(s, 1) @ leaves[2]
+    out.backward(g)
+    assert torch.allclose(out, r["out"], atol=1e-12)
+    for t, n in zip(leaves, "qkv"):
+        assert torch.allclose(t.grad, r[n], atol=1e-12)
+
+
+def test_struct_of_bytes_reaches_the_library():
+    # the structs go by address: a bytes object does
+    assert isinstance(_packed(), bytes)
+    assert ctypes.c_void_p in _abi.SIGNATURES["fsp_attention_packed"][1]
