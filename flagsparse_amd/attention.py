@@ -32,6 +32,7 @@ SUPPORTED_ATTENTION_DTYPES = (torch.bfloat16, torch.float16)
 _CODES = {torch.bfloat16: _abi.FSP_BF16, torch.float16: _abi.FSP_F16}
 _DIM_CAP = 128
 _TOKENS_CAP = 2**31 - 1
+_STEP_CAP = 2**23
 
 # The argument structs of include/flagsparse_hip.h: 8-byte fields, "d" the scale.
 _CACHE = struct.Struct("7q 4q 4q 2q")
@@ -98,10 +99,11 @@ def _check_heads(heads, kv_heads):
 
 
 def _rows(t):
-    """``t`` itself where the kernels can read it (contiguous last axis, 16-byte rows), else a
-    copy."""
+    """``t`` itself where the kernels can read it (contiguous last axis, 16-byte rows, tokens that do
+    not overlap and lie within 2^23 elements of each other), else a copy."""
     s = t.stride()
-    if s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and t.data_ptr() % 16 == 0:
+    if s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and t.data_ptr() % 16 == 0 and \
+            t.shape[2] <= s[0] <= _STEP_CAP:
         return t
     return _aligned(t.contiguous())
 

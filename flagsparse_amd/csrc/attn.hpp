@@ -19,6 +19,57 @@ constexpr float kLn2 = 0.6931471805599453f;
 typedef __bf16 bf16;
 typedef _Float16 f16;
 
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+typedef f16 f16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+template <typename T> struct Vec;
+template <> struct Vec<bf16> { typedef bf16x8 v8; typedef bf16x4 v4; };
+template <> struct Vec<f16> { typedef f16x8 v8; typedef f16x4 v4; };
+template <typename T> using V8 = typename Vec<T>::v8;
+template <typename T> using V4 = typename Vec<T>::v4;
+
+// C += A B on the matrix cores, 32 x 32 x 16.  Lane l holds A[l % 32][8 * (l / 32) + 0..7],
+// B[8 * (l / 32) + 0..7][l % 32] and, in register r, C[8 * (r / 4) + 4 * (l / 32) + r % 4][l % 32].
+// The order of the 16 summed elements is free as long as A and B share it.
+__device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// 16 x 16 x 32: A[l % 16][8 * (l / 16) + 0..7], B[8 * (l / 16) + 0..7][l % 16],
+// C[4 * (l / 16) + r][l % 16].
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+typedef __attribute__((address_space(3))) char lds_char;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) s16x8 lds_s16x8;
+
+// A transposed read of 16-bit elements from LDS: in each group of 16 lanes, lane j names four
+// consecutive elements of row j / 4, columns 4 * (j % 4) + 0..3, and gets column j of the four rows.
+__device__ __forceinline__ s16x4 lds_transposed(const lds_char* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+}
+
+// The other half's value: lanes l and l + 32 exchange.
+__device__ __forceinline__ float other_half(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                  false);
+  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
   for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
