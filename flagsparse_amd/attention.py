@@ -418,8 +418,8 @@ class PreparedAttention:
         self.q_tokens = int(q_len.sum())
         self.k_tokens = int(k_len.sum())
         self.device = device
-        tile = int(_abi.lib().fsp_attention_packed_tile())
-        lists = [_tiles(q_len, k_len, tile, causal, keys)
+        tile = [int(_abi.lib().fsp_attention_packed_tile(keys)) for keys in (0, 1)]
+        lists = [_tiles(q_len, k_len, tile[keys], causal, keys)
                  for keys in (False, True) for causal in (False, True)]
         flat = torch.from_numpy(np.concatenate(lists)).to(device)
         ends = np.cumsum([0] + [len(t) for t in lists])
@@ -599,7 +599,7 @@ def _backward(prepared, grad_out, q, k, v, out, lse, causal, window, scale):
     dq, dk, dv = (torch.empty(t.shape, dtype=dt, device=dev) for t in (q, k, v))
     if q.shape[0] or k.shape[0]:
         grad_out, q, k, v, out = (_rows(t) for t in (grad_out, q, k, v, out))
-        work = torch.empty(lse.shape, dtype=torch.float32, device=dev)
+        work = torch.empty((2, q.shape[1], q.shape[0]), dtype=torch.float32, device=dev)
         stream = _abi.raw_stream(dev)
         prepared._on(stream)
         _abi.check(_abi.lib().fsp_attention_packed_backward(

@@ -42,23 +42,49 @@ __device__ __forceinline__ void seen_by(const Shape& s, const Tile& t, int i, in
   }
 }
 
-// Keys of one step, and how their rows lie in LDS: PITCH bytes each in chunks of 16, the chunks of a
-// row permuted so that the lanes of one read meet different banks (K: by the row, for reads of one
-// chunk of many rows; V: by the row's place in four, for transposed reads of four rows).
-constexpr int kKeys = 64;
+// Key j of a sequence is seen by the queries [lo, hi).
+__device__ __forceinline__ void seen_of(const Shape& s, const Tile& t, int j, int& lo, int& hi) {
+  lo = 0;
+  hi = t.nq;
+  if (s.causal) {
+    lo = j - t.nk + t.nq;
+    if (s.window && lo < t.nq - s.window) hi = lo + s.window;
+    if (lo < 0) lo = 0;
+  }
+}
+
+// Rows of one step, and how they lie in LDS: PITCH bytes each in chunks of 16, a row's chunks permuted
+// by the row so that the lanes of one read meet different banks, in reads of one chunk of 8 (or
+// 16) consecutive rows and in transposed reads of four chunks of four rows.
+constexpr int kRows = 64;
 
 template <int DP>
 struct Lay {
   static constexpr int PITCH = DP <= 64 ? 128 : 256;
   static constexpr int CH = PITCH / 16;
-  static constexpr int BYTES = kKeys * PITCH;
-  __device__ static int swizzle_k(int row) { return row & (CH - 1); }
-  __device__ static int swizzle_v(int row) { return CH == 8 ? (row & 2) << 1 : (row & 3) << 2; }
+  static constexpr int BYTES = kRows * PITCH;
+  __device__ static int swizzle(int r) {
+    const int r0 = r & 1, r1 = (r >> 1) & 1, r2 = (r >> 2) & 1, r3 = (r >> 3) & 1;
+    return CH == 8 ? (r1 << 2 | r2 << 1 | (r0 ^ r3)) : (r1 << 3 | r0 << 2 | r2 << 1 | (r1 ^ r3));
+  }
+  // Where lane finds 8 elements of row lane % 32, from 8 * (lane / 32) on; 16 * i elements on and
+  // 32 * u rows on: (this ^ 32 * i) + 32 * u * PITCH.
+  __device__ static int row_at(int lane) {
+    return (lane & 31) * PITCH + (((lane >> 5) ^ swizzle(lane & 31)) << 4);
+  }
+  // What lane names in a transposed read of the columns 0..31 of rows 4 * (lane / 32) + 0..3: it gets
+  // column lane % 32.  32 * n columns on: this ^ 64 * n; 8 rows on: (this ^ 16) + 8 * PITCH;
+  // 16 * i rows on: + 16 * i * PITCH.
+  __device__ static int col_at(int lane) {
+    const int j = lane & 15, row = 4 * (lane >> 5) + (j >> 2);
+    const int chunk = (2 * ((lane >> 4) & 1) + ((j & 3) >> 1)) ^ swizzle(row);
+    return row * PITCH + chunk * 16 + (j & 1) * 8;
+  }
 };
 
 // Rows [0, n) of a 16-bit array, ``bytes`` apart, straight to LDS: 1024 bytes a wave and load.  What lies
 // past the rows or the head's dim is read as zero: the buffer's bounds end there.
-template <int DP, bool V>
+template <int DP>
 __device__ __forceinline__ void load_rows(char* lds, const void* src, int n, uint32_t bytes, int dim,
                                           int wave, int lane) {
   typedef Lay<DP> L;
@@ -66,15 +92,30 @@ __device__ __forceinline__ void load_rows(char* lds, const void* src, int n, uin
       const_cast<void*>(src), 0, (int)((uint32_t)(n - 1) * bytes + 2 * dim), 0x00027000);
   constexpr int PER = L::BYTES / 1024 / 4;  // loads of a wave
   constexpr int ROWS = 1024 / L::PITCH;     // rows of a load
+  const int chunk = (lane % L::CH) ^ L::swizzle(lane / L::CH);
+  const uint32_t first = (uint32_t)(wave * PER * ROWS + lane / L::CH) * bytes;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int row = (wave * PER + i) * ROWS + lane / L::CH;
-    const int chunk = (lane % L::CH) ^ (V ? L::swizzle_v(row) : L::swizzle_k(row));
-    const uint32_t at = 8 * chunk < dim ? row * bytes + 16 * chunk : 0x80000000u;
+  for (int i = 0; i < PER; ++i) {  // swizzle(a ^ b) = swizzle(a) ^ swizzle(b)
+    const int at = 16 * (chunk ^ L::swizzle(i * ROWS));
     __builtin_amdgcn_raw_ptr_buffer_load_lds(
-        rsrc, (__attribute__((address_space(3))) void*)(lds + (wave * PER + i) * 1024), 16, (int)at,
-        0, 0, 0);
+        rsrc, (__attribute__((address_space(3))) void*)(lds + (wave * PER + i) * 1024), 16,
+        (int)(at < 2 * dim ? first + i * ROWS * bytes + at : 0x80000000u), 0, 0, 0);
   }
+}
+
+// Matrix operands from LDS: 8 consecutive elements of a row a lane, and 8 rows' elements of a column
+// (rows 16 * i + {0..3, 8..11} + 4 * (lane / 32), the ones that the lane's accumulator registers
+// 8 * i..8 * i + 7 stand for).
+template <typename T>
+__device__ __forceinline__ V8<T> row_frag(const lds_char* p) {
+  return __builtin_bit_cast(V8<T>, *(const lds_s16x8*)p);
+}
+
+template <typename T, int PITCH>
+__device__ __forceinline__ V8<T> col_frag(const lds_char* base, int at, int i) {
+  const s16x4 low = lds_transposed(base + at + 16 * i * PITCH);
+  const s16x4 high = lds_transposed(base + (at ^ 16) + (16 * i + 8) * PITCH);
+  return __builtin_bit_cast(V8<T>, __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
 template <typename T>
@@ -85,12 +126,36 @@ __device__ __forceinline__ V8<T> to16(const f32x16& x, int at) {
   return __builtin_convertvector(v, V8<T>);
 }
 
+// One row of a result from the accumulators of its column, times f.
+template <typename T, int NT>
+__device__ __forceinline__ void store_rows(T* to, const f32x16 (&x)[NT], float f, int dim, int half) {
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int d = 32 * i + 2 * r + 4 * half;
+      if (d < dim) {
+        f32x4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = x[i][r + e] * f;
+        *reinterpret_cast<V4<T>*>(to + d) = __builtin_convertvector(y, V4<T>);
+      }
+    }
+}
+
 // Scores are scale * q . k, and weights exp(score - max) = exp2(c q . k - c max) with c = scale *
-// log2(e) > 0: a negative scale turns q's sign, a zero one makes q zero.
+// log2(e) > 0: a negative scale turns the sign of one factor, and one that is zero, or too small to
+// show in 32 bits, makes it zero.
+constexpr float kNoScale = 1e-30f;
+
 template <typename T>
 __device__ __forceinline__ V8<T> scaled_sign(V8<T> q, float scale) {
-  if (scale > 0) return q;
-  return scale < 0 ? -q : V8<T>{};
+  if (scale > kNoScale) return q;
+  return scale < -kNoScale ? -q : V8<T>{};
+}
+
+__device__ __forceinline__ float exp2_scale(float scale) {
+  return fabsf(scale) > kNoScale ? fabsf(scale) * kLog2e : 1.0f;
 }
 
 template <typename T, int DP>
@@ -122,7 +187,7 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(
       qf[i] = d < s.dim ? scaled_sign<T>(x, s.scale) : V8<T>{};
     }
   }
-  const float c = s.scale == 0 ? 1.0f : fabsf(s.scale) * kLog2e;
+  const float c = exp2_scale(s.scale);
 
   // the keys that this lane's row sees, and those of the wave's first and last rows
   int lo, hi, lo0, hi0, lo1, hi1, lot, hit, none;
@@ -140,21 +205,15 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(
   const T* kb = k + (int64_t)t.k_begin * k_token + g * k_head;
   const T* vb = v + (int64_t)t.k_begin * v_token + g * v_head;
   auto load = [&](int j0, char* sk, char* sv) {
-    const int n = min(kKeys, t.nk - j0);
-    load_rows<DP, false>(sk, kb + j0 * k_token, n, (uint32_t)(2 * k_token), s.dim, wave, lane);
-    load_rows<DP, true>(sv, vb + j0 * v_token, n, (uint32_t)(2 * v_token), s.dim, wave, lane);
+    const int n = min(kRows, t.nk - j0);
+    load_rows<DP>(sk, kb + j0 * k_token, n, (uint32_t)(2 * k_token), s.dim, wave, lane);
+    load_rows<DP>(sv, vb + j0 * v_token, n, (uint32_t)(2 * v_token), s.dim, wave, lane);
   };
-  const int k_at = col * L::PITCH + ((half ^ (col & (L::CH - 1))) << 4);
-  int v_at[NT];
-#pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    const int j = lane & 15, row = 4 * half + (j >> 2);
-    const int chunk = (4 * i + 2 * ((lane >> 4) & 1) + ((j & 3) >> 1)) ^ L::swizzle_v(row);
-    v_at[i] = row * L::PITCH + chunk * 16 + (j & 1) * 8;
-  }
+  const int k_at = L::row_at(lane);
+  const int v_at = L::col_at(lane);
 
   auto step = [&](int j0, const char* sk_, const char* sv_) {
-    if (!active || j0 >= hi1 || j0 + kKeys <= lo0) return;
+    if (!active || j0 >= hi1 || j0 + kRows <= lo0) return;
     const lds_char* sk = (const lds_char*)sk_;
     const lds_char* sv = (const lds_char*)sv_;
     f32x16 x[2];
@@ -163,12 +222,10 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(
       x[u] = f32x16{};
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
-        const V8<T> kf = __builtin_bit_cast(
-            V8<T>, *(const lds_s16x8*)(sk + (k_at ^ (i * 32)) + u * 32 * L::PITCH));
-        x[u] = mfma32(kf, qf[i], x[u]);
+        x[u] = mfma32(row_frag<T>(sk + (k_at ^ (i * 32)) + u * 32 * L::PITCH), qf[i], x[u]);
       }
     }
-    if (j0 + kKeys > hi0 || j0 < lo1) {
+    if (j0 + kRows > hi0 || j0 < lo1) {
       const int first = lo - j0 - 4 * half, last = hi - j0 - 4 * half;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -206,11 +263,7 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(
       const V8<T> pf = to16<T>(x[i / 2], 8 * (i % 2));
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const s16x4 low = lds_transposed(sv + v_at[n] + 16 * i * L::PITCH);
-        const s16x4 high = lds_transposed(sv + v_at[n] + (16 * i + 8) * L::PITCH);
-        const V8<T> vf = __builtin_bit_cast(
-            V8<T>, __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7));
-        o[n] = mfma32(vf, pf, o[n]);
+        o[n] = mfma32(col_frag<T, L::PITCH>(sv, v_at ^ (64 * n), i), pf, o[n]);
       }
     }
   };
@@ -219,15 +272,15 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(
   if (j0 < hit) load(j0, s_k0, s_v0);
   __syncthreads();
   while (j0 < hit) {
-    if (j0 + kKeys < hit) load(j0 + kKeys, s_k1, s_v1);
+    if (j0 + kRows < hit) load(j0 + kRows, s_k1, s_v1);
     step(j0, s_k0, s_v0);
     __syncthreads();
-    j0 += kKeys;
+    j0 += kRows;
     if (j0 >= hit) break;
-    if (j0 + kKeys < hit) load(j0 + kKeys, s_k0, s_v0);
+    if (j0 + kRows < hit) load(j0 + kRows, s_k0, s_v0);
     step(j0, s_k1, s_v1);
     __syncthreads();
-    j0 += kKeys;
+    j0 += kRows;
   }
 
   sum += other_half(sum);
@@ -235,135 +288,297 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(
   const int64_t row = t.first + mine;
   const float inv = sum > 0 ? 1.0f / sum : (sum == 0 ? 0.0f : sum);
   if (half == 0) lse[row * s.heads + a] = sum == 0 ? -INFINITY : (top * c + log2f(sum)) * kLn2;
-  T* to = out + row * o_token + a * o_head;
+  if (sum == 0)  // nothing seen: zeros, whatever lies in the rows of V
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
-#pragma unroll
-    for (int r = 0; r < 16; r += 4) {
-      const int d = 32 * i + 2 * r + 4 * half;
-      if (d < s.dim) {
-        f32x4 y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = sum == 0 ? 0.0f : o[i][r + e] * inv;
-        *reinterpret_cast<V4<T>*>(to + d) = __builtin_convertvector(y, V4<T>);
-      }
-    }
+    for (int i = 0; i < NT; ++i) o[i] = f32x16{};
+  store_rows<T, NT>(out + row * o_token + a * o_head, o, inv, s.dim, half);
 }
 
-// Gradient of the queries, a wave a row as above; also writes delta = grad_out . out.
-template <typename T>
-__global__ __launch_bounds__(kWave) void attention_grad_q_kernel(
-    Shape s, const Tile* __restrict__ tiles, const T* __restrict__ q, int64_t q_token,
+// The normalised weights of the keys' gradients are taken times 2^up: float16 holds those of long rows
+// (2^-14 and less) with fewer bits.
+template <typename T> struct Lift { static constexpr float up = 0, down = 1; };
+template <> struct Lift<f16> { static constexpr float up = 14, down = 1.0f / 16384; };
+
+// Gradient of the queries: the forward pass's loop over keys with dP^T = V grad_out^T beside S^T; dS^T
+// is the operand of dQ^T = K^T dS^T where it lies.
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 2) void attention_grad_q_kernel(
+    Shape s, const Tile* __restrict__ tiles, int n_tiles, const T* __restrict__ q, int64_t q_token,
     int64_t q_head, const T* __restrict__ k, int64_t k_token, int64_t k_head,
     const T* __restrict__ v, int64_t v_token, int64_t v_head, const T* __restrict__ out,
     int64_t o_token, int64_t o_head, const float* __restrict__ lse, const T* __restrict__ go,
     int64_t go_token, int64_t go_head, T* __restrict__ dq, int64_t dq_token, int64_t dq_head,
-    float* __restrict__ delta) {
-  __shared__ float s_q[kAttnDimCap], s_g[kAttnDimCap];
-  const Tile t = tiles[blockIdx.x];
-  const int a = blockIdx.y, lane = threadIdx.x, g = a / (s.heads / s.kv_heads);
-  for (int r = 0; r < t.rows; ++r) {
-    const int64_t row = t.first + r;
-    __syncthreads();
-    float dl = 0;
-    for (int d = lane; d < s.dim; d += kWave) {
-      s_q[d] = (float)q[row * q_token + a * q_head + d];
-      s_g[d] = (float)go[row * go_token + a * go_head + d];
-      dl += s_g[d] * (float)out[row * o_token + a * o_head + d];
-    }
-    __syncthreads();
-    dl = wave_add(dl);
-    if (lane == 0) delta[row * s.heads + a] = dl;
-    const float e0 = lse[row * s.heads + a];
-    int lo, hi;
-    seen_by(s, t, t.at + r, lo, hi);
-    float acc[2] = {0, 0};
-    for (int j0 = lo; j0 < hi; j0 += kWave) {
-      const int j = j0 + lane;
-      float ds = 0;
-      if (j < hi) {
-        const T* kr = k + (int64_t)(t.k_begin + j) * k_token + g * k_head;
-        const T* vr = v + (int64_t)(t.k_begin + j) * v_token + g * v_head;
-        float x = 0, dp = 0;
-        for (int d = 0; d < s.dim; ++d) {
-          x += s_q[d] * (float)kr[d];
-          dp += s_g[d] * (float)vr[d];
-        }
-        ds = expf(x * s.scale - e0) * (dp - dl) * s.scale;
-      }
-      for (int e = 0; e < kWave && j0 + e < hi; ++e) {
-        const float de = __shfl(ds, e);
-        const T* kr = k + (int64_t)(t.k_begin + j0 + e) * k_token + g * k_head;
-        for (int u = 0; u < 2; ++u)
-          if (lane + u * kWave < s.dim) acc[u] += de * (float)kr[lane + u * kWave];
-      }
-    }
-    for (int u = 0; u < 2; ++u)
-      if (lane + u * kWave < s.dim)
-        dq[row * dq_token + a * dq_head + lane + u * kWave] = (T)acc[u];
+    float* __restrict__ stats, int64_t q_tokens) {
+  typedef Lay<DP> L;
+  constexpr int NS = DP / 16, NT = DP / 32;
+  __shared__ __attribute__((aligned(1024))) char s_k0[L::BYTES], s_v0[L::BYTES], s_k1[L::BYTES],
+      s_v1[L::BYTES];
+  int tile, a;
+  tile_and_head(blockIdx.x, n_tiles, s.heads, tile, a);
+  const Tile t = tiles[tile];
+  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = a / (s.heads / s.kv_heads);
+  const int mine = wave * 32 + col;
+  const bool active = wave * 32 < t.rows;
+  const int64_t row = t.first + (int64_t)min(mine, t.rows - 1);
+
+  V8<T> qf[NS], gf[NS];
+  float delta = 0;
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    const int d = 16 * i + 8 * half, at = d < s.dim ? d : 0;
+    const V8<T> x = *reinterpret_cast<const V8<T>*>(q + row * q_token + a * q_head + at);
+    const V8<T> y = *reinterpret_cast<const V8<T>*>(go + row * go_token + a * go_head + at);
+    const V8<T> z = *reinterpret_cast<const V8<T>*>(out + row * o_token + a * o_head + at);
+    qf[i] = d < s.dim ? scaled_sign<T>(x, s.scale) : V8<T>{};
+    gf[i] = d < s.dim ? y : V8<T>{};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) delta += d < s.dim ? (float)y[e] * (float)z[e] : 0.0f;
   }
+  delta += other_half(delta);
+  const float c = exp2_scale(s.scale);
+  float base = lse[row * s.heads + a];
+  base = base == -INFINITY ? INFINITY : base * kLog2e;
+  // what the keys' gradients start their products from: see there
+  if (half == 0 && mine < t.rows) {
+    stats[a * q_tokens + row] = (Lift<T>::up - base) / c;
+    stats[(s.heads + a) * q_tokens + row] = -delta;
+  }
+
+  int lo, hi, lo0, hi0, lo1, hi1, lot, hit, none;
+  seen_by(s, t, t.at + min(mine, t.rows - 1), lo, hi);
+  seen_by(s, t, t.at + min(wave * 32, t.rows - 1), lo0, hi0);
+  seen_by(s, t, t.at + min(wave * 32 + 31, t.rows - 1), lo1, hi1);
+  seen_by(s, t, t.at, lot, none);
+  seen_by(s, t, t.at + t.rows - 1, none, hit);
+
+  f32x16 acc[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) acc[i] = f32x16{};
+
+  const T* kb = k + (int64_t)t.k_begin * k_token + g * k_head;
+  const T* vb = v + (int64_t)t.k_begin * v_token + g * v_head;
+  auto load = [&](int j0, char* sk, char* sv) {
+    const int n = min(kRows, t.nk - j0);
+    load_rows<DP>(sk, kb + j0 * k_token, n, (uint32_t)(2 * k_token), s.dim, wave, lane);
+    load_rows<DP>(sv, vb + j0 * v_token, n, (uint32_t)(2 * v_token), s.dim, wave, lane);
+  };
+  const int r_at = L::row_at(lane);
+  const int c_at = L::col_at(lane);
+
+  auto step = [&](int j0, const char* sk_, const char* sv_) {
+    if (!active || j0 >= hi1 || j0 + kRows <= lo0) return;
+    const lds_char* sk = (const lds_char*)sk_;
+    const lds_char* sv = (const lds_char*)sv_;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      f32x16 x{}, y{};
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        x = mfma32(row_frag<T>(sk + (r_at ^ (i * 32)) + u * 32 * L::PITCH), qf[i], x);
+        y = mfma32(row_frag<T>(sv + (r_at ^ (i * 32)) + u * 32 * L::PITCH), gf[i], y);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], c, -base)) * (y[r] - delta);
+      if (j0 + kRows > hi0 || j0 < lo1) {
+        const int first = lo - j0 - 4 * half, last = hi - j0 - 4 * half;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int j = 32 * u + 8 * (r / 4) + r % 4;
+          x[r] = j >= first && j < last ? x[r] : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const V8<T> f = to16<T>(x, 8 * i);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          acc[n] = mfma32(col_frag<T, L::PITCH>(sk, c_at ^ (64 * n), 2 * u + i), f, acc[n]);
+      }
+    }
+  };
+
+  int j0 = lot;
+  if (j0 < hit) load(j0, s_k0, s_v0);
+  __syncthreads();
+  while (j0 < hit) {
+    if (j0 + kRows < hit) load(j0 + kRows, s_k1, s_v1);
+    step(j0, s_k0, s_v0);
+    __syncthreads();
+    j0 += kRows;
+    if (j0 >= hit) break;
+    if (j0 + kRows < hit) load(j0 + kRows, s_k0, s_v0);
+    step(j0, s_k1, s_v1);
+    __syncthreads();
+    j0 += kRows;
+  }
+  if (mine < t.rows)
+    store_rows<T, NT>(dq + row * dq_token + a * dq_head, acc, s.scale, s.dim, half);
 }
 
-// Gradients of the keys and values, a wave a key row: 64 queries at a time.
-template <typename T>
-__global__ __launch_bounds__(kWave) void attention_grad_kv_kernel(
-    Shape s, const Tile* __restrict__ tiles, const T* __restrict__ q, int64_t q_token,
+// Gradients of the keys and values, 64 keys a workgroup, over the heads of the group and their
+// queries.  S and dP are [queries, keys], so P and dS are the operands of dV^T = grad_out^T P and
+// dK^T = Q^T dS where they lie.  The products start from a row's -lse / scale and -delta, so that they
+// give S - lse and dP - delta.  Two waves share 32 keys, one to every other 32 queries; their sums
+// are joined through LDS at the end.
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 2) void attention_grad_kv_kernel(
+    Shape s, const Tile* __restrict__ tiles, int n_tiles, const T* __restrict__ q, int64_t q_token,
     int64_t q_head, const T* __restrict__ k, int64_t k_token, int64_t k_head,
-    const T* __restrict__ v, int64_t v_token, int64_t v_head, const float* __restrict__ lse,
-    const T* __restrict__ go, int64_t go_token, int64_t go_head,
-    const float* __restrict__ delta, T* __restrict__ dk, int64_t dk_token, int64_t dk_head,
-    T* __restrict__ dv, int64_t dv_token, int64_t dv_head) {
-  __shared__ float s_k[kAttnDimCap], s_v[kAttnDimCap];
-  const Tile t = tiles[blockIdx.x];
-  const int g = blockIdx.y, lane = threadIdx.x, group = s.heads / s.kv_heads;
-  for (int r = 0; r < t.rows; ++r) {
-    const int64_t row = t.first + r;
-    const int j = t.at + r;
-    __syncthreads();
-    for (int d = lane; d < s.dim; d += kWave) {
-      s_k[d] = (float)k[row * k_token + g * k_head + d];
-      s_v[d] = (float)v[row * v_token + g * v_head + d];
+    const T* __restrict__ v, int64_t v_token, int64_t v_head, const T* __restrict__ go,
+    int64_t go_token, int64_t go_head, const float* __restrict__ stats, int64_t q_tokens,
+    T* __restrict__ dk, int64_t dk_token, int64_t dk_head, T* __restrict__ dv, int64_t dv_token,
+    int64_t dv_head) {
+  typedef Lay<DP> L;
+  constexpr int NS = DP / 16, NT = DP / 32;
+  __shared__ __attribute__((aligned(1024))) char s_q0[L::BYTES], s_g0[L::BYTES], s_q1[L::BYTES],
+      s_g1[L::BYTES];
+  __shared__ __attribute__((aligned(256))) float s_x0[kRows], s_y0[kRows], s_x1[kRows], s_y1[kRows];
+  int tile, g;
+  tile_and_head(blockIdx.x, n_tiles, s.kv_heads, tile, g);
+  const Tile t = tiles[tile];
+  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int part = wave & 1, k0 = (wave >> 1) * 32, mine = k0 + col;
+  const bool active = k0 < t.rows;
+  const int group = s.heads / s.kv_heads;
+  const int64_t row = t.first + (int64_t)min(mine, t.rows - 1);
+
+  V8<T> kf[NS], vf[NS];
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    const int d = 16 * i + 8 * half, at = d < s.dim ? d : 0;
+    const V8<T> x = *reinterpret_cast<const V8<T>*>(k + row * k_token + g * k_head + at);
+    const V8<T> y = *reinterpret_cast<const V8<T>*>(v + row * v_token + g * v_head + at);
+    kf[i] = d < s.dim ? scaled_sign<T>(x, s.scale) : V8<T>{};
+    vf[i] = d < s.dim ? y : V8<T>{};
+  }
+  const float c = exp2_scale(s.scale);
+
+  // the queries that see this lane's key, those that see any of the wave's and of the tile's
+  int lo, hi, lo0, hi0, lo1, hi1, lot, hit, none;
+  seen_of(s, t, t.at + min(mine, t.rows - 1), lo, hi);
+  seen_of(s, t, t.at + min(k0, t.rows - 1), lo0, hi0);
+  seen_of(s, t, t.at + min(k0 + 31, t.rows - 1), lo1, hi1);
+  seen_of(s, t, t.at, lot, none);
+  seen_of(s, t, t.at + t.rows - 1, none, hit);
+
+  f32x16 ak[NT], av[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) ak[i] = av[i] = f32x16{};
+
+  const int r_at = L::row_at(lane) + part * 32 * L::PITCH;
+  const int c_at = L::col_at(lane) + part * 32 * L::PITCH;
+
+  auto load = [&](int a, int i0, char* sq, char* sg, float* sx, float* sy) {
+    const int n = min(kRows, t.nq - i0);
+    const int64_t first = (int64_t)t.q_begin + i0;
+    // the rows' offsets are made anew in every step: kept, they would not fit the registers
+    int l = lane;
+    asm volatile("" : "+v"(l));
+    load_rows<DP>(sq, q + first * q_token + a * q_head, n, (uint32_t)(2 * q_token), s.dim, wave, l);
+    load_rows<DP>(sg, go + first * go_token + a * go_head, n, (uint32_t)(2 * go_token), s.dim, wave, l);
+    if (wave < 2) {
+      const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<float*>(stats + (wave * s.heads + a) * q_tokens + first), 0, 4 * n, 0x00027000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rsrc, (__attribute__((address_space(3))) void*)(wave ? sy : sx), 4, 4 * l, 0, 0, 0);
     }
-    __syncthreads();
-    int lo = 0, hi = t.nq;  // the queries that see key j
-    if (s.causal) {
-      lo = j - t.nk + t.nq;
-      if (s.window && lo < t.nq - s.window) hi = lo + s.window;
-      if (lo < 0) lo = 0;
+  };
+
+  auto step = [&](int i0, const char* sq_, const char* sg_, const float* sx, const float* sy) {
+    const int i1 = i0 + 32 * part;  // the wave's first query
+    if (!active || i1 >= hi1 || i1 + 32 <= lo0) return;
+    const lds_char* sq = (const lds_char*)sq_;
+    const lds_char* sg = (const lds_char*)sg_;
+    int ra = r_at, ca = c_at;  // what is made of them is made anew, as in load
+    asm volatile("" : "+v"(ra), "+v"(ca));
+    f32x16 x, y;
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const f32x4 x0 = *reinterpret_cast<const f32x4*>(sx + 32 * part + 2 * r + 4 * half);
+      const f32x4 y0 = *reinterpret_cast<const f32x4*>(sy + 32 * part + 2 * r + 4 * half);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[r + e] = x0[e], y[r + e] = y0[e];
     }
-    float ak[2] = {0, 0}, av[2] = {0, 0};
-    for (int a = g * group; a < (g + 1) * group; ++a) {
-      for (int i0 = lo; i0 < hi; i0 += kWave) {
-        const int64_t i = t.q_begin + i0 + lane;
-        float p = 0, ds = 0;
-        if (i0 + lane < hi) {
-          const T* qr = q + i * q_token + a * q_head;
-          const T* gr = go + i * go_token + a * go_head;
-          float x = 0, dp = 0;
-          for (int d = 0; d < s.dim; ++d) {
-            x += s_k[d] * (float)qr[d];
-            dp += s_v[d] * (float)gr[d];
-          }
-          p = expf(x * s.scale - lse[i * s.heads + a]);
-          ds = p * (dp - delta[i * s.heads + a]) * s.scale;
-        }
-        for (int e = 0; e < kWave && i0 + e < hi; ++e) {
-          const float pe = __shfl(p, e), de = __shfl(ds, e);
-          const T* qr = q + (int64_t)(t.q_begin + i0 + e) * q_token + a * q_head;
-          const T* gr = go + (int64_t)(t.q_begin + i0 + e) * go_token + a * go_head;
-          for (int u = 0; u < 2; ++u)
-            if (lane + u * kWave < s.dim) {
-              ak[u] += de * (float)qr[lane + u * kWave];
-              av[u] += pe * (float)gr[lane + u * kWave];
-            }
-        }
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      x = mfma32(row_frag<T>(sq + (ra ^ (i * 32))), kf[i], x);
+      y = mfma32(row_frag<T>(sg + (ra ^ (i * 32))), vf[i], y);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      x[r] = __builtin_amdgcn_exp2f(x[r] * c);
+      y[r] *= x[r] * Lift<T>::down;
+    }
+    if (i1 + 32 > hi0 || i1 < lo1) {
+      const int first = lo - i1 - 4 * half, last = hi - i1 - 4 * half;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int i = 8 * (r / 4) + r % 4;
+        const bool in = i >= first && i < last;
+        x[r] = in ? x[r] : 0.0f;
+        y[r] = in ? y[r] : 0.0f;
       }
     }
-    for (int u = 0; u < 2; ++u)
-      if (lane + u * kWave < s.dim) {
-        dk[row * dk_token + g * dk_head + lane + u * kWave] = (T)ak[u];
-        dv[row * dv_token + g * dv_head + lane + u * kWave] = (T)av[u];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const V8<T> p = to16<T>(x, 8 * i), ds = to16<T>(y, 8 * i);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        av[n] = mfma32(col_frag<T, L::PITCH>(sg, ca ^ (64 * n), i), p, av[n]);
+        ak[n] = mfma32(col_frag<T, L::PITCH>(sq, ca ^ (64 * n), i), ds, ak[n]);
       }
+    }
+  };
+
+  // the steps of every head of the group, one after the other
+  const int steps = hit > lot ? (hit - lot + kRows - 1) / kRows : 0;
+  const int total = steps * group;
+  int a = g * group, i0 = lot, a1 = a, i1 = lot;  // of this step, and of the one being loaded
+  auto next = [&] {
+    i1 += kRows;
+    if (i1 >= hit) i1 = lot, ++a1;
+  };
+  if (total) load(a, i0, s_q0, s_g0, s_x0, s_y0);
+  __syncthreads();
+  for (int n = 0; n < total;) {
+    next();
+    if (n + 1 < total) load(a1, i1, s_q1, s_g1, s_x1, s_y1);
+    step(i0, s_q0, s_g0, s_x0, s_y0);
+    __syncthreads();
+    a = a1, i0 = i1;
+    if (++n >= total) break;
+    next();
+    if (n + 1 < total) load(a1, i1, s_q0, s_g0, s_x0, s_y0);
+    step(i0, s_q1, s_g1, s_x1, s_y1);
+    __syncthreads();
+    a = a1, i0 = i1;
+    ++n;
+  }
+
+  // join the two waves of the same keys, the even ones' sums first
+  float* joined = reinterpret_cast<float*>((wave >> 1) ? s_q1 : s_q0);
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    f32x16* acc = which ? ak : av;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      if (part == 1)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) joined[r * 64 + lane] = acc[i][r];
+      __syncthreads();
+      if (part == 0)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] += joined[r * 64 + lane];
+      __syncthreads();
+    }
+  }
+  if (part == 0 && mine < t.rows) {
+    store_rows<T, NT>(dv + row * dv_token + g * dv_head, av, Lift<T>::down, s.dim, half);
+    store_rows<T, NT>(dk + row * dk_token + g * dk_head, ak, s.scale, s.dim, half);
   }
 }
 
@@ -392,31 +607,37 @@ int launch_forward_dim(const fsp_attention_packed_args& a, hipStream_t st) {
   return launch_forward<T, 128>(a, st);
 }
 
-template <typename T>
+template <typename T, int DP>
 int launch_backward(const fsp_attention_packed_args& a, hipStream_t st) {
+  float* stats = static_cast<float*>(a.workspace);
   if (a.n_q_tiles > 0) {
-    hipLaunchKernelGGL((attention_grad_q_kernel<T>),
-                       dim3((unsigned)a.n_q_tiles, (unsigned)a.heads), dim3(kWave), 0, st,
-                       shape_of(a), reinterpret_cast<const Tile*>(a.q_tiles), in<T>(a.q),
-                       a.q_token, a.q_head, in<T>(a.k), a.k_token, a.k_head, in<T>(a.v),
-                       a.v_token, a.v_head, in<T>(a.out), a.out_token, a.out_head, a.lse,
-                       in<T>(a.grad_out), a.grad_out_token, a.grad_out_head,
-                       static_cast<T*>(a.grad_q), a.grad_q_token, a.grad_q_head,
-                       static_cast<float*>(a.workspace));
+    hipLaunchKernelGGL((attention_grad_q_kernel<T, DP>), dim3((unsigned)(a.n_q_tiles * a.heads)),
+                       dim3(256), 0, st, shape_of(a), reinterpret_cast<const Tile*>(a.q_tiles),
+                       (int)a.n_q_tiles, in<T>(a.q), a.q_token, a.q_head, in<T>(a.k), a.k_token,
+                       a.k_head, in<T>(a.v), a.v_token, a.v_head, in<T>(a.out), a.out_token,
+                       a.out_head, a.lse, in<T>(a.grad_out), a.grad_out_token, a.grad_out_head,
+                       static_cast<T*>(a.grad_q), a.grad_q_token, a.grad_q_head, stats,
+                       a.q_tokens);
     if (int rc = check_hip(hipGetLastError(), "attention_grad_q_kernel launch")) return rc;
   }
   if (a.n_k_tiles > 0) {
-    hipLaunchKernelGGL((attention_grad_kv_kernel<T>),
-                       dim3((unsigned)a.n_k_tiles, (unsigned)a.kv_heads), dim3(kWave), 0, st,
-                       shape_of(a), reinterpret_cast<const Tile*>(a.k_tiles), in<T>(a.q),
+    hipLaunchKernelGGL((attention_grad_kv_kernel<T, DP>),
+                       dim3((unsigned)(a.n_k_tiles * a.kv_heads)), dim3(256), 0, st, shape_of(a),
+                       reinterpret_cast<const Tile*>(a.k_tiles), (int)a.n_k_tiles, in<T>(a.q),
                        a.q_token, a.q_head, in<T>(a.k), a.k_token, a.k_head, in<T>(a.v),
-                       a.v_token, a.v_head, a.lse, in<T>(a.grad_out), a.grad_out_token,
-                       a.grad_out_head, static_cast<const float*>(a.workspace),
-                       static_cast<T*>(a.grad_k), a.grad_k_token, a.grad_k_head,
-                       static_cast<T*>(a.grad_v), a.grad_v_token, a.grad_v_head);
+                       a.v_token, a.v_head, in<T>(a.grad_out), a.grad_out_token, a.grad_out_head,
+                       stats, a.q_tokens, static_cast<T*>(a.grad_k), a.grad_k_token,
+                       a.grad_k_head, static_cast<T*>(a.grad_v), a.grad_v_token, a.grad_v_head);
     return check_hip(hipGetLastError(), "attention_grad_kv_kernel launch");
   }
   return FSP_OK;
+}
+
+template <typename T>
+int launch_backward_dim(const fsp_attention_packed_args& a, hipStream_t st) {
+  if (a.dim <= 64) return launch_backward<T, 64>(a, st);
+  if (a.dim <= 96) return launch_backward<T, 96>(a, st);
+  return launch_backward<T, 128>(a, st);
 }
 
 int check_packed(const fsp_attention_packed_args& a, const std::string& who) {
@@ -428,9 +649,12 @@ int check_packed(const fsp_attention_packed_args& a, const std::string& who) {
       a.q_tokens > 0x7fffffffLL || a.k_tokens > 0x7fffffffLL || a.window > 0x7fffffffLL ||
       a.n_q_tiles > kMaxBlocks / a.heads || a.n_k_tiles > kMaxBlocks / a.heads)
     return set_error(FSP_EINVAL, who + ": size out of range");
-  if ((a.k_tokens > 1 && (a.k_token < a.dim || a.v_token < a.dim)) || a.k_token > kTokenStep ||
-      a.v_token > kTokenStep)
-    return set_error(FSP_EINVAL, who + ": a key's step must lie between dim and 2^23");
+  auto step = [&](int64_t tokens, int64_t by) {
+    return (tokens < 2 || by >= a.dim) && by >= 0 && by <= kTokenStep;
+  };
+  if (!step(a.q_tokens, a.q_token) || !step(a.k_tokens, a.k_token) ||
+      !step(a.k_tokens, a.v_token) || (a.n_k_tiles > 0 && !step(a.q_tokens, a.grad_out_token)))
+    return set_error(FSP_EINVAL, who + ": a token's step must lie between dim and 2^23");
   if (a.window && !a.causal) return set_error(FSP_EINVAL, who + ": window needs causal");
   if ((a.n_q_tiles > 0 && (!a.q_tiles || !a.q || !a.out || !a.lse)) ||
       (a.n_k_tiles > 0 && !a.k_tiles) || (a.k_tokens > 0 && (!a.k || !a.v)))
@@ -446,7 +670,7 @@ int check_packed(const fsp_attention_packed_args& a, const std::string& who) {
 
 using namespace fsp;
 
-extern "C" int64_t fsp_attention_packed_tile(void) { return kTile; }
+extern "C" int64_t fsp_attention_packed_tile(int keys) { return keys ? kRows : kTile; }
 
 extern "C" int fsp_attention_packed(const fsp_attention_packed_args* args, void* stream) {
   if (!args) return set_error(FSP_EINVAL, "fsp_attention_packed: null arguments");
@@ -470,5 +694,5 @@ extern "C" int fsp_attention_packed_backward(const fsp_attention_packed_args* ar
       !aligned16(a.grad_v, a.grad_v_token, a.grad_v_head))
     return set_error(FSP_EINVAL, "fsp_attention_packed_backward: rows must be 16-byte aligned");
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return a.dtype == FSP_BF16 ? launch_backward<bf16>(a, st) : launch_backward<f16>(a, st);
+  return a.dtype == FSP_BF16 ? launch_backward_dim<bf16>(a, st) : launch_backward_dim<f16>(a, st);
 }

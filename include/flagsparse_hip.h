@@ -753,12 +753,12 @@ int fsp_attention_paged(const struct fsp_attention_paged_args* args, void* strea
  * i of nq sees key j of nk if j <= i + nk - nq; a window > 0 (causal only) hides the keys
  * j <= i + nk - nq - window.  lse [q_tokens, heads] float32.
  *
- * Work lists (fsp_attention_packed_tile()'s rows to a tile, any order): a tile is 8 int32,
+ * Work lists (fsp_attention_packed_tile(keys) rows to a tile, any order): a tile is 8 int32,
  * {first row, rows, first row's place in its sequence, sequence's q begin, q count, k begin,
  * k count, 0}; q_tiles cover the queries, k_tiles (backward only) the keys.
  *
  * Backward: grad_out by its steps, out and lse of the forward pass; grad_q, grad_k, grad_v are
- * written whole.  workspace: float32 [q_tokens, heads].
+ * written whole.  workspace: float32 [2, heads, q_tokens].
  */
 struct fsp_attention_packed_args {
   int64_t dtype, heads, kv_heads, dim, q_tokens, k_tokens, causal, window;
@@ -786,7 +786,7 @@ struct fsp_attention_packed_args {
   int64_t grad_v_token, grad_v_head;
   void* workspace;
 };
-int64_t fsp_attention_packed_tile(void);
+int64_t fsp_attention_packed_tile(int keys);
 int fsp_attention_packed(const struct fsp_attention_packed_args* args, void* stream);
 int fsp_attention_packed_backward(const struct fsp_attention_packed_args* args, void* stream);
 
