@@ -120,7 +120,8 @@ SIGNATURES = {
     "fsp_run": (_i32, [_p, _p, _p, _p]),
     "fsp_attention_dim_cap": (_i64, []),
     "fsp_paged_append": (_i32, [_p, _p]),
-    "fsp_attention_paged_workspace": (_i64, [_p]),
+    "fsp_attention_paged_piece": (_i64, [_i64, _i64]),
+    "fsp_attention_paged_workspace": (_i64, [_i64, _i64, _i64]),
     "fsp_attention_paged": (_i32, [_p, _p]),
     "fsp_attention_packed_tile": (_i64, [_i32]),
     "fsp_attention_packed": (_i32, [_p, _p]),

@@ -37,7 +37,7 @@ _STEP_CAP = 2**23
 # The argument structs of include/flagsparse_hip.h: 8-byte fields, "d" the scale.
 _CACHE = struct.Struct("7q 4q 4q 2q")
 _APPEND = struct.Struct("5q 3q 3q 3q 3q 4q")
-_PAGED = struct.Struct("2qd 3q 3q 3q")
+_PAGED = struct.Struct("2qd 3q 3q 3q 4q")
 _PACKED = struct.Struct("8qd 4q 3q 3q 3q 3q q 3q 3q 3q 3q q")
 
 
@@ -166,18 +166,23 @@ class PreparedPagedKV:
     most tokens that the pages of one sequence hold."""
 
     __slots__ = ("k_pages", "v_pages", "indptr", "indices", "batch", "n_pages", "page_size",
-                 "kv_heads", "dim", "room", "_streams", "_bytes")
+                 "kv_heads", "dim", "room", "_piece", "_pieces", "_slots", "_streams")
 
-    def __init__(self, k_pages, v_pages, indptr, indices, longest):
+    def __init__(self, k_pages, v_pages, indptr, indices, pages):
         self.k_pages = k_pages
         self.v_pages = v_pages
         self.indptr = indptr
         self.indices = indices
         self.batch = indptr.numel() - 1
         self.n_pages, self.page_size, self.kv_heads, self.dim = (int(n) for n in k_pages.shape)
-        self.room = int(longest) * self.page_size
+        rooms = pages * self.page_size
+        self.room = int(rooms.max()) if len(rooms) else 0
+        # the pieces that attention is cut into
+        self._piece = int(_abi.lib().fsp_attention_paged_piece(int(rooms.sum()), self.kv_heads))
+        table, slots = _pieces(rooms, self._piece)
+        both = torch.from_numpy(np.concatenate([table.ravel(), slots])).to(k_pages.device)
+        self._pieces, self._slots = both[:table.size].view(-1, 4), both[table.size:]
         self._streams = _Streams()
-        self._bytes = {}  # workspace of a decoding call, by number of heads
 
     @property
     def dtype(self):
@@ -197,7 +202,18 @@ class PreparedPagedKV:
 
     def _on(self, stream):
         if stream not in self._streams.seen:
-            self._streams.mark(stream, self.device, (self.indptr, self.indices))
+            self._streams.mark(stream, self.device, (self.indptr, self.indices, self._pieces))
+
+
+def _pieces(rooms, piece):
+    """(the pieces of ``piece`` tokens that sequences with these rooms may come to hold, each sequence's
+    first), as the kernels read them."""
+    n = np.maximum(1, -(-rooms // piece))
+    slots = np.cumsum(n) - n
+    seq = np.repeat(np.arange(len(rooms)), n)
+    at = np.arange(len(seq)) - slots[seq]
+    table = np.stack([seq, at * piece, slots[seq], np.zeros_like(seq)], axis=1)
+    return table.astype(np.int32), slots.astype(np.int32)
 
 
 def _check_pages(t, name):
@@ -246,7 +262,7 @@ def prepare_paged_kv(k_pages, v_pages, indptr, indices):
         raise ValueError("indptr must have at least one entry")
     if indices.numel() * page_size > _TOKENS_CAP:
         raise ValueError("the page table must hold fewer than 2^31 tokens")
-    (first, last, decreases, longest, least, most), idx, ptr = csr_check(
+    (first, last, decreases, _, least, most), idx, ptr = csr_check(
         indices.contiguous(), indptr.contiguous(), 32)
     if first != 0:
         raise ValueError("indptr[0] must be 0")
@@ -261,8 +277,10 @@ def prepare_paged_kv(k_pages, v_pages, indptr, indices):
         idx = idx.clone()
     if ptr.data_ptr() == indptr.data_ptr():
         ptr = ptr.clone()
+    pages = np.diff(ptr.cpu().numpy().astype(np.int64))
+    prepared = PreparedPagedKV(k_pages, v_pages, ptr, idx, pages)
     torch.cuda.current_stream(k_pages.device).synchronize()  # calls may come from other streams
-    return PreparedPagedKV(k_pages, v_pages, ptr, idx, longest if indices.numel() else 0)
+    return prepared
 
 
 def _paged_of(prepared, k_pages, v_pages, indptr, indices, lengths):
@@ -383,20 +401,16 @@ def flagsparse_attention_paged(q, lengths, *, prepared=None, k_pages=None, v_pag
         stream = _abi.raw_stream(dev)
         kv._on(stream)
         L = _abi.lib()
-        cache = kv._packed()
-
-        def pack(workspace):
-            return cache + _PAGED.pack(
-                heads, window, scale, q.data_ptr(), q.stride(0), q.stride(1), res.data_ptr(),
-                res.stride(0), res.stride(1), 0 if lse is None else lse.data_ptr(), n.data_ptr(),
-                workspace)
-
-        need = kv._bytes.get(heads)
-        if need is None:
-            need = kv._bytes[heads] = int(L.fsp_attention_paged_workspace(pack(0)))
-        work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        _abi.check(L.fsp_attention_paged(pack(0 if work is None else work.data_ptr()), stream),
-                   "fsp_attention_paged")
+        n_pieces, work = kv._pieces.shape[0], None
+        if n_pieces > kv.batch:
+            work = torch.empty(int(L.fsp_attention_paged_workspace(n_pieces, heads, kv.dim)),
+                               dtype=torch.uint8, device=dev)
+        args = kv._packed() + _PAGED.pack(
+            heads, window, scale, q.data_ptr(), q.stride(0), q.stride(1), res.data_ptr(),
+            res.stride(0), res.stride(1), 0 if lse is None else lse.data_ptr(), n.data_ptr(),
+            0 if work is None else work.data_ptr(), kv._pieces.data_ptr(), kv._slots.data_ptr(),
+            n_pieces, kv._piece)
+        _abi.check(L.fsp_attention_paged(args, stream), "fsp_attention_paged")
     if copied:
         out.copy_(res)
         res = out

@@ -143,21 +143,6 @@ __device__ __forceinline__ void store_rows(T* to, const f32x16 (&x)[NT], float f
     }
 }
 
-// Scores are scale * q . k, and weights exp(score - max) = exp2(c q . k - c max) with c = scale *
-// log2(e) > 0: a negative scale turns the sign of one factor, and one that is zero, or too small to
-// show in 32 bits, makes it zero.
-constexpr float kNoScale = 1e-30f;
-
-template <typename T>
-__device__ __forceinline__ V8<T> scaled_sign(V8<T> q, float scale) {
-  if (scale > kNoScale) return q;
-  return scale < -kNoScale ? -q : V8<T>{};
-}
-
-__device__ __forceinline__ float exp2_scale(float scale) {
-  return fabsf(scale) > kNoScale ? fabsf(scale) * kLog2e : 1.0f;
-}
-
 template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void attention_packed_kernel(
     Shape s, const Tile* __restrict__ tiles, int n_tiles, const T* __restrict__ q, int64_t q_token,

@@ -70,6 +70,21 @@ __device__ __forceinline__ float other_half(float v) {
   return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
 }
 
+// Scores are scale * q . k, and weights exp(score - max) = exp2(c q . k - c max) with c = scale *
+// log2(e) > 0: a negative scale turns the sign of one factor, and one that is zero, or too small to
+// show in 32 bits, makes it zero.
+constexpr float kNoScale = 1e-30f;
+
+template <typename T>
+__device__ __forceinline__ V8<T> scaled_sign(V8<T> q, float scale) {
+  if (scale > kNoScale) return q;
+  return scale < -kNoScale ? -q : V8<T>{};
+}
+
+__device__ __forceinline__ float exp2_scale(float scale) {
+  return fabsf(scale) > kNoScale ? fabsf(scale) * kLog2e : 1.0f;
+}
+
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
   for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));

@@ -81,55 +81,262 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(
   }
 }
 
-// One wave a query row: 64 keys at a time, a lane to a key for the scores and to elements of the
-// head for the products.
-template <typename T>
-__global__ __launch_bounds__(kWave) void attention_paged_kernel(
-    Cache c, const T* __restrict__ k_pages, const T* __restrict__ v_pages,
-    const T* __restrict__ q, int64_t q_token, int64_t q_head, T* __restrict__ out,
-    int64_t out_token, int64_t out_head, float* __restrict__ lse,
-    const int32_t* __restrict__ lengths, int heads, int window, float scale) {
-  __shared__ float s_q[kAttnDimCap];
-  const int b = blockIdx.x / heads, a = blockIdx.x % heads, lane = threadIdx.x;
-  const int g = a / (heads / c.kv_heads);
-  const T* qr = q + b * q_token + a * q_head;
-  for (int d = lane; d < c.dim; d += kWave) s_q[d] = (float)qr[d];
-  __syncthreads();
-  const int first = c.indptr[b], last = c.indptr[b + 1], n = lengths[b];
-  const bool ok = n >= 0 && n <= (int64_t)(last - first) * c.page_size;
-  float m = -INFINITY, l = 0, acc[2] = {0, 0};
-  for (int j0 = window && n > window ? n - window : 0; ok && j0 < n; j0 += kWave) {
-    const int j = j0 + lane;
-    float s = -INFINITY;
-    int64_t voff = 0;
-    if (j < n) {
-      const int64_t page = c.indices[first + j / c.page_size];
-      const T* kr = k_pages + page * c.k_page + (j % c.page_size) * c.k_slot + g * c.k_head;
-      voff = page * c.v_page + (j % c.page_size) * c.v_slot + g * c.v_head;
-      s = 0;
-      for (int d = 0; d < c.dim; ++d) s += s_q[d] * (float)kr[d];
-      s *= scale;
-    }
-    const float top = fmaxf(m, wave_max(s));
-    const float base = top == -INFINITY ? 0.0f : top;
-    const float p = expf(s - base), fade = expf(m - base);
-    l = l * fade + wave_add(p);
-    acc[0] *= fade;
-    acc[1] *= fade;
-    m = top;
-    for (int e = 0; e < kWave && j0 + e < n; ++e) {
-      const float pe = __shfl(p, e);
-      const T* vr = v_pages + __shfl(voff, e);
-      for (int u = 0; u < 2; ++u)
-        if (lane + u * kWave < c.dim) acc[u] += pe * (float)vr[lane + u * kWave];
+// Attention of one query per sequence.  A workgroup takes a piece of a sequence's tokens for one key
+// head and up to 16 of the query heads that share it; its four waves take every fourth 32 keys.
+//
+// Keys and values go from memory to the matrix instructions' registers with no stop in LDS.  With
+// S^T = K Q^T lane l has head l % 16 and, of 32 keys, the eight 4 * (l / 16) + {0..3, 16..19}: its
+// weights are the operand of O^T = V^T P^T as they lie, since the order of the summed keys is free.
+// For V a lane loads DP / 16 consecutive elements of those same eight keys, and the operand of one
+// product is one element of each: pairs of 16-bit halves, a byte permutation each.  Row m of product
+// i is element DP / 16 * m + i of the head, so a lane's results are consecutive.
+//
+// Where each key lies (its page, its place in it) is found once for the piece and kept in LDS.
+constexpr int kHeadTile = 16;
+constexpr int kPieceMost = 1024;
+
+struct Piece {
+  int seq, begin, slot, pad;  // tokens [begin, begin + piece) of seq; slot: of the sequence's first piece
+};
+
+struct PagedShape {
+  int heads, window, piece;
+  float scale;
+};
+
+// Tokens [first, last) are seen by the query; ok: the pages hold them.
+__device__ __forceinline__ bool paged_range(const Cache& c, int b, int n, int window, int& first,
+                                            int& last) {
+  const bool ok = n >= 0 && n <= (int64_t)(c.indptr[b + 1] - c.indptr[b]) * c.page_size;
+  last = ok ? n : 0;
+  first = window && last > window ? last - window : 0;
+  return ok;
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attention_paged_kernel(
+    Cache c, PagedShape s, const Piece* __restrict__ pieces, const T* __restrict__ k_pages,
+    const T* __restrict__ v_pages, const T* __restrict__ q, int64_t q_token, int64_t q_head,
+    T* __restrict__ out, int64_t out_token, int64_t out_head, float* __restrict__ lse,
+    const int32_t* __restrict__ lengths, float* __restrict__ part_o, f32x2* __restrict__ part_ml) {
+  constexpr int E = DP / 16, NS = DP / 32, W = 4;  // elements of V and steps of K a lane; waves
+  typedef T VE __attribute__((ext_vector_type(E)));
+  __shared__ int64_t s_k[kPieceMost], s_v[kPieceMost];
+  __shared__ f32x2 s_ml[W][kHeadTile];
+  __shared__ __attribute__((aligned(16))) float s_o[W][kHeadTile][DP + 4];
+
+  const int group = s.heads / c.kv_heads, tiles = (group + kHeadTile - 1) / kHeadTile;
+  int id = blockIdx.x;
+  const int g = id % c.kv_heads;
+  id /= c.kv_heads;
+  const int ht = id % tiles;
+  const Piece pc = pieces[id / tiles];
+  const int b = pc.seq, lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int first, last;
+  const bool ok = paged_range(c, b, lengths[b], s.window, first, last);
+  const int n_heads = min(kHeadTile, group - ht * kHeadTile), head0 = g * group + ht * kHeadTile;
+  // the sequence's pieces in use, and whether this one is
+  const int p0 = first / s.piece, p1 = max(p0 + 1, (last + s.piece - 1) / s.piece);
+  const int mine = pc.begin / s.piece;
+  if (mine < p0 || mine >= p1) return;
+  const int begin = max(first, pc.begin), n = min(last, pc.begin + s.piece) - begin;
+
+  V8<T> qf[NS];
+  {
+    const T* qr = q + b * q_token + (head0 + min(col, n_heads - 1)) * q_head;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const int d = 32 * i + 8 * quad;
+      const V8<T> x = *reinterpret_cast<const V8<T>*>(qr + (d < c.dim ? d : 0));
+      qf[i] = d < c.dim ? scaled_sign<T>(x, s.scale) : V8<T>{};
     }
   }
-  T* o = out + b * out_token + a * out_head;
+  const float cs = exp2_scale(s.scale);
+
+  // where the keys lie; those past the end stand for the first one, and weigh nothing
+  const int padded = (n + 127) & ~127;
+  const int pages = c.indptr[b];
+  for (int i = threadIdx.x; i < padded; i += 256) {
+    const uint32_t j = begin + (i < n ? i : 0);
+    const uint32_t at = j / (uint32_t)c.page_size;
+    const int64_t page = n > 0 ? c.indices[pages + at] : 0, slot = j - at * c.page_size;
+    s_k[i] = page * c.k_page + slot * c.k_slot;
+    s_v[i] = page * c.v_page + slot * c.v_slot;
+  }
+  __syncthreads();
+
+  const T* kb = k_pages + g * c.k_head;
+  const T* vb = v_pages + g * c.v_head;
+  V8<T> kf[2][NS];
+  VE vf[8];
+  auto load_k = [&](int j) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const T* row = kb + s_k[j + 16 * u + col];
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        const int d = 32 * i + 8 * quad;
+        kf[u][i] = *reinterpret_cast<const V8<T>*>(row + (d < c.dim ? d : 0));
+      }
+    }
+    if (c.dim < DP) {  // past the head: zeros, as in q, or an infinity there would show
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < NS; ++i) kf[u][i] = 32 * i + 8 * quad < c.dim ? kf[u][i] : V8<T>{};
+    }
+  };
+  const int ve = E * col < c.dim ? E * col : 0;
+  auto load_v = [&](int j) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      vf[e] = *reinterpret_cast<const VE*>(vb + s_v[j + 16 * (e / 4) + 4 * quad + e % 4] + ve);
+  };
+
+  float top = -INFINITY, sum = 0;
+  f32x4 o[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) o[i] = f32x4{};
+
+  int j = 32 * wave;
+  if (j < n) load_k(j), load_v(j);
+  for (; j < n; j += 32 * W) {
+    f32x4 x[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      x[u] = f32x4{};
+#pragma unroll
+      for (int i = 0; i < NS; ++i) x[u] = mfma16(kf[u][i], qf[i], x[u]);
+    }
+    if (j + 32 * W < n) load_k(j + 32 * W);
+    const bool partial = j + 32 > n;
+    if (partial) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool in = j + 16 * (e / 4) + 4 * quad + e % 4 < n;
+        x[e / 4][e % 4] = in ? x[e / 4][e % 4] : -INFINITY;
+        vf[e] = in ? vf[e] : VE{};
+      }
+    }
+    float m = x[0][0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) m = fmaxf(m, x[e / 4][e % 4]);
+    // the weights are taken against an older maximum until a head's grows by more than 2^8 of it
+    if (__any((m - top) * cs > 8.0f)) {
+      m = fmaxf(m, __shfl_xor(m, 16));
+      m = fmaxf(m, __shfl_xor(m, 32));
+      const float now = fmaxf(top, m);
+      const float fade = top == -INFINITY ? 0.0f : exp2f((top - now) * cs);
+      top = now;
+      sum *= fade;
+#pragma unroll
+      for (int i = 0; i < E; ++i) o[i] *= fade;
+    }
+    const float base = top == -INFINITY ? 0.0f : top * cs;
+    f32x8 p;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      p[e] = __builtin_amdgcn_exp2f(fmaf(x[e / 4][e % 4], cs, -base));
+      sum += p[e];
+    }
+    const V8<T> pf = __builtin_convertvector(p, V8<T>);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      V8<T> a;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a[e] = vf[e][i];
+      o[i] = mfma16(a, pf, o[i]);
+    }
+    if (j + 32 * W < n) load_v(j + 32 * W);
+  }
+
+  // join the waves
+  sum += __shfl_xor(sum, 16);
+  sum += __shfl_xor(sum, 32);
+  const float ml = top == -INFINITY ? -INFINITY : top * cs;
+  if (quad == 0) s_ml[wave][col] = f32x2{ml, sum};
+#pragma unroll
+  for (int i = 0; i < E; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s_o[wave][col][4 * E * quad + E * r + i] = o[i][r];
+  __syncthreads();
+  const bool split = p1 - p0 > 1;
   const float nan = __builtin_nanf("");
-  for (int u = 0; u < 2; ++u)
-    if (lane + u * kWave < c.dim)
-      o[lane + u * kWave] = (T)(!ok ? nan : l > 0 ? acc[u] / l : acc[u]);
-  if (lse && lane == 0) lse[(int64_t)b * heads + a] = ok ? m + logf(l) : nan;
+  for (int i = threadIdx.x; i < n_heads * (DP / 4); i += 256) {
+    const int h = i / (DP / 4), d = i % (DP / 4) * 4;
+    if (d >= c.dim) continue;
+    float most = -INFINITY, total = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) most = fmaxf(most, s_ml[w][h].x);
+    f32x4 y{};
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const f32x2 v = s_ml[w][h];
+      const float f = v.x == -INFINITY ? 0.0f : exp2f(v.x - most);
+      if (v.y == 0) continue;  // saw nothing: its sums are zeros
+      total += f * v.y;
+      y += f * *reinterpret_cast<const f32x4*>(&s_o[w][h][d]);
+    }
+    if (split) {
+      const int64_t at = ((int64_t)(pc.slot + mine)) * s.heads + head0 + h;
+      *reinterpret_cast<f32x4*>(part_o + at * c.dim + d) = y;
+      if (d == 0) part_ml[at] = f32x2{most, total};
+    } else {
+      const float f = total == 0 ? 0.0f : 1.0f / total;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = ok ? y[e] * f : nan;
+      *reinterpret_cast<V4<T>*>(out + b * out_token + (head0 + h) * out_head + d) =
+          __builtin_convertvector(y, V4<T>);
+      if (lse && d == 0)
+        lse[(int64_t)b * s.heads + head0 + h] =
+            !ok ? nan : total == 0 ? -INFINITY : (most + log2f(total)) * kLn2;
+    }
+  }
+}
+
+// Joins the pieces of sequences that have several: a workgroup a sequence and head, a wave to every
+// fourth piece.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_paged_join_kernel(
+    Cache c, PagedShape s, const int32_t* __restrict__ slots, T* __restrict__ out,
+    int64_t out_token, int64_t out_head, float* __restrict__ lse,
+    const int32_t* __restrict__ lengths, const float* __restrict__ part_o,
+    const f32x2* __restrict__ part_ml) {
+  __shared__ f32x2 s_ml[4];
+  __shared__ f32x2 s_o[4][64];
+  const int b = blockIdx.x / s.heads, h = blockIdx.x % s.heads;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int first, last;
+  paged_range(c, b, lengths[b], s.window, first, last);
+  const int p0 = first / s.piece, p1 = max(p0 + 1, (last + s.piece - 1) / s.piece);
+  if (p1 - p0 < 2) return;
+  const int64_t at = (int64_t)slots[b] * s.heads + h;
+  float most = -INFINITY, total = 0;
+  for (int p = p0 + lane; p < p1; p += 64) most = fmaxf(most, part_ml[at + (int64_t)p * s.heads].x);
+  most = wave_max(most);
+  f32x2 y{};
+  const int d = 2 * lane < c.dim ? 2 * lane : 0;
+  for (int p = p0 + wave; p < p1; p += 4) {
+    const int64_t i = at + (int64_t)p * s.heads;
+    const f32x2 v = part_ml[i];
+    const float f = v.x == -INFINITY ? 0.0f : exp2f(v.x - most);
+    total += f * v.y;
+    y += f * *reinterpret_cast<const f32x2*>(part_o + i * c.dim + d);
+  }
+  if (lane == 0) s_ml[wave] = f32x2{most, total};
+  s_o[wave][lane] = y;
+  __syncthreads();
+  if (wave) return;
+  total = s_ml[0].y + s_ml[1].y + s_ml[2].y + s_ml[3].y;
+  y = s_o[0][lane] + s_o[1][lane] + s_o[2][lane] + s_o[3][lane];
+  const float f = total == 0 ? 0.0f : 1.0f / total;
+  if (2 * lane < c.dim) {
+    T* to = out + b * out_token + h * out_head + 2 * lane;
+    to[0] = (T)(y.x * f);
+    to[1] = (T)(y.y * f);
+  }
+  if (lse && lane == 0) lse[(int64_t)b * s.heads + h] = total == 0 ? -INFINITY : (most + log2f(total)) * kLn2;
 }
 
 int check_cache(const fsp_paged_cache& c, const std::string& who) {
@@ -165,15 +372,34 @@ int launch_append(const fsp_paged_append_args& a, hipStream_t st) {
   return check_hip(hipGetLastError(), "paged_append_kernel launch");
 }
 
-template <typename T>
+int64_t paged_workgroups(const fsp_attention_paged_args& a) {
+  const int64_t group = a.heads / a.cache.kv_heads;
+  return a.n_pieces * a.cache.kv_heads * ((group + kHeadTile - 1) / kHeadTile);
+}
+
+template <typename T, int DP>
 int launch_paged(const fsp_attention_paged_args& a, hipStream_t st) {
-  hipLaunchKernelGGL((attention_paged_kernel<T>), dim3((unsigned)(a.cache.batch * a.heads)),
-                     dim3(kWave), 0, st, cache_of(a.cache),
+  const PagedShape s{(int)a.heads, (int)a.window, (int)a.piece, (float)a.scale};
+  float* part_o = static_cast<float*>(a.workspace);
+  f32x2* part_ml = reinterpret_cast<f32x2*>(part_o + a.n_pieces * a.heads * a.cache.dim);
+  hipLaunchKernelGGL((attention_paged_kernel<T, DP>), dim3((unsigned)paged_workgroups(a)),
+                     dim3(256), 0, st, cache_of(a.cache), s,
+                     reinterpret_cast<const Piece*>(a.pieces),
                      static_cast<const T*>(a.cache.k_pages),
                      static_cast<const T*>(a.cache.v_pages), static_cast<const T*>(a.q),
                      a.q_token, a.q_head, static_cast<T*>(a.out), a.out_token, a.out_head, a.lse,
-                     a.lengths, (int)a.heads, (int)a.window, (float)a.scale);
-  return check_hip(hipGetLastError(), "attention_paged_kernel launch");
+                     a.lengths, part_o, part_ml);
+  if (int rc = check_hip(hipGetLastError(), "attention_paged_kernel launch")) return rc;
+  if (a.n_pieces == a.cache.batch) return FSP_OK;  // a piece each
+  hipLaunchKernelGGL((attention_paged_join_kernel<T>), dim3((unsigned)(a.cache.batch * a.heads)),
+                     dim3(256), 0, st, cache_of(a.cache), s, a.slots, static_cast<T*>(a.out),
+                     a.out_token, a.out_head, a.lse, a.lengths, part_o, part_ml);
+  return check_hip(hipGetLastError(), "attention_paged_join_kernel launch");
+}
+
+template <typename T>
+int launch_paged_dim(const fsp_attention_paged_args& a, hipStream_t st) {
+  return a.cache.dim <= 64 ? launch_paged<T, 64>(a, st) : launch_paged<T, 128>(a, st);
 }
 
 }  // namespace
@@ -205,31 +431,38 @@ extern "C" int fsp_paged_append(const fsp_paged_append_args* args, void* stream)
   return a.cache.dtype == FSP_BF16 ? launch_append<bf16>(a, st) : launch_append<f16>(a, st);
 }
 
-static int check_paged(const fsp_attention_paged_args& a) {
-  const char* who = "fsp_attention_paged";
-  if (int rc = check_cache(a.cache, who)) return rc;
-  if (a.heads < 1 || a.heads % a.cache.kv_heads || a.heads > 0xffff)
-    return set_error(FSP_EINVAL, "fsp_attention_paged: heads must be a multiple of kv_heads");
-  if (a.window < 0 || a.window > 0x7fffffffLL)
-    return set_error(FSP_EINVAL, "fsp_attention_paged: window");
-  if (a.cache.batch * a.heads > kMaxBlocks)
-    return set_error(FSP_EINVAL, "fsp_attention_paged: more rows than a launch holds");
-  return FSP_OK;
+extern "C" int64_t fsp_attention_paged_piece(int64_t tokens, int64_t kv_heads) {
+  // a thousand workgroups, if pieces of 128 tokens (one step of the four waves) give them
+  int64_t piece = 128;
+  while (piece < kPieceMost && tokens / piece * kv_heads > 1024) piece *= 2;
+  return piece;
 }
 
-extern "C" int64_t fsp_attention_paged_workspace(const fsp_attention_paged_args* args) {
-  return 0;
+extern "C" int64_t fsp_attention_paged_workspace(int64_t n_pieces, int64_t heads, int64_t dim) {
+  if (n_pieces < 0 || heads < 0 || dim < 0) return 0;
+  return n_pieces * heads * (dim + 2) * (int64_t)sizeof(float);
 }
 
 extern "C" int fsp_attention_paged(const fsp_attention_paged_args* args, void* stream) {
   if (!args) return set_error(FSP_EINVAL, "fsp_attention_paged: null arguments");
   const fsp_attention_paged_args& a = *args;
-  if (int rc = check_paged(a)) return rc;
+  if (int rc = check_cache(a.cache, "fsp_attention_paged")) return rc;
+  if (a.heads < 1 || a.heads % a.cache.kv_heads || a.heads > 0xffff)
+    return set_error(FSP_EINVAL, "fsp_attention_paged: heads must be a multiple of kv_heads");
+  if (a.window < 0 || a.window > 0x7fffffffLL)
+    return set_error(FSP_EINVAL, "fsp_attention_paged: window");
+  if (a.piece < 128 || a.piece > kPieceMost || a.piece % 128)
+    return set_error(FSP_EINVAL, "fsp_attention_paged: piece must be a multiple of 128 up to 1024");
+  if (a.n_pieces < a.cache.batch || a.n_pieces > 0x7fffffffLL || a.cache.batch * a.heads > kMaxBlocks ||
+      paged_workgroups(a) > kMaxBlocks)
+    return set_error(FSP_EINVAL, "fsp_attention_paged: pieces out of range");
   if (a.cache.batch == 0) return FSP_OK;
-  if (!a.q || !a.out || !a.lengths)
+  if (!a.q || !a.out || !a.lengths || !a.pieces || !a.slots ||
+      (a.n_pieces > a.cache.batch && !a.workspace))
     return set_error(FSP_EINVAL, "fsp_attention_paged: null pointer");
-  if (!aligned16(a.q, a.q_token, a.q_head) || !aligned16(a.out, a.out_token, a.out_head))
+  if (!aligned16(a.q, a.q_token, a.q_head) || !aligned16(a.out, a.out_token, a.out_head) ||
+      reinterpret_cast<uintptr_t>(a.workspace) % 16)
     return set_error(FSP_EINVAL, "fsp_attention_paged: rows must be 16-byte aligned");
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return a.cache.dtype == FSP_BF16 ? launch_paged<bf16>(a, st) : launch_paged<f16>(a, st);
+  return a.cache.dtype == FSP_BF16 ? launch_paged_dim<bf16>(a, st) : launch_paged_dim<f16>(a, st);
 }

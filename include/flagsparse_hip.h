@@ -730,7 +730,13 @@ int fsp_paged_append(const struct fsp_paged_append_args* args, void* stream);
  * Attention of one query per sequence over the cache: q, out [batch, heads, dim], lse
  * [batch, heads] float32 or NULL.  Key j of sequence b is seen if j >= lengths[b] - window
  * (window 0: every key).  A length that is negative or more than the sequence's pages hold gives
- * NaN.  workspace: fsp_attention_paged_workspace() bytes (0: NULL will do).
+ * NaN.
+ *
+ * The work is cut into pieces of `piece` tokens (fsp_attention_paged_piece() for a cache whose table
+ * has room for `tokens` of them): pieces [n_pieces, 4] holds {sequence, first token, slots[sequence],
+ * 0} for each piece of each sequence's room, in order, one at least for each; slots [batch] the
+ * number of pieces before the sequence's first.  workspace: fsp_attention_paged_workspace() bytes,
+ * 16-byte aligned, unless every sequence has one piece.
  */
 struct fsp_attention_paged_args {
   struct fsp_paged_cache cache;
@@ -743,8 +749,12 @@ struct fsp_attention_paged_args {
   float* lse;
   const int32_t* lengths;
   void* workspace;
+  const int32_t* pieces;
+  const int32_t* slots;
+  int64_t n_pieces, piece;
 };
-int64_t fsp_attention_paged_workspace(const struct fsp_attention_paged_args* args);
+int64_t fsp_attention_paged_piece(int64_t tokens, int64_t kv_heads);
+int64_t fsp_attention_paged_workspace(int64_t n_pieces, int64_t heads, int64_t dim);
 int fsp_attention_paged(const struct fsp_attention_paged_args* args, void* stream);
 
 /*

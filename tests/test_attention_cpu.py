@@ -50,9 +50,29 @@ def test_struct_sizes():
     # 8-byte fields, as in the header
     assert attention._CACHE.size == 8 * 17
     assert attention._APPEND.size == 8 * 21
-    assert attention._PAGED.size == 8 * 12
+    assert attention._PAGED.size == 8 * 16
     assert attention._PACKED.size == 8 * (9 + 4 + 12 + 1 + 12 + 1)
     assert _abi.lib().fsp_attention_dim_cap() == attention._DIM_CAP
+
+
+@pytest.mark.parametrize("rooms", [[], [0], [128, 0, 129, 1], [5000, 16, 128]])
+def test_pieces_cover_the_rooms(rooms):
+    table, slots = attention._pieces(np.array(rooms, dtype=np.int64), 128)
+    at = 0
+    for b, room in enumerate(rooms):
+        assert slots[b] == at
+        for i in range(max(1, -(-room // 128))):
+            assert table[at].tolist() == [b, 128 * i, slots[b], 0]
+            at += 1
+    assert at == len(table)
+
+
+def test_piece_sizes():
+    L = _abi.lib()
+    for tokens in (0, 1, 1000, 50000, 10**6, 2**31):
+        for heads in (1, 8, 64):
+            piece = L.fsp_attention_paged_piece(tokens, heads)
+            assert 128 <= piece <= 1024 and piece % 128 == 0
 
 
 def _packed(**kw):
@@ -96,7 +116,7 @@ def _cache(**kw):
 
 
 _PAGED_ARGS = dict(heads=4, window=0, scale=0.125, q=64, qt=256, qh=64, out=64, ot=256, oh=64, lse=0,
-                   lengths=16, work=16)
+                   lengths=16, work=16, pieces=16, slots=16, n_pieces=3, piece=128)
 _APPEND_ARGS = dict(n_tokens=2, heads=4, half=32, rows=64, interleaved=0, k=64, kt=128, kh=64, v=64,
                     vt=128, vh=64, q=64, qt=256, qh=64, qo=64, qot=256, qoh=64, cos=16, sin=16,
                     tokens=0, lengths=16)
@@ -115,7 +135,9 @@ def test_cache_refusals_of_the_library(status, kw):
 
 
 @pytest.mark.parametrize("kw", [{"heads": 3}, {"heads": 0}, {"window": -1}, {"q": 0}, {"out": 0},
-                                {"lengths": 0}, {"q": 72}, {"oh": 2}])
+                                {"lengths": 0}, {"q": 72}, {"oh": 2}, {"work": 0}, {"work": 8},
+                                {"pieces": 0}, {"slots": 0}, {"n_pieces": 1}, {"n_pieces": 1 << 40},
+                                {"piece": 0}, {"piece": 2048}, {"piece": 130}])
 def test_paged_refusals_of_the_library(kw):
     L = _abi.lib()
     args = _cache() + attention._PAGED.pack(*(_PAGED_ARGS | kw).values())
