@@ -674,7 +674,8 @@ int fsp_run(const void* call, const void* in, void* out, void* stream);
  * aligned; packed arrays have token steps from dim to 2^23.  heads is a multiple of kv_heads; query head a reads key head a / (heads / kv_heads).
  * Sums, softmax statistics and gradients are held in 32 bits and rounded once at the end; the
  * weights are rounded to the inputs' type before their product with the values (the matrix
- * instructions' operand type).  The arguments come as a struct of 8-byte fields.
+ * instructions' operand type).  The arguments come as a struct of 8-byte fields, those that change
+ * from call to call at its end.
  *
  * With S_ij = scale * q_i . k_j over the keys j that query i sees, lse_i = log sum_j exp(S_ij),
  * P_ij = exp(S_ij - lse_i): out_i = sum_j P_ij v_j.  A query that sees no key has out 0 and lse
@@ -711,14 +712,11 @@ struct fsp_paged_cache {
 struct fsp_paged_append_args {
   struct fsp_paged_cache cache;
   int64_t n_tokens, heads, half, table_rows, interleaved;
+  int64_t k_token, k_head, v_token, v_head, q_token, q_head, q_out_token, q_out_head;
   const void* k;
-  int64_t k_token, k_head;
   const void* v;
-  int64_t v_token, v_head;
   const void* q;
-  int64_t q_token, q_head;
   void* q_out;
-  int64_t q_out_token, q_out_head;
   const float* cos;
   const float* sin;
   const int32_t* token_indptr;
@@ -740,18 +738,16 @@ int fsp_paged_append(const struct fsp_paged_append_args* args, void* stream);
  */
 struct fsp_attention_paged_args {
   struct fsp_paged_cache cache;
-  int64_t heads, window;
+  const int32_t* pieces;
+  const int32_t* slots;
+  int64_t n_pieces, piece, heads, window;
   double scale;
+  int64_t q_token, q_head, out_token, out_head;
   const void* q;
-  int64_t q_token, q_head;
   void* out;
-  int64_t out_token, out_head;
   float* lse;
   const int32_t* lengths;
   void* workspace;
-  const int32_t* pieces;
-  const int32_t* slots;
-  int64_t n_pieces, piece;
 };
 int64_t fsp_attention_paged_piece(int64_t tokens, int64_t kv_heads);
 int64_t fsp_attention_paged_workspace(int64_t n_pieces, int64_t heads, int64_t dim);
@@ -777,23 +773,18 @@ struct fsp_attention_packed_args {
   int64_t n_q_tiles;
   const int32_t* k_tiles;
   int64_t n_k_tiles;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;
+  int64_t grad_out_token, grad_out_head, grad_q_token, grad_q_head;
+  int64_t grad_k_token, grad_k_head, grad_v_token, grad_v_head;
   const void* q;
-  int64_t q_token, q_head;
   const void* k;
-  int64_t k_token, k_head;
   const void* v;
-  int64_t v_token, v_head;
   void* out;
-  int64_t out_token, out_head;
   float* lse;
   const void* grad_out;
-  int64_t grad_out_token, grad_out_head;
   void* grad_q;
-  int64_t grad_q_token, grad_q_head;
   void* grad_k;
-  int64_t grad_k_token, grad_k_head;
   void* grad_v;
-  int64_t grad_v_token, grad_v_head;
   void* workspace;
 };
 int64_t fsp_attention_packed_tile(int keys);

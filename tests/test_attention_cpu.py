@@ -49,9 +49,9 @@ def test_exports_have_a_name_in_the_package():
 def test_struct_sizes():
     # 8-byte fields, as in the header
     assert attention._CACHE.size == 8 * 17
-    assert attention._APPEND.size == 8 * 21
-    assert attention._PAGED.size == 8 * 16
-    assert attention._PACKED.size == 8 * (9 + 4 + 12 + 1 + 12 + 1)
+    assert attention._APPEND.size + attention._APPEND_AT.size == 8 * 21
+    assert attention._PAGED.size + attention._PAGED_AT.size == 8 * 16
+    assert attention._PACKED.size + attention._PACKED_AT.size == 8 * (13 + 16 + 10)
     assert _abi.lib().fsp_attention_dim_cap() == attention._DIM_CAP
 
 
@@ -83,9 +83,11 @@ def _packed(**kw):
     a |= {"lse": 16, "work": 16} | kw
     order = ["dtype", "heads", "kv_heads", "dim", "q_tokens", "k_tokens", "causal", "window", "scale",
              "q_tiles", "n_q_tiles", "k_tiles", "n_k_tiles"]
-    order += [n + e for n in ("q", "k", "v", "out") for e in ("", "_token", "_head")] + ["lse"]
-    order += [n + e for n in ("go", "gq", "gk", "gv") for e in ("", "_token", "_head")] + ["work"]
-    return attention._PACKED.pack(*(a[n] for n in order))
+    eight = ("q", "k", "v", "out", "go", "gq", "gk", "gv")
+    order += [n + e for n in eight for e in ("_token", "_head")]
+    at = [*eight[:4], "lse", *eight[4:], "work"]
+    return attention._PACKED.pack(*(a[n] for n in order)) + \
+        attention._PACKED_AT.pack(*(a[n] for n in at))
 
 
 @pytest.mark.parametrize("status,kw", [
@@ -115,11 +117,21 @@ def _cache(**kw):
     return attention._CACHE.pack(*a.values())
 
 
-_PAGED_ARGS = dict(heads=4, window=0, scale=0.125, q=64, qt=256, qh=64, out=64, ot=256, oh=64, lse=0,
-                   lengths=16, work=16, pieces=16, slots=16, n_pieces=3, piece=128)
-_APPEND_ARGS = dict(n_tokens=2, heads=4, half=32, rows=64, interleaved=0, k=64, kt=128, kh=64, v=64,
-                    vt=128, vh=64, q=64, qt=256, qh=64, qo=64, qot=256, qoh=64, cos=16, sin=16,
-                    tokens=0, lengths=16)
+_PAGED_ARGS = dict(pieces=16, slots=16, n_pieces=3, piece=128, heads=4, window=0, scale=0.125, qt=256,
+                   qh=64, ot=256, oh=64, q=64, out=64, lse=0, lengths=16, work=16)
+_APPEND_ARGS = dict(n_tokens=2, heads=4, half=32, rows=64, interleaved=0, kt=128, kh=64, vt=128, vh=64,
+                    qt=256, qh=64, qot=256, qoh=64, k=64, v=64, q=64, qo=64, cos=16, sin=16, tokens=0,
+                    lengths=16)
+
+
+def _paged(**kw):
+    a = list((_PAGED_ARGS | kw).values())
+    return attention._PAGED.pack(*a[:11]) + attention._PAGED_AT.pack(*a[11:])
+
+
+def _append(**kw):
+    a = list((_APPEND_ARGS | kw).values())
+    return attention._APPEND.pack(*a[:13]) + attention._APPEND_AT.pack(*a[13:])
 
 
 @pytest.mark.parametrize("status,kw", [
@@ -129,8 +141,8 @@ _APPEND_ARGS = dict(n_tokens=2, heads=4, half=32, rows=64, interleaved=0, k=64, 
 def test_cache_refusals_of_the_library(status, kw):
     L = _abi.lib()
     c = _cache(**kw)
-    assert L.fsp_attention_paged(c + attention._PAGED.pack(*_PAGED_ARGS.values()), None) == status
-    assert L.fsp_paged_append(c + attention._APPEND.pack(*_APPEND_ARGS.values()), None) == status
+    assert L.fsp_attention_paged(c + _paged(), None) == status
+    assert L.fsp_paged_append(c + _append(), None) == status
     assert L.fsp_attention_paged(None, None) == -1 and L.fsp_paged_append(None, None) == -1
 
 
@@ -140,7 +152,7 @@ def test_cache_refusals_of_the_library(status, kw):
                                 {"piece": 0}, {"piece": 2048}, {"piece": 130}])
 def test_paged_refusals_of_the_library(kw):
     L = _abi.lib()
-    args = _cache() + attention._PAGED.pack(*(_PAGED_ARGS | kw).values())
+    args = _cache() + _paged(**kw)
     assert L.fsp_attention_paged(args, None) == -1
 
 
@@ -149,7 +161,7 @@ def test_paged_refusals_of_the_library(kw):
                                 {"rows": 1 << 32}])
 def test_append_refusals_of_the_library(kw):
     L = _abi.lib()
-    args = _cache() + attention._APPEND.pack(*(_APPEND_ARGS | kw).values())
+    args = _cache() + _append(**kw)
     assert L.fsp_paged_append(args, None) == -1
 
 
