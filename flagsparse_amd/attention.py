@@ -593,6 +593,10 @@ def _pack(prepared, q, k, v, causal, window, scale, out, grads=()):
                         k_tiles.data_ptr(), k_tiles.shape[0] if grads else 0, *steps)
 
 
+def _tracked(t):
+    return isinstance(t, torch.Tensor) and t.requires_grad
+
+
 def _run_forward(prepared, head, q, k, v, res):
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
     if q.shape[0]:
@@ -647,8 +651,7 @@ def flagsparse_attention_packed(q, k, v, indptr=None, k_indptr=None, *, prepared
     [tokens, heads] if ``return_lse``.  The output is differentiable with respect to q, k and v where
     they require a gradient (the log-sum-exp is not)."""
     key = None
-    wanted = torch.is_grad_enabled() and any(
-        isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k, v))
+    wanted = torch.is_grad_enabled() and (_tracked(q) or _tracked(k) or _tracked(v))
     if out is None and not wanted and type(prepared) is PreparedAttention and \
             type(scale) in _PLAIN and type(window) in _PLAIN and type(causal) in _PLAIN:
         key = _layouts(q, k, v) + (causal, window, scale)

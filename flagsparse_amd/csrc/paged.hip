@@ -13,71 +13,129 @@ struct Cache {
   int batch, page_size, dim, kv_heads;
 };
 
-// One workgroup a token.
-template <typename T>
+// How the first 2 * half elements of a head turn: not at all; by pairs half apart or of neighbours, eight
+// elements of a vector against eight others or among themselves; or element by element, where
+// half is no whole number of vectors.
+enum { kStill, kHalves, kNeighbours, kEach };
+
+// Eight elements from d on of a head that turns by row ``turn`` of the table.
+template <typename T, int MODE>
+__device__ __forceinline__ V8<T> turned(const T* row, int d, const float* cos, const float* sin,
+                                        int half, int interleaved) {
+  const V8<T> x = *reinterpret_cast<const V8<T>*>(row + d);
+  if (MODE == kStill || d >= 2 * half) return x;
+  f32x8 y = __builtin_convertvector(x, f32x8);
+  if constexpr (MODE == kHalves) {
+    const bool low = d < half;
+    const int j = low ? d : d - half;
+    const f32x8 z = __builtin_convertvector(
+        *reinterpret_cast<const V8<T>*>(row + (low ? d + half : j)), f32x8);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const f32x4 c = *reinterpret_cast<const f32x4*>(cos + j + 4 * u);
+      const f32x4 s = *reinterpret_cast<const f32x4*>(sin + j + 4 * u);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        y[4 * u + e] = y[4 * u + e] * c[e] + (low ? -z[4 * u + e] : z[4 * u + e]) * s[e];
+    }
+  } else if constexpr (MODE == kNeighbours) {
+    const f32x4 c = *reinterpret_cast<const f32x4*>(cos + d / 2);
+    const f32x4 s = *reinterpret_cast<const f32x4*>(sin + d / 2);
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float u = y[e], v = y[e + 1];
+      y[e] = u * c[e / 2] - v * s[e / 2];
+      y[e + 1] = u * s[e / 2] + v * c[e / 2];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int at = d + e;
+      if (at < 2 * half) {
+        const bool low = interleaved ? !(at & 1) : at < half;
+        const int j = interleaved ? at >> 1 : low ? at : at - half;
+        const float z = (float)row[interleaved ? at ^ 1 : low ? at + half : j];
+        y[e] = y[e] * cos[j] + (low ? -z : z) * sin[j];
+      }
+    }
+  }
+  return __builtin_convertvector(y, V8<T>);
+}
+
+struct AppendShape {
+  int64_t n_tokens, k_token, k_head, v_token, v_head, q_token, q_head, qo_token, qo_head;
+  int heads, half, table_rows, interleaved, parts;
+};
+
+// A wave to a token, or to one of ``parts`` interleaved parts of its vectors of eight elements, where
+// there are few tokens.  Bound by memory for prompts (a read and a write of every element) and by
+// the chain token -> sequence -> page -> row for single tokens.
+template <typename T, int MODE>
 __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(
-    Cache c, T* __restrict__ k_pages, T* __restrict__ v_pages, const T* __restrict__ k,
-    int64_t k_token, int64_t k_head, const T* __restrict__ v, int64_t v_token, int64_t v_head,
-    const T* __restrict__ q, int64_t q_token, int64_t q_head, T* __restrict__ q_out,
-    int64_t qo_token, int64_t qo_head, const float* __restrict__ cos,
-    const float* __restrict__ sin, const int32_t* __restrict__ tokens,
-    const int32_t* __restrict__ lengths, int heads, int half, int table_rows, int interleaved) {
-  const int64_t t = blockIdx.x;
+    Cache c, AppendShape s, T* __restrict__ k_pages, T* __restrict__ v_pages,
+    const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ q,
+    T* __restrict__ q_out, const float* __restrict__ cos, const float* __restrict__ sin,
+    const int32_t* __restrict__ tokens, const int32_t* __restrict__ lengths) {
+  const int lane = threadIdx.x & 63;
+  const int64_t unit = (int64_t)blockIdx.x * (kAppendThreads / kWave) +
+                       __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t t = unit / s.parts;
+  if (t >= s.n_tokens) return;
   int b = (int)t;
   int64_t pos;
   bool mine = true;
-  if (tokens) {
-    int lo = 0, hi = c.batch;  // the last sequence that starts at or before t
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (tokens[mid] <= t) lo = mid; else hi = mid;
+  if (tokens) {  // the last sequence that starts at or before t, 64 at a look
+    b = -1;
+    for (int at = 0; at < c.batch; at += kWave) {
+      const int n = __popcll(__ballot(at + lane < c.batch && tokens[min(at + lane, c.batch)] <= t));
+      b += n;
+      if (n < kWave) break;
     }
-    b = lo;
-    mine = tokens[b] <= t && t < tokens[b + 1];
-    pos = (int64_t)lengths[b] - tokens[b + 1] + t;
+    b = __builtin_amdgcn_readfirstlane(max(b, 0));
+    const int begin = tokens[b], end = tokens[b + 1];
+    mine = begin <= t && t < end;
+    pos = (int64_t)lengths[b] - end + t;
   } else {
     pos = (int64_t)lengths[b] - 1;
   }
   const int first = c.indptr[b], last = c.indptr[b + 1];
   const bool ok = mine && pos >= 0 && pos < (int64_t)(last - first) * c.page_size &&
-                  (half == 0 || pos < table_rows);
-  const float nan = __builtin_nanf("");
+                  (MODE == kStill || pos < s.table_rows);
   int64_t page = 0, slot = 0;
   if (ok) {
-    page = c.indices[first + pos / c.page_size];
-    slot = pos % c.page_size;
+    const uint32_t at = (uint32_t)pos / (uint32_t)c.page_size;
+    page = c.indices[first + at];
+    slot = (uint32_t)pos - at * c.page_size;
+    cos += pos * s.half;
+    sin += pos * s.half;
   }
-  const int per = c.dim;
-  for (int i = threadIdx.x; i < (heads + 2 * c.kv_heads) * per; i += kAppendThreads) {
+  const T nan = (T)__builtin_nanf("");
+  const uint32_t per = c.dim / 8, rows = s.heads + 2 * c.kv_heads;
+  const T* kr = k + t * s.k_token;
+  const T* vr = v + t * s.v_token;
+  const T* qr = q + t * s.q_token;
+  T* kt = k_pages + page * c.k_page + slot * c.k_slot;
+  T* vt = v_pages + page * c.v_page + slot * c.v_slot;
+  T* qt = q_out + t * s.qo_token;
+#pragma unroll 2
+  for (uint32_t i = (uint32_t)(unit % s.parts) * kWave + lane; i < rows * per; i += s.parts * kWave) {
     int h = i / per;
-    const int d = i % per;
-    const T* row;
-    T* to;
-    bool turn = true;
-    if (h < c.kv_heads) {
-      row = k + t * k_token + h * k_head;
-      to = k_pages + page * c.k_page + slot * c.k_slot + h * c.k_head;
-    } else if (h < 2 * c.kv_heads) {
-      h -= c.kv_heads;
-      row = v + t * v_token + h * v_head;
-      to = v_pages + page * c.v_page + slot * c.v_slot + h * c.v_head;
-      turn = false;
-    } else {
-      h -= 2 * c.kv_heads;
-      row = q + t * q_token + h * q_head;
-      to = q_out + t * qo_token + h * qo_head;
-      if (!ok) to[d] = (T)nan;
+    const int d = 8 * (i - h * per);
+    if (h < s.heads) {
+      V8<T> x{nan, nan, nan, nan, nan, nan, nan, nan};
+      if (ok) x = turned<T, MODE>(qr + h * s.q_head, d, cos, sin, s.half, s.interleaved);
+      *reinterpret_cast<V8<T>*>(qt + h * s.qo_head + d) = x;
+    } else if (ok) {
+      h -= s.heads;
+      if (h < c.kv_heads) {
+        *reinterpret_cast<V8<T>*>(kt + h * c.k_head + d) =
+            turned<T, MODE>(kr + h * s.k_head, d, cos, sin, s.half, s.interleaved);
+      } else {
+        h -= c.kv_heads;
+        *reinterpret_cast<V8<T>*>(vt + h * c.v_head + d) =
+            *reinterpret_cast<const V8<T>*>(vr + h * s.v_head + d);
+      }
     }
-    if (!ok) continue;
-    float x = (float)row[d];
-    if (turn && d < 2 * half) {
-      const bool low = interleaved ? !(d & 1) : d < half;
-      const int j = interleaved ? d >> 1 : (low ? d : d - half);
-      const int mate = interleaved ? (d ^ 1) : (low ? d + half : d - half);
-      const float y = (float)row[mate], cs = cos[pos * half + j], sn = sin[pos * half + j];
-      x = low ? x * cs - y * sn : y * sn + x * cs;
-    }
-    to[d] = (T)x;
   }
 }
 
@@ -360,16 +418,32 @@ Cache cache_of(const fsp_paged_cache& c) {
           c.v_head, (int)c.batch, (int)c.page_size, (int)c.dim, (int)c.kv_heads};
 }
 
-template <typename T>
+template <typename T, int MODE>
 int launch_append(const fsp_paged_append_args& a, hipStream_t st) {
-  hipLaunchKernelGGL((paged_append_kernel<T>), dim3((unsigned)a.n_tokens), dim3(kAppendThreads), 0,
-                     st, cache_of(a.cache), static_cast<T*>(a.cache.k_pages),
-                     static_cast<T*>(a.cache.v_pages), static_cast<const T*>(a.k), a.k_token,
-                     a.k_head, static_cast<const T*>(a.v), a.v_token, a.v_head,
-                     static_cast<const T*>(a.q), a.q_token, a.q_head, static_cast<T*>(a.q_out),
-                     a.q_out_token, a.q_out_head, a.cos, a.sin, a.token_indptr, a.lengths,
-                     (int)a.heads, (int)a.half, (int)a.table_rows, (int)a.interleaved);
+  const int64_t steps = ((a.heads + 2 * a.cache.kv_heads) * (a.cache.dim / 8) + kWave - 1) / kWave;
+  int64_t parts = (4096 + a.n_tokens - 1) / a.n_tokens;  // waves enough for every SIMD
+  if (parts > steps) parts = steps;
+  const AppendShape s{a.n_tokens, a.k_token, a.k_head,    a.v_token,         a.v_head,           a.q_token,
+                      a.q_head,   a.q_out_token, a.q_out_head, (int)a.heads, (int)a.half, (int)a.table_rows,
+                      (int)a.interleaved, (int)parts};
+  constexpr int kWaves = kAppendThreads / kWave;
+  hipLaunchKernelGGL((paged_append_kernel<T, MODE>),
+                     dim3((unsigned)((a.n_tokens * parts + kWaves - 1) / kWaves)),
+                     dim3(kAppendThreads), 0, st, cache_of(a.cache), s,
+                     static_cast<T*>(a.cache.k_pages), static_cast<T*>(a.cache.v_pages),
+                     static_cast<const T*>(a.k), static_cast<const T*>(a.v),
+                     static_cast<const T*>(a.q), static_cast<T*>(a.q_out), a.cos, a.sin,
+                     a.token_indptr, a.lengths);
   return check_hip(hipGetLastError(), "paged_append_kernel launch");
+}
+
+template <typename T>
+int launch_append_mode(const fsp_paged_append_args& a, hipStream_t st) {
+  const bool aligned = (reinterpret_cast<uintptr_t>(a.cos) | reinterpret_cast<uintptr_t>(a.sin)) % 16 == 0;
+  if (a.half == 0) return launch_append<T, kStill>(a, st);
+  if (aligned && !a.interleaved && a.half % 8 == 0) return launch_append<T, kHalves>(a, st);
+  if (aligned && a.interleaved && a.half % 4 == 0) return launch_append<T, kNeighbours>(a, st);
+  return launch_append<T, kEach>(a, st);
 }
 
 int64_t paged_workgroups(const fsp_attention_paged_args& a) {
@@ -428,7 +502,7 @@ extern "C" int fsp_paged_append(const fsp_paged_append_args* args, void* stream)
       !aligned16(a.q, a.q_token, a.q_head) || !aligned16(a.q_out, a.q_out_token, a.q_out_head))
     return set_error(FSP_EINVAL, "fsp_paged_append: rows must be 16-byte aligned");
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return a.cache.dtype == FSP_BF16 ? launch_append<bf16>(a, st) : launch_append<f16>(a, st);
+  return a.cache.dtype == FSP_BF16 ? launch_append_mode<bf16>(a, st) : launch_append_mode<f16>(a, st);
 }
 
 extern "C" int64_t fsp_attention_paged_piece(int64_t tokens, int64_t kv_heads) {
