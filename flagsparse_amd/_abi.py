@@ -120,6 +120,7 @@ SIGNATURES = {
     "fsp_run": (_i32, [_p, _p, _p, _p]),
     "fsp_attention_dim_cap": (_i64, []),
     "fsp_paged_append": (_i32, [_p, _p]),
+    "fsp_attention_paged_counts": (_i64, [_i64, _i64, _i64, _i64, _i64]),
     "fsp_attention_paged_piece": (_i64, [_i64, _i64]),
     "fsp_attention_paged_workspace": (_i64, [_i64, _i64, _i64]),
     "fsp_attention_paged": (_i32, [_p, _p]),

@@ -38,7 +38,7 @@ _STEP_CAP = 2**23
 # shapes, steps and types settle comes first, then the addresses of its arrays.
 _CACHE = struct.Struct("17q")
 _APPEND, _APPEND_AT = struct.Struct("13q"), struct.Struct("8q")
-_PAGED, _PAGED_AT = struct.Struct("6qd4q"), struct.Struct("5q")
+_PAGED, _PAGED_AT = struct.Struct("6qd4q"), struct.Struct("6q")
 _PACKED, _PACKED_AT = struct.Struct("8qd20q"), struct.Struct("10q")
 
 # A prepared object keeps the first part for each layout of arrays that it has checked, so that the
@@ -184,7 +184,8 @@ class PreparedPagedKV:
     most tokens that the pages of one sequence hold."""
 
     __slots__ = ("k_pages", "v_pages", "dtype", "device", "indptr", "indices", "batch", "n_pages", "page_size",
-                 "kv_heads", "dim", "room", "_piece", "_pieces", "_slots", "_streams", "_calls")
+                 "kv_heads", "dim", "room", "_piece", "_pieces", "_first", "_most", "_streams",
+                 "_calls", "_counts", "_parts")
 
     def __init__(self, k_pages, v_pages, indptr, indices, pages):
         self.k_pages = k_pages
@@ -199,9 +200,11 @@ class PreparedPagedKV:
         self.room = int(rooms.max()) if len(rooms) else 0
         # the pieces that attention is cut into
         self._piece = int(_abi.lib().fsp_attention_paged_piece(int(rooms.sum()), self.kv_heads))
-        table, slots = _pieces(rooms, self._piece)
-        both = torch.from_numpy(np.concatenate([table.ravel(), slots])).to(k_pages.device)
-        self._pieces, self._slots = both[:table.size].view(-1, 4), both[table.size:]
+        table, first, self._most = _pieces(pages, self.page_size, self._piece)
+        both = torch.from_numpy(np.concatenate([table.ravel(), first])).to(k_pages.device)
+        self._pieces, self._first = both[:table.size].view(-1, 8), both[table.size:]
+        self._parts = {}  # counts of arrivals that a call needs, by its heads
+        self._counts = _abi.Calls()  # those counts, by stream and heads
         self._streams = _Streams()
         self._calls = _abi.Calls()
 
@@ -221,15 +224,18 @@ class PreparedPagedKV:
         return stream
 
 
-def _pieces(rooms, piece):
-    """(the pieces of ``piece`` tokens that sequences with these rooms may come to hold, each sequence's
-    first), as the kernels read them."""
+def _pieces(pages, page_size, piece):
+    """(the pieces of ``piece`` tokens that sequences with so many pages may come to hold, the sequences'
+    first ones, the most that one has), as the kernels read them."""
+    rooms = pages * page_size
     n = np.maximum(1, -(-rooms // piece))
     slots = np.cumsum(n) - n
     seq = np.repeat(np.arange(len(rooms)), n)
     at = np.arange(len(seq)) - slots[seq]
-    table = np.stack([seq, at * piece, slots[seq], np.zeros_like(seq)], axis=1)
-    return table.astype(np.int32), slots.astype(np.int32)
+    none = np.zeros_like(seq)
+    table = np.stack([seq, at * piece, slots[seq], (np.cumsum(pages) - pages)[seq], rooms[seq],
+                      none, none, none], axis=1)
+    return table.astype(np.int32), slots.astype(np.int32), int(n.max(initial=1))
 
 
 def _check_pages(t, name):
@@ -441,7 +447,7 @@ def flagsparse_attention_paged(q, lengths, *, prepared=None, k_pages=None, v_pag
     res, copied = _result(out, "out", q.shape, dt, dev)
     rows = _rows(q)
     head = kv._packed() + _PAGED.pack(
-        kv._pieces.data_ptr(), kv._slots.data_ptr(), kv._pieces.shape[0], kv._piece, heads, past,
+        kv._pieces.data_ptr(), kv._first.data_ptr(), kv._pieces.shape[0], kv._piece, heads, past,
         factor, *rows.stride()[:2], *res.stride()[:2])
     lse = _attend(kv, head, rows, res, n, return_lse)
     if key is not None and rows is q and n is lengths:
@@ -454,16 +460,26 @@ def flagsparse_attention_paged(q, lengths, *, prepared=None, k_pages=None, v_pag
 
 def _attend(kv, head, q, res, lengths, return_lse):
     """The launch; returns the log-sum-exp, if asked for."""
-    heads, dev, L = q.shape[1], q.device, _abi.lib()
+    heads, dev = q.shape[1], q.device
     lse = torch.empty((kv.batch, heads), dtype=torch.float32, device=dev) if return_lse else None
-    pieces, work = kv._pieces.shape[0], None
+    if not kv.batch:
+        return lse
+    stream, pieces, work, counts = kv._on(), kv._pieces.shape[0], None, None
     if pieces > kv.batch:
         work = torch.empty(pieces * heads * (kv.dim + 2), dtype=torch.float32, device=dev)
-    if kv.batch:
-        status = L.fsp_attention_paged(head + _PAGED_AT.pack(
-            q.data_ptr(), res.data_ptr(), _at(lse), lengths.data_ptr(), _at(work)), kv._on())
-        if status:
-            _abi.check(status, "fsp_attention_paged")
+        need = kv._parts.get(heads)
+        if need is None:
+            need = kv._parts[heads] = int(_abi.lib().fsp_attention_paged_counts(
+                pieces, kv._most, kv.batch, heads, kv.kv_heads))
+        counts = kv._counts.get((stream, heads))
+        if need and counts is None:
+            counts = torch.zeros(need, dtype=torch.int32, device=dev)
+            if not torch.cuda.is_current_stream_capturing():  # else they are the graph's
+                kv._counts[stream, heads] = counts
+    status = _abi.lib().fsp_attention_paged(head + _PAGED_AT.pack(
+        q.data_ptr(), res.data_ptr(), _at(lse), lengths.data_ptr(), _at(work), _at(counts)), stream)
+    if status:
+        _abi.check(status, "fsp_attention_paged")
     return lse
 
 

@@ -169,7 +169,7 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(
     for (int i = 0; i < NS; ++i) {
       const int d = 16 * i + 8 * half;
       const V8<T> x = *reinterpret_cast<const V8<T>*>(qr + (d < s.dim ? d : 0));
-      qf[i] = d < s.dim ? scaled_sign<T>(x, s.scale) : V8<T>{};
+      qf[i] = scaled_sign<T>(x, s.scale, d < s.dim);
     }
   }
   const float c = exp2_scale(s.scale);
@@ -316,10 +316,10 @@ __global__ __launch_bounds__(256, 2) void attention_grad_q_kernel(
     const V8<T> x = *reinterpret_cast<const V8<T>*>(q + row * q_token + a * q_head + at);
     const V8<T> y = *reinterpret_cast<const V8<T>*>(go + row * go_token + a * go_head + at);
     const V8<T> z = *reinterpret_cast<const V8<T>*>(out + row * o_token + a * o_head + at);
-    qf[i] = d < s.dim ? scaled_sign<T>(x, s.scale) : V8<T>{};
-    gf[i] = d < s.dim ? y : V8<T>{};
+    qf[i] = scaled_sign<T>(x, s.scale, d < s.dim);
+    gf[i] = keep_if<T>(y, d < s.dim);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) delta += d < s.dim ? (float)y[e] * (float)z[e] : 0.0f;
+    for (int e = 0; e < 8; ++e) delta += (float)gf[i][e] * (float)keep_if<T>(z, d < s.dim)[e];
   }
   delta += other_half(delta);
   const float c = exp2_scale(s.scale);
@@ -437,8 +437,8 @@ __global__ __launch_bounds__(256, 2) void attention_grad_kv_kernel(
     const int d = 16 * i + 8 * half, at = d < s.dim ? d : 0;
     const V8<T> x = *reinterpret_cast<const V8<T>*>(k + row * k_token + g * k_head + at);
     const V8<T> y = *reinterpret_cast<const V8<T>*>(v + row * v_token + g * v_head + at);
-    kf[i] = d < s.dim ? scaled_sign<T>(x, s.scale) : V8<T>{};
-    vf[i] = d < s.dim ? y : V8<T>{};
+    kf[i] = scaled_sign<T>(x, s.scale, d < s.dim);
+    vf[i] = keep_if<T>(y, d < s.dim);
   }
   const float c = exp2_scale(s.scale);
 

@@ -75,10 +75,19 @@ __device__ __forceinline__ float other_half(float v) {
 // show in 32 bits, makes it zero.
 constexpr float kNoScale = 1e-30f;
 
+// Eight elements, or zeros.  A mask, not a choice: a choice becomes a branch around the load, and loads
+// in branches wait for each other.
 template <typename T>
-__device__ __forceinline__ V8<T> scaled_sign(V8<T> q, float scale) {
-  if (scale > kNoScale) return q;
-  return scale < -kNoScale ? -q : V8<T>{};
+__device__ __forceinline__ V8<T> keep_if(V8<T> x, bool in) {
+  const int m = in ? -1 : 0;
+  return __builtin_bit_cast(V8<T>, __builtin_bit_cast(i32x4, x) & i32x4{m, m, m, m});
+}
+
+template <typename T>
+__device__ __forceinline__ V8<T> scaled_sign(V8<T> q, float scale, bool in) {
+  const int m = scale < 0 ? (int)0x80008000 : 0;
+  const i32x4 x = __builtin_bit_cast(i32x4, keep_if<T>(q, in && fabsf(scale) > kNoScale));
+  return __builtin_bit_cast(V8<T>, x ^ i32x4{m, m, m, m});
 }
 
 __device__ __forceinline__ float exp2_scale(float scale) {

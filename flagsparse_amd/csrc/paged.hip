@@ -139,11 +139,32 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(
   }
 }
 
+// Results that another workgroup, perhaps of another XCD, picks up: stored past this XCD's L2 and read
+// past the reader's, so that a wait for the stores (all_stored) is all that has to come between
+// them and the word that they are there.  A release and an acquire of everything write back and drop
+// an L2 each time instead: 96 sequences of up to 4096 tokens took 59 us with them, 41 us so.
+__device__ __forceinline__ void put(float* to, float a, float b) {
+  const uint64_t v = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(to), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__device__ __forceinline__ f32x2 get(const float* from) {
+  const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(from), __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_AGENT);
+  return f32x2{__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))};
+}
+
+__device__ __forceinline__ void all_stored() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
 // Attention of one query per sequence.  A workgroup takes a piece of a sequence's tokens for one key
 // head and up to 16 of the query heads that share it; its four waves take every fourth 32 keys.
 //
-// Keys and values go from memory to the matrix instructions' registers with no stop in LDS.  With
-// S^T = K Q^T lane l has head l % 16 and, of 32 keys, the eight 4 * (l / 16) + {0..3, 16..19}: its
+// Values go from memory to the matrix instructions' registers with no stop in LDS, keys with a short
+// one: with a lane to a key a load would fetch 64 bytes of each of 16 rows, and whole rows are the
+// faster to fetch (a bare loop of such loads over 3.2 GB: 64 bytes 540 us, rows 490), so that a wave
+// writes the rows to LDS of its own and reads its lanes' keys there.  With S^T = K Q^T lane l has head l % 16 and, of 32 keys, the eight 4 * (l / 16) + {0..3, 16..19}: its
 // weights are the operand of O^T = V^T P^T as they lie, since the order of the summed keys is free.
 // For V a lane loads DP / 16 consecutive elements of those same eight keys, and the operand of one
 // product is one element of each: pairs of 16-bit halves, a byte permutation each.  Row m of product
@@ -152,49 +173,68 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(
 // Where each key lies (its page, its place in it) is found once for the piece and kept in LDS.
 constexpr int kHeadTile = 16;
 constexpr int kPieceMost = 1024;
+// The workgroup that finishes a sequence joins its pieces where they are at most so many and all
+// workgroups are on the chip at once (three to a CU): the wait for their stores then holds up nobody.
+// Else a second launch does.  1000 tokens, 16 heads of 64: 10.7 us a call joined so, 13.2 by a second
+// launch, both bound by the host (9.2 and 8.5 us in a graph); 6 sequences of 131072 tokens, pieces
+// of 1024: 645 and 583 us.
+constexpr int kJoinMost = 8;
+constexpr int kResident = 3 * 256;
 
+// Tokens [begin, begin + piece) of seq, of the room that its pages give; slot: of the sequence's first
+// piece; page: its first place in the page table.
 struct Piece {
-  int seq, begin, slot, pad;  // tokens [begin, begin + piece) of seq; slot: of the sequence's first piece
+  int seq, begin, slot, page, room, pad[3];
 };
 
+// Workgroups go to the 8 XCDs in turn: a piece's heads, which lie side by side in memory, go to one.
+// With a head to an XCD each L2 would see every eighth 256 bytes, a few of its channels.
+__device__ __forceinline__ void piece_and_head(int block, int n_pieces, int heads, int& piece, int& head) {
+  const int set = block / (8 * heads), in = block - set * 8 * heads;
+  const int width = min(8, n_pieces - 8 * set);  // pieces of this set
+  piece = 8 * set + in % width;
+  head = in / width;
+}
+
 struct PagedShape {
-  int heads, window, piece;
+  int heads, window, piece, n_pieces;
   float scale;
 };
 
-// Tokens [first, last) are seen by the query; ok: the pages hold them.
-__device__ __forceinline__ bool paged_range(const Cache& c, int b, int n, int window, int& first,
-                                            int& last) {
-  const bool ok = n >= 0 && n <= (int64_t)(c.indptr[b + 1] - c.indptr[b]) * c.page_size;
-  last = ok ? n : 0;
-  first = window && last > window ? last - window : 0;
-  return ok;
-}
-
-template <typename T, int DP>
-__global__ __launch_bounds__(256) void attention_paged_kernel(
+//
+// The next step's keys are asked for once this step's scores are made, its values once this step's
+// output is; without conditions (the last step asks for its own again), so that the wait for the
+// values does not wait for the keys asked for after them.  EXACT: the head has DP elements.
+// NT: loads that do not claim a place in the caches.
+template <typename T, int DP, bool EXACT, bool NT>
+__global__ __launch_bounds__(256, 3) void attention_paged_kernel(
     Cache c, PagedShape s, const Piece* __restrict__ pieces, const T* __restrict__ k_pages,
     const T* __restrict__ v_pages, const T* __restrict__ q, int64_t q_token, int64_t q_head,
     T* __restrict__ out, int64_t out_token, int64_t out_head, float* __restrict__ lse,
-    const int32_t* __restrict__ lengths, float* __restrict__ part_o, f32x2* __restrict__ part_ml) {
+    const int32_t* __restrict__ lengths, float* part_o, float* part_ml, unsigned* arrived) {
   constexpr int E = DP / 16, NS = DP / 32, W = 4;  // elements of V and steps of K a lane; waves
   typedef T VE __attribute__((ext_vector_type(E)));
-  __shared__ int64_t s_k[kPieceMost], s_v[kPieceMost];
+  constexpr int CH = DP / 8, KL = DP / 16;  // chunks of 16 bytes in a row; loads of 32 rows of K
+  __shared__ int64_t s_k[kPieceMost], s_v[kPieceMost];  // where the keys and values lie
+  // each wave's keys; then, its sums
+  typedef float Sums[kHeadTile][DP + 4];
+  static_assert(sizeof(Sums) >= 64 * DP, "");
+  __shared__ __attribute__((aligned(16))) char s_raw[W * sizeof(Sums)];
   __shared__ f32x2 s_ml[W][kHeadTile];
-  __shared__ __attribute__((aligned(16))) float s_o[W][kHeadTile][DP + 4];
-
+  Sums* s_o = reinterpret_cast<Sums*>(s_raw);
   const int group = s.heads / c.kv_heads, tiles = (group + kHeadTile - 1) / kHeadTile;
-  int id = blockIdx.x;
-  const int g = id % c.kv_heads;
-  id /= c.kv_heads;
-  const int ht = id % tiles;
-  const Piece pc = pieces[id / tiles];
+  int piece, g, ht;
+  piece_and_head(blockIdx.x, s.n_pieces, c.kv_heads * tiles, piece, ht);
+  g = ht / tiles;
+  ht -= g * tiles;
+  const Piece pc = pieces[piece];
   const int b = pc.seq, lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int first, last;
-  const bool ok = paged_range(c, b, lengths[b], s.window, first, last);
   const int n_heads = min(kHeadTile, group - ht * kHeadTile), head0 = g * group + ht * kHeadTile;
-  // the sequence's pieces in use, and whether this one is
+  const int length = lengths[b];
+  const bool ok = length >= 0 && length <= pc.room;
+  // the query sees tokens [first, last); the sequence's pieces in use, and whether this is one
+  const int last = ok ? length : 0, first = s.window && last > s.window ? last - s.window : 0;
   const int p0 = first / s.piece, p1 = max(p0 + 1, (last + s.piece - 1) / s.piece);
   const int mine = pc.begin / s.piece;
   if (mine < p0 || mine >= p1) return;
@@ -207,18 +247,17 @@ __global__ __launch_bounds__(256) void attention_paged_kernel(
     for (int i = 0; i < NS; ++i) {
       const int d = 32 * i + 8 * quad;
       const V8<T> x = *reinterpret_cast<const V8<T>*>(qr + (d < c.dim ? d : 0));
-      qf[i] = d < c.dim ? scaled_sign<T>(x, s.scale) : V8<T>{};
+      qf[i] = scaled_sign<T>(x, s.scale, d < c.dim);
     }
   }
   const float cs = exp2_scale(s.scale);
 
   // where the keys lie; those past the end stand for the first one, and weigh nothing
   const int padded = (n + 127) & ~127;
-  const int pages = c.indptr[b];
   for (int i = threadIdx.x; i < padded; i += 256) {
     const uint32_t j = begin + (i < n ? i : 0);
     const uint32_t at = j / (uint32_t)c.page_size;
-    const int64_t page = n > 0 ? c.indices[pages + at] : 0, slot = j - at * c.page_size;
+    const int64_t page = n > 0 ? c.indices[pc.page + at] : 0, slot = j - at * c.page_size;
     s_k[i] = page * c.k_page + slot * c.k_slot;
     s_v[i] = page * c.v_page + slot * c.v_slot;
   }
@@ -226,30 +265,23 @@ __global__ __launch_bounds__(256) void attention_paged_kernel(
 
   const T* kb = k_pages + g * c.k_head;
   const T* vb = v_pages + g * c.v_head;
-  V8<T> kf[2][NS];
+  i32x4 kr[KL];
   VE vf[8];
+  // load i: rows 64 / CH * i + lane / CH, chunk lane % CH of each; it lies in LDS at chunk ^ row
+  const int k_row = lane / CH, k_chunk = lane % CH;
   auto load_k = [&](int j) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const T* row = kb + s_k[j + 16 * u + col];
-#pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        const int d = 32 * i + 8 * quad;
-        kf[u][i] = *reinterpret_cast<const V8<T>*>(row + (d < c.dim ? d : 0));
-      }
-    }
-    if (c.dim < DP) {  // past the head: zeros, as in q, or an infinity there would show
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int i = 0; i < NS; ++i) kf[u][i] = 32 * i + 8 * quad < c.dim ? kf[u][i] : V8<T>{};
-    }
+    for (int i = 0; i < KL; ++i)
+      kr[i] = ld_stream<NT>(reinterpret_cast<const i32x4*>(
+          kb + s_k[j + 64 / CH * i + k_row] + (EXACT || 8 * k_chunk < c.dim ? 8 * k_chunk : 0)));
   };
+  char* s_rows = s_raw + wave * sizeof(Sums);
   const int ve = E * col < c.dim ? E * col : 0;
   auto load_v = [&](int j) {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      vf[e] = *reinterpret_cast<const VE*>(vb + s_v[j + 16 * (e / 4) + 4 * quad + e % 4] + ve);
+      vf[e] = ld_stream<NT>(reinterpret_cast<const VE*>(
+          vb + s_v[j + 16 * (e / 4) + 4 * quad + e % 4] + ve));
   };
 
   float top = -INFINITY, sum = 0;
@@ -260,14 +292,27 @@ __global__ __launch_bounds__(256) void attention_paged_kernel(
   int j = 32 * wave;
   if (j < n) load_k(j), load_v(j);
   for (; j < n; j += 32 * W) {
+#pragma unroll
+    for (int i = 0; i < KL; ++i) {
+      const int row = 64 / CH * i + k_row;
+      // past the head: zeros, as in q, or an infinity there would show
+      *reinterpret_cast<i32x4*>(s_rows + row * 2 * DP + 16 * (k_chunk ^ (row & (CH - 1)))) =
+          EXACT ? kr[i] : kr[i] & (8 * k_chunk < c.dim ? -1 : 0);
+    }
     f32x4 x[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       x[u] = f32x4{};
 #pragma unroll
-      for (int i = 0; i < NS; ++i) x[u] = mfma16(kf[u][i], qf[i], x[u]);
+      for (int i = 0; i < NS; ++i) {
+        const int row = 16 * u + col;
+        x[u] = mfma16(*reinterpret_cast<const V8<T>*>(
+                          s_rows + row * 2 * DP + 16 * ((4 * i + quad) ^ (row & (CH - 1)))),
+                      qf[i], x[u]);
+      }
     }
-    if (j + 32 * W < n) load_k(j + 32 * W);
+    const int next = j + 32 * W < n ? j + 32 * W : j;
+    load_k(next);
     const bool partial = j + 32 > n;
     if (partial) {
 #pragma unroll
@@ -306,7 +351,7 @@ __global__ __launch_bounds__(256) void attention_paged_kernel(
       for (int e = 0; e < 8; ++e) a[e] = vf[e][i];
       o[i] = mfma16(a, pf, o[i]);
     }
-    if (j + 32 * W < n) load_v(j + 32 * W);
+    load_v(next);
   }
 
   // join the waves
@@ -337,9 +382,10 @@ __global__ __launch_bounds__(256) void attention_paged_kernel(
       y += f * *reinterpret_cast<const f32x4*>(&s_o[w][h][d]);
     }
     if (split) {
-      const int64_t at = ((int64_t)(pc.slot + mine)) * s.heads + head0 + h;
-      *reinterpret_cast<f32x4*>(part_o + at * c.dim + d) = y;
-      if (d == 0) part_ml[at] = f32x2{most, total};
+      const int64_t at = (int64_t)(pc.slot + mine) * s.heads + head0 + h;
+      put(part_o + at * c.dim + d, y.x, y.y);
+      put(part_o + at * c.dim + d + 2, y.z, y.w);
+      if (d == 0) put(part_ml + 2 * at, most, total);
     } else {
       const float f = total == 0 ? 0.0f : 1.0f / total;
 #pragma unroll
@@ -351,42 +397,103 @@ __global__ __launch_bounds__(256) void attention_paged_kernel(
             !ok ? nan : total == 0 ? -INFINITY : (most + log2f(total)) * kLn2;
     }
   }
+  if (!split || !arrived) return;  // without counts, another launch joins them
+
+  // The last workgroup of a sequence's pieces to arrive joins them, in their order, and leaves the
+  // count as it was before the call.
+  __shared__ unsigned s_before;
+  all_stored();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    unsigned* count = arrived + ((int64_t)b * c.kv_heads + g) * tiles + ht;
+    s_before = atomicAdd(count, 1u);
+    if (s_before == (unsigned)(p1 - p0 - 1)) atomicExch(count, 0u);
+  }
+  __syncthreads();
+  if (s_before != (unsigned)(p1 - p0 - 1)) return;
+  const int64_t at = (int64_t)(pc.slot + p0) * s.heads + head0;  // the first piece's first head
+  const int count = p1 - p0;
+  constexpr int PER = 256 / (DP / 4);  // heads side by side, each by DP / 4 threads
+  for (int h0 = 0; h0 < n_heads; h0 += PER) {
+    const int h = h0 + threadIdx.x / (DP / 4), d = threadIdx.x % (DP / 4) * 4;
+    if (h >= n_heads) break;
+    const float* ml = part_ml + 2 * (at + h);
+    const float* o4 = part_o + (at + h) * c.dim + (d < c.dim ? d : 0);
+    const int64_t ml_step = 2 * (int64_t)s.heads, o_step = (int64_t)s.heads * c.dim;
+    float most = -INFINITY, total = 0;
+    f32x4 y{};
+    for (int p = 0; p < count; p += kJoinMost) {  // their loads are under way together
+      f32x2 v[kJoinMost], u[kJoinMost], w[kJoinMost];
+#pragma unroll
+      for (int e = 0; e < kJoinMost; ++e) {
+        const int64_t i = min(p + e, count - 1);
+        v[e] = get(ml + i * ml_step);
+        u[e] = get(o4 + i * o_step);
+        w[e] = get(o4 + i * o_step + 2);
+      }
+#pragma unroll
+      for (int e = 0; e < kJoinMost; ++e) {
+        if (p + e >= count) break;
+        const float now = fmaxf(most, v[e].x);
+        const float base = now == -INFINITY ? 0.0f : now;
+        const float fade = exp2f(most - base), f = exp2f(v[e].x - base);
+        most = now;
+        total = total * fade + f * v[e].y;
+        y = y * fade + f * f32x4{u[e].x, u[e].y, w[e].x, w[e].y};
+      }
+    }
+    if (d >= c.dim) continue;
+    y *= total == 0 ? 0.0f : 1.0f / total;
+    *reinterpret_cast<V4<T>*>(out + b * out_token + (head0 + h) * out_head + d) =
+        __builtin_convertvector(y, V4<T>);
+    if (lse && d == 0)
+      lse[(int64_t)b * s.heads + head0 + h] =
+          total == 0 ? -INFINITY : (most + log2f(total)) * kLn2;
+  }
 }
 
-// Joins the pieces of sequences that have several: a workgroup a sequence and head, a wave to every
-// fourth piece.
+// Joins the pieces of sequences that have several, in their order: a workgroup a sequence and head, a
+// quarter of the pieces a wave, the pieces' weights first.
 template <typename T>
 __global__ __launch_bounds__(256) void attention_paged_join_kernel(
-    Cache c, PagedShape s, const int32_t* __restrict__ slots, T* __restrict__ out,
+    Cache c, PagedShape s, const int32_t* __restrict__ first_piece, T* __restrict__ out,
     int64_t out_token, int64_t out_head, float* __restrict__ lse,
     const int32_t* __restrict__ lengths, const float* __restrict__ part_o,
     const f32x2* __restrict__ part_ml) {
-  __shared__ f32x2 s_ml[4];
   __shared__ f32x2 s_o[4][64];
+  __shared__ float s_total[4];
   const int b = blockIdx.x / s.heads, h = blockIdx.x % s.heads;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int first, last;
-  paged_range(c, b, lengths[b], s.window, first, last);
-  const int p0 = first / s.piece, p1 = max(p0 + 1, (last + s.piece - 1) / s.piece);
-  if (p1 - p0 < 2) return;
-  const int64_t at = (int64_t)slots[b] * s.heads + h;
-  float most = -INFINITY, total = 0;
-  for (int p = p0 + lane; p < p1; p += 64) most = fmaxf(most, part_ml[at + (int64_t)p * s.heads].x);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int length = lengths[b], room = (c.indptr[b + 1] - c.indptr[b]) * c.page_size;
+  const int last = length >= 0 && length <= room ? length : 0;
+  const int first = s.window && last > s.window ? last - s.window : 0;
+  const int p0 = first / s.piece, p1 = max(p0 + 1, (last + s.piece - 1) / s.piece), n = p1 - p0;
+  if (n < 2) return;
+  const int64_t at = (int64_t)(first_piece[b] + p0) * s.heads + h;
+  const f32x2* ml = part_ml + at;
+  const float* o = part_o + at * c.dim + (2 * lane < c.dim ? 2 * lane : 0);
+  float most = -INFINITY;
+  for (int p = lane; p < n; p += 64) most = fmaxf(most, ml[(int64_t)p * s.heads].x);
   most = wave_max(most);
+  const float base = most == -INFINITY ? 0.0f : most;
+  const int per = (n + 3) / 4, begin = wave * per, end = min(n, begin + per);
+  float total = 0;
   f32x2 y{};
-  const int d = 2 * lane < c.dim ? 2 * lane : 0;
-  for (int p = p0 + wave; p < p1; p += 4) {
-    const int64_t i = at + (int64_t)p * s.heads;
-    const f32x2 v = part_ml[i];
-    const float f = v.x == -INFINITY ? 0.0f : exp2f(v.x - most);
+  for (int p = begin; p < end; p += 64) {  // 64 pieces' weights, a lane each
+    const f32x2 v = p + lane < end ? ml[(int64_t)(p + lane) * s.heads] : f32x2{-INFINITY, 0};
+    const float f = exp2f(v.x - base);
     total += f * v.y;
-    y += f * *reinterpret_cast<const f32x2*>(part_o + i * c.dim + d);
+    const int m = min(64, end - p);
+#pragma unroll 8
+    for (int e = 0; e < m; ++e)
+      y += __shfl(f, e) * *reinterpret_cast<const f32x2*>(o + (int64_t)(p + e) * s.heads * c.dim);
   }
-  if (lane == 0) s_ml[wave] = f32x2{most, total};
+  total = wave_add(total);
+  if (lane == 0) s_total[wave] = total;
   s_o[wave][lane] = y;
   __syncthreads();
   if (wave) return;
-  total = s_ml[0].y + s_ml[1].y + s_ml[2].y + s_ml[3].y;
+  total = s_total[0] + s_total[1] + s_total[2] + s_total[3];
   y = s_o[0][lane] + s_o[1][lane] + s_o[2][lane] + s_o[3][lane];
   const float f = total == 0 ? 0.0f : 1.0f / total;
   if (2 * lane < c.dim) {
@@ -394,7 +501,8 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(
     to[0] = (T)(y.x * f);
     to[1] = (T)(y.y * f);
   }
-  if (lse && lane == 0) lse[(int64_t)b * s.heads + h] = total == 0 ? -INFINITY : (most + log2f(total)) * kLn2;
+  if (lse && lane == 0)
+    lse[(int64_t)b * s.heads + h] = total == 0 ? -INFINITY : (most + log2f(total)) * kLn2;
 }
 
 int check_cache(const fsp_paged_cache& c, const std::string& who) {
@@ -451,29 +559,44 @@ int64_t paged_workgroups(const fsp_attention_paged_args& a) {
   return a.n_pieces * a.cache.kv_heads * ((group + kHeadTile - 1) / kHeadTile);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool EXACT, bool NT>
 int launch_paged(const fsp_attention_paged_args& a, hipStream_t st) {
-  const PagedShape s{(int)a.heads, (int)a.window, (int)a.piece, (float)a.scale};
+  const PagedShape s{(int)a.heads, (int)a.window, (int)a.piece, (int)a.n_pieces, (float)a.scale};
   float* part_o = static_cast<float*>(a.workspace);
-  f32x2* part_ml = reinterpret_cast<f32x2*>(part_o + a.n_pieces * a.heads * a.cache.dim);
-  hipLaunchKernelGGL((attention_paged_kernel<T, DP>), dim3((unsigned)paged_workgroups(a)),
+  float* part_ml = part_o + a.n_pieces * a.heads * a.cache.dim;
+  hipLaunchKernelGGL((attention_paged_kernel<T, DP, EXACT, NT>), dim3((unsigned)paged_workgroups(a)),
                      dim3(256), 0, st, cache_of(a.cache), s,
                      reinterpret_cast<const Piece*>(a.pieces),
                      static_cast<const T*>(a.cache.k_pages),
                      static_cast<const T*>(a.cache.v_pages), static_cast<const T*>(a.q),
                      a.q_token, a.q_head, static_cast<T*>(a.out), a.out_token, a.out_head, a.lse,
-                     a.lengths, part_o, part_ml);
+                     a.lengths, part_o, part_ml, static_cast<unsigned*>(a.arrived));
   if (int rc = check_hip(hipGetLastError(), "attention_paged_kernel launch")) return rc;
-  if (a.n_pieces == a.cache.batch) return FSP_OK;  // a piece each
+  if (a.arrived || a.n_pieces == a.cache.batch) return FSP_OK;
   hipLaunchKernelGGL((attention_paged_join_kernel<T>), dim3((unsigned)(a.cache.batch * a.heads)),
-                     dim3(256), 0, st, cache_of(a.cache), s, a.slots, static_cast<T*>(a.out),
-                     a.out_token, a.out_head, a.lse, a.lengths, part_o, part_ml);
+                     dim3(256), 0, st, cache_of(a.cache), s, a.first_piece,
+                     static_cast<T*>(a.out), a.out_token, a.out_head, a.lse, a.lengths, part_o,
+                     reinterpret_cast<const f32x2*>(part_ml));
   return check_hip(hipGetLastError(), "attention_paged_join_kernel launch");
+}
+
+// A cache that the last-level cache (256 MB) cannot hold from step to step is read with loads that
+// leave no lines behind, unless several workgroups read the same keys.  6 sequences of 131072 tokens,
+// 3.2 GB: 601 us with ordinary loads, 554 so; 200 MB read again and again: 42 and 55 us.
+template <typename T, int DP, bool EXACT>
+int launch_paged_nt(const fsp_attention_paged_args& a, hipStream_t st) {
+  const int64_t bytes = a.cache.table_len * a.cache.page_size * a.cache.kv_heads * a.cache.dim * 4;
+  return bytes > (256 << 20) && a.heads / a.cache.kv_heads <= kHeadTile
+             ? launch_paged<T, DP, EXACT, true>(a, st)
+             : launch_paged<T, DP, EXACT, false>(a, st);
 }
 
 template <typename T>
 int launch_paged_dim(const fsp_attention_paged_args& a, hipStream_t st) {
-  return a.cache.dim <= 64 ? launch_paged<T, 64>(a, st) : launch_paged<T, 128>(a, st);
+  if (a.cache.dim == 64) return launch_paged_nt<T, 64, true>(a, st);
+  if (a.cache.dim < 64) return launch_paged_nt<T, 64, false>(a, st);
+  if (a.cache.dim < 128) return launch_paged_nt<T, 128, false>(a, st);
+  return launch_paged_nt<T, 128, true>(a, st);
 }
 
 }  // namespace
@@ -506,10 +629,19 @@ extern "C" int fsp_paged_append(const fsp_paged_append_args* args, void* stream)
 }
 
 extern "C" int64_t fsp_attention_paged_piece(int64_t tokens, int64_t kv_heads) {
-  // a thousand workgroups, if pieces of 128 tokens (one step of the four waves) give them
-  int64_t piece = 128;
+  // Two steps of the four waves, longer while that leaves a round of workgroups.  Pieces of 128 / 256 /
+  // 512 / 1024 tokens, us: 96 sequences of up to 4096 tokens, 8 heads 58 / 55 / 55 / 61; 6 of 131072,
+  // 8 heads 888 / 717 / 614 / 554; 18 of up to 4183, 2 heads 11 / 12 / 13 / 16
+  int64_t piece = 256;
   while (piece < kPieceMost && tokens / piece * kv_heads > 1024) piece *= 2;
   return piece;
+}
+
+extern "C" int64_t fsp_attention_paged_counts(int64_t n_pieces, int64_t most, int64_t batch,
+                                              int64_t heads, int64_t kv_heads) {
+  if (batch < 0 || heads < 1 || kv_heads < 1 || n_pieces <= batch || most > kJoinMost) return 0;
+  const int64_t per = kv_heads * ((heads / kv_heads + kHeadTile - 1) / kHeadTile);
+  return n_pieces * per <= kResident ? batch * per : 0;
 }
 
 extern "C" int64_t fsp_attention_paged_workspace(int64_t n_pieces, int64_t heads, int64_t dim) {
@@ -531,8 +663,8 @@ extern "C" int fsp_attention_paged(const fsp_attention_paged_args* args, void* s
       paged_workgroups(a) > kMaxBlocks)
     return set_error(FSP_EINVAL, "fsp_attention_paged: pieces out of range");
   if (a.cache.batch == 0) return FSP_OK;
-  if (!a.q || !a.out || !a.lengths || !a.pieces || !a.slots ||
-      (a.n_pieces > a.cache.batch && !a.workspace))
+  if (!a.q || !a.out || !a.lengths || !a.pieces ||
+      (a.n_pieces > a.cache.batch && (!a.workspace || (!a.arrived && !a.first_piece))))
     return set_error(FSP_EINVAL, "fsp_attention_paged: null pointer");
   if (!aligned16(a.q, a.q_token, a.q_head) || !aligned16(a.out, a.out_token, a.out_head) ||
       reinterpret_cast<uintptr_t>(a.workspace) % 16)

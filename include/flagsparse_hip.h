@@ -731,15 +731,19 @@ int fsp_paged_append(const struct fsp_paged_append_args* args, void* stream);
  * NaN.
  *
  * The work is cut into pieces of `piece` tokens (fsp_attention_paged_piece() for a cache whose table
- * has room for `tokens` of them): pieces [n_pieces, 4] holds {sequence, first token, slots[sequence],
- * 0} for each piece of each sequence's room, in order, one at least for each; slots [batch] the
- * number of pieces before the sequence's first.  workspace: fsp_attention_paged_workspace() bytes,
- * 16-byte aligned, unless every sequence has one piece.
+ * has room for `tokens` of them): pieces [n_pieces, 8] holds {sequence, first token, the sequence's
+ * first piece, page_indptr[sequence], its pages' room in tokens, 0, 0, 0} for each piece of each
+ * sequence's room, in order, one at least for each; first_piece [batch] the sequences' first ones.
+ * Unless every sequence has one piece: workspace, fsp_attention_paged_workspace() bytes, 16-byte
+ * aligned, and either arrived, 32-bit counts that are zero, as the call leaves them (calls that may
+ * overlap have counts of their own), or NULL, which takes a second launch;
+ * fsp_attention_paged_counts() says how many counts, or 0 where the second launch is the faster
+ * (most: the most pieces of one sequence).
  */
 struct fsp_attention_paged_args {
   struct fsp_paged_cache cache;
   const int32_t* pieces;
-  const int32_t* slots;
+  const int32_t* first_piece;
   int64_t n_pieces, piece, heads, window;
   double scale;
   int64_t q_token, q_head, out_token, out_head;
@@ -748,7 +752,10 @@ struct fsp_attention_paged_args {
   float* lse;
   const int32_t* lengths;
   void* workspace;
+  void* arrived;
 };
+int64_t fsp_attention_paged_counts(int64_t n_pieces, int64_t most, int64_t batch, int64_t heads,
+                                   int64_t kv_heads);
 int64_t fsp_attention_paged_piece(int64_t tokens, int64_t kv_heads);
 int64_t fsp_attention_paged_workspace(int64_t n_pieces, int64_t heads, int64_t dim);
 int fsp_attention_paged(const struct fsp_attention_paged_args* args, void* stream);

@@ -50,19 +50,21 @@ def test_struct_sizes():
     # 8-byte fields, as in the header
     assert attention._CACHE.size == 8 * 17
     assert attention._APPEND.size + attention._APPEND_AT.size == 8 * 21
-    assert attention._PAGED.size + attention._PAGED_AT.size == 8 * 16
+    assert attention._PAGED.size + attention._PAGED_AT.size == 8 * 17
     assert attention._PACKED.size + attention._PACKED_AT.size == 8 * (13 + 16 + 10)
     assert _abi.lib().fsp_attention_dim_cap() == attention._DIM_CAP
 
 
-@pytest.mark.parametrize("rooms", [[], [0], [128, 0, 129, 1], [5000, 16, 128]])
-def test_pieces_cover_the_rooms(rooms):
-    table, slots = attention._pieces(np.array(rooms, dtype=np.int64), 128)
+@pytest.mark.parametrize("pages", [[], [0], [8, 0, 9, 1], [320, 1, 8]])
+def test_pieces_cover_the_rooms(pages):
+    table, firsts, most = attention._pieces(np.array(pages, dtype=np.int64), 16, 128)
     at = 0
-    for b, room in enumerate(rooms):
-        assert slots[b] == at
-        for i in range(max(1, -(-room // 128))):
-            assert table[at].tolist() == [b, 128 * i, slots[b], 0]
+    assert most == max([1] + [-(-16 * n // 128) for n in pages])
+    for b, n in enumerate(pages):
+        first = at
+        assert firsts[b] == first
+        for i in range(max(1, -(-16 * n // 128))):
+            assert table[at].tolist() == [b, 128 * i, first, sum(pages[:b]), 16 * n, 0, 0, 0]
             at += 1
     assert at == len(table)
 
@@ -117,8 +119,8 @@ def _cache(**kw):
     return attention._CACHE.pack(*a.values())
 
 
-_PAGED_ARGS = dict(pieces=16, slots=16, n_pieces=3, piece=128, heads=4, window=0, scale=0.125, qt=256,
-                   qh=64, ot=256, oh=64, q=64, out=64, lse=0, lengths=16, work=16)
+_PAGED_ARGS = dict(pieces=16, first=16, n_pieces=3, piece=128, heads=4, window=0, scale=0.125, qt=256,
+                   qh=64, ot=256, oh=64, q=64, out=64, lse=0, lengths=16, work=16, counts=16)
 _APPEND_ARGS = dict(n_tokens=2, heads=4, half=32, rows=64, interleaved=0, kt=128, kh=64, vt=128, vh=64,
                     qt=256, qh=64, qot=256, qoh=64, k=64, v=64, q=64, qo=64, cos=16, sin=16, tokens=0,
                     lengths=16)
@@ -148,7 +150,7 @@ def test_cache_refusals_of_the_library(status, kw):
 
 @pytest.mark.parametrize("kw", [{"heads": 3}, {"heads": 0}, {"window": -1}, {"q": 0}, {"out": 0},
                                 {"lengths": 0}, {"q": 72}, {"oh": 2}, {"work": 0}, {"work": 8},
-                                {"pieces": 0}, {"slots": 0}, {"n_pieces": 1}, {"n_pieces": 1 << 40},
+                                {"pieces": 0}, {"counts": 0, "first": 0}, {"n_pieces": 1}, {"n_pieces": 1 << 40},
                                 {"piece": 0}, {"piece": 2048}, {"piece": 130}])
 def test_paged_refusals_of_the_library(kw):
     L = _abi.lib()

@@ -114,6 +114,24 @@ def test_many_sequences(dev):
     _decode(dev, [(7 * i) % 40 for i in range(700)], 8, 2, 1, 64, BF)
 
 
+def test_caches_past_the_last_level(dev):
+    # a table of more than 256 MB is read by other loads
+    pages, page, g, d, n = 16 * 1024, 64, 2, 128, 3000
+    kp = torch.empty(pages, page, g, d, dtype=HF, device=dev)
+    vp = torch.empty(pages, page, g, d, dtype=HF, device=dev)
+    k, v = (_normal(s, n, g, d, dtype=HF) for s in (1, 2))
+    kv = fs.prepare_paged_kv(kp, vp, torch.tensor([0, 50, pages], device=dev),
+                             torch.arange(pages, device=dev).flip(0))
+    lengths = torch.tensor([n, 1], device=dev)
+    fs.flagsparse_paged_append(torch.cat([k, k[:1]]).to(dev), torch.cat([v, v[:1]]).to(dev), lengths,
+                               torch.tensor([0, n, n + 1], device=dev), prepared=kv)
+    q = _normal(3, 2, 6, d, dtype=HF).to(dev)
+    out, lse = fs.flagsparse_attention_paged(q, lengths, prepared=kv, return_lse=True)
+    want = _want(q, [k, k[:1]], [v, v[:1]], [n, 1], None, d**-0.5)
+    ref.check("out", out, want["out"])
+    ref.check("lse", lse, want["lse"])
+
+
 def test_lengths_change_and_tables_are_copies(dev):
     lengths = [300, 50]
     kp, vp, ip, ix, k, v = _cache(dev, lengths, 16, 2, 64, BF)
