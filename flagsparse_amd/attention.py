@@ -39,7 +39,7 @@ _STEP_CAP = 2**23
 _CACHE = struct.Struct("17q")
 _APPEND, _APPEND_AT = struct.Struct("13q"), struct.Struct("8q")
 _PAGED, _PAGED_AT = struct.Struct("6qd4q"), struct.Struct("6q")
-_PACKED, _PACKED_AT = struct.Struct("8qd20q"), struct.Struct("10q")
+_PACKED, _PACKED_AT = struct.Struct("10qd20q"), struct.Struct("10q")
 
 # A prepared object keeps the first part for each layout of arrays that it has checked, so that the
 # next call with such arrays is a look-up and a launch.
@@ -491,13 +491,14 @@ class PreparedAttention:
     one sequence's rows, those with the most to do first, so that the last ones to finish are
     short."""
 
-    __slots__ = ("batch", "q_tokens", "k_tokens", "device", "_tiles", "_streams", "_calls")
+    __slots__ = ("batch", "q_tokens", "k_tokens", "device", "_longest", "_tiles", "_streams", "_calls")
 
     def __init__(self, q_len, k_len, device):
         self.batch = len(q_len)
         self.q_tokens = int(q_len.sum())
         self.k_tokens = int(k_len.sum())
         self.device = device
+        self._longest = tuple(int(n.max(initial=0)) for n in (q_len, k_len))
         tile = [int(_abi.lib().fsp_attention_packed_tile(keys)) for keys in (0, 1)]
         lists = [_tiles(q_len, k_len, tile[keys], causal, keys)
                  for keys in (False, True) for causal in (False, True)]
@@ -605,7 +606,7 @@ def _pack(prepared, q, k, v, causal, window, scale, out, grads=()):
     steps = [n for t in (q, k, v, out, *grads) for n in t.stride()[:2]]
     steps += [0] * (16 - len(steps))
     return _PACKED.pack(_CODES[q.dtype], q.shape[1], k.shape[1], q.shape[2], q.shape[0],
-                        k.shape[0], causal, window, scale, q_tiles.data_ptr(), q_tiles.shape[0],
+                        k.shape[0], *prepared._longest, causal, window, scale, q_tiles.data_ptr(), q_tiles.shape[0],
                         k_tiles.data_ptr(), k_tiles.shape[0] if grads else 0, *steps)
 
 
@@ -692,17 +693,22 @@ def _backward(prepared, grad_out, q, k, v, out, lse, causal, window, scale, key=
     flat = lse.contiguous()
     grads = tuple(torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
     head = _pack(prepared, *rows[1:4], causal, window, scale, rows[4], (rows[0], *grads))
-    _run_backward(prepared, head, rows, flat, grads)
+    kept = head, int(_abi.lib().fsp_attention_packed_workspace(
+        prepared._tiles[True, causal].shape[0], q.shape[1], k.shape[1], q.shape[2], q.shape[0],
+        k.shape[0]))
+    _run_backward(prepared, kept, rows, flat, grads)
     if key is not None and flat is lse and all(
             x is y for x, y in zip(rows, (grad_out, q, k, v, out))):
-        _keep(prepared._calls, key, head)
+        _keep(prepared._calls, key, kept)
     return grads
 
 
-def _run_backward(prepared, head, rows, lse, grads):
+def _run_backward(prepared, kept, rows, lse, grads):
+    """``kept``: the arguments up to the addresses, and the bytes of workspace."""
+    head, room = kept
     grad_out, q, k, v, out = rows
     if q.shape[0] or k.shape[0]:
-        work = torch.empty((2, q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
+        work = torch.empty(room, dtype=torch.uint8, device=q.device)
         status = _abi.lib().fsp_attention_packed_backward(head + _PACKED_AT.pack(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
             grad_out.data_ptr(), grads[0].data_ptr(), grads[1].data_ptr(), grads[2].data_ptr(),

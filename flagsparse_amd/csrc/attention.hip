@@ -103,6 +103,20 @@ __device__ __forceinline__ void load_rows(char* lds, const void* src, int n, uin
   }
 }
 
+// The order of the LDS reads and matrix instructions before it: AHEAD reads, then a product and a read
+// in turn, then the products that are left.  Left to itself the compiler reads an operand just
+// before its product and waits out the LDS's latency each time.
+template <int READS, int AHEAD>
+__device__ __forceinline__ void read_ahead() {
+  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+  for (int i = 0; i < READS - AHEAD; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+}
+
 // Matrix operands from LDS: 8 consecutive elements of a row a lane, and 8 rows' elements of a column
 // (rows 16 * i + {0..3, 8..11} + 4 * (lane / 32), the ones that the lane's accumulator registers
 // 8 * i..8 * i + 7 stand for).
@@ -138,29 +152,35 @@ __device__ __forceinline__ void store_rows(T* to, const f32x16 (&x)[NT], float f
         f32x4 y;
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = x[i][r + e] * f;
-        *reinterpret_cast<V4<T>*>(to + d) = __builtin_convertvector(y, V4<T>);
+        if constexpr (std::is_same<T, float>::value)
+          *reinterpret_cast<f32x4*>(to + d) = y;
+        else
+          *reinterpret_cast<V4<T>*>(to + d) = __builtin_convertvector(y, V4<T>);
       }
     }
 }
 
-template <typename T, int DP>
-__global__ __launch_bounds__(256, 2) void attention_packed_kernel(
+// A wave to 32 queries and, of every PARTS * 64 keys, 64: with PARTS = 2 two waves share the queries,
+// and their sums are joined at the end.  That halves the chain of steps where there are too few
+// workgroups to fill the chip (PARTS_FIGURES).
+template <typename T, int DP, int PARTS>
+__global__ __launch_bounds__(256 * PARTS, 2) void attention_packed_kernel(
     Shape s, const Tile* __restrict__ tiles, int n_tiles, const T* __restrict__ q, int64_t q_token,
     int64_t q_head, const T* __restrict__ k, int64_t k_token, int64_t k_head,
     const T* __restrict__ v, int64_t v_token, int64_t v_head, T* __restrict__ out,
     int64_t o_token, int64_t o_head, float* __restrict__ lse) {
   typedef Lay<DP> L;
   constexpr int NS = DP / 16, NT = DP / 32;
-  __shared__ __attribute__((aligned(1024))) char s_k0[L::BYTES], s_v0[L::BYTES], s_k1[L::BYTES],
-      s_v1[L::BYTES];
+  constexpr int BYTES = PARTS * L::BYTES, ROWS = PARTS * kRows;
+  __shared__ __attribute__((aligned(1024))) char s_k0[BYTES], s_v0[BYTES], s_k1[BYTES], s_v1[BYTES];
   int tile, a;
   tile_and_head(blockIdx.x, n_tiles, s.heads, tile, a);
   const Tile t = tiles[tile];
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = a / (s.heads / s.kv_heads);
-  const int mine = wave * 32 + col;  // this lane's row of the tile
-  const bool active = wave * 32 < t.rows;
+  const int part = wave / 4, q0 = (wave % 4) * 32, mine = q0 + col;  // this lane's row of the tile
+  const bool active = q0 < t.rows;
 
   V8<T> qf[NS];
   {
@@ -177,8 +197,8 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(
   // the keys that this lane's row sees, and those of the wave's first and last rows
   int lo, hi, lo0, hi0, lo1, hi1, lot, hit, none;
   seen_by(s, t, t.at + min(mine, t.rows - 1), lo, hi);
-  seen_by(s, t, t.at + min(wave * 32, t.rows - 1), lo0, hi0);
-  seen_by(s, t, t.at + min(wave * 32 + 31, t.rows - 1), lo1, hi1);
+  seen_by(s, t, t.at + min(q0, t.rows - 1), lo0, hi0);
+  seen_by(s, t, t.at + min(q0 + 31, t.rows - 1), lo1, hi1);
   seen_by(s, t, t.at, lot, none);
   seen_by(s, t, t.at + t.rows - 1, none, hit);
 
@@ -190,7 +210,7 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(
   const T* kb = k + (int64_t)t.k_begin * k_token + g * k_head;
   const T* vb = v + (int64_t)t.k_begin * v_token + g * v_head;
   auto load = [&](int j0, char* sk, char* sv) {
-    const int n = min(kRows, t.nk - j0);
+    const int n = min(ROWS, t.nk - j0);
     load_rows<DP>(sk, kb + j0 * k_token, n, (uint32_t)(2 * k_token), s.dim, wave, lane);
     load_rows<DP>(sv, vb + j0 * v_token, n, (uint32_t)(2 * v_token), s.dim, wave, lane);
   };
@@ -198,9 +218,10 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(
   const int v_at = L::col_at(lane);
 
   auto step = [&](int j0, const char* sk_, const char* sv_) {
+    j0 += part * kRows;
     if (!active || j0 >= hi1 || j0 + kRows <= lo0) return;
-    const lds_char* sk = (const lds_char*)sk_;
-    const lds_char* sv = (const lds_char*)sv_;
+    const lds_char* sk = (const lds_char*)sk_ + part * L::BYTES;
+    const lds_char* sv = (const lds_char*)sv_ + part * L::BYTES;
     f32x16 x[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -210,6 +231,7 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(
         x[u] = mfma32(row_frag<T>(sk + (k_at ^ (i * 32)) + u * 32 * L::PITCH), qf[i], x[u]);
       }
     }
+    read_ahead<2 * NS, NS>();
     if (j0 + kRows > hi0 || j0 < lo1) {
       const int first = lo - j0 - 4 * half, last = hi - j0 - 4 * half;
 #pragma unroll
@@ -251,24 +273,48 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(
         o[n] = mfma32(col_frag<T, L::PITCH>(sv, v_at ^ (64 * n), i), pf, o[n]);
       }
     }
+    __builtin_amdgcn_sched_group_barrier(0x100, 4 * NT, 1);  // the first values early
   };
 
   int j0 = lot;
   if (j0 < hit) load(j0, s_k0, s_v0);
   __syncthreads();
   while (j0 < hit) {
-    if (j0 + kRows < hit) load(j0 + kRows, s_k1, s_v1);
+    if (j0 + ROWS < hit) load(j0 + ROWS, s_k1, s_v1);
     step(j0, s_k0, s_v0);
     __syncthreads();
-    j0 += kRows;
+    j0 += ROWS;
     if (j0 >= hit) break;
-    if (j0 + kRows < hit) load(j0 + kRows, s_k0, s_v0);
+    if (j0 + ROWS < hit) load(j0 + ROWS, s_k0, s_v0);
     step(j0, s_k1, s_v1);
     __syncthreads();
-    j0 += kRows;
+    j0 += ROWS;
   }
 
   sum += other_half(sum);
+  if constexpr (PARTS > 1) {
+    float* theirs = reinterpret_cast<float*>(wave % 4 == 0 ? s_k0 : wave % 4 == 1 ? s_v0 : wave % 4 == 2 ? s_k1 : s_v1);
+    __shared__ f32x2 s_stat[4][64];
+    static_assert(NT * 16 * 64 * 4 <= BYTES, "");
+    if (part == 1) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) theirs[(16 * i + r) * 64 + lane] = o[i][r];
+      s_stat[wave % 4][lane] = f32x2{top, sum};
+    }
+    __syncthreads();
+    if (part == 1) return;
+    const f32x2 other = s_stat[wave][lane];
+    const float now = fmaxf(top, other.x), base = now == -INFINITY ? 0.0f : now;
+    const float f0 = exp2f((top - base) * c), f1 = exp2f((other.x - base) * c);
+    top = now;
+    sum = sum * f0 + other.y * f1;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[i][r] = o[i][r] * f0 + theirs[(16 * i + r) * 64 + lane] * f1;
+  }
   if (mine >= t.rows) return;
   const int64_t row = t.first + mine;
   const float inv = sum > 0 ? 1.0f / sum : (sum == 0 ? 0.0f : sum);
@@ -286,8 +332,8 @@ template <> struct Lift<f16> { static constexpr float up = 14, down = 1.0f / 163
 
 // Gradient of the queries: the forward pass's loop over keys with dP^T = V grad_out^T beside S^T; dS^T
 // is the operand of dQ^T = K^T dS^T where it lies.
-template <typename T, int DP>
-__global__ __launch_bounds__(256, 2) void attention_grad_q_kernel(
+template <typename T, int DP, int PARTS>
+__global__ __launch_bounds__(256 * PARTS, 2) void attention_grad_q_kernel(
     Shape s, const Tile* __restrict__ tiles, int n_tiles, const T* __restrict__ q, int64_t q_token,
     int64_t q_head, const T* __restrict__ k, int64_t k_token, int64_t k_head,
     const T* __restrict__ v, int64_t v_token, int64_t v_head, const T* __restrict__ out,
@@ -296,16 +342,16 @@ __global__ __launch_bounds__(256, 2) void attention_grad_q_kernel(
     float* __restrict__ stats, int64_t q_tokens) {
   typedef Lay<DP> L;
   constexpr int NS = DP / 16, NT = DP / 32;
-  __shared__ __attribute__((aligned(1024))) char s_k0[L::BYTES], s_v0[L::BYTES], s_k1[L::BYTES],
-      s_v1[L::BYTES];
+  constexpr int BYTES = PARTS * L::BYTES, ROWS = PARTS * kRows;
+  __shared__ __attribute__((aligned(1024))) char s_k0[BYTES], s_v0[BYTES], s_k1[BYTES], s_v1[BYTES];
   int tile, a;
   tile_and_head(blockIdx.x, n_tiles, s.heads, tile, a);
   const Tile t = tiles[tile];
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = a / (s.heads / s.kv_heads);
-  const int mine = wave * 32 + col;
-  const bool active = wave * 32 < t.rows;
+  const int part = wave / 4, q0 = (wave % 4) * 32, mine = q0 + col;
+  const bool active = q0 < t.rows;
   const int64_t row = t.first + (int64_t)min(mine, t.rows - 1);
 
   V8<T> qf[NS], gf[NS];
@@ -326,15 +372,15 @@ __global__ __launch_bounds__(256, 2) void attention_grad_q_kernel(
   float base = lse[row * s.heads + a];
   base = base == -INFINITY ? INFINITY : base * kLog2e;
   // what the keys' gradients start their products from: see there
-  if (half == 0 && mine < t.rows) {
+  if (part == 0 && half == 0 && mine < t.rows) {
     stats[a * q_tokens + row] = (Lift<T>::up - base) / c;
     stats[(s.heads + a) * q_tokens + row] = -delta;
   }
 
   int lo, hi, lo0, hi0, lo1, hi1, lot, hit, none;
   seen_by(s, t, t.at + min(mine, t.rows - 1), lo, hi);
-  seen_by(s, t, t.at + min(wave * 32, t.rows - 1), lo0, hi0);
-  seen_by(s, t, t.at + min(wave * 32 + 31, t.rows - 1), lo1, hi1);
+  seen_by(s, t, t.at + min(q0, t.rows - 1), lo0, hi0);
+  seen_by(s, t, t.at + min(q0 + 31, t.rows - 1), lo1, hi1);
   seen_by(s, t, t.at, lot, none);
   seen_by(s, t, t.at + t.rows - 1, none, hit);
 
@@ -345,7 +391,7 @@ __global__ __launch_bounds__(256, 2) void attention_grad_q_kernel(
   const T* kb = k + (int64_t)t.k_begin * k_token + g * k_head;
   const T* vb = v + (int64_t)t.k_begin * v_token + g * v_head;
   auto load = [&](int j0, char* sk, char* sv) {
-    const int n = min(kRows, t.nk - j0);
+    const int n = min(ROWS, t.nk - j0);
     load_rows<DP>(sk, kb + j0 * k_token, n, (uint32_t)(2 * k_token), s.dim, wave, lane);
     load_rows<DP>(sv, vb + j0 * v_token, n, (uint32_t)(2 * v_token), s.dim, wave, lane);
   };
@@ -353,9 +399,10 @@ __global__ __launch_bounds__(256, 2) void attention_grad_q_kernel(
   const int c_at = L::col_at(lane);
 
   auto step = [&](int j0, const char* sk_, const char* sv_) {
+    j0 += part * kRows;
     if (!active || j0 >= hi1 || j0 + kRows <= lo0) return;
-    const lds_char* sk = (const lds_char*)sk_;
-    const lds_char* sv = (const lds_char*)sv_;
+    const lds_char* sk = (const lds_char*)sk_ + part * L::BYTES;
+    const lds_char* sv = (const lds_char*)sv_ + part * L::BYTES;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       f32x16 x{}, y{};
@@ -389,15 +436,29 @@ __global__ __launch_bounds__(256, 2) void attention_grad_q_kernel(
   if (j0 < hit) load(j0, s_k0, s_v0);
   __syncthreads();
   while (j0 < hit) {
-    if (j0 + kRows < hit) load(j0 + kRows, s_k1, s_v1);
+    if (j0 + ROWS < hit) load(j0 + ROWS, s_k1, s_v1);
     step(j0, s_k0, s_v0);
     __syncthreads();
-    j0 += kRows;
+    j0 += ROWS;
     if (j0 >= hit) break;
-    if (j0 + kRows < hit) load(j0 + kRows, s_k0, s_v0);
+    if (j0 + ROWS < hit) load(j0 + ROWS, s_k0, s_v0);
     step(j0, s_k1, s_v1);
     __syncthreads();
-    j0 += kRows;
+    j0 += ROWS;
+  }
+  if constexpr (PARTS > 1) {
+    float* theirs = reinterpret_cast<float*>(wave % 4 == 0 ? s_k0 : wave % 4 == 1 ? s_v0 : wave % 4 == 2 ? s_k1 : s_v1);
+    if (part == 1)
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) theirs[(16 * i + r) * 64 + lane] = acc[i][r];
+    __syncthreads();
+    if (part == 1) return;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][r] += theirs[(16 * i + r) * 64 + lane];
   }
   if (mine < t.rows)
     store_rows<T, NT>(dq + row * dq_token + a * dq_head, acc, s.scale, s.dim, half);
@@ -406,29 +467,31 @@ __global__ __launch_bounds__(256, 2) void attention_grad_q_kernel(
 // Gradients of the keys and values, 64 keys a workgroup, over the heads of the group and their
 // queries.  S and dP are [queries, keys], so P and dS are the operands of dV^T = grad_out^T P and
 // dK^T = Q^T dS where they lie.  The products start from a row's -lse / scale and -delta, so that they
-// give S - lse and dP - delta.  Two waves share 32 keys, one to every other 32 queries; their sums
-// are joined through LDS at the end.
-template <typename T, int DP>
-__global__ __launch_bounds__(256, 2) void attention_grad_kv_kernel(
+// give S - lse and dP - delta.  PARTS waves share 32 keys, one to every PARTS-th 32 queries;
+// their sums are joined through LDS at the end, in their order.
+template <typename T, int DP, int PARTS>
+__global__ __launch_bounds__(128 * PARTS, 2) void attention_grad_kv_kernel(
     Shape s, const Tile* __restrict__ tiles, int n_tiles, const T* __restrict__ q, int64_t q_token,
     int64_t q_head, const T* __restrict__ k, int64_t k_token, int64_t k_head,
     const T* __restrict__ v, int64_t v_token, int64_t v_head, const T* __restrict__ go,
     int64_t go_token, int64_t go_head, const float* __restrict__ stats, int64_t q_tokens,
     T* __restrict__ dk, int64_t dk_token, int64_t dk_head, T* __restrict__ dv, int64_t dv_token,
-    int64_t dv_head) {
+    int64_t dv_head, int split, float* __restrict__ sums, int64_t k_tokens) {
   typedef Lay<DP> L;
   constexpr int NS = DP / 16, NT = DP / 32;
-  __shared__ __attribute__((aligned(1024))) char s_q0[L::BYTES], s_g0[L::BYTES], s_q1[L::BYTES],
-      s_g1[L::BYTES];
-  __shared__ __attribute__((aligned(256))) float s_x0[kRows], s_y0[kRows], s_x1[kRows], s_y1[kRows];
+  constexpr int ROWS = 32 * PARTS, BYTES = ROWS * L::PITCH;
+  __shared__ __attribute__((aligned(1024))) char s_q0[BYTES], s_g0[BYTES], s_q1[BYTES], s_g1[BYTES];
+  __shared__ __attribute__((aligned(256))) float s_x0[ROWS], s_y0[ROWS], s_x1[ROWS], s_y1[ROWS];
   int tile, g;
-  tile_and_head(blockIdx.x, n_tiles, s.kv_heads, tile, g);
+  tile_and_head(blockIdx.x, n_tiles, s.kv_heads * split, tile, g);
+  const int share = g % split;  // of the group's heads
+  g /= split;
   const Tile t = tiles[tile];
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int part = wave & 1, k0 = (wave >> 1) * 32, mine = k0 + col;
+  const int part = wave % PARTS, block = wave / PARTS, k0 = block * 32, mine = k0 + col;
   const bool active = k0 < t.rows;
-  const int group = s.heads / s.kv_heads;
+  const int group = s.heads / s.kv_heads / split;
   const int64_t row = t.first + (int64_t)min(mine, t.rows - 1);
 
   V8<T> kf[NS], vf[NS];
@@ -458,18 +521,20 @@ __global__ __launch_bounds__(256, 2) void attention_grad_kv_kernel(
   const int c_at = L::col_at(lane) + part * 32 * L::PITCH;
 
   auto load = [&](int a, int i0, char* sq, char* sg, float* sx, float* sy) {
-    const int n = min(kRows, t.nq - i0);
+    const int n = min(ROWS, t.nq - i0);
     const int64_t first = (int64_t)t.q_begin + i0;
     // the rows' offsets are made anew in every step: kept, they would not fit the registers
     int l = lane;
     asm volatile("" : "+v"(l));
     load_rows<DP>(sq, q + first * q_token + a * q_head, n, (uint32_t)(2 * q_token), s.dim, wave, l);
     load_rows<DP>(sg, go + first * go_token + a * go_head, n, (uint32_t)(2 * go_token), s.dim, wave, l);
-    if (wave < 2) {
+    if (wave < PARTS) {  // 64 rows' statistics a wave
+      const int which = wave & 1, at = (wave >> 1) * 64;
       const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<float*>(stats + (wave * s.heads + a) * q_tokens + first), 0, 4 * n, 0x00027000);
+          const_cast<float*>(stats + (which * s.heads + a) * q_tokens + first), 0, 4 * n, 0x00027000);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rsrc, (__attribute__((address_space(3))) void*)(wave ? sy : sx), 4, 4 * l, 0, 0, 0);
+          rsrc, (__attribute__((address_space(3))) void*)((which ? sy : sx) + at), 4, 4 * (at + l), 0,
+          0, 0);
     }
   };
 
@@ -520,11 +585,11 @@ __global__ __launch_bounds__(256, 2) void attention_grad_kv_kernel(
   };
 
   // the steps of every head of the group, one after the other
-  const int steps = hit > lot ? (hit - lot + kRows - 1) / kRows : 0;
+  const int steps = hit > lot ? (hit - lot + ROWS - 1) / ROWS : 0;
   const int total = steps * group;
-  int a = g * group, i0 = lot, a1 = a, i1 = lot;  // of this step, and of the one being loaded
+  int a = (g * split + share) * group, i0 = lot, a1 = a, i1 = lot;  // of this step, and of the one being loaded
   auto next = [&] {
-    i1 += kRows;
+    i1 += ROWS;
     if (i1 >= hit) i1 = lot, ++a1;
   };
   if (total) load(a, i0, s_q0, s_g0, s_x0, s_y0);
@@ -544,27 +609,56 @@ __global__ __launch_bounds__(256, 2) void attention_grad_kv_kernel(
     ++n;
   }
 
-  // join the two waves of the same keys, the even ones' sums first
-  float* joined = reinterpret_cast<float*>((wave >> 1) ? s_q1 : s_q0);
+  // join the waves of the same keys
+  float* joined = reinterpret_cast<float*>(block ? s_q1 : s_q0);
+  static_assert((PARTS - 1) * 16 * 64 * 4 <= BYTES, "");
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     f32x16* acc = which ? ak : av;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      if (part == 1)
+      if (part)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) joined[r * 64 + lane] = acc[i][r];
+        for (int r = 0; r < 16; ++r) joined[(16 * (part - 1) + r) * 64 + lane] = acc[i][r];
       __syncthreads();
       if (part == 0)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i][r] += joined[r * 64 + lane];
+        for (int p = 0; p < PARTS - 1; ++p)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][r] += joined[(16 * p + r) * 64 + lane];
       __syncthreads();
     }
   }
   if (part == 0 && mine < t.rows) {
+    if (split > 1) {
+      float* to = sums + ((int64_t)(share * s.kv_heads + g) * k_tokens + row) * s.dim;
+      store_rows<float, NT>(to, av, Lift<T>::down, s.dim, half);
+      store_rows<float, NT>(to + (int64_t)split * s.kv_heads * k_tokens * s.dim, ak, s.scale, s.dim, half);
+      return;
+    }
     store_rows<T, NT>(dv + row * dv_token + g * dv_head, av, Lift<T>::down, s.dim, half);
     store_rows<T, NT>(dk + row * dk_token + g * dk_head, ak, s.scale, s.dim, half);
   }
+}
+
+// The keys' and values' gradients as the sums of ``split`` shares of the heads, in their order: a thread
+// to four elements.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_grad_kv_sum_kernel(
+    Shape s, int split, const float* __restrict__ sums, int64_t k_tokens, T* __restrict__ dk,
+    int64_t dk_token, int64_t dk_head, T* __restrict__ dv, int64_t dv_token, int64_t dv_head) {
+  const int64_t each = (int64_t)s.kv_heads * k_tokens * s.dim;  // elements of one share
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= 2 * each) return;
+  const bool keys = i >= each;
+  const int64_t at = keys ? i - each : i;
+  const float* from = sums + (keys ? split * each : 0) + at;
+  f32x4 y = *reinterpret_cast<const f32x4*>(from);
+  for (int p = 1; p < split; ++p) y += *reinterpret_cast<const f32x4*>(from + p * each);
+  const int64_t row = at / s.dim;
+  const int64_t g = row / k_tokens, t = row - g * k_tokens;
+  T* to = (keys ? dk + t * dk_token + g * dk_head : dv + t * dv_token + g * dv_head) + at % s.dim;
+  *reinterpret_cast<V4<T>*>(to) = __builtin_convertvector(y, V4<T>);
 }
 
 template <typename T>
@@ -575,45 +669,101 @@ Shape shape_of(const fsp_attention_packed_args& a) {
           (float)a.scale};
 }
 
-template <typename T, int DP>
+// Where the workgroups of one tile and head would not fill the chip (two to a CU, four up to a dim of
+// 64) and have long chains of steps, twice as many waves share a tile.
+// LAUNCH_FIGURES
+constexpr int64_t kCus = 256, kLong = 1024;
+
+int64_t seen_at_most(const fsp_attention_packed_args& a, int64_t longest) {
+  return a.window && a.window < longest ? a.window : longest;
+}
+
+bool share_queries(const fsp_attention_packed_args& a) {
+  return a.n_q_tiles * a.heads <= (a.dim <= 64 ? 4 : 2) * kCus && seen_at_most(a, a.k_longest) >= kLong;
+}
+
+bool share_keys(const fsp_attention_packed_args& a, int split) {
+  return a.n_k_tiles * a.kv_heads * split <= 2 * kCus &&
+         a.heads / a.kv_heads / split * seen_at_most(a, a.q_longest) >= kLong;
+}
+
+// Shares of a group's heads that go to workgroups of their own, for their sums to be added by another
+// launch: as many as two workgroups to a CU take.
+// SPLIT_FIGURES
+int split_heads(int64_t n_k_tiles, int64_t heads, int64_t kv_heads) {
+  const int64_t group = heads / kv_heads, n = n_k_tiles * kv_heads;
+  int64_t split = 1;
+  for (int64_t i = 2; i <= group && i * n <= 2 * kCus; ++i)
+    if (group % i == 0) split = i;
+  return (int)split;
+}
+
+template <typename T, int DP, int PARTS>
 int launch_forward(const fsp_attention_packed_args& a, hipStream_t st) {
-  hipLaunchKernelGGL((attention_packed_kernel<T, DP>), dim3((unsigned)(a.n_q_tiles * a.heads)),
-                     dim3(256), 0, st, shape_of(a), reinterpret_cast<const Tile*>(a.q_tiles),
-                     (int)a.n_q_tiles, in<T>(a.q), a.q_token, a.q_head, in<T>(a.k), a.k_token,
-                     a.k_head, in<T>(a.v), a.v_token, a.v_head, static_cast<T*>(a.out),
-                     a.out_token, a.out_head, a.lse);
+  hipLaunchKernelGGL((attention_packed_kernel<T, DP, PARTS>),
+                     dim3((unsigned)(a.n_q_tiles * a.heads)), dim3(256 * PARTS), 0, st, shape_of(a),
+                     reinterpret_cast<const Tile*>(a.q_tiles), (int)a.n_q_tiles, in<T>(a.q),
+                     a.q_token, a.q_head, in<T>(a.k), a.k_token, a.k_head, in<T>(a.v), a.v_token,
+                     a.v_head, static_cast<T*>(a.out), a.out_token, a.out_head, a.lse);
   return check_hip(hipGetLastError(), "attention_packed_kernel launch");
+}
+
+template <typename T, int DP>
+int launch_forward_parts(const fsp_attention_packed_args& a, hipStream_t st) {
+  return share_queries(a) ? launch_forward<T, DP, 2>(a, st) : launch_forward<T, DP, 1>(a, st);
 }
 
 template <typename T>
 int launch_forward_dim(const fsp_attention_packed_args& a, hipStream_t st) {
-  if (a.dim <= 64) return launch_forward<T, 64>(a, st);
-  if (a.dim <= 96) return launch_forward<T, 96>(a, st);
-  return launch_forward<T, 128>(a, st);
+  if (a.dim <= 64) return launch_forward_parts<T, 64>(a, st);
+  if (a.dim <= 96) return launch_forward_parts<T, 96>(a, st);
+  return launch_forward_parts<T, 128>(a, st);
+}
+
+template <typename T, int DP, int PARTS>
+int launch_grad_q(const fsp_attention_packed_args& a, hipStream_t st) {
+  hipLaunchKernelGGL((attention_grad_q_kernel<T, DP, PARTS>),
+                     dim3((unsigned)(a.n_q_tiles * a.heads)), dim3(256 * PARTS), 0, st, shape_of(a),
+                     reinterpret_cast<const Tile*>(a.q_tiles), (int)a.n_q_tiles, in<T>(a.q),
+                     a.q_token, a.q_head, in<T>(a.k), a.k_token, a.k_head, in<T>(a.v), a.v_token,
+                     a.v_head, in<T>(a.out), a.out_token, a.out_head, a.lse, in<T>(a.grad_out),
+                     a.grad_out_token, a.grad_out_head, static_cast<T*>(a.grad_q), a.grad_q_token,
+                     a.grad_q_head, static_cast<float*>(a.workspace), a.q_tokens);
+  return check_hip(hipGetLastError(), "attention_grad_q_kernel launch");
+}
+
+template <typename T, int DP, int PARTS>
+int launch_grad_kv(const fsp_attention_packed_args& a, int split, hipStream_t st) {
+  float* stats = static_cast<float*>(a.workspace);
+  float* sums = stats + ((2 * a.heads * a.q_tokens + 3) & ~int64_t(3));
+  hipLaunchKernelGGL((attention_grad_kv_kernel<T, DP, PARTS>),
+                     dim3((unsigned)(a.n_k_tiles * a.kv_heads * split)), dim3(128 * PARTS), 0, st,
+                     shape_of(a), reinterpret_cast<const Tile*>(a.k_tiles), (int)a.n_k_tiles,
+                     in<T>(a.q), a.q_token, a.q_head, in<T>(a.k), a.k_token, a.k_head, in<T>(a.v),
+                     a.v_token, a.v_head, in<T>(a.grad_out), a.grad_out_token, a.grad_out_head,
+                     stats, a.q_tokens, static_cast<T*>(a.grad_k), a.grad_k_token, a.grad_k_head,
+                     static_cast<T*>(a.grad_v), a.grad_v_token, a.grad_v_head, split, sums,
+                     a.k_tokens);
+  if (int rc = check_hip(hipGetLastError(), "attention_grad_kv_kernel launch")) return rc;
+  if (split == 1) return FSP_OK;
+  const int64_t quads = a.kv_heads * a.k_tokens * a.dim / 2;
+  hipLaunchKernelGGL((attention_grad_kv_sum_kernel<T>), dim3((unsigned)((quads + 255) / 256)),
+                     dim3(256), 0, st, shape_of(a), split, sums, a.k_tokens,
+                     static_cast<T*>(a.grad_k), a.grad_k_token, a.grad_k_head,
+                     static_cast<T*>(a.grad_v), a.grad_v_token, a.grad_v_head);
+  return check_hip(hipGetLastError(), "attention_grad_kv_sum_kernel launch");
 }
 
 template <typename T, int DP>
 int launch_backward(const fsp_attention_packed_args& a, hipStream_t st) {
-  float* stats = static_cast<float*>(a.workspace);
   if (a.n_q_tiles > 0) {
-    hipLaunchKernelGGL((attention_grad_q_kernel<T, DP>), dim3((unsigned)(a.n_q_tiles * a.heads)),
-                       dim3(256), 0, st, shape_of(a), reinterpret_cast<const Tile*>(a.q_tiles),
-                       (int)a.n_q_tiles, in<T>(a.q), a.q_token, a.q_head, in<T>(a.k), a.k_token,
-                       a.k_head, in<T>(a.v), a.v_token, a.v_head, in<T>(a.out), a.out_token,
-                       a.out_head, a.lse, in<T>(a.grad_out), a.grad_out_token, a.grad_out_head,
-                       static_cast<T*>(a.grad_q), a.grad_q_token, a.grad_q_head, stats,
-                       a.q_tokens);
-    if (int rc = check_hip(hipGetLastError(), "attention_grad_q_kernel launch")) return rc;
+    const int rc = share_queries(a) ? launch_grad_q<T, DP, 2>(a, st) : launch_grad_q<T, DP, 1>(a, st);
+    if (rc) return rc;
   }
   if (a.n_k_tiles > 0) {
-    hipLaunchKernelGGL((attention_grad_kv_kernel<T, DP>),
-                       dim3((unsigned)(a.n_k_tiles * a.kv_heads)), dim3(256), 0, st, shape_of(a),
-                       reinterpret_cast<const Tile*>(a.k_tiles), (int)a.n_k_tiles, in<T>(a.q),
-                       a.q_token, a.q_head, in<T>(a.k), a.k_token, a.k_head, in<T>(a.v),
-                       a.v_token, a.v_head, in<T>(a.grad_out), a.grad_out_token, a.grad_out_head,
-                       stats, a.q_tokens, static_cast<T*>(a.grad_k), a.grad_k_token,
-                       a.grad_k_head, static_cast<T*>(a.grad_v), a.grad_v_token, a.grad_v_head);
-    return check_hip(hipGetLastError(), "attention_grad_kv_kernel launch");
+    const int split = split_heads(a.n_k_tiles, a.heads, a.kv_heads);
+    return share_keys(a, split) ? launch_grad_kv<T, DP, 4>(a, split, st)
+                                : launch_grad_kv<T, DP, 2>(a, split, st);
   }
   return FSP_OK;
 }
@@ -630,7 +780,7 @@ int check_packed(const fsp_attention_packed_args& a, const std::string& who) {
   if (!attn_dim(a.dim)) return set_error(FSP_ENOTSUP, who + ": dim");
   if (a.kv_heads < 1 || a.heads < 1 || a.heads % a.kv_heads || a.heads > 0xffff)
     return set_error(FSP_EINVAL, who + ": heads must be a multiple of kv_heads");
-  if (a.q_tokens < 0 || a.k_tokens < 0 || a.n_q_tiles < 0 || a.n_k_tiles < 0 || a.window < 0 ||
+  if (a.q_tokens < 0 || a.k_tokens < 0 || a.n_q_tiles < 0 || a.n_k_tiles < 0 || a.window < 0 || a.q_longest < 0 || a.k_longest < 0 ||
       a.q_tokens > 0x7fffffffLL || a.k_tokens > 0x7fffffffLL || a.window > 0x7fffffffLL ||
       a.n_q_tiles > kMaxBlocks / a.heads || a.n_k_tiles > kMaxBlocks / a.heads)
     return set_error(FSP_EINVAL, who + ": size out of range");
@@ -655,6 +805,14 @@ int check_packed(const fsp_attention_packed_args& a, const std::string& who) {
 
 using namespace fsp;
 
+extern "C" int64_t fsp_attention_packed_workspace(int64_t n_k_tiles, int64_t heads, int64_t kv_heads,
+                                                  int64_t dim, int64_t q_tokens, int64_t k_tokens) {
+  if (n_k_tiles < 0 || heads < 1 || kv_heads < 1 || dim < 0 || q_tokens < 0 || k_tokens < 0) return 0;
+  const int split = split_heads(n_k_tiles, heads, kv_heads);
+  const int64_t stats = (2 * heads * q_tokens + 3) & ~int64_t(3);
+  return sizeof(float) * (stats + (split > 1 ? 2 * split * kv_heads * k_tokens * dim : 0));
+}
+
 extern "C" int64_t fsp_attention_packed_tile(int keys) { return keys ? kRows : kTile; }
 
 extern "C" int fsp_attention_packed(const fsp_attention_packed_args* args, void* stream) {
@@ -671,8 +829,10 @@ extern "C" int fsp_attention_packed_backward(const fsp_attention_packed_args* ar
   const fsp_attention_packed_args& a = *args;
   if (int rc = check_packed(a, "fsp_attention_packed_backward")) return rc;
   if ((a.n_q_tiles > 0 && (!a.grad_out || !a.grad_q || !a.workspace)) ||
-      (a.n_k_tiles > 0 && (!a.grad_k || !a.grad_v)))
+      (a.n_k_tiles > 0 && (!a.grad_k || !a.grad_v || !a.workspace)))
     return set_error(FSP_EINVAL, "fsp_attention_packed_backward: null pointer");
+  if (reinterpret_cast<uintptr_t>(a.workspace) % 16)
+    return set_error(FSP_EINVAL, "fsp_attention_packed_backward: workspace must be 16-byte aligned");
   if (!aligned16(a.grad_out, a.grad_out_token, a.grad_out_head) ||
       !aligned16(a.grad_q, a.grad_q_token, a.grad_q_head) ||
       !aligned16(a.grad_k, a.grad_k_token, a.grad_k_head) ||

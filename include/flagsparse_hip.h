@@ -771,10 +771,11 @@ int fsp_attention_paged(const struct fsp_attention_paged_args* args, void* strea
  * k count, 0}; q_tiles cover the queries, k_tiles (backward only) the keys.
  *
  * Backward: grad_out by its steps, out and lse of the forward pass; grad_q, grad_k, grad_v are
- * written whole.  workspace: float32 [2, heads, q_tokens].
+ * written whole.  workspace: fsp_attention_packed_workspace() bytes, 16-byte aligned.  q_longest,
+ * k_longest: the longest sequence (they decide how the work is shared out, not what is computed).
  */
 struct fsp_attention_packed_args {
-  int64_t dtype, heads, kv_heads, dim, q_tokens, k_tokens, causal, window;
+  int64_t dtype, heads, kv_heads, dim, q_tokens, k_tokens, q_longest, k_longest, causal, window;
   double scale;
   const int32_t* q_tiles;
   int64_t n_q_tiles;
@@ -795,6 +796,8 @@ struct fsp_attention_packed_args {
   void* workspace;
 };
 int64_t fsp_attention_packed_tile(int keys);
+int64_t fsp_attention_packed_workspace(int64_t n_k_tiles, int64_t heads, int64_t kv_heads, int64_t dim,
+                                       int64_t q_tokens, int64_t k_tokens);
 int fsp_attention_packed(const struct fsp_attention_packed_args* args, void* stream);
 int fsp_attention_packed_backward(const struct fsp_attention_packed_args* args, void* stream);
 

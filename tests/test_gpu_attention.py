@@ -79,6 +79,21 @@ def test_window(dev, window):
     _both(dev, [100, 200], [333, 150], 2, 1, 128, HF, True, window)
 
 
+def test_many_sharing_few(dev):
+    # few key tiles under many heads: shares of a group's heads are summed by another launch
+    _both(dev, [130], [130], 16, 1, 64, BF, True, None)
+    _both(dev, [70, 3], [200, 64], 24, 2, 128, HF, True, 50)
+    _both(dev, [90], [0], 8, 1, 64, BF, False, None)
+    _both(dev, [33, 0], [40, 10], 60, 4, 40, BF, True, None)
+
+
+def test_long_chains_with_many_heads(dev):
+    # more workgroups than the chip takes at once, and chains that are shared by more waves
+    _both(dev, [1300], [1300], 4, 2, 128, BF, True, None)
+    _both(dev, [1, 1500], [1100, 1200], 2, 1, 64, HF, True, 1050)
+    _both(dev, [40] * 70, [40] * 70, 16, 8, 96, HF, True, None)
+
+
 @pytest.mark.parametrize("scale", [0.0, 1.0, -0.3])
 def test_scale(dev, scale):
     _both(dev, [100, 20], [100, 20], 2, 1, 32, HF, True, None, scale=scale)
