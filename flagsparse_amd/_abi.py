@@ -125,7 +125,7 @@ SIGNATURES = {
     "fsp_attention_paged_workspace": (_i64, [_i64, _i64, _i64]),
     "fsp_attention_paged": (_i32, [_p, _p]),
     "fsp_attention_packed_tile": (_i64, [_i32]),
-    "fsp_attention_packed_workspace": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "fsp_attention_packed_workspace": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i32]),
     "fsp_attention_packed": (_i32, [_p, _p]),
     "fsp_attention_packed_backward": (_i32, [_p, _p]),
 }

@@ -695,7 +695,7 @@ def _backward(prepared, grad_out, q, k, v, out, lse, causal, window, scale, key=
     head = _pack(prepared, *rows[1:4], causal, window, scale, rows[4], (rows[0], *grads))
     kept = head, int(_abi.lib().fsp_attention_packed_workspace(
         prepared._tiles[True, causal].shape[0], q.shape[1], k.shape[1], q.shape[2], q.shape[0],
-        k.shape[0]))
+        k.shape[0], causal and not window))
     _run_backward(prepared, kept, rows, flat, grads)
     if key is not None and flat is lse and all(
             x is y for x, y in zip(rows, (grad_out, q, k, v, out))):

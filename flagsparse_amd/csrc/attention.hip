@@ -161,8 +161,7 @@ __device__ __forceinline__ void store_rows(T* to, const f32x16 (&x)[NT], float f
 }
 
 // A wave to 32 queries and, of every PARTS * 64 keys, 64: with PARTS = 2 two waves share the queries,
-// and their sums are joined at the end.  That halves the chain of steps where there are too few
-// workgroups to fill the chip (PARTS_FIGURES).
+// and their sums are joined at the end: half the chain of steps (share_queries).
 template <typename T, int DP, int PARTS>
 __global__ __launch_bounds__(256 * PARTS, 2) void attention_packed_kernel(
     Shape s, const Tile* __restrict__ tiles, int n_tiles, const T* __restrict__ q, int64_t q_token,
@@ -333,7 +332,7 @@ template <> struct Lift<f16> { static constexpr float up = 14, down = 1.0f / 163
 // Gradient of the queries: the forward pass's loop over keys with dP^T = V grad_out^T beside S^T; dS^T
 // is the operand of dQ^T = K^T dS^T where it lies.
 template <typename T, int DP, int PARTS>
-__global__ __launch_bounds__(256 * PARTS, 2) void attention_grad_q_kernel(
+__global__ __launch_bounds__(256 * PARTS, DP <= 64 ? 3 : 2) void attention_grad_q_kernel(
     Shape s, const Tile* __restrict__ tiles, int n_tiles, const T* __restrict__ q, int64_t q_token,
     int64_t q_head, const T* __restrict__ k, int64_t k_token, int64_t k_head,
     const T* __restrict__ v, int64_t v_token, int64_t v_head, const T* __restrict__ out,
@@ -669,31 +668,43 @@ Shape shape_of(const fsp_attention_packed_args& a) {
           (float)a.scale};
 }
 
-// Where the workgroups of one tile and head would not fill the chip (two to a CU, four up to a dim of
-// 64) and have long chains of steps, twice as many waves share a tile.
-// LAUNCH_FIGURES
-constexpr int64_t kCus = 256, kLong = 1024;
+// Twice as many waves share a tile where that fills CUs, or shortens the chains that the others end up
+// waiting for: those of a long causal sequence without a window, where the tiles are uneven and all
+// on the chip at once.  Measured without and with it, us, 16 heads over 4 (tiles times heads):
+// forward, dim 128: one sequence of 2048 (256) 41 / 33, of 4096 (512) 91 / 82, under a window of 1024
+// 45 / 49; dim 64, whose workgroups go four to a CU: 4096 (512) 53 / 46, two of 4096 (1024) 90 / 85.
+// Gradient of the queries, dim 128: 2048 56 / 48, 4096 under a window 63 / 70; 8192, 8 heads 232 / 203.
+// Gradients of the keys, dim 128: 3000, 4 heads over 4 (188) 48 / 35; two of 4096 (512) 378 / 286; two
+// of 2048 under a window (512) 77 / 96; three short ones (40) 9 / 12.
+constexpr int64_t kCus = 256;
 
 int64_t seen_at_most(const fsp_attention_packed_args& a, int64_t longest) {
   return a.window && a.window < longest ? a.window : longest;
 }
 
-bool share_queries(const fsp_attention_packed_args& a) {
-  return a.n_q_tiles * a.heads <= (a.dim <= 64 ? 4 : 2) * kCus && seen_at_most(a, a.k_longest) >= kLong;
+bool share_queries(const fsp_attention_packed_args& a, int64_t fill) {
+  const int64_t n = a.n_q_tiles * a.heads;
+  return seen_at_most(a, a.k_longest) >= 512 &&
+         (n <= fill || (n <= 2 * kCus && a.causal && !a.window && a.k_longest >= 2048));
 }
 
 bool share_keys(const fsp_attention_packed_args& a, int split) {
-  return a.n_k_tiles * a.kv_heads * split <= 2 * kCus &&
-         a.heads / a.kv_heads / split * seen_at_most(a, a.q_longest) >= kLong;
+  const int64_t n = a.n_k_tiles * a.kv_heads * split;
+  return (n <= kCus && a.heads / a.kv_heads / split * seen_at_most(a, a.q_longest) >= 1024) ||
+         (n <= 2 * kCus && a.causal && !a.window && a.q_longest >= 4096);
 }
 
 // Shares of a group's heads that go to workgroups of their own, for their sums to be added by another
-// launch: as many as two workgroups to a CU take.
-// SPLIT_FIGURES
-int split_heads(int64_t n_k_tiles, int64_t heads, int64_t kv_heads) {
+// launch: as many as three workgroups to a CU take, or five and a half where the tiles are uneven
+// (causal without a window) and smaller ones even them out.  Gradients of the keys with the limit at
+// 2, 3, 4 and 6, us: 12 ragged sequences up to 2500, 16 heads of 64 over 4: 135 / 80 / 79 / 56, under a
+// window of 1024 61 / 43 / 43 / 48; 4096 under that window, heads of 128: 85 / 83 / 95 / 95; 5000, 32 heads
+// of 128 over 8: 485 / 488 / 492 / 424; 4096, 24 heads over 8: 220 / 218 / 218 / 233.
+int split_heads(int64_t n_k_tiles, int64_t heads, int64_t kv_heads, bool uneven) {
   const int64_t group = heads / kv_heads, n = n_k_tiles * kv_heads;
+  const int64_t most = uneven ? 11 * kCus / 2 : 3 * kCus;
   int64_t split = 1;
-  for (int64_t i = 2; i <= group && i * n <= 2 * kCus; ++i)
+  for (int64_t i = 2; i <= group && i * n <= most; ++i)
     if (group % i == 0) split = i;
   return (int)split;
 }
@@ -710,7 +721,7 @@ int launch_forward(const fsp_attention_packed_args& a, hipStream_t st) {
 
 template <typename T, int DP>
 int launch_forward_parts(const fsp_attention_packed_args& a, hipStream_t st) {
-  return share_queries(a) ? launch_forward<T, DP, 2>(a, st) : launch_forward<T, DP, 1>(a, st);
+  return share_queries(a, DP <= 64 ? 4 * kCus : kCus) ? launch_forward<T, DP, 2>(a, st) : launch_forward<T, DP, 1>(a, st);
 }
 
 template <typename T>
@@ -757,11 +768,11 @@ int launch_grad_kv(const fsp_attention_packed_args& a, int split, hipStream_t st
 template <typename T, int DP>
 int launch_backward(const fsp_attention_packed_args& a, hipStream_t st) {
   if (a.n_q_tiles > 0) {
-    const int rc = share_queries(a) ? launch_grad_q<T, DP, 2>(a, st) : launch_grad_q<T, DP, 1>(a, st);
+    const int rc = share_queries(a, kCus) ? launch_grad_q<T, DP, 2>(a, st) : launch_grad_q<T, DP, 1>(a, st);
     if (rc) return rc;
   }
   if (a.n_k_tiles > 0) {
-    const int split = split_heads(a.n_k_tiles, a.heads, a.kv_heads);
+    const int split = split_heads(a.n_k_tiles, a.heads, a.kv_heads, a.causal && !a.window);
     return share_keys(a, split) ? launch_grad_kv<T, DP, 4>(a, split, st)
                                 : launch_grad_kv<T, DP, 2>(a, split, st);
   }
@@ -806,9 +817,10 @@ int check_packed(const fsp_attention_packed_args& a, const std::string& who) {
 using namespace fsp;
 
 extern "C" int64_t fsp_attention_packed_workspace(int64_t n_k_tiles, int64_t heads, int64_t kv_heads,
-                                                  int64_t dim, int64_t q_tokens, int64_t k_tokens) {
+                                                  int64_t dim, int64_t q_tokens, int64_t k_tokens,
+                                                  int uneven) {
   if (n_k_tiles < 0 || heads < 1 || kv_heads < 1 || dim < 0 || q_tokens < 0 || k_tokens < 0) return 0;
-  const int split = split_heads(n_k_tiles, heads, kv_heads);
+  const int split = split_heads(n_k_tiles, heads, kv_heads, uneven);
   const int64_t stats = (2 * heads * q_tokens + 3) & ~int64_t(3);
   return sizeof(float) * (stats + (split > 1 ? 2 * split * kv_heads * k_tokens * dim : 0));
 }

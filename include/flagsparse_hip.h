@@ -771,7 +771,8 @@ int fsp_attention_paged(const struct fsp_attention_paged_args* args, void* strea
  * k count, 0}; q_tiles cover the queries, k_tiles (backward only) the keys.
  *
  * Backward: grad_out by its steps, out and lse of the forward pass; grad_q, grad_k, grad_v are
- * written whole.  workspace: fsp_attention_packed_workspace() bytes, 16-byte aligned.  q_longest,
+ * written whole.  workspace: fsp_attention_packed_workspace() bytes (uneven: causal
+ * and no window), 16-byte aligned.  q_longest,
  * k_longest: the longest sequence (they decide how the work is shared out, not what is computed).
  */
 struct fsp_attention_packed_args {
@@ -797,7 +798,7 @@ struct fsp_attention_packed_args {
 };
 int64_t fsp_attention_packed_tile(int keys);
 int64_t fsp_attention_packed_workspace(int64_t n_k_tiles, int64_t heads, int64_t kv_heads, int64_t dim,
-                                       int64_t q_tokens, int64_t k_tokens);
+                                       int64_t q_tokens, int64_t k_tokens, int uneven);
 int fsp_attention_packed(const struct fsp_attention_packed_args* args, void* stream);
 int fsp_attention_packed_backward(const struct fsp_attention_packed_args* args, void* stream);
 
