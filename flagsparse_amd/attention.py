@@ -666,7 +666,11 @@ def flagsparse_attention_packed(q, k, v, indptr=None, k_indptr=None, *, prepared
     j <= i + nk - nq, the last query all of them; ``window``: only the last ``window`` of those.
     ``scale``: dim ** -0.5 by default.  Returns [tokens, heads, dim], with the float32 log-sum-exp
     [tokens, heads] if ``return_lse``.  The output is differentiable with respect to q, k and v where
-    they require a gradient (the log-sum-exp is not)."""
+    they require a gradient (the log-sum-exp is not).
+
+    What is not finite in k reaches the rows that see it.  In v it reaches those, and may reach rows of
+    the same sequence and block of 64 keys that do not (their weight is zero, and zero times it is
+    NaN), as it does in a product of the weights' matrix; it never reaches another sequence."""
     key = None
     wanted = torch.is_grad_enabled() and (_tracked(q) or _tracked(k) or _tracked(v))
     if out is None and not wanted and type(prepared) is PreparedAttention and \

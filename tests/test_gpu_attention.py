@@ -233,6 +233,19 @@ def test_sequences_do_not_touch_each_other(dev):
         assert torch.equal(a[keep], b[keep])
 
 
+def test_keys_that_are_not_finite_reach_the_rows_that_see_them(dev):
+    # a masked score is chosen away, whatever it is
+    n, h = 150, 2
+    q, k, v, _ = _inputs(dev, [n], [n], h, h, 64, BF)
+    ip = _indptr([n], dev)
+    clean = fs.flagsparse_attention_packed(q, k, v, ip)
+    k[100, 0, 3] = float("nan")
+    k[120, 1] = float("inf")
+    out = fs.flagsparse_attention_packed(q, k, v, ip)
+    assert torch.equal(out[:100, 0], clean[:100, 0]) and torch.equal(out[:120, 1], clean[:120, 1])
+    assert torch.isnan(out[100:, 0]).all() and torch.isnan(out[120:, 1]).all()
+
+
 def test_equal_calls_give_equal_bits(dev):
     lengths = [400, 1, 233]
     q, k, v, g = _inputs(dev, lengths, lengths, 8, 2, 128, BF)
