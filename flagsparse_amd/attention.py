@@ -47,6 +47,15 @@ _KEPT_LAYOUTS = 64
 _PLAIN = (type(None), bool, int, float)  # the settings a layout is kept with, by their values
 
 
+_CONTIGUOUS = torch.contiguous_format
+
+
+def _like(shape, dtype, device):
+    """A pattern for new arrays: ``torch.empty_like(pattern, memory_format=_CONTIGUOUS)`` takes a third of
+    the time of torch.empty with a shape, a type and a device.  One element of memory."""
+    return torch.empty(1, dtype=dtype, device=device).expand(shape)
+
+
 def _keep(calls, key, value):
     if len(calls) >= _KEPT_LAYOUTS:
         calls.clear()
@@ -185,7 +194,7 @@ class PreparedPagedKV:
 
     __slots__ = ("k_pages", "v_pages", "dtype", "device", "indptr", "indices", "batch", "n_pages", "page_size",
                  "kv_heads", "dim", "room", "_piece", "_pieces", "_first", "_most", "_streams",
-                 "_calls", "_counts", "_parts")
+                 "_calls", "_counts")
 
     def __init__(self, k_pages, v_pages, indptr, indices, pages):
         self.k_pages = k_pages
@@ -203,8 +212,7 @@ class PreparedPagedKV:
         table, first, self._most = _pieces(pages, self.page_size, self._piece)
         both = torch.from_numpy(np.concatenate([table.ravel(), first])).to(k_pages.device)
         self._pieces, self._first = both[:table.size].view(-1, 8), both[table.size:]
-        self._parts = {}  # counts of arrivals that a call needs, by its heads
-        self._counts = _abi.Calls()  # those counts, by stream and heads
+        self._counts = _abi.Calls()  # the pieces' counts of arrivals, by stream and number
         self._streams = _Streams()
         self._calls = _abi.Calls()
 
@@ -345,8 +353,9 @@ def flagsparse_paged_append(k, v, lengths, token_indptr=None, *, prepared=None, 
         kept = prepared._calls.get(key)
         if kept is not None and not (k.data_ptr() | v.data_ptr()) % 16 and (
                 q is None or q.data_ptr() % 16 == 0):
-            res = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            _append(prepared, kept, k, v, q, res, cos, sin, token_indptr, lengths)
+            head, like = kept
+            res = None if q is None else torch.empty_like(like, memory_format=_CONTIGUOUS)
+            _append(prepared, head, k, v, q, res, cos, sin, token_indptr, lengths)
             return res
     kv, n = _paged_of(prepared, k_pages, v_pages, indptr, indices, lengths)
     dev, dt = kv.device, kv.dtype
@@ -397,7 +406,7 @@ def flagsparse_paged_append(k, v, lengths, token_indptr=None, *, prepared=None, 
         _append(kv, head, k, v, q, res, cos, sin, token_indptr, n)
         if key is not None and all(x is y for x, y in zip(
                 (k, v, q, cos, sin, n, token_indptr), given)):
-            _keep(kv._calls, key, head)
+            _keep(kv._calls, key, (head, None if q is None else _like(q.shape, dt, dev)))
     if copied:
         out.copy_(res)
         res = out
@@ -432,7 +441,7 @@ def flagsparse_attention_paged(q, lengths, *, prepared=None, k_pages=None, v_pag
         key = _layouts(q, lengths) + (scale, window)
         kept = prepared._calls.get(key)
         if kept is not None and q.data_ptr() % 16 == 0:
-            res = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            res = torch.empty_like(kept[1], memory_format=_CONTIGUOUS)
             lse = _attend(prepared, kept, q, res, lengths, return_lse)
             return (res, lse) if return_lse else res
     kv, n = _paged_of(prepared, k_pages, v_pages, indptr, indices, lengths)
@@ -446,36 +455,40 @@ def flagsparse_attention_paged(q, lengths, *, prepared=None, k_pages=None, v_pag
     factor, past = _scale_of(scale, kv.dim), _window_of(window)
     res, copied = _result(out, "out", q.shape, dt, dev)
     rows = _rows(q)
-    head = kv._packed() + _PAGED.pack(
-        kv._pieces.data_ptr(), kv._first.data_ptr(), kv._pieces.shape[0], kv._piece, heads, past,
-        factor, *rows.stride()[:2], *res.stride()[:2])
-    lse = _attend(kv, head, rows, res, n, return_lse)
+    # what such calls share: the arguments, patterns of their arrays, the counts of arrivals they need
+    pieces, need, room = kv._pieces.shape[0], 0, None
+    if pieces > kv.batch:
+        need = int(_abi.lib().fsp_attention_paged_counts(pieces, kv._most, kv.batch, heads,
+                                                         kv.kv_heads))
+        room = _like((pieces * heads * (kv.dim + 2),), torch.float32, dev)
+    kept = (kv._packed() + _PAGED.pack(
+        kv._pieces.data_ptr(), kv._first.data_ptr(), pieces, kv._piece, heads, past, factor,
+        *rows.stride()[:2], *res.stride()[:2]), _like(q.shape, dt, dev),
+        _like((kv.batch, heads), torch.float32, dev), room, need)
+    lse = _attend(kv, kept, rows, res, n, return_lse)
     if key is not None and rows is q and n is lengths:
-        _keep(kv._calls, key, head)
+        _keep(kv._calls, key, kept)
     if copied:
         out.copy_(res)
         res = out
     return (res, lse) if return_lse else res
 
 
-def _attend(kv, head, q, res, lengths, return_lse):
+def _attend(kv, kept, q, res, lengths, return_lse):
     """The launch; returns the log-sum-exp, if asked for."""
-    heads, dev = q.shape[1], q.device
-    lse = torch.empty((kv.batch, heads), dtype=torch.float32, device=dev) if return_lse else None
+    head, _, like_lse, room, need = kept
+    lse = torch.empty_like(like_lse, memory_format=_CONTIGUOUS) if return_lse else None
     if not kv.batch:
         return lse
-    stream, pieces, work, counts = kv._on(), kv._pieces.shape[0], None, None
-    if pieces > kv.batch:
-        work = torch.empty(pieces * heads * (kv.dim + 2), dtype=torch.float32, device=dev)
-        need = kv._parts.get(heads)
-        if need is None:
-            need = kv._parts[heads] = int(_abi.lib().fsp_attention_paged_counts(
-                pieces, kv._most, kv.batch, heads, kv.kv_heads))
-        counts = kv._counts.get((stream, heads))
-        if need and counts is None:
-            counts = torch.zeros(need, dtype=torch.int32, device=dev)
-            if not torch.cuda.is_current_stream_capturing():  # else they are the graph's
-                kv._counts[stream, heads] = counts
+    stream, work, counts = kv._on(), None, None
+    if room is not None:
+        work = torch.empty_like(room, memory_format=_CONTIGUOUS)
+        if need:
+            counts = kv._counts.get((stream, need))
+            if counts is None:
+                counts = torch.zeros(need, dtype=torch.int32, device=kv.device)
+                if not torch.cuda.is_current_stream_capturing():  # else they are the graph's
+                    kv._counts[stream, need] = counts
     status = _abi.lib().fsp_attention_paged(head + _PAGED_AT.pack(
         q.data_ptr(), res.data_ptr(), _at(lse), lengths.data_ptr(), _at(work), _at(counts)), stream)
     if status:
@@ -614,24 +627,24 @@ def _tracked(t):
     return isinstance(t, torch.Tensor) and t.requires_grad
 
 
-def _run_forward(prepared, head, q, k, v, res):
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+def _run_forward(prepared, head, q, k, v, res, lse):
     if q.shape[0]:
         status = _abi.lib().fsp_attention_packed(head + _PACKED_AT.pack(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), res.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, 0),
             prepared._on())
         if status:
             _abi.check(status, "fsp_attention_packed")
-    return lse
 
 
 def _forward(prepared, q, k, v, causal, window, scale, out=None, key=None):
     res, copied = _result(out, "out", q.shape, q.dtype, q.device)
     rows = _rows(q), _rows(k), _rows(v)
     head = _pack(prepared, *rows, causal, window, scale, res)
-    lse = _run_forward(prepared, head, *rows, res)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+    _run_forward(prepared, head, *rows, res, lse)
     if key is not None and rows[0] is q and rows[1] is k and rows[2] is v:
-        _keep(prepared._calls, key, head)
+        _keep(prepared._calls, key, (head, _like(q.shape, q.dtype, q.device),
+                                     _like(lse.shape, lse.dtype, lse.device)))
     if copied:
         out.copy_(res)
         res = out
@@ -678,8 +691,10 @@ def flagsparse_attention_packed(q, k, v, indptr=None, k_indptr=None, *, prepared
         key = _layouts(q, k, v) + (causal, window, scale)
         kept = prepared._calls.get(key)
         if kept is not None and not (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
-            res = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            lse = _run_forward(prepared, kept, q, k, v, res)
+            head, like, like_lse = kept
+            res = torch.empty_like(like, memory_format=_CONTIGUOUS)
+            lse = torch.empty_like(like_lse, memory_format=_CONTIGUOUS)
+            _run_forward(prepared, head, q, k, v, res, lse)
             return (res, lse) if return_lse else res
     prepared, causal, window = _packed_inputs(q, k, v, indptr, k_indptr, prepared, causal, window)
     scale = _scale_of(scale, q.shape[2])
@@ -697,9 +712,11 @@ def _backward(prepared, grad_out, q, k, v, out, lse, causal, window, scale, key=
     flat = lse.contiguous()
     grads = tuple(torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
     head = _pack(prepared, *rows[1:4], causal, window, scale, rows[4], (rows[0], *grads))
-    kept = head, int(_abi.lib().fsp_attention_packed_workspace(
+    room = int(_abi.lib().fsp_attention_packed_workspace(
         prepared._tiles[True, causal].shape[0], q.shape[1], k.shape[1], q.shape[2], q.shape[0],
         k.shape[0], causal and not window))
+    kept = (head, _like((room,), torch.uint8, q.device),
+            tuple(_like(t.shape, t.dtype, t.device) for t in grads))
     _run_backward(prepared, kept, rows, flat, grads)
     if key is not None and flat is lse and all(
             x is y for x, y in zip(rows, (grad_out, q, k, v, out))):
@@ -708,11 +725,11 @@ def _backward(prepared, grad_out, q, k, v, out, lse, causal, window, scale, key=
 
 
 def _run_backward(prepared, kept, rows, lse, grads):
-    """``kept``: the arguments up to the addresses, and the bytes of workspace."""
-    head, room = kept
+    """``kept``: the arguments up to the addresses, and a pattern of the workspace."""
+    head, room, _ = kept
     grad_out, q, k, v, out = rows
     if q.shape[0] or k.shape[0]:
-        work = torch.empty(room, dtype=torch.uint8, device=q.device)
+        work = torch.empty_like(room, memory_format=_CONTIGUOUS)
         status = _abi.lib().fsp_attention_packed_backward(head + _PACKED_AT.pack(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
             grad_out.data_ptr(), grads[0].data_ptr(), grads[1].data_ptr(), grads[2].data_ptr(),
@@ -732,10 +749,7 @@ def flagsparse_attention_packed_backward(grad_out, q, k, v, out, lse, indptr=Non
         kept = prepared._calls.get(key)
         if kept is not None and not (grad_out.data_ptr() | q.data_ptr() | k.data_ptr() |
                                      v.data_ptr() | out.data_ptr()) % 16:
-            dt, dev = q.dtype, q.device
-            grads = (torch.empty(q.shape, dtype=dt, device=dev),
-                     torch.empty(k.shape, dtype=dt, device=dev),
-                     torch.empty(v.shape, dtype=dt, device=dev))
+            grads = tuple([torch.empty_like(t, memory_format=_CONTIGUOUS) for t in kept[2]])
             _run_backward(prepared, kept, rows, lse, grads)
             return grads
     prepared, causal, window = _packed_inputs(q, k, v, indptr, k_indptr, prepared, causal, window)
