@@ -39,7 +39,7 @@ _STEP_CAP = 2**23
 _CACHE = struct.Struct("17q")
 _APPEND, _APPEND_AT = struct.Struct("13q"), struct.Struct("8q")
 _PAGED, _PAGED_AT = struct.Struct("6qd4q"), struct.Struct("6q")
-_PACKED, _PACKED_AT = struct.Struct("10qd20q"), struct.Struct("10q")
+_PACKED, _PACKED_AT = struct.Struct("10qd22q"), struct.Struct("10q")
 
 # A prepared object keeps the first part for each layout of arrays that it has checked, so that the
 # next call with such arrays is a look-up and a launch.
@@ -192,8 +192,8 @@ class PreparedPagedKV:
     is a copy: a table that changes (another batch, more pages) is prepared anew.  ``room`` is the
     most tokens that the pages of one sequence hold."""
 
-    __slots__ = ("k_pages", "v_pages", "dtype", "device", "indptr", "indices", "batch", "n_pages", "page_size",
-                 "kv_heads", "dim", "room", "_piece", "_pieces", "_first", "_most", "_streams",
+    __slots__ = ("k_pages", "v_pages", "dtype", "device", "indptr", "indices", "batch", "n_pages",
+                 "page_size", "kv_heads", "dim", "room", "_piece", "_pieces", "_first", "_most", "_streams",
                  "_calls", "_counts")
 
     def __init__(self, k_pages, v_pages, indptr, indices, pages):
@@ -512,14 +512,13 @@ class PreparedAttention:
         self.k_tokens = int(k_len.sum())
         self.device = device
         self._longest = tuple(int(n.max(initial=0)) for n in (q_len, k_len))
-        tile = [int(_abi.lib().fsp_attention_packed_tile(keys)) for keys in (0, 1)]
-        lists = [_tiles(q_len, k_len, tile[keys], causal, keys)
-                 for keys in (False, True) for causal in (False, True)]
+        # (queries, queries in half tiles, keys; causal) -> the list
+        names = [(which, causal) for which in range(3) for causal in (False, True)]
+        lists = [_tiles(q_len, k_len, int(_abi.lib().fsp_attention_packed_tile(which)), causal,
+                        which == 2) for which, causal in names]
         flat = torch.from_numpy(np.concatenate(lists)).to(device)
         ends = np.cumsum([0] + [len(t) for t in lists])
-        # (over keys, causal) -> the list
-        self._tiles = {(keys, causal): flat[ends[2 * keys + causal]:ends[2 * keys + causal + 1]]
-                       for keys in (False, True) for causal in (False, True)}
+        self._tiles = {name: flat[ends[i]:ends[i + 1]] for i, name in enumerate(names)}
         self._streams = _Streams()
         self._calls = _abi.Calls()
 
@@ -615,12 +614,13 @@ def _packed_inputs(q, k, v, indptr, k_indptr, prepared, causal, window):
 
 def _pack(prepared, q, k, v, causal, window, scale, out, grads=()):
     """A call's arguments up to the addresses; grads: grad_out, grad_q, grad_k, grad_v."""
-    q_tiles, k_tiles = prepared._tiles[False, causal], prepared._tiles[True, causal]
+    q_tiles, halves, k_tiles = (prepared._tiles[which, causal] for which in range(3))
     steps = [n for t in (q, k, v, out, *grads) for n in t.stride()[:2]]
     steps += [0] * (16 - len(steps))
     return _PACKED.pack(_CODES[q.dtype], q.shape[1], k.shape[1], q.shape[2], q.shape[0],
-                        k.shape[0], *prepared._longest, causal, window, scale, q_tiles.data_ptr(), q_tiles.shape[0],
-                        k_tiles.data_ptr(), k_tiles.shape[0] if grads else 0, *steps)
+                        k.shape[0], *prepared._longest, causal, window, scale,
+                        q_tiles.data_ptr(), q_tiles.shape[0], halves.data_ptr(), halves.shape[0], k_tiles.data_ptr(),
+                        k_tiles.shape[0] if grads else 0, *steps)
 
 
 def _tracked(t):
@@ -713,7 +713,7 @@ def _backward(prepared, grad_out, q, k, v, out, lse, causal, window, scale, key=
     grads = tuple(torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
     head = _pack(prepared, *rows[1:4], causal, window, scale, rows[4], (rows[0], *grads))
     room = int(_abi.lib().fsp_attention_packed_workspace(
-        prepared._tiles[True, causal].shape[0], q.shape[1], k.shape[1], q.shape[2], q.shape[0],
+        prepared._tiles[2, causal].shape[0], q.shape[1], k.shape[1], q.shape[2], q.shape[0],
         k.shape[0], causal and not window))
     kept = (head, _like((room,), torch.uint8, q.device),
             tuple(_like(t.shape, t.dtype, t.device) for t in grads))

@@ -82,24 +82,26 @@ struct Lay {
   }
 };
 
-// Rows [0, n) of a 16-bit array, ``bytes`` apart, straight to LDS: 1024 bytes a wave and load.  What lies
-// past the rows or the head's dim is read as zero: the buffer's bounds end there.
-template <int DP>
+// Rows [0, n) of a 16-bit array, ``bytes`` apart, straight to LDS: ROWS of them by WAVES waves, 1024
+// bytes a wave and load.  What lies past the rows or the head's dim is read as zero: the buffer's
+// bounds end there.
+template <int DP, int ROWS, int WAVES>
 __device__ __forceinline__ void load_rows(char* lds, const void* src, int n, uint32_t bytes, int dim,
                                           int wave, int lane) {
   typedef Lay<DP> L;
   const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<void*>(src), 0, (int)((uint32_t)(n - 1) * bytes + 2 * dim), 0x00027000);
-  constexpr int PER = L::BYTES / 1024 / 4;  // loads of a wave
-  constexpr int ROWS = 1024 / L::PITCH;     // rows of a load
-  const int chunk = (lane % L::CH) ^ L::swizzle(lane / L::CH);
-  const uint32_t first = (uint32_t)(wave * PER * ROWS + lane / L::CH) * bytes;
+  constexpr int PER = ROWS * L::PITCH / 1024 / WAVES;  // loads of a wave
+  constexpr int EACH = 1024 / L::PITCH;                // rows of a load
+  // swizzle(a ^ b) = swizzle(a) ^ swizzle(b): the wave's, the lane's and the load's rows share no bit
+  const int chunk = (lane % L::CH) ^ L::swizzle(lane / L::CH) ^ L::swizzle(wave * PER * EACH);
+  const uint32_t first = (uint32_t)(wave * PER * EACH + lane / L::CH) * bytes;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {  // swizzle(a ^ b) = swizzle(a) ^ swizzle(b)
-    const int at = 16 * (chunk ^ L::swizzle(i * ROWS));
+  for (int i = 0; i < PER; ++i) {
+    const int at = 16 * (chunk ^ L::swizzle(i * EACH));
     __builtin_amdgcn_raw_ptr_buffer_load_lds(
         rsrc, (__attribute__((address_space(3))) void*)(lds + (wave * PER + i) * 1024), 16,
-        (int)(at < 2 * dim ? first + i * ROWS * bytes + at : 0x80000000u), 0, 0, 0);
+        (int)(at < 2 * dim ? first + i * EACH * bytes + at : 0x80000000u), 0, 0, 0);
   }
 }
 
@@ -160,10 +162,11 @@ __device__ __forceinline__ void store_rows(T* to, const f32x16 (&x)[NT], float f
     }
 }
 
-// A wave to 32 queries and, of every PARTS * 64 keys, 64: with PARTS = 2 two waves share the queries,
-// and their sums are joined at the end: half the chain of steps (share_queries).
-template <typename T, int DP, int PARTS>
-__global__ __launch_bounds__(256 * PARTS, 2) void attention_packed_kernel(
+// A tile of BLOCKS * 32 queries.  A wave goes to 32 of them and, of every PARTS * 64 keys, to 64: with
+// PARTS = 2 two waves share the queries, and their sums are joined at the end: half the chain of
+// steps (share_queries, halve_tiles).
+template <typename T, int DP, int BLOCKS, int PARTS>
+__global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_packed_kernel(
     Shape s, const Tile* __restrict__ tiles, int n_tiles, const T* __restrict__ q, int64_t q_token,
     int64_t q_head, const T* __restrict__ k, int64_t k_token, int64_t k_head,
     const T* __restrict__ v, int64_t v_token, int64_t v_head, T* __restrict__ out,
@@ -178,7 +181,8 @@ __global__ __launch_bounds__(256 * PARTS, 2) void attention_packed_kernel(
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = a / (s.heads / s.kv_heads);
-  const int part = wave / 4, q0 = (wave % 4) * 32, mine = q0 + col;  // this lane's row of the tile
+  const int part = wave / BLOCKS, block = wave % BLOCKS, q0 = block * 32;
+  const int mine = q0 + col;  // this lane's row of the tile
   const bool active = q0 < t.rows;
 
   V8<T> qf[NS];
@@ -210,8 +214,10 @@ __global__ __launch_bounds__(256 * PARTS, 2) void attention_packed_kernel(
   const T* vb = v + (int64_t)t.k_begin * v_token + g * v_head;
   auto load = [&](int j0, char* sk, char* sv) {
     const int n = min(ROWS, t.nk - j0);
-    load_rows<DP>(sk, kb + j0 * k_token, n, (uint32_t)(2 * k_token), s.dim, wave, lane);
-    load_rows<DP>(sv, vb + j0 * v_token, n, (uint32_t)(2 * v_token), s.dim, wave, lane);
+    load_rows<DP, ROWS, BLOCKS * PARTS>(sk, kb + j0 * k_token, n, (uint32_t)(2 * k_token), s.dim,
+                                        wave, lane);
+    load_rows<DP, ROWS, BLOCKS * PARTS>(sv, vb + j0 * v_token, n, (uint32_t)(2 * v_token), s.dim,
+                                        wave, lane);
   };
   const int k_at = L::row_at(lane);
   const int v_at = L::col_at(lane);
@@ -292,19 +298,22 @@ __global__ __launch_bounds__(256 * PARTS, 2) void attention_packed_kernel(
 
   sum += other_half(sum);
   if constexpr (PARTS > 1) {
-    float* theirs = reinterpret_cast<float*>(wave % 4 == 0 ? s_k0 : wave % 4 == 1 ? s_v0 : wave % 4 == 2 ? s_k1 : s_v1);
-    __shared__ f32x2 s_stat[4][64];
+    float* theirs = reinterpret_cast<float*>(block == 0   ? s_k0
+                                             : block == 1 ? s_v0
+                                             : block == 2 ? s_k1
+                                                          : s_v1);
+    __shared__ f32x2 s_stat[BLOCKS][64];
     static_assert(NT * 16 * 64 * 4 <= BYTES, "");
     if (part == 1) {
 #pragma unroll
       for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) theirs[(16 * i + r) * 64 + lane] = o[i][r];
-      s_stat[wave % 4][lane] = f32x2{top, sum};
+      s_stat[block][lane] = f32x2{top, sum};
     }
     __syncthreads();
     if (part == 1) return;
-    const f32x2 other = s_stat[wave][lane];
+    const f32x2 other = s_stat[block][lane];
     const float now = fmaxf(top, other.x), base = now == -INFINITY ? 0.0f : now;
     const float f0 = exp2f((top - base) * c), f1 = exp2f((other.x - base) * c);
     top = now;
@@ -337,8 +346,8 @@ constexpr int kFewKeys = 128;
 
 // Gradient of the queries: the forward pass's loop over keys with dP^T = V grad_out^T beside S^T; dS^T
 // is the operand of dQ^T = K^T dS^T where it lies.
-template <typename T, int DP, int PARTS>
-__global__ __launch_bounds__(256 * PARTS, DP <= 64 ? 3 : 2) void attention_grad_q_kernel(
+template <typename T, int DP, int BLOCKS, int PARTS>
+__global__ __launch_bounds__(64 * BLOCKS * PARTS, DP <= 64 ? 3 : 2) void attention_grad_q_kernel(
     Shape s, const Tile* __restrict__ tiles, int n_tiles, const T* __restrict__ q, int64_t q_token,
     int64_t q_head, const T* __restrict__ k, int64_t k_token, int64_t k_head,
     const T* __restrict__ v, int64_t v_token, int64_t v_head, const T* __restrict__ out,
@@ -355,7 +364,7 @@ __global__ __launch_bounds__(256 * PARTS, DP <= 64 ? 3 : 2) void attention_grad_
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = a / (s.heads / s.kv_heads);
-  const int part = wave / 4, q0 = (wave % 4) * 32, mine = q0 + col;
+  const int part = wave / BLOCKS, block = wave % BLOCKS, q0 = block * 32, mine = q0 + col;
   const bool active = q0 < t.rows;
   const int64_t row = t.first + (int64_t)min(mine, t.rows - 1);
 
@@ -392,8 +401,10 @@ __global__ __launch_bounds__(256 * PARTS, DP <= 64 ? 3 : 2) void attention_grad_
   const T* vb = v + (int64_t)t.k_begin * v_token + g * v_head;
   auto load = [&](int j0, char* sk, char* sv) {
     const int n = min(ROWS, t.nk - j0);
-    load_rows<DP>(sk, kb + j0 * k_token, n, (uint32_t)(2 * k_token), s.dim, wave, lane);
-    load_rows<DP>(sv, vb + j0 * v_token, n, (uint32_t)(2 * v_token), s.dim, wave, lane);
+    load_rows<DP, ROWS, BLOCKS * PARTS>(sk, kb + j0 * k_token, n, (uint32_t)(2 * k_token), s.dim,
+                                        wave, lane);
+    load_rows<DP, ROWS, BLOCKS * PARTS>(sv, vb + j0 * v_token, n, (uint32_t)(2 * v_token), s.dim,
+                                        wave, lane);
   };
   const int r_at = L::row_at(lane);
   const int c_at = L::col_at(lane);
@@ -490,7 +501,10 @@ __global__ __launch_bounds__(256 * PARTS, DP <= 64 ? 3 : 2) void attention_grad_
     }
   });
   if constexpr (PARTS > 1) {
-    float* theirs = reinterpret_cast<float*>(wave % 4 == 0 ? s_k0 : wave % 4 == 1 ? s_v0 : wave % 4 == 2 ? s_k1 : s_v1);
+    float* theirs = reinterpret_cast<float*>(block == 0   ? s_k0
+                                             : block == 1 ? s_v0
+                                             : block == 2 ? s_k1
+                                                          : s_v1);
     if (part == 1)
 #pragma unroll
       for (int i = 0; i < NT; ++i)
@@ -569,8 +583,10 @@ __global__ __launch_bounds__(128 * PARTS, 2) void attention_grad_kv_kernel(
     // the rows' offsets are made anew in every step: kept, they would not fit the registers
     int l = lane;
     asm volatile("" : "+v"(l));
-    load_rows<DP>(sq, q + first * q_token + a * q_head, n, (uint32_t)(2 * q_token), s.dim, wave, l);
-    load_rows<DP>(sg, go + first * go_token + a * go_head, n, (uint32_t)(2 * go_token), s.dim, wave, l);
+    load_rows<DP, ROWS, 2 * PARTS>(sq, q + first * q_token + a * q_head, n,
+                                   (uint32_t)(2 * q_token), s.dim, wave, l);
+    load_rows<DP, ROWS, 2 * PARTS>(sg, go + first * go_token + a * go_head, n,
+                                   (uint32_t)(2 * go_token), s.dim, wave, l);
     if (wave < PARTS) {  // 64 rows' statistics a wave
       const int which = wave & 1, at = (wave >> 1) * 64;
       const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
@@ -630,7 +646,8 @@ __global__ __launch_bounds__(128 * PARTS, 2) void attention_grad_kv_kernel(
   // the steps of every head of the group, one after the other
   const int steps = hit > lot ? (hit - lot + ROWS - 1) / ROWS : 0;
   const int total = steps * group;
-  int a = (g * split + share) * group, i0 = lot, a1 = a, i1 = lot;  // of this step, and of the one being loaded
+  int a = (g * split + share) * group, i0 = lot;  // of this step
+  int a1 = a, i1 = lot;                           // of the one being loaded
   auto next = [&] {
     i1 += ROWS;
     if (i1 >= hit) i1 = lot, ++a1;
@@ -732,6 +749,16 @@ bool share_queries(const fsp_attention_packed_args& a, int64_t fill) {
          (n <= fill || (n <= 2 * kCus && a.causal && !a.window && a.k_longest >= 2048));
 }
 
+// Tiles of half the queries, with two waves to 32 of them, where whole tiles would leave CUs without any
+// and there is more than one step of keys.  Measured without and with them, us (tiles times heads):
+// forward, dim 128: one sequence of 512, 16 heads (64) 14.4 / 12.6, of 2048, 4 heads (64) 31.9 / 30.1, of
+// 4000, 8 heads (256) 58 / 64; four of 64, 4 heads (16) 6.0 / 7.9; dim 64, whose workgroups go two
+// to a CU: 2048, 8 heads (128) 22.4 / 18.5, 4000 (256) 39.6 / 35.4.  Gradient of the queries, dim 128:
+// 512 (64) 20.4 / 15.9, 2048 (64) 44.8 / 38.6, 4000 (256) 82 / 86; dim 64: 2048 (128) 28.9 / 25.3.
+bool halve_tiles(const fsp_attention_packed_args& a, int64_t most) {
+  return a.n_q_tiles * a.heads <= most && seen_at_most(a, a.k_longest) > kRows;
+}
+
 bool share_keys(const fsp_attention_packed_args& a, int split) {
   const int64_t n = a.n_k_tiles * a.kv_heads * split;
   return (n <= kCus && a.heads / a.kv_heads / split * seen_at_most(a, a.q_longest) >= 1024) ||
@@ -753,11 +780,13 @@ int split_heads(int64_t n_k_tiles, int64_t heads, int64_t kv_heads, bool uneven)
   return (int)split;
 }
 
-template <typename T, int DP, int PARTS>
+template <typename T, int DP, int BLOCKS, int PARTS>
 int launch_forward(const fsp_attention_packed_args& a, hipStream_t st) {
-  hipLaunchKernelGGL((attention_packed_kernel<T, DP, PARTS>),
-                     dim3((unsigned)(a.n_q_tiles * a.heads)), dim3(256 * PARTS), 0, st, shape_of(a),
-                     reinterpret_cast<const Tile*>(a.q_tiles), (int)a.n_q_tiles, in<T>(a.q),
+  const int32_t* tiles = BLOCKS == 2 ? a.q_halves : a.q_tiles;
+  const int64_t n = BLOCKS == 2 ? a.n_q_halves : a.n_q_tiles;
+  hipLaunchKernelGGL((attention_packed_kernel<T, DP, BLOCKS, PARTS>),
+                     dim3((unsigned)(n * a.heads)), dim3(64 * BLOCKS * PARTS), 0, st, shape_of(a),
+                     reinterpret_cast<const Tile*>(tiles), (int)n, in<T>(a.q),
                      a.q_token, a.q_head, in<T>(a.k), a.k_token, a.k_head, in<T>(a.v), a.v_token,
                      a.v_head, static_cast<T*>(a.out), a.out_token, a.out_head, a.lse);
   return check_hip(hipGetLastError(), "attention_packed_kernel launch");
@@ -765,7 +794,9 @@ int launch_forward(const fsp_attention_packed_args& a, hipStream_t st) {
 
 template <typename T, int DP>
 int launch_forward_parts(const fsp_attention_packed_args& a, hipStream_t st) {
-  return share_queries(a, DP <= 64 ? 4 * kCus : kCus) ? launch_forward<T, DP, 2>(a, st) : launch_forward<T, DP, 1>(a, st);
+  if (halve_tiles(a, DP <= 64 ? kCus : kCus / 2)) return launch_forward<T, DP, 2, 2>(a, st);
+  return share_queries(a, DP <= 64 ? 4 * kCus : kCus) ? launch_forward<T, DP, 4, 2>(a, st)
+                                                      : launch_forward<T, DP, 4, 1>(a, st);
 }
 
 template <typename T>
@@ -775,11 +806,13 @@ int launch_forward_dim(const fsp_attention_packed_args& a, hipStream_t st) {
   return launch_forward_parts<T, 128>(a, st);
 }
 
-template <typename T, int DP, int PARTS>
+template <typename T, int DP, int BLOCKS, int PARTS>
 int launch_grad_q(const fsp_attention_packed_args& a, hipStream_t st) {
-  hipLaunchKernelGGL((attention_grad_q_kernel<T, DP, PARTS>),
-                     dim3((unsigned)(a.n_q_tiles * a.heads)), dim3(256 * PARTS), 0, st, shape_of(a),
-                     reinterpret_cast<const Tile*>(a.q_tiles), (int)a.n_q_tiles, in<T>(a.q),
+  const int32_t* tiles = BLOCKS == 2 ? a.q_halves : a.q_tiles;
+  const int64_t n = BLOCKS == 2 ? a.n_q_halves : a.n_q_tiles;
+  hipLaunchKernelGGL((attention_grad_q_kernel<T, DP, BLOCKS, PARTS>),
+                     dim3((unsigned)(n * a.heads)), dim3(64 * BLOCKS * PARTS), 0, st, shape_of(a),
+                     reinterpret_cast<const Tile*>(tiles), (int)n, in<T>(a.q),
                      a.q_token, a.q_head, in<T>(a.k), a.k_token, a.k_head, in<T>(a.v), a.v_token,
                      a.v_head, in<T>(a.out), a.out_token, a.out_head, a.lse, in<T>(a.grad_out),
                      a.grad_out_token, a.grad_out_head, static_cast<T*>(a.grad_q), a.grad_q_token,
@@ -812,7 +845,9 @@ int launch_grad_kv(const fsp_attention_packed_args& a, int split, hipStream_t st
 template <typename T, int DP>
 int launch_backward(const fsp_attention_packed_args& a, hipStream_t st) {
   if (a.n_q_tiles > 0) {
-    const int rc = share_queries(a, kCus) ? launch_grad_q<T, DP, 2>(a, st) : launch_grad_q<T, DP, 1>(a, st);
+    const int rc = halve_tiles(a, kCus / 2) ? launch_grad_q<T, DP, 2, 2>(a, st)
+                   : share_queries(a, kCus) ? launch_grad_q<T, DP, 4, 2>(a, st)
+                                            : launch_grad_q<T, DP, 4, 1>(a, st);
     if (rc) return rc;
   }
   if (a.n_k_tiles > 0) {
@@ -835,9 +870,11 @@ int check_packed(const fsp_attention_packed_args& a, const std::string& who) {
   if (!attn_dim(a.dim)) return set_error(FSP_ENOTSUP, who + ": dim");
   if (a.kv_heads < 1 || a.heads < 1 || a.heads % a.kv_heads || a.heads > 0xffff)
     return set_error(FSP_EINVAL, who + ": heads must be a multiple of kv_heads");
-  if (a.q_tokens < 0 || a.k_tokens < 0 || a.n_q_tiles < 0 || a.n_k_tiles < 0 || a.window < 0 || a.q_longest < 0 || a.k_longest < 0 ||
+  if (a.q_tokens < 0 || a.k_tokens < 0 || a.n_q_tiles < 0 || a.n_k_tiles < 0 ||
+      a.n_q_halves < 0 || a.window < 0 || a.q_longest < 0 || a.k_longest < 0 ||
       a.q_tokens > 0x7fffffffLL || a.k_tokens > 0x7fffffffLL || a.window > 0x7fffffffLL ||
-      a.n_q_tiles > kMaxBlocks / a.heads || a.n_k_tiles > kMaxBlocks / a.heads)
+      a.n_q_tiles > kMaxBlocks / a.heads || a.n_q_halves > kMaxBlocks / a.heads ||
+      a.n_k_tiles > kMaxBlocks / a.heads)
     return set_error(FSP_EINVAL, who + ": size out of range");
   auto step = [&](int64_t tokens, int64_t by) {
     return (tokens < 2 || by >= a.dim) && by >= 0 && by <= kTokenStep;
@@ -846,7 +883,7 @@ int check_packed(const fsp_attention_packed_args& a, const std::string& who) {
       !step(a.k_tokens, a.v_token) || (a.n_k_tiles > 0 && !step(a.q_tokens, a.grad_out_token)))
     return set_error(FSP_EINVAL, who + ": a token's step must lie between dim and 2^23");
   if (a.window && !a.causal) return set_error(FSP_EINVAL, who + ": window needs causal");
-  if ((a.n_q_tiles > 0 && (!a.q_tiles || !a.q || !a.out || !a.lse)) ||
+  if ((a.n_q_tiles > 0 && (!a.q_tiles || !a.q_halves || !a.q || !a.out || !a.lse)) ||
       (a.n_k_tiles > 0 && !a.k_tiles) || (a.k_tokens > 0 && (!a.k || !a.v)))
     return set_error(FSP_EINVAL, who + ": null pointer");
   if (!aligned16(a.q, a.q_token, a.q_head) || !aligned16(a.k, a.k_token, a.k_head) ||
@@ -869,7 +906,9 @@ extern "C" int64_t fsp_attention_packed_workspace(int64_t n_k_tiles, int64_t hea
   return sizeof(float) * (stats + (split > 1 ? 2 * split * kv_heads * k_tokens * dim : 0));
 }
 
-extern "C" int64_t fsp_attention_packed_tile(int keys) { return keys ? kRows : kTile; }
+extern "C" int64_t fsp_attention_packed_tile(int which) {
+  return which == 0 ? kTile : which == 1 ? kTile / 2 : kRows;
+}
 
 extern "C" int fsp_attention_packed(const fsp_attention_packed_args* args, void* stream) {
   if (!args) return set_error(FSP_EINVAL, "fsp_attention_packed: null arguments");

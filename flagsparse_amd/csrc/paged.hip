@@ -164,8 +164,8 @@ __device__ __forceinline__ void all_stored() {
 // Values go from memory to the matrix instructions' registers with no stop in LDS, keys with a short
 // one: with a lane to a key a load would fetch 64 bytes of each of 16 rows, and whole rows are the
 // faster to fetch (a bare loop of such loads over 3.2 GB: 64 bytes 540 us, rows 490), so that a wave
-// writes the rows to LDS of its own and reads its lanes' keys there.  With S^T = K Q^T lane l has head l % 16 and, of 32 keys, the eight 4 * (l / 16) + {0..3, 16..19}: its
-// weights are the operand of O^T = V^T P^T as they lie, since the order of the summed keys is free.
+// writes the rows to LDS of its own and reads its lanes' keys there.  With S^T = K Q^T lane l has head
+// l % 16 and, of 32 keys, the eight 4 * (l / 16) + {0..3, 16..19}: its weights are the operand of O^T = V^T P^T as they lie, since the order of the summed keys is free.
 // For V a lane loads DP / 16 consecutive elements of those same eight keys, and the operand of one
 // product is one element of each: pairs of 16-bit halves, a byte permutation each.  Row m of product
 // i is element DP / 16 * m + i of the head, so a lane's results are consecutive.

@@ -766,9 +766,10 @@ int fsp_attention_paged(const struct fsp_attention_paged_args* args, void* strea
  * i of nq sees key j of nk if j <= i + nk - nq; a window > 0 (causal only) hides the keys
  * j <= i + nk - nq - window.  lse [q_tokens, heads] float32.
  *
- * Work lists (fsp_attention_packed_tile(keys) rows to a tile, any order): a tile is 8 int32,
- * {first row, rows, first row's place in its sequence, sequence's q begin, q count, k begin,
- * k count, 0}; q_tiles cover the queries, k_tiles (backward only) the keys.
+ * Work lists, in any order: a tile is 8 int32, {first row, rows, first row's place in its sequence,
+ * sequence's q begin, q count, k begin, k count, 0}; q_tiles cover the queries in
+ * fsp_attention_packed_tile(0) rows, q_halves in fsp_attention_packed_tile(1) rows, k_tiles
+ * (backward only) the keys in fsp_attention_packed_tile(2) rows.
  *
  * Backward: grad_out by its steps, out and lse of the forward pass; grad_q, grad_k, grad_v are
  * written whole.  workspace: fsp_attention_packed_workspace() bytes (uneven: causal
@@ -780,6 +781,8 @@ struct fsp_attention_packed_args {
   double scale;
   const int32_t* q_tiles;
   int64_t n_q_tiles;
+  const int32_t* q_halves;
+  int64_t n_q_halves;
   const int32_t* k_tiles;
   int64_t n_k_tiles;
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;
@@ -796,7 +799,7 @@ struct fsp_attention_packed_args {
   void* grad_v;
   void* workspace;
 };
-int64_t fsp_attention_packed_tile(int keys);
+int64_t fsp_attention_packed_tile(int which);
 int64_t fsp_attention_packed_workspace(int64_t n_k_tiles, int64_t heads, int64_t kv_heads, int64_t dim,
                                        int64_t q_tokens, int64_t k_tokens, int uneven);
 int fsp_attention_packed(const struct fsp_attention_packed_args* args, void* stream);

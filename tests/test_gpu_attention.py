@@ -94,6 +94,15 @@ def test_long_chains_with_many_heads(dev):
     _both(dev, [40] * 70, [40] * 70, 16, 8, 96, HF, True, None)
 
 
+@pytest.mark.parametrize("dim", [64, 96, 128])
+@pytest.mark.parametrize("lengths,heads", [([64], 4), ([65], 4), ([64] * 5, 60), ([65] * 3, 60),
+                                           ([600], 40), ([520, 3], 54)])
+def test_shares_of_a_tile(dev, lengths, heads, dim):
+    # few and many workgroups, chains of one step of keys and of several
+    _both(dev, lengths, lengths, heads, 2, dim, BF, True, None)
+    _both(dev, lengths, lengths, heads, 2, dim, HF, False, None)
+
+
 @pytest.mark.parametrize("scale", [0.0, 1.0, -0.3])
 def test_scale(dev, scale):
     _both(dev, [100, 20], [100, 20], 2, 1, 32, HF, True, None, scale=scale)
