@@ -210,6 +210,10 @@ class PreparedPagedKV:
         # the pieces that attention is cut into
         self._piece = int(_abi.lib().fsp_attention_paged_piece(int(rooms.sum()), self.kv_heads))
         table, first, self._most = _pieces(pages, self.page_size, self._piece)
+        # long pieces first, for short ones to even out the end: 96 ragged sequences of up to 4096 tokens,
+        # 8 heads of 128: 51 us, 55 in the sequences' order
+        held = np.minimum(self._piece, table[:, 4] - table[:, 1])
+        table = table[np.argsort(-held, kind="stable")]
         both = torch.from_numpy(np.concatenate([table.ravel(), first])).to(k_pages.device)
         self._pieces, self._first = both[:table.size].view(-1, 8), both[table.size:]
         self._counts = _abi.Calls()  # the pieces' counts of arrivals, by stream and number

@@ -175,8 +175,8 @@ constexpr int kHeadTile = 16;
 constexpr int kPieceMost = 1024;
 // The workgroup that finishes a sequence joins its pieces where they are at most so many and all
 // workgroups are on the chip at once (three to a CU): the wait for their stores then holds up nobody.
-// Else a second launch does.  1000 tokens, 16 heads of 64: 10.7 us a call joined so, 13.2 by a second
-// launch, both bound by the host (9.2 and 8.5 us in a graph); 6 sequences of 131072 tokens, pieces
+// Else a second launch does.  1000 tokens, 16 heads of 64: 8.7 us a call joined so, 11.9 by a second
+// launch, both bound by the host (9.2 and 8.4 us in a graph); 6 sequences of 131072 tokens, pieces
 // of 1024: 645 and 583 us.
 constexpr int kJoinMost = 8;
 constexpr int kResident = 3 * 256;
@@ -452,56 +452,80 @@ __global__ __launch_bounds__(256, 3) void attention_paged_kernel(
   }
 }
 
-// Joins the pieces of sequences that have several, in their order: a workgroup a sequence and head, a
-// quarter of the pieces a wave, the pieces' weights first.
+// Joins the pieces of sequences that have several: a workgroup a sequence and head, half a wave to every
+// eighth piece, eight of each at a time with their weights, so that up to 64 pieces wait for memory
+// once.
 template <typename T>
 __global__ __launch_bounds__(256) void attention_paged_join_kernel(
     Cache c, PagedShape s, const int32_t* __restrict__ first_piece, T* __restrict__ out,
     int64_t out_token, int64_t out_head, float* __restrict__ lse,
     const int32_t* __restrict__ lengths, const float* __restrict__ part_o,
     const f32x2* __restrict__ part_ml) {
-  __shared__ f32x2 s_o[4][64];
-  __shared__ float s_total[4];
+  constexpr int W = 8, U = 8;
+  __shared__ f32x4 s_o[W][32];
+  __shared__ f32x2 s_ml[W];
   const int b = blockIdx.x / s.heads, h = blockIdx.x % s.heads;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int d = 4 * (threadIdx.x & 31), mine = threadIdx.x >> 5;
   const int length = lengths[b], room = (c.indptr[b + 1] - c.indptr[b]) * c.page_size;
+  const int slot = first_piece[b];
   const int last = length >= 0 && length <= room ? length : 0;
   const int first = s.window && last > s.window ? last - s.window : 0;
   const int p0 = first / s.piece, p1 = max(p0 + 1, (last + s.piece - 1) / s.piece), n = p1 - p0;
   if (n < 2) return;
-  const int64_t at = (int64_t)(first_piece[b] + p0) * s.heads + h;
+  const int64_t at = (int64_t)(slot + p0) * s.heads + h;
   const f32x2* ml = part_ml + at;
-  const float* o = part_o + at * c.dim + (2 * lane < c.dim ? 2 * lane : 0);
-  float most = -INFINITY;
-  for (int p = lane; p < n; p += 64) most = fmaxf(most, ml[(int64_t)p * s.heads].x);
-  most = wave_max(most);
+  const float* o = part_o + at * c.dim + (d < c.dim ? d : 0);
+  float most = -INFINITY, total = 0;
+  f32x4 y{};
+  for (int p = mine; p < n; p += W * U) {
+    f32x2 v[U];
+    f32x4 u[U];
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      const int64_t i = (int64_t)min(p + W * e, n - 1) * s.heads;
+      v[e] = ml[i];
+      u[e] = *reinterpret_cast<const f32x4*>(o + i * c.dim);
+    }
+    float now = most;
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      v[e] = p + W * e < n ? v[e] : f32x2{-INFINITY, 0};
+      now = fmaxf(now, v[e].x);
+    }
+    const float base = now == -INFINITY ? 0.0f : now;
+    const float fade = exp2f(most - base);
+    most = now;
+    total *= fade;
+    y *= fade;
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      const float f = exp2f(v[e].x - base);
+      total += f * v[e].y;
+      y += f * u[e];
+    }
+  }
+  s_o[mine][threadIdx.x & 31] = y;
+  if (d == 0) s_ml[mine] = f32x2{most, total};
+  __syncthreads();
+  if (threadIdx.x >= 32) return;
+  most = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < W; ++w) most = fmaxf(most, s_ml[w].x);
   const float base = most == -INFINITY ? 0.0f : most;
-  const int per = (n + 3) / 4, begin = wave * per, end = min(n, begin + per);
-  float total = 0;
-  f32x2 y{};
-  for (int p = begin; p < end; p += 64) {  // 64 pieces' weights, a lane each
-    const f32x2 v = p + lane < end ? ml[(int64_t)(p + lane) * s.heads] : f32x2{-INFINITY, 0};
+  total = 0;
+  y = f32x4{};
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    const f32x2 v = s_ml[w];
     const float f = exp2f(v.x - base);
     total += f * v.y;
-    const int m = min(64, end - p);
-#pragma unroll 8
-    for (int e = 0; e < m; ++e)
-      y += __shfl(f, e) * *reinterpret_cast<const f32x2*>(o + (int64_t)(p + e) * s.heads * c.dim);
+    y += f * s_o[w][threadIdx.x];
   }
-  total = wave_add(total);
-  if (lane == 0) s_total[wave] = total;
-  s_o[wave][lane] = y;
-  __syncthreads();
-  if (wave) return;
-  total = s_total[0] + s_total[1] + s_total[2] + s_total[3];
-  y = s_o[0][lane] + s_o[1][lane] + s_o[2][lane] + s_o[3][lane];
-  const float f = total == 0 ? 0.0f : 1.0f / total;
-  if (2 * lane < c.dim) {
-    T* to = out + b * out_token + h * out_head + 2 * lane;
-    to[0] = (T)(y.x * f);
-    to[1] = (T)(y.y * f);
-  }
-  if (lse && lane == 0)
+  y *= total == 0 ? 0.0f : 1.0f / total;
+  if (d < c.dim)
+    *reinterpret_cast<V4<T>*>(out + b * out_token + h * out_head + d) =
+        __builtin_convertvector(y, V4<T>);
+  if (lse && d == 0)
     lse[(int64_t)b * s.heads + h] = total == 0 ? -INFINITY : (most + log2f(total)) * kLn2;
 }
 

@@ -733,7 +733,8 @@ int fsp_paged_append(const struct fsp_paged_append_args* args, void* stream);
  * The work is cut into pieces of `piece` tokens (fsp_attention_paged_piece() for a cache whose table
  * has room for `tokens` of them): pieces [n_pieces, 8] holds {sequence, first token, the sequence's
  * first piece, page_indptr[sequence], its pages' room in tokens, 0, 0, 0} for each piece of each
- * sequence's room, in order, one at least for each; first_piece [batch] the sequences' first ones.
+ * sequence's room, one at least for each, in the order in which they are to start; a piece's number
+ * is its sequence's first one plus first token / piece; first_piece [batch] the sequences' first.
  * Unless every sequence has one piece: workspace, fsp_attention_paged_workspace() bytes, 16-byte
  * aligned, and either arrived, 32-bit counts that are zero, as the call leaves them (calls that may
  * overlap have counts of their own), or NULL, which takes a second launch;
