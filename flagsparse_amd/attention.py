@@ -39,7 +39,7 @@ _STEP_CAP = 2**23
 _CACHE = struct.Struct("17q")
 _APPEND, _APPEND_AT = struct.Struct("13q"), struct.Struct("8q")
 _PAGED, _PAGED_AT = struct.Struct("6qd4q"), struct.Struct("6q")
-_PACKED, _PACKED_AT = struct.Struct("10qd22q"), struct.Struct("10q")
+_PACKED, _PACKED_AT = struct.Struct("10qd24q"), struct.Struct("10q")
 
 # A prepared object keeps the first part for each layout of arrays that it has checked, so that the
 # next call with such arrays is a look-up and a launch.
@@ -516,10 +516,10 @@ class PreparedAttention:
         self.k_tokens = int(k_len.sum())
         self.device = device
         self._longest = tuple(int(n.max(initial=0)) for n in (q_len, k_len))
-        # (queries, queries in half tiles, keys; causal) -> the list
-        names = [(which, causal) for which in range(3) for causal in (False, True)]
+        # (queries, queries in half tiles, keys, keys in half tiles; causal) -> the list
+        names = [(which, causal) for which in range(4) for causal in (False, True)]
         lists = [_tiles(q_len, k_len, int(_abi.lib().fsp_attention_packed_tile(which)), causal,
-                        which == 2) for which, causal in names]
+                        which >= 2) for which, causal in names]
         flat = torch.from_numpy(np.concatenate(lists)).to(device)
         ends = np.cumsum([0] + [len(t) for t in lists])
         self._tiles = {name: flat[ends[i]:ends[i + 1]] for i, name in enumerate(names)}
@@ -618,13 +618,13 @@ def _packed_inputs(q, k, v, indptr, k_indptr, prepared, causal, window):
 
 def _pack(prepared, q, k, v, causal, window, scale, out, grads=()):
     """A call's arguments up to the addresses; grads: grad_out, grad_q, grad_k, grad_v."""
-    q_tiles, halves, k_tiles = (prepared._tiles[which, causal] for which in range(3))
+    lists = [prepared._tiles[which, causal] for which in range(4)]
     steps = [n for t in (q, k, v, out, *grads) for n in t.stride()[:2]]
     steps += [0] * (16 - len(steps))
     return _PACKED.pack(_CODES[q.dtype], q.shape[1], k.shape[1], q.shape[2], q.shape[0],
                         k.shape[0], *prepared._longest, causal, window, scale,
-                        q_tiles.data_ptr(), q_tiles.shape[0], halves.data_ptr(), halves.shape[0], k_tiles.data_ptr(),
-                        k_tiles.shape[0] if grads else 0, *steps)
+                        *(n for i, t in enumerate(lists)
+                          for n in (t.data_ptr(), t.shape[0] if i < 2 or grads else 0)), *steps)
 
 
 def _tracked(t):

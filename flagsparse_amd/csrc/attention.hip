@@ -521,13 +521,13 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, DP <= 64 ? 3 : 2) void attenti
     store_rows<T, NT>(dq + row * dq_token + a * dq_head, acc, s.scale, s.dim, half);
 }
 
-// Gradients of the keys and values, 64 keys a workgroup, over the heads of the group and their
+// Gradients of the keys and values, BLOCKS * 32 keys a workgroup, over the heads of the group and their
 // queries.  S and dP are [queries, keys], so P and dS are the operands of dV^T = grad_out^T P and
 // dK^T = Q^T dS where they lie.  The products start from a row's -lse / scale and -delta, so that they
 // give S - lse and dP - delta.  PARTS waves share 32 keys, one to every PARTS-th 32 queries;
 // their sums are joined through LDS at the end, in their order.
-template <typename T, int DP, int PARTS>
-__global__ __launch_bounds__(128 * PARTS, 2) void attention_grad_kv_kernel(
+template <typename T, int DP, int BLOCKS, int PARTS>
+__global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_grad_kv_kernel(
     Shape s, const Tile* __restrict__ tiles, int n_tiles, const T* __restrict__ q, int64_t q_token,
     int64_t q_head, const T* __restrict__ k, int64_t k_token, int64_t k_head,
     const T* __restrict__ v, int64_t v_token, int64_t v_head, const T* __restrict__ go,
@@ -583,9 +583,9 @@ __global__ __launch_bounds__(128 * PARTS, 2) void attention_grad_kv_kernel(
     // the rows' offsets are made anew in every step: kept, they would not fit the registers
     int l = lane;
     asm volatile("" : "+v"(l));
-    load_rows<DP, ROWS, 2 * PARTS>(sq, q + first * q_token + a * q_head, n,
+    load_rows<DP, ROWS, BLOCKS * PARTS>(sq, q + first * q_token + a * q_head, n,
                                    (uint32_t)(2 * q_token), s.dim, wave, l);
-    load_rows<DP, ROWS, 2 * PARTS>(sg, go + first * go_token + a * go_head, n,
+    load_rows<DP, ROWS, BLOCKS * PARTS>(sg, go + first * go_token + a * go_head, n,
                                    (uint32_t)(2 * go_token), s.dim, wave, l);
     if (wave < PARTS) {  // 64 rows' statistics a wave
       const int which = wave & 1, at = (wave >> 1) * 64;
@@ -736,7 +736,8 @@ Shape shape_of(const fsp_attention_packed_args& a) {
 // 45 / 49; dim 64, whose workgroups go four to a CU: 4096 (512) 53 / 46, two of 4096 (1024) 90 / 85.
 // Gradient of the queries, dim 128: 2048 56 / 48, 4096 under a window 63 / 70; 8192, 8 heads 232 / 203.
 // Gradients of the keys, dim 128: 3000, 4 heads over 4 (188) 48 / 35; two of 4096 (512) 378 / 286; two
-// of 2048 under a window (512) 77 / 96; three short ones (40) 9 / 12.
+// of 2048 under a window (512) 77 / 96; three short ones (40) 9 / 12; the whole backward pass of 900, 16
+// heads (240) 50.3 / 48.5, of two of 700, 8 heads (176) 42.7 / 42.7.
 constexpr int64_t kCus = 256;
 
 int64_t seen_at_most(const fsp_attention_packed_args& a, int64_t longest) {
@@ -761,8 +762,19 @@ bool halve_tiles(const fsp_attention_packed_args& a, int64_t most) {
 
 bool share_keys(const fsp_attention_packed_args& a, int split) {
   const int64_t n = a.n_k_tiles * a.kv_heads * split;
-  return (n <= kCus && a.heads / a.kv_heads / split * seen_at_most(a, a.q_longest) >= 1024) ||
+  return (n <= kCus && a.heads / a.kv_heads / split * seen_at_most(a, a.q_longest) >= 768) ||
          (n <= 2 * kCus && a.causal && !a.window && a.q_longest >= 4096);
+}
+
+// Tiles of half the keys, with four waves to them, where whole ones leave CUs without any.  Measured
+// without and with them, us, the whole backward pass (tiles times heads): dim 128: two of 256, 4 heads (32)
+// 29.7 / 30.6, one of 500, 16 heads over 4 (128) 40.7 / 38.1, 4000, 2 heads (126) 136 / 127, 2000, 8
+// heads (256) 79 / 84; dim 64: 65 tokens 15.8 / 15.4, two of 256 (32) 19.9 / 18.9, 2000, 8 heads (256)
+// 49.2 / 46.8.
+bool halve_keys(const fsp_attention_packed_args& a, int split) {
+  const bool small = a.dim <= 64;
+  return a.n_k_tiles * a.kv_heads * split <= (small ? kCus : kCus / 2) &&
+         seen_at_most(a, a.q_longest) > (small ? kRows : 4 * kRows);
 }
 
 // Shares of a group's heads that go to workgroups of their own, for their sums to be added by another
@@ -820,13 +832,15 @@ int launch_grad_q(const fsp_attention_packed_args& a, hipStream_t st) {
   return check_hip(hipGetLastError(), "attention_grad_q_kernel launch");
 }
 
-template <typename T, int DP, int PARTS>
+template <typename T, int DP, int BLOCKS, int PARTS>
 int launch_grad_kv(const fsp_attention_packed_args& a, int split, hipStream_t st) {
+  const int32_t* tiles = BLOCKS == 1 ? a.k_halves : a.k_tiles;
+  const int64_t n = BLOCKS == 1 ? a.n_k_halves : a.n_k_tiles;
   float* stats = static_cast<float*>(a.workspace);
   float* sums = stats + ((2 * a.heads * a.q_tokens + 3) & ~int64_t(3));
-  hipLaunchKernelGGL((attention_grad_kv_kernel<T, DP, PARTS>),
-                     dim3((unsigned)(a.n_k_tiles * a.kv_heads * split)), dim3(128 * PARTS), 0, st,
-                     shape_of(a), reinterpret_cast<const Tile*>(a.k_tiles), (int)a.n_k_tiles,
+  hipLaunchKernelGGL((attention_grad_kv_kernel<T, DP, BLOCKS, PARTS>),
+                     dim3((unsigned)(n * a.kv_heads * split)), dim3(64 * BLOCKS * PARTS), 0, st,
+                     shape_of(a), reinterpret_cast<const Tile*>(tiles), (int)n,
                      in<T>(a.q), a.q_token, a.q_head, in<T>(a.k), a.k_token, a.k_head, in<T>(a.v),
                      a.v_token, a.v_head, in<T>(a.grad_out), a.grad_out_token, a.grad_out_head,
                      stats, a.q_tokens, static_cast<T*>(a.grad_k), a.grad_k_token, a.grad_k_head,
@@ -852,8 +866,9 @@ int launch_backward(const fsp_attention_packed_args& a, hipStream_t st) {
   }
   if (a.n_k_tiles > 0) {
     const int split = split_heads(a.n_k_tiles, a.heads, a.kv_heads, a.causal && !a.window);
-    return share_keys(a, split) ? launch_grad_kv<T, DP, 4>(a, split, st)
-                                : launch_grad_kv<T, DP, 2>(a, split, st);
+    if (halve_keys(a, split)) return launch_grad_kv<T, DP, 1, 4>(a, split, st);
+    return share_keys(a, split) ? launch_grad_kv<T, DP, 2, 4>(a, split, st)
+                                : launch_grad_kv<T, DP, 2, 2>(a, split, st);
   }
   return FSP_OK;
 }
@@ -871,10 +886,10 @@ int check_packed(const fsp_attention_packed_args& a, const std::string& who) {
   if (a.kv_heads < 1 || a.heads < 1 || a.heads % a.kv_heads || a.heads > 0xffff)
     return set_error(FSP_EINVAL, who + ": heads must be a multiple of kv_heads");
   if (a.q_tokens < 0 || a.k_tokens < 0 || a.n_q_tiles < 0 || a.n_k_tiles < 0 ||
-      a.n_q_halves < 0 || a.window < 0 || a.q_longest < 0 || a.k_longest < 0 ||
+      a.n_q_halves < 0 || a.n_k_halves < 0 || a.window < 0 || a.q_longest < 0 || a.k_longest < 0 ||
       a.q_tokens > 0x7fffffffLL || a.k_tokens > 0x7fffffffLL || a.window > 0x7fffffffLL ||
       a.n_q_tiles > kMaxBlocks / a.heads || a.n_q_halves > kMaxBlocks / a.heads ||
-      a.n_k_tiles > kMaxBlocks / a.heads)
+      a.n_k_tiles > kMaxBlocks / a.heads || a.n_k_halves > kMaxBlocks / a.heads)
     return set_error(FSP_EINVAL, who + ": size out of range");
   auto step = [&](int64_t tokens, int64_t by) {
     return (tokens < 2 || by >= a.dim) && by >= 0 && by <= kTokenStep;
@@ -884,7 +899,7 @@ int check_packed(const fsp_attention_packed_args& a, const std::string& who) {
     return set_error(FSP_EINVAL, who + ": a token's step must lie between dim and 2^23");
   if (a.window && !a.causal) return set_error(FSP_EINVAL, who + ": window needs causal");
   if ((a.n_q_tiles > 0 && (!a.q_tiles || !a.q_halves || !a.q || !a.out || !a.lse)) ||
-      (a.n_k_tiles > 0 && !a.k_tiles) || (a.k_tokens > 0 && (!a.k || !a.v)))
+      (a.n_k_tiles > 0 && (!a.k_tiles || !a.k_halves)) || (a.k_tokens > 0 && (!a.k || !a.v)))
     return set_error(FSP_EINVAL, who + ": null pointer");
   if (!aligned16(a.q, a.q_token, a.q_head) || !aligned16(a.k, a.k_token, a.k_head) ||
       !aligned16(a.v, a.v_token, a.v_head) || !aligned16(a.out, a.out_token, a.out_head))
@@ -907,7 +922,7 @@ extern "C" int64_t fsp_attention_packed_workspace(int64_t n_k_tiles, int64_t hea
 }
 
 extern "C" int64_t fsp_attention_packed_tile(int which) {
-  return which == 0 ? kTile : which == 1 ? kTile / 2 : kRows;
+  return which == 0 ? kTile : which == 1 ? kTile / 2 : which == 2 ? kRows : kRows / 2;
 }
 
 extern "C" int fsp_attention_packed(const fsp_attention_packed_args* args, void* stream) {

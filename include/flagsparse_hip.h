@@ -769,8 +769,8 @@ int fsp_attention_paged(const struct fsp_attention_paged_args* args, void* strea
  *
  * Work lists, in any order: a tile is 8 int32, {first row, rows, first row's place in its sequence,
  * sequence's q begin, q count, k begin, k count, 0}; q_tiles cover the queries in
- * fsp_attention_packed_tile(0) rows, q_halves in fsp_attention_packed_tile(1) rows, k_tiles
- * (backward only) the keys in fsp_attention_packed_tile(2) rows.
+ * fsp_attention_packed_tile(0) rows, q_halves in fsp_attention_packed_tile(1) rows, k_tiles and
+ * k_halves (backward only) the keys in fsp_attention_packed_tile(2) and (3) rows.
  *
  * Backward: grad_out by its steps, out and lse of the forward pass; grad_q, grad_k, grad_v are
  * written whole.  workspace: fsp_attention_packed_workspace() bytes (uneven: causal
@@ -786,6 +786,8 @@ struct fsp_attention_packed_args {
   int64_t n_q_halves;
   const int32_t* k_tiles;
   int64_t n_k_tiles;
+  const int32_t* k_halves;
+  int64_t n_k_halves;
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;
   int64_t grad_out_token, grad_out_head, grad_q_token, grad_q_head;
   int64_t grad_k_token, grad_k_head, grad_v_token, grad_v_head;

@@ -51,7 +51,7 @@ def test_struct_sizes():
     assert attention._CACHE.size == 8 * 17
     assert attention._APPEND.size + attention._APPEND_AT.size == 8 * 21
     assert attention._PAGED.size + attention._PAGED_AT.size == 8 * 17
-    assert attention._PACKED.size + attention._PACKED_AT.size == 8 * (17 + 16 + 10)
+    assert attention._PACKED.size + attention._PACKED_AT.size == 8 * (19 + 16 + 10)
     assert _abi.lib().fsp_attention_dim_cap() == attention._DIM_CAP
 
 
@@ -78,13 +78,15 @@ def test_piece_sizes():
 
 
 def _packed(**kw):
-    a = dict(dtype=2, heads=4, kv_heads=2, dim=64, q_tokens=8, k_tokens=8, q_longest=8, k_longest=8, causal=1, window=0,
-             scale=0.125, q_tiles=16, n_q_tiles=1, q_halves=16, n_q_halves=2, k_tiles=16, n_k_tiles=1)
+    a = dict(dtype=2, heads=4, kv_heads=2, dim=64, q_tokens=8, k_tokens=8, q_longest=8, k_longest=8,
+             causal=1, window=0, scale=0.125, q_tiles=16, n_q_tiles=1, q_halves=16, n_q_halves=2,
+             k_tiles=16, n_k_tiles=1, k_halves=16, n_k_halves=2)
     for n in ("q", "k", "v", "out", "go", "gq", "gk", "gv"):
         a |= {n: 64, n + "_token": 256, n + "_head": 64}
     a |= {"lse": 16, "work": 16} | kw
-    order = ["dtype", "heads", "kv_heads", "dim", "q_tokens", "k_tokens", "q_longest", "k_longest", "causal", "window", "scale",
-             "q_tiles", "n_q_tiles", "q_halves", "n_q_halves", "k_tiles", "n_k_tiles"]
+    order = ["dtype", "heads", "kv_heads", "dim", "q_tokens", "k_tokens", "q_longest", "k_longest",
+             "causal", "window", "scale", "q_tiles", "n_q_tiles", "q_halves", "n_q_halves", "k_tiles",
+             "n_k_tiles", "k_halves", "n_k_halves"]
     eight = ("q", "k", "v", "out", "go", "gq", "gk", "gv")
     order += [n + e for n in eight for e in ("_token", "_head")]
     at = [*eight[:4], "lse", *eight[4:], "work"]

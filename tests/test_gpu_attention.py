@@ -96,7 +96,7 @@ def test_long_chains_with_many_heads(dev):
 
 @pytest.mark.parametrize("dim", [64, 96, 128])
 @pytest.mark.parametrize("lengths,heads", [([64], 4), ([65], 4), ([64] * 5, 60), ([65] * 3, 60),
-                                           ([600], 40), ([520, 3], 54)])
+                                           ([600], 40), ([520, 3], 54), ([300, 65], 8)])
 def test_shares_of_a_tile(dev, lengths, heads, dim):
     # few and many workgroups, chains of one step of keys and of several
     _both(dev, lengths, lengths, heads, 2, dim, BF, True, None)
