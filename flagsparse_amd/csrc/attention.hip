@@ -643,14 +643,16 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_grad_kv_kern
     }
   };
 
-  // the steps of every head of the group, one after the other
+  // From the last queries back, the heads of the group in turn: the tiles of a sequence that started
+  // together read the same rows together, wherever their keys' first queries lie.  Two sequences of 4096,
+  // 32 heads of 128 over 8: 1.98 GB past the L2s with a head after the other from its first query
+  // on, 0.56 GB so; forward and backward 1222 and 1194 us.
   const int steps = hit > lot ? (hit - lot + ROWS - 1) / ROWS : 0;
-  const int total = steps * group;
-  int a = (g * split + share) * group, i0 = lot;  // of this step
-  int a1 = a, i1 = lot;                           // of the one being loaded
+  const int total = steps * group, a0 = (g * split + share) * group;
+  int a = a0, i0 = lot + (steps - 1) * ROWS;  // of this step
+  int a1 = a, i1 = i0;                        // of the one being loaded
   auto next = [&] {
-    i1 += ROWS;
-    if (i1 >= hit) i1 = lot, ++a1;
+    if (++a1 == a0 + group) a1 = a0, i1 -= ROWS;
   };
   if (total) load(a, i0, s_q0, s_g0, s_x0, s_y0);
   __syncthreads();
