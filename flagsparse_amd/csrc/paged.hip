@@ -68,8 +68,10 @@ struct AppendShape {
 };
 
 // A wave to a token, or to one of ``parts`` interleaved parts of its vectors of eight elements, where
-// there are few tokens.  Bound by memory for prompts (a read and a write of every element) and by
-// the chain token -> sequence -> page -> row for single tokens.
+// there are few tokens.  Bound by memory for prompts (a read and a write of every element: 24 of up to 2000
+// tokens, 16 query and 16 key heads of 64, 111 MB in 20.8 us, 5.3 TB/s, part of it still in the
+// last-level cache) and by the chain token -> sequence -> page -> row for single tokens (16 tokens, 32
+// query and 8 key heads of 128: 3.8 us).  An element a thread took 48 us for those prompts.
 template <typename T, int MODE>
 __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(
     Cache c, AppendShape s, T* __restrict__ k_pages, T* __restrict__ v_pages,
@@ -165,8 +167,9 @@ __device__ __forceinline__ void all_stored() {
 // one: with a lane to a key a load would fetch 64 bytes of each of 16 rows, and whole rows are the
 // faster to fetch (a bare loop of such loads over 3.2 GB: 64 bytes 540 us, rows 490), so that a wave
 // writes the rows to LDS of its own and reads its lanes' keys there.  With S^T = K Q^T lane l has head
-// l % 16 and, of 32 keys, the eight 4 * (l / 16) + {0..3, 16..19}: its weights are the operand of O^T = V^T P^T as they lie, since the order of the summed keys is free.
-// For V a lane loads DP / 16 consecutive elements of those same eight keys, and the operand of one
+// l % 16 and, of 32 keys, the eight 4 * (l / 16) + {0..3, 16..19}: its weights are the operand of
+// O^T = V^T P^T as they lie, since the order of the summed keys is free.  For V a lane loads DP / 16
+// consecutive elements of those same eight keys, and the operand of one
 // product is one element of each: pairs of 16-bit halves, a byte permutation each.  Row m of product
 // i is element DP / 16 * m + i of the head, so a lane's results are consecutive.
 //
@@ -201,11 +204,16 @@ struct PagedShape {
   float scale;
 };
 
-//
 // The next step's keys are asked for once this step's scores are made, its values once this step's
-// output is; without conditions (the last step asks for its own again), so that the wait for the
-// values does not wait for the keys asked for after them.  EXACT: the head has DP elements.
-// NT: loads that do not claim a place in the caches.
+// output is; without conditions (the last step asks for one row that it has had; for all of its own,
+// which NT loads may have to fetch anew, 2 sequences of 102400 tokens, 16 heads took 292 us, so 278),
+// so that the wait for the values does not wait for the keys asked for after them.  EXACT: the head
+// has DP elements.  NT: loads that do not claim a place in the caches.
+//
+// Bound by memory for long caches: 6 sequences of 131072 tokens, 8 heads of 128, 64 queries, 3.2 GB,
+// 533 us, 6.0 TB/s of the 6.3 of a bare read; 96 ragged ones of up to 4096, 200 MB, 43 us, 4.7 TB/s: less
+// than two rounds of workgroups, each with the chain piece -> length -> page -> keys before it.  For
+// 1000 tokens that chain, the join and the launch are all of its 7.8 us.
 template <typename T, int DP, bool EXACT, bool NT>
 __global__ __launch_bounds__(256, 3) void attention_paged_kernel(
     Cache c, PagedShape s, const Piece* __restrict__ pieces, const T* __restrict__ k_pages,
@@ -269,19 +277,20 @@ __global__ __launch_bounds__(256, 3) void attention_paged_kernel(
   VE vf[8];
   // load i: rows 64 / CH * i + lane / CH, chunk lane % CH of each; it lies in LDS at chunk ^ row
   const int k_row = lane / CH, k_chunk = lane % CH;
-  auto load_k = [&](int j) {
+  auto load_k = [&](int j, int most) {
 #pragma unroll
     for (int i = 0; i < KL; ++i)
       kr[i] = ld_stream<NT>(reinterpret_cast<const i32x4*>(
-          kb + s_k[j + 64 / CH * i + k_row] + (EXACT || 8 * k_chunk < c.dim ? 8 * k_chunk : 0)));
+          kb + s_k[min(j + 64 / CH * i + k_row, most)] +
+          (EXACT || 8 * k_chunk < c.dim ? 8 * k_chunk : 0)));
   };
   char* s_rows = s_raw + wave * sizeof(Sums);
   const int ve = E * col < c.dim ? E * col : 0;
-  auto load_v = [&](int j) {
+  auto load_v = [&](int j, int most) {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       vf[e] = ld_stream<NT>(reinterpret_cast<const VE*>(
-          vb + s_v[j + 16 * (e / 4) + 4 * quad + e % 4] + ve));
+          vb + s_v[min(j + 16 * (e / 4) + 4 * quad + e % 4, most)] + ve));
   };
 
   float top = -INFINITY, sum = 0;
@@ -290,7 +299,7 @@ __global__ __launch_bounds__(256, 3) void attention_paged_kernel(
   for (int i = 0; i < E; ++i) o[i] = f32x4{};
 
   int j = 32 * wave;
-  if (j < n) load_k(j), load_v(j);
+  if (j < n) load_k(j, kPieceMost), load_v(j, kPieceMost);
   for (; j < n; j += 32 * W) {
 #pragma unroll
     for (int i = 0; i < KL; ++i) {
@@ -311,8 +320,9 @@ __global__ __launch_bounds__(256, 3) void attention_paged_kernel(
                       qf[i], x[u]);
       }
     }
-    const int next = j + 32 * W < n ? j + 32 * W : j;
-    load_k(next);
+    const bool more = j + 32 * W < n;
+    const int next = more ? j + 32 * W : j, most = more ? kPieceMost : j;
+    load_k(next, most);
     const bool partial = j + 32 > n;
     if (partial) {
 #pragma unroll
@@ -351,7 +361,7 @@ __global__ __launch_bounds__(256, 3) void attention_paged_kernel(
       for (int e = 0; e < 8; ++e) a[e] = vf[e][i];
       o[i] = mfma16(a, pf, o[i]);
     }
-    load_v(next);
+    load_v(next, most);
   }
 
   // join the waves
@@ -383,9 +393,14 @@ __global__ __launch_bounds__(256, 3) void attention_paged_kernel(
     }
     if (split) {
       const int64_t at = (int64_t)(pc.slot + mine) * s.heads + head0 + h;
-      put(part_o + at * c.dim + d, y.x, y.y);
-      put(part_o + at * c.dim + d + 2, y.z, y.w);
-      if (d == 0) put(part_ml + 2 * at, most, total);
+      if (arrived) {
+        put(part_o + at * c.dim + d, y.x, y.y);
+        put(part_o + at * c.dim + d + 2, y.z, y.w);
+        if (d == 0) put(part_ml + 2 * at, most, total);
+      } else {
+        *reinterpret_cast<f32x4*>(part_o + at * c.dim + d) = y;
+        if (d == 0) *reinterpret_cast<f32x2*>(part_ml + 2 * at) = f32x2{most, total};
+      }
     } else {
       const float f = total == 0 ? 0.0f : 1.0f / total;
 #pragma unroll
