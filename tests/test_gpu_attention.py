@@ -293,6 +293,23 @@ def test_offsets_past_32_bits(dev):
         ref.check(name, x, want[name])
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_the_longest_steps_between_tokens(dev, d):
+    # the longest that the kernels take as they are: a tile's rows span almost 2^31 bytes
+    n, step = 300, 1 << 23
+    room = torch.empty(n * step, dtype=BF, device=dev)
+    q, k, v, g = _inputs(dev, [n], [n], 1, 1, d, BF)
+    views = [room[d * i:].as_strided((n, 1, d), (step, d, 1)) for i in range(5)]
+    for t, x in zip(views, (q, k, v, g)):
+        t.copy_(x)
+    ip = _indptr([n], dev)
+    out, lse = fs.flagsparse_attention_packed(*views[:3], ip, out=views[4], return_lse=True)
+    grads = fs.flagsparse_attention_packed_backward(views[3], *views[:3], out, lse, ip)
+    want = ref.packed(q, k, v, [n], [n], True, None, d**-0.5, g)
+    for name, x in zip(("out", "lse", "q", "k", "v"), (out, lse, *grads)):
+        ref.check(name, x, want[name])
+
+
 def test_nothing_to_do(dev):
     for q_len, k_len in (([], []), ([0, 0], [0, 0]), ([0], [5]), ([5], [0])):
         q, k, v, g = _inputs(dev, q_len, k_len, 2, 1, 64, HF)
