@@ -176,13 +176,14 @@ __device__ __forceinline__ void all_stored() {
 // Where each key lies (its page, its place in it) is found once for the piece and kept in LDS.
 constexpr int kHeadTile = 16;
 constexpr int kPieceMost = 1024;
-// The workgroup that finishes a sequence joins its pieces where they are at most so many and all
-// workgroups are on the chip at once (three to a CU): the wait for their stores then holds up nobody.
-// Else a second launch does.  1000 tokens, 16 heads of 64: 8.7 us a call joined so, 11.9 by a second
-// launch, both bound by the host (9.2 and 8.4 us in a graph); 6 sequences of 131072 tokens, pieces
-// of 1024: 645 and 583 us.
+// The workgroup that finishes a sequence joins its pieces where they are at most so many and the
+// workgroups no more than a few rounds of the chip's (three to a CU): each waits for its stores, which
+// in many rounds holds up those that follow.  Else a second launch does.  By a second launch and so, us: 1000 tokens, 16 heads of 64 11.9 / 8.7 a
+// call, both bound by the host (8.4 / 9.2 in a graph); 96 ragged sequences of up to 4096, 8 heads of
+// 128 (1344 workgroups) 49.5 / 44.6; 200 of 2048, 16 heads of 64 (6400) 263 / 283; 400 of 1500, 8 heads
+// of 128 (6400) 418 / 408.  Up to 27 pieces 15.7 / 20.7 (2 of 6760, 8 heads), up to 128 542 / 560.
 constexpr int kJoinMost = 8;
-constexpr int kResident = 3 * 256;
+constexpr int kJoinBlocks = 8 * 256;
 
 // Tokens [begin, begin + piece) of seq, of the room that its pages give; slot: of the sequence's first
 // piece; page: its first place in the page table.
@@ -211,9 +212,9 @@ struct PagedShape {
 // has DP elements.  NT: loads that do not claim a place in the caches.
 //
 // Bound by memory for long caches: 6 sequences of 131072 tokens, 8 heads of 128, 64 queries, 3.2 GB,
-// 533 us, 6.0 TB/s of the 6.3 of a bare read; 96 ragged ones of up to 4096, 200 MB, 43 us, 4.7 TB/s: less
-// than two rounds of workgroups, each with the chain piece -> length -> page -> keys before it.  For
-// 1000 tokens that chain, the join and the launch are all of its 7.8 us.
+// 533 us, 6.0 TB/s of the 6.3 of a bare read, as for 256 of 4096, 32 queries; 96 ragged ones of up to
+// 4096, 200 MB, 44 us, 4.6 TB/s: less than two rounds of workgroups, each with the chain piece -> length
+// -> page -> keys before it.  For 1000 tokens that chain, the join and the launch are all of its 7.8 us.
 template <typename T, int DP, bool EXACT, bool NT>
 __global__ __launch_bounds__(256, 3) void attention_paged_kernel(
     Cache c, PagedShape s, const Piece* __restrict__ pieces, const T* __restrict__ k_pages,
@@ -680,7 +681,7 @@ extern "C" int64_t fsp_attention_paged_counts(int64_t n_pieces, int64_t most, in
                                               int64_t heads, int64_t kv_heads) {
   if (batch < 0 || heads < 1 || kv_heads < 1 || n_pieces <= batch || most > kJoinMost) return 0;
   const int64_t per = kv_heads * ((heads / kv_heads + kHeadTile - 1) / kHeadTile);
-  return n_pieces * per <= kResident ? batch * per : 0;
+  return n_pieces * per <= kJoinBlocks ? batch * per : 0;
 }
 
 extern "C" int64_t fsp_attention_paged_workspace(int64_t n_pieces, int64_t heads, int64_t dim) {
