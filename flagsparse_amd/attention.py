@@ -745,7 +745,11 @@ def _run_backward(prepared, kept, rows, lse, grads):
 def flagsparse_attention_packed_backward(grad_out, q, k, v, out, lse, indptr=None, k_indptr=None, *,
                                          prepared=None, causal=True, window=None, scale=None):
     """(grad_q, grad_k, grad_v) of flagsparse_attention_packed: ``grad_out`` is the gradient of its
-    output, ``out`` and ``lse`` what it returned, the other arguments its own."""
+    output, ``out`` and ``lse`` what it returned, the other arguments its own.
+
+    Sums are float32 and in a fixed order: equal calls give equal bits.  What is not finite may reach
+    rows of the same sequence within 64 queries or keys of those that it belongs to, as in the
+    forward pass; it never reaches another sequence."""
     key, rows = None, (grad_out, q, k, v, out)
     if type(prepared) is PreparedAttention and type(scale) in _PLAIN and \
             type(window) in _PLAIN and type(causal) in _PLAIN:

@@ -114,6 +114,26 @@ def test_many_sequences(dev):
     _decode(dev, [(7 * i) % 40 for i in range(700)], 8, 2, 1, 64, BF)
 
 
+@pytest.mark.parametrize("heads,batch", [(16, 60), (10, 220)])
+def test_pieces_over_rounds_of_workgroups(dev, heads, batch):
+    # two pieces each, more than the chip takes at once: joined by the last to arrive, or another launch
+    g, d, page, each = heads // 2, 64, 64, 24
+    kp, vp = (_normal(s, batch * each, page, g, d, dtype=BF) for s in (1, 2))
+    lengths = [page * each - 13 * i % 700 for i in range(batch)]
+    k, v = ([x[each * b:each * (b + 1)].flatten(0, 1)[:n] for b, n in enumerate(lengths)]
+            for x in (kp, vp))
+    kv = fs.prepare_paged_kv(kp.to(dev), vp.to(dev), torch.arange(batch + 1, device=dev) * each,
+                             torch.arange(batch * each, device=dev))
+    q, n = _normal(3, batch, heads, d, dtype=BF).to(dev), torch.tensor(lengths, device=dev)
+    out, lse = fs.flagsparse_attention_paged(q, n, prepared=kv, return_lse=True)
+    for _ in range(20):
+        again, _ = fs.flagsparse_attention_paged(q, n, prepared=kv, return_lse=True)
+        assert torch.equal(out, again)
+    want = _want(q, k, v, lengths, None, d**-0.5)
+    ref.check("out", out, want["out"])
+    ref.check("lse", lse, want["lse"])
+
+
 def test_caches_past_the_last_level(dev):
     # a table of more than 256 MB is read by other loads
     pages, page, g, d, n = 16 * 1024, 64, 2, 128, 3000
