@@ -960,8 +960,12 @@ extern "C" int fsp_attention_packed_backward(const fsp_attention_packed_args* ar
   if (!args) return set_error(FSP_EINVAL, "fsp_attention_packed_backward: null arguments");
   const fsp_attention_packed_args& a = *args;
   if (int rc = check_packed(a, "fsp_attention_packed_backward")) return rc;
+  // without queries, and with one share of the heads, there is nothing to keep
+  const bool work = a.n_k_tiles > 0 && fsp_attention_packed_workspace(a.n_k_tiles, a.heads, a.kv_heads, a.dim,
+                                                                      a.q_tokens, a.k_tokens,
+                                                                      a.causal && !a.window) > 0;
   if ((a.n_q_tiles > 0 && (!a.grad_out || !a.grad_q || !a.workspace)) ||
-      (a.n_k_tiles > 0 && (!a.grad_k || !a.grad_v || !a.workspace)))
+      (a.n_k_tiles > 0 && (!a.grad_k || !a.grad_v)) || (work && !a.workspace))
     return set_error(FSP_EINVAL, "fsp_attention_packed_backward: null pointer");
   if (reinterpret_cast<uintptr_t>(a.workspace) % 16)
     return set_error(FSP_EINVAL, "fsp_attention_packed_backward: workspace must be 16-byte aligned");

@@ -774,8 +774,8 @@ int fsp_attention_paged(const struct fsp_attention_paged_args* args, void* strea
  *
  * Backward: grad_out by its steps, out and lse of the forward pass; grad_q, grad_k, grad_v are
  * written whole.  workspace: fsp_attention_packed_workspace() bytes (uneven: causal
- * and no window), 16-byte aligned.  q_longest,
- * k_longest: the longest sequence (they decide how the work is shared out, not what is computed).
+ * and no window), 16-byte aligned; NULL will do for none.  q_longest, k_longest: the longest
+ * sequence (they decide how the work is shared out, not what is computed).
  */
 struct fsp_attention_packed_args {
   int64_t dtype, heads, kv_heads, dim, q_tokens, k_tokens, q_longest, k_longest, causal, window;

@@ -402,3 +402,20 @@ def test_refusals(dev):
         with pytest.raises(kind):
             f()
             pytest.fail(f"refusal {n} did not come")
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(2, 2), (1, 1), (4, 2)])
+@pytest.mark.parametrize("q_len,k_len", [([0], [5]), ([0, 0], [70, 3])])
+def test_gradients_of_a_batch_without_queries(dev, q_len, k_len, heads, kv_heads):
+    # where the heads of a group are not shared out the workspace has no bytes
+    q, k, v, g = _inputs(dev, q_len, k_len, heads, kv_heads, 64, BF)
+    p = fs.prepare_attention_packed(_indptr(q_len, dev), _indptr(k_len, dev))
+    for _ in range(2):
+        out, lse = fs.flagsparse_attention_packed(q, k, v, prepared=p, return_lse=True)
+        grads = fs.flagsparse_attention_packed_backward(g, q, k, v, out, lse, prepared=p)
+        for x, t in zip(grads, (q, k, v)):
+            assert x.shape == t.shape and not x.any()
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    fs.flagsparse_attention_packed(*leaves, prepared=p).backward(g)
+    for t in leaves:
+        assert t.grad.shape == t.shape and not t.grad.any()
