@@ -411,6 +411,8 @@ def flagsparse_paged_append(k, v, lengths, token_indptr=None, *, prepared=None, 
         if key is not None and all(x is y for x, y in zip(
                 (k, v, q, cos, sin, n, token_indptr), given)):
             _keep(kv._calls, key, (head, None if q is None else _like(q.shape, dt, dev)))
+    elif res is not None:  # tokens of no sequence
+        res.fill_(float("nan"))
     if copied:
         out.copy_(res)
         res = out

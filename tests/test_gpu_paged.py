@@ -424,3 +424,21 @@ def test_refusals(dev):
         with pytest.raises(kind):
             f()
             pytest.fail(f"refusal {i} did not come")
+
+
+def test_tokens_of_no_sequence_at_all(dev):
+    # an empty batch whose offsets leave every token out
+    kp = torch.zeros(1, 16, 1, 64, dtype=BF, device=dev)
+    none = torch.zeros(0, dtype=torch.int32, device=dev)
+    kv = fs.prepare_paged_kv(kp, kp.clone(), torch.zeros(1, dtype=torch.int32, device=dev), none)
+    q = _normal(1, 5, 3, 64, dtype=BF).to(dev)
+    for _ in range(2):
+        room = [torch.zeros(5, 3, 64, dtype=BF, device=dev) for _ in range(4)]
+        del room  # what a fresh array is likely to hold
+        got = fs.flagsparse_paged_append(q[:, :1], q[:, :1], none, torch.zeros(1, device=dev,
+                                         dtype=torch.int32), prepared=kv, q=q)
+        assert torch.isnan(got).all()
+    out = torch.zeros(5, 3, 65, dtype=BF, device=dev)[:, :, 1:]
+    assert fs.flagsparse_paged_append(q[:, :1], q[:, :1], none, torch.zeros(1, device=dev,
+                                      dtype=torch.int32), prepared=kv, q=q, out=out) is out
+    assert torch.isnan(out).all() and not kp.any()
