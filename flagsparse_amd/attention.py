@@ -151,14 +151,32 @@ def _check_out(out, name, shape, dtype, device):
         raise TypeError(f"{name} dtype must be {dtype}")
 
 
-def _result(out, name, shape, dtype, device):
-    """(the array the kernel writes, whether ``out`` is to be copied from it)."""
+def _overlap(a, b):
+    """Whether the arrays may share memory; slices side by side in the rows of one array do not."""
+    if not a.numel() or not b.numel():
+        return False
+    size = a.element_size()
+    row_a, row_b = (1 + sum((n - 1) * s for n, s in zip(t.shape[1:], t.stride()[1:])) for t in (a, b))
+    step, gap = a.stride(0), b.data_ptr() - a.data_ptr()
+    if gap >= size * (row_a + (a.shape[0] - 1) * step) or \
+            -gap >= size * (row_b + (b.shape[0] - 1) * b.stride(0)):
+        return False
+    if step > 0 and step == b.stride(0):
+        at = gap // size % step  # of b's rows in a's
+        return at < row_a or at + row_b > step
+    return True
+
+
+def _result(out, name, shape, dtype, device, *inputs):
+    """(the array the kernel writes, whether ``out`` is to be copied from it): a kernel reads its inputs
+    while it writes, so it never writes over them."""
     if out is None:
         return torch.empty(shape, dtype=dtype, device=device), False
     _check_out(out, name, shape, dtype, device)
     s = out.stride()
     if s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and out.data_ptr() % 16 == 0 and \
-            (s[0] or shape[0] < 2) and (s[1] or shape[1] < 2):
+            (s[0] or shape[0] < 2) and (s[1] or shape[1] < 2) and \
+            not any(_overlap(out, t) for t in inputs):
         return out, False
     return torch.empty(shape, dtype=dtype, device=device), True
 
@@ -347,8 +365,9 @@ def flagsparse_paged_append(k, v, lengths, token_indptr=None, *, prepared=None, 
     every head of ``k`` and ``q`` are rotated by pairs, (a, b) -> (a cos - b sin, a sin + b cos):
     elements half apart, or neighbours with ``interleaved``.  Without them nothing is rotated.
 
-    Returns the rotated ``q`` [tokens, heads, dim] (written to ``out`` where given), or None
-    without ``q``.  The pages that new tokens go to belong to one sequence each.  With
+    Returns the rotated ``q`` [tokens, heads, dim] (written to ``out`` where given, which may be ``q``),
+    or None without ``q``.  The pages that new tokens go to belong to one sequence each, and ``k``,
+    ``v`` and ``q`` lie outside the cache.  With
     ``prepared`` nothing is waited for, so lengths are not checked: a token whose position is
     negative or past its sequence's pages is not stored and its row of ``q`` comes back as NaN."""
     key = None
@@ -398,7 +417,7 @@ def flagsparse_paged_append(k, v, lengths, token_indptr=None, *, prepared=None, 
         if q.shape[0] != tokens:
             raise ValueError(f"q must have {tokens} tokens, got {q.shape[0]}")
         heads = q.shape[1]
-        res, copied = _result(out, "out", q.shape, dt, dev)
+        res, copied = _result(out, "out", q.shape, dt, dev, q, k, v)
         q = _rows(q)
     elif out is not None:
         raise ValueError("out is for the rotated q")
@@ -459,7 +478,7 @@ def flagsparse_attention_paged(q, lengths, *, prepared=None, k_pages=None, v_pag
     heads = q.shape[1]
     _check_heads(heads, kv.kv_heads)
     factor, past = _scale_of(scale, kv.dim), _window_of(window)
-    res, copied = _result(out, "out", q.shape, dt, dev)
+    res, copied = _result(out, "out", q.shape, dt, dev, q, kv.k_pages, kv.v_pages)
     rows = _rows(q)
     # what such calls share: the arguments, patterns of their arrays, the counts of arrivals they need
     pieces, need, room = kv._pieces.shape[0], 0, None
@@ -643,7 +662,7 @@ def _run_forward(prepared, head, q, k, v, res, lse):
 
 
 def _forward(prepared, q, k, v, causal, window, scale, out=None, key=None):
-    res, copied = _result(out, "out", q.shape, q.dtype, q.device)
+    res, copied = _result(out, "out", q.shape, q.dtype, q.device, q, k, v)
     rows = _rows(q), _rows(k), _rows(v)
     head = _pack(prepared, *rows, causal, window, scale, res)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)

@@ -671,7 +671,9 @@ int fsp_run(const void* call, const void* in, void* out, void* stream);
  * axis is contiguous; a token's and a head's step are given in elements (a slice of one
  * fused projection; a step of 0 for a broadcast head of an input).  dim is a
  * multiple of 8 up to fsp_attention_dim_cap(), steps are multiples of 8 and bases 16-byte
- * aligned; packed arrays have token steps from dim to 2^23.  heads is a multiple of kv_heads; query head a reads key head a / (heads / kv_heads).
+ * aligned; packed arrays have token steps from dim to 2^23.  What a call writes shares no memory
+ * with what it reads (flagsparse_amd/attention.py makes a copy where an output does).  heads is a
+ * multiple of kv_heads; query head a reads key head a / (heads / kv_heads).
  * Sums, softmax statistics and gradients are held in 32 bits and rounded once at the end; the
  * weights are rounded to the inputs' type before their product with the values (the matrix
  * instructions' operand type).  The arguments come as a struct of 8-byte fields, those that change

@@ -203,3 +203,40 @@ def test_struct_of_bytes_reaches_the_library():
     # the structs go by address: a bytes object does
     assert isinstance(_packed(), bytes)
     assert ctypes.c_void_p in _abi.SIGNATURES["fsp_attention_packed"][1]
+
+
+def _elements(t):
+    i = sum(torch.arange(n).view(-1, *(1,) * (t.ndim - 1 - d)) * s
+            for d, (n, s) in enumerate(zip(t.shape, t.stride())))
+    return set((t.data_ptr() + t.element_size() * i).flatten().tolist())
+
+
+def test_outputs_over_inputs_are_seen():
+    # an output that shares an element with an input is not written by the kernel that reads it
+    room = torch.zeros(4096, dtype=torch.float16)
+    gen = torch.Generator().manual_seed(1)
+
+    def some():
+        n, h, d, s0, s1, at = (int(torch.randint(0, m, (1,), generator=gen)) for m in
+                               (5, 4, 9, 6, 4, 200))
+        return room.as_strided((n, h, 8 * (d % 2) + 8), (8 * [0, 1, 3, 8, 8, 9][s0], 8 * s1, 1), at)
+
+    shared = 0
+    for _ in range(3000):
+        a, b = some(), some()
+        if a.numel() and b.numel() and _elements(a) & _elements(b):
+            assert attention._overlap(a, b) and attention._overlap(b, a)
+            shared += 1
+    assert shared > 300
+
+
+def test_slices_side_by_side_do_not_overlap():
+    fused = torch.zeros(7, 8, 16, dtype=torch.float16)
+    q, k, v = fused[:, :4], fused[:, 4:6], fused[:, 6:]
+    for a, b in ((q, k), (k, q), (q, v), (k, v), (fused[:3], fused[3:]), (q, torch.zeros_like(q)),
+                 (q, q[:0])):
+        assert not attention._overlap(a, b)
+    for a, b in ((q, q), (fused[:, 3:5], q), (q, fused[:, 3:5]), (fused[1:], fused[:-1]),
+                 (q, fused[:, :, None].expand(7, 8, 2, 16)[:, 0, :1].expand(7, 4, 16)),
+                 (q, fused.view(7, 2, 4, 16))):
+        assert attention._overlap(a, b)

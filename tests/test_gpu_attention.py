@@ -419,3 +419,24 @@ def test_gradients_of_a_batch_without_queries(dev, q_len, k_len, heads, kv_heads
     fs.flagsparse_attention_packed(*leaves, prepared=p).backward(g)
     for t in leaves:
         assert t.grad.shape == t.shape and not t.grad.any()
+
+
+def test_outputs_over_inputs(dev):
+    # written after everything is read: over the queries, the keys, the values, or slices of each
+    lengths, h, d = [300, 65, 1], 4, 64
+    n = sum(lengths)
+    ip = _indptr(lengths, dev)
+    first = _normal(1, n + 1, 3 * h, d, dtype=BF, dev=dev)
+
+    def parts():
+        fused = first.clone()
+        return fused, fused[:n, :h], fused[:n, h:2 * h], fused[:n, 2 * h:]
+
+    _, q, k, v = parts()
+    want = fs.flagsparse_attention_packed(q, k, v, ip)
+    for place in (lambda f: f[:n, :h], lambda f: f[:n, h:2 * h], lambda f: f[:n, 2 * h:],
+                  lambda f: f[1:, :h], lambda f: f[1:, 2:h + 2], lambda f: f[:n, 2 * h - 1:3 * h - 1]):
+        fused, q, k, v = parts()
+        out = place(fused)
+        assert fs.flagsparse_attention_packed(q, k, v, ip, out=out) is out
+        assert torch.equal(out, want)

@@ -442,3 +442,47 @@ def test_tokens_of_no_sequence_at_all(dev):
     assert fs.flagsparse_paged_append(q[:, :1], q[:, :1], none, torch.zeros(1, device=dev,
                                       dtype=torch.int32), prepared=kv, q=q, out=out) is out
     assert torch.isnan(out).all() and not kp.any()
+
+
+@pytest.mark.parametrize("tokens", [3, 700])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dim,half", [(40, 20), (64, 32), (72, 17), (80, 40), (96, 48), (112, 56), (128, 64)])
+def test_append_over_its_queries(dev, dim, half, interleaved, tokens):
+    # out on q, on a slice that is partly q's, on k and on v: what the call gives elsewhere
+    g, h, page = 2, 32, 16
+    pages = -(-tokens // page)
+    cos, sin = (t.to(dev) for t in _table(tokens, half))
+    first = _normal(1, tokens + 1, h + 2 * g, dim, dtype=HF).to(dev)
+    n, at = torch.tensor([tokens], device=dev), torch.tensor([0, tokens], device=dev)
+
+    def call(place):
+        kp, vp = torch.zeros(2, pages, page, g, dim, dtype=HF, device=dev)
+        kv = fs.prepare_paged_kv(kp, vp, torch.tensor([0, pages], device=dev),
+                                 torch.arange(pages, device=dev))
+        fused = first.clone()
+        q, k, v = fused[:tokens, :h], fused[:tokens, h:h + g], fused[:tokens, h + g:]
+        out = None if place is None else place(fused)
+        got = fs.flagsparse_paged_append(k, v, n, at, prepared=kv, q=q, cos=cos, sin=sin,
+                                         interleaved=interleaved, out=out)
+        assert out is None or got is out
+        return got.clone(), kp, vp
+
+    want = call(None)
+    for place in (lambda f: f[:tokens, :h], lambda f: f[1:, :h], lambda f: f[:tokens, 2 * g:],
+                  lambda f: f[:tokens, 1:h + 1]):
+        for a, b in zip(call(place), want):
+            assert torch.equal(a, b)
+
+
+def test_paged_attention_over_its_queries(dev):
+    lengths = [900, 3, 0, 77]
+    kp, vp, ip, ix, _, _ = _cache(dev, lengths, 16, 2, 64, BF)
+    kv = fs.prepare_paged_kv(kp, vp, ip, ix)
+    n = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    first = _normal(1, 5, 8, 64, dtype=BF).to(dev)
+    want = fs.flagsparse_attention_paged(first[:4], n, prepared=kv)
+    for place in (lambda f: f[:4], lambda f: f[1:]):
+        room = first.clone()
+        out = place(room)
+        assert fs.flagsparse_attention_paged(room[:4], n, prepared=kv, out=out) is out
+        assert torch.equal(out, want)
