@@ -499,6 +499,18 @@ def flagsparse_attention_paged(q, lengths, *, prepared=None, k_pages=None, v_pag
     return (res, lse) if return_lse else res
 
 
+def _arrivals(kv, stream, need):
+    """The counts that the pieces' arrivals are kept in, zeros between calls: one array a stream, whose
+    calls follow each other.  A graph has its own, zeroed in each replay: it may run beside this
+    stream's calls and beside other graphs that were captured here."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(need, dtype=torch.int32, device=kv.device)
+    counts = kv._counts.get((stream, need))
+    if counts is None:
+        counts = kv._counts[stream, need] = torch.zeros(need, dtype=torch.int32, device=kv.device)
+    return counts
+
+
 def _attend(kv, kept, q, res, lengths, return_lse):
     """The launch; returns the log-sum-exp, if asked for."""
     head, _, like_lse, room, need = kept
@@ -509,11 +521,7 @@ def _attend(kv, kept, q, res, lengths, return_lse):
     if room is not None:
         work = torch.empty_like(room, memory_format=_CONTIGUOUS)
         if need:
-            counts = kv._counts.get((stream, need))
-            if counts is None:
-                counts = torch.zeros(need, dtype=torch.int32, device=kv.device)
-                if not torch.cuda.is_current_stream_capturing():  # else they are the graph's
-                    kv._counts[stream, need] = counts
+            counts = _arrivals(kv, stream, need)
     status = _abi.lib().fsp_attention_paged(head + _PAGED_AT.pack(
         q.data_ptr(), res.data_ptr(), _at(lse), lengths.data_ptr(), _at(work), _at(counts)), stream)
     if status:

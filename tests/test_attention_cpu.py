@@ -240,3 +240,22 @@ def test_slices_side_by_side_do_not_overlap():
                  (q, fused[:, :, None].expand(7, 8, 2, 16)[:, 0, :1].expand(7, 4, 16)),
                  (q, fused.view(7, 2, 4, 16))):
         assert attention._overlap(a, b)
+
+
+def test_a_graph_has_counts_of_its_own(monkeypatch):
+    # of a stream with calls before: neither theirs, nor another graph's, nor kept for later calls
+    class Cache:
+        device, _counts = torch.device("cpu"), _abi.Calls()
+
+    capturing = False
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+    kept = attention._arrivals(Cache, 7, 5)
+    assert attention._arrivals(Cache, 7, 5) is kept and attention._arrivals(Cache, 8, 5) is not kept
+    before = dict(Cache._counts)
+    capturing = True
+    graphs = [attention._arrivals(Cache, 7, 5) for _ in range(2)]
+    assert len({t.data_ptr() for t in (kept, *graphs)}) == 3
+    for t in graphs:
+        assert t.dtype == torch.int32 and t.shape == (5,) and not t.any()
+    assert Cache._counts.keys() == before.keys()
+    assert all(Cache._counts[n] is before[n] for n in before)

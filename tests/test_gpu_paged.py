@@ -486,3 +486,37 @@ def test_paged_attention_over_its_queries(dev):
         out = place(room)
         assert fs.flagsparse_attention_paged(room[:4], n, prepared=kv, out=out) is out
         assert torch.equal(out, want)
+
+
+def test_graphs_of_a_warm_stream_beside_its_calls(dev):
+    # two graphs captured on a stream that has run the call, replayed on others beside it
+    lengths = [900, 3, 2000, 77]
+    kp, vp, ip, ix, _, _ = _cache(dev, lengths, 16, 2, 64, BF)
+    kv = fs.prepare_paged_kv(kp, vp, ip, ix)
+    n = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    q = _normal(2, 4, 40, 64, dtype=BF).to(dev)
+    streams = [torch.cuda.Stream(dev) for _ in range(3)]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(streams[0]):
+        want = fs.flagsparse_attention_paged(q, n, prepared=kv)
+        assert kv._counts  # the pieces are joined in the kernel
+        torch.cuda.synchronize()
+        graphs = []
+        for _ in range(2):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=streams[0]):
+                held = fs.flagsparse_attention_paged(q, n, prepared=kv)
+            graphs.append((g, held))
+    torch.cuda.synchronize()
+    for _ in range(30):
+        got = []
+        for (g, _), s in zip(graphs, streams[1:]):
+            with torch.cuda.stream(s):
+                g.replay()
+        with torch.cuda.stream(streams[0]):
+            got = [fs.flagsparse_attention_paged(q, n, prepared=kv) for _ in range(3)]
+        torch.cuda.synchronize()
+        for x in (*got, *(held for _, held in graphs)):
+            assert torch.equal(x, want)
+    for counts in kv._counts.values():
+        assert not counts.any()
