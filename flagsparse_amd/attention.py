@@ -31,7 +31,7 @@ SUPPORTED_ATTENTION_DTYPES = (torch.bfloat16, torch.float16)
 
 _CODES = {torch.bfloat16: _abi.FSP_BF16, torch.float16: _abi.FSP_F16}
 _DIM_CAP = 128
-_TOKENS_CAP = 2**31 - 1
+_TOKENS_CAP = 2**31 - 1024  # a place past the last token by a step of any kernel is still an int32
 _STEP_CAP = 2**23
 
 # The argument structs of include/flagsparse_hip.h: 8-byte fields, "d" the scale.  What a call's
@@ -105,7 +105,7 @@ def _check_tensor(t, name, dtype=None, device=None, heads=None, dim=None):
     if dim is not None and t.shape[2] != dim:
         raise ValueError(f"{name} must have dim {dim}, got {t.shape[2]}")
     if t.shape[0] > _TOKENS_CAP:
-        raise ValueError(f"{name} must have fewer than 2^31 tokens")
+        raise ValueError(f"{name} must have at most 2^31 - 1024 tokens")
 
 
 def _check_dim(dim):
@@ -190,7 +190,7 @@ def _int32(t, name, length, device):
     if t.dtype not in SUPPORTED_INDEX_DTYPES:
         raise TypeError(f"{name} dtype must be torch.int32 or torch.int64")
     if t.dtype == torch.int64:
-        t = t.clamp(-1, _TOKENS_CAP).to(torch.int32)
+        t = t.clamp(-1, 2**31 - 1).to(torch.int32)
     return t.contiguous()
 
 
@@ -301,7 +301,7 @@ def prepare_paged_kv(k_pages, v_pages, indptr, indices):
     _check_dim(dim)
     if page_size < 1 or kv_heads < 1:
         raise ValueError("pages must hold at least one token and one head")
-    if n_pages * page_size > _TOKENS_CAP:
+    if n_pages * page_size > 2**31 - 1:
         raise ValueError("the cache must hold fewer than 2^31 tokens")
     for t, name in ((indptr, "indptr"), (indices, "indices")):
         if not torch.is_tensor(t) or t.ndim != 1:
@@ -313,7 +313,7 @@ def prepare_paged_kv(k_pages, v_pages, indptr, indices):
     if indptr.numel() < 1:
         raise ValueError("indptr must have at least one entry")
     if indices.numel() * page_size > _TOKENS_CAP:
-        raise ValueError("the page table must hold fewer than 2^31 tokens")
+        raise ValueError("the page table must hold at most 2^31 - 1024 tokens")
     (first, last, decreases, _, least, most), idx, ptr = csr_check(
         indices.contiguous(), indptr.contiguous(), 32)
     if first != 0:
@@ -598,7 +598,7 @@ def _host_lengths(indptr, name):
     if (np.diff(p) < 0).any():
         raise ValueError(f"{name} must be nondecreasing")
     if p[-1] > _TOKENS_CAP:
-        raise ValueError(f"{name} must count fewer than 2^31 tokens")
+        raise ValueError(f"{name} must count at most 2^31 - 1024 tokens")
     return np.diff(p)
 
 

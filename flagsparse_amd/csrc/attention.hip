@@ -909,7 +909,7 @@ int check_packed(const fsp_attention_packed_args& a, const std::string& who) {
     return set_error(FSP_EINVAL, who + ": heads must be a multiple of kv_heads");
   if (a.q_tokens < 0 || a.k_tokens < 0 || a.n_q_tiles < 0 || a.n_k_tiles < 0 ||
       a.n_q_halves < 0 || a.n_k_halves < 0 || a.window < 0 || a.q_longest < 0 || a.k_longest < 0 ||
-      a.q_tokens > 0x7fffffffLL || a.k_tokens > 0x7fffffffLL || a.window > 0x7fffffffLL ||
+      a.q_tokens > kAttnTokensCap || a.k_tokens > kAttnTokensCap || a.window > 0x7fffffffLL ||
       a.n_q_tiles > kMaxBlocks / a.heads || a.n_q_halves > kMaxBlocks / a.heads ||
       a.n_k_tiles > kMaxBlocks / a.heads || a.n_k_halves > kMaxBlocks / a.heads)
     return set_error(FSP_EINVAL, who + ": size out of range");

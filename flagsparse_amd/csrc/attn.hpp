@@ -13,6 +13,9 @@
 namespace fsp {
 
 constexpr int64_t kAttnDimCap = 128;
+// Tokens of a batch or of a page table: a place that lies past the last one by less than a step (up to
+// 1024 tokens) is still an int.
+constexpr int64_t kAttnTokensCap = 0x80000000LL - 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 

@@ -551,8 +551,8 @@ int check_cache(const fsp_paged_cache& c, const std::string& who) {
   if (c.kv_heads < 1 || c.page_size < 1 || c.n_pages < 0 || c.batch < 0 || c.table_len < 0)
     return set_error(FSP_EINVAL, who + ": negative or zero size");
   if (c.kv_heads > 0xffff || c.batch > 0x7fffffffLL || c.page_size > 0x7fffffffLL ||
-      c.n_pages > 0x7fffffffLL / c.page_size || c.table_len > 0x7fffffffLL / c.page_size)
-    return set_error(FSP_EINVAL, who + ": size exceeds 2^31-1 tokens");
+      c.n_pages > 0x7fffffffLL / c.page_size || c.table_len > kAttnTokensCap / c.page_size)
+    return set_error(FSP_EINVAL, who + ": size exceeds 2^31-1024 tokens");
   if (c.batch > 0 && (!c.page_indptr || (c.table_len > 0 && (!c.page_indices || !c.k_pages || !c.v_pages))))
     return set_error(FSP_EINVAL, who + ": null pointer");
   if (!aligned16(c.k_pages, c.k_page | c.k_slot, c.k_head) ||

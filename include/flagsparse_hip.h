@@ -690,7 +690,7 @@ int64_t fsp_attention_dim_cap(void);
  * by their steps, and a page table in CSR form: sequence b's tokens lie in pages
  * page_indices[page_indptr[b] .. page_indptr[b + 1]), in order, each within [0, n_pages).
  * lengths[b]: the tokens that sequence b holds (the ones appended in this step included), at most
- * its pages' room.
+ * its pages' room.  table_len * page_size is at most 2^31 - 1024, n_pages * page_size less than 2^31.
  */
 struct fsp_paged_cache {
   int64_t dtype, kv_heads, dim, page_size, n_pages, batch, table_len;
@@ -767,7 +767,8 @@ int fsp_attention_paged(const struct fsp_attention_paged_args* args, void* strea
  * Attention over packed sequences: sequence b's queries are tokens
  * [q_indptr[b], q_indptr[b + 1]), its keys [k_indptr[b], k_indptr[b + 1]).  With causal != 0 query
  * i of nq sees key j of nk if j <= i + nk - nq; a window > 0 (causal only) hides the keys
- * j <= i + nk - nq - window.  lse [q_tokens, heads] float32.
+ * j <= i + nk - nq - window.  lse [q_tokens, heads] float32.  q_tokens and k_tokens are at most
+ * 2^31 - 1024.
  *
  * Work lists, in any order: a tile is 8 int32, {first row, rows, first row's place in its sequence,
  * sequence's q begin, q count, k begin, k count, 0}; q_tiles cover the queries in

@@ -259,3 +259,16 @@ def test_a_graph_has_counts_of_its_own(monkeypatch):
         assert t.dtype == torch.int32 and t.shape == (5,) and not t.any()
     assert Cache._counts.keys() == before.keys()
     assert all(Cache._counts[n] is before[n] for n in before)
+
+
+@pytest.mark.parametrize("tokens", [2**31 - 1023, 2**31 - 16, 2**31 - 1])
+def test_lengths_that_a_step_would_pass_32_bits_from(tokens):
+    # places up to a step (1024 tokens) past the last token are 32-bit numbers in the kernels
+    L = _abi.lib()
+    for kw in ({"q_tokens": tokens}, {"k_tokens": tokens}):
+        assert L.fsp_attention_packed(_packed(**kw), None) == -1
+        assert L.fsp_attention_packed_backward(_packed(**kw), None) == -1
+    c = _cache(table_len=tokens, page_size=1)
+    assert L.fsp_attention_paged(c + _paged(), None) == -1
+    assert L.fsp_paged_append(c + _append(), None) == -1
+    assert attention._TOKENS_CAP == 2**31 - 1024

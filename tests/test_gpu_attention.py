@@ -440,3 +440,11 @@ def test_outputs_over_inputs(dev):
         out = place(fused)
         assert fs.flagsparse_attention_packed(q, k, v, ip, out=out) is out
         assert torch.equal(out, want)
+
+
+def test_batches_that_are_too_long(dev):
+    for n in (2**31 - 1023, 2**31 - 1, 2**33):
+        with pytest.raises(ValueError):
+            fs.prepare_attention_packed(torch.tensor([0, n], device=dev))
+        with pytest.raises(ValueError):
+            fs.prepare_attention_packed(torch.tensor([0, 1], device=dev), torch.tensor([0, n], device=dev))

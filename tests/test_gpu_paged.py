@@ -520,3 +520,30 @@ def test_graphs_of_a_warm_stream_beside_its_calls(dev):
             assert torch.equal(x, want)
     for counts in kv._counts.values():
         assert not counts.any()
+
+
+def test_the_longest_sequence(dev):
+    # one page, named over and over: the last token that a table can hold, and what it sees
+    page, g, h, d, n = 1024, 1, 2, 8, 2**31 - 1024
+    kp, vp = torch.zeros(2, 1, page, g, d, dtype=BF, device=dev)
+    k, v = (_normal(s, page, g, d, dtype=BF) for s in (1, 2))
+    kp.copy_(k[None]), vp.copy_(v[None])
+    with pytest.raises(ValueError):
+        fs.prepare_paged_kv(kp[:, :512], vp[:, :512], torch.tensor([0, 2**22 - 1], device=dev),
+                            torch.zeros(2**22 - 1, dtype=torch.int32, device=dev))
+    kv = fs.prepare_paged_kv(kp, vp, torch.tensor([0, n // page], device=dev),
+                             torch.zeros(n // page, dtype=torch.int32, device=dev))
+    assert kv.room == n
+    q = _normal(3, 1, h, d, dtype=BF).to(dev)
+    length = torch.tensor([n], dtype=torch.int32, device=dev)
+    k[-1], v[-1] = 2.0, 3.0
+    fs.flagsparse_paged_append(k[-1:].to(dev), v[-1:].to(dev), length, prepared=kv)
+    assert torch.equal(kp[0].cpu(), k) and torch.equal(vp[0].cpu(), v)
+    for window in (1, 700, 5000):
+        out, lse = fs.flagsparse_attention_paged(q, length, prepared=kv, window=window, return_lse=True)
+        at = torch.arange(n - window, n) % page
+        want = ref.packed(q, k[at], v[at], [1], [window], True, None, d**-0.5)
+        ref.check("out", out, want["out"])
+        ref.check("lse", lse, want["lse"])
+    length += 1
+    assert torch.isnan(fs.flagsparse_attention_paged(q, length, prepared=kv, window=700)).all()
