@@ -119,11 +119,17 @@ def _check_heads(heads, kv_heads):
         raise ValueError(f"query heads ({heads}) must be a multiple of key heads ({kv_heads})")
 
 
+def _steps(t):
+    """The steps of all axes but the last, as the kernels are given them: that of an axis of one element
+    says nothing (contiguous() keeps it, whatever it is), so a row's takes its place."""
+    return [s if n > 1 else t.shape[-1] for n, s in zip(t.shape[:-1], t.stride())]
+
+
 def _rows(t):
     """``t`` itself where the kernels can read it (contiguous last axis, 16-byte rows, tokens that do
     not overlap and lie within 2^23 elements of each other), else a copy."""
-    s = t.stride()
-    if s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and t.data_ptr() % 16 == 0 and \
+    s = _steps(t)
+    if t.stride(2) == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and t.data_ptr() % 16 == 0 and \
             t.shape[2] <= s[0] <= _STEP_CAP:
         return t
     return _aligned(t.contiguous())
@@ -173,9 +179,9 @@ def _result(out, name, shape, dtype, device, *inputs):
     if out is None:
         return torch.empty(shape, dtype=dtype, device=device), False
     _check_out(out, name, shape, dtype, device)
-    s = out.stride()
-    if s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and out.data_ptr() % 16 == 0 and \
-            (s[0] or shape[0] < 2) and (s[1] or shape[1] < 2) and \
+    s = _steps(out)
+    if out.stride(2) == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and out.data_ptr() % 16 == 0 and \
+            all(s) and \
             not any(_overlap(out, t) for t in inputs):
         return out, False
     return torch.empty(shape, dtype=dtype, device=device), True
@@ -240,11 +246,9 @@ class PreparedPagedKV:
 
     def _packed(self):
         k, v = self.k_pages, self.v_pages
-        ks, vs = k.stride(), v.stride()
         return _CACHE.pack(_CODES[k.dtype], self.kv_heads, self.dim, self.page_size, self.n_pages,
-                           self.batch, self.indices.numel(), k.data_ptr(), ks[0], ks[1], ks[2],
-                           v.data_ptr(), vs[0], vs[1], vs[2], self.indptr.data_ptr(),
-                           self.indices.data_ptr())
+                           self.batch, self.indices.numel(), k.data_ptr(), *_steps(k), v.data_ptr(),
+                           *_steps(v), self.indptr.data_ptr(), self.indices.data_ptr())
 
     def _on(self):
         """The current stream, on which the arrays are marked as used."""
@@ -277,8 +281,8 @@ def _check_pages(t, name):
         raise ValueError(f"{name} must be a CUDA tensor")
     if t.dtype not in SUPPORTED_ATTENTION_DTYPES:
         raise TypeError(f"{name} dtype must be torch.bfloat16 or torch.float16")
-    if t.numel() and (t.stride(3) != 1 or any(n % 8 for n in t.stride()[:3]) or
-                      t.data_ptr() % 16):
+    if t.numel() and (t.stride(3) != 1 or t.data_ptr() % 16 or
+                      any(s % 8 for n, s in zip(t.shape[:3], t.stride()) if n > 1)):
         raise ValueError(f"{name} must have a contiguous last axis and 16-byte aligned rows")
 
 
@@ -423,9 +427,9 @@ def flagsparse_paged_append(k, v, lengths, token_indptr=None, *, prepared=None, 
         raise ValueError("out is for the rotated q")
     if tokens and kv.batch:
         k, v = _rows(k), _rows(v)
-        steps = (*q.stride()[:2], *res.stride()[:2]) if heads else (0, 0, 0, 0)
+        steps = (*_steps(q), *_steps(res)) if heads else (0, 0, 0, 0)
         head = kv._packed() + _APPEND.pack(tokens, heads, half, rows, bool(interleaved),
-                                           *k.stride()[:2], *v.stride()[:2], *steps)
+                                           *_steps(k), *_steps(v), *steps)
         _append(kv, head, k, v, q, res, cos, sin, token_indptr, n)
         if key is not None and all(x is y for x, y in zip(
                 (k, v, q, cos, sin, n, token_indptr), given)):
@@ -488,7 +492,7 @@ def flagsparse_attention_paged(q, lengths, *, prepared=None, k_pages=None, v_pag
         room = _like((pieces * heads * (kv.dim + 2),), torch.float32, dev)
     kept = (kv._packed() + _PAGED.pack(
         kv._pieces.data_ptr(), kv._first.data_ptr(), pieces, kv._piece, heads, past, factor,
-        *rows.stride()[:2], *res.stride()[:2]), _like(q.shape, dt, dev),
+        *_steps(rows), *_steps(res)), _like(q.shape, dt, dev),
         _like((kv.batch, heads), torch.float32, dev), room, need)
     lse = _attend(kv, kept, rows, res, n, return_lse)
     if key is not None and rows is q and n is lengths:
@@ -648,7 +652,7 @@ def _packed_inputs(q, k, v, indptr, k_indptr, prepared, causal, window):
 def _pack(prepared, q, k, v, causal, window, scale, out, grads=()):
     """A call's arguments up to the addresses; grads: grad_out, grad_q, grad_k, grad_v."""
     lists = [prepared._tiles[which, causal] for which in range(4)]
-    steps = [n for t in (q, k, v, out, *grads) for n in t.stride()[:2]]
+    steps = [n for t in (q, k, v, out, *grads) for n in _steps(t)]
     steps += [0] * (16 - len(steps))
     return _PACKED.pack(_CODES[q.dtype], q.shape[1], k.shape[1], q.shape[2], q.shape[0],
                         k.shape[0], *prepared._longest, causal, window, scale,

@@ -272,3 +272,17 @@ def test_lengths_that_a_step_would_pass_32_bits_from(tokens):
     assert L.fsp_attention_paged(c + _paged(), None) == -1
     assert L.fsp_paged_append(c + _append(), None) == -1
     assert attention._TOKENS_CAP == 2**31 - 1024
+
+
+@pytest.mark.parametrize("tokens,heads", [(1, 4), (5, 1), (1, 1), (5, 4)])
+def test_rows_have_steps_that_the_kernels_take(tokens, heads):
+    # whatever an axis of one element has as its step, which contiguous() keeps
+    for room, s0, s1 in ((5000, 515, 64), (5000, 512, 67), (5000, 515, 67), (5000, 512, 64), (5000, 3, 5)):
+        t = torch.zeros(room, dtype=torch.float16).as_strided((tokens, heads, 64), (s0, s1, 1))
+        if t.data_ptr() % 16:
+            continue
+        r = attention._rows(t)
+        s = attention._steps(r)
+        assert torch.equal(r, t) and s[0] % 8 == 0 and s[1] % 8 == 0 and 64 <= s[0] <= 2**23
+        if (tokens == 1 or s0 == 512) and (heads == 1 or s1 == 64):
+            assert r is t  # no copy for a step that says nothing

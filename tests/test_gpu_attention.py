@@ -448,3 +448,18 @@ def test_batches_that_are_too_long(dev):
             fs.prepare_attention_packed(torch.tensor([0, n], device=dev))
         with pytest.raises(ValueError):
             fs.prepare_attention_packed(torch.tensor([0, 1], device=dev), torch.tensor([0, n], device=dev))
+
+
+def test_one_token_of_a_wider_array(dev):
+    # the step of an axis of one element is no multiple of anything, and contiguous() keeps it
+    h, g, d = 4, 2, 64
+    wide = _normal(1, 3, (h + 2 * g) * d + 3, dtype=BF, dev=dev)[:, :-3].unflatten(1, (-1, d))[:1]
+    assert wide.stride(0) % 8 and wide.is_contiguous()
+    q, k, v = wide[:, :h], wide[:, h:h + g], wide[:, h + g:]
+    grad = _normal(4, 2, h * d + 5, dtype=BF, dev=dev)[:, :h * d].unflatten(1, (h, d))[:1]
+    ip = _indptr([1], dev)
+    out, lse = fs.flagsparse_attention_packed(q, k, v, ip, return_lse=True)
+    grads = fs.flagsparse_attention_packed_backward(grad, q, k, v, out, lse, ip)
+    want = ref.packed(q, k, v, [1], [1], True, None, d**-0.5, grad)
+    for name, x in zip(("out", "lse", "q", "k", "v"), (out, lse, *grads)):
+        ref.check(name, x, want[name])

@@ -547,3 +547,21 @@ def test_the_longest_sequence(dev):
         ref.check("lse", lse, want["lse"])
     length += 1
     assert torch.isnan(fs.flagsparse_attention_paged(q, length, prepared=kv, window=700)).all()
+
+
+def test_one_token_and_one_head_of_wider_arrays(dev):
+    # the step of an axis of one element is no multiple of anything
+    g, h, d, n = 1, 3, 64, 40
+    kp, vp, ip, ix, k, v = _cache(dev, [n], 16, g, d, BF)
+    kp, vp = (t.as_strided(t.shape, (*t.stride()[:2], 5, 1)) for t in (kp, vp))
+    kv = fs.prepare_paged_kv(kp, vp, ip, ix)
+    fused = _normal(5, 2, (h + 2 * g) * d + 3, dtype=BF).to(dev)[:, :-3].unflatten(1, (-1, d))[:1]
+    assert fused.stride(0) % 8 and fused.is_contiguous()
+    length = torch.tensor([n], device=dev)
+    got = fs.flagsparse_paged_append(fused[:, h:h + g], fused[:, h + g:], length, prepared=kv,
+                                     q=fused[:, :h])
+    assert torch.equal(got, fused[:, :h])
+    out = fs.flagsparse_attention_paged(fused[:, :h], length, prepared=kv)
+    k, v = k[0].clone(), v[0].clone()
+    k[-1], v[-1] = fused[0, h:h + g].cpu(), fused[0, h + g:].cpu()
+    ref.check("out", out, _want(fused[:, :h], [k], [v], [n], None, d**-0.5)["out"])
