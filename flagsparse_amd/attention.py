@@ -33,6 +33,7 @@ _CODES = {torch.bfloat16: _abi.FSP_BF16, torch.float16: _abi.FSP_F16}
 _DIM_CAP = 128
 _TOKENS_CAP = 2**31 - 1024  # a place past the last token by a step of any kernel is still an int32
 _STEP_CAP = 2**23
+_FLOAT_MAX = (2 - 2.0**-23) * 2.0**127
 
 # The argument structs of include/flagsparse_hip.h: 8-byte fields, "d" the scale.  What a call's
 # shapes, steps and types settle comes first, then the addresses of its arrays.
@@ -136,7 +137,10 @@ def _rows(t):
 
 
 def _scale_of(scale, dim):
-    return dim ** -0.5 if scale is None else float(scale)
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not abs(scale) <= _FLOAT_MAX:
+        raise ValueError("scale must be finite in float32")
+    return scale
 
 
 def _window_of(window):

@@ -919,6 +919,7 @@ int check_packed(const fsp_attention_packed_args& a, const std::string& who) {
   if (!step(a.q_tokens, a.q_token) || !step(a.k_tokens, a.k_token) ||
       !step(a.k_tokens, a.v_token) || (a.n_k_tiles > 0 && !step(a.q_tokens, a.grad_out_token)))
     return set_error(FSP_EINVAL, who + ": a token's step must lie between dim and 2^23");
+  if (!isfinite((float)a.scale)) return set_error(FSP_EINVAL, who + ": scale must be finite in 32 bits");
   if (a.window && !a.causal) return set_error(FSP_EINVAL, who + ": window needs causal");
   if ((a.n_q_tiles > 0 && (!a.q_tiles || !a.q_halves || !a.q || !a.out || !a.lse)) ||
       (a.n_k_tiles > 0 && (!a.k_tiles || !a.k_halves)) || (a.k_tokens > 0 && (!a.k || !a.v)))

@@ -695,6 +695,8 @@ extern "C" int fsp_attention_paged(const fsp_attention_paged_args* args, void* s
   if (int rc = check_cache(a.cache, "fsp_attention_paged")) return rc;
   if (a.heads < 1 || a.heads % a.cache.kv_heads || a.heads > 0xffff)
     return set_error(FSP_EINVAL, "fsp_attention_paged: heads must be a multiple of kv_heads");
+  if (!isfinite((float)a.scale))
+    return set_error(FSP_EINVAL, "fsp_attention_paged: scale must be finite in 32 bits");
   if (a.window < 0 || a.window > 0x7fffffffLL)
     return set_error(FSP_EINVAL, "fsp_attention_paged: window");
   if (a.piece < 128 || a.piece > kPieceMost || a.piece % 128)

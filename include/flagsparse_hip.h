@@ -681,7 +681,7 @@ int fsp_run(const void* call, const void* in, void* out, void* stream);
  *
  * With S_ij = scale * q_i . k_j over the keys j that query i sees, lse_i = log sum_j exp(S_ij),
  * P_ij = exp(S_ij - lse_i): out_i = sum_j P_ij v_j.  A query that sees no key has out 0 and lse
- * minus infinity.
+ * minus infinity.  scale is finite in float32.
  */
 int64_t fsp_attention_dim_cap(void);
 

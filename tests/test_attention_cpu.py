@@ -286,3 +286,13 @@ def test_rows_have_steps_that_the_kernels_take(tokens, heads):
         assert torch.equal(r, t) and s[0] % 8 == 0 and s[1] % 8 == 0 and 64 <= s[0] <= 2**23
         if (tokens == 1 or s0 == 512) and (heads == 1 or s1 == 64):
             assert r is t  # no copy for a step that says nothing
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 1e39])
+def test_scales_of_the_library_are_finite(scale):
+    L = _abi.lib()
+    assert L.fsp_attention_packed(_packed(scale=scale), None) == -1
+    assert L.fsp_attention_packed_backward(_packed(scale=scale), None) == -1
+    assert L.fsp_attention_paged(_cache() + _paged(scale=scale), None) == -1
+    with pytest.raises(ValueError):
+        attention._scale_of(scale, 64)

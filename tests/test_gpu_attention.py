@@ -463,3 +463,15 @@ def test_one_token_of_a_wider_array(dev):
     want = ref.packed(q, k, v, [1], [1], True, None, d**-0.5, grad)
     for name, x in zip(("out", "lse", "q", "k", "v"), (out, lse, *grads)):
         ref.check(name, x, want[name])
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 1e39])
+def test_scales_that_are_not_finite(dev, scale):
+    q, k, v, g = _inputs(dev, [10], [10], 2, 2, 64, BF)
+    p = fs.prepare_attention_packed(_indptr([10], dev))
+    out, lse = fs.flagsparse_attention_packed(q, k, v, prepared=p, return_lse=True)
+    for _ in range(2):
+        with pytest.raises(ValueError):
+            fs.flagsparse_attention_packed(q, k, v, prepared=p, scale=scale)
+        with pytest.raises(ValueError):
+            fs.flagsparse_attention_packed_backward(g, q, k, v, out, lse, prepared=p, scale=scale)

@@ -565,3 +565,12 @@ def test_one_token_and_one_head_of_wider_arrays(dev):
     k, v = k[0].clone(), v[0].clone()
     k[-1], v[-1] = fused[0, h:h + g].cpu(), fused[0, h + g:].cpu()
     ref.check("out", out, _want(fused[:, :h], [k], [v], [n], None, d**-0.5)["out"])
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), 1e39])
+def test_scales_that_are_not_finite(dev, scale):
+    kp, vp, ip, ix, _, _ = _cache(dev, [20], 16, 2, 64, BF)
+    kv = fs.prepare_paged_kv(kp, vp, ip, ix)
+    q = torch.zeros(1, 4, 64, dtype=BF, device=dev)
+    with pytest.raises(ValueError):
+        fs.flagsparse_attention_paged(q, torch.tensor([20], device=dev), prepared=kv, scale=scale)
