@@ -22,6 +22,7 @@ import struct
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _abi
 from ._common import SUPPORTED_INDEX_DTYPES, _aligned
@@ -466,7 +467,8 @@ def flagsparse_attention_paged(q, lengths, *, prepared=None, k_pages=None, v_pag
     ``q``: [sequences, heads, dim]; ``lengths[b]``: the tokens that sequence b holds, the query's
     own among them (0: the sequence is empty, and its output is zeros).  ``window``: only the last
     ``window`` tokens are seen.  ``scale``: dim ** -0.5 by default.  Returns [sequences, heads, dim],
-    with the float32 log-sum-exp [sequences, heads] if ``return_lse``.  With ``prepared`` nothing is
+    with the float32 log-sum-exp [sequences, heads] if ``return_lse``; neither is differentiable, nor
+    is what flagsparse_paged_append gives.  With ``prepared`` nothing is
     waited for, so lengths are not checked: one that its sequence's pages cannot hold gives NaN."""
     key = None
     if out is None and type(prepared) is PreparedPagedKV and type(scale) in _PLAIN and \
@@ -668,6 +670,19 @@ def _tracked(t):
     return isinstance(t, torch.Tensor) and t.requires_grad
 
 
+def _has_tangent(*tensors):
+    """Whether one carries a tangent of forward-mode differentiation; no level open is the quick answer."""
+    if getattr(forward_ad, "_current_level", 0) < 0:
+        return False
+    return any(forward_ad.unpack_dual(t).tangent is not None for t in tensors
+               if isinstance(t, torch.Tensor))
+
+
+def _refuse_tangents(*tensors):
+    if _has_tangent(*tensors):
+        raise NotImplementedError("the gradient has no forward-mode derivative")
+
+
 def _run_forward(prepared, head, q, k, v, res, lse):
     if q.shape[0]:
         status = _abi.lib().fsp_attention_packed(head + _PACKED_AT.pack(
@@ -706,6 +721,7 @@ class _Differentiable(torch.autograd.Function):
     def backward(ctx, grad, _):
         q, k, v, out, lse = ctx.saved_tensors
         prepared, causal, window, scale = ctx.rest
+        _refuse_tangents(grad, q, k, v)
         grads = _backward(prepared, grad, q, k, v, out, lse, causal, window, scale)
         return *grads, None, None, None, None
 
@@ -720,13 +736,14 @@ def flagsparse_attention_packed(q, k, v, indptr=None, k_indptr=None, *, prepared
     j <= i + nk - nq, the last query all of them; ``window``: only the last ``window`` of those.
     ``scale``: dim ** -0.5 by default.  Returns [tokens, heads, dim], with the float32 log-sum-exp
     [tokens, heads] if ``return_lse``.  The output is differentiable with respect to q, k and v where
-    they require a gradient (the log-sum-exp is not).
+    they require a gradient (the log-sum-exp is not); forward-mode tangents raise NotImplementedError.
 
     What is not finite in k reaches the rows that see it.  In v it reaches those, and may reach rows of
     the same sequence and block of 64 keys that do not (their weight is zero, and zero times it is
     NaN), as it does in a product of the weights' matrix; it never reaches another sequence."""
     key = None
-    wanted = torch.is_grad_enabled() and (_tracked(q) or _tracked(k) or _tracked(v))
+    wanted = torch.is_grad_enabled() and (_tracked(q) or _tracked(k) or _tracked(v)) or \
+        _has_tangent(q, k, v)  # which _Differentiable refuses
     if out is None and not wanted and type(prepared) is PreparedAttention and \
             type(scale) in _PLAIN and type(window) in _PLAIN and type(causal) in _PLAIN:
         key = _layouts(q, k, v) + (causal, window, scale)
@@ -782,12 +799,14 @@ def _run_backward(prepared, kept, rows, lse, grads):
 def flagsparse_attention_packed_backward(grad_out, q, k, v, out, lse, indptr=None, k_indptr=None, *,
                                          prepared=None, causal=True, window=None, scale=None):
     """(grad_q, grad_k, grad_v) of flagsparse_attention_packed: ``grad_out`` is the gradient of its
-    output, ``out`` and ``lse`` what it returned, the other arguments its own.
+    output, ``out`` and ``lse`` what it returned, the other arguments its own.  The gradients are not
+    differentiable themselves.
 
     Sums are float32 and in a fixed order: equal calls give equal bits.  What is not finite may reach
     rows of the same sequence within 64 queries or keys of those that it belongs to, as in the
     forward pass; it never reaches another sequence."""
     key, rows = None, (grad_out, q, k, v, out)
+    _refuse_tangents(*rows, lse)
     if type(prepared) is PreparedAttention and type(scale) in _PLAIN and \
             type(window) in _PLAIN and type(causal) in _PLAIN:
         key = _layouts(*rows, lse) + (causal, window, scale)

@@ -296,3 +296,13 @@ def test_scales_of_the_library_are_finite(scale):
     assert L.fsp_attention_paged(_cache() + _paged(scale=scale), None) == -1
     with pytest.raises(ValueError):
         attention._scale_of(scale, 64)
+
+
+def test_tangents_are_seen():
+    t = torch.zeros(3)
+    assert not attention._has_tangent(t, None)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(t, torch.ones(3))
+        assert attention._has_tangent(t, dual) and not attention._has_tangent(t, None)
+        with torch.no_grad():
+            assert attention._has_tangent(dual)

@@ -475,3 +475,39 @@ def test_scales_that_are_not_finite(dev, scale):
             fs.flagsparse_attention_packed(q, k, v, prepared=p, scale=scale)
         with pytest.raises(ValueError):
             fs.flagsparse_attention_packed_backward(g, q, k, v, out, lse, prepared=p, scale=scale)
+
+
+def test_tangents_are_refused(dev):
+    # forward-mode derivatives have no kernel: an error, never an output without its tangent
+    q, k, v, _ = _inputs(dev, [10], [10], 2, 2, 64, BF)
+    p = fs.prepare_attention_packed(_indptr([10], dev))
+    for _ in range(2):
+        want = fs.flagsparse_attention_packed(q, k, v, prepared=p)
+    with torch.autograd.forward_ad.dual_level():
+        for which in range(3):
+            args = [torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)) if i == which else t
+                    for i, t in enumerate((q, k, v))]
+            with pytest.raises(NotImplementedError):
+                fs.flagsparse_attention_packed(*args, prepared=p)
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                fs.flagsparse_attention_packed(*args, prepared=p)
+        assert torch.equal(fs.flagsparse_attention_packed(q, k, v, prepared=p), want)
+
+
+def test_tangents_of_the_gradient_are_refused(dev):
+    q, k, v, g = _inputs(dev, [10], [10], 2, 2, 64, BF)
+    p = fs.prepare_attention_packed(_indptr([10], dev))
+    out, lse = fs.flagsparse_attention_packed(q, k, v, prepared=p, return_lse=True)
+    args = [g, q, k, v, out, lse]
+    for _ in range(2):
+        fs.flagsparse_attention_packed_backward(*args, prepared=p)
+    leaf = q.clone().requires_grad_()
+    res = fs.flagsparse_attention_packed(leaf, k, v, prepared=p)
+    with torch.autograd.forward_ad.dual_level():
+        for i, t in enumerate(args):
+            dual = torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+            with pytest.raises(NotImplementedError):
+                fs.flagsparse_attention_packed_backward(*args[:i], dual, *args[i + 1:], prepared=p)
+        dual = torch.autograd.forward_ad.make_dual(g, torch.ones_like(g))
+        with pytest.raises(NotImplementedError):
+            torch.autograd.grad(res, leaf, dual)
