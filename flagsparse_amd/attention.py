@@ -249,8 +249,18 @@ class PreparedPagedKV:
         self._streams = _Streams()
         self._calls = _abi.Calls()
 
+    def _where(self):
+        """Where the pages lie.  Their storage is the caller's and may move (resized, or another one
+        behind the same tensors): kept argument blocks are looked up by it too."""
+        return self.k_pages.data_ptr(), self.v_pages.data_ptr()
+
     def _packed(self):
         k, v = self.k_pages, self.v_pages
+        for t, name in ((k, "k_pages"), (v, "v_pages")):
+            _check_pages(t, name)
+            if t.dtype != self.dtype or t.device != self.device or \
+                    t.shape != (self.n_pages, self.page_size, self.kv_heads, self.dim):
+                raise ValueError(f"{name} are not what was prepared: prepare the cache anew")
         return _CACHE.pack(_CODES[k.dtype], self.kv_heads, self.dim, self.page_size, self.n_pages,
                            self.batch, self.indices.numel(), k.data_ptr(), *_steps(k), v.data_ptr(),
                            *_steps(v), self.indptr.data_ptr(), self.indices.data_ptr())
@@ -381,7 +391,7 @@ def flagsparse_paged_append(k, v, lengths, token_indptr=None, *, prepared=None, 
     negative or past its sequence's pages is not stored and its row of ``q`` comes back as NaN."""
     key = None
     if out is None and type(prepared) is PreparedPagedKV:
-        key = _layouts(k, v, q, cos, sin, lengths, token_indptr) + (bool(interleaved),)
+        key = _layouts(k, v, q, cos, sin, lengths, token_indptr) + (bool(interleaved), prepared._where())
         kept = prepared._calls.get(key)
         if kept is not None and not (k.data_ptr() | v.data_ptr()) % 16 and (
                 q is None or q.data_ptr() % 16 == 0):
@@ -473,7 +483,7 @@ def flagsparse_attention_paged(q, lengths, *, prepared=None, k_pages=None, v_pag
     key = None
     if out is None and type(prepared) is PreparedPagedKV and type(scale) in _PLAIN and \
             type(window) in _PLAIN:
-        key = _layouts(q, lengths) + (scale, window)
+        key = _layouts(q, lengths) + (scale, window, prepared._where())
         kept = prepared._calls.get(key)
         if kept is not None and q.data_ptr() % 16 == 0:
             res = torch.empty_like(kept[1], memory_format=_CONTIGUOUS)

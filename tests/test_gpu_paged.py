@@ -574,3 +574,31 @@ def test_scales_that_are_not_finite(dev, scale):
     q = torch.zeros(1, 4, 64, dtype=BF, device=dev)
     with pytest.raises(ValueError):
         fs.flagsparse_attention_paged(q, torch.tensor([20], device=dev), prepared=kv, scale=scale)
+
+
+def test_pages_whose_storage_moves(dev):
+    # the tensors are the caller's: what they hold at the time of a call is what is read and written
+    lengths = [300, 50]
+    kp, vp, ip, ix, k, v = _cache(dev, lengths, 16, 2, 64, BF)
+    kv = fs.prepare_paged_kv(kp, vp, ip, ix)
+    n = torch.tensor(lengths, device=dev)
+    q = _normal(99, 2, 4, 64, dtype=BF).to(dev)
+    new = _normal(98, 2, 2, 64, dtype=BF).to(dev)
+    for _ in range(2):
+        fs.flagsparse_paged_append(new, new, n, prepared=kv)
+        fs.flagsparse_attention_paged(q, n, prepared=kv)
+    old = kp.detach(), vp.detach()  # keeps the old storage
+    kp.data, vp.data = kp * 2, vp * 0.5
+    before = [t.clone() for t in old]
+    k, v = [t * 2 for t in k], [t * 0.5 for t in v]
+    for b in range(2):
+        k[b][-1] = v[b][-1] = new[b].cpu() * 4
+    for _ in range(2):
+        fs.flagsparse_paged_append(new * 4, new * 4, n, prepared=kv)
+        out = fs.flagsparse_attention_paged(q, n, prepared=kv)
+        ref.check("out", out, _want(q, k, v, lengths, None, 0.125)["out"])
+    for a, b in zip(old, before):
+        assert torch.equal(a.nan_to_num(), b.nan_to_num())
+    kp.data = kp[:-1]
+    with pytest.raises(ValueError):
+        fs.flagsparse_attention_paged(q, n, prepared=kv, scale=0.5)
