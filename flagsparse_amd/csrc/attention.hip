@@ -352,6 +352,36 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_packed_kerne
 template <typename T> struct Lift { static constexpr float up = 0, down = 1; };
 template <> struct Lift<f16> { static constexpr float up = 14, down = 1.0f / 16384; };
 
+// Gradients far from 1 in float16: dS is rounded as 2^n times itself, with an n of the lane's query (or
+// key) that falls whenever 2^n dS would pass kHighest, and the sums fall with it; so that its largest
+// elements lie between 2^11 and 2^15, whatever the size of grad_out and v, and what float16 holds with
+// fewer bits is 2^25 times smaller.  As it is, dS of 2048 keys and a grad_out of 2^-13 lies below
+// float16's normal numbers (grad_k off by 28 times the bound that one rounding gives), and that of large
+// gradients past its largest.  Without and with it, us, forward and backward: two sequences of
+// 4096, 32 heads of 128 over 8 1271 / 1314; 12 ragged ones, window 1024, 16 heads of 64 over 4 104 / 112;
+// 7 short ones, 12 heads of 96 42.7 / 46.0.
+constexpr int kRaise = 60;  // n to begin with: 2^n dS is a float32 for all float16 inputs
+constexpr float kHighest = 32768.0f;
+
+// By how much n falls (0 most of the time) for 16 of a lane's elements and those of its other half.
+template <int NT>
+__device__ __forceinline__ int lower(f32x16& y, f32x16 (&acc)[NT]) {
+  // what is masked is zero by now: chosen later, 16 masks would be kept until then
+  asm volatile("" : "+v"(y));
+  float m = 0;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) m = fmaxf(m, fabsf(y[r]));
+  if (!__any(m > kHighest)) return 0;
+  m = fmaxf(m, other_half(m));
+  // what is not finite stays so
+  const int by = m > kHighest && m < INFINITY ? __builtin_amdgcn_frexp_expf(m) - 12 : 0;
+  const float f = ldexpf(1.0f, -by);
+  y *= f;
+#pragma unroll
+  for (int i = 0; i < NT; ++i) acc[i] *= f;
+  return by;
+}
+
 // Query tiles that see at most so many keys make delta anew.  Error of the queries' gradient against 64
 // bits over that of one rounding (bfloat16, 12 packed sequences up to 2500; two of 4096): 1.59 and 1.50
 // without, 1.47 and 1.45 with it, 1.45 and 1.44 with 256 keys; backward of 30 sequences of 200, 32 heads
@@ -497,6 +527,9 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, DP <= 64 ? 3 : 2) void attenti
     stats[(s.heads + a) * q_tokens + row] = -delta;
   }
 
+  constexpr bool RAISED = std::is_same<T, f16>::value;
+  int n = RAISED ? kRaise : 0;
+  base -= n;
   walk([&](int j0, const lds_char* sk, const lds_char* sv) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -507,6 +540,11 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, DP <= 64 ? 3 : 2) void attenti
       for (int r = 0; r < 16; ++r)
         x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], c, -base)) * (y[r] - delta);
       hide(j0, u, x);
+      if constexpr (RAISED) {
+        const int by = lower(x, acc);
+        base += by;
+        n -= by;
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const V8<T> f = to16<T>(x, 8 * i);
@@ -516,6 +554,10 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, DP <= 64 ? 3 : 2) void attenti
       }
     }
   });
+  if constexpr (RAISED) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) acc[i] *= ldexpf(1.0f, -n);
+  }
   if constexpr (PARTS > 1) {
     float* theirs = reinterpret_cast<float*>(block == 0   ? s_k0
                                              : block == 1 ? s_v0
@@ -581,9 +623,8 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_grad_kv_kern
   }
   const float c = exp2_scale(s.scale);
 
-  // the queries that see this lane's key, those that see any of the wave's and of the tile's
-  int lo, hi, lo0, hi0, lo1, hi1, lot, hit, none;
-  seen_of(s, t, t.at + min(mine, t.rows - 1), lo, hi);
+  // the queries that see any of the wave's keys and of the tile's
+  int lo0, hi0, lo1, hi1, lot, hit, none;
   seen_of(s, t, t.at + min(k0, t.rows - 1), lo0, hi0);
   seen_of(s, t, t.at + min(k0 + 31, t.rows - 1), lo1, hi1);
   seen_of(s, t, t.at, lot, none);
@@ -592,6 +633,9 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_grad_kv_kern
   f32x16 ak[NT], av[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) ak[i] = av[i] = f32x16{};
+
+  constexpr bool RAISED = std::is_same<T, f16>::value;
+  float raised = RAISED ? ldexpf(Lift<T>::down, kRaise) : 1.0f;  // 2^n, and P's lift taken back
 
   const int r_at = L::row_at(lane) + part * 32 * L::PITCH;
   const int c_at = L::col_at(lane) + part * 32 * L::PITCH;
@@ -639,9 +683,12 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_grad_kv_kern
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       x[r] = __builtin_amdgcn_exp2f(x[r] * c);
-      y[r] *= x[r] * Lift<T>::down;
+      y[r] *= x[r] * raised;
     }
     if (i1 + 32 > hi0 || i1 < lo1) {
+      int key = mine, lo, hi;  // what sees this lane's key: made anew, as above
+      asm volatile("" : "+v"(key));
+      seen_of(s, t, t.at + min(key, t.rows - 1), lo, hi);
       const int first = lo - i1 - 4 * half, last = hi - i1 - 4 * half;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -651,6 +698,7 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_grad_kv_kern
         y[r] = in ? y[r] : 0.0f;
       }
     }
+    if constexpr (RAISED) raised = ldexpf(raised, -lower(y, ak));
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const V8<T> p = to16<T>(x, 8 * i), ds = to16<T>(y, 8 * i);
@@ -690,6 +738,10 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_grad_kv_kern
     ++n;
   }
 
+  if constexpr (RAISED) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) ak[i] *= Lift<T>::down / raised;
+  }
   // join the waves of the same keys
   float* joined = reinterpret_cast<float*>(block ? s_q1 : s_q0);
   static_assert((PARTS - 1) * 16 * 64 * 4 <= BYTES, "");

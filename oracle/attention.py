@@ -60,8 +60,10 @@ def one(q, k, v, mask, scale, grad=None):
     return r
 
 
-def packed(q, k, v, q_len, k_len, causal, window, scale, grad=None):
-    """Every sequence and head: {name: (value, bound)} in float64 on the CPU, in q's type's bounds."""
+def packed(q, k, v, q_len, k_len, causal, window, scale, grad=None, small=1.0):
+    """Every sequence and head: {name: (value, bound)} in float64 on the CPU, in q's type's bounds.
+    ``small``: what the type's smallest steps may cost an operand, in units of tiny; a kernel that
+    multiplies its weights by 2^n before it rounds them has 2^-n."""
     u, tiny = U[q.dtype], TINY[q.dtype]
     h, g = q.shape[1], k.shape[1]
     q, k, v = (t.detach().cpu().double() for t in (q, k, v))
@@ -83,20 +85,20 @@ def packed(q, k, v, q_len, k_len, causal, window, scale, grad=None):
             size = float(r["size"])
             res["out"][0][a, x], res["lse"][0][a, x] = r["out"], r["lse"]
             res["out"][1][a, x] = (u + f * size) * r["abs_out"] + u * r["out"].abs() + \
-                tiny * (1 + v[b, y].abs().sum(0))
+                tiny * (1 + small * v[b, y].abs().sum(0))
             res["lse"][1][a, x] = f * size
             if grad is None:
                 continue
             res["q"][0][a, x] = r["q"]
             res["q"][1][a, x] = u * (r["q"].abs() + r["abs_q"] + r["rough_q"]) + \
-                f * size * (r["abs_q"] + r["sums_q"]) + tiny * (1 + r["all_q"])
+                f * size * (r["abs_q"] + r["sums_q"]) + tiny * (1 + small * r["all_q"])
             if nk:
                 # rounded once over the group: its own rounding is added below
                 res["k"][0][b, y] += r["k"]
                 res["v"][0][b, y] += r["v"]
                 res["k"][1][b, y] += u * (r["abs_k"] + r["rough_k"]) + \
-                    f * size * (r["abs_k"] + r["sums_k"]) + tiny * (1 + r["all_k"])
-                res["v"][1][b, y] += (u + f * size) * r["abs_v"] + tiny * (1 + r["all_v"])
+                    f * size * (r["abs_k"] + r["sums_k"]) + tiny * (1 + small * r["all_k"])
+                res["v"][1][b, y] += (u + f * size) * r["abs_v"] + tiny * (1 + small * r["all_v"])
         tq, tk = tq + nq, tk + nk
     if grad is not None:
         for n in ("k", "v"):

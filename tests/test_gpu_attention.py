@@ -511,3 +511,24 @@ def test_tangents_of_the_gradient_are_refused(dev):
         dual = torch.autograd.forward_ad.make_dual(g, torch.ones_like(g))
         with pytest.raises(NotImplementedError):
             torch.autograd.grad(res, leaf, dual)
+
+
+@pytest.mark.parametrize("lengths,heads,kv_heads,dim", [([2048], 2, 1, 64), ([700] * 4, 16, 8, 128),
+                                                        ([300, 65], 4, 2, 40)])
+@pytest.mark.parametrize("gain,v_gain", [(2.0**-13, 1.0), (2.0**-10, 1.0), (1000.0, 30.0)])
+def test_small_and_large_gradients_in_float16(dev, gain, v_gain, lengths, heads, kv_heads, dim):
+    # dS lies far from 1: below float16's normal numbers, or past its largest, while the gradient
+    # that is looked at lies among them, by a large q beside a small k or the other way round.
+    # Scores do not change with it, nor does dS
+    print(f"gradients times {gain} {v_gain} {lengths} {heads} {kv_heads} {dim}", flush=True)
+    q, k, v, g = _inputs(dev, lengths, lengths, heads, kv_heads, dim, HF)
+    v, g = (v * v_gain).to(HF), (g.float() * gain).to(HF)
+    p = fs.prepare_attention_packed(_indptr(lengths, dev))
+    for up, names in ((64.0, "k" if gain < 1 else "q"), (1 / 64.0, "q" if gain < 1 else "k")):
+        a, b = (q.float() * up).to(HF), (k.float() / up).to(HF)
+        out, lse = fs.flagsparse_attention_packed(a, b, v, prepared=p, return_lse=True)
+        grads = dict(zip("qkv", fs.flagsparse_attention_packed_backward(g, a, b, v, out, lse,
+                                                                        prepared=p)))
+        want = ref.packed(a, b, v, lengths, lengths, True, None, dim**-0.5, g, small=0.0)
+        for name in names + "v":
+            ref.check(name, grads[name], want[name])
