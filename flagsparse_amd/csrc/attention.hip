@@ -163,7 +163,7 @@ __device__ __forceinline__ void store_rows(T* to, const f32x16 (&x)[NT], float f
 }
 
 // out = sum_j w_j v_j / sum_j w_j with w_j = exp2(c q . k_j - m), m a maximum of the row that follows it
-// within a factor of 2^8.  With S^T = K Q^T a query is a lane: its maximum and sum are its own (and
+// (Weights).  With S^T = K Q^T a query is a lane: its maximum and sum are its own (and
 // the other half's, 32 lanes on), and its weights are the operand of O^T = V^T P^T where they lie, in
 // registers.  Keys and values go straight to LDS, the next step's while this one is worked on; weights
 // are rounded to the inputs' type for the second product, as its operands have to be, and all sums
@@ -267,8 +267,7 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_packed_kerne
 #pragma unroll
       for (int r = 0; r < 16; ++r) m = fmaxf(m, x[u][r]);
     m = fmaxf(m, other_half(m));
-    // The weights are taken against an older maximum until a row's grows by more than 2^8 of it
-    if (__any((m - top) * c > 8.0f)) {
+    if (__any((m - top) * c > Weights<T>::lag)) {
       const float now = fmaxf(top, m);
       const float fade = top == -INFINITY ? 0.0f : exp2f((top - now) * c);
       top = now;
@@ -276,7 +275,7 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_packed_kerne
 #pragma unroll
       for (int i = 0; i < NT; ++i) o[i] *= fade;
     }
-    const float base = top == -INFINITY ? 0.0f : top * c;
+    const float base = top == -INFINITY ? 0.0f : top * c - Weights<T>::up;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -340,7 +339,9 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_packed_kerne
   if (mine >= t.rows) return;
   const int64_t row = t.first + mine;
   const float inv = sum > 0 ? 1.0f / sum : (sum == 0 ? 0.0f : sum);
-  if (half == 0) lse[row * s.heads + a] = sum == 0 ? -INFINITY : (top * c + log2f(sum)) * kLn2;
+  if (half == 0)
+    lse[row * s.heads + a] =
+        sum == 0 ? -INFINITY : (top * c + log2f(sum * Weights<T>::down)) * kLn2;
   if (sum == 0)  // nothing seen: zeros, whatever lies in the rows of V
 #pragma unroll
     for (int i = 0; i < NT; ++i) o[i] = f32x16{};

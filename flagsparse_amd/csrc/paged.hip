@@ -336,8 +336,7 @@ __global__ __launch_bounds__(256, 3) void attention_paged_kernel(
     float m = x[0][0];
 #pragma unroll
     for (int e = 1; e < 8; ++e) m = fmaxf(m, x[e / 4][e % 4]);
-    // the weights are taken against an older maximum until a head's grows by more than 2^8 of it
-    if (__any((m - top) * cs > 8.0f)) {
+    if (__any((m - top) * cs > Weights<T>::lag)) {
       m = fmaxf(m, __shfl_xor(m, 16));
       m = fmaxf(m, __shfl_xor(m, 32));
       const float now = fmaxf(top, m);
@@ -347,7 +346,7 @@ __global__ __launch_bounds__(256, 3) void attention_paged_kernel(
 #pragma unroll
       for (int i = 0; i < E; ++i) o[i] *= fade;
     }
-    const float base = top == -INFINITY ? 0.0f : top * cs;
+    const float base = top == -INFINITY ? 0.0f : top * cs - Weights<T>::up;
     f32x8 p;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -368,7 +367,7 @@ __global__ __launch_bounds__(256, 3) void attention_paged_kernel(
   // join the waves
   sum += __shfl_xor(sum, 16);
   sum += __shfl_xor(sum, 32);
-  const float ml = top == -INFINITY ? -INFINITY : top * cs;
+  const float ml = top == -INFINITY ? -INFINITY : top * cs;  // of all sums alike, 2^up is left in them
   if (quad == 0) s_ml[wave][col] = f32x2{ml, sum};
 #pragma unroll
   for (int i = 0; i < E; ++i)
@@ -410,7 +409,7 @@ __global__ __launch_bounds__(256, 3) void attention_paged_kernel(
           __builtin_convertvector(y, V4<T>);
       if (lse && d == 0)
         lse[(int64_t)b * s.heads + head0 + h] =
-            !ok ? nan : total == 0 ? -INFINITY : (most + log2f(total)) * kLn2;
+            !ok ? nan : total == 0 ? -INFINITY : (most + log2f(total * Weights<T>::down)) * kLn2;
     }
   }
   if (!split || !arrived) return;  // without counts, another launch joins them
@@ -464,7 +463,7 @@ __global__ __launch_bounds__(256, 3) void attention_paged_kernel(
         __builtin_convertvector(y, V4<T>);
     if (lse && d == 0)
       lse[(int64_t)b * s.heads + head0 + h] =
-          total == 0 ? -INFINITY : (most + log2f(total)) * kLn2;
+          total == 0 ? -INFINITY : (most + log2f(total * Weights<T>::down)) * kLn2;
   }
 }
 
@@ -542,7 +541,8 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(
     *reinterpret_cast<V4<T>*>(out + b * out_token + h * out_head + d) =
         __builtin_convertvector(y, V4<T>);
   if (lse && d == 0)
-    lse[(int64_t)b * s.heads + h] = total == 0 ? -INFINITY : (most + log2f(total)) * kLn2;
+    lse[(int64_t)b * s.heads + h] =
+        total == 0 ? -INFINITY : (most + log2f(total * Weights<T>::down)) * kLn2;
 }
 
 int check_cache(const fsp_paged_cache& c, const std::string& who) {

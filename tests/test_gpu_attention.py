@@ -532,3 +532,18 @@ def test_small_and_large_gradients_in_float16(dev, gain, v_gain, lengths, heads,
         want = ref.packed(a, b, v, lengths, lengths, True, None, dim**-0.5, g, small=0.0)
         for name in names + "v":
             ref.check(name, grads[name], want[name])
+
+
+def test_one_key_above_all_others_in_float16(dev):
+    # a key that outweighs the others by 16 e-folds and has a value of zero: the output is what the
+    # others' small weights leave of it.  Weights are rounded as 2^11 times themselves
+    n, h, d = 4096, 2, 64
+    q = torch.zeros(3, h, d, dtype=HF)
+    q[..., 0] = 16.0
+    k = torch.zeros(n, h, d, dtype=HF)
+    k[..., 0] = -8.0
+    v = _normal(1, n, h, d, dtype=HF, dev="cpu").abs()
+    k[77], v[77] = 0.0, 0.0
+    q, k, v = (t.to(dev) for t in (q, k, v))
+    out = fs.flagsparse_attention_packed(q, k, v, _indptr([3], dev), _indptr([n], dev), causal=False)
+    ref.check("out", out, ref.packed(q, k, v, [3], [n], False, None, d**-0.5, small=2.0**-11)["out"])

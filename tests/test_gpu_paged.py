@@ -602,3 +602,20 @@ def test_pages_whose_storage_moves(dev):
     kp.data = kp[:-1]
     with pytest.raises(ValueError):
         fs.flagsparse_attention_paged(q, n, prepared=kv, scale=0.5)
+
+
+def test_one_key_above_all_others_in_float16(dev):
+    # as with packed sequences: weights are rounded as 2^11 times themselves
+    n, g, h, d, page = 250, 1, 2, 64, 16
+    q = torch.zeros(1, h, d, dtype=HF)
+    q[..., 0] = 16.0
+    k = torch.zeros(n, g, d, dtype=HF)
+    k[..., 0] = -8.0
+    v = _normal(1, n, g, d, dtype=HF).abs()
+    k[77], v[77] = 0.0, 0.0
+    kp, vp = (torch.zeros(16, page, g, d, dtype=HF) for _ in range(2))
+    kp.view(-1, g, d)[:n], vp.view(-1, g, d)[:n] = k, v
+    out = fs.flagsparse_attention_paged(
+        q.to(dev), torch.tensor([n], device=dev), k_pages=kp.to(dev), v_pages=vp.to(dev),
+        indptr=torch.tensor([0, 16], device=dev), indices=torch.arange(16, device=dev))
+    ref.check("out", out, ref.packed(q, k, v, [1], [n], True, None, d**-0.5, small=2.0**-11)["out"])
