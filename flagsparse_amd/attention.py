@@ -44,7 +44,8 @@ _PAGED, _PAGED_AT = struct.Struct("6qd4q"), struct.Struct("6q")
 _PACKED, _PACKED_AT = struct.Struct("10qd24q"), struct.Struct("10q")
 
 # A prepared object keeps the first part for each layout of arrays that it has checked, so that the
-# next call with such arrays is a look-up and a launch.
+# next call with such arrays is a look-up and a launch.  Of a cache it holds the pages' addresses, which
+# the look-up goes by too: their storage is the caller's, and may move.
 _KEPT_LAYOUTS = 64
 _PLAIN = (type(None), bool, int, float)  # the settings a layout is kept with, by their values
 
@@ -249,11 +250,6 @@ class PreparedPagedKV:
         self._streams = _Streams()
         self._calls = _abi.Calls()
 
-    def _where(self):
-        """Where the pages lie.  Their storage is the caller's and may move (resized, or another one
-        behind the same tensors): kept argument blocks are looked up by it too."""
-        return self.k_pages.data_ptr(), self.v_pages.data_ptr()
-
     def _packed(self):
         k, v = self.k_pages, self.v_pages
         for t, name in ((k, "k_pages"), (v, "v_pages")):
@@ -391,7 +387,8 @@ def flagsparse_paged_append(k, v, lengths, token_indptr=None, *, prepared=None, 
     negative or past its sequence's pages is not stored and its row of ``q`` comes back as NaN."""
     key = None
     if out is None and type(prepared) is PreparedPagedKV:
-        key = _layouts(k, v, q, cos, sin, lengths, token_indptr) + (bool(interleaved), prepared._where())
+        key = _layouts(k, v, q, cos, sin, lengths, token_indptr) + (
+            bool(interleaved), prepared.k_pages.data_ptr(), prepared.v_pages.data_ptr())
         kept = prepared._calls.get(key)
         if kept is not None and not (k.data_ptr() | v.data_ptr()) % 16 and (
                 q is None or q.data_ptr() % 16 == 0):
@@ -483,7 +480,8 @@ def flagsparse_attention_paged(q, lengths, *, prepared=None, k_pages=None, v_pag
     key = None
     if out is None and type(prepared) is PreparedPagedKV and type(scale) in _PLAIN and \
             type(window) in _PLAIN:
-        key = _layouts(q, lengths) + (scale, window, prepared._where())
+        key = _layouts(q, lengths) + (scale, window, prepared.k_pages.data_ptr(),
+                                      prepared.v_pages.data_ptr())
         kept = prepared._calls.get(key)
         if kept is not None and q.data_ptr() % 16 == 0:
             res = torch.empty_like(kept[1], memory_format=_CONTIGUOUS)
