@@ -800,7 +800,7 @@ template <typename T>
 const T* in(const void* p) { return static_cast<const T*>(p); }
 
 Shape shape_of(const fsp_attention_packed_args& a) {
-  return {(int)a.heads, (int)a.kv_heads, (int)a.dim, (int)a.causal, (int)a.window,
+  return {(int)a.heads, (int)a.kv_heads, (int)a.dim, a.causal != 0, (int)a.window,
           (float)a.scale};
 }
 

@@ -573,7 +573,7 @@ int launch_append(const fsp_paged_append_args& a, hipStream_t st) {
   if (parts > steps) parts = steps;
   const AppendShape s{a.n_tokens, a.k_token, a.k_head,    a.v_token,         a.v_head,           a.q_token,
                       a.q_head,   a.q_out_token, a.q_out_head, (int)a.heads, (int)a.half, (int)a.table_rows,
-                      (int)a.interleaved, (int)parts};
+                      a.interleaved != 0, (int)parts};
   constexpr int kWaves = kAppendThreads / kWave;
   hipLaunchKernelGGL((paged_append_kernel<T, MODE>),
                      dim3((unsigned)((a.n_tokens * parts + kWaves - 1) / kWaves)),

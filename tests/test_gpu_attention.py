@@ -547,3 +547,19 @@ def test_one_key_above_all_others_in_float16(dev):
     q, k, v = (t.to(dev) for t in (q, k, v))
     out = fs.flagsparse_attention_packed(q, k, v, _indptr([3], dev), _indptr([n], dev), causal=False)
     ref.check("out", out, ref.packed(q, k, v, [3], [n], False, None, d**-0.5, small=2.0**-11)["out"])
+
+
+def test_flags_of_the_library_are_not_cut_to_32_bits(dev):
+    from flagsparse_amd import _abi, attention
+
+    q, k, v, _ = _inputs(dev, [100], [100], 2, 2, 64, BF)
+    p = fs.prepare_attention_packed(_indptr([100], dev))
+    want, lse = fs.flagsparse_attention_packed(q, k, v, prepared=p, return_lse=True)
+    out = torch.empty_like(q)
+    head = list(attention._PACKED.unpack(attention._pack(p, q, k, v, True, 0, 0.125, out)))
+    assert head[8] == 1
+    head[8] = 1 << 32
+    args = attention._PACKED.pack(*head) + attention._PACKED_AT.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, 0)
+    _abi.check(_abi.lib().fsp_attention_packed(args, p._on()), "fsp_attention_packed")
+    assert torch.equal(out, want)
