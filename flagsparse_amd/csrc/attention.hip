@@ -6,7 +6,7 @@ namespace {
 
 constexpr int kTile = 128;  // query rows of a workgroup, 32 a wave
 
-constexpr int64_t kTokenStep = 1 << 23;  // 64 rows' bytes are a 32-bit offset
+constexpr int64_t kTokenStep = 1 << 23;  // the bytes of a load's 128 rows are a 32-bit offset
 
 struct Tile {
   int first, rows, at, q_begin, nq, k_begin, nk, pad;

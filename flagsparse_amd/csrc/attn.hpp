@@ -1,4 +1,4 @@
-// What the attention kernels share: the 16-bit types, wave reductions, argument checks.
+// What the attention kernels share: the 16-bit types, matrix products, argument checks.
 #pragma once
 
 #include <hip/hip_bf16.h>
@@ -103,18 +103,6 @@ __device__ __forceinline__ V8<T> scaled_sign(V8<T> q, float scale, bool in) {
 
 __device__ __forceinline__ float exp2_scale(float scale) {
   return fabsf(scale) > kNoScale ? fabsf(scale) * kLog2e : 1.0f;
-}
-
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-  return v;
-}
-
-__device__ __forceinline__ float wave_add(float v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  return v;
 }
 
 inline bool aligned16(const void* p, int64_t a, int64_t b) {
