@@ -563,3 +563,19 @@ def test_flags_of_the_library_are_not_cut_to_32_bits(dev):
         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, 0)
     _abi.check(_abi.lib().fsp_attention_packed(args, p._on()), "fsp_attention_packed")
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("which", ["q", "k", "v", "qk", "qv", "kv"])
+def test_gradients_of_some_inputs(dev, which):
+    lengths = [100, 31]
+    arrays = dict(zip("qkvg", _inputs(dev, lengths, lengths, 4, 2, 64, BF)))
+    g = arrays.pop("g")
+    p = fs.prepare_attention_packed(_indptr(lengths, dev))
+    out, lse = fs.flagsparse_attention_packed(*arrays.values(), prepared=p, return_lse=True)
+    want = fs.flagsparse_attention_packed_backward(g, *arrays.values(), out, lse, prepared=p)
+    leaves = {n: t.clone().requires_grad_(n in which) for n, t in arrays.items()}
+    res, stat = fs.flagsparse_attention_packed(*leaves.values(), prepared=p, return_lse=True)
+    assert torch.equal(res, out) and torch.equal(stat, lse) and not stat.requires_grad
+    res.backward(g)
+    for (n, t), w in zip(leaves.items(), want):
+        assert torch.equal(t.grad, w) if n in which else t.grad is None

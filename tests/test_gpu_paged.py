@@ -619,3 +619,13 @@ def test_one_key_above_all_others_in_float16(dev):
         q.to(dev), torch.tensor([n], device=dev), k_pages=kp.to(dev), v_pages=vp.to(dev),
         indptr=torch.tensor([0, 16], device=dev), indices=torch.arange(16, device=dev))
     ref.check("out", out, ref.packed(q, k, v, [1], [n], True, None, d**-0.5, small=2.0**-11)["out"])
+
+
+@pytest.mark.parametrize("lengths", [[900, 3, 2000, 77], [7000, 1, 520]])
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(33, 1, 72, HF), (40, 2, 40, BF), (23, 1, 80, HF),
+                                                      (6, 2, 120, BF), (64, 2, 128, HF), (4, 4, 8, BF)])
+def test_pieces_of_odd_heads_and_dims(dev, heads, kv_heads, dim, dtype, lengths):
+    # several pieces a sequence, joined by the last of them to arrive or by another launch, with head
+    # tiles that are not full, several to a key head, and dims that fill no tile
+    _decode(dev, lengths, 16, heads, kv_heads, dim, dtype)
+    _decode(dev, lengths, 16, heads, kv_heads, dim, dtype, window=600, room=3)
