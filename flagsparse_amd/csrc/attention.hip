@@ -173,12 +173,13 @@ __device__ __forceinline__ void store_rows(T* to, const f32x16 (&x)[NT], float f
 // PARTS = 2 two waves share the queries, and their sums are joined at the end: half the chain of
 // steps (share_queries, halve_tiles).
 //
-// At full fill bound by the matrix cores' rate at the power that they are given: 16384 tokens, 16 heads of
-// 128 over 2, causal, 1.1e12 operations in 1010 to 1030 us, 1.08 PFLOP/s at 1.75 to 1.95 GHz, where a
-// library's 8192^3 product reaches 1.2; neither LDS (no bank conflicts) nor memory (0.36 GB) holds it
-// up.  Two heads a workgroup over the same keys, or four buffers in turn, were no faster (284 / 289,
-// 279 / 282 us).  16 ragged prompts of up to 2047, 32 heads over 8: 82 us, 0.69 PFLOP/s: short loops
-// between the first loads and the last stores.
+// 16384 tokens, 16 heads of 128 over 2, causal: 1.1e12 operations in 990 to 1030 us, 1.07 to 1.11 PFLOP/s,
+// where a library's 8192^3 product reaches 1.21.  Products take 62 % of the SIMDs' cycles, vector
+// instructions 46 %, both at a time 23 %: the two mostly follow each other, at the clock that their power
+// leaves (1.75 GHz); neither LDS (no bank conflicts) nor memory (0.36 GB) holds it up.  Two heads a workgroup
+// over the same keys, or four buffers in turn, were no faster (284 / 289, 279 / 282 us).  16 ragged prompts
+// of up to 2047, 32 heads over 8: 82 us, 0.69 PFLOP/s: short loops between the first loads and the last
+// stores, 38 % of the cycles with neither.
 template <typename T, int DP, int BLOCKS, int PARTS>
 __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_packed_kernel(
     Shape s, const Tile* __restrict__ tiles, int n_tiles, const T* __restrict__ q, int64_t q_token,

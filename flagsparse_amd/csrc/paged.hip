@@ -176,12 +176,13 @@ __device__ __forceinline__ void all_stored() {
 // Where each key lies (its page, its place in it) is found once for the piece and kept in LDS.
 constexpr int kHeadTile = 16;
 constexpr int kPieceMost = 1024;
-// The workgroup that finishes a sequence joins its pieces where they are at most so many and the
-// workgroups no more than a few rounds of the chip's (three to a CU): each waits for its stores, which
-// in many rounds holds up those that follow.  Else a second launch does.  By a second launch and so, us: 1000 tokens, 16 heads of 64 11.9 / 8.7 a
-// call, both bound by the host (8.4 / 9.2 in a graph); 96 ragged sequences of up to 4096, 8 heads of
-// 128 (1344 workgroups) 49.5 / 44.6; 200 of 2048, 16 heads of 64 (6400) 263 / 283; 400 of 1500, 8 heads
-// of 128 (6400) 418 / 408.  Up to 27 pieces 15.7 / 20.7 (2 of 6760, 8 heads), up to 128 542 / 560.
+// The workgroup that finishes a sequence joins its pieces where they are at most so many and the workgroups
+// no more than a few rounds of the chip's (three to a CU): each waits for its stores, which in many rounds
+// holds up those that follow.  Else a second launch does.  By a second launch and so, us: 1000 tokens, 16
+// heads of 64 11.9 / 8.7 a call, both bound by the host (8.4 / 9.2 in a graph, whose replays zero the
+// counts); 96 ragged sequences of up to 4096, 8 heads of 128 (1344 workgroups) 49.5 / 44.6; 200 of 2048, 16
+// heads of 64 (6400) 263 / 283; 400 of 1500, 8 heads of 128 (6400) 418 / 408.  Up to 27 pieces 15.7 / 20.7 (2
+// of 6760, 8 heads), up to 128 542 / 560.
 constexpr int kJoinMost = 8;
 constexpr int kJoinBlocks = 8 * 256;
 
@@ -212,7 +213,7 @@ struct PagedShape {
 // has DP elements.  NT: loads that do not claim a place in the caches.
 //
 // Bound by memory for long caches: 6 sequences of 131072 tokens, 8 heads of 128, 64 queries, 3.2 GB,
-// 533 us, 6.0 TB/s of the 6.3 of a bare read, as for 256 of 4096, 32 queries; 96 ragged ones of up to
+// 532 us, 6.1 TB/s of the 7.0 of a plain read, as for 256 of 4096, 32 queries; 96 ragged ones of up to
 // 4096, 200 MB, 44 us, 4.6 TB/s: less than two rounds of workgroups, each with the chain piece -> length
 // -> page -> keys before it.  For 1000 tokens that chain, the join and the launch are all of its 7.8 us.
 template <typename T, int DP, bool EXACT, bool NT>
