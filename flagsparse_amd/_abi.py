@@ -18,7 +18,7 @@ FSP_F64 = 1
 FSP_BF16 = 2
 FSP_F16 = 3
 FSP_CUT_PIECES = 2
-ABI_VERSION = 20
+ABI_VERSION = 21
 
 _lib = None
 
@@ -124,10 +124,14 @@ SIGNATURES = {
     "fsp_attention_paged_piece": (_i64, [_i64, _i64]),
     "fsp_attention_paged_workspace": (_i64, [_i64, _i64, _i64]),
     "fsp_attention_paged": (_i32, [_p, _p]),
+    "fsp_attention_paged_sinks": (_i32, [_p, _i64, _p]),
     "fsp_attention_packed_tile": (_i64, [_i32]),
     "fsp_attention_packed_workspace": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i32]),
     "fsp_attention_packed": (_i32, [_p, _p]),
     "fsp_attention_packed_backward": (_i32, [_p, _p]),
+    "fsp_attention_packed_sinks": (_i32, [_p, _i64, _p]),
+    "fsp_attention_packed_sinks_backward": (_i32, [_p, _i64, _p, _i64, _p]),
+    "fsp_attention_packed_sinks_workspace": (_i64, [_i64] * 10),
 }
 
 

@@ -154,6 +154,15 @@ def _window_of(window):
     return min(window, _TOKENS_CAP)
 
 
+def _sinks_of(sinks, window):
+    sinks = 0 if sinks is None else int(sinks)
+    if sinks < 0:
+        raise ValueError("sinks must be a number of tokens, 0 or more")
+    if sinks and not window:
+        raise ValueError("sinks need a window")
+    return min(sinks, _TOKENS_CAP)
+
+
 def _check_out(out, name, shape, dtype, device):
     if not torch.is_tensor(out) or tuple(out.shape) != tuple(shape):
         raise ValueError(f"{name} must be a tensor of shape {tuple(shape)}")
@@ -467,20 +476,20 @@ def _append(kv, head, k, v, q, res, cos, sin, token_indptr, lengths):
 
 
 def flagsparse_attention_paged(q, lengths, *, prepared=None, k_pages=None, v_pages=None,
-                               indptr=None, indices=None, scale=None, window=None, out=None,
-                               return_lse=False):
+                               indptr=None, indices=None, scale=None, window=None, sinks=0,
+                               out=None, return_lse=False):
     """Attention of one query per sequence over what a paged cache holds of it.
 
     ``q``: [sequences, heads, dim]; ``lengths[b]``: the tokens that sequence b holds, the query's
     own among them (0: the sequence is empty, and its output is zeros).  ``window``: only the last
-    ``window`` tokens are seen.  ``scale``: dim ** -0.5 by default.  Returns [sequences, heads, dim],
+    ``window`` tokens are seen, and with ``sinks`` the first ``sinks`` too.  ``scale``: dim ** -0.5 by default.  Returns [sequences, heads, dim],
     with the float32 log-sum-exp [sequences, heads] if ``return_lse``; neither is differentiable, nor
     is what flagsparse_paged_append gives.  With ``prepared`` nothing is
     waited for, so lengths are not checked: one that its sequence's pages cannot hold gives NaN."""
     key = None
     if out is None and type(prepared) is PreparedPagedKV and type(scale) in _PLAIN and \
-            type(window) in _PLAIN:
-        key = _layouts(q, lengths) + (scale, window, prepared.k_pages.data_ptr(),
+            type(window) in _PLAIN and type(sinks) in _PLAIN:
+        key = _layouts(q, lengths) + (scale, window, sinks, prepared.k_pages.data_ptr(),
                                       prepared.v_pages.data_ptr())
         kept = prepared._calls.get(key)
         if kept is not None and q.data_ptr() % 16 == 0:
@@ -496,6 +505,7 @@ def flagsparse_attention_paged(q, lengths, *, prepared=None, k_pages=None, v_pag
     heads = q.shape[1]
     _check_heads(heads, kv.kv_heads)
     factor, past = _scale_of(scale, kv.dim), _window_of(window)
+    first = _sinks_of(sinks, past)
     res, copied = _result(out, "out", q.shape, dt, dev, q, kv.k_pages, kv.v_pages)
     rows = _rows(q)
     # what such calls share: the arguments, patterns of their arrays, the counts of arrivals they need
@@ -507,7 +517,7 @@ def flagsparse_attention_paged(q, lengths, *, prepared=None, k_pages=None, v_pag
     kept = (kv._packed() + _PAGED.pack(
         kv._pieces.data_ptr(), kv._first.data_ptr(), pieces, kv._piece, heads, past, factor,
         *_steps(rows), *_steps(res)), _like(q.shape, dt, dev),
-        _like((kv.batch, heads), torch.float32, dev), room, need)
+        _like((kv.batch, heads), torch.float32, dev), room, need, first)
     lse = _attend(kv, kept, rows, res, n, return_lse)
     if key is not None and rows is q and n is lengths:
         _keep(kv._calls, key, kept)
@@ -531,7 +541,7 @@ def _arrivals(kv, stream, need):
 
 def _attend(kv, kept, q, res, lengths, return_lse):
     """The launch; returns the log-sum-exp, if asked for."""
-    head, _, like_lse, room, need = kept
+    head, _, like_lse, room, need, sinks = kept
     lse = torch.empty_like(like_lse, memory_format=_CONTIGUOUS) if return_lse else None
     if not kv.batch:
         return lse
@@ -540,8 +550,12 @@ def _attend(kv, kept, q, res, lengths, return_lse):
         work = torch.empty_like(room, memory_format=_CONTIGUOUS)
         if need:
             counts = _arrivals(kv, stream, need)
-    status = _abi.lib().fsp_attention_paged(head + _PAGED_AT.pack(
-        q.data_ptr(), res.data_ptr(), _at(lse), lengths.data_ptr(), _at(work), _at(counts)), stream)
+    args = head + _PAGED_AT.pack(q.data_ptr(), res.data_ptr(), _at(lse), lengths.data_ptr(),
+                                 _at(work), _at(counts))
+    if sinks:
+        status = _abi.lib().fsp_attention_paged_sinks(args, sinks, stream)
+    else:
+        status = _abi.lib().fsp_attention_paged(args, stream)
     if status:
         _abi.check(status, "fsp_attention_paged")
     return lse
@@ -555,7 +569,8 @@ class PreparedAttention:
     one sequence's rows, those with the most to do first, so that the last ones to finish are
     short."""
 
-    __slots__ = ("batch", "q_tokens", "k_tokens", "device", "_longest", "_tiles", "_streams", "_calls")
+    __slots__ = ("batch", "q_tokens", "k_tokens", "device", "_longest", "_tiles", "_sequences",
+                 "_streams", "_calls")
 
     def __init__(self, q_len, k_len, device):
         self.batch = len(q_len)
@@ -567,9 +582,13 @@ class PreparedAttention:
         names = [(which, causal) for which in range(4) for causal in (False, True)]
         lists = [_tiles(q_len, k_len, int(_abi.lib().fsp_attention_packed_tile(which)), causal,
                         which >= 2) for which, causal in names]
-        flat = torch.from_numpy(np.concatenate(lists)).to(device)
+        sequences = np.zeros((self.batch, 8), dtype=np.int32)
+        sequences[:, 3:7] = np.stack([np.cumsum(q_len) - q_len, q_len, np.cumsum(k_len) - k_len, k_len],
+                                     axis=1)
+        flat = torch.from_numpy(np.concatenate(lists + [sequences])).to(device)
         ends = np.cumsum([0] + [len(t) for t in lists])
         self._tiles = {name: flat[ends[i]:ends[i + 1]] for i, name in enumerate(names)}
+        self._sequences = flat[ends[-1]:]
         self._streams = _Streams()
         self._calls = _abi.Calls()
 
@@ -637,8 +656,8 @@ def prepare_attention_packed(indptr, k_indptr=None):
     return prepared
 
 
-def _packed_inputs(q, k, v, indptr, k_indptr, prepared, causal, window):
-    """(prepared, causal, window) of a call whose arrays are checked against each other."""
+def _packed_inputs(q, k, v, indptr, k_indptr, prepared, causal, window, sinks):
+    """(prepared, causal, window, sinks) of a call whose arrays are checked against each other."""
     _check_tensor(q, "q")
     _check_tensor(k, "k", q.dtype, q.device, None, q.shape[2])
     _check_tensor(v, "v", q.dtype, q.device, k.shape[1], q.shape[2])
@@ -647,6 +666,7 @@ def _packed_inputs(q, k, v, indptr, k_indptr, prepared, causal, window):
     window = _window_of(window)
     if window and not causal:
         raise ValueError("window needs causal=True")
+    sinks = _sinks_of(sinks, window)
     if prepared is None:
         if indptr is None:
             raise ValueError("indptr is required when prepared is not provided")
@@ -660,7 +680,7 @@ def _packed_inputs(q, k, v, indptr, k_indptr, prepared, causal, window):
     if k.shape[0] != prepared.k_tokens or v.shape[0] != prepared.k_tokens:
         raise ValueError(f"k and v must have {prepared.k_tokens} tokens, got {k.shape[0]} and "
                          f"{v.shape[0]}")
-    return prepared, bool(causal), window
+    return prepared, bool(causal), window, sinks
 
 
 def _pack(prepared, q, k, v, causal, window, scale, out, grads=()):
@@ -691,23 +711,26 @@ def _refuse_tangents(*tensors):
         raise NotImplementedError("the gradient has no forward-mode derivative")
 
 
-def _run_forward(prepared, head, q, k, v, res, lse):
+def _run_forward(prepared, head, sinks, q, k, v, res, lse):
     if q.shape[0]:
-        status = _abi.lib().fsp_attention_packed(head + _PACKED_AT.pack(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), res.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, 0),
-            prepared._on())
+        args = head + _PACKED_AT.pack(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), res.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, 0)
+        if sinks:
+            status = _abi.lib().fsp_attention_packed_sinks(args, sinks, prepared._on())
+        else:
+            status = _abi.lib().fsp_attention_packed(args, prepared._on())
         if status:
             _abi.check(status, "fsp_attention_packed")
 
 
-def _forward(prepared, q, k, v, causal, window, scale, out=None, key=None):
+def _forward(prepared, q, k, v, causal, window, sinks, scale, out=None, key=None):
     res, copied = _result(out, "out", q.shape, q.dtype, q.device, q, k, v)
     rows = _rows(q), _rows(k), _rows(v)
     head = _pack(prepared, *rows, causal, window, scale, res)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-    _run_forward(prepared, head, *rows, res, lse)
+    _run_forward(prepared, head, sinks, *rows, res, lse)
     if key is not None and rows[0] is q and rows[1] is k and rows[2] is v:
-        _keep(prepared._calls, key, (head, _like(q.shape, q.dtype, q.device),
+        _keep(prepared._calls, key, (head, sinks, _like(q.shape, q.dtype, q.device),
                                      _like(lse.shape, lse.dtype, lse.device)))
     if copied:
         out.copy_(res)
@@ -717,10 +740,10 @@ def _forward(prepared, q, k, v, causal, window, scale, out=None, key=None):
 
 class _Differentiable(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, prepared, causal, window, scale):
-        out, lse = _forward(prepared, q, k, v, causal, window, scale)
+    def forward(ctx, q, k, v, prepared, causal, window, sinks, scale):
+        out, lse = _forward(prepared, q, k, v, causal, window, sinks, scale)
         ctx.save_for_backward(q, k, v, out, lse)
-        ctx.rest = (prepared, causal, window, scale)
+        ctx.rest = (prepared, causal, window, sinks, scale)
         ctx.mark_non_differentiable(lse)
         return out, lse
 
@@ -728,20 +751,21 @@ class _Differentiable(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad, _):
         q, k, v, out, lse = ctx.saved_tensors
-        prepared, causal, window, scale = ctx.rest
+        prepared, causal, window, sinks, scale = ctx.rest
         _refuse_tangents(grad, q, k, v)
-        grads = _backward(prepared, grad, q, k, v, out, lse, causal, window, scale)
-        return *grads, None, None, None, None
+        grads = _backward(prepared, grad, q, k, v, out, lse, causal, window, sinks, scale)
+        return *grads, None, None, None, None, None
 
 
 def flagsparse_attention_packed(q, k, v, indptr=None, k_indptr=None, *, prepared=None, causal=True,
-                                window=None, scale=None, out=None, return_lse=False):
+                                window=None, sinks=0, scale=None, out=None, return_lse=False):
     """Attention over packed sequences.
 
     ``q``: [tokens, heads, dim]; ``k``, ``v``: [key tokens, kv_heads, dim]; the sequences are given
     by ``indptr`` / ``k_indptr`` (checked by this call, which waits for them) or by ``prepared``
     (prepare_attention_packed).  With ``causal`` query i of nq sees key j of nk if
-    j <= i + nk - nq, the last query all of them; ``window``: only the last ``window`` of those.
+    j <= i + nk - nq, the last query all of them; ``window``: only the last ``window`` of those, and with
+    ``sinks`` the sequence's first ``sinks`` keys too.
     ``scale``: dim ** -0.5 by default.  Returns [tokens, heads, dim], with the float32 log-sum-exp
     [tokens, heads] if ``return_lse``.  The output is differentiable with respect to q, k and v where
     they require a gradient (the log-sum-exp is not); forward-mode tangents raise NotImplementedError.
@@ -753,35 +777,41 @@ def flagsparse_attention_packed(q, k, v, indptr=None, k_indptr=None, *, prepared
     wanted = torch.is_grad_enabled() and (_tracked(q) or _tracked(k) or _tracked(v)) or \
         _has_tangent(q, k, v)  # which _Differentiable refuses
     if out is None and not wanted and type(prepared) is PreparedAttention and \
-            type(scale) in _PLAIN and type(window) in _PLAIN and type(causal) in _PLAIN:
-        key = _layouts(q, k, v) + (causal, window, scale)
+            type(scale) in _PLAIN and type(window) in _PLAIN and type(causal) in _PLAIN and \
+            type(sinks) in _PLAIN:
+        key = _layouts(q, k, v) + (causal, window, sinks, scale)
         kept = prepared._calls.get(key)
         if kept is not None and not (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
-            head, like, like_lse = kept
+            head, first, like, like_lse = kept
             res = torch.empty_like(like, memory_format=_CONTIGUOUS)
             lse = torch.empty_like(like_lse, memory_format=_CONTIGUOUS)
-            _run_forward(prepared, head, q, k, v, res, lse)
+            _run_forward(prepared, head, first, q, k, v, res, lse)
             return (res, lse) if return_lse else res
-    prepared, causal, window = _packed_inputs(q, k, v, indptr, k_indptr, prepared, causal, window)
+    prepared, causal, window, sinks = _packed_inputs(q, k, v, indptr, k_indptr, prepared, causal,
+                                                     window, sinks)
     scale = _scale_of(scale, q.shape[2])
     if wanted:
         if out is not None:
             raise RuntimeError("out cannot be given where q, k or v require a gradient")
-        res, lse = _Differentiable.apply(q, k, v, prepared, causal, window, scale)
+        res, lse = _Differentiable.apply(q, k, v, prepared, causal, window, sinks, scale)
     else:
-        res, lse = _forward(prepared, q, k, v, causal, window, scale, out, key)
+        res, lse = _forward(prepared, q, k, v, causal, window, sinks, scale, out, key)
     return (res, lse) if return_lse else res
 
 
-def _backward(prepared, grad_out, q, k, v, out, lse, causal, window, scale, key=None):
+def _backward(prepared, grad_out, q, k, v, out, lse, causal, window, sinks, scale, key=None):
     rows = tuple(_rows(t) for t in (grad_out, q, k, v, out))
     flat = lse.contiguous()
     grads = tuple(torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
     head = _pack(prepared, *rows[1:4], causal, window, scale, rows[4], (rows[0], *grads))
-    room = int(_abi.lib().fsp_attention_packed_workspace(
-        prepared._tiles[2, causal].shape[0], q.shape[1], k.shape[1], q.shape[2], q.shape[0],
-        k.shape[0], causal and not window))
-    kept = (head, _like((room,), torch.uint8, q.device),
+    sizes = (prepared._tiles[2, causal].shape[0], q.shape[1], k.shape[1], q.shape[2], q.shape[0],
+             k.shape[0])
+    if sinks:
+        room = int(_abi.lib().fsp_attention_packed_sinks_workspace(
+            *sizes, prepared._longest[1], prepared.batch, window, sinks))
+    else:
+        room = int(_abi.lib().fsp_attention_packed_workspace(*sizes, causal and not window))
+    kept = (head, sinks, _like((room,), torch.uint8, q.device),
             tuple(_like(t.shape, t.dtype, t.device) for t in grads))
     _run_backward(prepared, kept, rows, flat, grads)
     if key is not None and flat is lse and all(
@@ -792,20 +822,25 @@ def _backward(prepared, grad_out, q, k, v, out, lse, causal, window, scale, key=
 
 def _run_backward(prepared, kept, rows, lse, grads):
     """``kept``: the arguments up to the addresses, and a pattern of the workspace."""
-    head, room, _ = kept
+    head, sinks, room, _ = kept
     grad_out, q, k, v, out = rows
     if q.shape[0] or k.shape[0]:
         work = torch.empty_like(room, memory_format=_CONTIGUOUS)
-        status = _abi.lib().fsp_attention_packed_backward(head + _PACKED_AT.pack(
+        args = head + _PACKED_AT.pack(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
             grad_out.data_ptr(), grads[0].data_ptr(), grads[1].data_ptr(), grads[2].data_ptr(),
-            work.data_ptr()), prepared._on())
+            work.data_ptr())
+        if sinks:
+            status = _abi.lib().fsp_attention_packed_sinks_backward(
+                args, sinks, prepared._sequences.data_ptr(), prepared.batch, prepared._on())
+        else:
+            status = _abi.lib().fsp_attention_packed_backward(args, prepared._on())
         if status:
             _abi.check(status, "fsp_attention_packed_backward")
 
 
 def flagsparse_attention_packed_backward(grad_out, q, k, v, out, lse, indptr=None, k_indptr=None, *,
-                                         prepared=None, causal=True, window=None, scale=None):
+                                         prepared=None, causal=True, window=None, sinks=0, scale=None):
     """(grad_q, grad_k, grad_v) of flagsparse_attention_packed: ``grad_out`` is the gradient of its
     output, ``out`` and ``lse`` what it returned, the other arguments its own.  The gradients are not
     differentiable themselves.
@@ -816,19 +851,20 @@ def flagsparse_attention_packed_backward(grad_out, q, k, v, out, lse, indptr=Non
     key, rows = None, (grad_out, q, k, v, out)
     _refuse_tangents(*rows, lse)
     if type(prepared) is PreparedAttention and type(scale) in _PLAIN and \
-            type(window) in _PLAIN and type(causal) in _PLAIN:
-        key = _layouts(*rows, lse) + (causal, window, scale)
+            type(window) in _PLAIN and type(causal) in _PLAIN and type(sinks) in _PLAIN:
+        key = _layouts(*rows, lse) + (causal, window, sinks, scale)
         kept = prepared._calls.get(key)
         if kept is not None and not (grad_out.data_ptr() | q.data_ptr() | k.data_ptr() |
                                      v.data_ptr() | out.data_ptr()) % 16:
-            grads = tuple([torch.empty_like(t, memory_format=_CONTIGUOUS) for t in kept[2]])
+            grads = tuple([torch.empty_like(t, memory_format=_CONTIGUOUS) for t in kept[3]])
             _run_backward(prepared, kept, rows, lse, grads)
             return grads
-    prepared, causal, window = _packed_inputs(q, k, v, indptr, k_indptr, prepared, causal, window)
+    prepared, causal, window, sinks = _packed_inputs(q, k, v, indptr, k_indptr, prepared, causal,
+                                                     window, sinks)
     for t, name in ((grad_out, "grad_out"), (out, "out")):
         _check_tensor(t, name, q.dtype, q.device, q.shape[1], q.shape[2])
         if t.shape[0] != q.shape[0]:
             raise ValueError(f"{name} must have {q.shape[0]} tokens, got {t.shape[0]}")
     _check_out(lse, "lse", q.shape[:2], torch.float32, q.device)
-    return _backward(prepared, grad_out, q, k, v, out, lse, causal, window,
+    return _backward(prepared, grad_out, q, k, v, out, lse, causal, window, sinks,
                      _scale_of(scale, q.shape[2]), key)

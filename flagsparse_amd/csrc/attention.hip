@@ -12,9 +12,22 @@ struct Tile {
   int first, rows, at, q_begin, nq, k_begin, nk, pad;
 };
 
+// sinks: so many first keys of a sequence stay visible to queries whose window has left them.
 struct Shape {
   int heads, kv_heads, dim, causal, window;
   float scale;
+  int sinks;
+};
+
+// The keys that a tile of queries reads in steps of ROWS: the first ``sinks`` that lie before its window,
+// and what its window holds, [lot, hit).  Step i starts at key at(i); those of the first keys end at ``sinks``.
+template <bool SINKS, int ROWS>
+struct Walk {
+  int lot, sinks, skip, end;
+  __device__ Walk(const Shape& s, int lot, int hit)
+      : lot(lot), sinks(SINKS ? min(s.sinks, lot) : 0), skip(SINKS ? (sinks + ROWS - 1) / ROWS * ROWS : 0),
+        end(hit > lot ? hit - lot + skip : 0) {}
+  __device__ int at(int i) const { return SINKS && i < skip ? i : lot + i - skip; }
 };
 
 // Workgroups go to the 8 XCDs in turn.  Where the heads divide by them, each XCD has heads of its own, so
@@ -180,7 +193,7 @@ __device__ __forceinline__ void store_rows(T* to, const f32x16 (&x)[NT], float f
 // over the same keys, or four buffers in turn, were no faster (284 / 289, 279 / 282 us).  16 ragged prompts
 // of up to 2047, 32 heads over 8: 82 us, 0.69 PFLOP/s: short loops between the first loads and the last
 // stores, 38 % of the cycles with neither.
-template <typename T, int DP, int BLOCKS, int PARTS>
+template <typename T, int DP, int BLOCKS, int PARTS, bool SINKS>
 __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_packed_kernel(
     Shape s, const Tile* __restrict__ tiles, int n_tiles, const T* __restrict__ q, int64_t q_token,
     int64_t q_head, const T* __restrict__ k, int64_t k_token, int64_t k_head,
@@ -237,9 +250,13 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_packed_kerne
   const int k_at = L::row_at(lane);
   const int v_at = L::col_at(lane);
 
-  auto step = [&](int j0, const char* sk_, const char* sv_) {
-    j0 += part * kRows;
-    if (!active || j0 >= hi1 || j0 + kRows <= lo0) return;
+  const Walk<SINKS, ROWS> walk(s, lot, hit);
+  auto step = [&](int i0, const char* sk_, const char* sv_) {
+    const int j0 = walk.at(i0) + part * kRows;
+    const bool early = SINKS && i0 < walk.skip;  // keys before the tile's window
+    if (!active || (early ? j0 >= walk.sinks
+                          : j0 >= hi1 || (j0 + kRows <= lo0 && !(SINKS && j0 < s.sinks))))
+      return;
     const lds_char* sk = (const lds_char*)sk_ + part * L::BYTES;
     const lds_char* sv = (const lds_char*)sv_ + part * L::BYTES;
     f32x16 x[2];
@@ -252,14 +269,15 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_packed_kerne
       }
     }
     read_ahead<2 * NS, NS>();
-    if (j0 + kRows > hi0 || j0 < lo1) {
-      const int first = lo - j0 - 4 * half, last = hi - j0 - 4 * half;
+    if (early || j0 + kRows > hi0 || j0 < lo1) {
+      const int first = (early ? 0 : lo) - j0 - 4 * half;
+      const int last = (early ? walk.sinks : hi) - j0 - 4 * half, keep = s.sinks - j0 - 4 * half;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int j = 32 * u + 8 * (r / 4) + r % 4;
-          x[u][r] = j >= first && j < last ? x[u][r] : -INFINITY;
+          x[u][r] = (j >= first || (SINKS && j < keep)) && j < last ? x[u][r] : -INFINITY;
         }
     }
     float m = x[0][0];
@@ -295,19 +313,19 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_packed_kerne
     __builtin_amdgcn_sched_group_barrier(0x100, 4 * NT, 1);  // the first values early
   };
 
-  int j0 = lot;
-  if (j0 < hit) load(j0, s_k0, s_v0);
+  int i0 = 0;
+  if (i0 < walk.end) load(walk.at(i0), s_k0, s_v0);
   __syncthreads();
-  while (j0 < hit) {
-    if (j0 + ROWS < hit) load(j0 + ROWS, s_k1, s_v1);
-    step(j0, s_k0, s_v0);
+  while (i0 < walk.end) {
+    if (i0 + ROWS < walk.end) load(walk.at(i0 + ROWS), s_k1, s_v1);
+    step(i0, s_k0, s_v0);
     __syncthreads();
-    j0 += ROWS;
-    if (j0 >= hit) break;
-    if (j0 + ROWS < hit) load(j0 + ROWS, s_k0, s_v0);
-    step(j0, s_k1, s_v1);
+    i0 += ROWS;
+    if (i0 >= walk.end) break;
+    if (i0 + ROWS < walk.end) load(walk.at(i0 + ROWS), s_k0, s_v0);
+    step(i0, s_k1, s_v1);
     __syncthreads();
-    j0 += ROWS;
+    i0 += ROWS;
   }
 
   sum += other_half(sum);
@@ -394,7 +412,7 @@ constexpr int kFewKeys = 128;
 // = P^T (dP^T - delta), delta = grad_out . out, is the operand of dQ^T = K^T dS^T where it lies.  P comes
 // from the rows' lse, so nothing of the size of S is kept.  Bound as the forward pass: two sequences of
 // 4096, 32 heads of 128 over 8, causal, 4.2e11 operations in 413 us, 1.0 PFLOP/s.
-template <typename T, int DP, int BLOCKS, int PARTS>
+template <typename T, int DP, int BLOCKS, int PARTS, bool SINKS>
 __global__ __launch_bounds__(64 * BLOCKS * PARTS, DP <= 64 ? 3 : 2) void attention_grad_q_kernel(
     Shape s, const Tile* __restrict__ tiles, int n_tiles, const T* __restrict__ q, int64_t q_token,
     int64_t q_head, const T* __restrict__ k, int64_t k_token, int64_t k_head,
@@ -467,50 +485,57 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, DP <= 64 ? 3 : 2) void attenti
       y = mfma32(row_frag<T>(sv + (r_at ^ (i * 32)) + u * 32 * L::PITCH), gf[i], y);
     }
   };
-  auto hide = [&](int j0, int u, f32x16& x) {
-    if (j0 + kRows > hi0 || j0 < lo1) {
-      const int first = lo - j0 - 4 * half, last = hi - j0 - 4 * half;
+  const Walk<SINKS, ROWS> keys(s, lot, hit);
+  // whether any of the wave's rows sees any of n keys from j0 on
+  auto unseen = [&](int j0, int n, bool early) {
+    return early ? j0 >= keys.sinks : j0 >= hi1 || (j0 + n <= lo0 && !(SINKS && j0 < s.sinks));
+  };
+  auto hide = [&](int j0, int u, bool early, f32x16& x) {
+    if (early || j0 + kRows > hi0 || j0 < lo1) {
+      const int first = (early ? 0 : lo) - j0 - 4 * half;
+      const int last = (early ? keys.sinks : hi) - j0 - 4 * half, keep = s.sinks - j0 - 4 * half;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int j = 32 * u + 8 * (r / 4) + r % 4;
-        x[r] = j >= first && j < last ? x[r] : 0.0f;
+        x[r] = (j >= first || (SINKS && j < keep)) && j < last ? x[r] : 0.0f;
       }
     }
   };
   auto walk = [&](auto&& step) {
-    auto wave_step = [&](int j0, const char* sk, const char* sv) {
-      j0 += part * kRows;
-      if (!active || j0 >= hi1 || j0 + kRows <= lo0) return;
-      step(j0, (const lds_char*)sk + part * L::BYTES, (const lds_char*)sv + part * L::BYTES);
+    auto wave_step = [&](int i0, const char* sk, const char* sv) {
+      const int j0 = keys.at(i0) + part * kRows;
+      const bool early = SINKS && i0 < keys.skip;  // keys before the tile's window
+      if (!active || unseen(j0, kRows, early)) return;
+      step(j0, early, (const lds_char*)sk + part * L::BYTES, (const lds_char*)sv + part * L::BYTES);
     };
-    int j0 = lot;
-    if (j0 < hit) load(j0, s_k0, s_v0);
+    int i0 = 0;
+    if (i0 < keys.end) load(keys.at(i0), s_k0, s_v0);
     __syncthreads();
-    while (j0 < hit) {
-      if (j0 + ROWS < hit) load(j0 + ROWS, s_k1, s_v1);
-      wave_step(j0, s_k0, s_v0);
+    while (i0 < keys.end) {
+      if (i0 + ROWS < keys.end) load(keys.at(i0 + ROWS), s_k1, s_v1);
+      wave_step(i0, s_k0, s_v0);
       __syncthreads();
-      j0 += ROWS;
-      if (j0 >= hit) break;
-      if (j0 + ROWS < hit) load(j0 + ROWS, s_k0, s_v0);
-      wave_step(j0, s_k1, s_v1);
+      i0 += ROWS;
+      if (i0 >= keys.end) break;
+      if (i0 + ROWS < keys.end) load(keys.at(i0 + ROWS), s_k0, s_v0);
+      wave_step(i0, s_k1, s_v1);
       __syncthreads();
-      j0 += ROWS;
+      i0 += ROWS;
     }
   };
 
   // An output of few keys is large, and so is what its rounding does to delta = grad_out . out: there
   // delta is made anew, as the sum of the weights times dP.
-  if (hit - lot <= kFewKeys) {
+  if (hit - lot + keys.sinks <= kFewKeys) {
     delta = 0;
-    walk([&](int j0, const lds_char* sk, const lds_char* sv) {
+    walk([&](int j0, bool early, const lds_char* sk, const lds_char* sv) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         f32x16 x, y;
         products(sk, sv, u, x, y);
 #pragma unroll
         for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], c, -base)) * y[r];
-        hide(j0, u, x);
+        hide(j0, u, early, x);
 #pragma unroll
         for (int r = 0; r < 16; ++r) delta += x[r];
       }
@@ -532,16 +557,16 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, DP <= 64 ? 3 : 2) void attenti
   constexpr bool RAISED = std::is_same<T, f16>::value;
   int n = RAISED ? kRaise : 0;
   base -= n;
-  walk([&](int j0, const lds_char* sk, const lds_char* sv) {
+  walk([&](int j0, bool early, const lds_char* sk, const lds_char* sv) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      if (j0 + 32 * u >= hi1 || j0 + 32 * u + 32 <= lo0) continue;
+      if (unseen(j0 + 32 * u, 32, early)) continue;
       f32x16 x, y;
       products(sk, sv, u, x, y);
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], c, -base)) * (y[r] - delta);
-      hide(j0, u, x);
+      hide(j0, u, early, x);
       if constexpr (RAISED) {
         const int by = lower(x, acc);
         base += by;
@@ -581,6 +606,53 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, DP <= 64 ? 3 : 2) void attenti
     store_rows<T, NT>(dq + row * dq_token + a * dq_head, acc, s.scale, s.dim, half);
 }
 
+// Where first keys stay visible to all later queries, their tiles would have many times the others' work
+// under a window: with SINKS they go to jobs of ``chunk`` queries each, whose sums another launch adds in
+// their order.  Slot q_begin / chunk + b + i is the job of the queries [i * chunk, (i + 1) * chunk) of sequence b:
+// no two are the same, and there are at most q_tokens / chunk + batch.  A slot holds, for each share
+// of the heads, key head and first key, the values' sums and then the keys'.
+struct Jobs {
+  const Tile* sequences;  // rows, first row, ..: unused; q_begin, nq, k_begin, nk
+  float* sums;
+  int batch, chunk, slots, tiles, blocks;  // tiles of first keys a sequence; workgroups of all jobs
+};
+
+template <int ROWS>
+__device__ __forceinline__ float* job_sums(const Jobs& jobs, const Shape& s, int split, int slot, int share,
+                                           int g, int row) {
+  return jobs.sums + ((((int64_t)slot * split + share) * s.kv_heads + g) * (2 * jobs.tiles * ROWS) + row) * s.dim;
+}
+
+// The tile of first keys, key head, share and queries [from, to) of job n; false if there are none.
+template <int ROWS>
+__device__ __forceinline__ bool job_of(const Jobs& jobs, const Shape& s, int split, int n, Tile& t, int& g,
+                                       int& slot, int& from, int& to) {
+  const int per = s.kv_heads * split;
+  g = n % per;
+  n /= per;
+  slot = n % jobs.slots;
+  const int at = n / jobs.slots * ROWS, lane = threadIdx.x & 63;
+  if (at / ROWS >= jobs.tiles) return false;
+  int b = 0;  // the last sequence whose slots start at or before this one, 64 at a look
+  for (int i = 0; i < jobs.batch; i += kWave) {
+    const bool in = i + lane < jobs.batch &&
+                    jobs.sequences[min(i + lane, jobs.batch - 1)].q_begin / jobs.chunk + i + lane <= slot;
+    const int count = __popcll(__ballot(in));
+    b += count;
+    if (count < kWave) break;
+  }
+  b = __builtin_amdgcn_readfirstlane(b - 1);
+  t = jobs.sequences[b];
+  const int64_t begin = (int64_t)(slot - t.q_begin / jobs.chunk - b) * jobs.chunk;
+  t.first = t.k_begin + at;
+  t.at = at;
+  t.rows = min(ROWS, t.nk - at);
+  if (begin >= t.nq || at >= min(t.nk, s.sinks)) return false;
+  from = (int)begin;
+  to = (int)min(begin + jobs.chunk, (int64_t)t.nq);
+  return true;
+}
+
 // Gradients of the keys and values, BLOCKS * 32 keys a workgroup, over the heads of the group and their
 // queries.  S and dP are [queries, keys], so P and dS are the operands of dV^T = grad_out^T P and
 // dK^T = Q^T dS where they lie.  The products start from a row's -lse / scale and -delta, so that they
@@ -589,24 +661,30 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, DP <= 64 ? 3 : 2) void attenti
 // sums of dQ over the workgroups of a row's keys would cost atomics whose order changes results, or
 // 32-bit copies in memory.  Bound as the forward pass: two sequences of 4096, 32 heads of 128 over 8,
 // causal, 5.5e11 operations in 577 us, 0.96 PFLOP/s.
-template <typename T, int DP, int BLOCKS, int PARTS>
+template <typename T, int DP, int BLOCKS, int PARTS, bool SINKS>
 __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_grad_kv_kernel(
     Shape s, const Tile* __restrict__ tiles, int n_tiles, const T* __restrict__ q, int64_t q_token,
     int64_t q_head, const T* __restrict__ k, int64_t k_token, int64_t k_head,
     const T* __restrict__ v, int64_t v_token, int64_t v_head, const T* __restrict__ go,
     int64_t go_token, int64_t go_head, const float* __restrict__ stats, int64_t q_tokens,
     T* __restrict__ dk, int64_t dk_token, int64_t dk_head, T* __restrict__ dv, int64_t dv_token,
-    int64_t dv_head, int split, float* __restrict__ sums, int64_t k_tokens) {
+    int64_t dv_head, int split, float* __restrict__ sums, int64_t k_tokens, Jobs jobs) {
   typedef Lay<DP> L;
   constexpr int NS = DP / 16, NT = DP / 32;
   constexpr int ROWS = 32 * PARTS, BYTES = ROWS * L::PITCH;
   __shared__ __attribute__((aligned(1024))) char s_q0[BYTES], s_g0[BYTES], s_q1[BYTES], s_g1[BYTES];
   __shared__ __attribute__((aligned(256))) float s_x0[ROWS], s_y0[ROWS], s_x1[ROWS], s_y1[ROWS];
-  int tile, g;
-  tile_and_head(blockIdx.x, n_tiles, s.kv_heads * split, tile, g);
+  int tile, g, slot = -1, from = 0, to = 0x7fffffff;
+  Tile t;
+  if (SINKS && (int)blockIdx.x < jobs.blocks) {
+    if (!job_of<32 * BLOCKS>(jobs, s, split, blockIdx.x, t, g, slot, from, to)) return;
+  } else {
+    tile_and_head(blockIdx.x - (SINKS ? jobs.blocks : 0), n_tiles, s.kv_heads * split, tile, g);
+    t = tiles[tile];
+    if (SINKS && t.at < s.sinks) return;
+  }
   const int share = g % split;  // of the group's heads
   g /= split;
-  const Tile t = tiles[tile];
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int part = wave % PARTS, block = wave / PARTS, k0 = block * 32, mine = k0 + col;
@@ -627,10 +705,26 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_grad_kv_kern
 
   // the queries that see any of the wave's keys and of the tile's
   int lo0, hi0, lo1, hi1, lot, hit, none;
-  seen_of(s, t, t.at + min(k0, t.rows - 1), lo0, hi0);
-  seen_of(s, t, t.at + min(k0 + 31, t.rows - 1), lo1, hi1);
-  seen_of(s, t, t.at, lot, none);
-  seen_of(s, t, t.at + t.rows - 1, none, hit);
+  auto sees = [&](int at, int& lo, int& hi) {  // which queries of the job see the sequence's key ``at``
+    seen_of(s, t, at, lo, hi);
+    if constexpr (SINKS) {
+      if (at < s.sinks) hi = t.nq;
+      lo = max(lo, from);
+      hi = min(hi, to);
+    }
+  };
+  {
+    const int first = t.at + min(k0, t.rows - 1), last = t.at + min(k0 + 31, t.rows - 1);
+    sees(first, lo0, hi0);
+    sees(last, lo1, hi1);
+    sees(t.at, lot, none);
+    sees(t.at + t.rows - 1, none, hit);
+    if constexpr (SINKS) {  // first keys, which all queries see, and others after them
+      hit = max(hit, t.at < s.sinks ? min(t.nq, to) : 0);
+      hi1 = max(hi0, hi1);
+      sees(min(max(first, s.sinks), last), none, hi0);
+    }
+  }
 
   f32x16 ak[NT], av[NT];
 #pragma unroll
@@ -690,7 +784,7 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_grad_kv_kern
     if (i1 + 32 > hi0 || i1 < lo1) {
       int key = mine, lo, hi;  // what sees this lane's key: made anew, as above
       asm volatile("" : "+v"(key));
-      seen_of(s, t, t.at + min(key, t.rows - 1), lo, hi);
+      sees(t.at + min(key, t.rows - 1), lo, hi);
       const int first = lo - i1 - 4 * half, last = hi - i1 - 4 * half;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -765,6 +859,12 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_grad_kv_kern
     }
   }
   if (part == 0 && mine < t.rows) {
+    if (SINKS && slot >= 0) {
+      float* to_v = job_sums<32 * BLOCKS>(jobs, s, split, slot, share, g, t.at + mine);
+      store_rows<float, NT>(to_v, av, Lift<T>::down, s.dim, half);
+      store_rows<float, NT>(to_v + (int64_t)jobs.tiles * 32 * BLOCKS * s.dim, ak, s.scale, s.dim, half);
+      return;
+    }
     if (split > 1) {
       float* to = sums + ((int64_t)(share * s.kv_heads + g) * k_tokens + row) * s.dim;
       store_rows<float, NT>(to, av, Lift<T>::down, s.dim, half);
@@ -797,12 +897,47 @@ __global__ __launch_bounds__(256) void attention_grad_kv_sum_kernel(
   *reinterpret_cast<V4<T>*>(to) = __builtin_convertvector(y, V4<T>);
 }
 
+// The first keys' and their values' gradients as the sums of their jobs, chunk by chunk and in each the shares
+// of the heads: a thread to four elements, a workgroup's of one sequence and key head.
+template <typename T, int ROWS>
+__global__ __launch_bounds__(256) void attention_grad_sinks_sum_kernel(
+    Shape s, int split, Jobs jobs, T* __restrict__ dk, int64_t dk_token, int64_t dk_head,
+    T* __restrict__ dv, int64_t dv_token, int64_t dv_head) {
+  const int quads = s.dim / 4, per = 2 * jobs.tiles * ROWS * quads, blocks = (per + 255) / 256;
+  const int i = (blockIdx.x % blocks) * 256 + threadIdx.x;
+  const int g = blockIdx.x / blocks % s.kv_heads, b = blockIdx.x / blocks / s.kv_heads;
+  if (i >= per) return;
+  const Tile t = jobs.sequences[b];
+  const int d = i % quads * 4, of = i / quads;
+  const bool keys = of >= jobs.tiles * ROWS;
+  const int row = keys ? of - jobs.tiles * ROWS : of;
+  // the rows of the tiles that have a first key
+  if (row >= t.nk || row / ROWS * ROWS >= min(t.nk, s.sinks)) return;
+  int lot, hit;
+  seen_of(s, t, row / ROWS * ROWS, lot, hit);
+  f32x4 y{};
+  if (lot < t.nq)
+    for (int c = lot / jobs.chunk; c <= (t.nq - 1) / jobs.chunk; ++c)
+      for (int p = 0; p < split; ++p)
+        y += *reinterpret_cast<const f32x4*>(
+            job_sums<ROWS>(jobs, s, split, t.q_begin / jobs.chunk + b + c, p, g, of) + d);
+  const int64_t at = t.k_begin + row;
+  T* to = keys ? dk + at * dk_token + g * dk_head : dv + at * dv_token + g * dv_head;
+  *reinterpret_cast<V4<T>*>(to + d) = __builtin_convertvector(y, V4<T>);
+}
+
 template <typename T>
 const T* in(const void* p) { return static_cast<const T*>(p); }
 
-Shape shape_of(const fsp_attention_packed_args& a) {
-  return {(int)a.heads, (int)a.kv_heads, (int)a.dim, a.causal != 0, (int)a.window,
-          (float)a.scale};
+// A call's arguments, with its first keys and, for a backward pass, the sequences.
+struct Call : fsp_attention_packed_args {
+  int64_t sinks = 0, batch = 0;
+  const int32_t* sequences = nullptr;
+};
+
+Shape shape_of(const Call& a) {
+  return {(int)a.heads, (int)a.kv_heads, (int)a.dim, a.causal != 0, (int)a.window, (float)a.scale,
+          (int)a.sinks};
 }
 
 // Twice as many waves share a tile where that fills CUs, or shortens the chains that the others end up
@@ -816,11 +951,11 @@ Shape shape_of(const fsp_attention_packed_args& a) {
 // heads (240) 50.3 / 48.5, of two of 700, 8 heads (176) 42.7 / 42.7.
 constexpr int64_t kCus = 256;
 
-int64_t seen_at_most(const fsp_attention_packed_args& a, int64_t longest) {
-  return a.window && a.window < longest ? a.window : longest;
+int64_t seen_at_most(const Call& a, int64_t longest) {
+  return a.window && a.window + a.sinks < longest ? a.window + a.sinks : longest;
 }
 
-bool share_queries(const fsp_attention_packed_args& a, int64_t fill) {
+bool share_queries(const Call& a, int64_t fill) {
   const int64_t n = a.n_q_tiles * a.heads;
   return seen_at_most(a, a.k_longest) >= 512 &&
          (n <= fill || (n <= 2 * kCus && a.causal && !a.window && a.k_longest >= 2048));
@@ -832,11 +967,11 @@ bool share_queries(const fsp_attention_packed_args& a, int64_t fill) {
 // 4000, 8 heads (256) 58 / 64; four of 64, 4 heads (16) 6.0 / 7.9; dim 64, whose workgroups go two
 // to a CU: 2048, 8 heads (128) 22.4 / 18.5, 4000 (256) 39.6 / 35.4.  Gradient of the queries, dim 128:
 // 512 (64) 20.4 / 15.9, 2048 (64) 44.8 / 38.6, 4000 (256) 82 / 86; dim 64: 2048 (128) 28.9 / 25.3.
-bool halve_tiles(const fsp_attention_packed_args& a, int64_t most) {
+bool halve_tiles(const Call& a, int64_t most) {
   return a.n_q_tiles * a.heads <= most && seen_at_most(a, a.k_longest) > kRows;
 }
 
-bool share_keys(const fsp_attention_packed_args& a, int split) {
+bool share_keys(const Call& a, int split) {
   const int64_t n = a.n_k_tiles * a.kv_heads * split;
   return (n <= kCus && a.heads / a.kv_heads / split * seen_at_most(a, a.q_longest) >= 768) ||
          (n <= 2 * kCus && a.causal && !a.window && a.q_longest >= 4096);
@@ -847,7 +982,7 @@ bool share_keys(const fsp_attention_packed_args& a, int split) {
 // 29.7 / 30.6, one of 500, 16 heads over 4 (128) 40.7 / 38.1, 4000, 2 heads (126) 136 / 127, 2000, 8
 // heads (256) 79 / 84; dim 64: 65 tokens 15.8 / 15.4, two of 256 (32) 19.9 / 18.9, 2000, 8 heads (256)
 // 49.2 / 46.8.
-bool halve_keys(const fsp_attention_packed_args& a, int split) {
+bool halve_keys(const Call& a, int split) {
   const bool small = a.dim <= 64;
   return a.n_k_tiles * a.kv_heads * split <= (small ? kCus : kCus / 2) &&
          seen_at_most(a, a.q_longest) > (small ? kRows : 4 * kRows);
@@ -868,11 +1003,11 @@ int split_heads(int64_t n_k_tiles, int64_t heads, int64_t kv_heads, bool uneven)
   return (int)split;
 }
 
-template <typename T, int DP, int BLOCKS, int PARTS>
-int launch_forward(const fsp_attention_packed_args& a, hipStream_t st) {
+template <typename T, int DP, int BLOCKS, int PARTS, bool SINKS>
+int launch_forward(const Call& a, hipStream_t st) {
   const int32_t* tiles = BLOCKS == 2 ? a.q_halves : a.q_tiles;
   const int64_t n = BLOCKS == 2 ? a.n_q_halves : a.n_q_tiles;
-  hipLaunchKernelGGL((attention_packed_kernel<T, DP, BLOCKS, PARTS>),
+  hipLaunchKernelGGL((attention_packed_kernel<T, DP, BLOCKS, PARTS, SINKS>),
                      dim3((unsigned)(n * a.heads)), dim3(64 * BLOCKS * PARTS), 0, st, shape_of(a),
                      reinterpret_cast<const Tile*>(tiles), (int)n, in<T>(a.q),
                      a.q_token, a.q_head, in<T>(a.k), a.k_token, a.k_head, in<T>(a.v), a.v_token,
@@ -880,25 +1015,25 @@ int launch_forward(const fsp_attention_packed_args& a, hipStream_t st) {
   return check_hip(hipGetLastError(), "attention_packed_kernel launch");
 }
 
-template <typename T, int DP>
-int launch_forward_parts(const fsp_attention_packed_args& a, hipStream_t st) {
-  if (halve_tiles(a, DP <= 64 ? kCus : kCus / 2)) return launch_forward<T, DP, 2, 2>(a, st);
-  return share_queries(a, DP <= 64 ? 4 * kCus : kCus) ? launch_forward<T, DP, 4, 2>(a, st)
-                                                      : launch_forward<T, DP, 4, 1>(a, st);
+template <typename T, int DP, bool SINKS>
+int launch_forward_parts(const Call& a, hipStream_t st) {
+  if (halve_tiles(a, DP <= 64 ? kCus : kCus / 2)) return launch_forward<T, DP, 2, 2, SINKS>(a, st);
+  return share_queries(a, DP <= 64 ? 4 * kCus : kCus) ? launch_forward<T, DP, 4, 2, SINKS>(a, st)
+                                                      : launch_forward<T, DP, 4, 1, SINKS>(a, st);
 }
 
-template <typename T>
-int launch_forward_dim(const fsp_attention_packed_args& a, hipStream_t st) {
-  if (a.dim <= 64) return launch_forward_parts<T, 64>(a, st);
-  if (a.dim <= 96) return launch_forward_parts<T, 96>(a, st);
-  return launch_forward_parts<T, 128>(a, st);
+template <typename T, bool SINKS>
+int launch_forward_dim(const Call& a, hipStream_t st) {
+  if (a.dim <= 64) return launch_forward_parts<T, 64, SINKS>(a, st);
+  if (a.dim <= 96) return launch_forward_parts<T, 96, SINKS>(a, st);
+  return launch_forward_parts<T, 128, SINKS>(a, st);
 }
 
-template <typename T, int DP, int BLOCKS, int PARTS>
-int launch_grad_q(const fsp_attention_packed_args& a, hipStream_t st) {
+template <typename T, int DP, int BLOCKS, int PARTS, bool SINKS>
+int launch_grad_q(const Call& a, hipStream_t st) {
   const int32_t* tiles = BLOCKS == 2 ? a.q_halves : a.q_tiles;
   const int64_t n = BLOCKS == 2 ? a.n_q_halves : a.n_q_tiles;
-  hipLaunchKernelGGL((attention_grad_q_kernel<T, DP, BLOCKS, PARTS>),
+  hipLaunchKernelGGL((attention_grad_q_kernel<T, DP, BLOCKS, PARTS, SINKS>),
                      dim3((unsigned)(n * a.heads)), dim3(64 * BLOCKS * PARTS), 0, st, shape_of(a),
                      reinterpret_cast<const Tile*>(tiles), (int)n, in<T>(a.q),
                      a.q_token, a.q_head, in<T>(a.k), a.k_token, a.k_head, in<T>(a.v), a.v_token,
@@ -908,55 +1043,95 @@ int launch_grad_q(const fsp_attention_packed_args& a, hipStream_t st) {
   return check_hip(hipGetLastError(), "attention_grad_q_kernel launch");
 }
 
-template <typename T, int DP, int BLOCKS, int PARTS>
-int launch_grad_kv(const fsp_attention_packed_args& a, int split, hipStream_t st) {
+// Queries of a job of the first keys: about what the other tiles have under their window.
+int64_t chunk_of(int64_t window) {
+  const int64_t least = 512;
+  return window <= least ? least : (window + 127) / 128 * 128;
+}
+
+int64_t job_slots(int64_t q_tokens, int64_t batch, int64_t window) {
+  return q_tokens / chunk_of(window) + batch;
+}
+
+// Elements of one share's sums over all keys, and of the jobs' of the first keys in tiles of ``rows``.
+int64_t share_floats(int split, int64_t kv_heads, int64_t k_tokens, int64_t dim) {
+  return split > 1 ? 2 * split * kv_heads * k_tokens * dim : 0;
+}
+
+int64_t first_keys(int64_t sinks, int64_t k_longest) { return sinks < k_longest ? sinks : k_longest; }
+
+Jobs jobs_of(const Call& a, int split, int rows, float* sums) {
+  Jobs j;
+  j.sequences = reinterpret_cast<const Tile*>(a.sequences);
+  j.sums = sums + share_floats(split, a.kv_heads, a.k_tokens, a.dim);
+  j.batch = (int)a.batch;
+  j.chunk = (int)chunk_of(a.window);
+  j.slots = (int)job_slots(a.q_tokens, a.batch, a.window);
+  j.tiles = (int)((first_keys(a.sinks, a.k_longest) + rows - 1) / rows);
+  j.blocks = (int)((j.tiles * (int64_t)j.slots * a.kv_heads * split + 7) / 8 * 8);
+  return j;
+}
+
+template <typename T, int DP, int BLOCKS, int PARTS, bool SINKS>
+int launch_grad_kv(const Call& a, int split, hipStream_t st) {
   const int32_t* tiles = BLOCKS == 1 ? a.k_halves : a.k_tiles;
   const int64_t n = BLOCKS == 1 ? a.n_k_halves : a.n_k_tiles;
   float* stats = static_cast<float*>(a.workspace);
   float* sums = stats + ((2 * a.heads * a.q_tokens + 3) & ~int64_t(3));
-  hipLaunchKernelGGL((attention_grad_kv_kernel<T, DP, BLOCKS, PARTS>),
-                     dim3((unsigned)(n * a.kv_heads * split)), dim3(64 * BLOCKS * PARTS), 0, st,
+  const Jobs jobs = SINKS ? jobs_of(a, split, 32 * BLOCKS, sums) : Jobs{};
+  hipLaunchKernelGGL((attention_grad_kv_kernel<T, DP, BLOCKS, PARTS, SINKS>),
+                     dim3((unsigned)(jobs.blocks + n * a.kv_heads * split)), dim3(64 * BLOCKS * PARTS), 0, st,
                      shape_of(a), reinterpret_cast<const Tile*>(tiles), (int)n,
                      in<T>(a.q), a.q_token, a.q_head, in<T>(a.k), a.k_token, a.k_head, in<T>(a.v),
                      a.v_token, a.v_head, in<T>(a.grad_out), a.grad_out_token, a.grad_out_head,
                      stats, a.q_tokens, static_cast<T*>(a.grad_k), a.grad_k_token, a.grad_k_head,
                      static_cast<T*>(a.grad_v), a.grad_v_token, a.grad_v_head, split, sums,
-                     a.k_tokens);
+                     a.k_tokens, jobs);
   if (int rc = check_hip(hipGetLastError(), "attention_grad_kv_kernel launch")) return rc;
-  if (split == 1) return FSP_OK;
-  const int64_t quads = a.kv_heads * a.k_tokens * a.dim / 2;
-  hipLaunchKernelGGL((attention_grad_kv_sum_kernel<T>), dim3((unsigned)((quads + 255) / 256)),
-                     dim3(256), 0, st, shape_of(a), split, sums, a.k_tokens,
-                     static_cast<T*>(a.grad_k), a.grad_k_token, a.grad_k_head,
-                     static_cast<T*>(a.grad_v), a.grad_v_token, a.grad_v_head);
-  return check_hip(hipGetLastError(), "attention_grad_kv_sum_kernel launch");
-}
-
-template <typename T, int DP>
-int launch_backward(const fsp_attention_packed_args& a, hipStream_t st) {
-  if (a.n_q_tiles > 0) {
-    const int rc = halve_tiles(a, kCus / 2) ? launch_grad_q<T, DP, 2, 2>(a, st)
-                   : share_queries(a, kCus) ? launch_grad_q<T, DP, 4, 2>(a, st)
-                                            : launch_grad_q<T, DP, 4, 1>(a, st);
-    if (rc) return rc;
+  if (split > 1) {
+    const int64_t quads = a.kv_heads * a.k_tokens * a.dim / 2;
+    hipLaunchKernelGGL((attention_grad_kv_sum_kernel<T>), dim3((unsigned)((quads + 255) / 256)),
+                       dim3(256), 0, st, shape_of(a), split, sums, a.k_tokens,
+                       static_cast<T*>(a.grad_k), a.grad_k_token, a.grad_k_head,
+                       static_cast<T*>(a.grad_v), a.grad_v_token, a.grad_v_head);
+    if (int rc = check_hip(hipGetLastError(), "attention_grad_kv_sum_kernel launch")) return rc;
   }
-  if (a.n_k_tiles > 0) {
-    const int split = split_heads(a.n_k_tiles, a.heads, a.kv_heads, a.causal && !a.window);
-    if (halve_keys(a, split)) return launch_grad_kv<T, DP, 1, 4>(a, split, st);
-    return share_keys(a, split) ? launch_grad_kv<T, DP, 2, 4>(a, split, st)
-                                : launch_grad_kv<T, DP, 2, 2>(a, split, st);
+  if constexpr (SINKS) {  // after it: it has written over the first keys' gradients
+    const int64_t blocks = (2 * jobs.tiles * 32 * BLOCKS * (a.dim / 4) + 255) / 256;
+    hipLaunchKernelGGL((attention_grad_sinks_sum_kernel<T, 32 * BLOCKS>),
+                       dim3((unsigned)(blocks * a.kv_heads * a.batch)), dim3(256), 0, st, shape_of(a),
+                       split, jobs, static_cast<T*>(a.grad_k), a.grad_k_token, a.grad_k_head,
+                       static_cast<T*>(a.grad_v), a.grad_v_token, a.grad_v_head);
+    return check_hip(hipGetLastError(), "attention_grad_sinks_sum_kernel launch");
   }
   return FSP_OK;
 }
 
-template <typename T>
-int launch_backward_dim(const fsp_attention_packed_args& a, hipStream_t st) {
-  if (a.dim <= 64) return launch_backward<T, 64>(a, st);
-  if (a.dim <= 96) return launch_backward<T, 96>(a, st);
-  return launch_backward<T, 128>(a, st);
+template <typename T, int DP, bool SINKS>
+int launch_backward(const Call& a, hipStream_t st) {
+  if (a.n_q_tiles > 0) {
+    const int rc = halve_tiles(a, kCus / 2) ? launch_grad_q<T, DP, 2, 2, SINKS>(a, st)
+                   : share_queries(a, kCus) ? launch_grad_q<T, DP, 4, 2, SINKS>(a, st)
+                                            : launch_grad_q<T, DP, 4, 1, SINKS>(a, st);
+    if (rc) return rc;
+  }
+  if (a.n_k_tiles > 0) {
+    const int split = split_heads(a.n_k_tiles, a.heads, a.kv_heads, a.causal && !a.window);
+    if (halve_keys(a, split)) return launch_grad_kv<T, DP, 1, 4, SINKS>(a, split, st);
+    return share_keys(a, split) ? launch_grad_kv<T, DP, 2, 4, SINKS>(a, split, st)
+                                : launch_grad_kv<T, DP, 2, 2, SINKS>(a, split, st);
+  }
+  return FSP_OK;
 }
 
-int check_packed(const fsp_attention_packed_args& a, const std::string& who) {
+template <typename T, bool SINKS>
+int launch_backward_dim(const Call& a, hipStream_t st) {
+  if (a.dim <= 64) return launch_backward<T, 64, SINKS>(a, st);
+  if (a.dim <= 96) return launch_backward<T, 96, SINKS>(a, st);
+  return launch_backward<T, 128, SINKS>(a, st);
+}
+
+int check_packed(const Call& a, const std::string& who) {
   if (!attn_dtype(a.dtype)) return set_error(FSP_ENOTSUP, who + ": dtype");
   if (!attn_dim(a.dim)) return set_error(FSP_ENOTSUP, who + ": dim");
   if (a.kv_heads < 1 || a.heads < 1 || a.heads % a.kv_heads || a.heads > 0xffff)
@@ -975,6 +1150,8 @@ int check_packed(const fsp_attention_packed_args& a, const std::string& who) {
     return set_error(FSP_EINVAL, who + ": a token's step must lie between dim and 2^23");
   if (!isfinite((float)a.scale)) return set_error(FSP_EINVAL, who + ": scale must be finite in 32 bits");
   if (a.window && !a.causal) return set_error(FSP_EINVAL, who + ": window needs causal");
+  if (a.sinks < 0 || a.sinks > kAttnTokensCap || (a.sinks && !a.window))
+    return set_error(FSP_EINVAL, who + ": sinks need a window");
   if ((a.n_q_tiles > 0 && (!a.q_tiles || !a.q_halves || !a.q || !a.out || !a.lse)) ||
       (a.n_k_tiles > 0 && (!a.k_tiles || !a.k_halves)) || (a.k_tokens > 0 && (!a.k || !a.v)))
     return set_error(FSP_EINVAL, who + ": null pointer");
@@ -995,40 +1172,86 @@ extern "C" int64_t fsp_attention_packed_workspace(int64_t n_k_tiles, int64_t hea
   if (n_k_tiles < 0 || heads < 1 || kv_heads < 1 || dim < 0 || q_tokens < 0 || k_tokens < 0) return 0;
   const int split = split_heads(n_k_tiles, heads, kv_heads, uneven);
   const int64_t stats = (2 * heads * q_tokens + 3) & ~int64_t(3);
-  return sizeof(float) * (stats + (split > 1 ? 2 * split * kv_heads * k_tokens * dim : 0));
+  return sizeof(float) * (stats + share_floats(split, kv_heads, k_tokens, dim));
+}
+
+extern "C" int64_t fsp_attention_packed_sinks_workspace(int64_t n_k_tiles, int64_t heads,
+                                                        int64_t kv_heads, int64_t dim, int64_t q_tokens,
+                                                        int64_t k_tokens, int64_t k_longest,
+                                                        int64_t batch, int64_t window, int64_t sinks) {
+  const int64_t rest = fsp_attention_packed_workspace(n_k_tiles, heads, kv_heads, dim, q_tokens, k_tokens, 0);
+  if (rest <= 0 || sinks <= 0 || batch < 0 || window < 1 || k_longest < 0) return rest;
+  const int64_t rows = (first_keys(sinks, k_longest) + kRows - 1) / kRows * kRows;
+  return rest + sizeof(float) * 2 * job_slots(q_tokens, batch, window) *
+                    split_heads(n_k_tiles, heads, kv_heads, false) * kv_heads * rows * dim;
 }
 
 extern "C" int64_t fsp_attention_packed_tile(int which) {
   return which == 0 ? kTile : which == 1 ? kTile / 2 : which == 2 ? kRows : kRows / 2;
 }
 
-extern "C" int fsp_attention_packed(const fsp_attention_packed_args* args, void* stream) {
-  if (!args) return set_error(FSP_EINVAL, "fsp_attention_packed: null arguments");
-  const fsp_attention_packed_args& a = *args;
-  if (int rc = check_packed(a, "fsp_attention_packed")) return rc;
+namespace {
+
+int run_forward(const Call& a, const std::string& who, void* stream) {
+  if (int rc = check_packed(a, who)) return rc;
   if (a.n_q_tiles == 0) return FSP_OK;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return a.dtype == FSP_BF16 ? launch_forward_dim<bf16>(a, st) : launch_forward_dim<f16>(a, st);
+  if (a.sinks)
+    return a.dtype == FSP_BF16 ? launch_forward_dim<bf16, true>(a, st) : launch_forward_dim<f16, true>(a, st);
+  return a.dtype == FSP_BF16 ? launch_forward_dim<bf16, false>(a, st) : launch_forward_dim<f16, false>(a, st);
 }
 
-extern "C" int fsp_attention_packed_backward(const fsp_attention_packed_args* args, void* stream) {
-  if (!args) return set_error(FSP_EINVAL, "fsp_attention_packed_backward: null arguments");
-  const fsp_attention_packed_args& a = *args;
-  if (int rc = check_packed(a, "fsp_attention_packed_backward")) return rc;
+int run_backward(const Call& a, const std::string& who, void* stream) {
+  if (int rc = check_packed(a, who)) return rc;
   // without queries, and with one share of the heads, there is nothing to keep
-  const bool work = a.n_k_tiles > 0 && fsp_attention_packed_workspace(a.n_k_tiles, a.heads, a.kv_heads, a.dim,
-                                                                      a.q_tokens, a.k_tokens,
-                                                                      a.causal && !a.window) > 0;
+  const bool work = a.n_k_tiles > 0 && (a.sinks || fsp_attention_packed_workspace(
+      a.n_k_tiles, a.heads, a.kv_heads, a.dim, a.q_tokens, a.k_tokens, a.causal && !a.window) > 0);
   if ((a.n_q_tiles > 0 && (!a.grad_out || !a.grad_q || !a.workspace)) ||
       (a.n_k_tiles > 0 && (!a.grad_k || !a.grad_v)) || (work && !a.workspace))
-    return set_error(FSP_EINVAL, "fsp_attention_packed_backward: null pointer");
+    return set_error(FSP_EINVAL, who + ": null pointer");
   if (reinterpret_cast<uintptr_t>(a.workspace) % 16)
-    return set_error(FSP_EINVAL, "fsp_attention_packed_backward: workspace must be 16-byte aligned");
+    return set_error(FSP_EINVAL, who + ": workspace must be 16-byte aligned");
   if (!aligned16(a.grad_out, a.grad_out_token, a.grad_out_head) ||
       !aligned16(a.grad_q, a.grad_q_token, a.grad_q_head) ||
       !aligned16(a.grad_k, a.grad_k_token, a.grad_k_head) ||
       !aligned16(a.grad_v, a.grad_v_token, a.grad_v_head))
-    return set_error(FSP_EINVAL, "fsp_attention_packed_backward: rows must be 16-byte aligned");
+    return set_error(FSP_EINVAL, who + ": rows must be 16-byte aligned");
+  if (a.sinks && a.n_k_tiles > 0) {
+    if (a.batch < 1 || !a.sequences) return set_error(FSP_EINVAL, who + ": sequences");
+    // tiles of 32 keys, the most jobs
+    const int64_t tiles = (first_keys(a.sinks, a.k_longest) + kRows / 2 - 1) / (kRows / 2);
+    const int64_t all = kMaxBlocks / a.heads - a.n_k_halves - 8;
+    if (a.batch > kMaxBlocks || (tiles > 0 && job_slots(a.q_tokens, a.batch, a.window) > all / tiles) ||
+        a.batch > kMaxBlocks / a.kv_heads / (tiles * (kRows / 2) * (a.dim / 4) / 128 + 1))
+      return set_error(FSP_EINVAL, who + ": sinks of so many sequences");
+  }
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return a.dtype == FSP_BF16 ? launch_backward_dim<bf16>(a, st) : launch_backward_dim<f16>(a, st);
+  if (a.sinks)
+    return a.dtype == FSP_BF16 ? launch_backward_dim<bf16, true>(a, st) : launch_backward_dim<f16, true>(a, st);
+  return a.dtype == FSP_BF16 ? launch_backward_dim<bf16, false>(a, st) : launch_backward_dim<f16, false>(a, st);
+}
+
+}  // namespace
+
+extern "C" int fsp_attention_packed(const fsp_attention_packed_args* args, void* stream) {
+  if (!args) return set_error(FSP_EINVAL, "fsp_attention_packed: null arguments");
+  return run_forward({*args}, "fsp_attention_packed", stream);
+}
+
+extern "C" int fsp_attention_packed_backward(const fsp_attention_packed_args* args, void* stream) {
+  if (!args) return set_error(FSP_EINVAL, "fsp_attention_packed_backward: null arguments");
+  return run_backward({*args}, "fsp_attention_packed_backward", stream);
+}
+
+extern "C" int fsp_attention_packed_sinks(const fsp_attention_packed_args* args, int64_t sinks,
+                                          void* stream) {
+  if (!args) return set_error(FSP_EINVAL, "fsp_attention_packed_sinks: null arguments");
+  return run_forward({*args, sinks}, "fsp_attention_packed_sinks", stream);
+}
+
+extern "C" int fsp_attention_packed_sinks_backward(const fsp_attention_packed_args* args, int64_t sinks,
+                                                   const int32_t* sequences, int64_t batch,
+                                                   void* stream) {
+  if (!args) return set_error(FSP_EINVAL, "fsp_attention_packed_sinks_backward: null arguments");
+  return run_backward({*args, sinks, batch, sequences}, "fsp_attention_packed_sinks_backward", stream);
 }

@@ -204,6 +204,17 @@ __device__ __forceinline__ void piece_and_head(int block, int n_pieces, int head
 struct PagedShape {
   int heads, window, piece, n_pieces;
   float scale;
+  int sinks;
+};
+
+// What a query sees of the ``last`` tokens of its sequence under a window: they are counted as if the
+// first ones that stay visible lay right before the others, so that it sees the places [first, last), and
+// place e is token e from ``old`` on and e - first before it.
+struct Seen {
+  int first, old;
+  __device__ Seen(const PagedShape& s, int last)
+      : first(s.window ? (int)max((int64_t)last - s.window - s.sinks, (int64_t)0) : 0),
+        old(s.window ? max(last - s.window, 0) : 0) {}
 };
 
 // The next step's keys are asked for once this step's scores are made, its values once this step's
@@ -244,7 +255,9 @@ __global__ __launch_bounds__(256, 3) void attention_paged_kernel(
   const int length = lengths[b];
   const bool ok = length >= 0 && length <= pc.room;
   // the query sees tokens [first, last); the sequence's pieces in use, and whether this is one
-  const int last = ok ? length : 0, first = s.window && last > s.window ? last - s.window : 0;
+  const int last = ok ? length : 0;
+  const Seen seen(s, last);
+  const int first = seen.first;
   const int p0 = first / s.piece, p1 = max(p0 + 1, (last + s.piece - 1) / s.piece);
   const int mine = pc.begin / s.piece;
   if (mine < p0 || mine >= p1) return;
@@ -265,7 +278,8 @@ __global__ __launch_bounds__(256, 3) void attention_paged_kernel(
   // where the keys lie; those past the end stand for the first one, and weigh nothing
   const int padded = (n + 127) & ~127;
   for (int i = threadIdx.x; i < padded; i += 256) {
-    const uint32_t j = begin + (i < n ? i : 0);
+    const int e = begin + (i < n ? i : 0);
+    const uint32_t j = e < seen.old ? e - first : e;
     const uint32_t at = j / (uint32_t)c.page_size;
     const int64_t page = n > 0 ? c.indices[pc.page + at] : 0, slot = j - at * c.page_size;
     s_k[i] = page * c.k_page + slot * c.k_slot;
@@ -485,7 +499,7 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(
   const int length = lengths[b], room = (c.indptr[b + 1] - c.indptr[b]) * c.page_size;
   const int slot = first_piece[b];
   const int last = length >= 0 && length <= room ? length : 0;
-  const int first = s.window && last > s.window ? last - s.window : 0;
+  const int first = Seen(s, last).first;
   const int p0 = first / s.piece, p1 = max(p0 + 1, (last + s.piece - 1) / s.piece), n = p1 - p0;
   if (n < 2) return;
   const int64_t at = (int64_t)(slot + p0) * s.heads + h;
@@ -595,14 +609,19 @@ int launch_append_mode(const fsp_paged_append_args& a, hipStream_t st) {
   return launch_append<T, kEach>(a, st);
 }
 
+struct PagedCall : fsp_attention_paged_args {
+  int64_t sinks;
+};
+
 int64_t paged_workgroups(const fsp_attention_paged_args& a) {
   const int64_t group = a.heads / a.cache.kv_heads;
   return a.n_pieces * a.cache.kv_heads * ((group + kHeadTile - 1) / kHeadTile);
 }
 
 template <typename T, int DP, bool EXACT, bool NT>
-int launch_paged(const fsp_attention_paged_args& a, hipStream_t st) {
-  const PagedShape s{(int)a.heads, (int)a.window, (int)a.piece, (int)a.n_pieces, (float)a.scale};
+int launch_paged(const PagedCall& a, hipStream_t st) {
+  const PagedShape s{(int)a.heads,    (int)a.window,  (int)a.piece,
+                     (int)a.n_pieces, (float)a.scale, (int)a.sinks};
   float* part_o = static_cast<float*>(a.workspace);
   float* part_ml = part_o + a.n_pieces * a.heads * a.cache.dim;
   hipLaunchKernelGGL((attention_paged_kernel<T, DP, EXACT, NT>), dim3((unsigned)paged_workgroups(a)),
@@ -625,7 +644,7 @@ int launch_paged(const fsp_attention_paged_args& a, hipStream_t st) {
 // leave no lines behind, unless several workgroups read the same keys.  6 sequences of 131072 tokens,
 // 3.2 GB: 601 us with ordinary loads, 554 so; 200 MB read again and again: 42 and 55 us.
 template <typename T, int DP, bool EXACT>
-int launch_paged_nt(const fsp_attention_paged_args& a, hipStream_t st) {
+int launch_paged_nt(const PagedCall& a, hipStream_t st) {
   const int64_t bytes = a.cache.table_len * a.cache.page_size * a.cache.kv_heads * a.cache.dim * 4;
   return bytes > (256 << 20) && a.heads / a.cache.kv_heads <= kHeadTile
              ? launch_paged<T, DP, EXACT, true>(a, st)
@@ -633,7 +652,7 @@ int launch_paged_nt(const fsp_attention_paged_args& a, hipStream_t st) {
 }
 
 template <typename T>
-int launch_paged_dim(const fsp_attention_paged_args& a, hipStream_t st) {
+int launch_paged_dim(const PagedCall& a, hipStream_t st) {
   if (a.cache.dim == 64) return launch_paged_nt<T, 64, true>(a, st);
   if (a.cache.dim < 64) return launch_paged_nt<T, 64, false>(a, st);
   if (a.cache.dim < 128) return launch_paged_nt<T, 128, false>(a, st);
@@ -690,28 +709,42 @@ extern "C" int64_t fsp_attention_paged_workspace(int64_t n_pieces, int64_t heads
   return n_pieces * heads * (dim + 2) * (int64_t)sizeof(float);
 }
 
-extern "C" int fsp_attention_paged(const fsp_attention_paged_args* args, void* stream) {
-  if (!args) return set_error(FSP_EINVAL, "fsp_attention_paged: null arguments");
-  const fsp_attention_paged_args& a = *args;
-  if (int rc = check_cache(a.cache, "fsp_attention_paged")) return rc;
+namespace {
+
+int run_paged(const PagedCall& a, const std::string& who, void* stream) {
+  if (int rc = check_cache(a.cache, who)) return rc;
   if (a.heads < 1 || a.heads % a.cache.kv_heads || a.heads > 0xffff)
-    return set_error(FSP_EINVAL, "fsp_attention_paged: heads must be a multiple of kv_heads");
+    return set_error(FSP_EINVAL, who + ": heads must be a multiple of kv_heads");
   if (!isfinite((float)a.scale))
-    return set_error(FSP_EINVAL, "fsp_attention_paged: scale must be finite in 32 bits");
+    return set_error(FSP_EINVAL, who + ": scale must be finite in 32 bits");
   if (a.window < 0 || a.window > 0x7fffffffLL)
-    return set_error(FSP_EINVAL, "fsp_attention_paged: window");
+    return set_error(FSP_EINVAL, who + ": window");
+  if (a.sinks < 0 || a.sinks > 0x7fffffffLL || (a.sinks && !a.window))
+    return set_error(FSP_EINVAL, who + ": sinks need a window");
   if (a.piece < 128 || a.piece > kPieceMost || a.piece % 128)
-    return set_error(FSP_EINVAL, "fsp_attention_paged: piece must be a multiple of 128 up to 1024");
+    return set_error(FSP_EINVAL, who + ": piece must be a multiple of 128 up to 1024");
   if (a.n_pieces < a.cache.batch || a.n_pieces > 0x7fffffffLL || a.cache.batch * a.heads > kMaxBlocks ||
       paged_workgroups(a) > kMaxBlocks)
-    return set_error(FSP_EINVAL, "fsp_attention_paged: pieces out of range");
+    return set_error(FSP_EINVAL, who + ": pieces out of range");
   if (a.cache.batch == 0) return FSP_OK;
   if (!a.q || !a.out || !a.lengths || !a.pieces ||
       (a.n_pieces > a.cache.batch && (!a.workspace || (!a.arrived && !a.first_piece))))
-    return set_error(FSP_EINVAL, "fsp_attention_paged: null pointer");
+    return set_error(FSP_EINVAL, who + ": null pointer");
   if (!aligned16(a.q, a.q_token, a.q_head) || !aligned16(a.out, a.out_token, a.out_head) ||
       reinterpret_cast<uintptr_t>(a.workspace) % 16)
-    return set_error(FSP_EINVAL, "fsp_attention_paged: rows must be 16-byte aligned");
+    return set_error(FSP_EINVAL, who + ": rows must be 16-byte aligned");
   hipStream_t st = static_cast<hipStream_t>(stream);
   return a.cache.dtype == FSP_BF16 ? launch_paged_dim<bf16>(a, st) : launch_paged_dim<f16>(a, st);
+}
+
+}  // namespace
+
+extern "C" int fsp_attention_paged(const fsp_attention_paged_args* args, void* stream) {
+  if (!args) return set_error(FSP_EINVAL, "fsp_attention_paged: null arguments");
+  return run_paged({*args, 0}, "fsp_attention_paged", stream);
+}
+
+extern "C" int fsp_attention_paged_sinks(const fsp_attention_paged_args* args, int64_t sinks, void* stream) {
+  if (!args) return set_error(FSP_EINVAL, "fsp_attention_paged_sinks: null arguments");
+  return run_paged({*args, sinks}, "fsp_attention_paged_sinks", stream);
 }

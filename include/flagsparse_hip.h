@@ -762,6 +762,9 @@ int64_t fsp_attention_paged_counts(int64_t n_pieces, int64_t most, int64_t batch
 int64_t fsp_attention_paged_piece(int64_t tokens, int64_t kv_heads);
 int64_t fsp_attention_paged_workspace(int64_t n_pieces, int64_t heads, int64_t dim);
 int fsp_attention_paged(const struct fsp_attention_paged_args* args, void* stream);
+/* The same where the sequence's first `sinks` tokens stay visible under a window (sinks > 0: window > 0):
+ * key j is seen if j >= lengths[b] - window or j < sinks. */
+int fsp_attention_paged_sinks(const struct fsp_attention_paged_args* args, int64_t sinks, void* stream);
 
 /*
  * Attention over packed sequences: sequence b's queries are tokens
@@ -810,6 +813,19 @@ int64_t fsp_attention_packed_workspace(int64_t n_k_tiles, int64_t heads, int64_t
                                        int64_t q_tokens, int64_t k_tokens, int uneven);
 int fsp_attention_packed(const struct fsp_attention_packed_args* args, void* stream);
 int fsp_attention_packed_backward(const struct fsp_attention_packed_args* args, void* stream);
+/*
+ * The same where each sequence's first `sinks` keys stay visible under a window (sinks > 0: window > 0):
+ * a window hides the keys sinks <= j <= i + nk - nq - window.  The backward pass takes the sequences
+ * as tiles, [batch, 8] int32 {0, 0, 0, q begin, q count, k begin, k count, 0} in their order,
+ * and a workspace of fsp_attention_packed_sinks_workspace() bytes.
+ */
+int fsp_attention_packed_sinks(const struct fsp_attention_packed_args* args, int64_t sinks, void* stream);
+int fsp_attention_packed_sinks_backward(const struct fsp_attention_packed_args* args, int64_t sinks,
+                                        const int32_t* sequences, int64_t batch, void* stream);
+int64_t fsp_attention_packed_sinks_workspace(int64_t n_k_tiles, int64_t heads, int64_t kv_heads,
+                                             int64_t dim, int64_t q_tokens, int64_t k_tokens,
+                                             int64_t k_longest, int64_t batch, int64_t window,
+                                             int64_t sinks);
 
 #ifdef __cplusplus
 }

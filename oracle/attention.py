@@ -19,14 +19,14 @@ TINY = {torch.bfloat16: 2.0**-133, torch.float16: 2.0**-25}
 SLACK = 1.05  # second order
 
 
-def seen(nq, nk, causal, window):
+def seen(nq, nk, causal, window, sinks=0):
     i = torch.arange(nq)[:, None] + nk - nq
     j = torch.arange(nk)
     m = torch.ones(nq, nk, dtype=torch.bool)
     if causal:
         m &= j <= i
     if window:
-        m &= j > i - window
+        m &= (j > i - window) | (j < sinks)
     return m
 
 
@@ -60,8 +60,9 @@ def one(q, k, v, mask, scale, grad=None):
     return r
 
 
-def packed(q, k, v, q_len, k_len, causal, window, scale, grad=None, small=1.0):
+def packed(q, k, v, q_len, k_len, causal, window, scale, grad=None, small=1.0, sinks=0, masks=None):
     """Every sequence and head: {name: (value, bound)} in float64 on the CPU, in q's type's bounds.
+    ``masks``: what the queries of each sequence see, where it is not what causal and window say.
     ``small``: what the type's smallest steps may cost an operand, in units of tiny; a kernel that
     multiplies its weights by 2^n before it rounds them has 2^-n."""
     u, tiny = U[q.dtype], TINY[q.dtype]
@@ -76,8 +77,8 @@ def packed(q, k, v, q_len, k_len, causal, window, scale, grad=None, small=1.0):
                 "v": (torch.zeros_like(v), torch.zeros_like(v))}
     tq = tk = 0
     f = 2.0**-20
-    for nq, nk in zip(q_len, k_len):
-        mask = seen(nq, nk, causal, window)
+    for n, (nq, nk) in enumerate(zip(q_len, k_len)):
+        mask = seen(nq, nk, causal, window, sinks) if masks is None else masks[n]
         a, b = slice(tq, tq + nq), slice(tk, tk + nk)
         for x in range(h):
             y = x // (h // g)

@@ -1,0 +1,87 @@
+"""First tokens that stay visible under a window, without a GPU: refusals of the library and its sizes."""
+
+import numpy as np
+import pytest
+import torch
+
+import flagsparse_amd as fs
+from flagsparse_amd import _abi, attention
+from oracle import attention as ref
+from tests import test_attention_cpu as base
+
+
+@pytest.mark.parametrize("sinks,window,status", [(-1, 5, -1), (4, 0, -1), (2**31, 5, -1), (2**40, 5, -1)])
+def test_refusals_of_the_library(sinks, window, status):
+    L = _abi.lib()
+    assert L.fsp_attention_packed_sinks(base._packed(window=window), sinks, None) == status
+    assert L.fsp_attention_packed_sinks_backward(base._packed(window=window), sinks, 64, 1, None) == status
+    assert L.fsp_attention_paged_sinks(base._cache() + base._paged(window=window), sinks, None) == status
+    assert L.fsp_last_error()
+
+
+def test_null_arguments():
+    L = _abi.lib()
+    assert L.fsp_attention_packed_sinks(None, 4, None) == -1
+    assert L.fsp_attention_packed_sinks_backward(None, 4, None, 0, None) == -1
+    assert L.fsp_attention_paged_sinks(None, 4, None) == -1
+    for sequences, batch in ((None, 1), (64, 0), (64, -1), (64, 2**40)):
+        assert L.fsp_attention_packed_sinks_backward(base._packed(window=5), 4, sequences, batch, None) == -1
+    assert L.fsp_attention_packed_sinks_backward(base._packed(window=5, work=0), 4, 64, 1, None) == -1
+
+
+@pytest.mark.parametrize("kw", [{"dtype": 0}, {"dim": 132}, {"heads": 3}, {"q": 72}, {"q_tokens": 2**31 - 1}])
+def test_what_the_calls_without_refuse(kw):
+    L = _abi.lib()
+    kw = {"window": 5} | kw
+    assert L.fsp_attention_packed_sinks(base._packed(**kw), 4, None) < 0
+    assert L.fsp_attention_packed_sinks_backward(base._packed(**kw), 4, 64, 1, None) < 0
+
+
+def test_jobs_that_a_launch_cannot_hold():
+    # jobs of 32 first keys and 512 queries each, times the key heads, are workgroups of one launch
+    many = base._packed(window=5, q_tokens=2**31 - 1024, k_tokens=2**31 - 1024, k_longest=2**31 - 1024)
+    assert _abi.lib().fsp_attention_packed_sinks_backward(many, 2**31 - 1024, 64, 1, None) == -1
+
+
+@pytest.mark.parametrize("q_len,chunk", [([0], 512), ([5, 0, 700, 512, 513], 512), ([1] * 900, 512),
+                                         ([1024, 0, 0, 3], 640)])
+def test_slots_of_jobs_are_apart(q_len, chunk):
+    # slot q_begin / chunk + b + i for the i-th chunk of sequence b, fewer than q_tokens / chunk + batch
+    begin = np.cumsum(q_len) - q_len
+    taken = [int(q) // chunk + b + i for b, (q, n) in enumerate(zip(begin, q_len))
+             for i in range(-(-n // chunk))]
+    assert len(set(taken)) == len(taken)
+    assert not taken or max(taken) < sum(q_len) // chunk + len(q_len)
+
+
+def test_workspace_holds_the_jobs():
+    L = _abi.lib()
+    sizes = (40, 8, 2, 64, 1000, 1000)
+    without = L.fsp_attention_packed_workspace(*sizes, 0)
+    assert L.fsp_attention_packed_sinks_workspace(*sizes, 600, 3, 100, 0) == without
+    rows = L.fsp_attention_packed_sinks_workspace(*sizes, 600, 3, 100, 4) - without
+    # 1000 / 512 + 3 slots, two key heads, 64 rows of keys and of values, 32 bits, shares of 4 heads
+    assert rows % (4 * 2 * 64 * 2 * 64 * 4) == 0 and rows // (4 * 2 * 64 * 2 * 64 * 4) in (1, 2, 4)
+    assert L.fsp_attention_packed_sinks_workspace(*sizes, 600, 3, 100, 70) - without == 2 * rows
+    assert L.fsp_attention_packed_sinks_workspace(*sizes, 600, 3, 100, 2**30) - without == 10 * rows
+
+
+def test_sinks_of():
+    assert attention._sinks_of(None, 0) == 0 and attention._sinks_of(0, 0) == 0
+    assert attention._sinks_of(3, 5) == 3 and attention._sinks_of(2**40, 5) == 2**31 - 1024
+    for sinks, window in ((3, 0), (-1, 5)):
+        with pytest.raises(ValueError):
+            attention._sinks_of(sinks, window)
+
+
+def test_reference_sees_first_keys():
+    m = ref.seen(4, 6, True, 2, 1)
+    assert m.tolist() == [[True, True, True, False, False, False], [True, False, True, True, False, False],
+                          [True, False, False, True, True, False], [True, False, False, False, True, True]]
+    assert torch.equal(ref.seen(4, 6, True, 2, 0), ref.seen(4, 6, True, 2))
+
+
+def test_refusals_that_need_no_device():
+    q = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        fs.flagsparse_attention_packed(q, q, q, torch.tensor([0, 4]), window=2, sinks=1)
