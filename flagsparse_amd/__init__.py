@@ -22,6 +22,7 @@ from .attention import (
     flagsparse_attention_packed,
     flagsparse_attention_packed_backward,
     flagsparse_attention_paged,
+    flagsparse_attention_paged_tree,
     flagsparse_paged_append,
     prepare_attention_packed,
     prepare_paged_kv,
@@ -80,6 +81,7 @@ ATTENTION_EXPORTS = (
     "flagsparse_attention_packed",
     "flagsparse_attention_packed_backward",
     "flagsparse_attention_paged",
+    "flagsparse_attention_paged_tree",
     "flagsparse_paged_append",
 )
 

@@ -5,6 +5,7 @@ batch, or over the pages that a cache holds of each sequence (``indices``: the p
 
 * ``flagsparse_paged_append``: new keys and values, rotated by their positions, into the cache;
 * ``flagsparse_attention_paged``: one new query per sequence over all that the cache holds of it;
+* ``flagsparse_attention_paged_tree``: the queries of a tree of drafted tokens, of which each sees its way;
 * ``flagsparse_attention_packed`` and ``..._backward``: whole sequences, packed one after the other,
   causal, with a sliding window, or between two batches of sequences; with its gradient.
 
@@ -42,6 +43,7 @@ _CACHE = struct.Struct("17q")
 _APPEND, _APPEND_AT = struct.Struct("13q"), struct.Struct("8q")
 _PAGED, _PAGED_AT = struct.Struct("6qd4q"), struct.Struct("6q")
 _PACKED, _PACKED_AT = struct.Struct("10qd24q"), struct.Struct("10q")
+_TREE, _TREE_AT = struct.Struct("6qd7q"), struct.Struct("7q")
 
 # A prepared object keeps the first part for each layout of arrays that it has checked, so that the
 # next call with such arrays is a look-up and a launch.  Of a cache it holds the pages' addresses, which
@@ -202,8 +204,8 @@ def _result(out, name, shape, dtype, device, *inputs):
     return torch.empty(shape, dtype=dtype, device=device), True
 
 
-def _int32(t, name, length, device):
-    """A contiguous int32 device array of ``length``."""
+def _int32(t, name, length, device, least=-1):
+    """A contiguous int32 device array of ``length``; what is less than ``least`` in 64 bits becomes it."""
     if not torch.is_tensor(t) or t.ndim != 1 or t.numel() != length:
         raise ValueError(f"{name} must be a 1D tensor of length {length}")
     if not t.is_cuda or t.device != device:
@@ -211,7 +213,7 @@ def _int32(t, name, length, device):
     if t.dtype not in SUPPORTED_INDEX_DTYPES:
         raise TypeError(f"{name} dtype must be torch.int32 or torch.int64")
     if t.dtype == torch.int64:
-        t = t.clamp(-1, 2**31 - 1).to(torch.int32)
+        t = t.clamp(least, 2**31 - 1).to(torch.int32)
     return t.contiguous()
 
 
@@ -233,7 +235,7 @@ class PreparedPagedKV:
 
     __slots__ = ("k_pages", "v_pages", "dtype", "device", "indptr", "indices", "batch", "n_pages",
                  "page_size", "kv_heads", "dim", "room", "_piece", "_pieces", "_first", "_most", "_streams",
-                 "_calls", "_counts")
+                 "_calls", "_counts", "_held", "_lists")
 
     def __init__(self, k_pages, v_pages, indptr, indices, pages):
         self.k_pages = k_pages
@@ -246,15 +248,12 @@ class PreparedPagedKV:
         self.n_pages, self.page_size, self.kv_heads, self.dim = (int(n) for n in k_pages.shape)
         rooms = pages * self.page_size
         self.room = int(rooms.max()) if len(rooms) else 0
+        self._held = pages  # of each sequence, on the host
+        self._lists = {}  # pieces of other sizes, or under a window: see _list
         # the pieces that attention is cut into
         self._piece = int(_abi.lib().fsp_attention_paged_piece(int(rooms.sum()), self.kv_heads))
-        table, first, self._most = _pieces(pages, self.page_size, self._piece)
-        # long pieces first, for short ones to even out the end: 96 ragged sequences of up to 4096 tokens,
-        # 8 heads of 128: 51 us, 55 in the sequences' order
-        held = np.minimum(self._piece, table[:, 4] - table[:, 1])
-        table = table[np.argsort(-held, kind="stable")]
-        both = torch.from_numpy(np.concatenate([table.ravel(), first])).to(k_pages.device)
-        self._pieces, self._first = both[:table.size].view(-1, 8), both[table.size:]
+        self._pieces, self._first, self._most = _on_device(
+            *_pieces(pages, self.page_size, self._piece), self._piece, k_pages.device)
         self._counts = _abi.Calls()  # the pieces' counts of arrivals, by stream and number
         self._streams = _Streams()
         self._calls = _abi.Calls()
@@ -277,12 +276,44 @@ class PreparedPagedKV:
             self._streams.mark(stream, self.device, (self.indptr, self.indices, self._pieces))
         return stream
 
+    def _tokens(self, sight):
+        """The tokens of all sequences that a call reads which sees ``sight`` of each (0: all)."""
+        rooms = self._held * self.page_size
+        return int((np.minimum(rooms, sight) if sight else rooms).sum())
 
-def _pieces(pages, page_size, piece):
+    def _list(self, piece, sight):
+        """(pieces, first pieces, most of one sequence, streams that they are marked on): pieces of
+        ``piece`` tokens, of each sequence no more than ``sight`` tokens in a row can touch (0: all of
+        its room), made when first asked for and kept."""
+        kept = self._lists.get((piece, sight))
+        if kept is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a call's first run with these sizes builds its work list, which "
+                                   "cannot be captured: make one such call before the capture")
+            table = _on_device(*_pieces(self._held, self.page_size, piece, sight), piece, self.device)
+            torch.cuda.current_stream(self.device).synchronize()  # calls may come from other streams
+            kept = (*table, _Streams())
+            _keep(self._lists, (piece, sight), kept)
+        return kept
+
+
+def _on_device(table, first, most, piece, device):
+    """The lists of _pieces on the device.  Long pieces first, for short ones to even out the end: 96 ragged
+    sequences of up to 4096 tokens, 8 heads of 128: 51 us, 55 in the sequences' order."""
+    held = np.minimum(piece, table[:, 4] - table[:, 1])
+    table = table[np.argsort(-held, kind="stable")]
+    both = torch.from_numpy(np.concatenate([table.ravel(), first])).to(device)
+    return both[:table.size].view(-1, 8), both[table.size:], most
+
+
+def _pieces(pages, page_size, piece, sight=0):
     """(the pieces of ``piece`` tokens that sequences with so many pages may come to hold, the sequences'
-    first ones, the most that one has), as the kernels read them."""
+    first ones, the most that one has), as the kernels read them; ``sight``: as many as so many tokens in a
+    row can touch, counted from the first one that they do."""
     rooms = pages * page_size
     n = np.maximum(1, -(-rooms // piece))
+    if sight:
+        n = np.minimum(n, -(-sight // piece) + 1)
     slots = np.cumsum(n) - n
     seq = np.repeat(np.arange(len(rooms)), n)
     at = np.arange(len(seq)) - slots[seq]
@@ -558,6 +589,133 @@ def _attend(kv, kept, q, res, lengths, return_lse):
         status = _abi.lib().fsp_attention_paged(args, stream)
     if status:
         _abi.check(status, "fsp_attention_paged")
+    return lse
+
+
+def flagsparse_attention_paged_tree(q, lengths, token_indptr=None, *, parents=None, longest=None,
+                                    prepared=None, k_pages=None, v_pages=None, indptr=None,
+                                    indices=None, scale=None, window=None, sinks=0, out=None,
+                                    return_lse=False):
+    """Attention of trees of drafted tokens over a paged cache that holds them, after the text that they
+    go on from (flagsparse_paged_append).
+
+    ``q``: [tokens, heads, dim], the drafted tokens of each sequence one after the other: sequence b's are
+    ``token_indptr[b]`` to ``token_indptr[b + 1]`` (None: as many for each); ``lengths[b]`` is what
+    sequence b holds with them.  ``parents``: [tokens], for each the place, among its sequence's
+    drafted tokens, of the token before it, which comes earlier, or -1 where that is the text's last one
+    (None: each follows the one before it).  A token sees the text, the drafted tokens on its way up
+    the tree, and itself.  ``window`` and ``sinks`` go by positions, as in flagsparse_attention_paged: a
+    drafted token's is the text's length plus the tokens before it on its way.  ``longest``: no
+    sequence has more drafted tokens, at most 256 (by default 256; a smaller one saves work).
+
+    Returns [tokens, heads, dim], with the float32 log-sum-exp [tokens, heads] if ``return_lse``; neither is
+    differentiable.  With ``prepared`` nothing is waited for, so indices are not checked: rows of a
+    sequence with more drafted tokens than ``longest``, or a length that its pages cannot hold or less than
+    its drafted tokens, rows whose parents do not come earlier, and rows of no sequence are NaN.  What
+    is not finite in a hidden drafted token's value may reach other rows of its sequence (its weight is zero,
+    and zero times it is NaN), in its key it does not.  The first call of its sizes builds a work list
+    and cannot be captured."""
+    key = None
+    if out is None and type(prepared) is PreparedPagedKV and type(scale) in _PLAIN and \
+            type(window) in _PLAIN and type(sinks) in _PLAIN and type(longest) in _PLAIN:
+        key = _layouts(q, lengths, token_indptr, parents) + (
+            "tree", scale, window, sinks, longest, prepared.k_pages.data_ptr(),
+            prepared.v_pages.data_ptr())
+        kept = prepared._calls.get(key)
+        if kept is not None and q.data_ptr() % 16 == 0:
+            res = torch.empty_like(kept[1], memory_format=_CONTIGUOUS)
+            lse = _attend_tree(prepared, kept, q, res, lengths, token_indptr, parents, return_lse)
+            return (res, lse) if return_lse else res
+    kv, n = _paged_of(prepared, k_pages, v_pages, indptr, indices, lengths)
+    dev, dt = kv.device, kv.dtype
+    _check_tensor(q, "q", dt, dev, None, kv.dim)
+    tokens, heads = q.shape[:2]
+    _check_heads(heads, kv.kv_heads)
+    given = (q, lengths, token_indptr, parents)
+    most = int(_abi.lib().fsp_attention_tree_drafts())
+    longest = most if longest is None else int(longest)
+    if longest < 0 or longest > most:
+        raise ValueError(f"longest must lie between 0 and {most}")
+    if token_indptr is None:
+        each = tokens // max(kv.batch, 1)
+        if each * kv.batch != tokens:
+            raise ValueError(f"q must have as many tokens for each of {kv.batch} sequences, got "
+                             f"{tokens}; other numbers need token_indptr")
+        if each > longest:
+            raise ValueError(f"a sequence may have at most {longest} drafted tokens, got {each}")
+        longest = each
+    else:
+        token_indptr = _int32(token_indptr, "token_indptr", kv.batch + 1, dev)
+        longest = min(longest, tokens)
+    if parents is not None:
+        parents = _int32(parents, "parents", tokens, dev, -2)
+    factor, past = _scale_of(scale, kv.dim), _window_of(window)
+    first = _sinks_of(sinks, past)
+    res, copied = _result(out, "out", q.shape, dt, dev, q, kv.k_pages, kv.v_pages)
+    rows = _rows(q)
+    if prepared is None:
+        _check_drafts(kv, n, token_indptr, parents, tokens, longest)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev) if return_lse else None
+    if not kv.batch or not longest:  # tokens of no sequence, or none
+        res.fill_(float("nan"))
+        if return_lse:
+            lse.fill_(float("nan"))
+    else:
+        sight = min(past + first + longest, _TOKENS_CAP) if past else 0
+        piece = int(_abi.lib().fsp_attention_tree_piece(kv._tokens(sight), kv.kv_heads,
+                                                        heads // kv.kv_heads, longest))
+        pieces, firsts, _, marked = kv._list(piece, sight)
+        n_pieces = pieces.shape[0]
+        room = None
+        if n_pieces > kv.batch:
+            room = _like((n_pieces * longest * heads * (kv.dim + 2),), torch.float32, dev)
+        head = kv._packed() + _TREE.pack(
+            pieces.data_ptr(), firsts.data_ptr(), n_pieces, piece, heads, past, factor, first, tokens,
+            longest, *_steps(rows), *_steps(res))
+        kept = (head, _like(q.shape, dt, dev), _like(q.shape[:2], torch.float32, dev), room,
+                (pieces, firsts), marked)
+        lse = _attend_tree(kv, kept, rows, res, n, token_indptr, parents, return_lse)
+        if key is not None and all(x is y for x, y in zip((rows, n, token_indptr, parents), given)):
+            _keep(kv._calls, key, kept)
+    if copied:
+        out.copy_(res)
+        res = out
+    return (res, lse) if return_lse else res
+
+
+def _check_drafts(kv, lengths, token_indptr, parents, tokens, longest):
+    """Of a call whose cache is not prepared: the host waits for it."""
+    if token_indptr is None:
+        count = torch.full((kv.batch,), longest, dtype=torch.int64, device=kv.device)
+    else:
+        p = token_indptr.to(torch.int64)
+        count = p[1:] - p[:-1]
+        if int(p[0]) != 0 or int(p[-1]) != tokens or bool((count < 0).any()):
+            raise ValueError(f"token_indptr must lead from 0 to {tokens} without decreasing")
+        if bool((count > longest).any()):
+            raise ValueError(f"a sequence may have at most {longest} drafted tokens")
+    if bool((count > lengths).any()):
+        raise ValueError("lengths must count the drafted tokens")
+    if parents is not None:
+        place = torch.arange(tokens, device=kv.device) - torch.repeat_interleave(
+            count.cumsum(0) - count, count)
+        if bool(((parents < -1) | (parents >= place)).any()):
+            raise ValueError("parents must come before their tokens, or be -1")
+
+
+def _attend_tree(kv, kept, q, res, lengths, token_indptr, parents, return_lse):
+    """The launch; returns the log-sum-exp, if asked for."""
+    head, _, like_lse, room, lists, marked = kept
+    lse = torch.empty_like(like_lse, memory_format=_CONTIGUOUS) if return_lse else None
+    stream = kv._on()
+    if stream not in marked.seen:
+        marked.mark(stream, kv.device, lists)
+    work = None if room is None else torch.empty_like(room, memory_format=_CONTIGUOUS)
+    args = head + _TREE_AT.pack(q.data_ptr(), res.data_ptr(), _at(lse), lengths.data_ptr(),
+                                _at(token_indptr), _at(parents), _at(work))
+    status = _abi.lib().fsp_attention_tree(args, stream)
+    if status:
+        _abi.check(status, "fsp_attention_tree")
     return lse
 
 

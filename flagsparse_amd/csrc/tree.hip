@@ -1,0 +1,484 @@
+// Attention of trees of drafted tokens over a paged cache that holds them at its sequences' ends.
+#include "paged.hpp"
+
+namespace fsp {
+namespace {
+
+constexpr int kDrafts = 256;     // drafted tokens of one sequence, at most
+constexpr int kTableKeys = 1024;  // keys whose places LDS holds at a time
+
+struct TreeShape {
+  int heads, window, sinks, piece, n_pieces, n_tokens, longest, tiles;
+  float scale;
+};
+
+// A sequence's drafted tokens and what of its keys any of them sees: the places [first, last), where
+// place e is token e from ``old`` on, and one of the first tokens, e - first, before it.
+struct Drafted {
+  int begin, count, past, first, old, last;
+  bool ok;
+  __device__ Drafted(const TreeShape& s, const int32_t* tokens, int b, int length, int room) {
+    begin = tokens ? tokens[b] : b * s.longest;
+    const int end = tokens ? tokens[b + 1] : begin + s.longest;
+    ok = begin >= 0 && begin <= end && end <= s.n_tokens && end - begin <= s.longest &&
+         length >= end - begin && length <= room;
+    count = ok ? end - begin : 0;
+    past = ok ? length - count : 0;
+    last = ok ? length : 0;
+    old = s.window ? max(past + 1 - s.window, 0) : 0;
+    first = s.window ? (int)max((int64_t)past + 1 - s.window - s.sinks, (int64_t)0) : 0;
+  }
+};
+
+// Rows of NaN for the tokens [from, to), those of one key head's queries.
+template <typename T>
+__device__ void nan_rows(T* out, int64_t out_token, int64_t out_head, float* lse, int heads, int head0, int group,
+                         int dim, int from, int to) {
+  const T nan = (T)__builtin_nanf("");
+  const int per = group * (dim / 8);
+  for (int64_t i = threadIdx.x; i < (int64_t)max(to - from, 0) * per; i += 256) {
+    const int64_t t = from + i / per;
+    const int h = head0 + (int)(i % per) / (dim / 8), d = (int)(i % per) % (dim / 8) * 8;
+    *reinterpret_cast<V8<T>*>(out + t * out_token + h * out_head + d) =
+        V8<T>{nan, nan, nan, nan, nan, nan, nan, nan};
+    if (lse && d == 0) lse[t * heads + h] = __builtin_nanf("");
+  }
+}
+
+// Which drafted tokens a row's token sees, itself among them, by its way up the tree, as words 1 .. 8 of
+// ``mask`` between one of ones and one of zeros; returns its depth, or -1 where the way does not lead up.
+__device__ __forceinline__ int row_mask(const TreeShape& s, const Drafted& t, const int* up, int i,
+                                        uint32_t* mask) {
+  mask[0] = ~0u;
+#pragma unroll
+  for (int w = 1; w < 10; ++w) mask[w] = 0;
+  int depth = i;
+  if (up) {
+    depth = 0;
+    for (int at = i;;) {
+      const int p = up[at];
+      if (p < -1 || p >= at) return -1;
+      if (p < 0) break;
+      at = p;
+      ++depth;
+    }
+  }
+  for (int at = i, n = 0; at >= 0; at = up ? up[at] : at - 1, ++n)
+    if (!s.window || n < s.window || t.past + depth - n < s.sinks) mask[1 + at / 32] |= 1u << (at & 31);
+  return depth;
+}
+
+// The rows are the drafted tokens' queries of the heads that share a key head, a token's side by side: row r is
+// token r / group, head r % group.  A workgroup takes a piece of a sequence's tokens for one key
+// head and RT * 16 rows, so that what it reads of the cache serves all of them; its four waves take
+// every fourth 32 keys.  Keys, values and products lie as in attention_paged_kernel, with RT times
+// the rows beside each key: a key's fragment is read from LDS once for all, a value's put together once.
+template <typename T, int DP, bool EXACT, bool NT, int RT>
+__global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attention_tree_kernel(
+    Cache c, TreeShape s, const Piece* __restrict__ pieces, const T* __restrict__ k_pages,
+    const T* __restrict__ v_pages, const T* __restrict__ q, int64_t q_token, int64_t q_head,
+    T* __restrict__ out, int64_t out_token, int64_t out_head, float* __restrict__ lse,
+    const int32_t* __restrict__ lengths, const int32_t* __restrict__ tokens,
+    const int32_t* __restrict__ parents, float* part_o, float* part_ml) {
+  constexpr int E = DP / 16, NS = DP / 32, W = 4, ROWS = 16 * RT;
+  typedef T VE __attribute__((ext_vector_type(E)));
+  constexpr int CH = DP / 8, KL = DP / 16;
+  __shared__ int64_t s_k[kTableKeys], s_v[kTableKeys];
+  typedef float Sums[16][DP + 4];
+  static_assert(sizeof(Sums) >= 64 * DP, "");
+  __shared__ __attribute__((aligned(16))) char s_raw[W * sizeof(Sums)];
+  __shared__ f32x2 s_ml[W][16];
+  __shared__ uint32_t s_mask[ROWS][11];
+  __shared__ int s_depth[ROWS], s_up[kDrafts];
+  Sums* s_o = reinterpret_cast<Sums*>(s_raw);
+  const int group = s.heads / c.kv_heads;
+  int piece, g, tile;
+  piece_and_head(blockIdx.x, s.n_pieces, c.kv_heads * s.tiles, piece, tile);
+  g = tile / s.tiles;
+  tile -= g * s.tiles;
+  const Piece pc = pieces[piece];
+  const int b = pc.seq, lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int head0 = g * group;
+  const Drafted t(s, tokens, b, lengths[b], pc.room);
+  if (pc.begin == 0 && tile == 0) {  // what belongs to no sequence, or to one that is not as it should be
+    const int from = tokens ? min(max(tokens[b], 0), s.n_tokens) : t.begin;
+    const int to = tokens ? min(max(tokens[b + 1], 0), s.n_tokens) : t.begin + s.longest;
+    if (!t.ok) nan_rows(out, out_token, out_head, lse, s.heads, head0, group, c.dim, from, to);
+    if (b == 0) nan_rows(out, out_token, out_head, lse, s.heads, head0, group, c.dim, 0, from);
+    if (b == c.batch - 1) nan_rows(out, out_token, out_head, lse, s.heads, head0, group, c.dim, to, s.n_tokens);
+  }
+  const int rows = t.count * group, r0 = tile * ROWS;
+  if (r0 >= rows) return;
+  const int p0 = t.first / s.piece, p1 = (t.last + s.piece - 1) / s.piece;
+  const int mine = p0 + pc.begin / s.piece;
+  if (mine >= p1) return;
+  const int begin = max(t.first, mine * s.piece);
+  const int end = (int)min((int64_t)t.last, ((int64_t)mine + 1) * s.piece);
+
+  V8<T> qf[RT][NS];
+#pragma unroll
+  for (int n = 0; n < RT; ++n) {
+    const int r = min(r0 + 16 * n + col, rows - 1);
+    const T* qr = q + (int64_t)(t.begin + r / group) * q_token + (head0 + r % group) * q_head;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const int d = 32 * i + 8 * quad;
+      const V8<T> x = *reinterpret_cast<const V8<T>*>(qr + (d < c.dim ? d : 0));
+      qf[n][i] = scaled_sign<T>(x, s.scale, d < c.dim);
+    }
+  }
+  const float cs = exp2_scale(s.scale);
+
+  const bool masked = s.window || end > t.past;
+  if (masked) {
+    if (parents)
+      for (int i = threadIdx.x; i < t.count; i += 256) s_up[i] = parents[t.begin + i];
+    __syncthreads();
+    if (threadIdx.x < ROWS)
+      s_depth[threadIdx.x] = row_mask(s, t, parents ? s_up : nullptr,
+                                      min(r0 + (int)threadIdx.x, rows - 1) / group, s_mask[threadIdx.x]);
+    __syncthreads();
+  }
+  int lo[RT];  // the first token that each row's window holds
+#pragma unroll
+  for (int n = 0; n < RT; ++n) lo[n] = s.window ? t.past + s_depth[16 * n + col] - s.window + 1 : 0;
+
+  const T* kb = k_pages + g * c.k_head;
+  const T* vb = v_pages + g * c.v_head;
+  i32x4 kr[KL];
+  VE vf[8];
+  const int k_row = lane / CH, k_chunk = lane % CH;
+  auto load_k = [&](int j, int most) {
+#pragma unroll
+    for (int i = 0; i < KL; ++i)
+      kr[i] = ld_stream<NT>(reinterpret_cast<const i32x4*>(
+          kb + s_k[min(j + 64 / CH * i + k_row, most)] +
+          (EXACT || 8 * k_chunk < c.dim ? 8 * k_chunk : 0)));
+  };
+  char* s_rows = s_raw + wave * sizeof(Sums);
+  const int ve = E * col < c.dim ? E * col : 0;
+  auto load_v = [&](int j, int most) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      vf[e] = ld_stream<NT>(reinterpret_cast<const VE*>(
+          vb + s_v[min(j + 16 * (e / 4) + 4 * quad + e % 4, most)] + ve));
+  };
+
+  float top[RT], sum[RT];
+  f32x4 o[RT][E];
+#pragma unroll
+  for (int n = 0; n < RT; ++n) {
+    top[n] = -INFINITY;
+    sum[n] = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) o[n][i] = f32x4{};
+  }
+
+  for (int c0 = begin; c0 < end; c0 += kTableKeys) {
+    const int n_keys = min(kTableKeys, end - c0), padded = (n_keys + 127) & ~127;
+    if (c0 > begin) __syncthreads();
+    for (int i = threadIdx.x; i < padded; i += 256) {
+      const int e = c0 + (i < n_keys ? i : 0);
+      const uint32_t j = e < t.old ? e - t.first : e;
+      const uint32_t at = j / (uint32_t)c.page_size;
+      const int64_t page = c.indices[pc.page + at], slot = j - at * c.page_size;
+      s_k[i] = page * c.k_page + slot * c.k_slot;
+      s_v[i] = page * c.v_page + slot * c.v_slot;
+    }
+    __syncthreads();
+    int j = 32 * wave;
+    if (j < n_keys) load_k(j, kTableKeys - 1), load_v(j, kTableKeys - 1);
+    for (; j < n_keys; j += 32 * W) {
+#pragma unroll
+      for (int i = 0; i < KL; ++i) {
+        const int row = 64 / CH * i + k_row;
+        *reinterpret_cast<i32x4*>(s_rows + row * 2 * DP + 16 * (k_chunk ^ (row & (CH - 1)))) =
+            EXACT ? kr[i] : kr[i] & (8 * k_chunk < c.dim ? -1 : 0);
+      }
+      f32x4 x[RT][2];
+#pragma unroll
+      for (int n = 0; n < RT; ++n) x[n][0] = x[n][1] = f32x4{};
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        V8<T> kf[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int row = 16 * u + col;
+          kf[u] = *reinterpret_cast<const V8<T>*>(s_rows + row * 2 * DP +
+                                                  16 * ((4 * i + quad) ^ (row & (CH - 1))));
+        }
+#pragma unroll
+        for (int n = 0; n < RT; ++n)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) x[n][u] = mfma16(kf[u], qf[n][i], x[n][u]);
+      }
+      const bool more = j + 32 * W < n_keys;
+      const int next = more ? j + 32 * W : j, most = more ? kTableKeys - 1 : j;
+      load_k(next, most);
+      const int e0 = c0 + j;  // the places of these keys
+      const bool tail = e0 + 32 > t.past, partial = j + 32 > n_keys;
+      if (partial) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) vf[e] = j + 16 * (e / 4) + 4 * quad + e % 4 < n_keys ? vf[e] : VE{};
+      }
+      V8<T> pf[RT];
+#pragma unroll
+      for (int n = 0; n < RT; ++n) {
+        if (partial || tail || __any(lo[n] > max(e0, t.old))) {
+          const int off = e0 - t.past, w = off >> 5, shift = off & 31;
+          uint32_t bits = ~0u;
+          if (tail) {
+            const uint32_t* m = s_mask[16 * n + col] + 1 + w;
+            bits = shift ? m[0] >> shift | m[1] << (32 - shift) : m[0];
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int k = 16 * (e / 4) + 4 * quad + e % 4, at = e0 + k;
+            const bool near = at >= lo[n] || at < s.sinks || at < t.old || at >= t.past;
+            const bool in = (bits >> k & 1) && near && j + k < n_keys;
+            x[n][e / 4][e % 4] = in ? x[n][e / 4][e % 4] : -INFINITY;
+          }
+        }
+        float m = x[n][0][0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) m = fmaxf(m, x[n][e / 4][e % 4]);
+        if (__any((m - top[n]) * cs > Weights<T>::lag)) {
+          m = fmaxf(m, __shfl_xor(m, 16));
+          m = fmaxf(m, __shfl_xor(m, 32));
+          const float now = fmaxf(top[n], m);
+          const float fade = top[n] == -INFINITY ? 0.0f : exp2f((top[n] - now) * cs);
+          top[n] = now;
+          sum[n] *= fade;
+#pragma unroll
+          for (int i = 0; i < E; ++i) o[n][i] *= fade;
+        }
+        const float base = top[n] == -INFINITY ? 0.0f : top[n] * cs - Weights<T>::up;
+        f32x8 p;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[e] = __builtin_amdgcn_exp2f(fmaf(x[n][e / 4][e % 4], cs, -base));
+          sum[n] += p[e];
+        }
+        pf[n] = __builtin_convertvector(p, V8<T>);
+      }
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        V8<T> a;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a[e] = vf[e][i];
+#pragma unroll
+        for (int n = 0; n < RT; ++n) o[n][i] = mfma16(a, pf[n], o[n][i]);
+      }
+      load_v(next, most);
+    }
+  }
+
+  // join the waves, 16 rows at a time
+  const bool split = p1 - p0 > 1;
+  const int64_t slot = (int64_t)(pc.slot + mine - p0) * s.longest * s.heads + (int64_t)g * s.longest * group;
+#pragma unroll
+  for (int n = 0; n < RT; ++n) {
+    if (r0 + 16 * n >= rows) break;
+    sum[n] += __shfl_xor(sum[n], 16);
+    sum[n] += __shfl_xor(sum[n], 32);
+    const float ml = top[n] == -INFINITY ? -INFINITY : top[n] * cs;
+    __syncthreads();
+    if (quad == 0) s_ml[wave][col] = f32x2{ml, sum[n]};
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s_o[wave][col][4 * E * quad + E * r + i] = o[n][i][r];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * (DP / 4); i += 256) {
+      const int row = i / (DP / 4), d = i % (DP / 4) * 4, r = r0 + 16 * n + row;
+      if (d >= c.dim || r >= rows) continue;
+      float most = -INFINITY, total = 0;
+#pragma unroll
+      for (int w = 0; w < W; ++w) most = fmaxf(most, s_ml[w][row].x);
+      f32x4 y{};
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const f32x2 v = s_ml[w][row];
+        const float f = v.x == -INFINITY ? 0.0f : exp2f(v.x - most);
+        if (v.y == 0) continue;  // saw nothing: its sums are zeros
+        total += f * v.y;
+        y += f * *reinterpret_cast<const f32x4*>(&s_o[w][row][d]);
+      }
+      if (masked && s_depth[16 * n + row] < 0) total = __builtin_nanf("");
+      if (split) {
+        *reinterpret_cast<f32x4*>(part_o + (slot + r) * c.dim + d) = y;
+        if (d == 0) *reinterpret_cast<f32x2*>(part_ml + 2 * (slot + r)) = f32x2{most, total};
+      } else {
+        const int64_t token = t.begin + r / group;
+        const int head = head0 + r % group;
+        y *= total == 0 ? 0.0f : 1.0f / total;
+        *reinterpret_cast<V4<T>*>(out + token * out_token + head * out_head + d) =
+            __builtin_convertvector(y, V4<T>);
+        if (lse && d == 0)
+          lse[token * s.heads + head] =
+              total == 0 ? -INFINITY : (most + log2f(total * Weights<T>::down)) * kLn2;
+      }
+    }
+  }
+}
+
+// Joins the pieces of sequences that have several: half a wave to a row, eight pieces of it at a time.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_tree_join_kernel(
+    Cache c, TreeShape s, const int32_t* __restrict__ first_piece, T* __restrict__ out, int64_t out_token,
+    int64_t out_head, float* __restrict__ lse, const int32_t* __restrict__ lengths,
+    const int32_t* __restrict__ tokens, const float* __restrict__ part_o,
+    const f32x2* __restrict__ part_ml) {
+  constexpr int U = 8;
+  const int group = s.heads / c.kv_heads;
+  const int per = (s.longest * s.heads + 7) / 8, b = blockIdx.x / per;
+  const int i = blockIdx.x % per * 8 + (threadIdx.x >> 5), d = 4 * (threadIdx.x & 31);
+  const int g = i / (s.longest * group), r = i % (s.longest * group);
+  const Drafted t(s, tokens, b, lengths[b], (c.indptr[b + 1] - c.indptr[b]) * c.page_size);
+  const int p0 = t.first / s.piece, n = (t.last + s.piece - 1) / s.piece - p0;
+  if (n < 2 || g >= c.kv_heads || r >= t.count * group) return;
+  const int64_t step = (int64_t)s.longest * s.heads;
+  const int64_t at = first_piece[b] * step + (int64_t)g * s.longest * group + r;
+  const f32x2* ml = part_ml + at;
+  const float* o = part_o + at * c.dim + (d < c.dim ? d : 0);
+  float most = -INFINITY, total = 0;
+  f32x4 y{};
+  for (int p = 0; p < n; p += U) {
+    f32x2 v[U];
+    f32x4 u[U];
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      const int64_t k = min(p + e, n - 1) * step;
+      v[e] = ml[k];
+      u[e] = *reinterpret_cast<const f32x4*>(o + k * c.dim);
+    }
+    float now = most;
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      v[e] = p + e < n ? v[e] : f32x2{-INFINITY, 0};
+      now = fmaxf(now, v[e].x);
+    }
+    const float base = now == -INFINITY ? 0.0f : now;
+    const float fade = exp2f(most - base);
+    most = now;
+    total *= fade;
+    y *= fade;
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      const float f = exp2f(v[e].x - base);
+      total += f * v[e].y;
+      y += f * u[e];
+    }
+  }
+  if (d >= c.dim) return;
+  y *= total == 0 ? 0.0f : 1.0f / total;
+  const int64_t token = t.begin + r / group;
+  const int head = g * group + r % group;
+  *reinterpret_cast<V4<T>*>(out + token * out_token + head * out_head + d) = __builtin_convertvector(y, V4<T>);
+  if (lse && d == 0)
+    lse[token * s.heads + head] = total == 0 ? -INFINITY : (most + log2f(total * Weights<T>::down)) * kLn2;
+}
+
+int row_tiles(int64_t longest, int64_t group) {
+  return longest * group <= 16 ? 1 : 2;
+}
+
+template <typename T, int DP, bool EXACT, bool NT, int RT>
+int launch_tree(const fsp_attention_tree_args& a, hipStream_t st) {
+  const int64_t group = a.heads / a.cache.kv_heads, tiles = (a.longest * group + 16 * RT - 1) / (16 * RT);
+  const TreeShape s{(int)a.heads,    (int)a.window,  (int)a.sinks, (int)a.piece,  (int)a.n_pieces,
+                    (int)a.n_tokens, (int)a.longest, (int)tiles,   (float)a.scale};
+  float* part_o = static_cast<float*>(a.workspace);
+  float* part_ml = part_o + a.n_pieces * a.longest * a.heads * a.cache.dim;
+  hipLaunchKernelGGL((attention_tree_kernel<T, DP, EXACT, NT, RT>),
+                     dim3((unsigned)(a.n_pieces * a.cache.kv_heads * tiles)), dim3(256), 0, st,
+                     cache_of(a.cache), s, reinterpret_cast<const Piece*>(a.pieces),
+                     static_cast<const T*>(a.cache.k_pages), static_cast<const T*>(a.cache.v_pages),
+                     static_cast<const T*>(a.q), a.q_token, a.q_head, static_cast<T*>(a.out), a.out_token,
+                     a.out_head, a.lse, a.lengths, a.token_indptr, a.parents, part_o, part_ml);
+  if (int rc = check_hip(hipGetLastError(), "attention_tree_kernel launch")) return rc;
+  if (a.n_pieces == a.cache.batch) return FSP_OK;
+  hipLaunchKernelGGL((attention_tree_join_kernel<T>),
+                     dim3((unsigned)(a.cache.batch * ((a.longest * a.heads + 7) / 8))), dim3(256), 0, st,
+                     cache_of(a.cache), s, a.first_piece, static_cast<T*>(a.out), a.out_token, a.out_head,
+                     a.lse, a.lengths, a.token_indptr, part_o, reinterpret_cast<const f32x2*>(part_ml));
+  return check_hip(hipGetLastError(), "attention_tree_join_kernel launch");
+}
+
+template <typename T, int DP, bool EXACT, bool NT>
+int launch_tree_rows(const fsp_attention_tree_args& a, hipStream_t st) {
+  const int rt = row_tiles(a.longest, a.heads / a.cache.kv_heads);
+  return rt == 1 ? launch_tree<T, DP, EXACT, NT, 1>(a, st) : launch_tree<T, DP, EXACT, NT, 2>(a, st);
+}
+
+template <typename T, int DP, bool EXACT>
+int launch_tree_nt(const fsp_attention_tree_args& a, hipStream_t st) {
+  const int64_t bytes = a.cache.table_len * a.cache.page_size * a.cache.kv_heads * a.cache.dim * 4;
+  return bytes > (256 << 20) && a.longest * a.heads / a.cache.kv_heads <= 32
+             ? launch_tree_rows<T, DP, EXACT, true>(a, st)
+             : launch_tree_rows<T, DP, EXACT, false>(a, st);
+}
+
+template <typename T>
+int launch_tree_dim(const fsp_attention_tree_args& a, hipStream_t st) {
+  if (a.cache.dim == 64) return launch_tree_nt<T, 64, true>(a, st);
+  if (a.cache.dim < 64) return launch_tree_nt<T, 64, false>(a, st);
+  if (a.cache.dim < 128) return launch_tree_nt<T, 128, false>(a, st);
+  return launch_tree_nt<T, 128, true>(a, st);
+}
+
+}  // namespace
+}  // namespace fsp
+
+using namespace fsp;
+
+extern "C" int64_t fsp_attention_tree_drafts(void) { return kDrafts; }
+
+extern "C" int64_t fsp_attention_tree_piece(int64_t tokens, int64_t kv_heads, int64_t group, int64_t longest) {
+  if (tokens < 0 || kv_heads < 1 || group < 1 || longest < 1) return 256;
+  const int64_t rows = 16 * row_tiles(longest, group), tiles = (longest * group + rows - 1) / rows;
+  int64_t piece = 256;
+  while (piece < 4096 && tokens / piece * kv_heads * tiles > 1024) piece *= 2;
+  return piece;
+}
+
+extern "C" int64_t fsp_attention_tree_workspace(int64_t n_pieces, int64_t heads, int64_t dim, int64_t longest) {
+  if (n_pieces < 0 || heads < 0 || dim < 0 || longest < 0) return 0;
+  return n_pieces * longest * heads * (dim + 2) * (int64_t)sizeof(float);
+}
+
+extern "C" int fsp_attention_tree(const fsp_attention_tree_args* args, void* stream) {
+  if (!args) return set_error(FSP_EINVAL, "fsp_attention_tree: null arguments");
+  const fsp_attention_tree_args& a = *args;
+  if (int rc = check_cache(a.cache, "fsp_attention_tree")) return rc;
+  if (a.heads < 1 || a.heads % a.cache.kv_heads || a.heads > 0xffff)
+    return set_error(FSP_EINVAL, "fsp_attention_tree: heads must be a multiple of kv_heads");
+  if (!isfinite((float)a.scale))
+    return set_error(FSP_EINVAL, "fsp_attention_tree: scale must be finite in 32 bits");
+  if (a.window < 0 || a.window > kAttnTokensCap || a.sinks < 0 || a.sinks > kAttnTokensCap ||
+      (a.sinks && !a.window))
+    return set_error(FSP_EINVAL, "fsp_attention_tree: window, or sinks without one");
+  if (a.piece < 128 || a.piece > (1 << 20) || a.piece % 128)
+    return set_error(FSP_EINVAL, "fsp_attention_tree: piece must be a multiple of 128 up to 2^20");
+  if (a.n_tokens < 0 || a.n_tokens > kAttnTokensCap || a.longest < 0 || a.longest > kDrafts ||
+      a.n_pieces < a.cache.batch || a.n_pieces > 0x7fffffffLL)
+    return set_error(FSP_EINVAL, "fsp_attention_tree: size out of range");
+  if (!a.token_indptr && a.n_tokens != a.longest * a.cache.batch)
+    return set_error(FSP_EINVAL, "fsp_attention_tree: longest tokens per sequence without token_indptr");
+  if (a.n_tokens == 0) return FSP_OK;
+  if (a.cache.batch == 0 || a.longest == 0)
+    return set_error(FSP_EINVAL, "fsp_attention_tree: tokens of no sequence");
+  const int64_t rows = a.longest * a.heads, group = a.heads / a.cache.kv_heads;
+  if (a.cache.batch > kMaxBlocks / ((rows + 7) / 8) ||
+      a.n_pieces > kMaxBlocks / (a.cache.kv_heads * ((a.longest * group + 15) / 16)))
+    return set_error(FSP_EINVAL, "fsp_attention_tree: pieces out of range");
+  if (!a.q || !a.out || !a.lengths || !a.pieces ||
+      (a.n_pieces > a.cache.batch && (!a.workspace || !a.first_piece)))
+    return set_error(FSP_EINVAL, "fsp_attention_tree: null pointer");
+  if (!aligned16(a.q, a.q_token, a.q_head) || !aligned16(a.out, a.out_token, a.out_head) ||
+      reinterpret_cast<uintptr_t>(a.workspace) % 16)
+    return set_error(FSP_EINVAL, "fsp_attention_tree: rows must be 16-byte aligned");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return a.cache.dtype == FSP_BF16 ? launch_tree_dim<bf16>(a, st) : launch_tree_dim<f16>(a, st);
+}

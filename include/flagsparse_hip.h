@@ -767,6 +767,44 @@ int fsp_attention_paged(const struct fsp_attention_paged_args* args, void* strea
 int fsp_attention_paged_sinks(const struct fsp_attention_paged_args* args, int64_t sinks, void* stream);
 
 /*
+ * Attention of trees of drafted tokens over the cache: q, out [n_tokens, heads, dim], lse
+ * [n_tokens, heads] float32 or NULL.  Sequence b's drafted tokens, at most fsp_attention_tree_drafts() and
+ * `longest`, are rows [token_indptr[b], token_indptr[b + 1]) (NULL: longest rows each) and the last ones that
+ * the cache holds of it (lengths[b] counts them).  parents[row]: the place, among its sequence's
+ * drafted tokens, of the one before it, a smaller place than its own, or -1 (NULL: a chain).  A row sees the
+ * tokens before the drafted ones, and of those the ones on its way up the tree, itself among them.  Its
+ * position is that of its sequence's first drafted token plus the length of its way; with a window it
+ * sees the positions p > its own - window and p < sinks.
+ * A row whose way does not lead up, the rows of a sequence with more drafted tokens than `longest`, with a
+ * length that its pages cannot hold or less than its drafted tokens, and rows of no sequence are NaN.
+ *
+ * Pieces as for fsp_attention_paged, of fsp_attention_tree_piece() tokens, but counted from the first piece
+ * that a window leaves: a sequence may have fewer than its room takes, (longest + window + sinks) /
+ * piece + 2 at least.  workspace: fsp_attention_tree_workspace() bytes unless every sequence has
+ * one piece.
+ */
+struct fsp_attention_tree_args {
+  struct fsp_paged_cache cache;
+  const int32_t* pieces;
+  const int32_t* first_piece;
+  int64_t n_pieces, piece, heads, window;
+  double scale;
+  int64_t sinks, n_tokens, longest;
+  int64_t q_token, q_head, out_token, out_head;
+  const void* q;
+  void* out;
+  float* lse;
+  const int32_t* lengths;
+  const int32_t* token_indptr;
+  const int32_t* parents;
+  void* workspace;
+};
+int64_t fsp_attention_tree_drafts(void);
+int64_t fsp_attention_tree_piece(int64_t tokens, int64_t kv_heads, int64_t group, int64_t longest);
+int64_t fsp_attention_tree_workspace(int64_t n_pieces, int64_t heads, int64_t dim, int64_t longest);
+int fsp_attention_tree(const struct fsp_attention_tree_args* args, void* stream);
+
+/*
  * Attention over packed sequences: sequence b's queries are tokens
  * [q_indptr[b], q_indptr[b + 1]), its keys [k_indptr[b], k_indptr[b + 1]).  With causal != 0 query
  * i of nq sees key j of nk if j <= i + nk - nq; a window > 0 (causal only) hides the keys
