@@ -24,6 +24,8 @@ from .attention import (
     flagsparse_attention_paged,
     flagsparse_attention_paged_tree,
     flagsparse_paged_append,
+    flagsparse_paged_copy,
+    flagsparse_paged_keep,
     prepare_attention_packed,
     prepare_paged_kv,
 )
@@ -83,6 +85,8 @@ ATTENTION_EXPORTS = (
     "flagsparse_attention_paged",
     "flagsparse_attention_paged_tree",
     "flagsparse_paged_append",
+    "flagsparse_paged_copy",
+    "flagsparse_paged_keep",
 )
 
 # Reference exports outside the SpMV / SpMM path (src/flagsparse/__init__.py:5-63).

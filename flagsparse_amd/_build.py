@@ -23,7 +23,7 @@ LIB_PATH = os.path.join(LIB_DIR, LIB_NAME)
 SOURCES = ("abi.cpp", "bound.cpp", "mtx.cpp", "plan.hip", "spmv.hip", "spmv_xcs.hip", "spmm.hip", "sddmm.hip",
            "index_stats.hip", "check.hip", "slices.hip",
            "spmm_slices.hip", "sddmm_slices.hip", "coo_sort.hip", "probe.hip", "paged.hip",
-           "attention.hip", "tree.hip")
+           "attention.hip", "tree.hip", "pages.hip")
 ARCH = "gfx950"
 
 # Packed-FP32 instructions (v_pk_*_f32) are disabled for all device code.

@@ -4,6 +4,8 @@ Sequences of different lengths are rows of a CSR pattern: ``indptr`` over the to
 batch, or over the pages that a cache holds of each sequence (``indices``: the pages).
 
 * ``flagsparse_paged_append``: new keys and values, rotated by their positions, into the cache;
+* ``flagsparse_paged_keep``: some of a sequence's last tokens stay and close up; ``flagsparse_paged_copy``:
+  pages are copied;
 * ``flagsparse_attention_paged``: one new query per sequence over all that the cache holds of it;
 * ``flagsparse_attention_paged_tree``: the queries of a tree of drafted tokens, of which each sees its way;
 * ``flagsparse_attention_packed`` and ``..._backward``: whole sequences, packed one after the other,
@@ -43,6 +45,7 @@ _CACHE = struct.Struct("17q")
 _APPEND, _APPEND_AT = struct.Struct("13q"), struct.Struct("8q")
 _PAGED, _PAGED_AT = struct.Struct("6qd4q"), struct.Struct("6q")
 _PACKED, _PACKED_AT = struct.Struct("10qd24q"), struct.Struct("10q")
+_KEEP, _KEEP_AT = struct.Struct("5q"), struct.Struct("5q")
 _TREE, _TREE_AT = struct.Struct("6qd7q"), struct.Struct("7q")
 
 # A prepared object keeps the first part for each layout of arrays that it has checked, so that the
@@ -410,7 +413,7 @@ def _paged_of(prepared, k_pages, v_pages, indptr, indices, lengths):
 
 def flagsparse_paged_append(k, v, lengths, token_indptr=None, *, prepared=None, k_pages=None,
                             v_pages=None, indptr=None, indices=None, q=None, cos=None, sin=None,
-                            interleaved=False, out=None):
+                            interleaved=False, parents=None, out=None):
     """Write new keys and values into a paged cache, rotated by their positions on the way.
 
     ``k``, ``v``: [tokens, kv_heads, dim], the new tokens of each sequence one after the other:
@@ -419,22 +422,26 @@ def flagsparse_paged_append(k, v, lengths, token_indptr=None, *, prepared=None, 
     ``lengths[b] - 1``.  ``cos``, ``sin``: float32 [positions, half]; the first 2 * half elements of
     every head of ``k`` and ``q`` are rotated by pairs, (a, b) -> (a cos - b sin, a sin + b cos):
     elements half apart, or neighbours with ``interleaved``.  Without them nothing is rotated.
+    ``parents``: the new tokens are drafted ones, at most 256 a sequence, that form trees
+    (flagsparse_attention_paged_tree): each is stored in its turn, but rotated by the position of its sequence's
+    first new token plus the tokens before it on its way up the tree.
 
     Returns the rotated ``q`` [tokens, heads, dim] (written to ``out`` where given, which may be ``q``),
     or None without ``q``.  The pages that new tokens go to belong to one sequence each, and ``k``,
     ``v`` and ``q`` lie outside the cache.  With
     ``prepared`` nothing is waited for, so lengths are not checked: a token whose position is
-    negative or past its sequence's pages is not stored and its row of ``q`` comes back as NaN."""
+    negative or past its sequence's pages, or whose parents do not come earlier, is not stored and its row of
+    ``q`` comes back as NaN."""
     key = None
     if out is None and type(prepared) is PreparedPagedKV:
-        key = _layouts(k, v, q, cos, sin, lengths, token_indptr) + (
+        key = _layouts(k, v, q, cos, sin, lengths, token_indptr, parents) + (
             bool(interleaved), prepared.k_pages.data_ptr(), prepared.v_pages.data_ptr())
         kept = prepared._calls.get(key)
         if kept is not None and not (k.data_ptr() | v.data_ptr()) % 16 and (
                 q is None or q.data_ptr() % 16 == 0):
             head, like = kept
             res = None if q is None else torch.empty_like(like, memory_format=_CONTIGUOUS)
-            _append(prepared, head, k, v, q, res, cos, sin, token_indptr, lengths)
+            _append(prepared, head, k, v, q, res, cos, sin, token_indptr, lengths, parents)
             return res
     kv, n = _paged_of(prepared, k_pages, v_pages, indptr, indices, lengths)
     dev, dt = kv.device, kv.dtype
@@ -443,13 +450,18 @@ def flagsparse_paged_append(k, v, lengths, token_indptr=None, *, prepared=None, 
     tokens = k.shape[0]
     if v.shape[0] != tokens:
         raise ValueError(f"v must have {tokens} tokens, got {v.shape[0]}")
-    given = (k, v, q, cos, sin, lengths, token_indptr)
+    given = (k, v, q, cos, sin, lengths, token_indptr, parents)
     if token_indptr is None:
         if tokens != kv.batch:
             raise ValueError(f"k must have one token for each of {kv.batch} sequences, got "
                              f"{tokens}; other numbers need token_indptr")
     else:
         token_indptr = _int32(token_indptr, "token_indptr", kv.batch + 1, dev)
+    if parents is not None:
+        parents = _int32(parents, "parents", tokens, dev, -2)
+        if prepared is None:
+            _check_drafts(kv, n, token_indptr, parents, tokens, 1 if token_indptr is None else
+                          int(_abi.lib().fsp_attention_tree_drafts()))
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin come together")
     half = rows = 0
@@ -482,9 +494,9 @@ def flagsparse_paged_append(k, v, lengths, token_indptr=None, *, prepared=None, 
         steps = (*_steps(q), *_steps(res)) if heads else (0, 0, 0, 0)
         head = kv._packed() + _APPEND.pack(tokens, heads, half, rows, bool(interleaved),
                                            *_steps(k), *_steps(v), *steps)
-        _append(kv, head, k, v, q, res, cos, sin, token_indptr, n)
+        _append(kv, head, k, v, q, res, cos, sin, token_indptr, n, parents)
         if key is not None and all(x is y for x, y in zip(
-                (k, v, q, cos, sin, n, token_indptr), given)):
+                (k, v, q, cos, sin, n, token_indptr, parents), given)):
             _keep(kv._calls, key, (head, None if q is None else _like(q.shape, dt, dev)))
     elif res is not None:  # tokens of no sequence
         res.fill_(float("nan"))
@@ -498,12 +510,128 @@ def _at(t):
     return 0 if t is None else t.data_ptr()
 
 
-def _append(kv, head, k, v, q, res, cos, sin, token_indptr, lengths):
+def _append(kv, head, k, v, q, res, cos, sin, token_indptr, lengths, parents):
     args = head + _APPEND_AT.pack(k.data_ptr(), v.data_ptr(), _at(q), _at(res), _at(cos), _at(sin),
                                   _at(token_indptr), lengths.data_ptr())
-    status = _abi.lib().fsp_paged_append(args, kv._on())
+    if parents is None:
+        status = _abi.lib().fsp_paged_append(args, kv._on())
+    else:
+        status = _abi.lib().fsp_paged_append_drafts(args, parents.data_ptr(), kv._on())
     if status:
         _abi.check(status, "fsp_paged_append")
+
+
+def flagsparse_paged_keep(keep, lengths, token_indptr=None, *, prepared=None, k_pages=None, v_pages=None,
+                          indptr=None, indices=None, into=None):
+    """Keep some of the last tokens of each sequence of a paged cache: drafted tokens that were accepted,
+    or what is left of a text.
+
+    ``keep``: [tokens], bool, the marks of the last tokens of each sequence one after the other: sequence
+    b's are ``token_indptr[b]`` to ``token_indptr[b + 1]`` (None: as many for each), as many as it may have;
+    ``lengths[b]`` is what sequence b holds.  The marked ones stay, in their order, and close up behind the
+    tokens before them: in place, where the pages they move in belong to one sequence each, or in the pages of
+    ``into``, another PreparedPagedKV with as many sequences, heads and dims, to which the tokens before them are
+    copied too (pages that the call does not read; several may lie in the same arrays).
+
+    Returns the new lengths, int32.  With ``prepared`` nothing is waited for, so lengths are not checked: where
+    one is more than its pages hold or less than its marked tokens, or ``into`` has no room for
+    what stays, nothing is moved and the new length is -1."""
+    key = None
+    if into is not None and not isinstance(into, PreparedPagedKV):
+        raise TypeError("into must be a PreparedPagedKV instance")
+    if type(prepared) is PreparedPagedKV:
+        key = _layouts(keep, lengths, token_indptr) + (
+            "keep", prepared.k_pages.data_ptr(), prepared.v_pages.data_ptr())
+        kept = prepared._calls.get(key)
+        if kept is not None:
+            return _keep_tokens(prepared, into, kept, keep, token_indptr, lengths)
+    kv, n = _paged_of(prepared, k_pages, v_pages, indptr, indices, lengths)
+    dev = kv.device
+    if not torch.is_tensor(keep) or keep.ndim != 1:
+        raise ValueError("keep must be a 1D tensor [tokens]")
+    if not keep.is_cuda or keep.device != dev:
+        raise ValueError(f"keep must be a CUDA tensor on {dev}")
+    if keep.dtype != torch.bool:
+        raise TypeError("keep dtype must be torch.bool")
+    tokens = keep.numel()
+    if tokens > _TOKENS_CAP:
+        raise ValueError("keep must have at most 2^31 - 1024 tokens")
+    given = (keep, n, token_indptr)
+    each = 0
+    if token_indptr is None:
+        each = tokens // max(kv.batch, 1)
+        if each * kv.batch != tokens:
+            raise ValueError(f"keep must have as many tokens for each of {kv.batch} sequences, got "
+                             f"{tokens}; other numbers need token_indptr")
+    else:
+        token_indptr = _int32(token_indptr, "token_indptr", kv.batch + 1, dev)
+    if prepared is None:
+        _check_drafts(kv, n, token_indptr, None, tokens, each if token_indptr is None else tokens)
+    keep = keep.contiguous()
+    kept = (kv._packed(), (tokens, each, kv._pieces.shape[0], kv._piece),
+            _like((kv.batch,), torch.int32, dev))
+    res = _keep_tokens(kv, into, kept, keep, token_indptr, n)
+    if key is not None and all(x is y for x, y in zip((keep, lengths, token_indptr), given)):
+        _keep(kv._calls, key, kept)
+    return res
+
+
+def _keep_tokens(kv, into, kept, keep, token_indptr, lengths):
+    """The launch; returns the new lengths.  What ``into`` holds is looked up by every call: it is an
+    argument, not a part of the prepared cache."""
+    head, sizes, like = kept
+    stream, other = kv._on(), head
+    if into is not None:
+        if into.device != kv.device or into.dtype != kv.dtype:
+            raise ValueError("into must be of the cache's type and on its device")
+        if (into.batch, into.kv_heads, into.dim) != (kv.batch, kv.kv_heads, kv.dim):
+            raise ValueError("into must have the cache's number of sequences, heads and dim")
+        other = into._packed()
+        into._on()
+    res = torch.empty_like(like, memory_format=_CONTIGUOUS)
+    status = _abi.lib().fsp_paged_keep(head + other + _KEEP.pack(into is not None, *sizes) + _KEEP_AT.pack(
+        kv._pieces.data_ptr(), keep.data_ptr(), _at(token_indptr), lengths.data_ptr(), res.data_ptr()), stream)
+    if status:
+        _abi.check(status, "fsp_paged_keep")
+    return res
+
+
+def flagsparse_paged_copy(sources, targets, *, prepared=None, k_pages=None, v_pages=None):
+    """Copy pages of a paged cache, keys and values: page ``sources[i]`` to page ``targets[i]``.
+
+    A sequence that branches shares the pages that both only read by its page table, and has its last one
+    copied.  ``sources``, ``targets``: [n], int32 or int64, numbers of the cache's pages; no page is the target
+    of two, and none that is a target is another's source.  The cache is given by ``prepared`` or by its
+    pages; with ``prepared`` nothing is waited for, so numbers are not checked: a pair with one outside the
+    cache copies nothing."""
+    if prepared is not None:
+        if not isinstance(prepared, PreparedPagedKV):
+            raise TypeError("prepared must be a PreparedPagedKV instance")
+        kv = prepared
+    else:
+        if k_pages is None or v_pages is None:
+            raise ValueError("k_pages and v_pages are required when prepared is not provided")
+        none = torch.zeros(1, dtype=torch.int32, device=k_pages.device if torch.is_tensor(k_pages) else None)
+        kv = prepare_paged_kv(k_pages, v_pages, none, none[:0])
+    for t, name in ((sources, "sources"), (targets, "targets")):
+        if not torch.is_tensor(t) or t.ndim != 1:
+            raise ValueError(f"{name} must be a 1D tensor")
+    n = sources.numel()
+    sources = _int32(sources, "sources", n, kv.device)
+    targets = _int32(targets, "targets", n, kv.device)
+    if prepared is None and n:
+        for t, name in ((sources, "sources"), (targets, "targets")):
+            if int(t.min()) < 0 or int(t.max()) >= kv.n_pages:
+                raise IndexError(f"{name} out of range for the cache's pages")
+        if torch.unique(targets).numel() != n:
+            raise ValueError("targets must be different pages")
+        if bool((torch.isin(sources, targets) & (sources != targets)).any()):
+            raise ValueError("a page cannot be a target and another one's source")
+    if n:
+        status = _abi.lib().fsp_paged_copy(kv._packed(), sources.data_ptr(), targets.data_ptr(), n,
+                                           _abi.raw_stream(kv.device))
+        if status:
+            _abi.check(status, "fsp_paged_copy")
 
 
 def flagsparse_attention_paged(q, lengths, *, prepared=None, k_pages=None, v_pages=None,

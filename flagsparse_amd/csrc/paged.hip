@@ -56,6 +56,29 @@ __device__ __forceinline__ V8<T> turned(const T* row, int d, const float* cos, c
   return __builtin_convertvector(y, V8<T>);
 }
 
+constexpr int kDrafts = 256;  // drafted tokens of one sequence, at most
+
+// The depth of token i of a sequence's ``count`` drafted ones, whose parents start at ``up``: the steps up to
+// one without; -1 where they do not lead up.  A wave holds all parents, and walks by the lanes that they
+// lie in.
+__device__ __forceinline__ int depth_of(const int32_t* up, int i, int count) {
+  const int lane = threadIdx.x & 63;
+  if (count > kDrafts) return -1;
+  int held[kDrafts / kWave];
+#pragma unroll
+  for (int k = 0; k < kDrafts / kWave; ++k) held[k] = up[min(k * kWave + lane, count - 1)];
+  int depth = 0;
+  for (int at = i;;) {
+    const int k = at / kWave;
+    const int from = k == 0 ? held[0] : k == 1 ? held[1] : k == 2 ? held[2] : held[3];
+    const int p = __builtin_amdgcn_readlane(from, at % kWave);
+    if (p < -1 || p >= at) return -1;
+    if (p < 0) return depth;
+    at = p;
+    ++depth;
+  }
+}
+
 struct AppendShape {
   int64_t n_tokens, k_token, k_head, v_token, v_head, q_token, q_head, qo_token, qo_head;
   int heads, half, table_rows, interleaved, parts;
@@ -71,14 +94,15 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(
     Cache c, AppendShape s, T* __restrict__ k_pages, T* __restrict__ v_pages,
     const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ q,
     T* __restrict__ q_out, const float* __restrict__ cos, const float* __restrict__ sin,
-    const int32_t* __restrict__ tokens, const int32_t* __restrict__ lengths) {
+    const int32_t* __restrict__ tokens, const int32_t* __restrict__ lengths,
+    const int32_t* __restrict__ parents) {
   const int lane = threadIdx.x & 63;
   const int64_t unit = (int64_t)blockIdx.x * (kAppendThreads / kWave) +
                        __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t t = unit / s.parts;
   if (t >= s.n_tokens) return;
-  int b = (int)t;
-  int64_t pos;
+  int b = (int)t, depth = 0;
+  int64_t pos, turn;  // its place, and its position for the rotation
   bool mine = true;
   if (tokens) {  // the last sequence that starts at or before t, 64 at a look
     b = -1;
@@ -90,20 +114,25 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(
     b = __builtin_amdgcn_readfirstlane(max(b, 0));
     const int begin = tokens[b], end = tokens[b + 1];
     mine = begin <= t && t < end;
-    pos = (int64_t)lengths[b] - end + t;
+    pos = turn = (int64_t)lengths[b] - end + t;
+    if (parents && mine) {
+      depth = __builtin_amdgcn_readfirstlane(depth_of(parents + begin, (int)(t - begin), end - begin));
+      turn = (int64_t)lengths[b] - (end - begin) + depth;
+    }
   } else {
-    pos = (int64_t)lengths[b] - 1;
+    pos = turn = (int64_t)lengths[b] - 1;
+    if (parents) depth = parents[t] == -1 ? 0 : -1;
   }
   const int first = c.indptr[b], last = c.indptr[b + 1];
-  const bool ok = mine && pos >= 0 && pos < (int64_t)(last - first) * c.page_size &&
-                  (MODE == kStill || pos < s.table_rows);
+  const bool ok = mine && depth >= 0 && pos >= 0 && turn >= 0 &&
+                  pos < (int64_t)(last - first) * c.page_size && (MODE == kStill || turn < s.table_rows);
   int64_t page = 0, slot = 0;
   if (ok) {
     const uint32_t at = (uint32_t)pos / (uint32_t)c.page_size;
     page = c.indices[first + at];
     slot = (uint32_t)pos - at * c.page_size;
-    cos += pos * s.half;
-    sin += pos * s.half;
+    cos += turn * s.half;
+    sin += turn * s.half;
   }
   const T nan = (T)__builtin_nanf("");
   const uint32_t per = c.dim / 8, rows = s.heads + 2 * c.kv_heads;
@@ -520,8 +549,12 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(
         total == 0 ? -INFINITY : (most + log2f(total * Weights<T>::down)) * kLn2;
 }
 
+struct AppendCall : fsp_paged_append_args {
+  const int32_t* parents;
+};
+
 template <typename T, int MODE>
-int launch_append(const fsp_paged_append_args& a, hipStream_t st) {
+int launch_append(const AppendCall& a, hipStream_t st) {
   const int64_t steps = ((a.heads + 2 * a.cache.kv_heads) * (a.cache.dim / 8) + kWave - 1) / kWave;
   int64_t parts = (4096 + a.n_tokens - 1) / a.n_tokens;  // waves enough for every SIMD
   if (parts > steps) parts = steps;
@@ -535,12 +568,12 @@ int launch_append(const fsp_paged_append_args& a, hipStream_t st) {
                      static_cast<T*>(a.cache.k_pages), static_cast<T*>(a.cache.v_pages),
                      static_cast<const T*>(a.k), static_cast<const T*>(a.v),
                      static_cast<const T*>(a.q), static_cast<T*>(a.q_out), a.cos, a.sin,
-                     a.token_indptr, a.lengths);
+                     a.token_indptr, a.lengths, a.parents);
   return check_hip(hipGetLastError(), "paged_append_kernel launch");
 }
 
 template <typename T>
-int launch_append_mode(const fsp_paged_append_args& a, hipStream_t st) {
+int launch_append_mode(const AppendCall& a, hipStream_t st) {
   const bool aligned = (reinterpret_cast<uintptr_t>(a.cos) | reinterpret_cast<uintptr_t>(a.sin)) % 16 == 0;
   if (a.half == 0) return launch_append<T, kStill>(a, st);
   if (aligned && !a.interleaved && a.half % 8 == 0) return launch_append<T, kHalves>(a, st);
@@ -605,26 +638,40 @@ using namespace fsp;
 
 extern "C" int64_t fsp_attention_dim_cap(void) { return kAttnDimCap; }
 
-extern "C" int fsp_paged_append(const fsp_paged_append_args* args, void* stream) {
-  if (!args) return set_error(FSP_EINVAL, "fsp_paged_append: null arguments");
-  const fsp_paged_append_args& a = *args;
-  if (int rc = check_cache(a.cache, "fsp_paged_append")) return rc;
+namespace {
+
+int run_append(const AppendCall& a, const std::string& who, void* stream) {
+  if (int rc = check_cache(a.cache, who)) return rc;
   if (a.n_tokens < 0 || a.heads < 0 || a.heads > 0xffff || a.half < 0 || a.table_rows < 0 ||
       2 * a.half > a.cache.dim || a.table_rows > 0x7fffffffLL || a.n_tokens > kMaxBlocks)
-    return set_error(FSP_EINVAL, "fsp_paged_append: size out of range");
+    return set_error(FSP_EINVAL, who + ": size out of range");
   if (a.n_tokens == 0) return FSP_OK;
   if (!a.token_indptr && a.n_tokens != a.cache.batch)
-    return set_error(FSP_EINVAL, "fsp_paged_append: one token per sequence without token_indptr");
+    return set_error(FSP_EINVAL, who + ": one token per sequence without token_indptr");
   if (a.cache.batch < 1)
-    return set_error(FSP_EINVAL, "fsp_paged_append: tokens of no sequence");
+    return set_error(FSP_EINVAL, who + ": tokens of no sequence");
   if (!a.k || !a.v || !a.lengths || (a.heads && (!a.q || !a.q_out)) ||
       (a.half && (!a.cos || !a.sin)))
-    return set_error(FSP_EINVAL, "fsp_paged_append: null pointer");
+    return set_error(FSP_EINVAL, who + ": null pointer");
   if (!aligned16(a.k, a.k_token, a.k_head) || !aligned16(a.v, a.v_token, a.v_head) ||
       !aligned16(a.q, a.q_token, a.q_head) || !aligned16(a.q_out, a.q_out_token, a.q_out_head))
-    return set_error(FSP_EINVAL, "fsp_paged_append: rows must be 16-byte aligned");
+    return set_error(FSP_EINVAL, who + ": rows must be 16-byte aligned");
   hipStream_t st = static_cast<hipStream_t>(stream);
   return a.cache.dtype == FSP_BF16 ? launch_append_mode<bf16>(a, st) : launch_append_mode<f16>(a, st);
+}
+
+}  // namespace
+
+extern "C" int fsp_paged_append(const fsp_paged_append_args* args, void* stream) {
+  if (!args) return set_error(FSP_EINVAL, "fsp_paged_append: null arguments");
+  return run_append({*args, nullptr}, "fsp_paged_append", stream);
+}
+
+extern "C" int fsp_paged_append_drafts(const fsp_paged_append_args* args, const int32_t* parents,
+                                       void* stream) {
+  if (!args) return set_error(FSP_EINVAL, "fsp_paged_append_drafts: null arguments");
+  if (!parents && args->n_tokens > 0) return set_error(FSP_EINVAL, "fsp_paged_append_drafts: null pointer");
+  return run_append({*args, parents}, "fsp_paged_append_drafts", stream);
 }
 
 extern "C" int64_t fsp_attention_paged_piece(int64_t tokens, int64_t kv_heads) {

@@ -1,0 +1,320 @@
+// Moving what a paged cache holds: tokens that stay close up, pages are copied.
+#include "paged.hpp"
+
+namespace fsp {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kList = 1024;  // tokens whose places LDS holds at a time
+
+// A sequence's marked tokens, its last ones: rows [begin, begin + count) of the marks, after ``past``
+// others.
+struct Marked {
+  int begin, count, past;
+  bool ok;
+  __device__ Marked(const int32_t* tokens, int each, int n_tokens, int b, int length, int room) {
+    begin = tokens ? tokens[b] : b * each;
+    const int end = tokens ? tokens[b + 1] : begin + each;
+    ok = begin >= 0 && begin <= end && end <= n_tokens && length >= end - begin && length <= room;
+    count = ok ? end - begin : 0;
+    past = ok ? length - count : 0;
+  }
+};
+
+struct KeepShape {
+  int n_tokens, each;
+  int64_t k_page, k_slot, k_head, v_page, v_slot, v_head;  // of the cache that is written
+  const int32_t *indptr, *indices;
+  int page_size;
+};
+
+// The tokens that stay of [at, at + kList) marks, their places in turn, to LDS; how many.
+__device__ __forceinline__ int list_kept(const uint8_t* keep, int at, int count, int* list) {
+  __shared__ int s_count[kList / kWave];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint64_t votes[kList / kThreads];
+#pragma unroll
+  for (int i = 0; i < kList / kThreads; ++i) {
+    const int t = at + i * kThreads + (int)threadIdx.x;
+    votes[i] = __ballot(t < count && keep[t]);
+    if (lane == 0) s_count[i * 4 + wave] = __popcll(votes[i]);
+  }
+  __syncthreads();
+  int total = 0, before[kList / kThreads];
+#pragma unroll
+  for (int i = 0; i < kList / kWave; ++i) {
+    if (i % 4 == wave) before[i / 4] = total;
+    total += s_count[i];
+  }
+#pragma unroll
+  for (int i = 0; i < kList / kThreads; ++i)
+    if (votes[i] >> lane & 1)
+      list[before[i] + __popcll(votes[i] & ((1ull << lane) - 1))] = at + i * kThreads + threadIdx.x;
+  __syncthreads();
+  return total;
+}
+
+// In place.  A workgroup takes one sequence, one key head and its keys or values, so that nobody else
+// writes what it reads.  The n-th token that stays comes from a place n or later, each from a later one than the one
+// before it: rows that are read after others were written are theirs still.  Of the rows of one step
+// all are read before any is written.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void paged_keep_kernel(
+    Cache c, KeepShape s, T* __restrict__ k_pages, T* __restrict__ v_pages,
+    const uint8_t* __restrict__ keep, const int32_t* __restrict__ tokens,
+    const int32_t* __restrict__ lengths, int32_t* __restrict__ kept) {
+  constexpr int U = 4;
+  __shared__ int s_list[kList];
+  const int per = 2 * c.kv_heads, b = blockIdx.x / per, which = blockIdx.x % per;
+  const bool values = which >= c.kv_heads;
+  const int g = values ? which - c.kv_heads : which;
+  const int first = c.indptr[b];
+  const Marked m(tokens, s.each, s.n_tokens, b, lengths[b], (c.indptr[b + 1] - first) * c.page_size);
+  T* pages = values ? v_pages + g * c.v_head : k_pages + g * c.k_head;
+  const int64_t page_step = values ? c.v_page : c.k_page, slot_step = values ? c.v_slot : c.k_slot;
+  const int chunks = c.dim / 8, rows = kThreads / chunks;  // rows side by side
+  const int row = threadIdx.x / chunks, d = threadIdx.x % chunks * 8;
+  auto place = [&](int pos) {
+    const uint32_t at = (uint32_t)pos / (uint32_t)c.page_size;
+    return pages + c.indices[first + at] * page_step + ((uint32_t)pos - at * c.page_size) * slot_step + d;
+  };
+  int stay = 0;
+  for (int at = 0; at < m.count; at += kList) {
+    const int n = list_kept(keep + m.begin, at, m.count, s_list);
+    for (int i = 0; i < n; i += rows * U) {
+      i32x4 x[U];
+      int from[U], to[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int r = min(i + u * rows + row, n - 1);  // one that is another's too is not written twice
+        to[u] = m.past + stay + r;
+        from[u] = m.past + s_list[r];
+        x[u] = *reinterpret_cast<const i32x4*>(place(from[u]));
+      }
+      all_stored();  // and read
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (row < rows && i + u * rows + row < n && from[u] != to[u])
+          *reinterpret_cast<i32x4*>(place(to[u])) = x[u];
+    }
+    stay += n;
+    __syncthreads();
+  }
+  if (which == 0 && threadIdx.x == 0) kept[b] = m.ok ? m.past + stay : -1;
+}
+
+// Into other pages: a workgroup takes a piece of a sequence's tokens, one key head and its keys or values.
+// How many tokens stay before the piece, and of all, it counts itself, four marks to a word.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void paged_keep_into_kernel(
+    Cache c, KeepShape s, const Piece* __restrict__ pieces, int piece_size, int n_pieces,
+    const T* __restrict__ k_pages, const T* __restrict__ v_pages, T* __restrict__ to_k,
+    T* __restrict__ to_v, const uint8_t* __restrict__ keep, const int32_t* __restrict__ tokens,
+    const int32_t* __restrict__ lengths, int32_t* __restrict__ kept) {
+  constexpr int U = 8;
+  __shared__ int s_list[kList];
+  __shared__ int s_before[4], s_all[4];
+  int piece, which;
+  piece_and_head(blockIdx.x, n_pieces, 2 * c.kv_heads, piece, which);
+  const Piece pc = pieces[piece];
+  const int b = pc.seq;
+  const bool values = which >= c.kv_heads;
+  const int g = values ? which - c.kv_heads : which;
+  const Marked m(tokens, s.each, s.n_tokens, b, lengths[b], pc.room);
+  const int length = m.past + m.count, end = min(length, pc.begin + piece_size);
+  if (pc.begin >= length && pc.begin > 0) return;
+
+  const uint8_t* marks = keep + m.begin;
+  int before = 0, all = 0;
+  {
+    // whole words of the array that the marks lie in, those of others masked
+    const uintptr_t at = reinterpret_cast<uintptr_t>(marks);
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(at & ~uintptr_t(3));
+    const int skip = (int)(at & 3), stop = pc.begin - m.past;
+    for (int64_t i = threadIdx.x; 4 * i < (int64_t)m.count + skip; i += kThreads) {
+      const int t = (int)(4 * i) - skip;
+      uint32_t w;
+      if (t >= 0 && t + 4 <= m.count) {
+        w = words[i];
+      } else {
+        w = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (t + e >= 0 && t + e < m.count) w |= (uint32_t)marks[t + e] << (8 * e);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int one = (w >> (8 * e) & 255) != 0;
+        all += one;
+        before += t + e < stop ? one : 0;
+      }
+    }
+#pragma unroll
+    for (int x = 1; x < kWave; x *= 2) {
+      before += __shfl_xor(before, x);
+      all += __shfl_xor(all, x);
+    }
+    if ((threadIdx.x & 63) == 0) {
+      s_before[threadIdx.x >> 6] = before;
+      s_all[threadIdx.x >> 6] = all;
+    }
+    __syncthreads();
+    before = s_before[0] + s_before[1] + s_before[2] + s_before[3];
+    all = s_all[0] + s_all[1] + s_all[2] + s_all[3];
+  }
+  const int first = s.indptr[b];
+  const bool ok = m.ok && m.past + all <= (int64_t)(s.indptr[b + 1] - first) * s.page_size;
+  if (pc.begin == 0 && which == 0 && threadIdx.x == 0) kept[b] = ok ? m.past + all : -1;
+  if (!ok) return;
+
+  const T* from = values ? v_pages + g * c.v_head : k_pages + g * c.k_head;
+  T* to = values ? to_v + g * s.v_head : to_k + g * s.k_head;
+  const int64_t from_page = values ? c.v_page : c.k_page, from_slot = values ? c.v_slot : c.k_slot;
+  const int64_t to_page = values ? s.v_page : s.k_page, to_slot = values ? s.v_slot : s.k_slot;
+  const int chunks = c.dim / 8, rows = kThreads / chunks;
+  const int row = threadIdx.x / chunks, d = threadIdx.x % chunks * 8;
+  if (pc.begin < m.past) {  // tokens before the marked ones stay where they are in the text
+    before = pc.begin;
+  } else {
+    before += m.past;
+  }
+  for (int at = pc.begin; at < end; at += kList) {
+    // the piece's tokens that stay, by their distance from at
+    const int whole = max(0, min(m.past, end) - at), upto = min(end, at + kList);
+    int n = min(whole, kList);
+    if (at + kList > m.past && upto > m.past) {
+      const int from_mark = max(at, m.past) - m.past;
+      n += list_kept(marks, from_mark, upto - m.past, s_list + n);
+    } else {
+      __syncthreads();
+    }
+    for (int i = 0; i < n; i += rows * U) {
+      i32x4 x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int r = min(i + u * rows + row, n - 1);
+        const uint32_t pos = r < whole ? at + r : m.past + s_list[r], p = pos / (uint32_t)c.page_size;
+        x[u] = *reinterpret_cast<const i32x4*>(from + c.indices[pc.page + p] * from_page +
+                                               (pos - p * c.page_size) * from_slot + d);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int r = i + u * rows + row;
+        if (row < rows && r < n) {
+          const uint32_t pos = before + r, p = pos / (uint32_t)s.page_size;
+          *reinterpret_cast<i32x4*>(to + s.indices[first + p] * to_page +
+                                    (pos - p * s.page_size) * to_slot + d) = x[u];
+        }
+      }
+    }
+    before += n;
+    __syncthreads();
+  }
+}
+
+// Page sources[i] to targets[i], ``parts`` workgroups to the keys or values of one, a vector of eight elements
+// a thread and step.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void paged_copy_kernel(
+    Cache c, int n_pages, T* __restrict__ k_pages, T* __restrict__ v_pages,
+    const int32_t* __restrict__ sources, const int32_t* __restrict__ targets, int parts) {
+  constexpr int U = 4;
+  const int part = blockIdx.x % parts, which = blockIdx.x / parts & 1;
+  const int64_t i = blockIdx.x / parts / 2;
+  const int source = sources[i], target = targets[i];
+  if (source < 0 || target < 0 || source >= n_pages || target >= n_pages || source == target) return;
+  const int64_t page = which ? c.v_page : c.k_page, slot = which ? c.v_slot : c.k_slot,
+                head = which ? c.v_head : c.k_head;
+  const T* from = (which ? v_pages : k_pages) + source * page;
+  T* to = (which ? v_pages : k_pages) + target * page;
+  const uint32_t chunks = c.dim / 8, line = chunks * c.kv_heads, all = line * c.page_size;
+  for (uint32_t at = part * kThreads + threadIdx.x; at < all; at += U * parts * kThreads) {
+    i32x4 x[U];
+    int64_t off[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t j = min(at + u * parts * kThreads, all - 1);
+      const uint32_t s = j / line, r = j - s * line, h = r / chunks;
+      off[u] = s * slot + h * head + (r - h * chunks) * 8;
+      x[u] = *reinterpret_cast<const i32x4*>(from + off[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (at + u * parts * kThreads < all) *reinterpret_cast<i32x4*>(to + off[u]) = x[u];
+  }
+}
+
+template <typename T>
+int launch_keep(const fsp_paged_keep_args& a, hipStream_t st) {
+  const fsp_paged_cache& to = a.into;
+  const KeepShape s{(int)a.n_tokens, (int)a.each, to.k_page, to.k_slot,       to.k_head,       to.v_page,
+                    to.v_slot,       to.v_head,   to.page_indptr, to.page_indices, (int)to.page_size};
+  if (!a.other) {
+    hipLaunchKernelGGL((paged_keep_kernel<T>), dim3((unsigned)(a.cache.batch * 2 * a.cache.kv_heads)),
+                       dim3(kThreads), 0, st, cache_of(a.cache), s, static_cast<T*>(a.cache.k_pages),
+                       static_cast<T*>(a.cache.v_pages), a.keep, a.token_indptr, a.lengths, a.kept);
+    return check_hip(hipGetLastError(), "paged_keep_kernel launch");
+  }
+  hipLaunchKernelGGL((paged_keep_into_kernel<T>), dim3((unsigned)(a.n_pieces * 2 * a.cache.kv_heads)),
+                     dim3(kThreads), 0, st, cache_of(a.cache), s, reinterpret_cast<const Piece*>(a.pieces),
+                     (int)a.piece, (int)a.n_pieces, static_cast<const T*>(a.cache.k_pages),
+                     static_cast<const T*>(a.cache.v_pages), static_cast<T*>(to.k_pages),
+                     static_cast<T*>(to.v_pages), a.keep, a.token_indptr, a.lengths, a.kept);
+  return check_hip(hipGetLastError(), "paged_keep_into_kernel launch");
+}
+
+template <typename T>
+int launch_copy(const fsp_paged_cache& c, const int32_t* sources, const int32_t* targets, int64_t n,
+                hipStream_t st) {
+  const int64_t steps = (c.page_size * c.kv_heads * (c.dim / 8) + kThreads - 1) / kThreads;
+  int64_t parts = (4096 + 2 * n - 1) / (2 * n);
+  if (parts > steps) parts = steps;
+  hipLaunchKernelGGL((paged_copy_kernel<T>), dim3((unsigned)(2 * n * parts)), dim3(kThreads), 0, st,
+                     cache_of(c), (int)c.n_pages, static_cast<T*>(c.k_pages), static_cast<T*>(c.v_pages),
+                     sources, targets, (int)parts);
+  return check_hip(hipGetLastError(), "paged_copy_kernel launch");
+}
+
+}  // namespace
+}  // namespace fsp
+
+using namespace fsp;
+
+extern "C" int fsp_paged_keep(const fsp_paged_keep_args* args, void* stream) {
+  if (!args) return set_error(FSP_EINVAL, "fsp_paged_keep: null arguments");
+  const fsp_paged_keep_args& a = *args;
+  if (int rc = check_cache(a.cache, "fsp_paged_keep")) return rc;
+  if (a.n_tokens < 0 || a.n_tokens > kAttnTokensCap || a.each < 0 ||
+      a.cache.batch > kMaxBlocks / (2 * a.cache.kv_heads))
+    return set_error(FSP_EINVAL, "fsp_paged_keep: size out of range");
+  if (a.cache.batch == 0) return FSP_OK;
+  if (!a.token_indptr && (a.each > a.n_tokens / a.cache.batch || a.each * a.cache.batch != a.n_tokens))
+    return set_error(FSP_EINVAL, "fsp_paged_keep: each tokens per sequence without token_indptr");
+  if ((a.n_tokens > 0 && !a.keep) || !a.lengths || !a.kept)
+    return set_error(FSP_EINVAL, "fsp_paged_keep: null pointer");
+  if (a.other) {
+    if (int rc = check_cache(a.into, "fsp_paged_keep")) return rc;
+    if (a.into.dtype != a.cache.dtype || a.into.kv_heads != a.cache.kv_heads || a.into.dim != a.cache.dim ||
+        a.into.batch != a.cache.batch)
+      return set_error(FSP_EINVAL, "fsp_paged_keep: the caches differ in type, heads, dim or sequences");
+    if (a.piece < 128 || a.piece > kList || a.piece % 128 || a.n_pieces < a.cache.batch || !a.pieces ||
+        a.n_pieces > kMaxBlocks / (2 * a.cache.kv_heads))
+      return set_error(FSP_EINVAL, "fsp_paged_keep: pieces");
+  }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  // rows are moved as they are: one kernel for both types of 16 bits
+  return launch_keep<f16>(a, st);
+}
+
+extern "C" int fsp_paged_copy(const fsp_paged_cache* cache, const int32_t* sources, const int32_t* targets,
+                              int64_t n, void* stream) {
+  if (!cache) return set_error(FSP_EINVAL, "fsp_paged_copy: null arguments");
+  if (int rc = check_cache(*cache, "fsp_paged_copy")) return rc;
+  if (n < 0 || n > kMaxBlocks / 4 || cache->page_size * cache->kv_heads > (1 << 30) / (cache->dim / 8))
+    return set_error(FSP_EINVAL, "fsp_paged_copy: size out of range");
+  if (n == 0) return FSP_OK;
+  if (!sources || !targets || (cache->n_pages > 0 && (!cache->k_pages || !cache->v_pages)))
+    return set_error(FSP_EINVAL, "fsp_paged_copy: null pointer");
+  return launch_copy<f16>(*cache, sources, targets, n, static_cast<hipStream_t>(stream));
+}

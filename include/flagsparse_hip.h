@@ -725,6 +725,43 @@ struct fsp_paged_append_args {
   const int32_t* lengths;
 };
 int fsp_paged_append(const struct fsp_paged_append_args* args, void* stream);
+/*
+ * The same for trees of drafted tokens, at most fsp_attention_tree_drafts() a sequence: parents[t] is the place,
+ * among its sequence's new tokens, of the one before token t, a smaller place than its own, or -1.  Token t is
+ * stored where it is without, but rotated by the position of its sequence's first new token plus the length
+ * of its way up.  A token whose way does not lead up, or of a sequence with more, is not stored, and its row
+ * of q_out is NaN.
+ */
+int fsp_paged_append_drafts(const struct fsp_paged_append_args* args, const int32_t* parents,
+                            void* stream);
+
+/*
+ * Of the last tokens of each sequence (token_indptr[b + 1] - token_indptr[b]; NULL: `each`, n_tokens / batch)
+ * those with a mark keep[token] other than 0 stay and close up behind the tokens before them: in
+ * their own pages, or with other != 0 in those of `into`, to which the tokens before them are copied too.  kept
+ * [batch]: the new lengths, or -1 where nothing was moved: a length that the pages cannot hold or less
+ * than the marked tokens, or one that `into` has no room for.  `into` has as many sequences, and
+ * its pages are none that the call reads.  pieces as for fsp_attention_paged (only with other != 0).
+ */
+struct fsp_paged_keep_args {
+  struct fsp_paged_cache cache;
+  struct fsp_paged_cache into;
+  int64_t other, n_tokens, each, n_pieces, piece;
+  const int32_t* pieces;
+  const uint8_t* keep;
+  const int32_t* token_indptr;
+  const int32_t* lengths;
+  int32_t* kept;
+};
+int fsp_paged_keep(const struct fsp_paged_keep_args* args, void* stream);
+
+/*
+ * Copies page sources[i] of k_pages and of v_pages to page targets[i], i in [0, n); nothing where either is
+ * outside the cache.  No page is the target of two, and none that is a target is another's source.
+ * The page table is not used.
+ */
+int fsp_paged_copy(const struct fsp_paged_cache* cache, const int32_t* sources, const int32_t* targets,
+                   int64_t n, void* stream);
 
 /*
  * Attention of one query per sequence over the cache: q, out [batch, heads, dim], lse

@@ -1,0 +1,148 @@
+"""Drafted trees, kept tokens and copied pages without a GPU: work lists, argument structs, the refusals of the
+library, and which drafted tokens the tests' reference lets a row see."""
+
+import numpy as np
+import pytest
+import torch
+
+import flagsparse_amd as fs
+from flagsparse_amd import _abi, attention
+from tests import test_attention_cpu as base
+from tests.test_gpu_tree import _masks, _ways
+
+_TREE_ARGS = dict(pieces=16, first=16, n_pieces=3, piece=256, heads=4, window=0, scale=0.125, sinks=0, tokens=6,
+                  longest=3, qt=256, qh=64, ot=256, oh=64, q=64, out=64, lse=0, lengths=16, indptr=16,
+                  parents=16, work=16)
+_KEEP_ARGS = dict(other=0, tokens=6, each=3, n_pieces=3, piece=256, pieces=16, keep=3, indptr=16, lengths=16,
+                  kept=16)
+
+
+def _tree(**kw):
+    a = list((_TREE_ARGS | kw).values())
+    return attention._TREE.pack(*a[:14]) + attention._TREE_AT.pack(*a[14:])
+
+
+def _keep(**kw):
+    a = list((_KEEP_ARGS | kw).values())
+    return attention._KEEP.pack(*a[:5]) + attention._KEEP_AT.pack(*a[5:])
+
+
+def test_struct_sizes():
+    assert attention._TREE.size + attention._TREE_AT.size == 8 * 21
+    assert attention._KEEP.size + attention._KEEP_AT.size == 8 * 10
+    assert _abi.lib().fsp_attention_tree_drafts() == 256
+
+
+@pytest.mark.parametrize("kw", [
+    {"heads": 3}, {"heads": 0}, {"window": -1}, {"window": 2**40}, {"sinks": 4}, {"sinks": -1, "window": 4},
+    {"sinks": 2**31, "window": 4}, {"scale": float("nan")}, {"scale": 1e39}, {"piece": 0}, {"piece": 130},
+    {"piece": 1 << 21}, {"n_pieces": 1}, {"n_pieces": 1 << 40}, {"tokens": -1}, {"tokens": 2**31},
+    {"longest": 257}, {"longest": -1}, {"longest": 0}, {"indptr": 0, "tokens": 5}, {"q": 0}, {"q": 72},
+    {"out": 0}, {"oh": 2}, {"qt": 12}, {"lengths": 0}, {"pieces": 0}, {"work": 0}, {"work": 8}, {"first": 0}])
+def test_tree_refusals_of_the_library(kw):
+    L = _abi.lib()
+    assert L.fsp_attention_tree(base._cache() + _tree(**kw), None) == -1
+    assert L.fsp_last_error()
+    assert L.fsp_attention_tree(None, None) == -1
+
+
+@pytest.mark.parametrize("kw", [{"tokens": -1}, {"tokens": 2**31}, {"each": -1}, {"each": 2, "indptr": 0},
+                                {"keep": 0}, {"lengths": 0}, {"kept": 0}])
+def test_keep_refusals_of_the_library(kw):
+    L, c = _abi.lib(), base._cache()
+    for other in (0, 1):
+        assert L.fsp_paged_keep(c + c + _keep(**({"other": other} | kw)), None) == -1
+    assert L.fsp_paged_keep(None, None) == -1
+
+
+@pytest.mark.parametrize("kw", [{"dtype": 3}, {"kv_heads": 1}, {"dim": 72}, {"batch": 1}, {"k": 0},
+                                {"page_size": 0}, {"kp": 4}])
+def test_keep_refuses_another_kind_of_cache(kw):
+    c = base._cache()
+    assert _abi.lib().fsp_paged_keep(c + base._cache(**kw) + _keep(other=1), None) == -1
+
+
+@pytest.mark.parametrize("kw", [{"pieces": 0}, {"n_pieces": 1}, {"n_pieces": 1 << 40}, {"piece": 0},
+                                {"piece": 2048}, {"piece": 200}])
+def test_keep_into_refuses_lists(kw):
+    c = base._cache()
+    assert _abi.lib().fsp_paged_keep(c + c + _keep(other=1, **kw), None) == -1
+
+
+@pytest.mark.parametrize("status,kw", [
+    (-3, {"dtype": 1}), (-3, {"dim": 130}), (-1, {"page_size": 0}), (-1, {"batch": -1}),
+    (-1, {"n_pages": 1 << 31}), (-1, {"table_len": 1 << 28}), (-1, {"k": 0}), (-1, {"v": 8}),
+    (-1, {"kp": 4}), (-1, {"indptr": 0}), (-1, {"indices": 0})])
+def test_cache_refusals_of_the_library(status, kw):
+    L, c = _abi.lib(), base._cache(**kw)
+    assert L.fsp_attention_tree(c + _tree(), None) == status
+    assert L.fsp_paged_keep(c + c + _keep(), None) == status
+    assert L.fsp_paged_copy(c, 16, 16, 4, None) == status
+    assert L.fsp_paged_append_drafts(c + base._append(), 16, None) == status
+
+
+def test_copy_and_append_refusals_of_the_library():
+    L, c = _abi.lib(), base._cache()
+    for args in ((c, None, 16, 4), (c, 16, None, 4), (c, 16, 16, -1), (c, 16, 16, 1 << 40), (None, 16, 16, 4)):
+        assert L.fsp_paged_copy(*args, None) == -1
+    assert L.fsp_paged_copy(c, None, None, 0, None) == 0
+    huge = base._cache(page_size=1 << 30, n_pages=1, table_len=1)
+    assert L.fsp_paged_copy(huge, 16, 16, 1, None) == -1  # its rows are counted in 32 bits
+    assert L.fsp_paged_append_drafts(c + base._append(), None, None) == -1
+    assert L.fsp_paged_append_drafts(None, 16, None) == -1
+    assert L.fsp_paged_append_drafts(c + base._append(half=33), 16, None) == -1
+
+
+@pytest.mark.parametrize("pages", [[], [0], [8, 0, 9, 1], [320, 1, 8]])
+@pytest.mark.parametrize("sight", [1, 100, 256, 257, 3000, 2**31 - 1024])
+def test_pieces_under_a_window(pages, sight):
+    # as many as ``sight`` tokens in a row can touch wherever they start, no more than the room takes
+    table, firsts, most = attention._pieces(np.array(pages, dtype=np.int64), 16, 256, sight)
+    at = 0
+    for b, n in enumerate(pages):
+        assert firsts[b] == at
+        room = max(1, -(-16 * n // 256))
+        need = max(len(set(range(s // 256, (s + min(sight, 6000) - 1) // 256 + 1))) for s in range(256))
+        count = int((table[:, 0] == b).sum())
+        assert min(room, need) <= count <= room
+        for i in range(count):
+            assert table[at].tolist() == [b, 256 * i, int(firsts[b]), sum(pages[:b]), 16 * n, 0, 0, 0]
+            at += 1
+    assert at == len(table) and most == max([1] + np.bincount(table[:, 0], minlength=1).tolist())
+
+
+def test_tree_piece_sizes():
+    L = _abi.lib()
+    for tokens in (0, 1, 1000, 50000, 10**6, 2**31):
+        for heads, group in ((1, 1), (8, 4), (64, 1), (1, 64)):
+            for longest in (1, 8, 64, 256):
+                piece = L.fsp_attention_tree_piece(tokens, heads, group, longest)
+                assert 128 <= piece <= 1 << 20 and piece % 128 == 0
+
+
+def test_ways_and_masks_of_the_reference():
+    assert _ways([-1, 0, 0, 2, -1]) == [[0], [0, 1], [0, 2], [0, 2, 3], [4]]
+    m = _masks([2], [[-1, 0, 0, 2]])[0]
+    assert m.int().tolist() == [[1, 1, 1, 0, 0, 0], [1, 1, 1, 1, 0, 0], [1, 1, 1, 0, 1, 0], [1, 1, 1, 0, 1, 1]]
+    m = _masks([2], [[-1, 0, 0, 2]], window=2, sinks=1)[0]
+    # positions 2, 3, 3, 4
+    assert m.int().tolist() == [[1, 1, 1, 0, 0, 0], [1, 0, 1, 1, 0, 0], [1, 0, 1, 0, 1, 0], [1, 0, 0, 0, 1, 1]]
+
+
+def test_refusals_that_need_no_device():
+    q = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
+    n = torch.tensor([4])
+    with pytest.raises(TypeError):
+        fs.flagsparse_attention_paged_tree(q, n, prepared=q)
+    with pytest.raises(ValueError):
+        fs.flagsparse_attention_paged_tree(q, n)
+    with pytest.raises(TypeError):
+        fs.flagsparse_paged_keep(n > 0, n, prepared=q)
+    with pytest.raises(ValueError):
+        fs.flagsparse_paged_keep(n > 0, n)
+    with pytest.raises(ValueError):
+        fs.flagsparse_paged_copy(n, n)
+    with pytest.raises(TypeError):
+        fs.flagsparse_paged_copy(n, n, prepared=q)
+    with pytest.raises(ValueError):
+        fs.flagsparse_paged_copy(n, n, k_pages=q[None], v_pages=q[None])
