@@ -1,10 +1,12 @@
 // Attention of trees of drafted tokens over a paged cache that holds them at its sequences' ends.
 #include "paged.hpp"
+#include "tiles.hpp"
 
 namespace fsp {
 namespace {
 
 constexpr int kDrafts = 256;     // drafted tokens of one sequence, at most
+constexpr int kWideFrom = 64;    // more rows than so many beside a key go to wide tiles
 constexpr int kTableKeys = 1024;  // keys whose places LDS holds at a time
 
 struct TreeShape {
@@ -45,13 +47,25 @@ __device__ void nan_rows(T* out, int64_t out_token, int64_t out_head, float* lse
   }
 }
 
+// The rows that belong to no sequence, and those of one that is not as it should be.
+template <typename T>
+__device__ __forceinline__ void nan_outside(const TreeShape& s, const Drafted& t, const int32_t* tokens, int b,
+                                            int batch, T* out, int64_t out_token, int64_t out_head, float* lse,
+                                            int head0, int group, int dim) {
+  const int from = tokens ? min(max(tokens[b], 0), s.n_tokens) : t.begin;
+  const int to = tokens ? min(max(tokens[b + 1], 0), s.n_tokens) : t.begin + s.longest;
+  if (!t.ok) nan_rows(out, out_token, out_head, lse, s.heads, head0, group, dim, from, to);
+  if (b == 0) nan_rows(out, out_token, out_head, lse, s.heads, head0, group, dim, 0, from);
+  if (b == batch - 1) nan_rows(out, out_token, out_head, lse, s.heads, head0, group, dim, to, s.n_tokens);
+}
+
 // Which drafted tokens a row's token sees, itself among them, by its way up the tree, as words 1 .. 8 of
 // ``mask`` between one of ones and one of zeros; returns its depth, or -1 where the way does not lead up.
 __device__ __forceinline__ int row_mask(const TreeShape& s, const Drafted& t, const int* up, int i,
                                         uint32_t* mask) {
   mask[0] = ~0u;
 #pragma unroll
-  for (int w = 1; w < 10; ++w) mask[w] = 0;
+  for (int w = 1; w < 11; ++w) mask[w] = 0;
   int depth = i;
   if (up) {
     depth = 0;
@@ -101,13 +115,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attention_tree_kernel(
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int head0 = g * group;
   const Drafted t(s, tokens, b, lengths[b], pc.room);
-  if (pc.begin == 0 && tile == 0) {  // what belongs to no sequence, or to one that is not as it should be
-    const int from = tokens ? min(max(tokens[b], 0), s.n_tokens) : t.begin;
-    const int to = tokens ? min(max(tokens[b + 1], 0), s.n_tokens) : t.begin + s.longest;
-    if (!t.ok) nan_rows(out, out_token, out_head, lse, s.heads, head0, group, c.dim, from, to);
-    if (b == 0) nan_rows(out, out_token, out_head, lse, s.heads, head0, group, c.dim, 0, from);
-    if (b == c.batch - 1) nan_rows(out, out_token, out_head, lse, s.heads, head0, group, c.dim, to, s.n_tokens);
-  }
+  if (pc.begin == 0 && tile == 0)
+    nan_outside(s, t, tokens, b, c.batch, out, out_token, out_head, lse, head0, group, c.dim);
   const int rows = t.count * group, r0 = tile * ROWS;
   if (r0 >= rows) return;
   const int p0 = t.first / s.piece, p1 = (t.last + s.piece - 1) / s.piece;
@@ -323,6 +332,214 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attention_tree_kernel(
   }
 }
 
+// Rows past a head's dim are read from here.
+__device__ const i32x4 kZeros = {0, 0, 0, 0};
+
+// Many rows: 128 of them a workgroup, 32 a wave, over the same 64 keys, which go straight to LDS by the places
+// that a table there holds, the next step's while this one's are worked on: as attention_packed_kernel, whose
+// comments say how the products lie.  The table's two halves of 256 keys are filled in turn.
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 2) void attention_tree_wide_kernel(
+    Cache c, TreeShape s, const Piece* __restrict__ pieces, const T* __restrict__ k_pages,
+    const T* __restrict__ v_pages, const T* __restrict__ q, int64_t q_token, int64_t q_head,
+    T* __restrict__ out, int64_t out_token, int64_t out_head, float* __restrict__ lse,
+    const int32_t* __restrict__ lengths, const int32_t* __restrict__ tokens,
+    const int32_t* __restrict__ parents, float* part_o, float* part_ml) {
+  typedef Lay<DP> L;
+  constexpr int NS = DP / 16, NT = DP / 32, ROWS = 128, HALF = 256;
+  __shared__ __attribute__((aligned(1024))) char s_k0[L::BYTES], s_v0[L::BYTES], s_k1[L::BYTES], s_v1[L::BYTES];
+  __shared__ int64_t s_k[2 * HALF], s_v[2 * HALF];
+  __shared__ uint32_t s_mask[ROWS][11];
+  __shared__ int s_depth[ROWS], s_up[kDrafts];
+  const int group = s.heads / c.kv_heads;
+  int piece, g, tile;
+  piece_and_head(blockIdx.x, s.n_pieces, c.kv_heads * s.tiles, piece, tile);
+  g = tile / s.tiles;
+  tile -= g * s.tiles;
+  const Piece pc = pieces[piece];
+  const int b = pc.seq, lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int head0 = g * group;
+  const Drafted t(s, tokens, b, lengths[b], pc.room);
+  if (pc.begin == 0 && tile == 0)
+    nan_outside(s, t, tokens, b, c.batch, out, out_token, out_head, lse, head0, group, c.dim);
+  const int rows = t.count * group, r0 = tile * ROWS;
+  if (r0 >= rows) return;
+  const int p0 = t.first / s.piece, p1 = (t.last + s.piece - 1) / s.piece;
+  const int mine = p0 + pc.begin / s.piece;
+  if (mine >= p1) return;
+  const int begin = max(t.first, mine * s.piece);
+  const int end = (int)min((int64_t)t.last, ((int64_t)mine + 1) * s.piece);
+  const int n = end - begin, steps = (n + kRows - 1) / kRows;
+
+  const int q0 = r0 + 32 * wave, row = q0 + col;
+  const bool active = q0 < rows;
+  V8<T> qf[NS];
+  {
+    const int r = min(row, rows - 1);
+    const T* qr = q + (int64_t)(t.begin + r / group) * q_token + (head0 + r % group) * q_head;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const int d = 16 * i + 8 * half;
+      const V8<T> x = *reinterpret_cast<const V8<T>*>(qr + (d < c.dim ? d : 0));
+      qf[i] = scaled_sign<T>(x, s.scale, d < c.dim);
+    }
+  }
+  const float cs = exp2_scale(s.scale);
+
+  // where key 256 * h + threadIdx.x of the piece lies; those past the end stand for the first one
+  auto place = [&](int h, int64_t& k, int64_t& v) {
+    const int i = HALF * h + threadIdx.x, e = begin + (i < n ? i : 0);
+    const uint32_t j = e < t.old ? e - t.first : e, at = j / (uint32_t)c.page_size;
+    const int64_t page = c.indices[pc.page + at], slot = j - at * c.page_size;
+    k = page * c.k_page + slot * c.k_slot;
+    v = page * c.v_page + slot * c.v_slot;
+  };
+#pragma unroll
+  for (int h = 0; h < 2; ++h) place(h, s_k[HALF * h + threadIdx.x], s_v[HALF * h + threadIdx.x]);
+  const bool masked = s.window || end > t.past;
+  if (masked && parents)
+    for (int i = threadIdx.x; i < t.count; i += 256) s_up[i] = parents[t.begin + i];
+  __syncthreads();
+
+  const T* kb = k_pages + g * c.k_head;
+  const T* vb = v_pages + g * c.v_head;
+  constexpr int PER = kRows * L::PITCH / 1024 / 4, EACH = 1024 / L::PITCH;
+  const int l_row = wave * PER * EACH + lane / L::CH;
+  const int l_chunk = (lane % L::CH) ^ L::swizzle(lane / L::CH) ^ L::swizzle(wave * PER * EACH);
+  auto load = [&](int step, char* sk, char* sv) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int at = (step * kRows & (2 * HALF - 1)) + l_row + i * EACH;
+      const int d = 8 * (l_chunk ^ L::swizzle(i * EACH));
+      const void* kp = d < c.dim ? (const void*)(kb + s_k[at] + d) : (const void*)&kZeros;
+      const void* vp = d < c.dim ? (const void*)(vb + s_v[at] + d) : (const void*)&kZeros;
+      typedef __attribute__((address_space(3))) void lds_void;
+      typedef const __attribute__((address_space(1))) void global_void;
+      __builtin_amdgcn_global_load_lds((global_void*)kp, (lds_void*)(sk + (wave * PER + i) * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((global_void*)vp, (lds_void*)(sv + (wave * PER + i) * 1024), 16, 0, 0);
+    }
+  };
+  load(0, s_k0, s_v0);
+  if (masked && threadIdx.x < ROWS)
+    s_depth[threadIdx.x] = row_mask(s, t, parents ? s_up : nullptr,
+                                    min(r0 + (int)threadIdx.x, rows - 1) / group, s_mask[threadIdx.x]);
+
+  f32x16 o[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) o[i] = f32x16{};
+  float top = -INFINITY, sum = 0;
+  const int k_at = L::row_at(lane), v_at = L::col_at(lane);
+  all_stored();
+  __syncthreads();
+  const int lo = s.window ? t.past + s_depth[32 * wave + col] - s.window + 1 : 0;
+
+  auto work = [&](int step, const char* sk_, const char* sv_) {
+    if (!active) return;
+    const lds_char* sk = (const lds_char*)sk_;
+    const lds_char* sv = (const lds_char*)sv_;
+    f32x16 x[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      x[u] = f32x16{};
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+        x[u] = mfma32(row_frag<T>(sk + (k_at ^ (i * 32)) + u * 32 * L::PITCH), qf[i], x[u]);
+    }
+    read_ahead<2 * NS, NS>();
+    const int j0 = step * kRows, e0 = begin + j0;
+    const bool tail = e0 + kRows > t.past;
+    if (tail || j0 + kRows > n || __any(lo > max(e0, t.old))) {
+      const int off = e0 - t.past, w = max(off, -64) >> 5, shift = off & 31;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        uint32_t bits = ~0u;
+        if (tail && w + u >= -1) {
+          const uint32_t* m = s_mask[32 * wave + col] + 1 + w + u;
+          bits = shift ? m[0] >> shift | m[1] << (32 - shift) : m[0];
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int k = 8 * (r / 4) + r % 4 + 4 * half, at = e0 + 32 * u + k;
+          const bool near = at >= lo || at < s.sinks || at < t.old || at >= t.past;
+          x[u][r] = (bits >> k & 1) && near && j0 + 32 * u + k < n ? x[u][r] : -INFINITY;
+        }
+      }
+    }
+    float m = x[0][0];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) m = fmaxf(m, x[u][r]);
+    m = fmaxf(m, other_half(m));
+    if (__any((m - top) * cs > Weights<T>::lag)) {
+      const float now = fmaxf(top, m);
+      const float fade = top == -INFINITY ? 0.0f : exp2f((top - now) * cs);
+      top = now;
+      sum *= fade;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) o[i] *= fade;
+    }
+    const float base = top == -INFINITY ? 0.0f : top * cs - Weights<T>::up;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        x[u][r] = __builtin_amdgcn_exp2f(fmaf(x[u][r], cs, -base));
+        sum += x[u][r];
+      }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const V8<T> pf = to16<T>(x[i / 2], 8 * (i % 2));
+#pragma unroll
+      for (int d = 0; d < NT; ++d)
+        o[d] = mfma32(col_frag<T, L::PITCH>(sv, v_at ^ (64 * d), i), pf, o[d]);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x100, 4 * NT, 1);  // the first values early
+  };
+  // one step; the table's other half is filled when the last of its keys have been asked for
+  auto pass = [&](int step, char* sk, char* sv, char* next_k, char* next_v) {
+    const bool fill = step % 4 == 0 && step > 0 && (step + 4) * kRows < n;
+    int64_t k, v;
+    if (fill) place(step / 4 + 1, k, v);
+    if (step + 1 < steps) load(step + 1, next_k, next_v);
+    work(step, sk, sv);
+    if (fill) {
+      const int at = (step / 4 + 1) % 2 * HALF + threadIdx.x;
+      s_k[at] = k;
+      s_v[at] = v;
+    }
+    all_stored();
+    __syncthreads();
+  };
+  for (int step = 0; step < steps;) {
+    pass(step, s_k0, s_v0, s_k1, s_v1);
+    if (++step >= steps) break;
+    pass(step, s_k1, s_v1, s_k0, s_v0);
+    ++step;
+  }
+
+  if (row >= rows) return;
+  sum += other_half(sum);
+  if (sum == 0)  // nothing seen: zeros, whatever lies in the rows of V
+#pragma unroll
+    for (int i = 0; i < NT; ++i) o[i] = f32x16{};
+  if (masked && s_depth[32 * wave + col] < 0) sum = __builtin_nanf("");
+  if (p1 - p0 > 1) {
+    const int64_t at = (int64_t)(pc.slot + mine - p0) * s.longest * s.heads + (int64_t)g * s.longest * group + row;
+    store_rows<float, NT>(part_o + at * c.dim, o, 1.0f, c.dim, half);
+    if (half == 0)
+      *reinterpret_cast<f32x2*>(part_ml + 2 * at) = f32x2{top == -INFINITY ? -INFINITY : top * cs, sum};
+    return;
+  }
+  const int64_t token = t.begin + row / group;
+  const int head = head0 + row % group;
+  if (half == 0 && lse)
+    lse[token * s.heads + head] =
+        sum == 0 ? -INFINITY : (top * cs + log2f(sum * Weights<T>::down)) * kLn2;
+  store_rows<T, NT>(out + token * out_token + head * out_head, o, sum == 0 ? 0.0f : 1.0f / sum, c.dim, half);
+}
+
 // Joins the pieces of sequences that have several: half a wave to a row, eight pieces of it at a time.
 template <typename T>
 __global__ __launch_bounds__(256) void attention_tree_join_kernel(
@@ -380,19 +597,21 @@ __global__ __launch_bounds__(256) void attention_tree_join_kernel(
     lse[token * s.heads + head] = total == 0 ? -INFINITY : (most + log2f(total * Weights<T>::down)) * kLn2;
 }
 
-int row_tiles(int64_t longest, int64_t group) {
-  return longest * group <= 16 ? 1 : 2;
+// Rows of a workgroup's tile.
+int64_t tile_rows(int64_t longest, int64_t group) {
+  const int64_t rows = longest * group;
+  return rows <= 16 ? 16 : rows <= kWideFrom ? 32 : 128;
 }
 
-template <typename T, int DP, bool EXACT, bool NT, int RT>
-int launch_tree(const fsp_attention_tree_args& a, hipStream_t st) {
-  const int64_t group = a.heads / a.cache.kv_heads, tiles = (a.longest * group + 16 * RT - 1) / (16 * RT);
+template <typename T, typename Kernel>
+int launch_tree(const fsp_attention_tree_args& a, Kernel kernel, hipStream_t st) {
+  const int64_t group = a.heads / a.cache.kv_heads, each = tile_rows(a.longest, group);
+  const int64_t tiles = (a.longest * group + each - 1) / each;
   const TreeShape s{(int)a.heads,    (int)a.window,  (int)a.sinks, (int)a.piece,  (int)a.n_pieces,
                     (int)a.n_tokens, (int)a.longest, (int)tiles,   (float)a.scale};
   float* part_o = static_cast<float*>(a.workspace);
   float* part_ml = part_o + a.n_pieces * a.longest * a.heads * a.cache.dim;
-  hipLaunchKernelGGL((attention_tree_kernel<T, DP, EXACT, NT, RT>),
-                     dim3((unsigned)(a.n_pieces * a.cache.kv_heads * tiles)), dim3(256), 0, st,
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(a.n_pieces * a.cache.kv_heads * tiles)), dim3(256), 0, st,
                      cache_of(a.cache), s, reinterpret_cast<const Piece*>(a.pieces),
                      static_cast<const T*>(a.cache.k_pages), static_cast<const T*>(a.cache.v_pages),
                      static_cast<const T*>(a.q), a.q_token, a.q_head, static_cast<T*>(a.out), a.out_token,
@@ -408,8 +627,9 @@ int launch_tree(const fsp_attention_tree_args& a, hipStream_t st) {
 
 template <typename T, int DP, bool EXACT, bool NT>
 int launch_tree_rows(const fsp_attention_tree_args& a, hipStream_t st) {
-  const int rt = row_tiles(a.longest, a.heads / a.cache.kv_heads);
-  return rt == 1 ? launch_tree<T, DP, EXACT, NT, 1>(a, st) : launch_tree<T, DP, EXACT, NT, 2>(a, st);
+  return tile_rows(a.longest, a.heads / a.cache.kv_heads) == 16
+             ? launch_tree<T>(a, attention_tree_kernel<T, DP, EXACT, NT, 1>, st)
+             : launch_tree<T>(a, attention_tree_kernel<T, DP, EXACT, NT, 2>, st);
 }
 
 template <typename T, int DP, bool EXACT>
@@ -422,9 +642,14 @@ int launch_tree_nt(const fsp_attention_tree_args& a, hipStream_t st) {
 
 template <typename T>
 int launch_tree_dim(const fsp_attention_tree_args& a, hipStream_t st) {
-  if (a.cache.dim == 64) return launch_tree_nt<T, 64, true>(a, st);
-  if (a.cache.dim < 64) return launch_tree_nt<T, 64, false>(a, st);
-  if (a.cache.dim < 128) return launch_tree_nt<T, 128, false>(a, st);
+  const int64_t dim = a.cache.dim;
+  if (tile_rows(a.longest, a.heads / a.cache.kv_heads) == 128)
+    return dim <= 64   ? launch_tree<T>(a, attention_tree_wide_kernel<T, 64>, st)
+           : dim <= 96 ? launch_tree<T>(a, attention_tree_wide_kernel<T, 96>, st)
+                       : launch_tree<T>(a, attention_tree_wide_kernel<T, 128>, st);
+  if (dim == 64) return launch_tree_nt<T, 64, true>(a, st);
+  if (dim < 64) return launch_tree_nt<T, 64, false>(a, st);
+  if (dim < 128) return launch_tree_nt<T, 128, false>(a, st);
   return launch_tree_nt<T, 128, true>(a, st);
 }
 
@@ -437,7 +662,7 @@ extern "C" int64_t fsp_attention_tree_drafts(void) { return kDrafts; }
 
 extern "C" int64_t fsp_attention_tree_piece(int64_t tokens, int64_t kv_heads, int64_t group, int64_t longest) {
   if (tokens < 0 || kv_heads < 1 || group < 1 || longest < 1) return 256;
-  const int64_t rows = 16 * row_tiles(longest, group), tiles = (longest * group + rows - 1) / rows;
+  const int64_t rows = tile_rows(longest, group), tiles = (longest * group + rows - 1) / rows;
   int64_t piece = 256;
   while (piece < 4096 && tokens / piece * kv_heads * tiles > 1024) piece *= 2;
   return piece;
