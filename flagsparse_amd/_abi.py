@@ -129,7 +129,8 @@ SIGNATURES = {
     "fsp_attention_paged": (_i32, [_p, _p]),
     "fsp_attention_paged_sinks": (_i32, [_p, _i64, _p]),
     "fsp_attention_tree_drafts": (_i64, []),
-    "fsp_attention_tree_piece": (_i64, [_i64, _i64, _i64, _i64]),
+    "fsp_attention_tree_rows": (_i64, [_i64, _i64]),
+    "fsp_attention_tree_counts": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "fsp_attention_tree_workspace": (_i64, [_i64, _i64, _i64, _i64]),
     "fsp_attention_tree": (_i32, [_p, _p]),
     "fsp_attention_packed_tile": (_i64, [_i32]),

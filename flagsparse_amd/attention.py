@@ -46,7 +46,7 @@ _APPEND, _APPEND_AT = struct.Struct("13q"), struct.Struct("8q")
 _PAGED, _PAGED_AT = struct.Struct("6qd4q"), struct.Struct("6q")
 _PACKED, _PACKED_AT = struct.Struct("10qd24q"), struct.Struct("10q")
 _KEEP, _KEEP_AT = struct.Struct("5q"), struct.Struct("5q")
-_TREE, _TREE_AT = struct.Struct("6qd7q"), struct.Struct("7q")
+_TREE, _TREE_AT = struct.Struct("6qd7q"), struct.Struct("8q")
 
 # A prepared object keeps the first part for each layout of arrays that it has checked, so that the
 # next call with such arrays is a look-up and a launch.  Of a cache it holds the pages' addresses, which
@@ -279,25 +279,57 @@ class PreparedPagedKV:
             self._streams.mark(stream, self.device, (self.indptr, self.indices, self._pieces))
         return stream
 
-    def _tokens(self, sight):
-        """The tokens of all sequences that a call reads which sees ``sight`` of each (0: all)."""
-        rooms = self._held * self.page_size
-        return int((np.minimum(rooms, sight) if sight else rooms).sum())
-
-    def _list(self, piece, sight):
-        """(pieces, first pieces, most of one sequence, streams that they are marked on): pieces of
-        ``piece`` tokens, of each sequence no more than ``sight`` tokens in a row can touch (0: all of
-        its room), made when first asked for and kept."""
-        kept = self._lists.get((piece, sight))
+    def _list(self, sight, each, slots, most, rows):
+        """(tokens of a piece, pieces, first pieces, most of one sequence, streams that they are marked on):
+        pieces of at most ``most`` tokens, of each sequence no more than ``sight`` tokens in a row can
+        touch (0: all of its room), that go to ``each`` workgroups of ``rows`` rows, of which ``slots`` run
+        at a time; made when first asked for and kept."""
+        key = (sight, each, slots, most, rows)
+        kept = self._lists.get(key)
         if kept is None:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("a call's first run with these sizes builds its work list, which "
                                    "cannot be captured: make one such call before the capture")
+            piece = _piece_of(self._held * self.page_size, *key)
             table = _on_device(*_pieces(self._held, self.page_size, piece, sight), piece, self.device)
             torch.cuda.current_stream(self.device).synchronize()  # calls may come from other streams
-            kept = (*table, _Streams())
-            _keep(self._lists, (piece, sight), kept)
+            kept = (piece, *table, _Streams())
+            _keep(self._lists, key, kept)
         return kept
+
+
+def _piece_of(rooms, sight, each, slots, most, rows):
+    """The tokens of a piece, from 256 to ``most``, by which the pieces of all sequences end soonest.  A
+    workgroup takes as long as its tokens, and 100 + 2 * rows for what it does before and after them
+    (its sums are written and read again); all of them take something between their sum over the
+    ``slots`` and rounds of ``slots`` that wait for each other.  Mostly that gives whole rounds of even pieces: 8
+    sequences of 30064, 8 key heads, 256 rows beside each (16 workgroups a piece), pieces of 2048 / 3840 /
+    4096 / 5120 / 7552 (one round) / 10112 tokens 391 / 368 / 373 / 379 / 361 / 398 us; 96 ragged ones of up to
+    8000, 32 rows, of 256 / 512 / 1024 / 2048 / 4096 111 / 98 / 90 / 87 / 89 us, 128 rows 152 / 131 / 116 / 112 /
+    142; 33 ragged ones under a window of 2047, 23 heads of 80, up to 26 tokens, of 128 / 256 / 512 / 1024
+    35 / 28 / 32 / 40."""
+    seen = np.minimum(rooms, sight) if sight else rooms
+    around = 100 + 2 * rows
+    longest = int(seen.max(initial=0))
+    best = (float("inf"), 256)
+    n = max(1, -(-longest // most))
+    while True:
+        piece = max(256, -(-longest // n // 128) * 128)
+        whole = seen // piece
+        rest = np.sort(seen - whole * piece)[::-1]
+        rest = rest[rest > 0]
+        count = int(whole.sum()) * each
+        starts = np.arange(0, max(1, count + each * len(rest)), slots)
+        firsts = np.full(len(starts), piece)
+        if len(rest):
+            after = np.maximum(starts - count, 0) // each
+            firsts = np.where(starts < count, piece, rest[np.minimum(after, len(rest) - 1)])
+        total = each * (int(seen.sum()) + around * (int(whole.sum()) + len(rest)))
+        rounds = float((firsts + around).sum())
+        best = min(best, (rounds + max(total / slots, float(firsts[0] + around)), piece))
+        if piece == 256:
+            return best[1]
+        n += 1 + n // 8
 
 
 def _on_device(table, first, most, piece, device):
@@ -568,8 +600,8 @@ def flagsparse_paged_keep(keep, lengths, token_indptr=None, *, prepared=None, k_
     if prepared is None:
         _check_drafts(kv, n, token_indptr, None, tokens, each if token_indptr is None else tokens)
     keep = keep.contiguous()
-    kept = (kv._packed(), (tokens, each, kv._pieces.shape[0], kv._piece),
-            _like((kv.batch,), torch.int32, dev))
+    head, sizes = kv._packed(), (tokens, each, kv._pieces.shape[0], kv._piece)
+    kept = (head, sizes, head + head + _KEEP.pack(0, *sizes), _like((kv.batch,), torch.int32, dev))
     res = _keep_tokens(kv, into, kept, keep, token_indptr, n)
     if key is not None and all(x is y for x, y in zip((keep, lengths, token_indptr), given)):
         _keep(kv._calls, key, kept)
@@ -579,17 +611,17 @@ def flagsparse_paged_keep(keep, lengths, token_indptr=None, *, prepared=None, k_
 def _keep_tokens(kv, into, kept, keep, token_indptr, lengths):
     """The launch; returns the new lengths.  What ``into`` holds is looked up by every call: it is an
     argument, not a part of the prepared cache."""
-    head, sizes, like = kept
-    stream, other = kv._on(), head
+    head, sizes, args, like = kept
+    stream = kv._on()
     if into is not None:
         if into.device != kv.device or into.dtype != kv.dtype:
             raise ValueError("into must be of the cache's type and on its device")
         if (into.batch, into.kv_heads, into.dim) != (kv.batch, kv.kv_heads, kv.dim):
             raise ValueError("into must have the cache's number of sequences, heads and dim")
-        other = into._packed()
+        args = head + into._packed() + _KEEP.pack(1, *sizes)
         into._on()
     res = torch.empty_like(like, memory_format=_CONTIGUOUS)
-    status = _abi.lib().fsp_paged_keep(head + other + _KEEP.pack(into is not None, *sizes) + _KEEP_AT.pack(
+    status = _abi.lib().fsp_paged_keep(args + _KEEP_AT.pack(
         kv._pieces.data_ptr(), keep.data_ptr(), _at(token_indptr), lengths.data_ptr(), res.data_ptr()), stream)
     if status:
         _abi.check(status, "fsp_paged_keep")
@@ -604,10 +636,16 @@ def flagsparse_paged_copy(sources, targets, *, prepared=None, k_pages=None, v_pa
     of two, and none that is a target is another's source.  The cache is given by ``prepared`` or by its
     pages; with ``prepared`` nothing is waited for, so numbers are not checked: a pair with one outside the
     cache copies nothing."""
+    key = None
     if prepared is not None:
         if not isinstance(prepared, PreparedPagedKV):
             raise TypeError("prepared must be a PreparedPagedKV instance")
         kv = prepared
+        key = _layouts(sources, targets) + ("copy", kv.k_pages.data_ptr(), kv.v_pages.data_ptr())
+        kept = kv._calls.get(key)
+        if kept is not None:
+            _copy_pages(kv, kept, sources, targets)
+            return
     else:
         if k_pages is None or v_pages is None:
             raise ValueError("k_pages and v_pages are required when prepared is not provided")
@@ -616,7 +654,7 @@ def flagsparse_paged_copy(sources, targets, *, prepared=None, k_pages=None, v_pa
     for t, name in ((sources, "sources"), (targets, "targets")):
         if not torch.is_tensor(t) or t.ndim != 1:
             raise ValueError(f"{name} must be a 1D tensor")
-    n = sources.numel()
+    n, given = sources.numel(), (sources, targets)
     sources = _int32(sources, "sources", n, kv.device)
     targets = _int32(targets, "targets", n, kv.device)
     if prepared is None and n:
@@ -627,11 +665,17 @@ def flagsparse_paged_copy(sources, targets, *, prepared=None, k_pages=None, v_pa
             raise ValueError("targets must be different pages")
         if bool((torch.isin(sources, targets) & (sources != targets)).any()):
             raise ValueError("a page cannot be a target and another one's source")
-    if n:
-        status = _abi.lib().fsp_paged_copy(kv._packed(), sources.data_ptr(), targets.data_ptr(), n,
-                                           _abi.raw_stream(kv.device))
-        if status:
-            _abi.check(status, "fsp_paged_copy")
+    kept = kv._packed(), n
+    _copy_pages(kv, kept, sources, targets)
+    if key is not None and sources is given[0] and targets is given[1]:
+        _keep(kv._calls, key, kept)
+
+
+def _copy_pages(kv, kept, sources, targets):
+    status = _abi.lib().fsp_paged_copy(kept[0], sources.data_ptr(), targets.data_ptr(), kept[1],
+                                       _abi.raw_stream(kv.device))
+    if status:
+        _abi.check(status, "fsp_paged_copy")
 
 
 def flagsparse_attention_paged(q, lengths, *, prepared=None, k_pages=None, v_pages=None,
@@ -641,7 +685,8 @@ def flagsparse_attention_paged(q, lengths, *, prepared=None, k_pages=None, v_pag
 
     ``q``: [sequences, heads, dim]; ``lengths[b]``: the tokens that sequence b holds, the query's
     own among them (0: the sequence is empty, and its output is zeros).  ``window``: only the last
-    ``window`` tokens are seen, and with ``sinks`` the first ``sinks`` too.  ``scale``: dim ** -0.5 by default.  Returns [sequences, heads, dim],
+    ``window`` tokens are seen, and with ``sinks`` the first ``sinks`` too (the first call with such sizes
+    builds a work list and cannot be captured).  ``scale``: dim ** -0.5 by default.  Returns [sequences, heads, dim],
     with the float32 log-sum-exp [sequences, heads] if ``return_lse``; neither is differentiable, nor
     is what flagsparse_paged_append gives.  With ``prepared`` nothing is
     waited for, so lengths are not checked: one that its sequence's pages cannot hold gives NaN."""
@@ -668,15 +713,19 @@ def flagsparse_attention_paged(q, lengths, *, prepared=None, k_pages=None, v_pag
     res, copied = _result(out, "out", q.shape, dt, dev, q, kv.k_pages, kv.v_pages)
     rows = _rows(q)
     # what such calls share: the arguments, patterns of their arrays, the counts of arrivals they need
-    pieces, need, room = kv._pieces.shape[0], 0, None
+    table, firsts, piece, most, marked = kv._pieces, kv._first, kv._piece, kv._most, None
+    if first:
+        tiles = -(-heads // kv.kv_heads // 16)
+        piece, table, firsts, most, marked = kv._list(min(past + first, _TOKENS_CAP), kv.kv_heads * tiles,
+                                                      768, 1024, 16)
+    pieces, need, room = table.shape[0], 0, None
     if pieces > kv.batch:
-        need = int(_abi.lib().fsp_attention_paged_counts(pieces, kv._most, kv.batch, heads,
-                                                         kv.kv_heads))
+        need = int(_abi.lib().fsp_attention_paged_counts(pieces, most, kv.batch, heads, kv.kv_heads))
         room = _like((pieces * heads * (kv.dim + 2),), torch.float32, dev)
     kept = (kv._packed() + _PAGED.pack(
-        kv._pieces.data_ptr(), kv._first.data_ptr(), pieces, kv._piece, heads, past, factor,
+        table.data_ptr(), firsts.data_ptr(), pieces, piece, heads, past, factor,
         *_steps(rows), *_steps(res)), _like(q.shape, dt, dev),
-        _like((kv.batch, heads), torch.float32, dev), room, need, first)
+        _like((kv.batch, heads), torch.float32, dev), room, need, first, (table, firsts), marked)
     lse = _attend(kv, kept, rows, res, n, return_lse)
     if key is not None and rows is q and n is lengths:
         _keep(kv._calls, key, kept)
@@ -700,11 +749,13 @@ def _arrivals(kv, stream, need):
 
 def _attend(kv, kept, q, res, lengths, return_lse):
     """The launch; returns the log-sum-exp, if asked for."""
-    head, _, like_lse, room, need, sinks = kept
+    head, _, like_lse, room, need, sinks, lists, marked = kept
     lse = torch.empty_like(like_lse, memory_format=_CONTIGUOUS) if return_lse else None
     if not kv.batch:
         return lse
     stream, work, counts = kv._on(), None, None
+    if marked is not None and stream not in marked.seen:
+        marked.mark(stream, kv.device, lists)
     if room is not None:
         work = torch.empty_like(room, memory_format=_CONTIGUOUS)
         if need:
@@ -789,18 +840,22 @@ def flagsparse_attention_paged_tree(q, lengths, token_indptr=None, *, parents=No
         if return_lse:
             lse.fill_(float("nan"))
     else:
-        sight = min(past + first + longest, _TOKENS_CAP) if past else 0
-        piece = int(_abi.lib().fsp_attention_tree_piece(kv._tokens(sight), kv.kv_heads,
-                                                        heads // kv.kv_heads, longest))
-        pieces, firsts, _, marked = kv._list(piece, sight)
-        n_pieces = pieces.shape[0]
-        room = None
+        # the same for all calls of a program, whatever numbers of tokens they have
+        sight = min(past + first + most, _TOKENS_CAP) if past else 0
+        group = heads // kv.kv_heads
+        of = int(_abi.lib().fsp_attention_tree_rows(group, longest))
+        # tiles of an average sequence: those of the longest trees are few
+        tiles = min(-(-group * longest // of), 1 + group * tokens // (kv.batch * of))
+        piece, pieces, firsts, longest_list, marked = kv._list(sight, kv.kv_heads * tiles, 512, 8192, of)
+        n_pieces, need, room = pieces.shape[0], 0, None
         if n_pieces > kv.batch:
+            need = int(_abi.lib().fsp_attention_tree_counts(n_pieces, longest_list, kv.batch, kv.kv_heads,
+                                                            group, longest))
             room = _like((n_pieces * longest * heads * (kv.dim + 2),), torch.float32, dev)
         head = kv._packed() + _TREE.pack(
             pieces.data_ptr(), firsts.data_ptr(), n_pieces, piece, heads, past, factor, first, tokens,
             longest, *_steps(rows), *_steps(res))
-        kept = (head, _like(q.shape, dt, dev), _like(q.shape[:2], torch.float32, dev), room,
+        kept = (head, _like(q.shape, dt, dev), _like(q.shape[:2], torch.float32, dev), room, need,
                 (pieces, firsts), marked)
         lse = _attend_tree(kv, kept, rows, res, n, token_indptr, parents, return_lse)
         if key is not None and all(x is y for x, y in zip((rows, n, token_indptr, parents), given)):
@@ -833,14 +888,15 @@ def _check_drafts(kv, lengths, token_indptr, parents, tokens, longest):
 
 def _attend_tree(kv, kept, q, res, lengths, token_indptr, parents, return_lse):
     """The launch; returns the log-sum-exp, if asked for."""
-    head, _, like_lse, room, lists, marked = kept
+    head, _, like_lse, room, need, lists, marked = kept
     lse = torch.empty_like(like_lse, memory_format=_CONTIGUOUS) if return_lse else None
     stream = kv._on()
     if stream not in marked.seen:
         marked.mark(stream, kv.device, lists)
     work = None if room is None else torch.empty_like(room, memory_format=_CONTIGUOUS)
+    counts = _arrivals(kv, stream, need) if need else None
     args = head + _TREE_AT.pack(q.data_ptr(), res.data_ptr(), _at(lse), lengths.data_ptr(),
-                                _at(token_indptr), _at(parents), _at(work))
+                                _at(token_indptr), _at(parents), _at(work), _at(counts))
     status = _abi.lib().fsp_attention_tree(args, stream)
     if status:
         _abi.check(status, "fsp_attention_tree")

@@ -248,9 +248,11 @@ __global__ __launch_bounds__(256, 3) void attention_paged_kernel(
   const Seen seen(s, last);
   const int first = seen.first;
   const int p0 = first / s.piece, p1 = max(p0 + 1, (last + s.piece - 1) / s.piece);
-  const int mine = pc.begin / s.piece;
+  // under a window with first tokens the list counts from the first piece in use
+  const int skip = s.sinks ? p0 : 0, mine = pc.begin / s.piece + skip;
   if (mine < p0 || mine >= p1) return;
-  const int begin = max(first, pc.begin), n = min(last, pc.begin + s.piece) - begin;
+  const int begin = max(first, mine * s.piece);
+  const int n = (int)min((int64_t)last, ((int64_t)mine + 1) * s.piece) - begin;
 
   V8<T> qf[NS];
   {
@@ -396,7 +398,7 @@ __global__ __launch_bounds__(256, 3) void attention_paged_kernel(
       y += f * *reinterpret_cast<const f32x4*>(&s_o[w][h][d]);
     }
     if (split) {
-      const int64_t at = (int64_t)(pc.slot + mine) * s.heads + head0 + h;
+      const int64_t at = (int64_t)(pc.slot + mine - skip) * s.heads + head0 + h;
       if (arrived) {
         put(part_o + at * c.dim + d, y.x, y.y);
         put(part_o + at * c.dim + d + 2, y.z, y.w);
@@ -430,7 +432,7 @@ __global__ __launch_bounds__(256, 3) void attention_paged_kernel(
   }
   __syncthreads();
   if (s_before != (unsigned)(p1 - p0 - 1)) return;
-  const int64_t at = (int64_t)(pc.slot + p0) * s.heads + head0;  // the first piece's first head
+  const int64_t at = (int64_t)(pc.slot + p0 - skip) * s.heads + head0;  // the first piece's first head
   const int count = p1 - p0;
   constexpr int PER = 256 / (DP / 4);  // heads side by side, each by DP / 4 threads
   for (int h0 = 0; h0 < n_heads; h0 += PER) {
@@ -491,7 +493,7 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(
   const int first = Seen(s, last).first;
   const int p0 = first / s.piece, p1 = max(p0 + 1, (last + s.piece - 1) / s.piece), n = p1 - p0;
   if (n < 2) return;
-  const int64_t at = (int64_t)(slot + p0) * s.heads + h;
+  const int64_t at = (int64_t)(slot + (s.sinks ? 0 : p0)) * s.heads + h;
   const f32x2* ml = part_ml + at;
   const float* o = part_o + at * c.dim + (d < c.dim ? d : 0);
   float most = -INFINITY, total = 0;

@@ -7,6 +7,12 @@ namespace {
 
 constexpr int kDrafts = 256;     // drafted tokens of one sequence, at most
 constexpr int kWideFrom = 64;    // more rows than so many beside a key go to wide tiles
+// The workgroup that finishes a sequence's tile of 16 rows joins its pieces where they are at most so many and the
+// workgroups few; else a second launch does.  By a launch and so, us: 1200 tokens, 16 heads of 64, 8 rows 12.5 /
+// 9.9; 4 sequences of 2000, 8 heads of 128, 16 rows 15.4 / 14.8; with 16 pieces 13.8 / 14.8.  More rows a workgroup
+// take it longer than a launch: 64 rows 20.9 / 23.7, 128 27 / 50.
+constexpr int kJoinMost = 8;
+constexpr int kJoinBlocks = 2048;
 constexpr int kTableKeys = 1024;  // keys whose places LDS holds at a time
 
 struct TreeShape {
@@ -82,6 +88,80 @@ __device__ __forceinline__ int row_mask(const TreeShape& s, const Drafted& t, co
   return depth;
 }
 
+// Bits of 32 keys, from bit x on.
+__device__ __forceinline__ uint32_t bits_from(int x) { return x <= 0 ? ~0u : x > 31 ? 0u : ~0u << x; }
+
+// Which of the 32 keys from place e0 on a row sees, whose first token by its window is ``lo``; ``count`` of them
+// are keys of the piece.
+__device__ __forceinline__ uint32_t seen_keys(const TreeShape& s, const Drafted& t, const uint32_t* mask, int lo,
+                                              int e0, int count) {
+  uint32_t bits = ~0u;
+  const int off = e0 - t.past;
+  if (off > -32) {
+    const uint32_t* m = mask + 1 + (off >> 5);
+    bits = off & 31 ? m[0] >> (off & 31) | m[1] << (32 - (off & 31)) : m[0];
+  }
+  const uint32_t far = ~bits_from(max(s.sinks, t.old) - e0);  // the first tokens that stay visible
+  return bits & (bits_from(lo - e0) | far | bits_from(t.past - e0)) & ~bits_from(count);
+}
+
+// x where bit K is set, else minus infinity; without a condition, which would hold a pair of scalar
+// registers for each element.
+template <int K>
+__device__ __forceinline__ float seen_or_none(uint32_t bits, float x) {
+  const uint32_t m = (uint32_t)((int)(bits << (31 - K)) >> 31);
+  return __uint_as_float((__float_as_uint(x) & m) | (0xff800000u & ~m));
+}
+
+// Whether this workgroup is the last of ``pieces`` to arrive, which joins them; it leaves the count as it was
+// before the call.  What they put is stored by then.
+__device__ __forceinline__ bool last_to_arrive(unsigned* count, int pieces) {
+  __shared__ unsigned s_before;
+  all_stored();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s_before = atomicAdd(count, 1u);
+    if (s_before == (unsigned)(pieces - 1)) atomicExch(count, 0u);
+  }
+  __syncthreads();
+  return s_before == (unsigned)(pieces - 1);
+}
+
+// Joins ``pieces`` of the rows [0, n) of a tile, in their order: row r's sums of a piece start at
+// part_o + (at + r) * dim, those of the next one ``step`` rows on.
+template <typename T, int DP, typename To>
+__device__ __forceinline__ void join_tile(const float* part_o, const float* part_ml, int64_t at, int64_t step,
+                                          int pieces, int n, int dim, const To& to) {
+  constexpr int U = 8, ACROSS = DP / 4;
+  for (int i = threadIdx.x; i < n * ACROSS; i += 256) {
+    const int r = i / ACROSS, d = i % ACROSS * 4;
+    const float* ml = part_ml + 2 * (at + r);
+    const float* o = part_o + (at + r) * dim + (d < dim ? d : 0);
+    float most = -INFINITY, total = 0;
+    f32x4 y{};
+    for (int p = 0; p < pieces; p += U) {  // their loads are under way together
+      f32x2 v[U], a[U], b[U];
+#pragma unroll
+      for (int e = 0; e < U; ++e) {
+        const int64_t k = min(p + e, pieces - 1) * step;
+        v[e] = get(ml + 2 * k);
+        a[e] = get(o + k * dim);
+        b[e] = get(o + k * dim + 2);
+      }
+#pragma unroll
+      for (int e = 0; e < U; ++e) {
+        if (p + e >= pieces) break;
+        const float now = fmaxf(most, v[e].x), base = now == -INFINITY ? 0.0f : now;
+        const float fade = exp2f(most - base), f = exp2f(v[e].x - base);
+        most = now;
+        total = total * fade + f * v[e].y;
+        y = y * fade + f * f32x4{a[e].x, a[e].y, b[e].x, b[e].y};
+      }
+    }
+    if (d < dim) to(r, d, y, most, total);
+  }
+}
+
 // The rows are the drafted tokens' queries of the heads that share a key head, a token's side by side: row r is
 // token r / group, head r % group.  A workgroup takes a piece of a sequence's tokens for one key
 // head and RT * 16 rows, so that what it reads of the cache serves all of them; its four waves take
@@ -93,7 +173,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attention_tree_kernel(
     const T* __restrict__ v_pages, const T* __restrict__ q, int64_t q_token, int64_t q_head,
     T* __restrict__ out, int64_t out_token, int64_t out_head, float* __restrict__ lse,
     const int32_t* __restrict__ lengths, const int32_t* __restrict__ tokens,
-    const int32_t* __restrict__ parents, float* part_o, float* part_ml) {
+    const int32_t* __restrict__ parents, float* part_o, float* part_ml, unsigned* arrived) {
   constexpr int E = DP / 16, NS = DP / 32, W = 4, ROWS = 16 * RT;
   typedef T VE __attribute__((ext_vector_type(E)));
   constexpr int CH = DP / 8, KL = DP / 16;
@@ -235,18 +315,14 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attention_tree_kernel(
 #pragma unroll
       for (int n = 0; n < RT; ++n) {
         if (partial || tail || __any(lo[n] > max(e0, t.old))) {
-          const int off = e0 - t.past, w = off >> 5, shift = off & 31;
-          uint32_t bits = ~0u;
-          if (tail) {
-            const uint32_t* m = s_mask[16 * n + col] + 1 + w;
-            bits = shift ? m[0] >> shift | m[1] << (32 - shift) : m[0];
-          }
+          const uint32_t bits = seen_keys(s, t, s_mask[16 * n + col], lo[n], e0, n_keys - j) >> (4 * quad);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int k = 16 * (e / 4) + 4 * quad + e % 4, at = e0 + k;
-            const bool near = at >= lo[n] || at < s.sinks || at < t.old || at >= t.past;
-            const bool in = (bits >> k & 1) && near && j + k < n_keys;
-            x[n][e / 4][e % 4] = in ? x[n][e / 4][e % 4] : -INFINITY;
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t b = bits >> (16 * u);
+            x[n][u][0] = seen_or_none<0>(b, x[n][u][0]);
+            x[n][u][1] = seen_or_none<1>(b, x[n][u][1]);
+            x[n][u][2] = seen_or_none<2>(b, x[n][u][2]);
+            x[n][u][3] = seen_or_none<3>(b, x[n][u][3]);
           }
         }
         float m = x[n][0][0];
@@ -285,7 +361,16 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attention_tree_kernel(
 
   // join the waves, 16 rows at a time
   const bool split = p1 - p0 > 1;
-  const int64_t slot = (int64_t)(pc.slot + mine - p0) * s.longest * s.heads + (int64_t)g * s.longest * group;
+  const int64_t step = (int64_t)s.longest * s.heads;  // rows of a piece
+  const int64_t slot = (pc.slot + mine - p0) * step + (int64_t)g * s.longest * group;
+  auto to_out = [&](int r, int d, f32x4 y, float most, float total) {
+    const int64_t token = t.begin + (r0 + r) / group;
+    const int head = head0 + (r0 + r) % group;
+    y *= total == 0 ? 0.0f : 1.0f / total;
+    *reinterpret_cast<V4<T>*>(out + token * out_token + head * out_head + d) = __builtin_convertvector(y, V4<T>);
+    if (lse && d == 0)
+      lse[token * s.heads + head] = total == 0 ? -INFINITY : (most + log2f(total * Weights<T>::down)) * kLn2;
+  };
 #pragma unroll
   for (int n = 0; n < RT; ++n) {
     if (r0 + 16 * n >= rows) break;
@@ -315,21 +400,23 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attention_tree_kernel(
         y += f * *reinterpret_cast<const f32x4*>(&s_o[w][row][d]);
       }
       if (masked && s_depth[16 * n + row] < 0) total = __builtin_nanf("");
-      if (split) {
+      if (!split) {
+        to_out(r - r0, d, y, most, total);
+      } else if (RT == 1 && arrived) {
+        put(part_o + (slot + r) * c.dim + d, y.x, y.y);
+        put(part_o + (slot + r) * c.dim + d + 2, y.z, y.w);
+        if (d == 0) put(part_ml + 2 * (slot + r), most, total);
+      } else {
         *reinterpret_cast<f32x4*>(part_o + (slot + r) * c.dim + d) = y;
         if (d == 0) *reinterpret_cast<f32x2*>(part_ml + 2 * (slot + r)) = f32x2{most, total};
-      } else {
-        const int64_t token = t.begin + r / group;
-        const int head = head0 + r % group;
-        y *= total == 0 ? 0.0f : 1.0f / total;
-        *reinterpret_cast<V4<T>*>(out + token * out_token + head * out_head + d) =
-            __builtin_convertvector(y, V4<T>);
-        if (lse && d == 0)
-          lse[token * s.heads + head] =
-              total == 0 ? -INFINITY : (most + log2f(total * Weights<T>::down)) * kLn2;
       }
     }
   }
+  if constexpr (RT > 1) return;
+  if (!split || !arrived) return;  // without counts, another launch joins them
+  if (last_to_arrive(arrived + ((int64_t)b * c.kv_heads + g) * s.tiles + tile, p1 - p0))
+    join_tile<T, DP>(part_o, part_ml, slot - (mine - p0) * step + r0, step, p1 - p0, min(ROWS, rows - r0),
+                     c.dim, to_out);
 }
 
 // Rows past a head's dim are read from here.
@@ -338,7 +425,7 @@ __device__ const i32x4 kZeros = {0, 0, 0, 0};
 // Many rows: 128 of them a workgroup, 32 a wave, over the same 64 keys, which go straight to LDS by the places
 // that a table there holds, the next step's while this one's are worked on: as attention_packed_kernel, whose
 // comments say how the products lie.  The table's two halves of 256 keys are filled in turn.
-template <typename T, int DP>
+template <typename T, int DP, bool EXACT>
 __global__ __launch_bounds__(256, 2) void attention_tree_wide_kernel(
     Cache c, TreeShape s, const Piece* __restrict__ pieces, const T* __restrict__ k_pages,
     const T* __restrict__ v_pages, const T* __restrict__ q, int64_t q_token, int64_t q_head,
@@ -387,16 +474,21 @@ __global__ __launch_bounds__(256, 2) void attention_tree_wide_kernel(
   }
   const float cs = exp2_scale(s.scale);
 
-  // where key 256 * h + threadIdx.x of the piece lies; those past the end stand for the first one
-  auto place = [&](int h, int64_t& k, int64_t& v) {
+  // the page of key 256 * h + threadIdx.x of the piece, and then where that lies; those past the end stand
+  // for the first one
+  auto key_of = [&](int h) {
     const int i = HALF * h + threadIdx.x, e = begin + (i < n ? i : 0);
-    const uint32_t j = e < t.old ? e - t.first : e, at = j / (uint32_t)c.page_size;
-    const int64_t page = c.indices[pc.page + at], slot = j - at * c.page_size;
-    k = page * c.k_page + slot * c.k_slot;
-    v = page * c.v_page + slot * c.v_slot;
+    return (uint32_t)(e < t.old ? e - t.first : e);
+  };
+  auto page_of = [&](int h) { return c.indices[pc.page + key_of(h) / (uint32_t)c.page_size]; };
+  auto place = [&](int h, int64_t page) {
+    const int64_t slot = key_of(h) % (uint32_t)c.page_size;
+    const int at = h % 2 * HALF + threadIdx.x;
+    s_k[at] = page * c.k_page + slot * c.k_slot;
+    s_v[at] = page * c.v_page + slot * c.v_slot;
   };
 #pragma unroll
-  for (int h = 0; h < 2; ++h) place(h, s_k[HALF * h + threadIdx.x], s_v[HALF * h + threadIdx.x]);
+  for (int h = 0; h < 2; ++h) place(h, page_of(h));
   const bool masked = s.window || end > t.past;
   if (masked && parents)
     for (int i = threadIdx.x; i < t.count; i += 256) s_up[i] = parents[t.begin + i];
@@ -407,17 +499,21 @@ __global__ __launch_bounds__(256, 2) void attention_tree_wide_kernel(
   constexpr int PER = kRows * L::PITCH / 1024 / 4, EACH = 1024 / L::PITCH;
   const int l_row = wave * PER * EACH + lane / L::CH;
   const int l_chunk = (lane % L::CH) ^ L::swizzle(lane / L::CH) ^ L::swizzle(wave * PER * EACH);
+  typedef __attribute__((address_space(3))) void lds_void;
+  typedef __attribute__((address_space(1))) void global_void;
   auto load = [&](int step, char* sk, char* sv) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int at = (step * kRows & (2 * HALF - 1)) + l_row + i * EACH;
       const int d = 8 * (l_chunk ^ L::swizzle(i * EACH));
-      const void* kp = d < c.dim ? (const void*)(kb + s_k[at] + d) : (const void*)&kZeros;
-      const void* vp = d < c.dim ? (const void*)(vb + s_v[at] + d) : (const void*)&kZeros;
-      typedef __attribute__((address_space(3))) void lds_void;
-      typedef const __attribute__((address_space(1))) void global_void;
-      __builtin_amdgcn_global_load_lds((global_void*)kp, (lds_void*)(sk + (wave * PER + i) * 1024), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((global_void*)vp, (lds_void*)(sv + (wave * PER + i) * 1024), 16, 0, 0);
+      uint64_t k = (uint64_t)(kb + s_k[at] + d), v = (uint64_t)(vb + s_v[at] + d);
+      if constexpr (!EXACT) {
+        asm volatile("" : "+v"(k), "+v"(v));  // a choice of addresses, not a branch around their reads
+        k = d < c.dim ? k : (uint64_t)&kZeros;
+        v = d < c.dim ? v : (uint64_t)&kZeros;
+      }
+      __builtin_amdgcn_global_load_lds((const global_void*)k, (lds_void*)(sk + (wave * PER + i) * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((const global_void*)v, (lds_void*)(sv + (wave * PER + i) * 1024), 16, 0, 0);
     }
   };
   load(0, s_k0, s_v0);
@@ -450,19 +546,16 @@ __global__ __launch_bounds__(256, 2) void attention_tree_wide_kernel(
     const int j0 = step * kRows, e0 = begin + j0;
     const bool tail = e0 + kRows > t.past;
     if (tail || j0 + kRows > n || __any(lo > max(e0, t.old))) {
-      const int off = e0 - t.past, w = max(off, -64) >> 5, shift = off & 31;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        uint32_t bits = ~0u;
-        if (tail && w + u >= -1) {
-          const uint32_t* m = s_mask[32 * wave + col] + 1 + w + u;
-          bits = shift ? m[0] >> shift | m[1] << (32 - shift) : m[0];
-        }
+        const uint32_t bits = seen_keys(s, t, s_mask[32 * wave + col], lo, e0 + 32 * u, n - j0 - 32 * u) >> (4 * half);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int k = 8 * (r / 4) + r % 4 + 4 * half, at = e0 + 32 * u + k;
-          const bool near = at >= lo || at < s.sinks || at < t.old || at >= t.past;
-          x[u][r] = (bits >> k & 1) && near && j0 + 32 * u + k < n ? x[u][r] : -INFINITY;
+        for (int r = 0; r < 16; r += 4) {
+          const uint32_t b = bits >> (2 * r);
+          x[u][r] = seen_or_none<0>(b, x[u][r]);
+          x[u][r + 1] = seen_or_none<1>(b, x[u][r + 1]);
+          x[u][r + 2] = seen_or_none<2>(b, x[u][r + 2]);
+          x[u][r + 3] = seen_or_none<3>(b, x[u][r + 3]);
         }
       }
     }
@@ -500,15 +593,11 @@ __global__ __launch_bounds__(256, 2) void attention_tree_wide_kernel(
   // one step; the table's other half is filled when the last of its keys have been asked for
   auto pass = [&](int step, char* sk, char* sv, char* next_k, char* next_v) {
     const bool fill = step % 4 == 0 && step > 0 && (step + 4) * kRows < n;
-    int64_t k, v;
-    if (fill) place(step / 4 + 1, k, v);
+    int page = 0;
+    if (fill) page = page_of(step / 4 + 1);
     if (step + 1 < steps) load(step + 1, next_k, next_v);
     work(step, sk, sv);
-    if (fill) {
-      const int at = (step / 4 + 1) % 2 * HALF + threadIdx.x;
-      s_k[at] = k;
-      s_v[at] = v;
-    }
+    if (fill) place(step / 4 + 1, page);
     all_stored();
     __syncthreads();
   };
@@ -525,19 +614,19 @@ __global__ __launch_bounds__(256, 2) void attention_tree_wide_kernel(
 #pragma unroll
     for (int i = 0; i < NT; ++i) o[i] = f32x16{};
   if (masked && s_depth[32 * wave + col] < 0) sum = __builtin_nanf("");
-  if (p1 - p0 > 1) {
-    const int64_t at = (int64_t)(pc.slot + mine - p0) * s.longest * s.heads + (int64_t)g * s.longest * group + row;
-    store_rows<float, NT>(part_o + at * c.dim, o, 1.0f, c.dim, half);
-    if (half == 0)
-      *reinterpret_cast<f32x2*>(part_ml + 2 * at) = f32x2{top == -INFINITY ? -INFINITY : top * cs, sum};
+  if (p1 - p0 == 1) {
+    const int64_t token = t.begin + row / group;
+    const int head = head0 + row % group;
+    if (half == 0 && lse)
+      lse[token * s.heads + head] =
+          sum == 0 ? -INFINITY : (top * cs + log2f(sum * Weights<T>::down)) * kLn2;
+    store_rows<T, NT>(out + token * out_token + head * out_head, o, sum == 0 ? 0.0f : 1.0f / sum, c.dim, half);
     return;
   }
-  const int64_t token = t.begin + row / group;
-  const int head = head0 + row % group;
-  if (half == 0 && lse)
-    lse[token * s.heads + head] =
-        sum == 0 ? -INFINITY : (top * cs + log2f(sum * Weights<T>::down)) * kLn2;
-  store_rows<T, NT>(out + token * out_token + head * out_head, o, sum == 0 ? 0.0f : 1.0f / sum, c.dim, half);
+  const int64_t at = (int64_t)(pc.slot + mine - p0) * s.longest * s.heads + (int64_t)g * s.longest * group + row;
+  store_rows<float, NT>(part_o + at * c.dim, o, 1.0f, c.dim, half);
+  if (half == 0)
+    *reinterpret_cast<f32x2*>(part_ml + 2 * at) = f32x2{top == -INFINITY ? -INFINITY : top * cs, sum};
 }
 
 // Joins the pieces of sequences that have several: half a wave to a row, eight pieces of it at a time.
@@ -603,8 +692,8 @@ int64_t tile_rows(int64_t longest, int64_t group) {
   return rows <= 16 ? 16 : rows <= kWideFrom ? 32 : 128;
 }
 
-template <typename T, typename Kernel>
-int launch_tree(const fsp_attention_tree_args& a, Kernel kernel, hipStream_t st) {
+template <typename T, typename Kernel, typename... More>
+int launch_tree(const fsp_attention_tree_args& a, Kernel kernel, hipStream_t st, More... more) {
   const int64_t group = a.heads / a.cache.kv_heads, each = tile_rows(a.longest, group);
   const int64_t tiles = (a.longest * group + each - 1) / each;
   const TreeShape s{(int)a.heads,    (int)a.window,  (int)a.sinks, (int)a.piece,  (int)a.n_pieces,
@@ -615,9 +704,10 @@ int launch_tree(const fsp_attention_tree_args& a, Kernel kernel, hipStream_t st)
                      cache_of(a.cache), s, reinterpret_cast<const Piece*>(a.pieces),
                      static_cast<const T*>(a.cache.k_pages), static_cast<const T*>(a.cache.v_pages),
                      static_cast<const T*>(a.q), a.q_token, a.q_head, static_cast<T*>(a.out), a.out_token,
-                     a.out_head, a.lse, a.lengths, a.token_indptr, a.parents, part_o, part_ml);
+                     a.out_head, a.lse, a.lengths, a.token_indptr, a.parents, part_o, part_ml,
+                     more...);
   if (int rc = check_hip(hipGetLastError(), "attention_tree_kernel launch")) return rc;
-  if (a.n_pieces == a.cache.batch) return FSP_OK;
+  if (a.n_pieces == a.cache.batch || (a.arrived && each == 16)) return FSP_OK;
   hipLaunchKernelGGL((attention_tree_join_kernel<T>),
                      dim3((unsigned)(a.cache.batch * ((a.longest * a.heads + 7) / 8))), dim3(256), 0, st,
                      cache_of(a.cache), s, a.first_piece, static_cast<T*>(a.out), a.out_token, a.out_head,
@@ -627,9 +717,10 @@ int launch_tree(const fsp_attention_tree_args& a, Kernel kernel, hipStream_t st)
 
 template <typename T, int DP, bool EXACT, bool NT>
 int launch_tree_rows(const fsp_attention_tree_args& a, hipStream_t st) {
+  unsigned* arrived = static_cast<unsigned*>(a.arrived);
   return tile_rows(a.longest, a.heads / a.cache.kv_heads) == 16
-             ? launch_tree<T>(a, attention_tree_kernel<T, DP, EXACT, NT, 1>, st)
-             : launch_tree<T>(a, attention_tree_kernel<T, DP, EXACT, NT, 2>, st);
+             ? launch_tree<T>(a, attention_tree_kernel<T, DP, EXACT, NT, 1>, st, arrived)
+             : launch_tree<T>(a, attention_tree_kernel<T, DP, EXACT, NT, 2>, st, arrived);
 }
 
 template <typename T, int DP, bool EXACT>
@@ -644,9 +735,11 @@ template <typename T>
 int launch_tree_dim(const fsp_attention_tree_args& a, hipStream_t st) {
   const int64_t dim = a.cache.dim;
   if (tile_rows(a.longest, a.heads / a.cache.kv_heads) == 128)
-    return dim <= 64   ? launch_tree<T>(a, attention_tree_wide_kernel<T, 64>, st)
-           : dim <= 96 ? launch_tree<T>(a, attention_tree_wide_kernel<T, 96>, st)
-                       : launch_tree<T>(a, attention_tree_wide_kernel<T, 128>, st);
+    return dim < 64     ? launch_tree<T>(a, attention_tree_wide_kernel<T, 64, false>, st)
+           : dim == 64  ? launch_tree<T>(a, attention_tree_wide_kernel<T, 64, true>, st)
+           : dim <= 96  ? launch_tree<T>(a, attention_tree_wide_kernel<T, 96, false>, st)
+           : dim == 128 ? launch_tree<T>(a, attention_tree_wide_kernel<T, 128, true>, st)
+                        : launch_tree<T>(a, attention_tree_wide_kernel<T, 128, false>, st);
   if (dim == 64) return launch_tree_nt<T, 64, true>(a, st);
   if (dim < 64) return launch_tree_nt<T, 64, false>(a, st);
   if (dim < 128) return launch_tree_nt<T, 128, false>(a, st);
@@ -660,12 +753,15 @@ using namespace fsp;
 
 extern "C" int64_t fsp_attention_tree_drafts(void) { return kDrafts; }
 
-extern "C" int64_t fsp_attention_tree_piece(int64_t tokens, int64_t kv_heads, int64_t group, int64_t longest) {
-  if (tokens < 0 || kv_heads < 1 || group < 1 || longest < 1) return 256;
-  const int64_t rows = tile_rows(longest, group), tiles = (longest * group + rows - 1) / rows;
-  int64_t piece = 256;
-  while (piece < 4096 && tokens / piece * kv_heads * tiles > 1024) piece *= 2;
-  return piece;
+extern "C" int64_t fsp_attention_tree_rows(int64_t group, int64_t longest) {
+  return group < 1 || longest < 1 ? 16 : tile_rows(longest, group);
+}
+
+extern "C" int64_t fsp_attention_tree_counts(int64_t n_pieces, int64_t most, int64_t batch, int64_t kv_heads,
+                                             int64_t group, int64_t longest) {
+  if (batch < 0 || kv_heads < 1 || group < 1 || longest < 1 || n_pieces <= batch || most > kJoinMost) return 0;
+  if (tile_rows(longest, group) != 16) return 0;
+  return n_pieces * kv_heads <= kJoinBlocks ? batch * kv_heads : 0;
 }
 
 extern "C" int64_t fsp_attention_tree_workspace(int64_t n_pieces, int64_t heads, int64_t dim, int64_t longest) {

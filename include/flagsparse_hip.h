@@ -800,7 +800,9 @@ int64_t fsp_attention_paged_piece(int64_t tokens, int64_t kv_heads);
 int64_t fsp_attention_paged_workspace(int64_t n_pieces, int64_t heads, int64_t dim);
 int fsp_attention_paged(const struct fsp_attention_paged_args* args, void* stream);
 /* The same where the sequence's first `sinks` tokens stay visible under a window (sinks > 0: window > 0):
- * key j is seen if j >= lengths[b] - window or j < sinks. */
+ * key j is seen if j >= lengths[b] - window or j < sinks.  A sequence's pieces are counted from the
+ * first one that the window leaves: it may have fewer than its room takes, (window + sinks) / piece + 2 at
+ * least. */
 int fsp_attention_paged_sinks(const struct fsp_attention_paged_args* args, int64_t sinks, void* stream);
 
 /*
@@ -815,10 +817,12 @@ int fsp_attention_paged_sinks(const struct fsp_attention_paged_args* args, int64
  * A row whose way does not lead up, the rows of a sequence with more drafted tokens than `longest`, with a
  * length that its pages cannot hold or less than its drafted tokens, and rows of no sequence are NaN.
  *
- * Pieces as for fsp_attention_paged, of fsp_attention_tree_piece() tokens, but counted from the first piece
+ * Pieces as for fsp_attention_paged, of a multiple of 128 tokens up to 2^20, but counted from the first piece
  * that a window leaves: a sequence may have fewer than its room takes, (longest + window + sinks) /
- * piece + 2 at least.  workspace: fsp_attention_tree_workspace() bytes unless every sequence has
- * one piece.
+ * piece + 2 at least.
+ * For a key head a piece goes to a workgroup for every fsp_attention_tree_rows() of its group * longest
+ * queries.  workspace: fsp_attention_tree_workspace() bytes unless every sequence has one piece, and arrived
+ * as for fsp_attention_paged, fsp_attention_tree_counts() counts, or NULL where that gives none.
  */
 struct fsp_attention_tree_args {
   struct fsp_paged_cache cache;
@@ -835,9 +839,12 @@ struct fsp_attention_tree_args {
   const int32_t* token_indptr;
   const int32_t* parents;
   void* workspace;
+  void* arrived;
 };
 int64_t fsp_attention_tree_drafts(void);
-int64_t fsp_attention_tree_piece(int64_t tokens, int64_t kv_heads, int64_t group, int64_t longest);
+int64_t fsp_attention_tree_counts(int64_t n_pieces, int64_t most, int64_t batch, int64_t kv_heads,
+                                  int64_t group, int64_t longest);
+int64_t fsp_attention_tree_rows(int64_t group, int64_t longest);
 int64_t fsp_attention_tree_workspace(int64_t n_pieces, int64_t heads, int64_t dim, int64_t longest);
 int fsp_attention_tree(const struct fsp_attention_tree_args* args, void* stream);
 

@@ -12,7 +12,7 @@ from tests.test_gpu_tree import _masks, _ways
 
 _TREE_ARGS = dict(pieces=16, first=16, n_pieces=3, piece=256, heads=4, window=0, scale=0.125, sinks=0, tokens=6,
                   longest=3, qt=256, qh=64, ot=256, oh=64, q=64, out=64, lse=0, lengths=16, indptr=16,
-                  parents=16, work=16)
+                  parents=16, work=16, counts=0)
 _KEEP_ARGS = dict(other=0, tokens=6, each=3, n_pieces=3, piece=256, pieces=16, keep=3, indptr=16, lengths=16,
                   kept=16)
 
@@ -28,7 +28,7 @@ def _keep(**kw):
 
 
 def test_struct_sizes():
-    assert attention._TREE.size + attention._TREE_AT.size == 8 * 21
+    assert attention._TREE.size + attention._TREE_AT.size == 8 * 22
     assert attention._KEEP.size + attention._KEEP_AT.size == 8 * 10
     assert _abi.lib().fsp_attention_tree_drafts() == 256
 
@@ -111,13 +111,27 @@ def test_pieces_under_a_window(pages, sight):
     assert at == len(table) and most == max([1] + np.bincount(table[:, 0], minlength=1).tolist())
 
 
-def test_tree_piece_sizes():
+@pytest.mark.parametrize("rooms", [[], [0], [16], [30064] * 8, [2048, 0, 300, 16], [131072, 5], [1] * 900,
+                                   [2**31 - 1024]])
+@pytest.mark.parametrize("sight", [0, 1, 700, 100000])
+def test_sizes_of_pieces(rooms, sight):
+    rooms = np.array(rooms, dtype=np.int64)
+    for each, slots, most, rows in ((1, 512, 8192, 128), (16, 512, 8192, 32), (8, 768, 1024, 16),
+                                    (400, 512, 8192, 128)):
+        piece = attention._piece_of(rooms, sight, each, slots, most, rows)
+        assert 256 <= piece <= most and piece % 128 == 0
+
+
+def test_pieces_fill_whole_rounds():
+    # 8 sequences, 16 workgroups a piece: four even pieces each are one round of 512
+    assert attention._piece_of(np.full(8, 30064), 0, 16, 512, 8192, 128) == 7552
+
+
+def test_rows_of_a_tile():
     L = _abi.lib()
-    for tokens in (0, 1, 1000, 50000, 10**6, 2**31):
-        for heads, group in ((1, 1), (8, 4), (64, 1), (1, 64)):
-            for longest in (1, 8, 64, 256):
-                piece = L.fsp_attention_tree_piece(tokens, heads, group, longest)
-                assert 128 <= piece <= 1 << 20 and piece % 128 == 0
+    assert L.fsp_attention_tree_rows(0, 4) == L.fsp_attention_tree_rows(4, 0) == 16
+    for group, longest in ((1, 1), (4, 4), (4, 8), (23, 26), (1, 256), (64, 256)):
+        assert L.fsp_attention_tree_rows(group, longest) in (16, 32, 128)
 
 
 def test_ways_and_masks_of_the_reference():

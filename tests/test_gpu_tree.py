@@ -301,7 +301,7 @@ def test_graphs_streams_and_equal_bits(dev):
         assert all(torch.equal(a, b) for a, b in zip(eager, got))
     assert all(torch.equal(a, b) for a, b in zip(want, got))
     again = copy.deepcopy(kv)
-    for pieces, firsts, _, _ in kv._lists.values():
+    for _, pieces, _, _, _ in kv._lists.values():
         pieces.zero_()  # the copy works on its own arrays
     assert all(torch.equal(a, b) for a, b in zip(want, step(again)))
 
