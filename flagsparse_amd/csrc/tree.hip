@@ -6,7 +6,10 @@ namespace fsp {
 namespace {
 
 constexpr int kDrafts = 256;     // drafted tokens of one sequence, at most
-constexpr int kWideFrom = 64;    // more rows than so many beside a key go to wide tiles
+// More rows than so many beside a key go to wide tiles.  Tiles of 32 rows / wide ones, us, 8 key heads of 128: 8
+// sequences of 30000, 36 rows 225 / 192, 64 rows 225 / 195; 4 of 2000, 64 rows 20.6 / 19.5; 96 ragged ones of up to
+// 8000, 64 rows 126 / 97; 4 heads of 64, 8 of 30000, 36 rows 68 / 59.
+constexpr int kWideFrom = 32;
 // The workgroup that finishes a sequence's tile of 16 rows joins its pieces where they are at most so many and the
 // workgroups few; else a second launch does.  By a launch and so, us: 1200 tokens, 16 heads of 64, 8 rows 12.5 /
 // 9.9; 4 sequences of 2000, 8 heads of 128, 16 rows 15.4 / 14.8; with 16 pieces 13.8 / 14.8.  More rows a workgroup
@@ -726,7 +729,7 @@ int launch_tree_rows(const fsp_attention_tree_args& a, hipStream_t st) {
 template <typename T, int DP, bool EXACT>
 int launch_tree_nt(const fsp_attention_tree_args& a, hipStream_t st) {
   const int64_t bytes = a.cache.table_len * a.cache.page_size * a.cache.kv_heads * a.cache.dim * 4;
-  return bytes > (256 << 20) && a.longest * a.heads / a.cache.kv_heads <= 32
+  return bytes > (256 << 20)
              ? launch_tree_rows<T, DP, EXACT, true>(a, st)
              : launch_tree_rows<T, DP, EXACT, false>(a, st);
 }
