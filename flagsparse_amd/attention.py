@@ -911,14 +911,16 @@ class PreparedAttention:
     one sequence's rows, those with the most to do first, so that the last ones to finish are
     short."""
 
-    __slots__ = ("batch", "q_tokens", "k_tokens", "device", "_longest", "_tiles", "_sequences",
-                 "_streams", "_calls")
+    __slots__ = ("batch", "q_tokens", "k_tokens", "device", "_longest", "_tiles", "_sequences", "_lengths",
+                 "_grouped", "_streams", "_calls")
 
     def __init__(self, q_len, k_len, device):
         self.batch = len(q_len)
         self.q_tokens = int(q_len.sum())
         self.k_tokens = int(k_len.sum())
         self.device = device
+        self._lengths = (q_len, k_len)
+        self._grouped = {}  # lists of the queries' tiles under first keys, by the heads of a group
         self._longest = tuple(int(n.max(initial=0)) for n in (q_len, k_len))
         # (queries, queries in half tiles, keys, keys in half tiles; causal) -> the list
         names = [(which, causal) for which in range(4) for causal in (False, True)]
@@ -940,6 +942,24 @@ class PreparedAttention:
         if stream not in self._streams.seen:
             self._streams.mark(stream, self.device, self._tiles.values())
         return stream
+
+    def _query_tiles(self, sinks, group):
+        """(tiles, half tiles, streams that they are marked on) of the queries; those under first keys depend on
+        the heads of a group, and are made when first asked for and kept."""
+        if not sinks:
+            return self._tiles[0, True], self._tiles[1, True], self._streams
+        kept = self._grouped.get(group)
+        if kept is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the first call with sinks builds its work list, which cannot be "
+                                   "captured: make one such call before the capture")
+            lists = [_tiles(*self._lengths, int(_abi.lib().fsp_attention_packed_sinks_tile(which, group)),
+                            True, False) for which in (0, 1)]
+            flat = torch.from_numpy(np.concatenate(lists)).to(self.device)
+            torch.cuda.current_stream(self.device).synchronize()  # calls may come from other streams
+            kept = (flat[:len(lists[0])], flat[len(lists[0]):], _Streams())
+            _keep(self._grouped, group, kept)
+        return kept
 
 
 def _tiles(q_len, k_len, tile, causal, keys):
@@ -1025,9 +1045,11 @@ def _packed_inputs(q, k, v, indptr, k_indptr, prepared, causal, window, sinks):
     return prepared, bool(causal), window, sinks
 
 
-def _pack(prepared, q, k, v, causal, window, scale, out, grads=()):
+def _pack(prepared, q, k, v, causal, window, scale, out, grads=(), sinks=0):
     """A call's arguments up to the addresses; grads: grad_out, grad_q, grad_k, grad_v."""
     lists = [prepared._tiles[which, causal] for which in range(4)]
+    if sinks:
+        lists[:2] = prepared._query_tiles(sinks, q.shape[1] // k.shape[1])[:2]
     steps = [n for t in (q, k, v, out, *grads) for n in _steps(t)]
     steps += [0] * (16 - len(steps))
     return _PACKED.pack(_CODES[q.dtype], q.shape[1], k.shape[1], q.shape[2], q.shape[0],
@@ -1053,11 +1075,20 @@ def _refuse_tangents(*tensors):
         raise NotImplementedError("the gradient has no forward-mode derivative")
 
 
+def _first_tiles(prepared, group):
+    """Marks the lists of a call with sinks as used on the current stream."""
+    *lists, marked = prepared._query_tiles(True, group)
+    stream = _abi.raw_stream(prepared.device)
+    if stream not in marked.seen:
+        marked.mark(stream, prepared.device, lists)
+
+
 def _run_forward(prepared, head, sinks, q, k, v, res, lse):
     if q.shape[0]:
         args = head + _PACKED_AT.pack(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), res.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, 0)
         if sinks:
+            _first_tiles(prepared, q.shape[1] // k.shape[1])
             status = _abi.lib().fsp_attention_packed_sinks(args, sinks, prepared._on())
         else:
             status = _abi.lib().fsp_attention_packed(args, prepared._on())
@@ -1068,7 +1099,7 @@ def _run_forward(prepared, head, sinks, q, k, v, res, lse):
 def _forward(prepared, q, k, v, causal, window, sinks, scale, out=None, key=None):
     res, copied = _result(out, "out", q.shape, q.dtype, q.device, q, k, v)
     rows = _rows(q), _rows(k), _rows(v)
-    head = _pack(prepared, *rows, causal, window, scale, res)
+    head = _pack(prepared, *rows, causal, window, scale, res, sinks=sinks)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
     _run_forward(prepared, head, sinks, *rows, res, lse)
     if key is not None and rows[0] is q and rows[1] is k and rows[2] is v:
@@ -1107,7 +1138,8 @@ def flagsparse_attention_packed(q, k, v, indptr=None, k_indptr=None, *, prepared
     by ``indptr`` / ``k_indptr`` (checked by this call, which waits for them) or by ``prepared``
     (prepare_attention_packed).  With ``causal`` query i of nq sees key j of nk if
     j <= i + nk - nq, the last query all of them; ``window``: only the last ``window`` of those, and with
-    ``sinks`` the sequence's first ``sinks`` keys too.
+    ``sinks`` the sequence's first ``sinks`` keys too (the first call with sinks builds a work list and cannot be
+    captured).
     ``scale``: dim ** -0.5 by default.  Returns [tokens, heads, dim], with the float32 log-sum-exp
     [tokens, heads] if ``return_lse``.  The output is differentiable with respect to q, k and v where
     they require a gradient (the log-sum-exp is not); forward-mode tangents raise NotImplementedError.
@@ -1145,7 +1177,7 @@ def _backward(prepared, grad_out, q, k, v, out, lse, causal, window, sinks, scal
     rows = tuple(_rows(t) for t in (grad_out, q, k, v, out))
     flat = lse.contiguous()
     grads = tuple(torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
-    head = _pack(prepared, *rows[1:4], causal, window, scale, rows[4], (rows[0], *grads))
+    head = _pack(prepared, *rows[1:4], causal, window, scale, rows[4], (rows[0], *grads), sinks)
     sizes = (prepared._tiles[2, causal].shape[0], q.shape[1], k.shape[1], q.shape[2], q.shape[0],
              k.shape[0])
     if sinks:
@@ -1173,6 +1205,7 @@ def _run_backward(prepared, kept, rows, lse, grads):
             grad_out.data_ptr(), grads[0].data_ptr(), grads[1].data_ptr(), grads[2].data_ptr(),
             work.data_ptr())
         if sinks:
+            _first_tiles(prepared, q.shape[1] // k.shape[1])
             status = _abi.lib().fsp_attention_packed_sinks_backward(
                 args, sinks, prepared._sequences.data_ptr(), prepared.batch, prepared._on())
         else:

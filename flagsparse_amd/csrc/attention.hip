@@ -12,22 +12,33 @@ struct Tile {
   int first, rows, at, q_begin, nq, k_begin, nk, pad;
 };
 
-// sinks: so many first keys of a sequence stay visible to queries whose window has left them.
+// sinks: so many first keys of a sequence stay visible to queries whose window has left them.  width: so many
+// heads of a group lie side by side in a tile of queries, each token's in turn (1 without sinks).
 struct Shape {
   int heads, kv_heads, dim, causal, window;
   float scale;
-  int sinks;
+  int sinks, width;
 };
 
-// The keys that a tile of queries reads in steps of ROWS: the first ``sinks`` that lie before its window,
-// and what its window holds, [lot, hit).  Step i starts at key at(i); those of the first keys end at ``sinks``.
-template <bool SINKS, int ROWS>
+// The keys that a tile of queries reads in steps: those that its window holds, [lot, hit), and the first ones
+// before them that stay visible, as if these lay right before lot: places [0, end), of which place i is key i
+// below ``sinks`` and key at(i) from there on.
+template <bool SINKS>
 struct Walk {
-  int lot, sinks, skip, end;
+  int lot, sinks, end;
   __device__ Walk(const Shape& s, int lot, int hit)
-      : lot(lot), sinks(SINKS ? min(s.sinks, lot) : 0), skip(SINKS ? (sinks + ROWS - 1) / ROWS * ROWS : 0),
-        end(hit > lot ? hit - lot + skip : 0) {}
-  __device__ int at(int i) const { return SINKS && i < skip ? i : lot + i - skip; }
+      : lot(lot), sinks(SINKS ? min(s.sinks, lot) : 0), end(hit > lot ? hit - lot + sinks : 0) {}
+  __device__ int at(int i) const { return lot - sinks + i; }
+  __device__ bool gap(int i) const { return SINKS && i < sinks && sinks < lot; }  // in a step from i on
+};
+
+// The rows of a tile of queries: row r is token r / width of the tile, of ``width`` heads from a on.
+template <bool SINKS>
+struct Rows {
+  int width;
+  __device__ Rows(const Shape& s) : width(SINKS ? s.width : 1) {}
+  __device__ int token(int r) const { return SINKS ? r / width : r; }
+  __device__ int head(int r) const { return SINKS ? r % width : 0; }
 };
 
 // Workgroups go to the 8 XCDs in turn.  Where the heads divide by them, each XCD has heads of its own, so
@@ -89,6 +100,32 @@ __device__ __forceinline__ void load_rows(char* lds, const void* src, int n, uin
   }
 }
 
+// The same where the first ``sinks`` - i0 of the rows lie at row i0 and the others, up to row n, from row lot on.
+template <int DP, int ROWS, int WAVES>
+__device__ __forceinline__ void load_rows_apart(char* lds, const void* src, int i0, int sinks, int lot, int n,
+                                                uint32_t bytes, int64_t step, int dim, int wave, int lane) {
+  typedef Lay<DP> L;
+  const char* from = static_cast<const char*>(src);
+  const int first = sinks - i0;
+  const __amdgpu_buffer_rsrc_t near = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<char*>(from + i0 * step), 0, (int)((uint32_t)(min(first, ROWS) - 1) * bytes + 2 * dim), 0x00027000);
+  const __amdgpu_buffer_rsrc_t far = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<char*>(from + lot * step), 0, (int)((uint32_t)(min(n - lot, ROWS) - 1) * bytes + 2 * dim),
+      0x00027000);
+  constexpr int PER = ROWS * L::PITCH / 1024 / WAVES, EACH = 1024 / L::PITCH;
+  const int chunk = (lane % L::CH) ^ L::swizzle(lane / L::CH) ^ L::swizzle(wave * PER * EACH);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int at = 16 * (chunk ^ L::swizzle(i * EACH)), r = (wave * PER + i) * EACH + lane / L::CH;
+    const uint32_t off = at < 2 * dim ? (uint32_t)(r < first ? r : r - first) * bytes + at : 0x80000000u;
+    typedef __attribute__((address_space(3))) void lds_void;
+    if (r < first)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(near, (lds_void*)(lds + (wave * PER + i) * 1024), 16, (int)off, 0, 0, 0);
+    else
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(far, (lds_void*)(lds + (wave * PER + i) * 1024), 16, (int)off, 0, 0, 0);
+  }
+}
+
 // out = sum_j w_j v_j / sum_j w_j with w_j = exp2(c q . k_j - m), m a maximum of the row that follows it
 // (Weights).  With S^T = K Q^T a query is a lane: its maximum and sum are its own (and
 // the other half's, 32 lanes on), and its weights are the operand of O^T = V^T P^T where they lie, in
@@ -118,18 +155,21 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_packed_kerne
   constexpr int BYTES = PARTS * L::BYTES, ROWS = PARTS * kRows;
   __shared__ __attribute__((aligned(1024))) char s_k0[BYTES], s_v0[BYTES], s_k1[BYTES], s_v1[BYTES];
   int tile, a;
-  tile_and_head(blockIdx.x, n_tiles, s.heads, tile, a);
+  tile_and_head(blockIdx.x, n_tiles, SINKS ? s.heads / s.width : s.heads, tile, a);
   const Tile t = tiles[tile];
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int g = a / (s.heads / s.kv_heads);
+  const Rows<SINKS> row_of(s);
+  if (SINKS) a *= row_of.width;
+  const int g = a / (s.heads / s.kv_heads), rows = t.rows * row_of.width;
   const int part = wave / BLOCKS, block = wave % BLOCKS, q0 = block * 32;
   const int mine = q0 + col;  // this lane's row of the tile
-  const bool active = q0 < t.rows;
+  const bool active = q0 < rows;
 
   V8<T> qf[NS];
   {
-    const T* qr = q + (t.first + (int64_t)min(mine, t.rows - 1)) * q_token + a * q_head;
+    const int r = min(mine, rows - 1);
+    const T* qr = q + (t.first + (int64_t)row_of.token(r)) * q_token + (a + row_of.head(r)) * q_head;
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
       const int d = 16 * i + 8 * half;
@@ -141,9 +181,9 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_packed_kerne
 
   // the keys that this lane's row sees, and those of the wave's first and last rows
   int lo, hi, lo0, hi0, lo1, hi1, lot, hit, none;
-  seen_by(s, t, t.at + min(mine, t.rows - 1), lo, hi);
-  seen_by(s, t, t.at + min(q0, t.rows - 1), lo0, hi0);
-  seen_by(s, t, t.at + min(q0 + 31, t.rows - 1), lo1, hi1);
+  seen_by(s, t, t.at + row_of.token(min(mine, rows - 1)), lo, hi);
+  seen_by(s, t, t.at + row_of.token(min(q0, rows - 1)), lo0, hi0);
+  seen_by(s, t, t.at + row_of.token(min(q0 + 31, rows - 1)), lo1, hi1);
   seen_by(s, t, t.at, lot, none);
   seen_by(s, t, t.at + t.rows - 1, none, hit);
 
@@ -154,8 +194,16 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_packed_kerne
 
   const T* kb = k + (int64_t)t.k_begin * k_token + g * k_head;
   const T* vb = v + (int64_t)t.k_begin * v_token + g * v_head;
-  auto load = [&](int j0, char* sk, char* sv) {
-    const int n = min(ROWS, t.nk - j0);
+  const Walk<SINKS> keys(s, lot, hit);
+  auto load = [&](int i0, char* sk, char* sv) {
+    if (keys.gap(i0)) {
+      load_rows_apart<DP, ROWS, BLOCKS * PARTS>(sk, kb, i0, keys.sinks, lot, t.nk, (uint32_t)(2 * k_token),
+                                                2 * k_token, s.dim, wave, lane);
+      load_rows_apart<DP, ROWS, BLOCKS * PARTS>(sv, vb, i0, keys.sinks, lot, t.nk, (uint32_t)(2 * v_token),
+                                                2 * v_token, s.dim, wave, lane);
+      return;
+    }
+    const int j0 = keys.at(i0), n = min(ROWS, t.nk - j0);
     load_rows<DP, ROWS, BLOCKS * PARTS>(sk, kb + j0 * k_token, n, (uint32_t)(2 * k_token), s.dim,
                                         wave, lane);
     load_rows<DP, ROWS, BLOCKS * PARTS>(sv, vb + j0 * v_token, n, (uint32_t)(2 * v_token), s.dim,
@@ -164,13 +212,10 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_packed_kerne
   const int k_at = L::row_at(lane);
   const int v_at = L::col_at(lane);
 
-  const Walk<SINKS, ROWS> walk(s, lot, hit);
   auto step = [&](int i0, const char* sk_, const char* sv_) {
-    const int j0 = walk.at(i0) + part * kRows;
-    const bool early = SINKS && i0 < walk.skip;  // keys before the tile's window
-    if (!active || (early ? j0 >= walk.sinks
-                          : j0 >= hi1 || (j0 + kRows <= lo0 && !(SINKS && j0 < s.sinks))))
-      return;
+    i0 += part * kRows;
+    const int j0 = keys.at(i0);  // the first key, or what it would be without the ones before the window
+    if (!active || j0 >= hi1 || (j0 + kRows <= lo0 && !(SINKS && i0 < s.sinks))) return;
     const lds_char* sk = (const lds_char*)sk_ + part * L::BYTES;
     const lds_char* sv = (const lds_char*)sv_ + part * L::BYTES;
     f32x16 x[2];
@@ -183,9 +228,8 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_packed_kerne
       }
     }
     read_ahead<2 * NS, NS>();
-    if (early || j0 + kRows > hi0 || j0 < lo1) {
-      const int first = (early ? 0 : lo) - j0 - 4 * half;
-      const int last = (early ? walk.sinks : hi) - j0 - 4 * half, keep = s.sinks - j0 - 4 * half;
+    if (j0 + kRows > hi0 || j0 < lo1) {
+      const int first = lo - j0 - 4 * half, last = hi - j0 - 4 * half, keep = s.sinks - i0 - 4 * half;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -228,15 +272,15 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_packed_kerne
   };
 
   int i0 = 0;
-  if (i0 < walk.end) load(walk.at(i0), s_k0, s_v0);
+  if (i0 < keys.end) load(i0, s_k0, s_v0);
   __syncthreads();
-  while (i0 < walk.end) {
-    if (i0 + ROWS < walk.end) load(walk.at(i0 + ROWS), s_k1, s_v1);
+  while (i0 < keys.end) {
+    if (i0 + ROWS < keys.end) load(i0 + ROWS, s_k1, s_v1);
     step(i0, s_k0, s_v0);
     __syncthreads();
     i0 += ROWS;
-    if (i0 >= walk.end) break;
-    if (i0 + ROWS < walk.end) load(walk.at(i0 + ROWS), s_k0, s_v0);
+    if (i0 >= keys.end) break;
+    if (i0 + ROWS < keys.end) load(i0 + ROWS, s_k0, s_v0);
     step(i0, s_k1, s_v1);
     __syncthreads();
     i0 += ROWS;
@@ -269,8 +313,9 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_packed_kerne
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[i][r] = o[i][r] * f0 + theirs[(16 * i + r) * 64 + lane] * f1;
   }
-  if (mine >= t.rows) return;
-  const int64_t row = t.first + mine;
+  if (mine >= rows) return;
+  const int64_t row = t.first + row_of.token(mine);
+  a += row_of.head(mine);
   const float inv = sum > 0 ? 1.0f / sum : (sum == 0 ? 0.0f : sum);
   if (half == 0)
     lse[row * s.heads + a] =
@@ -339,14 +384,17 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, DP <= 64 ? 3 : 2) void attenti
   constexpr int BYTES = PARTS * L::BYTES, ROWS = PARTS * kRows;
   __shared__ __attribute__((aligned(1024))) char s_k0[BYTES], s_v0[BYTES], s_k1[BYTES], s_v1[BYTES];
   int tile, a;
-  tile_and_head(blockIdx.x, n_tiles, s.heads, tile, a);
+  tile_and_head(blockIdx.x, n_tiles, SINKS ? s.heads / s.width : s.heads, tile, a);
   const Tile t = tiles[tile];
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int g = a / (s.heads / s.kv_heads);
+  const Rows<SINKS> row_of(s);
+  if (SINKS) a *= row_of.width;
+  const int g = a / (s.heads / s.kv_heads), rows = t.rows * row_of.width;
   const int part = wave / BLOCKS, block = wave % BLOCKS, q0 = block * 32, mine = q0 + col;
-  const bool active = q0 < t.rows;
-  const int64_t row = t.first + (int64_t)min(mine, t.rows - 1);
+  const bool active = q0 < rows;
+  const int64_t row = t.first + (int64_t)row_of.token(min(mine, rows - 1));
+  a += row_of.head(min(mine, rows - 1));
 
   V8<T> qf[NS], gf[NS];
   float delta = 0;
@@ -367,9 +415,9 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, DP <= 64 ? 3 : 2) void attenti
   base = base == -INFINITY ? INFINITY : base * kLog2e;
 
   int lo, hi, lo0, hi0, lo1, hi1, lot, hit, none;
-  seen_by(s, t, t.at + min(mine, t.rows - 1), lo, hi);
-  seen_by(s, t, t.at + min(q0, t.rows - 1), lo0, hi0);
-  seen_by(s, t, t.at + min(q0 + 31, t.rows - 1), lo1, hi1);
+  seen_by(s, t, t.at + row_of.token(min(mine, rows - 1)), lo, hi);
+  seen_by(s, t, t.at + row_of.token(min(q0, rows - 1)), lo0, hi0);
+  seen_by(s, t, t.at + row_of.token(min(q0 + 31, rows - 1)), lo1, hi1);
   seen_by(s, t, t.at, lot, none);
   seen_by(s, t, t.at + t.rows - 1, none, hit);
 
@@ -379,8 +427,16 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, DP <= 64 ? 3 : 2) void attenti
 
   const T* kb = k + (int64_t)t.k_begin * k_token + g * k_head;
   const T* vb = v + (int64_t)t.k_begin * v_token + g * v_head;
-  auto load = [&](int j0, char* sk, char* sv) {
-    const int n = min(ROWS, t.nk - j0);
+  const Walk<SINKS> keys(s, lot, hit);
+  auto load = [&](int i0, char* sk, char* sv) {
+    if (keys.gap(i0)) {
+      load_rows_apart<DP, ROWS, BLOCKS * PARTS>(sk, kb, i0, keys.sinks, lot, t.nk, (uint32_t)(2 * k_token),
+                                                2 * k_token, s.dim, wave, lane);
+      load_rows_apart<DP, ROWS, BLOCKS * PARTS>(sv, vb, i0, keys.sinks, lot, t.nk, (uint32_t)(2 * v_token),
+                                                2 * v_token, s.dim, wave, lane);
+      return;
+    }
+    const int j0 = keys.at(i0), n = min(ROWS, t.nk - j0);
     load_rows<DP, ROWS, BLOCKS * PARTS>(sk, kb + j0 * k_token, n, (uint32_t)(2 * k_token), s.dim,
                                         wave, lane);
     load_rows<DP, ROWS, BLOCKS * PARTS>(sv, vb + j0 * v_token, n, (uint32_t)(2 * v_token), s.dim,
@@ -399,15 +455,15 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, DP <= 64 ? 3 : 2) void attenti
       y = mfma32(row_frag<T>(sv + (r_at ^ (i * 32)) + u * 32 * L::PITCH), gf[i], y);
     }
   };
-  const Walk<SINKS, ROWS> keys(s, lot, hit);
-  // whether any of the wave's rows sees any of n keys from j0 on
-  auto unseen = [&](int j0, int n, bool early) {
-    return early ? j0 >= keys.sinks : j0 >= hi1 || (j0 + n <= lo0 && !(SINKS && j0 < s.sinks));
+  // whether none of the wave's rows sees any of n keys from place i0 on
+  auto unseen = [&](int i0, int n) {
+    const int j0 = keys.at(i0);
+    return j0 >= hi1 || (j0 + n <= lo0 && !(SINKS && i0 < s.sinks));
   };
-  auto hide = [&](int j0, int u, bool early, f32x16& x) {
-    if (early || j0 + kRows > hi0 || j0 < lo1) {
-      const int first = (early ? 0 : lo) - j0 - 4 * half;
-      const int last = (early ? keys.sinks : hi) - j0 - 4 * half, keep = s.sinks - j0 - 4 * half;
+  auto hide = [&](int i0, int u, f32x16& x) {
+    const int j0 = keys.at(i0);
+    if (j0 + kRows > hi0 || j0 < lo1) {
+      const int first = lo - j0 - 4 * half, last = hi - j0 - 4 * half, keep = s.sinks - i0 - 4 * half;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int j = 32 * u + 8 * (r / 4) + r % 4;
@@ -417,21 +473,20 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, DP <= 64 ? 3 : 2) void attenti
   };
   auto walk = [&](auto&& step) {
     auto wave_step = [&](int i0, const char* sk, const char* sv) {
-      const int j0 = keys.at(i0) + part * kRows;
-      const bool early = SINKS && i0 < keys.skip;  // keys before the tile's window
-      if (!active || unseen(j0, kRows, early)) return;
-      step(j0, early, (const lds_char*)sk + part * L::BYTES, (const lds_char*)sv + part * L::BYTES);
+      i0 += part * kRows;
+      if (!active || unseen(i0, kRows)) return;
+      step(i0, (const lds_char*)sk + part * L::BYTES, (const lds_char*)sv + part * L::BYTES);
     };
     int i0 = 0;
-    if (i0 < keys.end) load(keys.at(i0), s_k0, s_v0);
+    if (i0 < keys.end) load(i0, s_k0, s_v0);
     __syncthreads();
     while (i0 < keys.end) {
-      if (i0 + ROWS < keys.end) load(keys.at(i0 + ROWS), s_k1, s_v1);
+      if (i0 + ROWS < keys.end) load(i0 + ROWS, s_k1, s_v1);
       wave_step(i0, s_k0, s_v0);
       __syncthreads();
       i0 += ROWS;
       if (i0 >= keys.end) break;
-      if (i0 + ROWS < keys.end) load(keys.at(i0 + ROWS), s_k0, s_v0);
+      if (i0 + ROWS < keys.end) load(i0 + ROWS, s_k0, s_v0);
       wave_step(i0, s_k1, s_v1);
       __syncthreads();
       i0 += ROWS;
@@ -440,16 +495,16 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, DP <= 64 ? 3 : 2) void attenti
 
   // An output of few keys is large, and so is what its rounding does to delta = grad_out . out: there
   // delta is made anew, as the sum of the weights times dP.
-  if (hit - lot + keys.sinks <= kFewKeys) {
+  if (keys.end <= kFewKeys) {
     delta = 0;
-    walk([&](int j0, bool early, const lds_char* sk, const lds_char* sv) {
+    walk([&](int i0, const lds_char* sk, const lds_char* sv) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         f32x16 x, y;
         products(sk, sv, u, x, y);
 #pragma unroll
         for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], c, -base)) * y[r];
-        hide(j0, u, early, x);
+        hide(i0, u, x);
 #pragma unroll
         for (int r = 0; r < 16; ++r) delta += x[r];
       }
@@ -463,7 +518,7 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, DP <= 64 ? 3 : 2) void attenti
     }
   }
   // what the keys' gradients start their products from: see there
-  if (part == 0 && half == 0 && mine < t.rows) {
+  if (part == 0 && half == 0 && mine < rows) {
     stats[a * q_tokens + row] = (Lift<T>::up - base) / c;
     stats[(s.heads + a) * q_tokens + row] = -delta;
   }
@@ -471,16 +526,16 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, DP <= 64 ? 3 : 2) void attenti
   constexpr bool RAISED = std::is_same<T, f16>::value;
   int n = RAISED ? kRaise : 0;
   base -= n;
-  walk([&](int j0, bool early, const lds_char* sk, const lds_char* sv) {
+  walk([&](int i0, const lds_char* sk, const lds_char* sv) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      if (unseen(j0 + 32 * u, 32, early)) continue;
+      if (unseen(i0 + 32 * u, 32)) continue;
       f32x16 x, y;
       products(sk, sv, u, x, y);
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], c, -base)) * (y[r] - delta);
-      hide(j0, u, early, x);
+      hide(i0, u, x);
       if constexpr (RAISED) {
         const int by = lower(x, acc);
         base += by;
@@ -516,7 +571,7 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, DP <= 64 ? 3 : 2) void attenti
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][r] += theirs[(16 * i + r) * 64 + lane];
   }
-  if (mine < t.rows)
+  if (mine < rows)
     store_rows<T, NT>(dq + row * dq_token + a * dq_head, acc, s.scale, s.dim, half);
 }
 
@@ -843,15 +898,27 @@ __global__ __launch_bounds__(256) void attention_grad_sinks_sum_kernel(
 template <typename T>
 const T* in(const void* p) { return static_cast<const T*>(p); }
 
+// Under a window with first keys a tile of queries is of several heads of a group, the largest divisor of its
+// size up to 32: its rows see nearly the same keys, where as many queries of one head see as many more.
+// TIMES
+int heads_beside(int64_t group) {
+  int width = 1;
+  for (int i = 2; i <= 32; ++i)
+    if (group % i == 0) width = i;
+  return width;
+}
+
 // A call's arguments, with its first keys and, for a backward pass, the sequences.
 struct Call : fsp_attention_packed_args {
   int64_t sinks = 0, batch = 0;
   const int32_t* sequences = nullptr;
+  int width() const { return sinks ? heads_beside(heads / kv_heads) : 1; }
+  int64_t query_tiles() const { return n_q_tiles * heads / width(); }  // workgroups
 };
 
 Shape shape_of(const Call& a) {
   return {(int)a.heads, (int)a.kv_heads, (int)a.dim, a.causal != 0, (int)a.window, (float)a.scale,
-          (int)a.sinks};
+          (int)a.sinks, a.width()};
 }
 
 // Twice as many waves share a tile where that fills CUs, or shortens the chains that the others end up
@@ -870,7 +937,7 @@ int64_t seen_at_most(const Call& a, int64_t longest) {
 }
 
 bool share_queries(const Call& a, int64_t fill) {
-  const int64_t n = a.n_q_tiles * a.heads;
+  const int64_t n = a.query_tiles();
   return seen_at_most(a, a.k_longest) >= 512 &&
          (n <= fill || (n <= 2 * kCus && a.causal && !a.window && a.k_longest >= 2048));
 }
@@ -882,7 +949,7 @@ bool share_queries(const Call& a, int64_t fill) {
 // to a CU: 2048, 8 heads (128) 22.4 / 18.5, 4000 (256) 39.6 / 35.4.  Gradient of the queries, dim 128:
 // 512 (64) 20.4 / 15.9, 2048 (64) 44.8 / 38.6, 4000 (256) 82 / 86; dim 64: 2048 (128) 28.9 / 25.3.
 bool halve_tiles(const Call& a, int64_t most) {
-  return a.n_q_tiles * a.heads <= most && seen_at_most(a, a.k_longest) > kRows;
+  return a.query_tiles() <= most && seen_at_most(a, a.k_longest) > kRows;
 }
 
 bool share_keys(const Call& a, int split) {
@@ -922,7 +989,7 @@ int launch_forward(const Call& a, hipStream_t st) {
   const int32_t* tiles = BLOCKS == 2 ? a.q_halves : a.q_tiles;
   const int64_t n = BLOCKS == 2 ? a.n_q_halves : a.n_q_tiles;
   hipLaunchKernelGGL((attention_packed_kernel<T, DP, BLOCKS, PARTS, SINKS>),
-                     dim3((unsigned)(n * a.heads)), dim3(64 * BLOCKS * PARTS), 0, st, shape_of(a),
+                     dim3((unsigned)(n * a.heads / a.width())), dim3(64 * BLOCKS * PARTS), 0, st, shape_of(a),
                      reinterpret_cast<const Tile*>(tiles), (int)n, in<T>(a.q),
                      a.q_token, a.q_head, in<T>(a.k), a.k_token, a.k_head, in<T>(a.v), a.v_token,
                      a.v_head, static_cast<T*>(a.out), a.out_token, a.out_head, a.lse);
@@ -948,7 +1015,7 @@ int launch_grad_q(const Call& a, hipStream_t st) {
   const int32_t* tiles = BLOCKS == 2 ? a.q_halves : a.q_tiles;
   const int64_t n = BLOCKS == 2 ? a.n_q_halves : a.n_q_tiles;
   hipLaunchKernelGGL((attention_grad_q_kernel<T, DP, BLOCKS, PARTS, SINKS>),
-                     dim3((unsigned)(n * a.heads)), dim3(64 * BLOCKS * PARTS), 0, st, shape_of(a),
+                     dim3((unsigned)(n * a.heads / a.width())), dim3(64 * BLOCKS * PARTS), 0, st, shape_of(a),
                      reinterpret_cast<const Tile*>(tiles), (int)n, in<T>(a.q),
                      a.q_token, a.q_head, in<T>(a.k), a.k_token, a.k_head, in<T>(a.v), a.v_token,
                      a.v_head, in<T>(a.out), a.out_token, a.out_head, a.lse, in<T>(a.grad_out),
@@ -1155,6 +1222,10 @@ extern "C" int fsp_attention_packed(const fsp_attention_packed_args* args, void*
 extern "C" int fsp_attention_packed_backward(const fsp_attention_packed_args* args, void* stream) {
   if (!args) return set_error(FSP_EINVAL, "fsp_attention_packed_backward: null arguments");
   return run_backward({*args}, "fsp_attention_packed_backward", stream);
+}
+
+extern "C" int64_t fsp_attention_packed_sinks_tile(int which, int64_t group) {
+  return group < 1 ? 1 : (which == 0 ? kTile : kTile / 2) / heads_beside(group);
 }
 
 extern "C" int fsp_attention_packed_sinks(const fsp_attention_packed_args* args, int64_t sinks,

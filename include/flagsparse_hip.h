@@ -897,10 +897,12 @@ int fsp_attention_packed(const struct fsp_attention_packed_args* args, void* str
 int fsp_attention_packed_backward(const struct fsp_attention_packed_args* args, void* stream);
 /*
  * The same where each sequence's first `sinks` keys stay visible under a window (sinks > 0: window > 0):
- * a window hides the keys sinks <= j <= i + nk - nq - window.  The backward pass takes the sequences
+ * a window hides the keys sinks <= j <= i + nk - nq - window.  q_tiles and q_halves cover the queries in
+ * fsp_attention_packed_sinks_tile(0 and 1, heads / kv_heads) rows.  The backward pass takes the sequences
  * as tiles, [batch, 8] int32 {0, 0, 0, q begin, q count, k begin, k count, 0} in their order,
  * and a workspace of fsp_attention_packed_sinks_workspace() bytes.
  */
+int64_t fsp_attention_packed_sinks_tile(int which, int64_t group);
 int fsp_attention_packed_sinks(const struct fsp_attention_packed_args* args, int64_t sinks, void* stream);
 int fsp_attention_packed_sinks_backward(const struct fsp_attention_packed_args* args, int64_t sinks,
                                         const int32_t* sequences, int64_t batch, void* stream);
