@@ -866,12 +866,36 @@ __global__ __launch_bounds__(256) void attention_grad_kv_sum_kernel(
   *reinterpret_cast<V4<T>*>(to) = __builtin_convertvector(y, V4<T>);
 }
 
-// The first keys' and their values' gradients as the sums of their jobs, chunk by chunk and in each the shares
-// of the heads: a thread to four elements, a workgroup's of one sequence and key head.
+// The same for tiles of first keys, as the sums of their jobs, chunk by chunk and in each the shares of the
+// heads, by workgroups of their own, [0, of_jobs): a thread to four elements, a workgroup's of one sequence
+// and key head.  The others add the shares of all other keys.
 template <typename T, int ROWS>
 __global__ __launch_bounds__(256) void attention_grad_sinks_sum_kernel(
-    Shape s, int split, Jobs jobs, T* __restrict__ dk, int64_t dk_token, int64_t dk_head,
-    T* __restrict__ dv, int64_t dv_token, int64_t dv_head) {
+    Shape s, int split, Jobs jobs, int of_jobs, const float* __restrict__ sums, int64_t k_tokens,
+    T* __restrict__ dk, int64_t dk_token, int64_t dk_head, T* __restrict__ dv, int64_t dv_token,
+    int64_t dv_head) {
+  if ((int)blockIdx.x >= of_jobs) {
+    const int64_t each = (int64_t)s.kv_heads * k_tokens * s.dim;
+    const int64_t i = ((int64_t)(blockIdx.x - of_jobs) * 256 + threadIdx.x) * 4;
+    if (i >= 2 * each) return;
+    const bool keys = i >= each;
+    const int64_t at = keys ? i - each : i;
+    const int64_t row = at / s.dim, g = row / k_tokens, t = row - g * k_tokens;
+    int b = 0;  // the last sequence that starts at or before t
+    for (int end = jobs.batch; end - b > 1;) {
+      const int mid = (b + end) / 2;
+      if (jobs.sequences[mid].k_begin <= t) b = mid;
+      else end = mid;
+    }
+    const Tile q = jobs.sequences[b];
+    if ((t - q.k_begin) / ROWS * ROWS < s.sinks) return;
+    const float* from = sums + (keys ? split * each : 0) + at;
+    f32x4 y = *reinterpret_cast<const f32x4*>(from);
+    for (int p = 1; p < split; ++p) y += *reinterpret_cast<const f32x4*>(from + p * each);
+    T* to = (keys ? dk + t * dk_token + g * dk_head : dv + t * dv_token + g * dv_head) + at % s.dim;
+    *reinterpret_cast<V4<T>*>(to) = __builtin_convertvector(y, V4<T>);
+    return;
+  }
   const int quads = s.dim / 4, per = 2 * jobs.tiles * ROWS * quads, blocks = (per + 255) / 256;
   const int i = (blockIdx.x % blocks) * 256 + threadIdx.x;
   const int g = blockIdx.x / blocks % s.kv_heads, b = blockIdx.x / blocks / s.kv_heads;
@@ -881,7 +905,7 @@ __global__ __launch_bounds__(256) void attention_grad_sinks_sum_kernel(
   const bool keys = of >= jobs.tiles * ROWS;
   const int row = keys ? of - jobs.tiles * ROWS : of;
   // the rows of the tiles that have a first key
-  if (row >= t.nk || row / ROWS * ROWS >= min(t.nk, s.sinks)) return;
+  if (row >= t.nk || row / ROWS * ROWS >= s.sinks) return;
   int lot, hit;
   seen_of(s, t, row / ROWS * ROWS, lot, hit);
   f32x4 y{};
@@ -1069,23 +1093,21 @@ int launch_grad_kv(const Call& a, int split, hipStream_t st) {
                      static_cast<T*>(a.grad_v), a.grad_v_token, a.grad_v_head, split, sums,
                      a.k_tokens, jobs);
   if (int rc = check_hip(hipGetLastError(), "attention_grad_kv_kernel launch")) return rc;
-  if (split > 1) {
-    const int64_t quads = a.kv_heads * a.k_tokens * a.dim / 2;
-    hipLaunchKernelGGL((attention_grad_kv_sum_kernel<T>), dim3((unsigned)((quads + 255) / 256)),
-                       dim3(256), 0, st, shape_of(a), split, sums, a.k_tokens,
-                       static_cast<T*>(a.grad_k), a.grad_k_token, a.grad_k_head,
-                       static_cast<T*>(a.grad_v), a.grad_v_token, a.grad_v_head);
-    if (int rc = check_hip(hipGetLastError(), "attention_grad_kv_sum_kernel launch")) return rc;
-  }
-  if constexpr (SINKS) {  // after it: it has written over the first keys' gradients
-    const int64_t blocks = (2 * jobs.tiles * 32 * BLOCKS * (a.dim / 4) + 255) / 256;
+  const int64_t quads = split > 1 ? a.kv_heads * a.k_tokens * a.dim / 2 : 0;
+  if constexpr (SINKS) {
+    const int64_t of_jobs = (2 * jobs.tiles * 32 * BLOCKS * (a.dim / 4) + 255) / 256 * a.kv_heads * a.batch;
     hipLaunchKernelGGL((attention_grad_sinks_sum_kernel<T, 32 * BLOCKS>),
-                       dim3((unsigned)(blocks * a.kv_heads * a.batch)), dim3(256), 0, st, shape_of(a),
-                       split, jobs, static_cast<T*>(a.grad_k), a.grad_k_token, a.grad_k_head,
-                       static_cast<T*>(a.grad_v), a.grad_v_token, a.grad_v_head);
+                       dim3((unsigned)(of_jobs + (quads + 255) / 256)), dim3(256), 0, st, shape_of(a), split,
+                       jobs, (int)of_jobs, sums, a.k_tokens, static_cast<T*>(a.grad_k), a.grad_k_token,
+                       a.grad_k_head, static_cast<T*>(a.grad_v), a.grad_v_token, a.grad_v_head);
     return check_hip(hipGetLastError(), "attention_grad_sinks_sum_kernel launch");
   }
-  return FSP_OK;
+  if (split == 1) return FSP_OK;
+  hipLaunchKernelGGL((attention_grad_kv_sum_kernel<T>), dim3((unsigned)((quads + 255) / 256)),
+                     dim3(256), 0, st, shape_of(a), split, sums, a.k_tokens,
+                     static_cast<T*>(a.grad_k), a.grad_k_token, a.grad_k_head,
+                     static_cast<T*>(a.grad_v), a.grad_v_token, a.grad_v_head);
+  return check_hip(hipGetLastError(), "attention_grad_kv_sum_kernel launch");
 }
 
 template <typename T, int DP, bool SINKS>
@@ -1203,7 +1225,7 @@ int run_backward(const Call& a, const std::string& who, void* stream) {
     const int64_t tiles = (first_keys(a.sinks, a.k_longest) + kRows / 2 - 1) / (kRows / 2);
     const int64_t all = kMaxBlocks / a.heads - a.n_k_halves - 8;
     if (a.batch > kMaxBlocks || (tiles > 0 && job_slots(a.q_tokens, a.batch, a.window) > all / tiles) ||
-        a.batch > kMaxBlocks / a.kv_heads / (tiles * (kRows / 2) * (a.dim / 4) / 128 + 1))
+        a.batch > kMaxBlocks / 2 / a.kv_heads / (tiles * (kRows / 2) * (a.dim / 4) / 128 + 1))
       return set_error(FSP_EINVAL, who + ": sinks of so many sequences");
   }
   hipStream_t st = static_cast<hipStream_t>(stream);

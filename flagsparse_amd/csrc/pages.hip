@@ -104,34 +104,33 @@ __global__ __launch_bounds__(kThreads) void paged_keep_kernel(
   if (which == 0 && threadIdx.x == 0) kept[b] = m.ok ? m.past + stay : -1;
 }
 
-// Into other pages: a workgroup takes a piece of a sequence's tokens, one key head and its keys or values.
-// How many tokens stay before the piece, and of all, it counts itself, four marks to a word.
+// Into other pages: a workgroup takes kSpan of a sequence's tokens, all heads of their keys and values.  How many
+// tokens stay before them, and of all, it counts itself, four marks to a word.
+constexpr int kSpan = kWave;
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void paged_keep_into_kernel(
-    Cache c, KeepShape s, const Piece* __restrict__ pieces, int piece_size, int n_pieces,
-    const T* __restrict__ k_pages, const T* __restrict__ v_pages, T* __restrict__ to_k,
-    T* __restrict__ to_v, const uint8_t* __restrict__ keep, const int32_t* __restrict__ tokens,
+    Cache c, KeepShape s, const Piece* __restrict__ pieces, int piece_size, const T* __restrict__ k_pages,
+    const T* __restrict__ v_pages, T* __restrict__ to_k, T* __restrict__ to_v,
+    const uint8_t* __restrict__ keep, const int32_t* __restrict__ tokens,
     const int32_t* __restrict__ lengths, int32_t* __restrict__ kept) {
   constexpr int U = 8;
-  __shared__ int s_list[kList];
-  __shared__ int s_before[4], s_all[4];
-  int piece, which;
-  piece_and_head(blockIdx.x, n_pieces, 2 * c.kv_heads, piece, which);
-  const Piece pc = pieces[piece];
-  const int b = pc.seq;
-  const bool values = which >= c.kv_heads;
-  const int g = values ? which - c.kv_heads : which;
+  __shared__ int64_t s_from[2][kSpan], s_to[2][kSpan];  // where keys and values lie, and go
+  __shared__ int s_before[4], s_all[4], s_n;
+  const int parts = piece_size / kSpan;
+  const Piece pc = pieces[blockIdx.x / parts];
+  const int b = pc.seq, at = pc.begin + (int)(blockIdx.x % parts) * kSpan;
   const Marked m(tokens, s.each, s.n_tokens, b, lengths[b], pc.room);
-  const int length = m.past + m.count, end = min(length, pc.begin + piece_size);
-  if (pc.begin >= length && pc.begin > 0) return;
+  const int length = m.past + m.count;
+  if (at >= length && at > 0) return;
 
   const uint8_t* marks = keep + m.begin;
   int before = 0, all = 0;
   {
     // whole words of the array that the marks lie in, those of others masked
-    const uintptr_t at = reinterpret_cast<uintptr_t>(marks);
-    const uint32_t* words = reinterpret_cast<const uint32_t*>(at & ~uintptr_t(3));
-    const int skip = (int)(at & 3), stop = pc.begin - m.past;
+    const uintptr_t from = reinterpret_cast<uintptr_t>(marks);
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(from & ~uintptr_t(3));
+    const int skip = (int)(from & 3), stop = at - m.past;
     for (int64_t i = threadIdx.x; 4 * i < (int64_t)m.count + skip; i += kThreads) {
       const int t = (int)(4 * i) - skip;
       uint32_t w;
@@ -164,52 +163,48 @@ __global__ __launch_bounds__(kThreads) void paged_keep_into_kernel(
     all = s_all[0] + s_all[1] + s_all[2] + s_all[3];
   }
   const int first = s.indptr[b];
-  const bool ok = m.ok && m.past + all <= (int64_t)(s.indptr[b + 1] - first) * s.page_size;
-  if (pc.begin == 0 && which == 0 && threadIdx.x == 0) kept[b] = ok ? m.past + all : -1;
+  const bool ok = m.ok && m.past + (int64_t)all <= (int64_t)(s.indptr[b + 1] - first) * s.page_size;
+  if (at == 0 && threadIdx.x == 0) kept[b] = ok ? m.past + all : -1;
   if (!ok) return;
 
-  const T* from = values ? v_pages + g * c.v_head : k_pages + g * c.k_head;
-  T* to = values ? to_v + g * s.v_head : to_k + g * s.k_head;
-  const int64_t from_page = values ? c.v_page : c.k_page, from_slot = values ? c.v_slot : c.k_slot;
-  const int64_t to_page = values ? s.v_page : s.k_page, to_slot = values ? s.v_slot : s.k_slot;
-  const int chunks = c.dim / 8, rows = kThreads / chunks;
-  const int row = threadIdx.x / chunks, d = threadIdx.x % chunks * 8;
-  if (pc.begin < m.past) {  // tokens before the marked ones stay where they are in the text
-    before = pc.begin;
-  } else {
-    before += m.past;
+  if (threadIdx.x < kWave) {
+    const int pos = at + threadIdx.x;
+    const bool stays = pos < length && (pos < m.past || marks[pos - m.past]);
+    const uint64_t votes = __ballot(stays);
+    if (stays) {
+      const int n = __popcll(votes & ((1ull << threadIdx.x) - 1));
+      const uint32_t to = min(at, m.past) + before + n;  // the tokens before the marked ones all stay
+      const uint32_t p = (uint32_t)pos / (uint32_t)c.page_size, q = to / (uint32_t)s.page_size;
+      const int64_t page = c.indices[pc.page + p], slot = (uint32_t)pos - p * c.page_size;
+      const int64_t to_page = s.indices[first + q], to_slot = to - q * s.page_size;
+      s_from[0][n] = page * c.k_page + slot * c.k_slot;
+      s_from[1][n] = page * c.v_page + slot * c.v_slot;
+      s_to[0][n] = to_page * s.k_page + to_slot * s.k_slot;
+      s_to[1][n] = to_page * s.v_page + to_slot * s.v_slot;
+    }
+    if (threadIdx.x == 0) s_n = __popcll(votes);
   }
-  for (int at = pc.begin; at < end; at += kList) {
-    // the piece's tokens that stay, by their distance from at
-    const int whole = max(0, min(m.past, end) - at), upto = min(end, at + kList);
-    int n = min(whole, kList);
-    if (at + kList > m.past && upto > m.past) {
-      const int from_mark = max(at, m.past) - m.past;
-      n += list_kept(marks, from_mark, upto - m.past, s_list + n);
-    } else {
-      __syncthreads();
-    }
-    for (int i = 0; i < n; i += rows * U) {
+  __syncthreads();
+  const uint32_t chunks = c.dim / 8, line = chunks * c.kv_heads, items = s_n * line;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const T* from = which ? v_pages : k_pages;
+    T* to = which ? to_v : to_k;
+    const int64_t from_head = which ? c.v_head : c.k_head, to_head = which ? s.v_head : s.k_head;
+    for (uint32_t i = threadIdx.x; i < items; i += U * kThreads) {
       i32x4 x[U];
+      int64_t off[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int r = min(i + u * rows + row, n - 1);
-        const uint32_t pos = r < whole ? at + r : m.past + s_list[r], p = pos / (uint32_t)c.page_size;
-        x[u] = *reinterpret_cast<const i32x4*>(from + c.indices[pc.page + p] * from_page +
-                                               (pos - p * c.page_size) * from_slot + d);
+        const uint32_t j = min(i + u * kThreads, items - 1), n = j / line, r = j - n * line, h = r / chunks;
+        const int d = (r - h * chunks) * 8;
+        x[u] = *reinterpret_cast<const i32x4*>(from + s_from[which][n] + h * from_head + d);
+        off[u] = s_to[which][n] + h * to_head + d;
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int r = i + u * rows + row;
-        if (row < rows && r < n) {
-          const uint32_t pos = before + r, p = pos / (uint32_t)s.page_size;
-          *reinterpret_cast<i32x4*>(to + s.indices[first + p] * to_page +
-                                    (pos - p * s.page_size) * to_slot + d) = x[u];
-        }
-      }
+      for (int u = 0; u < U; ++u)
+        if (i + u * kThreads < items) *reinterpret_cast<i32x4*>(to + off[u]) = x[u];
     }
-    before += n;
-    __syncthreads();
   }
 }
 
@@ -256,9 +251,9 @@ int launch_keep(const fsp_paged_keep_args& a, hipStream_t st) {
                        static_cast<T*>(a.cache.v_pages), a.keep, a.token_indptr, a.lengths, a.kept);
     return check_hip(hipGetLastError(), "paged_keep_kernel launch");
   }
-  hipLaunchKernelGGL((paged_keep_into_kernel<T>), dim3((unsigned)(a.n_pieces * 2 * a.cache.kv_heads)),
+  hipLaunchKernelGGL((paged_keep_into_kernel<T>), dim3((unsigned)(a.n_pieces * (a.piece / kSpan))),
                      dim3(kThreads), 0, st, cache_of(a.cache), s, reinterpret_cast<const Piece*>(a.pieces),
-                     (int)a.piece, (int)a.n_pieces, static_cast<const T*>(a.cache.k_pages),
+                     (int)a.piece, static_cast<const T*>(a.cache.k_pages),
                      static_cast<const T*>(a.cache.v_pages), static_cast<T*>(to.k_pages),
                      static_cast<T*>(to.v_pages), a.keep, a.token_indptr, a.lengths, a.kept);
   return check_hip(hipGetLastError(), "paged_keep_into_kernel launch");
@@ -299,7 +294,8 @@ extern "C" int fsp_paged_keep(const fsp_paged_keep_args* args, void* stream) {
         a.into.batch != a.cache.batch)
       return set_error(FSP_EINVAL, "fsp_paged_keep: the caches differ in type, heads, dim or sequences");
     if (a.piece < 128 || a.piece > kList || a.piece % 128 || a.n_pieces < a.cache.batch || !a.pieces ||
-        a.n_pieces > kMaxBlocks / (2 * a.cache.kv_heads))
+        a.n_pieces > kMaxBlocks / (a.piece / kSpan) ||
+        a.cache.kv_heads * (a.cache.dim / 8) > 0x7fffffff / kSpan)
       return set_error(FSP_EINVAL, "fsp_paged_keep: pieces");
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
