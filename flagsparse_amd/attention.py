@@ -159,6 +159,13 @@ def _window_of(window):
     return min(window, _TOKENS_CAP)
 
 
+def _sight_of(window, sinks, most):
+    """(window, sinks) in numbers; (0, 0) where together they show all of ``most`` tokens."""
+    window = _window_of(window)
+    sinks = _sinks_of(sinks, window)
+    return (0, 0) if sinks and window + sinks >= most else (window, sinks)
+
+
 def _sinks_of(sinks, window):
     sinks = 0 if sinks is None else int(sinks)
     if sinks < 0:
@@ -571,6 +578,8 @@ def flagsparse_paged_keep(keep, lengths, token_indptr=None, *, prepared=None, k_
     key = None
     if into is not None and not isinstance(into, PreparedPagedKV):
         raise TypeError("into must be a PreparedPagedKV instance")
+    if into is not None and into is prepared:
+        raise ValueError("into must be another table; in place needs none")
     if type(prepared) is PreparedPagedKV:
         key = _layouts(keep, lengths, token_indptr) + (
             "keep", prepared.k_pages.data_ptr(), prepared.v_pages.data_ptr())
@@ -708,8 +717,7 @@ def flagsparse_attention_paged(q, lengths, *, prepared=None, k_pages=None, v_pag
                          f"{q.shape[0]}")
     heads = q.shape[1]
     _check_heads(heads, kv.kv_heads)
-    factor, past = _scale_of(scale, kv.dim), _window_of(window)
-    first = _sinks_of(sinks, past)
+    factor, (past, first) = _scale_of(scale, kv.dim), _sight_of(window, sinks, kv.room)
     res, copied = _result(out, "out", q.shape, dt, dev, q, kv.k_pages, kv.v_pages)
     rows = _rows(q)
     # what such calls share: the arguments, patterns of their arrays, the counts of arrivals they need
@@ -828,8 +836,7 @@ def flagsparse_attention_paged_tree(q, lengths, token_indptr=None, *, parents=No
         longest = min(longest, tokens)
     if parents is not None:
         parents = _int32(parents, "parents", tokens, dev, -2)
-    factor, past = _scale_of(scale, kv.dim), _window_of(window)
-    first = _sinks_of(sinks, past)
+    factor, (past, first) = _scale_of(scale, kv.dim), _sight_of(window, sinks, kv.room)
     res, copied = _result(out, "out", q.shape, dt, dev, q, kv.k_pages, kv.v_pages)
     rows = _rows(q)
     if prepared is None:
@@ -1025,10 +1032,9 @@ def _packed_inputs(q, k, v, indptr, k_indptr, prepared, causal, window, sinks):
     _check_tensor(v, "v", q.dtype, q.device, k.shape[1], q.shape[2])
     _check_heads(q.shape[1], k.shape[1])
     _check_dim(q.shape[2])
-    window = _window_of(window)
-    if window and not causal:
+    if _window_of(window) and not causal:
         raise ValueError("window needs causal=True")
-    sinks = _sinks_of(sinks, window)
+    _sinks_of(sinks, window)
     if prepared is None:
         if indptr is None:
             raise ValueError("indptr is required when prepared is not provided")
@@ -1042,7 +1048,7 @@ def _packed_inputs(q, k, v, indptr, k_indptr, prepared, causal, window, sinks):
     if k.shape[0] != prepared.k_tokens or v.shape[0] != prepared.k_tokens:
         raise ValueError(f"k and v must have {prepared.k_tokens} tokens, got {k.shape[0]} and "
                          f"{v.shape[0]}")
-    return prepared, bool(causal), window, sinks
+    return prepared, bool(causal), *_sight_of(window, sinks, prepared._longest[1])
 
 
 def _pack(prepared, q, k, v, causal, window, scale, out, grads=(), sinks=0):

@@ -1048,14 +1048,15 @@ int launch_grad_q(const Call& a, hipStream_t st) {
   return check_hip(hipGetLastError(), "attention_grad_q_kernel launch");
 }
 
-// Queries of a job of the first keys: about what the other tiles have under their window.
-int64_t chunk_of(int64_t window) {
-  const int64_t least = 512;
-  return window <= least ? least : (window + 127) / 128 * 128;
+// Queries of a job of the first keys: about what the other tiles have under their window, and no fewer than there
+// are first keys, whose tiles are workgroups enough then and whose sums would take more room than the keys.
+int64_t chunk_of(int64_t window, int64_t firsts) {
+  const int64_t least = window > firsts ? window : firsts;
+  return least <= 512 ? 512 : (least + 127) / 128 * 128;
 }
 
-int64_t job_slots(int64_t q_tokens, int64_t batch, int64_t window) {
-  return q_tokens / chunk_of(window) + batch;
+int64_t job_slots(int64_t q_tokens, int64_t batch, int64_t window, int64_t firsts) {
+  return q_tokens / chunk_of(window, firsts) + batch;
 }
 
 // Elements of one share's sums over all keys, and of the jobs' of the first keys in tiles of ``rows``.
@@ -1067,12 +1068,13 @@ int64_t first_keys(int64_t sinks, int64_t k_longest) { return sinks < k_longest 
 
 Jobs jobs_of(const Call& a, int split, int rows, float* sums) {
   Jobs j;
+  const int64_t firsts = first_keys(a.sinks, a.k_longest);
   j.sequences = reinterpret_cast<const Tile*>(a.sequences);
   j.sums = sums + share_floats(split, a.kv_heads, a.k_tokens, a.dim);
   j.batch = (int)a.batch;
-  j.chunk = (int)chunk_of(a.window);
-  j.slots = (int)job_slots(a.q_tokens, a.batch, a.window);
-  j.tiles = (int)((first_keys(a.sinks, a.k_longest) + rows - 1) / rows);
+  j.chunk = (int)chunk_of(a.window, firsts);
+  j.slots = (int)job_slots(a.q_tokens, a.batch, a.window, firsts);
+  j.tiles = (int)((firsts + rows - 1) / rows);
   j.blocks = (int)((j.tiles * (int64_t)j.slots * a.kv_heads * split + 7) / 8 * 8);
   return j;
 }
@@ -1184,8 +1186,8 @@ extern "C" int64_t fsp_attention_packed_sinks_workspace(int64_t n_k_tiles, int64
                                                         int64_t batch, int64_t window, int64_t sinks) {
   const int64_t rest = fsp_attention_packed_workspace(n_k_tiles, heads, kv_heads, dim, q_tokens, k_tokens, 0);
   if (rest <= 0 || sinks <= 0 || batch < 0 || window < 1 || k_longest < 0) return rest;
-  const int64_t rows = (first_keys(sinks, k_longest) + kRows - 1) / kRows * kRows;
-  return rest + sizeof(float) * 2 * job_slots(q_tokens, batch, window) *
+  const int64_t firsts = first_keys(sinks, k_longest), rows = (firsts + kRows - 1) / kRows * kRows;
+  return rest + sizeof(float) * 2 * job_slots(q_tokens, batch, window, firsts) *
                     split_heads(n_k_tiles, heads, kv_heads, false) * kv_heads * rows * dim;
 }
 
@@ -1222,9 +1224,9 @@ int run_backward(const Call& a, const std::string& who, void* stream) {
   if (a.sinks && a.n_k_tiles > 0) {
     if (a.batch < 1 || !a.sequences) return set_error(FSP_EINVAL, who + ": sequences");
     // tiles of 32 keys, the most jobs
-    const int64_t tiles = (first_keys(a.sinks, a.k_longest) + kRows / 2 - 1) / (kRows / 2);
+    const int64_t firsts = first_keys(a.sinks, a.k_longest), tiles = (firsts + kRows / 2 - 1) / (kRows / 2);
     const int64_t all = kMaxBlocks / a.heads - a.n_k_halves - 8;
-    if (a.batch > kMaxBlocks || (tiles > 0 && job_slots(a.q_tokens, a.batch, a.window) > all / tiles) ||
+    if (a.batch > kMaxBlocks || (tiles > 0 && job_slots(a.q_tokens, a.batch, a.window, firsts) > all / tiles) ||
         a.batch > kMaxBlocks / 2 / a.kv_heads / (tiles * (kRows / 2) * (a.dim / 4) / 128 + 1))
       return set_error(FSP_EINVAL, who + ": sinks of so many sequences");
   }

@@ -56,8 +56,6 @@ __device__ __forceinline__ V8<T> turned(const T* row, int d, const float* cos, c
   return __builtin_convertvector(y, V8<T>);
 }
 
-constexpr int kDrafts = 256;  // drafted tokens of one sequence, at most
-
 // The depth of token i of a sequence's ``count`` drafted ones, whose parents start at ``up``: the steps up to
 // one without; -1 where they do not lead up.  A wave holds all parents, and walks by the lanes that they
 // lie in.
@@ -115,6 +113,7 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(
     const int begin = tokens[b], end = tokens[b + 1];
     mine = begin <= t && t < end;
     pos = turn = (int64_t)lengths[b] - end + t;
+    if (parents && mine && (begin < 0 || end > s.n_tokens)) mine = false;  // its parents are not there
     if (parents && mine) {
       depth = __builtin_amdgcn_readfirstlane(depth_of(parents + begin, (int)(t - begin), end - begin));
       turn = (int64_t)lengths[b] - (end - begin) + depth;

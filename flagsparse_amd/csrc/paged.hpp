@@ -5,6 +5,8 @@
 
 namespace fsp {
 
+constexpr int kDrafts = 256;  // drafted tokens of one sequence, at most
+
 struct Cache {
   const int32_t *indptr, *indices;
   int64_t k_page, k_slot, k_head, v_page, v_slot, v_head;

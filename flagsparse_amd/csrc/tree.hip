@@ -5,7 +5,6 @@
 namespace fsp {
 namespace {
 
-constexpr int kDrafts = 256;     // drafted tokens of one sequence, at most
 // More rows than so many beside a key go to wide tiles.  Tiles of 32 rows / wide ones, us, 8 key heads of 128: 8
 // sequences of 30000, 36 rows 225 / 192, 64 rows 225 / 195; 4 of 2000, 64 rows 20.6 / 19.5; 96 ragged ones of up to
 // 8000, 64 rows 126 / 97; 4 heads of 64, 8 of 30000, 36 rows 68 / 59.

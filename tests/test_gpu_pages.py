@@ -110,6 +110,15 @@ def test_append_drafts_without_a_way(dev):
         assert torch.isnan(got.float()).all(-1).all(-1).cpu().nonzero().flatten().tolist() == fallen
         here = _slots(kv, 0, [90 + i for i in fallen])
         assert torch.equal(_bits(kv.k_pages[here]), _bits(before[here]))
+    # tokens that lead nowhere: no parent outside the array is looked at
+    for bad in ([-3, 9, 21], [0, 9, 2**31 - 1], [0, 2**40, 21], [-2**40, 5, 2**40], [30, 9, 21]):
+        parents = torch.tensor(flat, device=dev)
+        got = fs.flagsparse_paged_append(k, k, n, torch.tensor(bad, device=dev), prepared=kv, q=q,
+                                         parents=parents)
+        if bad[0] < 0:
+            assert torch.isnan(got[:5].float()).all()
+        if bad[2] > 21:
+            assert torch.isnan(got[9:].float()).all()
     # more than 256 of a sequence
     kv, _, _ = _cache(dev, [300], 16, 2, 64, BF)
     k = _normal(1, 257, 2, 64, dtype=BF).to(dev)
@@ -369,6 +378,8 @@ def test_refusals(dev):
         fs.flagsparse_paged_keep(keep.int(), n, tokens, prepared=kv)
     with pytest.raises(TypeError):
         fs.flagsparse_paged_keep(keep, n, tokens, prepared=kv, into=kv.k_pages)
+    with pytest.raises(ValueError):
+        fs.flagsparse_paged_keep(keep, n, tokens, prepared=kv, into=kv)
     for _ in range(2):  # a call that was made before, or not
         for into in (other, half, heads):
             with pytest.raises(ValueError):

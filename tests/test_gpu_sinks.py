@@ -79,6 +79,12 @@ def test_other_keys(dev, q_len, k_len):
     _both(dev, q_len, k_len, 2, 2, 128, HF, 5, 80)
 
 
+def test_many_first_keys(dev):
+    # jobs hold as many queries as there are first keys
+    _both(dev, [1900, 100], [1900, 100], 2, 1, 64, BF, 50, 700)
+    _both(dev, [1300], [1500], 4, 2, 128, HF, 3, 1200)
+
+
 def test_jobs_of_queries(dev):
     # first keys under more queries than one job of 512 or of the window has, in ragged batches
     _both(dev, [1700], [1700], 2, 1, 64, BF, 100, 4)

@@ -63,6 +63,7 @@ def test_workspace_holds_the_jobs():
     # 1000 / 512 + 3 slots, two key heads, 64 rows of keys and of values, 32 bits, shares of 4 heads
     assert rows % (4 * 2 * 64 * 2 * 64 * 4) == 0 and rows // (4 * 2 * 64 * 2 * 64 * 4) in (1, 2, 4)
     assert L.fsp_attention_packed_sinks_workspace(*sizes, 600, 3, 100, 70) - without == 2 * rows
+    # 600 of them, the longest sequence's, in jobs of 640 queries
     assert L.fsp_attention_packed_sinks_workspace(*sizes, 600, 3, 100, 2**30) - without == 10 * rows
 
 
@@ -72,6 +73,15 @@ def test_sinks_of():
     for sinks, window in ((3, 0), (-1, 5)):
         with pytest.raises(ValueError):
             attention._sinks_of(sinks, window)
+
+
+def test_windows_that_hide_nothing():
+    for window, sinks, most, want in ((5, 3, 8, (0, 0)), (5, 3, 9, (5, 3)), (5, 0, 4, (5, 0)), (None, 0, 4, (0, 0)),
+                                      (2**40, 2**40, 100, (0, 0)), (1, 7, 8, (0, 0)), (4, None, 2, (4, 0))):
+        assert attention._sight_of(window, sinks, most) == want
+    for window, sinks in ((None, 3), (5, -1), (0, 0), (-2, 0)):
+        with pytest.raises(ValueError):
+            attention._sight_of(window, sinks, 100)
 
 
 def test_reference_sees_first_keys():
