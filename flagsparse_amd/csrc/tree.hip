@@ -71,23 +71,32 @@ __device__ __forceinline__ void nan_outside(const TreeShape& s, const Drafted& t
 // ``mask`` between one of ones and one of zeros; returns its depth, or -1 where the way does not lead up.
 __device__ __forceinline__ int row_mask(const TreeShape& s, const Drafted& t, const int* up, int i,
                                         uint32_t* mask) {
-  mask[0] = ~0u;
+  auto clear = [&] {
+    mask[0] = ~0u;
 #pragma unroll
-  for (int w = 1; w < 11; ++w) mask[w] = 0;
-  int depth = i;
-  if (up) {
-    depth = 0;
-    for (int at = i;;) {
-      const int p = up[at];
-      if (p < -1 || p >= at) return -1;
-      if (p < 0) break;
-      at = p;
-      ++depth;
-    }
+    for (int w = 1; w < 11; ++w) mask[w] = 0;
+  };
+  clear();
+  int depth = 0;
+  for (int at = i;; ++depth) {
+    mask[1 + at / 32] |= 1u << (at & 31);
+    const int p = up ? up[at] : at - 1;
+    if (p < -1 || p >= at) return -1;
+    if (p < 0) break;
+    at = p;
   }
-  for (int at = i, n = 0; at >= 0; at = up ? up[at] : at - 1, ++n)
-    if (!s.window || n < s.window || t.past + depth - n < s.sinks) mask[1 + at / 32] |= 1u << (at & 31);
+  if (s.window && s.window <= depth) {  // the window leaves some of the way out
+    clear();
+    for (int at = i, n = 0; at >= 0; at = up ? up[at] : at - 1, ++n)
+      if (n < s.window || t.past + depth - n < s.sinks) mask[1 + at / 32] |= 1u << (at & 31);
+  }
   return depth;
+}
+
+// Whether the keys [begin, end) hold any that some row does not see: drafted ones, or some that a window leaves
+// deep rows only, whose depth is less than the number of them.
+__device__ __forceinline__ bool some_hidden(const TreeShape& s, const Drafted& t, int begin, int end) {
+  return end > t.past || (s.window && begin < t.past + t.count - s.window);
 }
 
 // Bits of 32 keys, from bit x on.
@@ -221,7 +230,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attention_tree_kernel(
   }
   const float cs = exp2_scale(s.scale);
 
-  const bool masked = s.window || end > t.past;
+  const bool masked = some_hidden(s, t, begin, end);
   if (masked) {
     if (parents)
       for (int i = threadIdx.x; i < t.count; i += 256) s_up[i] = parents[t.begin + i];
@@ -233,7 +242,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attention_tree_kernel(
   }
   int lo[RT];  // the first token that each row's window holds
 #pragma unroll
-  for (int n = 0; n < RT; ++n) lo[n] = s.window ? t.past + s_depth[16 * n + col] - s.window + 1 : 0;
+  for (int n = 0; n < RT; ++n) lo[n] = s.window && masked ? t.past + s_depth[16 * n + col] - s.window + 1 : 0;
 
   const T* kb = k_pages + g * c.k_head;
   const T* vb = v_pages + g * c.v_head;
@@ -491,7 +500,7 @@ __global__ __launch_bounds__(256, 2) void attention_tree_wide_kernel(
   };
 #pragma unroll
   for (int h = 0; h < 2; ++h) place(h, page_of(h));
-  const bool masked = s.window || end > t.past;
+  const bool masked = some_hidden(s, t, begin, end);
   if (masked && parents)
     for (int i = threadIdx.x; i < t.count; i += 256) s_up[i] = parents[t.begin + i];
   __syncthreads();
@@ -530,7 +539,7 @@ __global__ __launch_bounds__(256, 2) void attention_tree_wide_kernel(
   const int k_at = L::row_at(lane), v_at = L::col_at(lane);
   all_stored();
   __syncthreads();
-  const int lo = s.window ? t.past + s_depth[32 * wave + col] - s.window + 1 : 0;
+  const int lo = s.window && masked ? t.past + s_depth[32 * wave + col] - s.window + 1 : 0;
 
   auto work = [&](int step, const char* sk_, const char* sv_) {
     if (!active) return;
