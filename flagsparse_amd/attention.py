@@ -1032,9 +1032,10 @@ def _packed_inputs(q, k, v, indptr, k_indptr, prepared, causal, window, sinks):
     _check_tensor(v, "v", q.dtype, q.device, k.shape[1], q.shape[2])
     _check_heads(q.shape[1], k.shape[1])
     _check_dim(q.shape[2])
-    if _window_of(window) and not causal:
+    window = _window_of(window)
+    if window and not causal:
         raise ValueError("window needs causal=True")
-    _sinks_of(sinks, window)
+    sinks = _sinks_of(sinks, window)
     if prepared is None:
         if indptr is None:
             raise ValueError("indptr is required when prepared is not provided")
@@ -1048,7 +1049,7 @@ def _packed_inputs(q, k, v, indptr, k_indptr, prepared, causal, window, sinks):
     if k.shape[0] != prepared.k_tokens or v.shape[0] != prepared.k_tokens:
         raise ValueError(f"k and v must have {prepared.k_tokens} tokens, got {k.shape[0]} and "
                          f"{v.shape[0]}")
-    return prepared, bool(causal), *_sight_of(window, sinks, prepared._longest[1])
+    return prepared, bool(causal), window, sinks
 
 
 def _pack(prepared, q, k, v, causal, window, scale, out, grads=(), sinks=0):

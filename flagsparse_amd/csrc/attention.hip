@@ -366,6 +366,14 @@ __device__ __forceinline__ int lower(f32x16& y, f32x16 (&acc)[NT]) {
 // without, 1.47 and 1.45 with it, 1.45 and 1.44 with 256 keys; backward of 30 sequences of 200, 32 heads
 // 127 / 135 / 147 us, of two of 4096 no different.
 constexpr int kFewKeys = 128;
+// Under a window with first tokens, where no query may come to see many, the rule is finer: by what a tile's first
+// query sees, and by the dim, as what the output's rounding does to delta against what one rounding does to
+// the gradient falls with its root.  The same ratio without and with delta made anew, 2000 tokens, 264 keys a
+// query: dim 40 1.53 / 1.45, 64 1.50 / 1.45, 96 1.47 / 1.43; dim 64, 404 and 1204 keys: 1.50, 1.47 without.  It takes
+// about a third of this kernel's time: 6 sequences up to 1501, 270 keys, 12 heads of 96 21 / 29 us.
+__device__ __forceinline__ bool delta_anew(int dim, int seen) {
+  return seen <= 256 || dim < 64 || (dim < 80 && seen <= 512);
+}
 
 // Gradient of the queries: the forward pass's loop over keys with dP^T = V grad_out^T beside S^T; dS^T
 // = P^T (dP^T - delta), delta = grad_out . out, is the operand of dQ^T = K^T dS^T where it lies.  P comes
@@ -495,7 +503,10 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, DP <= 64 ? 3 : 2) void attenti
 
   // An output of few keys is large, and so is what its rounding does to delta = grad_out . out: there
   // delta is made anew, as the sum of the weights times dP.
-  if (keys.end <= kFewKeys) {
+  int first_lo, first_hi;
+  seen_by(s, t, t.at, first_lo, first_hi);
+  const int seen = SINKS ? first_hi - first_lo + min(s.sinks, first_lo) : keys.end;
+  if (SINKS ? delta_anew(s.dim, seen) : seen <= kFewKeys) {
     delta = 0;
     walk([&](int i0, const lds_char* sk, const lds_char* sv) {
 #pragma unroll
