@@ -229,14 +229,21 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_packed_kerne
     }
     read_ahead<2 * NS, NS>();
     if (j0 + kRows > hi0 || j0 < lo1) {
-      const int first = lo - j0 - 4 * half, last = hi - j0 - 4 * half, keep = s.sinks - i0 - 4 * half;
+      if constexpr (SINKS) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < 2; ++u)
+          seen_or_none((bits_from(lo - j0 - 32 * u) | ~bits_from(s.sinks - i0 - 32 * u)) &
+                           ~bits_from(hi - j0 - 32 * u), half, x[u]);
+      } else {
+        const int first = lo - j0 - 4 * half, last = hi - j0 - 4 * half;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int j = 32 * u + 8 * (r / 4) + r % 4;
-          x[u][r] = (j >= first || (SINKS && j < keep)) && j < last ? x[u][r] : -INFINITY;
-        }
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int j = 32 * u + 8 * (r / 4) + r % 4;
+            x[u][r] = j >= first && j < last ? x[u][r] : -INFINITY;
+          }
+      }
     }
     float m = x[0][0];
 #pragma unroll
@@ -471,11 +478,16 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, DP <= 64 ? 3 : 2) void attenti
   auto hide = [&](int i0, int u, f32x16& x) {
     const int j0 = keys.at(i0);
     if (j0 + kRows > hi0 || j0 < lo1) {
-      const int first = lo - j0 - 4 * half, last = hi - j0 - 4 * half, keep = s.sinks - i0 - 4 * half;
+      if constexpr (SINKS) {
+        seen_or_none<true>((bits_from(lo - j0 - 32 * u) | ~bits_from(s.sinks - i0 - 32 * u)) &
+                               ~bits_from(hi - j0 - 32 * u), half, x);
+      } else {
+        const int first = lo - j0 - 4 * half, last = hi - j0 - 4 * half;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int j = 32 * u + 8 * (r / 4) + r % 4;
-        x[r] = (j >= first || (SINKS && j < keep)) && j < last ? x[r] : 0.0f;
+        for (int r = 0; r < 16; ++r) {
+          const int j = 32 * u + 8 * (r / 4) + r % 4;
+          x[r] = j >= first && j < last ? x[r] : 0.0f;
+        }
       }
     }
   };
@@ -765,13 +777,19 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_grad_kv_kern
       int key = mine, lo, hi;  // what sees this lane's key: made anew, as above
       asm volatile("" : "+v"(key));
       sees(t.at + min(key, t.rows - 1), lo, hi);
-      const int first = lo - i1 - 4 * half, last = hi - i1 - 4 * half;
+      if constexpr (SINKS) {
+        const uint32_t bits = bits_from(lo - i1) & ~bits_from(hi - i1);
+        seen_or_none<true>(bits, half, x);
+        seen_or_none<true>(bits, half, y);
+      } else {
+        const int first = lo - i1 - 4 * half, last = hi - i1 - 4 * half;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int i = 8 * (r / 4) + r % 4;
-        const bool in = i >= first && i < last;
-        x[r] = in ? x[r] : 0.0f;
-        y[r] = in ? y[r] : 0.0f;
+        for (int r = 0; r < 16; ++r) {
+          const int i = 8 * (r / 4) + r % 4;
+          const bool in = i >= first && i < last;
+          x[r] = in ? x[r] : 0.0f;
+          y[r] = in ? y[r] : 0.0f;
+        }
       }
     }
     if constexpr (RAISED) raised = ldexpf(raised, -lower(y, ak));

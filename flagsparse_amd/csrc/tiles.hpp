@@ -91,4 +91,29 @@ __device__ __forceinline__ void store_rows(T* to, const f32x16 (&x)[NT], float f
     }
 }
 
+// Bits of 32 keys, from bit x on.
+__device__ __forceinline__ uint32_t bits_from(int x) { return x <= 0 ? ~0u : x > 31 ? 0u : ~0u << x; }
+
+// x where bit K is set, else minus infinity or, with ZERO, 0; without a condition, which would hold a pair of
+// scalar registers for each element.
+template <int K, bool ZERO = false>
+__device__ __forceinline__ float seen_or_none(uint32_t bits, float x) {
+  const uint32_t m = (uint32_t)((int)(bits << (31 - K)) >> 31);
+  return __uint_as_float((__float_as_uint(x) & m) | (ZERO ? 0u : 0xff800000u & ~m));
+}
+
+// The same for the 16 keys of 32 that an accumulator holds in this half of the lanes.
+template <bool ZERO = false>
+__device__ __forceinline__ void seen_or_none(uint32_t bits, int half, f32x16& x) {
+  bits >>= 4 * half;
+#pragma unroll
+  for (int r = 0; r < 16; r += 4) {
+    const uint32_t b = bits >> (2 * r);
+    x[r] = seen_or_none<0, ZERO>(b, x[r]);
+    x[r + 1] = seen_or_none<1, ZERO>(b, x[r + 1]);
+    x[r + 2] = seen_or_none<2, ZERO>(b, x[r + 2]);
+    x[r + 3] = seen_or_none<3, ZERO>(b, x[r + 3]);
+  }
+}
+
 }  // namespace fsp

@@ -99,9 +99,6 @@ __device__ __forceinline__ bool some_hidden(const TreeShape& s, const Drafted& t
   return end > t.past || (s.window && begin < t.past + t.count - s.window);
 }
 
-// Bits of 32 keys, from bit x on.
-__device__ __forceinline__ uint32_t bits_from(int x) { return x <= 0 ? ~0u : x > 31 ? 0u : ~0u << x; }
-
 // Which of the 32 keys from place e0 on a row sees, whose first token by its window is ``lo``; ``count`` of them
 // are keys of the piece.
 __device__ __forceinline__ uint32_t seen_keys(const TreeShape& s, const Drafted& t, const uint32_t* mask, int lo,
@@ -114,14 +111,6 @@ __device__ __forceinline__ uint32_t seen_keys(const TreeShape& s, const Drafted&
   }
   const uint32_t far = ~bits_from(max(s.sinks, t.old) - e0);  // the first tokens that stay visible
   return bits & (bits_from(lo - e0) | far | bits_from(t.past - e0)) & ~bits_from(count);
-}
-
-// x where bit K is set, else minus infinity; without a condition, which would hold a pair of scalar
-// registers for each element.
-template <int K>
-__device__ __forceinline__ float seen_or_none(uint32_t bits, float x) {
-  const uint32_t m = (uint32_t)((int)(bits << (31 - K)) >> 31);
-  return __uint_as_float((__float_as_uint(x) & m) | (0xff800000u & ~m));
 }
 
 // Whether this workgroup is the last of ``pieces`` to arrive, which joins them; it leaves the count as it was
@@ -558,17 +547,8 @@ __global__ __launch_bounds__(256, 2) void attention_tree_wide_kernel(
     const bool tail = e0 + kRows > t.past;
     if (tail || j0 + kRows > n || __any(lo > max(e0, t.old))) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint32_t bits = seen_keys(s, t, s_mask[32 * wave + col], lo, e0 + 32 * u, n - j0 - 32 * u) >> (4 * half);
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-          const uint32_t b = bits >> (2 * r);
-          x[u][r] = seen_or_none<0>(b, x[u][r]);
-          x[u][r + 1] = seen_or_none<1>(b, x[u][r + 1]);
-          x[u][r + 2] = seen_or_none<2>(b, x[u][r + 2]);
-          x[u][r + 3] = seen_or_none<3>(b, x[u][r + 3]);
-        }
-      }
+      for (int u = 0; u < 2; ++u)
+        seen_or_none(seen_keys(s, t, s_mask[32 * wave + col], lo, e0 + 32 * u, n - j0 - 32 * u), half, x[u]);
     }
     float m = x[0][0];
 #pragma unroll
