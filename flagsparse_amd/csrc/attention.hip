@@ -813,7 +813,11 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_grad_kv_kern
   int a = a0, i0 = lot + (steps - 1) * ROWS;  // of this step
   int a1 = a, i1 = i0;                        // of the one being loaded
   auto next = [&] {
-    if (++a1 == a0 + group) a1 = a0, i1 -= ROWS;
+    if constexpr (SINKS) {
+      if ((i1 -= ROWS) < lot) ++a1, i1 = lot + (steps - 1) * ROWS;
+    } else {
+      if (++a1 == a0 + group) a1 = a0, i1 -= ROWS;
+    }
   };
   if (total) load(a, i0, s_q0, s_g0, s_x0, s_y0);
   __syncthreads();
