@@ -599,12 +599,12 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, DP <= 64 ? 3 : 2) void attenti
 }
 
 // Where first keys stay visible to all later queries, their tiles would have many times the others' work
-// under a window: with SINKS they go to jobs of ``chunk`` queries each, whose sums another launch adds in
+// under a window (four of 4096 under 512: eight times): with SINKS they go to jobs of ``chunk`` queries each, whose sums another launch adds in
 // their order.  Slot q_begin / chunk + b + i is the job of the queries [i * chunk, (i + 1) * chunk) of sequence b:
 // no two are the same, and there are at most q_tokens / chunk + batch.  A slot holds, for each share
 // of the heads, key head and first key, the values' sums and then the keys'.
 struct Jobs {
-  const Tile* sequences;  // rows, first row, ..: unused; q_begin, nq, k_begin, nk
+  const Tile* sequences;  // of each its q_begin, nq, k_begin, nk
   float* sums;
   int batch, chunk, slots, tiles, blocks;  // tiles of first keys a sequence; workgroups of all jobs
 };
@@ -812,6 +812,9 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_grad_kv_kern
   const int total = steps * group, a0 = (g * split + share) * group;
   int a = a0, i0 = lot + (steps - 1) * ROWS;  // of this step
   int a1 = a, i1 = i0;                        // of the one being loaded
+  // Under a window with first keys the rows are few enough that a head after the other lets the tiles share
+  // them: two of 8192, 32 heads of 128 over 8, window 1024, forward and backward 1491 us with the heads
+  // in turn, 1374 so; four of 4096, 16 heads of 64 over 4, window 512 243 and 231 (416 MB past the L2s before).
   auto next = [&] {
     if constexpr (SINKS) {
       if ((i1 -= ROWS) < lot) ++a1, i1 = lot + (steps - 1) * ROWS;
@@ -901,7 +904,8 @@ __global__ __launch_bounds__(256) void attention_grad_kv_sum_kernel(
 
 // The same for tiles of first keys, as the sums of their jobs, chunk by chunk and in each the shares of the
 // heads, by workgroups of their own, [0, of_jobs): a thread to four elements, a workgroup's of one sequence
-// and key head.  The others add the shares of all other keys.
+// and key head.  The others add the shares of all other keys, whose sequence each thread looks up: one launch of
+// 5.7 us for 6 sequences up to 1501, 4 key heads of 96, where two took 4.3 and 4.2 and the gap between them.
 template <typename T, int ROWS>
 __global__ __launch_bounds__(256) void attention_grad_sinks_sum_kernel(
     Shape s, int split, Jobs jobs, int of_jobs, const float* __restrict__ sums, int64_t k_tokens,
@@ -956,8 +960,10 @@ template <typename T>
 const T* in(const void* p) { return static_cast<const T*>(p); }
 
 // Under a window with first keys a tile of queries is of several heads of a group, the largest divisor of its
-// size up to 32: its rows see nearly the same keys, where as many queries of one head see as many more.
-// TIMES
+// size up to 32: its rows see nearly the same keys, where as many queries of one head see as many more.  With
+// tiles of one head (and steps of their own for the first keys) and so, us: two of 8192, window 1024, 16 heads of
+// 128 over 4 170 / 166; forward and backward: four of 4096, window 512, 16 heads of 64 over 4 244 / 231; 6 ragged
+// ones up to 1501, window 200, 70 first keys, 12 heads of 96 over 4 77 / 67.
 int heads_beside(int64_t group) {
   int width = 1;
   for (int i = 2; i <= 32; ++i)

@@ -54,10 +54,11 @@ __device__ __forceinline__ int list_kept(const uint8_t* keep, int at, int count,
   return total;
 }
 
-// In place.  A workgroup takes one sequence, one key head and its keys or values, so that nobody else
+// In place, for drafted tokens.  A workgroup takes one sequence, one key head and its keys or values, so that nobody else
 // writes what it reads.  The n-th token that stays comes from a place n or later, each from a later one than the one
 // before it: rows that are read after others were written are theirs still.  Of the rows of one step
-// all are read before any is written.
+// all are read before any is written.  16 sequences of up to 26 drafted tokens, 8 heads of 128: 3.9 us, a chain
+// of dependent loads (offsets -> marks -> pages -> rows).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void paged_keep_kernel(
     Cache c, KeepShape s, T* __restrict__ k_pages, T* __restrict__ v_pages,
@@ -105,7 +106,9 @@ __global__ __launch_bounds__(kThreads) void paged_keep_kernel(
 }
 
 // Into other pages: a workgroup takes kSpan of a sequence's tokens, all heads of their keys and values.  How many
-// tokens stay before them, and of all, it counts itself, four marks to a word.
+// tokens stay before them, and of all, it counts itself, four marks to a word.  Bound by memory: half of 16
+// sequences of 8192, 8 heads of 128, 537 MB in 110 to 124 us, 4.3 to 4.9 TB/s, where a plain copy has 4.7 to 4.9.  A
+// workgroup to a head of 1024 tokens, whose rows of 256 bytes lie apart, took 155 us.
 constexpr int kSpan = kWave;
 
 template <typename T>
@@ -209,7 +212,8 @@ __global__ __launch_bounds__(kThreads) void paged_keep_into_kernel(
 }
 
 // Page sources[i] to targets[i], ``parts`` workgroups to the keys or values of one, a vector of eight elements
-// a thread and step.
+// a thread and step.  Bound by memory: 4001 pages of 16 tokens, 8 heads of 128, 524 MB in 109 us, 4.8 TB/s, a plain
+// copy's rate; 7 pages in 3.0 us, a launch and two dependent loads.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void paged_copy_kernel(
     Cache c, int n_pages, T* __restrict__ k_pages, T* __restrict__ v_pages,

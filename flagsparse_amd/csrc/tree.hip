@@ -167,6 +167,10 @@ __device__ __forceinline__ void join_tile(const float* part_o, const float* part
 // head and RT * 16 rows, so that what it reads of the cache serves all of them; its four waves take
 // every fourth 32 keys.  Keys, values and products lie as in attention_paged_kernel, with RT times
 // the rows beside each key: a key's fragment is read from LDS once for all, a value's put together once.
+// Bound by memory: 8 sequences of 30000, 8 heads of 128, 983 MB in 166 us with 8 rows, 174 us with 32, 5.7 to
+// 5.9 TB/s of the 7.0 of a plain read.  Rows for four tiles at once would not fit the registers (480 for dim 128).
+// For 1200 tokens, 16 heads of 64 and 8 rows the chain piece -> length, offsets -> pages -> keys and the join are
+// all of its 9 us.
 template <typename T, int DP, bool EXACT, bool NT, int RT>
 __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attention_tree_kernel(
     Cache c, TreeShape s, const Piece* __restrict__ pieces, const T* __restrict__ k_pages,
@@ -424,7 +428,13 @@ __device__ const i32x4 kZeros = {0, 0, 0, 0};
 
 // Many rows: 128 of them a workgroup, 32 a wave, over the same 64 keys, which go straight to LDS by the places
 // that a table there holds, the next step's while this one's are worked on: as attention_packed_kernel, whose
-// comments say how the products lie.  The table's two halves of 256 keys are filled in turn.
+// comments say how the products lie.  The table's two halves of 256 keys are filled in turn, the pages of
+// the next one asked for four steps before.  8 sequences of 30000, 8 heads of 128, 256 rows, 2.5e11 operations and
+// 983 MB: 288 us and 11 for the join, 0.84 PFLOP/s (a library's 8192^3 product: 1.21); products take 47 % of
+// the SIMDs' cycles, vector instructions 44 %, both at a time 16 %, at the 1.94 GHz that power leaves; no bank
+// conflicts.  128 rows: 203 us in all, 4.9 TB/s.  Choosing addresses for rows past a head's dim by a branch made
+// it 373 us, conditions instead of bits for the masks 348: they kept scalar registers in memory.  A higher
+// priority of waves in their products, or exponentials put between them, changed nothing (315 / 315, 312 / 320).
 template <typename T, int DP, bool EXACT>
 __global__ __launch_bounds__(256, 2) void attention_tree_wide_kernel(
     Cache c, TreeShape s, const Piece* __restrict__ pieces, const T* __restrict__ k_pages,
@@ -620,7 +630,9 @@ __global__ __launch_bounds__(256, 2) void attention_tree_wide_kernel(
     *reinterpret_cast<f32x2*>(part_ml + 2 * at) = f32x2{top == -INFINITY ? -INFINITY : top * cs, sum};
 }
 
-// Joins the pieces of sequences that have several: half a wave to a row, eight pieces of it at a time.
+// Joins the pieces of sequences that have several: half a wave to a row, eight pieces of it at a time (sixteen:
+// 24.3 / 26.0 us for 33 ragged sequences, 23 heads of 80, where it takes 7.6 of them).  Bound by its loads one after
+// the other: lengths and offsets, sums, and a second round from nine pieces on.
 template <typename T>
 __global__ __launch_bounds__(256) void attention_tree_join_kernel(
     Cache c, TreeShape s, const int32_t* __restrict__ first_piece, T* __restrict__ out, int64_t out_token,
