@@ -118,11 +118,11 @@ __device__ __forceinline__ void load_rows_apart(char* lds, const void* src, int 
   for (int i = 0; i < PER; ++i) {
     const int at = 16 * (chunk ^ L::swizzle(i * EACH)), r = (wave * PER + i) * EACH + lane / L::CH;
     const uint32_t off = at < 2 * dim ? (uint32_t)(r < first ? r : r - first) * bytes + at : 0x80000000u;
-    typedef __attribute__((address_space(3))) void lds_void;
+    const auto to = (__attribute__((address_space(3))) void*)(lds + (wave * PER + i) * 1024);
     if (r < first)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(near, (lds_void*)(lds + (wave * PER + i) * 1024), 16, (int)off, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(near, to, 16, (int)off, 0, 0, 0);
     else
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(far, (lds_void*)(lds + (wave * PER + i) * 1024), 16, (int)off, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(far, to, 16, (int)off, 0, 0, 0);
   }
 }
 
@@ -599,10 +599,11 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, DP <= 64 ? 3 : 2) void attenti
 }
 
 // Where first keys stay visible to all later queries, their tiles would have many times the others' work
-// under a window (four of 4096 under 512: eight times): with SINKS they go to jobs of ``chunk`` queries each, whose sums another launch adds in
-// their order.  Slot q_begin / chunk + b + i is the job of the queries [i * chunk, (i + 1) * chunk) of sequence b:
-// no two are the same, and there are at most q_tokens / chunk + batch.  A slot holds, for each share
-// of the heads, key head and first key, the values' sums and then the keys'.
+// under a window (four of 4096 under 512: eight times): with SINKS they go to jobs of ``chunk`` queries each,
+// whose sums another launch adds in their order.  Slot q_begin / chunk + b + i is the job of the queries
+// [i * chunk, (i + 1) * chunk) of sequence b: no two are the same, and there are at most
+// q_tokens / chunk + batch.  A slot holds, for each share of the heads, key head and first key, the
+// values' sums and then the keys'.
 struct Jobs {
   const Tile* sequences;  // of each its q_begin, nq, k_begin, nk
   float* sums;
@@ -814,7 +815,7 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_grad_kv_kern
   int a1 = a, i1 = i0;                        // of the one being loaded
   // Under a window with first keys the rows are few enough that a head after the other lets the tiles share
   // them: two of 8192, 32 heads of 128 over 8, window 1024, forward and backward 1491 us with the heads
-  // in turn, 1374 so; four of 4096, 16 heads of 64 over 4, window 512 243 and 231 (416 MB past the L2s before).
+  // in turn, 1374 so; four of 4096, 16 heads of 64 over 4, window 512 243 and 231 (416 and 149 MB past the L2s).
   auto next = [&] {
     if constexpr (SINKS) {
       if ((i1 -= ROWS) < lot) ++a1, i1 = lot + (steps - 1) * ROWS;
