@@ -5,8 +5,10 @@
 Training runs ``flagsparse_attention_packed`` and its gradient over sequences of different lengths,
 packed one after the other.  Generation runs the prompts through the same call while
 ``flagsparse_paged_append`` stores their keys and values, then goes on token by token with
-``flagsparse_paged_append`` and ``flagsparse_attention_paged``.  The task: a sequence repeats a short
-pattern, so that the model has to attend to where it saw the last token before.
+``flagsparse_paged_append`` and ``flagsparse_attention_paged``; or several tokens at a step, by trees of
+drafted tokens (``flagsparse_attention_paged_tree``), of which those that the model agrees with stay
+(``flagsparse_paged_keep``).  The task: a sequence repeats a short pattern, so that the model has to attend to where
+it saw the last token before.
 """
 
 import os
@@ -96,13 +98,11 @@ def train(model, device, steps, seed=1):
     return torch.stack(losses).tolist()
 
 
-@torch.no_grad()
-def generate(model, device, prompts, count):
-    """[prompt, count] new tokens and their logits [prompt, count, vocabulary]."""
+def read_prompts(model, device, prompts, room):
+    """(the cache with ``room`` places behind each prompt, lengths, last tokens, logits after them)."""
     cos, sin = tables(device)
-    batch_size = len(prompts)
     # every sequence gets the pages that it will need; in what order they lie does not matter
-    held = torch.tensor([-(-(len(p) + count) // PAGE) for p in prompts])
+    held = torch.tensor([-(-(len(p) + room) // PAGE) for p in prompts])
     indptr = torch.cat([torch.zeros(1, dtype=torch.int64), held.cumsum(0)]).to(device)
     pages = int(held.sum())
     cache = torch.zeros(2, pages, PAGE, KV_HEADS, DIM, dtype=torch.bfloat16, device=device)
@@ -120,9 +120,15 @@ def generate(model, device, prompts, count):
                                         q=fused[:, :HEADS + KV_HEADS], cos=cos, sin=sin)
     attended = fs.flagsparse_attention_packed(turned[:, :HEADS], turned[:, HEADS:], v, offsets)
     last = offsets[1:].long() - 1
-    logits = model.logits(x[last], attended[last])
+    return kv, lengths, tokens[last], model.logits(x[last], attended[last])
 
-    all_tokens, all_logits, current = [], [], tokens[last]
+
+@torch.no_grad()
+def generate(model, device, prompts, count):
+    """[prompt, count] new tokens and their logits [prompt, count, vocabulary]."""
+    cos, sin = tables(device)
+    kv, lengths, current, logits = read_prompts(model, device, prompts, count)
+    all_tokens, all_logits = [], []
     for step in range(count):
         chosen = logits.argmax(-1)
         all_tokens.append(chosen)
@@ -136,8 +142,62 @@ def generate(model, device, prompts, count):
         attended = fs.flagsparse_attention_paged(turned, lengths, prepared=kv)
         logits = model.logits(x, attended)
         current = chosen
-    assert all_tokens[0].shape == (batch_size,)
     return torch.stack(all_tokens, 1), torch.stack(all_logits, 1)
+
+
+def draft(text, breadth, depth):
+    """(tokens, parents) of a tree that starts at the last token of a text: what followed the token's last
+    ``breadth`` places before, ``depth`` tokens each."""
+    tokens, parents = [text[-1]], [-1]
+    places = [i for i, token in enumerate(text[:-1]) if token == text[-1]]
+    for place in places[-breadth:]:
+        at = 0
+        for token in text[place + 1:place + 1 + depth]:
+            same = [i for i, p in enumerate(parents) if p == at and tokens[i] == token]
+            if not same:
+                tokens.append(token)
+                parents.append(at)
+            at = same[0] if same else len(tokens) - 1
+    return tokens, parents
+
+
+@torch.no_grad()
+def generate_drafted(model, device, prompts, count, breadth=3, depth=5):
+    """([prompt, count] new tokens, the steps that they took): each step reads a tree of drafted tokens for each
+    sequence, and goes on from the last one of those that the model would have chosen."""
+    cos, sin = tables(device)
+    most = 1 + breadth * depth
+    kv, lengths, _, logits = read_prompts(model, device, prompts, count + 2 * most)
+    texts = [p.tolist() + [int(t)] for p, t in zip(prompts, logits.argmax(-1))]
+    steps = 0
+    while min(len(text) - len(p) for text, p in zip(texts, prompts)) < count:
+        trees = [draft(text, breadth, depth) if len(text) - len(p) < count else ([], [])
+                 for text, p in zip(texts, prompts)]
+        tokens = torch.tensor([t for tree in trees for t in tree[0]], device=device)
+        before = torch.tensor([tree[0][p] if p >= 0 else text[-2] for tree, text in zip(trees, texts)
+                               for p in tree[1]], device=device)
+        parents = torch.tensor([p for tree in trees for p in tree[1]], dtype=torch.int32, device=device)
+        new = torch.tensor([len(tree[0]) for tree in trees], dtype=torch.int32)
+        offsets = torch.cat([new.new_zeros(1), new.cumsum(0, dtype=torch.int32)]).to(device)
+        lengths = lengths + new.to(device)
+        x, fused = model.fused(tokens, before)
+        q, k, v = parts(fused)
+        turned = fs.flagsparse_paged_append(k, v, lengths, offsets, prepared=kv, q=q, cos=cos, sin=sin,
+                                            parents=parents)
+        attended = fs.flagsparse_attention_paged_tree(turned, lengths, offsets, parents=parents,
+                                                      longest=most, prepared=kv)
+        chosen = model.logits(x, attended).argmax(-1).tolist()
+        keep, at = torch.zeros(len(tokens), dtype=torch.bool), 0
+        for text, (drafted, ups) in zip(texts, trees):
+            here = 0 if drafted else None
+            while here is not None:  # down the tree as long as a child is what the model chooses
+                keep[at + here] = True
+                text.append(chosen[at + here])
+                here = next((i for i, p in enumerate(ups) if p == here and drafted[i] == text[-1]), None)
+            at += len(drafted)
+        lengths = fs.flagsparse_paged_keep(keep.to(device), lengths, offsets, prepared=kv)
+        steps += 1
+    return torch.tensor([text[len(p):len(p) + count] for text, p in zip(texts, prompts)]), steps
 
 
 def main():
@@ -152,6 +212,8 @@ def main():
     tokens, _ = generate(model, device, prompts, 12)
     for p, prompt, row in zip(patterns, prompts, tokens.tolist()):
         print("pattern", p.tolist(), "after", prompt.tolist(), "->", row)
+    tokens, steps = generate_drafted(model, device, prompts, 40)
+    print(f"40 tokens each by drafts in {steps} steps: {tokens.tolist()}")
 
 
 if __name__ == "__main__":
