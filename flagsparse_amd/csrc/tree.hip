@@ -94,9 +94,10 @@ __device__ __forceinline__ int row_mask(const TreeShape& s, const Drafted& t, co
 }
 
 // Whether the keys [begin, end) hold any that some row does not see: drafted ones, or some that a window leaves
-// deep rows only, whose depth is less than the number of them.
+// deep rows only, whose depth is less than the number of them.  Or whether a step that the end cuts, of 32 keys from
+// one before it on, reaches drafted ones: seen_keys reads the rows' masks for it.
 __device__ __forceinline__ bool some_hidden(const TreeShape& s, const Drafted& t, int begin, int end) {
-  return end > t.past || (s.window && begin < t.past + t.count - s.window);
+  return end > t.past - 32 || (s.window && begin < t.past + t.count - s.window);
 }
 
 // Which of the 32 keys from place e0 on a row sees, whose first token by its window is ``lo``; ``count`` of them

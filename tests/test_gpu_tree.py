@@ -181,6 +181,15 @@ def test_one_token_is_the_paged_call(dev):
     assert torch.isnan(got[3]).all()  # its pages hold nothing
 
 
+@pytest.mark.parametrize("heads", [2, 24, 40])
+def test_one_token_under_a_window_that_starts_anywhere(dev, heads):
+    # a piece that ends where all see its keys, in a step that is not whole; LDS holds what others left
+    x = _normal(5, 4096, 8, 128, dtype=BF).to(dev)
+    fs.flagsparse_attention_packed(x, x, x, torch.tensor([0, 4096], device=dev))
+    past = list(range(230, 790))
+    _check(dev, past, [[-1]] * len(past), 16, heads, 1, 64, BF, window=100)
+
+
 def test_what_is_not_as_it_should_be_is_nan(dev):
     past, new = [90, 40, 7], [9, 12, 5]
     trees = [_tree(n, s) for s, n in enumerate(new)]
