@@ -301,7 +301,7 @@ class PreparedPagedKV:
             table = _on_device(*_pieces(self._held, self.page_size, piece, sight), piece, self.device)
             torch.cuda.current_stream(self.device).synchronize()  # calls may come from other streams
             kept = (piece, *table, _Streams())
-            _keep(self._lists, key, kept)
+            kept = self._lists.setdefault(key, kept)  # for good: captured graphs read it
         return kept
 
 
@@ -965,7 +965,7 @@ class PreparedAttention:
             flat = torch.from_numpy(np.concatenate(lists)).to(self.device)
             torch.cuda.current_stream(self.device).synchronize()  # calls may come from other streams
             kept = (flat[:len(lists[0])], flat[len(lists[0]):], _Streams())
-            _keep(self._grouped, group, kept)
+            kept = self._grouped.setdefault(group, kept)  # for good: captured graphs read them
         return kept
 
 

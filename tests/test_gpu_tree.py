@@ -190,6 +190,17 @@ def test_one_token_under_a_window_that_starts_anywhere(dev, heads):
     _check(dev, past, [[-1]] * len(past), 16, heads, 1, 64, BF, window=100)
 
 
+def test_lists_stay_for_the_graphs_that_read_them(dev):
+    kv, _, _ = _cache(dev, [300], 16, 1, 64, BF)
+    n = torch.tensor([300], dtype=torch.int32, device=dev)
+    q = _normal(3, 4, 2, 64, dtype=BF).to(dev)
+    fs.flagsparse_attention_paged_tree(q, n, prepared=kv, window=9)
+    (first,) = kv._lists.values()
+    for window in range(10, 140):
+        fs.flagsparse_attention_paged_tree(q, n, prepared=kv, window=window)
+    assert any(kept is first for kept in kv._lists.values())
+
+
 def test_what_is_not_as_it_should_be_is_nan(dev):
     past, new = [90, 40, 7], [9, 12, 5]
     trees = [_tree(n, s) for s, n in enumerate(new)]
