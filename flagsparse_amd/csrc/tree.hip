@@ -38,6 +38,7 @@ struct Drafted {
     old = s.window ? max(past + 1 - s.window, 0) : 0;
     first = s.window ? (int)max((int64_t)past + 1 - s.window - s.sinks, (int64_t)0) : 0;
   }
+  __device__ int pieces_end(int piece) const { return last / piece + (last % piece > 0); }
 };
 
 // Rows of NaN for the tokens [from, to), those of one key head's queries.
@@ -204,7 +205,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attention_tree_kernel(
     nan_outside(s, t, tokens, b, c.batch, out, out_token, out_head, lse, head0, group, c.dim);
   const int rows = t.count * group, r0 = tile * ROWS;
   if (r0 >= rows) return;
-  const int p0 = t.first / s.piece, p1 = (t.last + s.piece - 1) / s.piece;
+  const int p0 = t.first / s.piece, p1 = t.pieces_end(s.piece);
   const int mine = p0 + pc.begin / s.piece;
   if (mine >= p1) return;
   const int begin = max(t.first, mine * s.piece);
@@ -463,7 +464,7 @@ __global__ __launch_bounds__(256, 2) void attention_tree_wide_kernel(
     nan_outside(s, t, tokens, b, c.batch, out, out_token, out_head, lse, head0, group, c.dim);
   const int rows = t.count * group, r0 = tile * ROWS;
   if (r0 >= rows) return;
-  const int p0 = t.first / s.piece, p1 = (t.last + s.piece - 1) / s.piece;
+  const int p0 = t.first / s.piece, p1 = t.pieces_end(s.piece);
   const int mine = p0 + pc.begin / s.piece;
   if (mine >= p1) return;
   const int begin = max(t.first, mine * s.piece);
@@ -646,7 +647,7 @@ __global__ __launch_bounds__(256) void attention_tree_join_kernel(
   const int i = blockIdx.x % per * 8 + (threadIdx.x >> 5), d = 4 * (threadIdx.x & 31);
   const int g = i / (s.longest * group), r = i % (s.longest * group);
   const Drafted t(s, tokens, b, lengths[b], (c.indptr[b + 1] - c.indptr[b]) * c.page_size);
-  const int p0 = t.first / s.piece, n = (t.last + s.piece - 1) / s.piece - p0;
+  const int p0 = t.first / s.piece, n = t.pieces_end(s.piece) - p0;
   if (n < 2 || g >= c.kv_heads || r >= t.count * group) return;
   const int64_t step = (int64_t)s.longest * s.heads;
   const int64_t at = first_piece[b] * step + (int64_t)g * s.longest * group + r;

@@ -1,6 +1,7 @@
 """Attention of trees of drafted tokens over a paged cache, against the formulas in 64 bits."""
 
 import copy
+import math
 import random
 
 import pytest
@@ -199,6 +200,26 @@ def test_lists_stay_for_the_graphs_that_read_them(dev):
     for window in range(10, 140):
         fs.flagsparse_attention_paged_tree(q, n, prepared=kv, window=window)
     assert any(kept is first for kept in kv._lists.values())
+
+
+def test_as_many_tokens_as_a_table_may_hold(dev):
+    # one page for all places: the softmax is that of one page, the sum of the weights is that of them all
+    page, times = 1 << 20, 2047
+    k = _normal(1, 1, page, 1, 8, dtype=BF).to(dev)
+    v = _normal(2, 1, page, 1, 8, dtype=BF).to(dev)
+    kv = fs.prepare_paged_kv(k, v, torch.tensor([0, times], device=dev), torch.zeros(times, dtype=torch.int32,
+                                                                                    device=dev))
+    q = _normal(3, 1, 2, 8, dtype=BF).to(dev)
+    n = torch.tensor([page * times], dtype=torch.int32, device=dev)
+    out, lse = fs.flagsparse_attention_paged_tree(q, n, prepared=kv, return_lse=True)
+    s = (k[0, :, 0].double() @ q[0].double().T) * 8**-0.5  # [page, heads]
+    want = torch.softmax(s, 0).T @ v[0, :, 0].double()
+    # a weight and the result are rounded to 8 bits, half a step each; sums in 32 bits are small beside it
+    bound = 2 * 2.0**-8 * (torch.softmax(s, 0).T @ v[0, :, 0].double().abs())
+    assert bool(((out[0].double() - want).abs() <= bound).all())
+    # sums in 32 bits, of all 2^18 pieces of 8192 keys one after the other, and a factor for each 8 of them: at most
+    # (2^18 + 2^15) 2^-24 of the sum; in a piece 2^9 a lane, 2^-15; weights and scores some 2^-20 more
+    assert float((lse[0].double() - (torch.logsumexp(s, 0) + math.log(times))).abs().max()) <= 2.0**-5
 
 
 def test_what_is_not_as_it_should_be_is_nan(dev):
