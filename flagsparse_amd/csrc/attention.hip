@@ -1225,7 +1225,9 @@ extern "C" int64_t fsp_attention_packed_sinks_workspace(int64_t n_k_tiles, int64
                                                         int64_t k_tokens, int64_t k_longest,
                                                         int64_t batch, int64_t window, int64_t sinks) {
   const int64_t rest = fsp_attention_packed_workspace(n_k_tiles, heads, kv_heads, dim, q_tokens, k_tokens, 0);
-  if (rest <= 0 || sinks <= 0 || batch < 0 || window < 1 || k_longest < 0) return rest;
+  if (sinks <= 0 || batch < 0 || window < 1 || k_longest < 0 || n_k_tiles < 0 || heads < 1 || kv_heads < 1 ||
+      dim < 0 || q_tokens < 0 || k_tokens < 0)
+    return rest;
   const int64_t firsts = first_keys(sinks, k_longest), rows = (firsts + kRows - 1) / kRows * kRows;
   return rest + sizeof(float) * 2 * job_slots(q_tokens, batch, window, firsts) *
                     split_heads(n_k_tiles, heads, kv_heads, false) * kv_heads * rows * dim;

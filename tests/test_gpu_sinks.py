@@ -79,6 +79,11 @@ def test_other_keys(dev, q_len, k_len):
     _both(dev, q_len, k_len, 2, 2, 128, HF, 5, 80)
 
 
+def test_no_queries(dev):
+    _both(dev, [0, 0], [9, 700], 2, 2, 64, BF, 30, 7)
+    _both(dev, [0], [100], 4, 1, 96, HF, 30, 70)
+
+
 def test_many_first_keys(dev):
     # jobs hold as many queries as there are first keys
     _both(dev, [1900, 100], [1900, 100], 2, 1, 64, BF, 50, 700)

@@ -67,6 +67,12 @@ def test_workspace_holds_the_jobs():
     assert L.fsp_attention_packed_sinks_workspace(*sizes, 600, 3, 100, 2**30) - without == 10 * rows
 
 
+def test_workspace_without_queries():
+    # two slots, two key heads in one share, 64 rows of keys and of values, 32 bits
+    assert _abi.lib().fsp_attention_packed_sinks_workspace(12, 2, 2, 64, 0, 709, 700, 2, 30, 7) == \
+        2 * 2 * 64 * 2 * 64 * 4
+
+
 def test_sinks_of():
     assert attention._sinks_of(None, 0) == 0 and attention._sinks_of(0, 0) == 0
     assert attention._sinks_of(3, 5) == 3 and attention._sinks_of(2**40, 5) == 2**31 - 1024
