@@ -1092,7 +1092,7 @@ int launch_grad_q(const Call& a, hipStream_t st) {
 // are first keys, whose tiles are workgroups enough then and whose sums would take more room than the keys.
 int64_t chunk_of(int64_t window, int64_t firsts) {
   const int64_t least = window > firsts ? window : firsts;
-  return least <= 512 ? 512 : (least + 127) / 128 * 128;
+  return least <= 512 ? 512 : least < kAttnTokensCap ? (least + 127) / 128 * 128 : kAttnTokensCap;
 }
 
 int64_t job_slots(int64_t q_tokens, int64_t batch, int64_t window, int64_t firsts) {
@@ -1269,7 +1269,7 @@ int run_backward(const Call& a, const std::string& who, void* stream) {
     const int64_t firsts = first_keys(a.sinks, a.k_longest), tiles = (firsts + kRows / 2 - 1) / (kRows / 2);
     const int64_t all = kMaxBlocks / a.heads - a.n_k_halves - 8;
     if (a.batch > kMaxBlocks || (tiles > 0 && job_slots(a.q_tokens, a.batch, a.window, firsts) > all / tiles) ||
-        a.batch > kMaxBlocks / 2 / a.kv_heads / (tiles * (kRows / 2) * (a.dim / 4) / 128 + 1))
+        a.batch > kMaxBlocks / 4 / a.kv_heads / (tiles * (kRows / 2) * (a.dim / 4) / 128 + 1))  // and of 2^31 vectors
       return set_error(FSP_EINVAL, who + ": sinks of so many sequences");
   }
   hipStream_t st = static_cast<hipStream_t>(stream);

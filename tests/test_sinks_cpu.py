@@ -43,6 +43,16 @@ def test_jobs_that_a_launch_cannot_hold():
     assert _abi.lib().fsp_attention_packed_sinks_backward(many, 2**31 - 1024, 64, 1, None) == -1
 
 
+def test_first_keys_that_numbers_cannot_hold():
+    # more than 2^30 vectors of four elements of their sums; and jobs of as many queries as there can be
+    many = base._packed(window=5, heads=1, kv_heads=1, dim=128, k_tokens=2**25 - 1024, k_longest=2**25 - 1024)
+    assert _abi.lib().fsp_attention_packed_sinks_backward(many, 2**25, 64, 1, None) == -1
+    assert b"sinks of so many" in _abi.lib().fsp_last_error()
+    sizes = (40, 8, 2, 64, 1000, 1000, 600, 3)
+    assert _abi.lib().fsp_attention_packed_sinks_workspace(*sizes, 2**31 - 1, 4) == \
+        _abi.lib().fsp_attention_packed_sinks_workspace(*sizes, 2**20, 4)
+
+
 @pytest.mark.parametrize("q_len,chunk", [([0], 512), ([5, 0, 700, 512, 513], 512), ([1] * 900, 512),
                                          ([1024, 0, 0, 3], 640)])
 def test_slots_of_jobs_are_apart(q_len, chunk):
