@@ -229,6 +229,36 @@ def raw_stream(device):
     return torch.cuda.current_stream(device).cuda_stream
 
 
+class _Elsewhere:
+    """The library with a device made the current one for each call."""
+
+    __slots__ = ("device",)
+
+    def __init__(self, device):
+        self.device = device
+
+    def __getattr__(self, name):
+        def call(*args):
+            with torch.cuda.device(self.device):
+                return getattr(lib(), name)(*args)
+        return call
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_one_device = None
+
+
+def lib_on(device):
+    """The library for launches on arrays of ``device``, whose default stream is the null one, that of
+    whatever device is current."""
+    global _one_device
+    if _one_device is None:
+        _one_device = torch.cuda.device_count() == 1
+    if _one_device or device.index is None or device.index == _current_device():
+        return lib()
+    return _Elsewhere(device)
+
+
 def caps():
     """Kernel capacities compiled into the library."""
     L = lib()

@@ -553,9 +553,9 @@ def _append(kv, head, k, v, q, res, cos, sin, token_indptr, lengths, parents):
     args = head + _APPEND_AT.pack(k.data_ptr(), v.data_ptr(), _at(q), _at(res), _at(cos), _at(sin),
                                   _at(token_indptr), lengths.data_ptr())
     if parents is None:
-        status = _abi.lib().fsp_paged_append(args, kv._on())
+        status = _abi.lib_on(kv.device).fsp_paged_append(args, kv._on())
     else:
-        status = _abi.lib().fsp_paged_append_drafts(args, parents.data_ptr(), kv._on())
+        status = _abi.lib_on(kv.device).fsp_paged_append_drafts(args, parents.data_ptr(), kv._on())
     if status:
         _abi.check(status, "fsp_paged_append")
 
@@ -630,7 +630,7 @@ def _keep_tokens(kv, into, kept, keep, token_indptr, lengths):
         args = head + into._packed() + _KEEP.pack(1, *sizes)
         into._on()
     res = torch.empty_like(like, memory_format=_CONTIGUOUS)
-    status = _abi.lib().fsp_paged_keep(args + _KEEP_AT.pack(
+    status = _abi.lib_on(kv.device).fsp_paged_keep(args + _KEEP_AT.pack(
         kv._pieces.data_ptr(), keep.data_ptr(), _at(token_indptr), lengths.data_ptr(), res.data_ptr()), stream)
     if status:
         _abi.check(status, "fsp_paged_keep")
@@ -681,7 +681,7 @@ def flagsparse_paged_copy(sources, targets, *, prepared=None, k_pages=None, v_pa
 
 
 def _copy_pages(kv, kept, sources, targets):
-    status = _abi.lib().fsp_paged_copy(kept[0], sources.data_ptr(), targets.data_ptr(), kept[1],
+    status = _abi.lib_on(kv.device).fsp_paged_copy(kept[0], sources.data_ptr(), targets.data_ptr(), kept[1],
                                        _abi.raw_stream(kv.device))
     if status:
         _abi.check(status, "fsp_paged_copy")
@@ -771,9 +771,9 @@ def _attend(kv, kept, q, res, lengths, return_lse):
     args = head + _PAGED_AT.pack(q.data_ptr(), res.data_ptr(), _at(lse), lengths.data_ptr(),
                                  _at(work), _at(counts))
     if sinks:
-        status = _abi.lib().fsp_attention_paged_sinks(args, sinks, stream)
+        status = _abi.lib_on(kv.device).fsp_attention_paged_sinks(args, sinks, stream)
     else:
-        status = _abi.lib().fsp_attention_paged(args, stream)
+        status = _abi.lib_on(kv.device).fsp_attention_paged(args, stream)
     if status:
         _abi.check(status, "fsp_attention_paged")
     return lse
@@ -904,7 +904,7 @@ def _attend_tree(kv, kept, q, res, lengths, token_indptr, parents, return_lse):
     counts = _arrivals(kv, stream, need) if need else None
     args = head + _TREE_AT.pack(q.data_ptr(), res.data_ptr(), _at(lse), lengths.data_ptr(),
                                 _at(token_indptr), _at(parents), _at(work), _at(counts))
-    status = _abi.lib().fsp_attention_tree(args, stream)
+    status = _abi.lib_on(kv.device).fsp_attention_tree(args, stream)
     if status:
         _abi.check(status, "fsp_attention_tree")
     return lse
@@ -1096,9 +1096,9 @@ def _run_forward(prepared, head, sinks, q, k, v, res, lse):
             q.data_ptr(), k.data_ptr(), v.data_ptr(), res.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, 0)
         if sinks:
             _first_tiles(prepared, q.shape[1] // k.shape[1])
-            status = _abi.lib().fsp_attention_packed_sinks(args, sinks, prepared._on())
+            status = _abi.lib_on(prepared.device).fsp_attention_packed_sinks(args, sinks, prepared._on())
         else:
-            status = _abi.lib().fsp_attention_packed(args, prepared._on())
+            status = _abi.lib_on(prepared.device).fsp_attention_packed(args, prepared._on())
         if status:
             _abi.check(status, "fsp_attention_packed")
 
@@ -1213,10 +1213,10 @@ def _run_backward(prepared, kept, rows, lse, grads):
             work.data_ptr())
         if sinks:
             _first_tiles(prepared, q.shape[1] // k.shape[1])
-            status = _abi.lib().fsp_attention_packed_sinks_backward(
+            status = _abi.lib_on(prepared.device).fsp_attention_packed_sinks_backward(
                 args, sinks, prepared._sequences.data_ptr(), prepared.batch, prepared._on())
         else:
-            status = _abi.lib().fsp_attention_packed_backward(args, prepared._on())
+            status = _abi.lib_on(prepared.device).fsp_attention_packed_backward(args, prepared._on())
         if status:
             _abi.check(status, "fsp_attention_packed_backward")
 
