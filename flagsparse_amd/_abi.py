@@ -252,6 +252,8 @@ def lib_on(device):
     """The library for launches on arrays of ``device``, whose default stream is the null one, that of
     whatever device is current."""
     global _one_device
+    if _one_device and _lib is not None:
+        return _lib
     if _one_device is None:
         _one_device = torch.cuda.device_count() == 1
     if _one_device or device.index is None or device.index == _current_device():
