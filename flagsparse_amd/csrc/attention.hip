@@ -1184,7 +1184,7 @@ int check_packed(const Call& a, const std::string& who) {
   if (a.q_tokens < 0 || a.k_tokens < 0 || a.n_q_tiles < 0 || a.n_k_tiles < 0 ||
       a.n_q_halves < 0 || a.n_k_halves < 0 || a.window < 0 || a.q_longest < 0 || a.k_longest < 0 ||
       a.q_tokens > kAttnTokensCap || a.k_tokens > kAttnTokensCap || a.window > 0x7fffffffLL ||
-      a.n_q_tiles > kMaxBlocks / a.heads || a.n_q_halves > kMaxBlocks / a.heads ||
+      a.n_q_tiles > kMaxBlocks / (a.heads / a.width()) || a.n_q_halves > kMaxBlocks / (a.heads / a.width()) ||
       a.n_k_tiles > kMaxBlocks / a.heads || a.n_k_halves > kMaxBlocks / a.heads)
     return set_error(FSP_EINVAL, who + ": size out of range");
   auto step = [&](int64_t tokens, int64_t by) {

@@ -111,3 +111,18 @@ def test_refusals_that_need_no_device():
     q = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
     with pytest.raises(ValueError):
         fs.flagsparse_attention_packed(q, q, q, torch.tensor([0, 4]), window=2, sinks=1)
+
+
+@pytest.mark.parametrize("heads,kv_heads,tokens", [(64, 8, 8_000_000), (32, 1, 4_000_000), (64, 1, 8_000_000),
+                                                   (48, 16, 8_000_000)])
+def test_tiles_of_several_heads_are_counted_as_workgroups(heads, kv_heads, tokens):
+    # a tile of fewer tokens holds as many more heads: as many tokens as without first ones, refused here only for
+    # the array that is missing
+    L = _abi.lib()
+    sizes = {"window": 5, "heads": heads, "kv_heads": kv_heads, "q_tokens": tokens, "k_tokens": tokens, "q": 0}
+    tiles, halves = (-(-tokens // L.fsp_attention_packed_sinks_tile(which, heads // kv_heads)) for which in (0, 1))
+    for n_tiles, n_halves, refusal in ((tiles, halves, b"null pointer"), (2**24, halves, b"out of range"),
+                                       (tiles, 2**24, b"out of range")):
+        args = base._packed(n_q_tiles=n_tiles, n_q_halves=n_halves, **sizes)
+        assert L.fsp_attention_packed_sinks(args, 4, None) == -1 and refusal in L.fsp_last_error()
+        assert L.fsp_attention_packed_sinks_backward(args, 4, 64, 1, None) == -1 and refusal in L.fsp_last_error()
