@@ -697,10 +697,20 @@ int64_t tile_rows(int64_t longest, int64_t group) {
   return rows <= 16 ? 16 : rows <= kWideFrom ? 32 : 128;
 }
 
+int64_t tiles_of(int64_t longest, int64_t group) {
+  const int64_t each = tile_rows(longest, group);
+  return (longest * group + each - 1) / each;
+}
+
+// Whether another launch joins the pieces.
+bool joined(const fsp_attention_tree_args& a) {
+  return a.n_pieces > a.cache.batch &&
+         !(a.arrived && tile_rows(a.longest, a.heads / a.cache.kv_heads) == 16);
+}
+
 template <typename T, typename Kernel, typename... More>
 int launch_tree(const fsp_attention_tree_args& a, Kernel kernel, hipStream_t st, More... more) {
-  const int64_t group = a.heads / a.cache.kv_heads, each = tile_rows(a.longest, group);
-  const int64_t tiles = (a.longest * group + each - 1) / each;
+  const int64_t tiles = tiles_of(a.longest, a.heads / a.cache.kv_heads);
   const TreeShape s{(int)a.heads,    (int)a.window,  (int)a.sinks, (int)a.piece,  (int)a.n_pieces,
                     (int)a.n_tokens, (int)a.longest, (int)tiles,   (float)a.scale};
   float* part_o = static_cast<float*>(a.workspace);
@@ -712,7 +722,7 @@ int launch_tree(const fsp_attention_tree_args& a, Kernel kernel, hipStream_t st,
                      a.out_head, a.lse, a.lengths, a.token_indptr, a.parents, part_o, part_ml,
                      more...);
   if (int rc = check_hip(hipGetLastError(), "attention_tree_kernel launch")) return rc;
-  if (a.n_pieces == a.cache.batch || (a.arrived && each == 16)) return FSP_OK;
+  if (!joined(a)) return FSP_OK;
   hipLaunchKernelGGL((attention_tree_join_kernel<T>),
                      dim3((unsigned)(a.cache.batch * ((a.longest * a.heads + 7) / 8))), dim3(256), 0, st,
                      cache_of(a.cache), s, a.first_piece, static_cast<T*>(a.out), a.out_token, a.out_head,
@@ -796,8 +806,8 @@ extern "C" int fsp_attention_tree(const fsp_attention_tree_args* args, void* str
   if (a.cache.batch == 0 || a.longest == 0)
     return set_error(FSP_EINVAL, "fsp_attention_tree: tokens of no sequence");
   const int64_t rows = a.longest * a.heads, group = a.heads / a.cache.kv_heads;
-  if (a.cache.batch > kMaxBlocks / ((rows + 7) / 8) ||
-      a.n_pieces > kMaxBlocks / (a.cache.kv_heads * ((a.longest * group + 15) / 16)))
+  if (a.n_pieces > kMaxBlocks / (a.cache.kv_heads * tiles_of(a.longest, group)) ||
+      (joined(a) && a.cache.batch > kMaxBlocks / ((rows + 7) / 8)))
     return set_error(FSP_EINVAL, "fsp_attention_tree: pieces out of range");
   if (!a.q || !a.out || !a.lengths || !a.pieces ||
       (a.n_pieces > a.cache.batch && (!a.workspace || !a.first_piece)))

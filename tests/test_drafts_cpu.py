@@ -160,3 +160,24 @@ def test_refusals_that_need_no_device():
         fs.flagsparse_paged_copy(n, n, prepared=q)
     with pytest.raises(ValueError):
         fs.flagsparse_paged_copy(n, n, k_pages=q[None], v_pages=q[None])
+
+
+@pytest.mark.parametrize("kw,refusal", [
+    ({"heads": 32, "longest": 256, "n_pieces": 262_143}, b"null pointer"),  # 2 x 32 tiles of 128 rows
+    ({"heads": 32, "longest": 256, "n_pieces": 262_144}, b"out of range"),
+    ({"heads": 4, "longest": 8, "n_pieces": 8_388_607}, b"null pointer"),  # 2 x 1 of 16
+    ({"heads": 4, "longest": 8, "n_pieces": 8_388_608}, b"out of range")])
+def test_pieces_of_a_launch(kw, refusal):
+    # as many workgroups as a launch holds: a piece has one for every tile of rows and key head
+    L = _abi.lib()
+    assert L.fsp_attention_tree(base._cache() + _tree(tokens=8, q=0, **kw), None) == -1
+    assert refusal in L.fsp_last_error()
+
+
+@pytest.mark.parametrize("kw,refusal", [
+    ({"n_pieces": 9000}, b"null pointer"),  # one each: nothing is joined
+    ({"n_pieces": 9001}, b"out of range")])
+def test_sequences_of_the_launch_that_joins(kw, refusal):
+    L = _abi.lib()
+    args = base._cache(batch=9000) + _tree(heads=64, longest=256, tokens=9000, q=0, **kw)
+    assert L.fsp_attention_tree(args, None) == -1 and refusal in L.fsp_last_error()
