@@ -18,7 +18,7 @@ FSP_F64 = 1
 FSP_BF16 = 2
 FSP_F16 = 3
 FSP_CUT_PIECES = 2
-ABI_VERSION = 21
+ABI_VERSION = 22
 
 _lib = None
 
@@ -133,6 +133,8 @@ SIGNATURES = {
     "fsp_attention_tree_counts": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "fsp_attention_tree_workspace": (_i64, [_i64, _i64, _i64, _i64]),
     "fsp_attention_tree": (_i32, [_p, _p]),
+    "fsp_attention_tree_by_tokens_workspace": (_i64, [_i64, _i64, _i64, _i64]),
+    "fsp_attention_tree_by_tokens": (_i32, [_p, _i64, _p]),
     "fsp_attention_packed_tile": (_i64, [_i32]),
     "fsp_attention_packed_workspace": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i32]),
     "fsp_attention_packed": (_i32, [_p, _p]),

@@ -793,7 +793,9 @@ def flagsparse_attention_paged_tree(q, lengths, token_indptr=None, *, parents=No
     (None: each follows the one before it).  A token sees the text, the drafted tokens on its way up
     the tree, and itself.  ``window`` and ``sinks`` go by positions, as in flagsparse_attention_paged: a
     drafted token's is the text's length plus the tokens before it on its way.  ``longest``: no
-    sequence has more drafted tokens, at most 256 (by default 256; a smaller one saves work).
+    sequence has more drafted tokens, at most 256 (by default 256; a smaller one saves work: each sequence has
+    workgroups for so many).  Sums of long texts' pieces take tokens * heads * (dim + 2) * 4 bytes for every 256 to
+    8192 tokens that the pages of one sequence hold, or less.
 
     Returns [tokens, heads, dim], with the float32 log-sum-exp [tokens, heads] if ``return_lse``; neither is
     differentiable.  With ``prepared`` nothing is waited for, so indices are not checked: rows of a
@@ -854,16 +856,20 @@ def flagsparse_attention_paged_tree(q, lengths, token_indptr=None, *, parents=No
         # tiles of an average sequence: those of the longest trees are few
         tiles = min(-(-group * longest // of), 1 + group * tokens // (kv.batch * of))
         piece, pieces, firsts, longest_list, marked = kv._list(sight, kv.kv_heads * tiles, 512, 8192, of)
-        n_pieces, need, room = pieces.shape[0], 0, None
+        n_pieces, need, room, by_tokens = pieces.shape[0], 0, None, 0
         if n_pieces > kv.batch:
             need = int(_abi.lib().fsp_attention_tree_counts(n_pieces, longest_list, kv.batch, kv.kv_heads,
                                                             group, longest))
-            room = _like((n_pieces * longest * heads * (kv.dim + 2),), torch.float32, dev)
+            size = int(_abi.lib().fsp_attention_tree_workspace(n_pieces, heads, kv.dim, longest))
+            less = int(_abi.lib().fsp_attention_tree_by_tokens_workspace(longest_list, tokens, heads, kv.dim))
+            if less < size:
+                by_tokens, size = longest_list, less
+            room = _like((size,), torch.uint8, dev)
         head = kv._packed() + _TREE.pack(
             pieces.data_ptr(), firsts.data_ptr(), n_pieces, piece, heads, past, factor, first, tokens,
             longest, *_steps(rows), *_steps(res))
         kept = (head, _like(q.shape, dt, dev), _like(q.shape[:2], torch.float32, dev), room, need,
-                (pieces, firsts), marked)
+                by_tokens, (pieces, firsts), marked)
         lse = _attend_tree(kv, kept, rows, res, n, token_indptr, parents, return_lse)
         if key is not None and all(x is y for x, y in zip((rows, n, token_indptr, parents), given)):
             _keep(kv._calls, key, kept)
@@ -895,7 +901,7 @@ def _check_drafts(kv, lengths, token_indptr, parents, tokens, longest):
 
 def _attend_tree(kv, kept, q, res, lengths, token_indptr, parents, return_lse):
     """The launch; returns the log-sum-exp, if asked for."""
-    head, _, like_lse, room, need, lists, marked = kept
+    head, _, like_lse, room, need, by_tokens, lists, marked = kept
     lse = torch.empty_like(like_lse, memory_format=_CONTIGUOUS) if return_lse else None
     stream = kv._on()
     if stream not in marked.seen:
@@ -904,7 +910,10 @@ def _attend_tree(kv, kept, q, res, lengths, token_indptr, parents, return_lse):
     counts = _arrivals(kv, stream, need) if need else None
     args = head + _TREE_AT.pack(q.data_ptr(), res.data_ptr(), _at(lse), lengths.data_ptr(),
                                 _at(token_indptr), _at(parents), _at(work), _at(counts))
-    status = _abi.lib_on(kv.device).fsp_attention_tree(args, stream)
+    if by_tokens:
+        status = _abi.lib_on(kv.device).fsp_attention_tree_by_tokens(args, by_tokens, stream)
+    else:
+        status = _abi.lib_on(kv.device).fsp_attention_tree(args, stream)
     if status:
         _abi.check(status, "fsp_attention_tree")
     return lse

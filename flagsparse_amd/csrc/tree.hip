@@ -20,6 +20,7 @@ constexpr int kTableKeys = 1024;  // keys whose places LDS holds at a time
 struct TreeShape {
   int heads, window, sinks, piece, n_pieces, n_tokens, longest, tiles;
   float scale;
+  int by_tokens;  // how partial sums lie: see Sums
 };
 
 // A sequence's drafted tokens and what of its keys any of them sees: the places [first, last), where
@@ -39,6 +40,19 @@ struct Drafted {
     first = s.window ? (int)max((int64_t)past + 1 - s.window - s.sinks, (int64_t)0) : 0;
   }
   __device__ int pieces_end(int piece) const { return last / piece + (last % piece > 0); }
+};
+
+// Where the partial sums of a sequence's rows for one key head start, and how many rows one piece's lie behind those
+// of the piece before.  By pieces, ``longest`` tokens' rows each, or by tokens, all rows of the call for each piece
+// that a sequence has at most: the caller takes the smaller.  Where most sequences have fewer drafted tokens than
+// ``longest``, or no bound is given, that is the second: 64 sequences with room for 131072 tokens and 8 drafted
+// ones each, 32 heads of 128, 136 MB instead of 4.4 GB (pieces of 8192).
+struct Sums {
+  int64_t first, step;
+  __device__ Sums(const TreeShape& s, const Drafted& t, int slot, int g, int group)
+      : first(s.by_tokens ? (int64_t)t.begin * s.heads + (int64_t)g * t.count * group
+                          : (int64_t)slot * s.longest * s.heads + (int64_t)g * s.longest * group),
+        step((int64_t)(s.by_tokens ? s.n_tokens : s.longest) * s.heads) {}
 };
 
 // Rows of NaN for the tokens [from, to), those of one key head's queries.
@@ -184,13 +198,13 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attention_tree_kernel(
   typedef T VE __attribute__((ext_vector_type(E)));
   constexpr int CH = DP / 8, KL = DP / 16;
   __shared__ int64_t s_k[kTableKeys], s_v[kTableKeys];
-  typedef float Sums[16][DP + 4];
-  static_assert(sizeof(Sums) >= 64 * DP, "");
-  __shared__ __attribute__((aligned(16))) char s_raw[W * sizeof(Sums)];
+  typedef float Rows[16][DP + 4];
+  static_assert(sizeof(Rows) >= 64 * DP, "");
+  __shared__ __attribute__((aligned(16))) char s_raw[W * sizeof(Rows)];
   __shared__ f32x2 s_ml[W][16];
   __shared__ uint32_t s_mask[ROWS][11];
   __shared__ int s_depth[ROWS], s_up[kDrafts];
-  Sums* s_o = reinterpret_cast<Sums*>(s_raw);
+  Rows* s_o = reinterpret_cast<Rows*>(s_raw);
   const int group = s.heads / c.kv_heads;
   int piece, g, tile;
   piece_and_head(blockIdx.x, s.n_pieces, c.kv_heads * s.tiles, piece, tile);
@@ -251,7 +265,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attention_tree_kernel(
           kb + s_k[min(j + 64 / CH * i + k_row, most)] +
           (EXACT || 8 * k_chunk < c.dim ? 8 * k_chunk : 0)));
   };
-  char* s_rows = s_raw + wave * sizeof(Sums);
+  char* s_rows = s_raw + wave * sizeof(Rows);
   const int ve = E * col < c.dim ? E * col : 0;
   auto load_v = [&](int j, int most) {
 #pragma unroll
@@ -367,8 +381,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attention_tree_kernel(
 
   // join the waves, 16 rows at a time
   const bool split = p1 - p0 > 1;
-  const int64_t step = (int64_t)s.longest * s.heads;  // rows of a piece
-  const int64_t slot = (pc.slot + mine - p0) * step + (int64_t)g * s.longest * group;
+  const Sums sums(s, t, pc.slot, g, group);
+  const int64_t slot = sums.first + (mine - p0) * sums.step;
   auto to_out = [&](int r, int d, f32x4 y, float most, float total) {
     const int64_t token = t.begin + (r0 + r) / group;
     const int head = head0 + (r0 + r) % group;
@@ -421,8 +435,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attention_tree_kernel(
   if constexpr (RT > 1) return;
   if (!split || !arrived) return;  // without counts, another launch joins them
   if (last_to_arrive(arrived + ((int64_t)b * c.kv_heads + g) * s.tiles + tile, p1 - p0))
-    join_tile<T, DP>(part_o, part_ml, slot - (mine - p0) * step + r0, step, p1 - p0, min(ROWS, rows - r0),
-                     c.dim, to_out);
+    join_tile<T, DP>(part_o, part_ml, sums.first + r0, sums.step, p1 - p0, min(ROWS, rows - r0), c.dim, to_out);
 }
 
 // Rows past a head's dim are read from here.
@@ -626,7 +639,8 @@ __global__ __launch_bounds__(256, 2) void attention_tree_wide_kernel(
     store_rows<T, NT>(out + token * out_token + head * out_head, o, sum == 0 ? 0.0f : 1.0f / sum, c.dim, half);
     return;
   }
-  const int64_t at = (int64_t)(pc.slot + mine - p0) * s.longest * s.heads + (int64_t)g * s.longest * group + row;
+  const Sums sums(s, t, pc.slot, g, group);
+  const int64_t at = sums.first + (mine - p0) * sums.step + row;
   store_rows<float, NT>(part_o + at * c.dim, o, 1.0f, c.dim, half);
   if (half == 0)
     *reinterpret_cast<f32x2*>(part_ml + 2 * at) = f32x2{top == -INFINITY ? -INFINITY : top * cs, sum};
@@ -649,8 +663,8 @@ __global__ __launch_bounds__(256) void attention_tree_join_kernel(
   const Drafted t(s, tokens, b, lengths[b], (c.indptr[b + 1] - c.indptr[b]) * c.page_size);
   const int p0 = t.first / s.piece, n = t.pieces_end(s.piece) - p0;
   if (n < 2 || g >= c.kv_heads || r >= t.count * group) return;
-  const int64_t step = (int64_t)s.longest * s.heads;
-  const int64_t at = first_piece[b] * step + (int64_t)g * s.longest * group + r;
+  const Sums sums(s, t, first_piece[b], g, group);
+  const int64_t step = sums.step, at = sums.first + r;
   const f32x2* ml = part_ml + at;
   const float* o = part_o + at * c.dim + (d < c.dim ? d : 0);
   float most = -INFINITY, total = 0;
@@ -697,24 +711,30 @@ int64_t tile_rows(int64_t longest, int64_t group) {
   return rows <= 16 ? 16 : rows <= kWideFrom ? 32 : 128;
 }
 
+// A call's arguments, with the most pieces of a sequence where partial sums lie by tokens (0: by pieces).
+struct TreeCall : fsp_attention_tree_args {
+  int64_t most = 0;
+};
+
 int64_t tiles_of(int64_t longest, int64_t group) {
   const int64_t each = tile_rows(longest, group);
   return (longest * group + each - 1) / each;
 }
 
 // Whether another launch joins the pieces.
-bool joined(const fsp_attention_tree_args& a) {
+bool joined(const TreeCall& a) {
   return a.n_pieces > a.cache.batch &&
          !(a.arrived && tile_rows(a.longest, a.heads / a.cache.kv_heads) == 16);
 }
 
 template <typename T, typename Kernel, typename... More>
-int launch_tree(const fsp_attention_tree_args& a, Kernel kernel, hipStream_t st, More... more) {
+int launch_tree(const TreeCall& a, Kernel kernel, hipStream_t st, More... more) {
   const int64_t tiles = tiles_of(a.longest, a.heads / a.cache.kv_heads);
   const TreeShape s{(int)a.heads,    (int)a.window,  (int)a.sinks, (int)a.piece,  (int)a.n_pieces,
-                    (int)a.n_tokens, (int)a.longest, (int)tiles,   (float)a.scale};
+                    (int)a.n_tokens, (int)a.longest, (int)tiles,   (float)a.scale,
+                    a.most > 0};
   float* part_o = static_cast<float*>(a.workspace);
-  float* part_ml = part_o + a.n_pieces * a.longest * a.heads * a.cache.dim;
+  float* part_ml = part_o + (a.most ? a.most * a.n_tokens : a.n_pieces * a.longest) * a.heads * a.cache.dim;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(a.n_pieces * a.cache.kv_heads * tiles)), dim3(256), 0, st,
                      cache_of(a.cache), s, reinterpret_cast<const Piece*>(a.pieces),
                      static_cast<const T*>(a.cache.k_pages), static_cast<const T*>(a.cache.v_pages),
@@ -731,7 +751,7 @@ int launch_tree(const fsp_attention_tree_args& a, Kernel kernel, hipStream_t st,
 }
 
 template <typename T, int DP, bool EXACT, bool NT>
-int launch_tree_rows(const fsp_attention_tree_args& a, hipStream_t st) {
+int launch_tree_rows(const TreeCall& a, hipStream_t st) {
   unsigned* arrived = static_cast<unsigned*>(a.arrived);
   return tile_rows(a.longest, a.heads / a.cache.kv_heads) == 16
              ? launch_tree<T>(a, attention_tree_kernel<T, DP, EXACT, NT, 1>, st, arrived)
@@ -739,7 +759,7 @@ int launch_tree_rows(const fsp_attention_tree_args& a, hipStream_t st) {
 }
 
 template <typename T, int DP, bool EXACT>
-int launch_tree_nt(const fsp_attention_tree_args& a, hipStream_t st) {
+int launch_tree_nt(const TreeCall& a, hipStream_t st) {
   const int64_t bytes = a.cache.table_len * a.cache.page_size * a.cache.kv_heads * a.cache.dim * 4;
   return bytes > (256 << 20)
              ? launch_tree_rows<T, DP, EXACT, true>(a, st)
@@ -747,7 +767,7 @@ int launch_tree_nt(const fsp_attention_tree_args& a, hipStream_t st) {
 }
 
 template <typename T>
-int launch_tree_dim(const fsp_attention_tree_args& a, hipStream_t st) {
+int launch_tree_dim(const TreeCall& a, hipStream_t st) {
   const int64_t dim = a.cache.dim;
   if (tile_rows(a.longest, a.heads / a.cache.kv_heads) == 128)
     return dim < 64     ? launch_tree<T>(a, attention_tree_wide_kernel<T, 64, false>, st)
@@ -784,37 +804,57 @@ extern "C" int64_t fsp_attention_tree_workspace(int64_t n_pieces, int64_t heads,
   return n_pieces * longest * heads * (dim + 2) * (int64_t)sizeof(float);
 }
 
-extern "C" int fsp_attention_tree(const fsp_attention_tree_args* args, void* stream) {
-  if (!args) return set_error(FSP_EINVAL, "fsp_attention_tree: null arguments");
-  const fsp_attention_tree_args& a = *args;
-  if (int rc = check_cache(a.cache, "fsp_attention_tree")) return rc;
+extern "C" int64_t fsp_attention_tree_by_tokens_workspace(int64_t most, int64_t n_tokens, int64_t heads,
+                                                          int64_t dim) {
+  if (most < 0 || n_tokens < 0 || heads < 0 || dim < 0) return 0;
+  return most * n_tokens * heads * (dim + 2) * (int64_t)sizeof(float);
+}
+
+namespace {
+
+int run_tree(const TreeCall& a, const std::string& who, void* stream) {
+  if (int rc = check_cache(a.cache, who)) return rc;
   if (a.heads < 1 || a.heads % a.cache.kv_heads || a.heads > 0xffff)
-    return set_error(FSP_EINVAL, "fsp_attention_tree: heads must be a multiple of kv_heads");
+    return set_error(FSP_EINVAL, who + ": heads must be a multiple of kv_heads");
   if (!isfinite((float)a.scale))
-    return set_error(FSP_EINVAL, "fsp_attention_tree: scale must be finite in 32 bits");
+    return set_error(FSP_EINVAL, who + ": scale must be finite in 32 bits");
   if (a.window < 0 || a.window > kAttnTokensCap || a.sinks < 0 || a.sinks > kAttnTokensCap ||
       (a.sinks && !a.window))
-    return set_error(FSP_EINVAL, "fsp_attention_tree: window, or sinks without one");
+    return set_error(FSP_EINVAL, who + ": window, or sinks without one");
   if (a.piece < 128 || a.piece > (1 << 20) || a.piece % 128)
-    return set_error(FSP_EINVAL, "fsp_attention_tree: piece must be a multiple of 128 up to 2^20");
+    return set_error(FSP_EINVAL, who + ": piece must be a multiple of 128 up to 2^20");
   if (a.n_tokens < 0 || a.n_tokens > kAttnTokensCap || a.longest < 0 || a.longest > kDrafts ||
       a.n_pieces < a.cache.batch || a.n_pieces > 0x7fffffffLL)
-    return set_error(FSP_EINVAL, "fsp_attention_tree: size out of range");
+    return set_error(FSP_EINVAL, who + ": size out of range");
   if (!a.token_indptr && a.n_tokens != a.longest * a.cache.batch)
-    return set_error(FSP_EINVAL, "fsp_attention_tree: longest tokens per sequence without token_indptr");
+    return set_error(FSP_EINVAL, who + ": longest tokens per sequence without token_indptr");
   if (a.n_tokens == 0) return FSP_OK;
   if (a.cache.batch == 0 || a.longest == 0)
-    return set_error(FSP_EINVAL, "fsp_attention_tree: tokens of no sequence");
+    return set_error(FSP_EINVAL, who + ": tokens of no sequence");
   const int64_t rows = a.longest * a.heads, group = a.heads / a.cache.kv_heads;
   if (a.n_pieces > kMaxBlocks / (a.cache.kv_heads * tiles_of(a.longest, group)) ||
       (joined(a) && a.cache.batch > kMaxBlocks / ((rows + 7) / 8)))
-    return set_error(FSP_EINVAL, "fsp_attention_tree: pieces out of range");
+    return set_error(FSP_EINVAL, who + ": pieces out of range");
   if (!a.q || !a.out || !a.lengths || !a.pieces ||
       (a.n_pieces > a.cache.batch && (!a.workspace || !a.first_piece)))
-    return set_error(FSP_EINVAL, "fsp_attention_tree: null pointer");
+    return set_error(FSP_EINVAL, who + ": null pointer");
   if (!aligned16(a.q, a.q_token, a.q_head) || !aligned16(a.out, a.out_token, a.out_head) ||
       reinterpret_cast<uintptr_t>(a.workspace) % 16)
-    return set_error(FSP_EINVAL, "fsp_attention_tree: rows must be 16-byte aligned");
+    return set_error(FSP_EINVAL, who + ": rows must be 16-byte aligned");
   hipStream_t st = static_cast<hipStream_t>(stream);
   return a.cache.dtype == FSP_BF16 ? launch_tree_dim<bf16>(a, st) : launch_tree_dim<f16>(a, st);
+}
+
+}  // namespace
+
+extern "C" int fsp_attention_tree(const fsp_attention_tree_args* args, void* stream) {
+  if (!args) return set_error(FSP_EINVAL, "fsp_attention_tree: null arguments");
+  return run_tree({*args}, "fsp_attention_tree", stream);
+}
+
+extern "C" int fsp_attention_tree_by_tokens(const fsp_attention_tree_args* args, int64_t most, void* stream) {
+  if (!args) return set_error(FSP_EINVAL, "fsp_attention_tree_by_tokens: null arguments");
+  if (most < 1 || most > args->n_pieces)
+    return set_error(FSP_EINVAL, "fsp_attention_tree_by_tokens: the pieces of one sequence");
+  return run_tree({*args, most}, "fsp_attention_tree_by_tokens", stream);
 }

@@ -847,6 +847,10 @@ int64_t fsp_attention_tree_counts(int64_t n_pieces, int64_t most, int64_t batch,
 int64_t fsp_attention_tree_rows(int64_t group, int64_t longest);
 int64_t fsp_attention_tree_workspace(int64_t n_pieces, int64_t heads, int64_t dim, int64_t longest);
 int fsp_attention_tree(const struct fsp_attention_tree_args* args, void* stream);
+/* The same with a workspace of fsp_attention_tree_by_tokens_workspace() bytes, for all rows of the call as often as
+ * one sequence has pieces at most: less where most sequences have fewer drafted tokens than `longest`. */
+int64_t fsp_attention_tree_by_tokens_workspace(int64_t most, int64_t n_tokens, int64_t heads, int64_t dim);
+int fsp_attention_tree_by_tokens(const struct fsp_attention_tree_args* args, int64_t most, void* stream);
 
 /*
  * Attention over packed sequences: sequence b's queries are tokens

@@ -181,3 +181,16 @@ def test_sequences_of_the_launch_that_joins(kw, refusal):
     L = _abi.lib()
     args = base._cache(batch=9000) + _tree(heads=64, longest=256, tokens=9000, q=0, **kw)
     assert L.fsp_attention_tree(args, None) == -1 and refusal in L.fsp_last_error()
+
+
+def test_partial_sums_by_tokens():
+    L = _abi.lib()
+    # 64 sequences with room for 131072 tokens, 8 drafted ones each, no bound of them: rows of 128 + 2 numbers
+    assert L.fsp_attention_tree_by_tokens_workspace(16, 512, 32, 128) == 16 * 512 * 32 * 130 * 4
+    assert L.fsp_attention_tree_workspace(1024, 32, 128, 256) == 32 * 16 * 512 * 32 * 130 * 4
+    assert L.fsp_attention_tree_by_tokens_workspace(-1, 512, 32, 128) == 0
+    assert L.fsp_attention_tree_by_tokens_workspace(2000, 2**31 - 1024, 64, 128) == 2000 * (2**31 - 1024) * 64 * 520
+    for most in (0, -1, 4):
+        assert L.fsp_attention_tree_by_tokens(base._cache() + _tree(), most, None) == -1
+    assert L.fsp_attention_tree_by_tokens(None, 1, None) == -1
+    assert L.fsp_attention_tree_by_tokens(base._cache() + _tree(q=0), 2, None) == -1

@@ -418,3 +418,45 @@ def test_no_tokens(dev):
     out = fs.flagsparse_attention_paged_tree(q, n[:0], torch.zeros(1, dtype=torch.int32, device=dev),
                                              prepared=empty)
     assert torch.isnan(out).all()
+
+
+def _long_cache(dev, batch, pages, heads, dim, dtype):
+    """A cache of ``batch`` sequences with room for pages * 64 tokens each, all in the same pages."""
+    k, v = (_normal(s, pages, 64, heads, dim, dtype=dtype).to(dev) for s in (1, 2))
+    table = torch.arange(pages, dtype=torch.int32, device=dev).repeat(batch)
+    return fs.prepare_paged_kv(k, v, torch.arange(0, batch * pages + 1, pages, device=dev), table)
+
+
+def test_memory_goes_by_the_drafted_tokens(dev):
+    # no bound of the drafted tokens, room for long texts: what a call takes goes by the tokens that there are
+    batch, heads, dim, each = 64, 16, 64, 6
+    kv = _long_cache(dev, batch, 512, 4, dim, BF)
+    n = torch.full((batch,), 900, dtype=torch.int32, device=dev)
+    q, tokens = _normal(3, batch * each, heads, dim, dtype=BF).to(dev), _indptr([each] * batch, dev)
+    parents = torch.full((batch * each,), -1, dtype=torch.int32, device=dev)
+    want = fs.flagsparse_attention_paged_tree(q, n, tokens, parents=parents, longest=each, prepared=kv)
+    assert fs.flagsparse_attention_paged_tree(q, n, tokens, parents=parents, prepared=kv).shape == q.shape
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats(dev)
+    before = torch.cuda.memory_allocated(dev)
+    out = fs.flagsparse_attention_paged_tree(q, n, tokens, parents=parents, prepared=kv)
+    torch.cuda.synchronize()
+    taken = torch.cuda.max_memory_allocated(dev) - before
+    # pieces of 256 tokens at least, the output beside them
+    assert taken <= 512 * 64 // 256 * batch * each * heads * (dim + 2) * 4 + 2 * q.numel() + 4096, taken
+    # two orders of the same sums, weights rounded to 8 bits by other maxima in each
+    s = float(kv.v_pages.float().abs().max())
+    assert float((out.float() - want.float()).abs().max()) <= 4 * 2.0**-8 * s
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 4, 64), (8, 2, 128), (23, 1, 80)])
+def test_partial_sums_of_ragged_trees(dev, heads, kv_heads, dim):
+    # many pieces, drafts of very different sizes, with a bound of them and without: sums by pieces and by tokens
+    past, new = [9000, 30, 4000, 0, 700], [3, 90, 0, 5, 1]
+    trees = [_tree(n, s) for s, n in enumerate(new)]
+    _check(dev, past, trees, 64, heads, kv_heads, dim, BF)
+    _check(dev, past, trees, 64, heads, kv_heads, dim, HF, longest=90, window=3000, sinks=7)
+    past, new = [6000, 5000, 300], [4, 4, 4]
+    trees = [_tree(n, s) for s, n in enumerate(new)]
+    _check(dev, past, trees, 64, heads, kv_heads, dim, BF, longest=4)
+    _check(dev, past, trees, 64, heads, kv_heads, dim, HF, room=60)
