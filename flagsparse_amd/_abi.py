@@ -142,6 +142,7 @@ SIGNATURES = {
     "fsp_attention_packed_sinks_tile": (_i64, [_i32, _i64]),
     "fsp_attention_packed_sinks": (_i32, [_p, _i64, _p]),
     "fsp_attention_packed_sinks_backward": (_i32, [_p, _i64, _p, _i64, _p]),
+    "fsp_attention_packed_sinks_chunk": (_i64, [_i64, _i64, _i64]),
     "fsp_attention_packed_sinks_workspace": (_i64, [_i64] * 10),
 }
 

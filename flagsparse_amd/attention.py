@@ -1196,9 +1196,10 @@ def _backward(prepared, grad_out, q, k, v, out, lse, causal, window, sinks, scal
     head = _pack(prepared, *rows[1:4], causal, window, scale, rows[4], (rows[0], *grads), sinks)
     sizes = (prepared._tiles[2, causal].shape[0], q.shape[1], k.shape[1], q.shape[2], q.shape[0],
              k.shape[0])
-    if sinks:
+    q_longest, k_longest = prepared._longest
+    if sinks and q_longest > _abi.lib().fsp_attention_packed_sinks_chunk(window, sinks, k_longest):
         room = int(_abi.lib().fsp_attention_packed_sinks_workspace(
-            *sizes, prepared._longest[1], prepared.batch, window, sinks))
+            *sizes, k_longest, prepared.batch, window, sinks))
     else:
         room = int(_abi.lib().fsp_attention_packed_workspace(*sizes, causal and not window))
     kept = (head, sinks, _like((room,), torch.uint8, q.device),

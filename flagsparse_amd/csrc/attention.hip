@@ -599,15 +599,20 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, DP <= 64 ? 3 : 2) void attenti
 }
 
 // Where first keys stay visible to all later queries, their tiles would have many times the others' work
-// under a window (four of 4096 under 512: eight times): with SINKS they go to jobs of ``chunk`` queries each,
-// whose sums another launch adds in their order.  Slot q_begin / chunk + b + i is the job of the queries
-// [i * chunk, (i + 1) * chunk) of sequence b: no two are the same, and there are at most
-// q_tokens / chunk + batch.  A slot holds, for each share of the heads, key head and first key, the
-// values' sums and then the keys'.
+// under a window (four of 4096 under 512: eight times): with SINKS those of sequences with more than ``chunk``
+// queries go to jobs of ``chunk`` queries each, whose sums another launch adds in their order.  Slot first_slot + i
+// is the job of the queries [i * chunk, (i + 1) * chunk) of sequence b: no two are the same, also where the first
+// slot is 2 * q_begin / chunk (``twice``), as x > 1 chunks are at most 2 * x slots, whole numbers of both; there
+// are at most q_tokens / chunk + batch, and so 2 * (q_tokens / chunk + 1).  A slot holds, for each share of the
+// heads, key head and first key, the values' sums and then the keys'.
 struct Jobs {
   const Tile* sequences;  // of each its q_begin, nq, k_begin, nk
   float* sums;
   int batch, chunk, slots, tiles, blocks;  // tiles of first keys a sequence; workgroups of all jobs
+  bool twice;
+  __device__ int first_slot(int q_begin, int b) const {
+    return twice ? (int)(2u * q_begin / (uint32_t)chunk) : q_begin / chunk + b;
+  }
 };
 
 template <int ROWS>
@@ -628,19 +633,19 @@ __device__ __forceinline__ bool job_of(const Jobs& jobs, const Shape& s, int spl
   if (at / ROWS >= jobs.tiles) return false;
   int b = 0;  // the last sequence whose slots start at or before this one, 64 at a look
   for (int i = 0; i < jobs.batch; i += kWave) {
-    const bool in = i + lane < jobs.batch &&
-                    jobs.sequences[min(i + lane, jobs.batch - 1)].q_begin / jobs.chunk + i + lane <= slot;
+    const int of = min(i + lane, jobs.batch - 1);
+    const bool in = i + lane < jobs.batch && jobs.first_slot(jobs.sequences[of].q_begin, of) <= slot;
     const int count = __popcll(__ballot(in));
     b += count;
     if (count < kWave) break;
   }
   b = __builtin_amdgcn_readfirstlane(b - 1);
   t = jobs.sequences[b];
-  const int64_t begin = (int64_t)(slot - t.q_begin / jobs.chunk - b) * jobs.chunk;
+  const int64_t begin = (int64_t)(slot - jobs.first_slot(t.q_begin, b)) * jobs.chunk;
   t.first = t.k_begin + at;
   t.at = at;
   t.rows = min(ROWS, t.nk - at);
-  if (begin >= t.nq || at >= min(t.nk, s.sinks)) return false;
+  if (t.nq <= jobs.chunk || begin >= t.nq || at >= min(t.nk, s.sinks)) return false;
   from = (int)begin;
   to = (int)min(begin + jobs.chunk, (int64_t)t.nq);
   return true;
@@ -674,7 +679,7 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_grad_kv_kern
   } else {
     tile_and_head(blockIdx.x - (SINKS ? jobs.blocks : 0), n_tiles, s.kv_heads * split, tile, g);
     t = tiles[tile];
-    if (SINKS && t.at < s.sinks) return;
+    if (SINKS && t.at < s.sinks && t.nq > jobs.chunk) return;
   }
   const int share = g % split;  // of the group's heads
   g /= split;
@@ -903,7 +908,7 @@ __global__ __launch_bounds__(256) void attention_grad_kv_sum_kernel(
   *reinterpret_cast<V4<T>*>(to) = __builtin_convertvector(y, V4<T>);
 }
 
-// The same for tiles of first keys, as the sums of their jobs, chunk by chunk and in each the shares of the
+// The same where first keys have jobs: theirs as the sums of these, chunk by chunk and in each the shares of the
 // heads, by workgroups of their own, [0, of_jobs): a thread to four elements, a workgroup's of one sequence
 // and key head.  The others add the shares of all other keys, whose sequence each thread looks up: one launch of
 // 5.7 us for 6 sequences up to 1501, 4 key heads of 96, where two took 4.3 and 4.2 and the gap between them.
@@ -926,7 +931,7 @@ __global__ __launch_bounds__(256) void attention_grad_sinks_sum_kernel(
       else end = mid;
     }
     const Tile q = jobs.sequences[b];
-    if ((t - q.k_begin) / ROWS * ROWS < s.sinks) return;
+    if ((t - q.k_begin) / ROWS * ROWS < s.sinks && q.nq > jobs.chunk) return;
     const float* from = sums + (keys ? split * each : 0) + at;
     f32x4 y = *reinterpret_cast<const f32x4*>(from);
     for (int p = 1; p < split; ++p) y += *reinterpret_cast<const f32x4*>(from + p * each);
@@ -943,7 +948,7 @@ __global__ __launch_bounds__(256) void attention_grad_sinks_sum_kernel(
   const bool keys = of >= jobs.tiles * ROWS;
   const int row = keys ? of - jobs.tiles * ROWS : of;
   // the rows of the tiles that have a first key
-  if (row >= t.nk || row / ROWS * ROWS >= s.sinks) return;
+  if (t.nq <= jobs.chunk || row >= t.nk || row / ROWS * ROWS >= s.sinks) return;
   int lot, hit;
   seen_of(s, t, row / ROWS * ROWS, lot, hit);
   f32x4 y{};
@@ -951,7 +956,7 @@ __global__ __launch_bounds__(256) void attention_grad_sinks_sum_kernel(
     for (int c = lot / jobs.chunk; c <= (t.nq - 1) / jobs.chunk; ++c)
       for (int p = 0; p < split; ++p)
         y += *reinterpret_cast<const f32x4*>(
-            job_sums<ROWS>(jobs, s, split, t.q_begin / jobs.chunk + b + c, p, g, of) + d);
+            job_sums<ROWS>(jobs, s, split, jobs.first_slot(t.q_begin, b) + c, p, g, of) + d);
   const int64_t at = t.k_begin + row;
   T* to = keys ? dk + at * dk_token + g * dk_head : dv + at * dv_token + g * dv_head;
   *reinterpret_cast<V4<T>*>(to + d) = __builtin_convertvector(y, V4<T>);
@@ -1095,8 +1100,12 @@ int64_t chunk_of(int64_t window, int64_t firsts) {
   return least <= 512 ? 512 : least < kAttnTokensCap ? (least + 127) / 128 * 128 : kAttnTokensCap;
 }
 
-int64_t job_slots(int64_t q_tokens, int64_t batch, int64_t window, int64_t firsts) {
-  return q_tokens / chunk_of(window, firsts) + batch;
+// By twice the chunks where most sequences have no job: 20000 of 64 tokens beside one of 1000, 8 key heads of 128, jobs
+// of 512 queries take 2.6 GB instead of 11.8.
+bool slots_twice(int64_t q_tokens, int64_t batch, int64_t chunk) { return q_tokens / chunk + 2 < batch; }
+
+int64_t job_slots(int64_t q_tokens, int64_t batch, int64_t chunk) {
+  return slots_twice(q_tokens, batch, chunk) ? 2 * (q_tokens / chunk + 1) : q_tokens / chunk + batch;
 }
 
 // Elements of one share's sums over all keys, and of the jobs' of the first keys in tiles of ``rows``.
@@ -1106,14 +1115,20 @@ int64_t share_floats(int split, int64_t kv_heads, int64_t k_tokens, int64_t dim)
 
 int64_t first_keys(int64_t sinks, int64_t k_longest) { return sinks < k_longest ? sinks : k_longest; }
 
+// Whether any sequence has more queries than one job.
+bool has_jobs(const Call& a) {
+  return a.sinks && a.q_longest > chunk_of(a.window, first_keys(a.sinks, a.k_longest));
+}
+
 Jobs jobs_of(const Call& a, int split, int rows, float* sums) {
   Jobs j;
-  const int64_t firsts = first_keys(a.sinks, a.k_longest);
+  const int64_t firsts = first_keys(a.sinks, a.k_longest), chunk = chunk_of(a.window, firsts);
   j.sequences = reinterpret_cast<const Tile*>(a.sequences);
   j.sums = sums + share_floats(split, a.kv_heads, a.k_tokens, a.dim);
   j.batch = (int)a.batch;
-  j.chunk = (int)chunk_of(a.window, firsts);
-  j.slots = (int)job_slots(a.q_tokens, a.batch, a.window, firsts);
+  j.chunk = (int)chunk;
+  j.slots = has_jobs(a) ? (int)job_slots(a.q_tokens, a.batch, chunk) : 0;
+  j.twice = slots_twice(a.q_tokens, a.batch, chunk);
   j.tiles = (int)((firsts + rows - 1) / rows);
   j.blocks = (int)((j.tiles * (int64_t)j.slots * a.kv_heads * split + 7) / 8 * 8);
   return j;
@@ -1136,7 +1151,7 @@ int launch_grad_kv(const Call& a, int split, hipStream_t st) {
                      a.k_tokens, jobs);
   if (int rc = check_hip(hipGetLastError(), "attention_grad_kv_kernel launch")) return rc;
   const int64_t quads = split > 1 ? a.kv_heads * a.k_tokens * a.dim / 2 : 0;
-  if constexpr (SINKS) {
+  if (SINKS && jobs.slots > 0) {
     const int64_t of_jobs = (2 * jobs.tiles * 32 * BLOCKS * (a.dim / 4) + 255) / 256 * a.kv_heads * a.batch;
     hipLaunchKernelGGL((attention_grad_sinks_sum_kernel<T, 32 * BLOCKS>),
                        dim3((unsigned)(of_jobs + (quads + 255) / 256)), dim3(256), 0, st, shape_of(a), split,
@@ -1229,8 +1244,12 @@ extern "C" int64_t fsp_attention_packed_sinks_workspace(int64_t n_k_tiles, int64
       dim < 0 || q_tokens < 0 || k_tokens < 0)
     return rest;
   const int64_t firsts = first_keys(sinks, k_longest), rows = (firsts + kRows - 1) / kRows * kRows;
-  return rest + sizeof(float) * 2 * job_slots(q_tokens, batch, window, firsts) *
+  return rest + sizeof(float) * 2 * job_slots(q_tokens, batch, chunk_of(window, firsts)) *
                     split_heads(n_k_tiles, heads, kv_heads, false) * kv_heads * rows * dim;
+}
+
+extern "C" int64_t fsp_attention_packed_sinks_chunk(int64_t window, int64_t sinks, int64_t k_longest) {
+  return window < 1 || sinks < 1 || k_longest < 0 ? 0 : chunk_of(window, first_keys(sinks, k_longest));
 }
 
 extern "C" int64_t fsp_attention_packed_tile(int which) {
@@ -1251,7 +1270,7 @@ int run_forward(const Call& a, const std::string& who, void* stream) {
 int run_backward(const Call& a, const std::string& who, void* stream) {
   if (int rc = check_packed(a, who)) return rc;
   // without queries, and with one share of the heads, there is nothing to keep
-  const bool work = a.n_k_tiles > 0 && (a.sinks || fsp_attention_packed_workspace(
+  const bool work = a.n_k_tiles > 0 && (has_jobs(a) || fsp_attention_packed_workspace(
       a.n_k_tiles, a.heads, a.kv_heads, a.dim, a.q_tokens, a.k_tokens, a.causal && !a.window) > 0);
   if ((a.n_q_tiles > 0 && (!a.grad_out || !a.grad_q || !a.workspace)) ||
       (a.n_k_tiles > 0 && (!a.grad_k || !a.grad_v)) || (work && !a.workspace))
@@ -1267,9 +1286,10 @@ int run_backward(const Call& a, const std::string& who, void* stream) {
     if (a.batch < 1 || !a.sequences) return set_error(FSP_EINVAL, who + ": sequences");
     // tiles of 32 keys, the most jobs
     const int64_t firsts = first_keys(a.sinks, a.k_longest), tiles = (firsts + kRows / 2 - 1) / (kRows / 2);
-    const int64_t all = kMaxBlocks / a.heads - a.n_k_halves - 8;
-    if (a.batch > kMaxBlocks || (tiles > 0 && job_slots(a.q_tokens, a.batch, a.window, firsts) > all / tiles) ||
-        a.batch > kMaxBlocks / 4 / a.kv_heads / (tiles * (kRows / 2) * (a.dim / 4) / 128 + 1))  // and of 2^31 vectors
+    const int64_t all = kMaxBlocks / a.heads - a.n_k_halves - 8, batch = has_jobs(a) ? a.batch : 1;
+    if (a.batch > 0x7fffffffLL ||
+        (tiles > 0 && job_slots(a.q_tokens, batch, chunk_of(a.window, firsts)) > all / tiles) ||
+        batch > kMaxBlocks / 4 / a.kv_heads / (tiles * (kRows / 2) * (a.dim / 4) / 128 + 1))  // and of 2^31 vectors
       return set_error(FSP_EINVAL, who + ": sinks of so many sequences");
   }
   hipStream_t st = static_cast<hipStream_t>(stream);

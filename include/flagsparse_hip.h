@@ -904,12 +904,14 @@ int fsp_attention_packed_backward(const struct fsp_attention_packed_args* args, 
  * a window hides the keys sinks <= j <= i + nk - nq - window.  q_tiles and q_halves cover the queries in
  * fsp_attention_packed_sinks_tile(0 and 1, heads / kv_heads) rows.  The backward pass takes the sequences
  * as tiles, [batch, 8] int32 {0, 0, 0, q begin, q count, k begin, k count, 0} in their order,
- * and a workspace of fsp_attention_packed_sinks_workspace() bytes.
+ * and a workspace of fsp_attention_packed_sinks_workspace() bytes, or where q_longest is no more than
+ * fsp_attention_packed_sinks_chunk() one as without sinks, fsp_attention_packed_workspace() with uneven = 0.
  */
 int64_t fsp_attention_packed_sinks_tile(int which, int64_t group);
 int fsp_attention_packed_sinks(const struct fsp_attention_packed_args* args, int64_t sinks, void* stream);
 int fsp_attention_packed_sinks_backward(const struct fsp_attention_packed_args* args, int64_t sinks,
                                         const int32_t* sequences, int64_t batch, void* stream);
+int64_t fsp_attention_packed_sinks_chunk(int64_t window, int64_t sinks, int64_t k_longest);
 int64_t fsp_attention_packed_sinks_workspace(int64_t n_k_tiles, int64_t heads, int64_t kv_heads,
                                              int64_t dim, int64_t q_tokens, int64_t k_tokens,
                                              int64_t k_longest, int64_t batch, int64_t window,

@@ -372,3 +372,34 @@ def test_tokens_through_a_cache_are_the_packed_rows(dev):
     want = ref.packed(q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1), [n, n], [n, n], True, 11,
                       d**-0.5, sinks=3)
     ref.check("out", torch.stack(outs, 1).flatten(0, 1), want["out"])
+
+
+def test_memory_of_short_sequences(dev):
+    # gradients of many short sequences take what the call without first tokens does, and of those with jobs
+    # room by their queries
+    def taken(lengths, sinks):
+        q, k, v, g = _inputs(dev, lengths, lengths, 4, 2, 64, BF)
+        kw = {"prepared": fs.prepare_attention_packed(_indptr(lengths, dev)), "window": 20, "sinks": sinks}
+        out, lse = fs.flagsparse_attention_packed(q, k, v, return_lse=True, **kw)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats(dev)
+        before = torch.cuda.memory_allocated(dev)
+        fs.flagsparse_attention_packed_backward(g, q, k, v, out, lse, **kw)
+        torch.cuda.synchronize()
+        return torch.cuda.max_memory_allocated(dev) - before
+
+    # the allocator gives a block whole where less than 1 MiB of it would be left: three gradients and a workspace
+    more = 4 << 20
+    short, slot = [30] * 3000, 2 * 64 * 64 * 4 * 2  # 64 keys, keys and values, of 64 numbers, two key heads
+    assert taken(short, 4) <= taken(short, 0) + more
+    mixed = short + [900]
+    assert taken(mixed, 4) <= taken(mixed, 0) + 2 * (sum(mixed) // 512 + 1) * slot + more
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(2, 2), (12, 2)])
+def test_short_sequences_beside_those_with_jobs(dev, heads, kv_heads):
+    # those with as many queries as one job take their first keys' gradients in the tiles themselves, shares and all
+    for lengths in ([3] * 90 + [700, 0, 512, 513] + [40] * 30 + [1100], [512, 300], [0, 5, 0, 513, 0]):
+        _both(dev, lengths, lengths, heads, kv_heads, 64, BF, 30, 6)
+    _both(dev, [40, 600, 0, 90], [300, 650, 70, 9], heads, kv_heads, 96, HF, 25, 100)
+    _both(dev, [300] * 9, [300] * 9, heads, kv_heads, 128, HF, 200, 130)

@@ -442,8 +442,9 @@ def test_memory_goes_by_the_drafted_tokens(dev):
     out = fs.flagsparse_attention_paged_tree(q, n, tokens, parents=parents, prepared=kv)
     torch.cuda.synchronize()
     taken = torch.cuda.max_memory_allocated(dev) - before
-    # pieces of 256 tokens at least, the output beside them
-    assert taken <= 512 * 64 // 256 * batch * each * heads * (dim + 2) * 4 + 2 * q.numel() + 4096, taken
+    # pieces of 256 tokens at least, the output beside them; the allocator gives a block whole where less than 1 MiB
+    # of it would be left
+    assert taken <= 512 * 64 // 256 * batch * each * heads * (dim + 2) * 4 + 2 * q.numel() + (2 << 20), taken
     # two orders of the same sums, weights rounded to 8 bits by other maxima in each
     s = float(kv.v_pages.float().abs().max())
     assert float((out.float() - want.float()).abs().max()) <= 4 * 2.0**-8 * s

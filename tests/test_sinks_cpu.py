@@ -126,3 +126,39 @@ def test_tiles_of_several_heads_are_counted_as_workgroups(heads, kv_heads, token
         args = base._packed(n_q_tiles=n_tiles, n_q_halves=n_halves, **sizes)
         assert L.fsp_attention_packed_sinks(args, 4, None) == -1 and refusal in L.fsp_last_error()
         assert L.fsp_attention_packed_sinks_backward(args, 4, 64, 1, None) == -1 and refusal in L.fsp_last_error()
+
+
+@pytest.mark.parametrize("q_len,chunk", [([5, 0, 700, 512, 513], 512), ([1] * 900 + [513] + [2] * 900, 512),
+                                         ([513] * 40, 512), ([1024, 0, 0, 641, 3, 640, 2000], 640),
+                                         ([2**30, 2**30 - 2000, 976], 512), ([0, 0], 512), ([511, 1, 513], 512)])
+def test_slots_by_twice_the_chunks_are_apart(q_len, chunk):
+    # slot 2 * q_begin / chunk + i for the i-th chunk of a sequence of more than one, no more than twice
+    # q_tokens / chunk + 1; the last sequence whose first slot is no later than a job's is the job's
+    begin = [int(n) for n in np.cumsum(q_len) - q_len]
+    first = [2 * q // chunk for q in begin]
+    taken = []
+    for b, (q, n) in enumerate(zip(begin, q_len)):
+        for i in list(range(-(-n // chunk)))[:3] + [max(0, -(-n // chunk) - 1)] if n > chunk else ():
+            assert max(x for x in range(len(first)) if first[x] <= first[b] + i) == b
+        if n > chunk:
+            taken.append((first[b], first[b] + -(-n // chunk)))
+    assert all(a[1] <= b[0] for a, b in zip(taken, taken[1:]))
+    assert not taken or taken[-1][1] <= 2 * (sum(q_len) // chunk + 1)
+
+
+def test_workspace_of_short_sequences():
+    L = _abi.lib()
+    # 20000 sequences of 64 tokens have no job: the workspace of the call without first ones
+    sizes = (20000, 32, 8, 128, 1_280_000, 1_280_000)
+    assert L.fsp_attention_packed_sinks_chunk(32, 4, 64) == 512
+    assert L.fsp_attention_packed_sinks_chunk(700, 4, 64) == 768 and L.fsp_attention_packed_sinks_chunk(0, 4, 64) == 0
+    assert L.fsp_attention_packed_sinks_chunk(32, 900, 2000) == 1024
+    # with one of 1000 beside them slots go by the queries, not by the sequences
+    rows = L.fsp_attention_packed_sinks_workspace(*sizes, 1000, 20001, 32, 4) - \
+        L.fsp_attention_packed_workspace(*sizes, 0)
+    assert rows == 2 * (1_280_000 // 512 + 1) * 8 * 2 * 64 * 128 * 4
+    # the library asks for no more: 58254 sequences were the most
+    args = dict(window=32, heads=32, kv_heads=8, dim=128, q_tokens=10**7, k_tokens=10**7, q_longest=64, k_longest=64,
+                go=0)
+    assert L.fsp_attention_packed_sinks_backward(base._packed(**args), 4, 64, 10**6, None) == -1
+    assert b"null pointer" in L.fsp_last_error()
