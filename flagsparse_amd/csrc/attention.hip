@@ -611,7 +611,7 @@ struct Jobs {
   int batch, chunk, slots, tiles, blocks;  // tiles of first keys a sequence; workgroups of all jobs
   bool twice;
   __device__ int first_slot(int q_begin, int b) const {
-    return twice ? (int)(2u * q_begin / (uint32_t)chunk) : q_begin / chunk + b;
+    return (int)(((uint32_t)q_begin << (twice ? 1 : 0)) / (uint32_t)chunk) + (twice ? 0 : b);
   }
 };
 
@@ -952,11 +952,12 @@ __global__ __launch_bounds__(256) void attention_grad_sinks_sum_kernel(
   int lot, hit;
   seen_of(s, t, row / ROWS * ROWS, lot, hit);
   f32x4 y{};
+  const int first = jobs.first_slot(t.q_begin, b);
+  const int from = (uint32_t)lot / (uint32_t)jobs.chunk, last = (uint32_t)(t.nq - 1) / (uint32_t)jobs.chunk;
   if (lot < t.nq)
-    for (int c = lot / jobs.chunk; c <= (t.nq - 1) / jobs.chunk; ++c)
+    for (int c = from; c <= last; ++c)
       for (int p = 0; p < split; ++p)
-        y += *reinterpret_cast<const f32x4*>(
-            job_sums<ROWS>(jobs, s, split, jobs.first_slot(t.q_begin, b) + c, p, g, of) + d);
+        y += *reinterpret_cast<const f32x4*>(job_sums<ROWS>(jobs, s, split, first + c, p, g, of) + d);
   const int64_t at = t.k_begin + row;
   T* to = keys ? dk + at * dk_token + g * dk_head : dv + at * dv_token + g * dv_head;
   *reinterpret_cast<V4<T>*>(to + d) = __builtin_convertvector(y, V4<T>);
