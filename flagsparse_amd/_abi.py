@@ -122,6 +122,7 @@ SIGNATURES = {
     "fsp_paged_append": (_i32, [_p, _p]),
     "fsp_paged_append_drafts": (_i32, [_p, _p, _p]),
     "fsp_paged_keep": (_i32, [_p, _p]),
+    "fsp_paged_keep_counted": (_i32, [_p, _p, _p, _p]),
     "fsp_paged_copy": (_i32, [_p, _p, _p, _i64, _p]),
     "fsp_attention_paged_counts": (_i64, [_i64, _i64, _i64, _i64, _i64]),
     "fsp_attention_paged_piece": (_i64, [_i64, _i64]),

@@ -48,6 +48,12 @@ _PACKED, _PACKED_AT = struct.Struct("10qd24q"), struct.Struct("10q")
 _KEEP, _KEEP_AT = struct.Struct("5q"), struct.Struct("5q")
 _TREE, _TREE_AT = struct.Struct("6qd7q"), struct.Struct("8q")
 
+# Where a text may have more marks than so many, they are counted by pieces before it is kept into other pages, by two
+# more launches.  Without and with that, half of the tokens kept, us: 16 texts of 8192, 8 heads of 128 120 / 124, 16 of
+# 16384 224 / 226, 8 of 32768 236 / 226, 4 of 131072 600 / 430; one head of 64, a text of 16384 12 / 19, of 32768 15 / 19,
+# 8 of 16384 26 / 21, one of 131072 79 / 22, of 2^20 3482 / 112.
+_COUNTED_FROM = 16384
+
 # A prepared object keeps the first part for each layout of arrays that it has checked, so that the
 # next call with such arrays is a look-up and a launch.  Of a cache it holds the pages' addresses, which
 # the look-up goes by too: their storage is the caller's, and may move.
@@ -610,7 +616,10 @@ def flagsparse_paged_keep(keep, lengths, token_indptr=None, *, prepared=None, k_
         _check_drafts(kv, n, token_indptr, None, tokens, each if token_indptr is None else tokens)
     keep = keep.contiguous()
     head, sizes = kv._packed(), (tokens, each, kv._pieces.shape[0], kv._piece)
-    kept = (head, sizes, head + head + _KEEP.pack(0, *sizes), _like((kv.batch,), torch.int32, dev))
+    counts = None  # of the pieces and the sequences
+    if min(tokens, kv.room) > _COUNTED_FROM:
+        counts = _like((kv._pieces.shape[0] + kv.batch,), torch.int32, dev)
+    kept = (head, sizes, head + head + _KEEP.pack(0, *sizes), _like((kv.batch,), torch.int32, dev), counts)
     res = _keep_tokens(kv, into, kept, keep, token_indptr, n)
     if key is not None and all(x is y for x, y in zip((keep, lengths, token_indptr), given)):
         _keep(kv._calls, key, kept)
@@ -620,7 +629,7 @@ def flagsparse_paged_keep(keep, lengths, token_indptr=None, *, prepared=None, k_
 def _keep_tokens(kv, into, kept, keep, token_indptr, lengths):
     """The launch; returns the new lengths.  What ``into`` holds is looked up by every call: it is an
     argument, not a part of the prepared cache."""
-    head, sizes, args, like = kept
+    head, sizes, args, like, counts = kept
     stream = kv._on()
     if into is not None:
         if into.device != kv.device or into.dtype != kv.dtype:
@@ -630,8 +639,13 @@ def _keep_tokens(kv, into, kept, keep, token_indptr, lengths):
         args = head + into._packed() + _KEEP.pack(1, *sizes)
         into._on()
     res = torch.empty_like(like, memory_format=_CONTIGUOUS)
-    status = _abi.lib_on(kv.device).fsp_paged_keep(args + _KEEP_AT.pack(
-        kv._pieces.data_ptr(), keep.data_ptr(), _at(token_indptr), lengths.data_ptr(), res.data_ptr()), stream)
+    args += _KEEP_AT.pack(kv._pieces.data_ptr(), keep.data_ptr(), _at(token_indptr), lengths.data_ptr(),
+                          res.data_ptr())
+    if into is None or counts is None:
+        status = _abi.lib_on(kv.device).fsp_paged_keep(args, stream)
+    else:
+        work = torch.empty_like(counts, memory_format=_CONTIGUOUS)
+        status = _abi.lib_on(kv.device).fsp_paged_keep_counted(args, kv._first.data_ptr(), work.data_ptr(), stream)
     if status:
         _abi.check(status, "fsp_paged_keep")
     return res

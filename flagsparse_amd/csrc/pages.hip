@@ -105,18 +105,78 @@ __global__ __launch_bounds__(kThreads) void paged_keep_kernel(
   if (which == 0 && threadIdx.x == 0) kept[b] = m.ok ? m.past + stay : -1;
 }
 
+// How many marks of a sequence's places [from, to), which are not all marked ones, stay: the same in all threads.
+__device__ __forceinline__ int kept_in(const uint8_t* marks, int past, int from, int to) {
+  __shared__ int s_count[kThreads / kWave];
+  int count = 0;
+  for (int pos = from + (int)threadIdx.x; pos < to; pos += kThreads) count += pos < past || marks[pos - past] != 0;
+#pragma unroll
+  for (int x = 1; x < kWave; x *= 2) count += __shfl_xor(count, x);
+  if ((threadIdx.x & 63) == 0) s_count[threadIdx.x >> 6] = count;
+  __syncthreads();
+  return s_count[0] + s_count[1] + s_count[2] + s_count[3];
+}
+
+// How many tokens of each piece stay: counts[the piece's place among those of its sequence, after the ones before].
+__global__ __launch_bounds__(kThreads) void paged_keep_count_kernel(
+    KeepShape s, const Piece* __restrict__ pieces, int piece_size, const uint8_t* __restrict__ keep,
+    const int32_t* __restrict__ tokens, const int32_t* __restrict__ lengths, int32_t* __restrict__ counts) {
+  const Piece pc = pieces[blockIdx.x];
+  const Marked m(tokens, s.each, s.n_tokens, pc.seq, lengths[pc.seq], pc.room);
+  const int64_t end = min((int64_t)pc.begin + piece_size, (int64_t)m.past + m.count);
+  const int count = kept_in(keep + m.begin, m.past, pc.begin, (int)end);
+  if (threadIdx.x == 0) counts[pc.slot + pc.begin / piece_size] = count;
+}
+
+// Each piece's count becomes what stays before it; totals[b]: what stays of sequence b.  A workgroup to a sequence.
+__global__ __launch_bounds__(kThreads) void paged_keep_before_kernel(
+    Cache c, int piece_size, const int32_t* __restrict__ first_piece, const int32_t* __restrict__ lengths,
+    int32_t* __restrict__ counts, int32_t* __restrict__ totals) {
+  __shared__ int s_sum[kThreads / kWave];
+  const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int room = (c.indptr[b + 1] - c.indptr[b]) * c.page_size;
+  const int length = min(max(lengths[b], 0), room);
+  const int n = length / piece_size + (length % piece_size > 0);
+  int32_t* of = counts + first_piece[b];
+  int before = 0;
+  for (int i0 = 0; i0 < n; i0 += kThreads) {
+    const int i = i0 + (int)threadIdx.x, own = i < n ? of[i] : 0;
+    int sum = own;
+#pragma unroll
+    for (int x = 1; x < kWave; x *= 2) {
+      const int other = __shfl_up(sum, x);
+      if (lane >= x) sum += other;
+    }
+    if (lane == 63) s_sum[wave] = sum;
+    __syncthreads();
+    int here = before;
+#pragma unroll
+    for (int w = 0; w < kThreads / kWave; ++w) {
+      if (w < wave) here += s_sum[w];
+      before += s_sum[w];
+    }
+    if (i < n) of[i] = here + sum - own;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) totals[b] = before;
+}
+
 // Into other pages: a workgroup takes kSpan of a sequence's tokens, all heads of their keys and values.  How many
-// tokens stay before them, and of all, it counts itself, four marks to a word.  Bound by memory: half of 16
-// sequences of 8192, 8 heads of 128, 537 MB in 110 to 124 us, 4.3 to 4.9 TB/s, where a plain copy has 4.7 to 4.9.  A
-// workgroup to a head of 1024 tokens, whose rows of 256 bytes lie apart, took 155 us.
+// tokens stay before them, and of all, it counts itself, four marks to a word; or, COUNTED, has two launches before
+// it count by pieces, as what all workgroups count grows with the square of the marks.  Bound by memory where heads
+// are large: half of 16 sequences of 8192, 8 heads of 128, 537 MB in 110 to 124 us, 4.3 to 4.9 TB/s, of 4 of 131072
+// 2147 MB in 430 us, 5.0 TB/s, where a plain copy has 4.7 to 4.9; one of 2^20 tokens, one head of 64, 268 MB in 112 us:
+// a workgroup moves 16 KB after its chain of loads.  A workgroup to a head of 1024 tokens, whose rows of 256 bytes
+// lie apart, took 155 us for the first.
 constexpr int kSpan = kWave;
 
-template <typename T>
+template <typename T, bool COUNTED>
 __global__ __launch_bounds__(kThreads) void paged_keep_into_kernel(
     Cache c, KeepShape s, const Piece* __restrict__ pieces, int piece_size, const T* __restrict__ k_pages,
     const T* __restrict__ v_pages, T* __restrict__ to_k, T* __restrict__ to_v,
     const uint8_t* __restrict__ keep, const int32_t* __restrict__ tokens,
-    const int32_t* __restrict__ lengths, int32_t* __restrict__ kept) {
+    const int32_t* __restrict__ lengths, int32_t* __restrict__ kept, const int32_t* __restrict__ counts,
+    const int32_t* __restrict__ totals) {
   constexpr int U = 8;
   __shared__ int64_t s_from[2][kSpan], s_to[2][kSpan];  // where keys and values lie, and go
   __shared__ int s_before[4], s_all[4], s_n;
@@ -128,8 +188,12 @@ __global__ __launch_bounds__(kThreads) void paged_keep_into_kernel(
   if (at >= length && at > 0) return;
 
   const uint8_t* marks = keep + m.begin;
-  int before = 0, all = 0;
-  {
+  int before = 0, all = 0;  // marks that stay
+  if constexpr (COUNTED) {
+    const int here = kept_in(marks, m.past, pc.begin, min(at, length));
+    before = counts[pc.slot + pc.begin / piece_size] + here - min(at, m.past);
+    all = m.ok ? totals[b] - m.past : 0;
+  } else {
     // whole words of the array that the marks lie in, those of others masked
     const uintptr_t from = reinterpret_cast<uintptr_t>(marks);
     const uint32_t* words = reinterpret_cast<const uint32_t*>(from & ~uintptr_t(3));
@@ -244,8 +308,14 @@ __global__ __launch_bounds__(kThreads) void paged_copy_kernel(
   }
 }
 
+// A call's arguments, with the places of counts by pieces, or none.
+struct KeepCall : fsp_paged_keep_args {
+  const int32_t* first_piece = nullptr;
+  int32_t* counts = nullptr;
+};
+
 template <typename T>
-int launch_keep(const fsp_paged_keep_args& a, hipStream_t st) {
+int launch_keep(const KeepCall& a, hipStream_t st) {
   const fsp_paged_cache& to = a.into;
   const KeepShape s{(int)a.n_tokens, (int)a.each, to.k_page, to.k_slot,       to.k_head,       to.v_page,
                     to.v_slot,       to.v_head,   to.page_indptr, to.page_indices, (int)to.page_size};
@@ -255,11 +325,22 @@ int launch_keep(const fsp_paged_keep_args& a, hipStream_t st) {
                        static_cast<T*>(a.cache.v_pages), a.keep, a.token_indptr, a.lengths, a.kept);
     return check_hip(hipGetLastError(), "paged_keep_kernel launch");
   }
-  hipLaunchKernelGGL((paged_keep_into_kernel<T>), dim3((unsigned)(a.n_pieces * (a.piece / kSpan))),
-                     dim3(kThreads), 0, st, cache_of(a.cache), s, reinterpret_cast<const Piece*>(a.pieces),
-                     (int)a.piece, static_cast<const T*>(a.cache.k_pages),
+  const Piece* pieces = reinterpret_cast<const Piece*>(a.pieces);
+  int32_t* totals = nullptr;
+  if (a.counts) {
+    totals = a.counts + a.n_pieces;
+    hipLaunchKernelGGL(paged_keep_count_kernel, dim3((unsigned)a.n_pieces), dim3(kThreads), 0, st, s, pieces,
+                       (int)a.piece, a.keep, a.token_indptr, a.lengths, a.counts);
+    if (int rc = check_hip(hipGetLastError(), "paged_keep_count_kernel launch")) return rc;
+    hipLaunchKernelGGL(paged_keep_before_kernel, dim3((unsigned)a.cache.batch), dim3(kThreads), 0, st,
+                       cache_of(a.cache), (int)a.piece, a.first_piece, a.lengths, a.counts, totals);
+    if (int rc = check_hip(hipGetLastError(), "paged_keep_before_kernel launch")) return rc;
+  }
+  hipLaunchKernelGGL((a.counts ? paged_keep_into_kernel<T, true> : paged_keep_into_kernel<T, false>),
+                     dim3((unsigned)(a.n_pieces * (a.piece / kSpan))), dim3(kThreads), 0, st, cache_of(a.cache),
+                     s, pieces, (int)a.piece, static_cast<const T*>(a.cache.k_pages),
                      static_cast<const T*>(a.cache.v_pages), static_cast<T*>(to.k_pages),
-                     static_cast<T*>(to.v_pages), a.keep, a.token_indptr, a.lengths, a.kept);
+                     static_cast<T*>(to.v_pages), a.keep, a.token_indptr, a.lengths, a.kept, a.counts, totals);
   return check_hip(hipGetLastError(), "paged_keep_into_kernel launch");
 }
 
@@ -280,31 +361,47 @@ int launch_copy(const fsp_paged_cache& c, const int32_t* sources, const int32_t*
 
 using namespace fsp;
 
-extern "C" int fsp_paged_keep(const fsp_paged_keep_args* args, void* stream) {
-  if (!args) return set_error(FSP_EINVAL, "fsp_paged_keep: null arguments");
-  const fsp_paged_keep_args& a = *args;
-  if (int rc = check_cache(a.cache, "fsp_paged_keep")) return rc;
+namespace {
+
+int run_keep(const KeepCall& a, const std::string& who, void* stream) {
+  if (int rc = check_cache(a.cache, who)) return rc;
   if (a.n_tokens < 0 || a.n_tokens > kAttnTokensCap || a.each < 0 ||
       a.cache.batch > kMaxBlocks / (2 * a.cache.kv_heads))
-    return set_error(FSP_EINVAL, "fsp_paged_keep: size out of range");
+    return set_error(FSP_EINVAL, who + ": size out of range");
   if (a.cache.batch == 0) return FSP_OK;
   if (!a.token_indptr && (a.each > a.n_tokens / a.cache.batch || a.each * a.cache.batch != a.n_tokens))
-    return set_error(FSP_EINVAL, "fsp_paged_keep: each tokens per sequence without token_indptr");
+    return set_error(FSP_EINVAL, who + ": each tokens per sequence without token_indptr");
   if ((a.n_tokens > 0 && !a.keep) || !a.lengths || !a.kept)
-    return set_error(FSP_EINVAL, "fsp_paged_keep: null pointer");
+    return set_error(FSP_EINVAL, who + ": null pointer");
   if (a.other) {
-    if (int rc = check_cache(a.into, "fsp_paged_keep")) return rc;
+    if (int rc = check_cache(a.into, who)) return rc;
     if (a.into.dtype != a.cache.dtype || a.into.kv_heads != a.cache.kv_heads || a.into.dim != a.cache.dim ||
         a.into.batch != a.cache.batch)
-      return set_error(FSP_EINVAL, "fsp_paged_keep: the caches differ in type, heads, dim or sequences");
+      return set_error(FSP_EINVAL, who + ": the caches differ in type, heads, dim or sequences");
     if (a.piece < 128 || a.piece > kList || a.piece % 128 || a.n_pieces < a.cache.batch || !a.pieces ||
         a.n_pieces > kMaxBlocks / (a.piece / kSpan) ||
         a.cache.kv_heads * (a.cache.dim / 8) > 0x7fffffff / kSpan)
-      return set_error(FSP_EINVAL, "fsp_paged_keep: pieces");
+      return set_error(FSP_EINVAL, who + ": pieces");
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
   // rows are moved as they are: one kernel for both types of 16 bits
   return launch_keep<f16>(a, st);
+}
+
+}  // namespace
+
+extern "C" int fsp_paged_keep(const fsp_paged_keep_args* args, void* stream) {
+  if (!args) return set_error(FSP_EINVAL, "fsp_paged_keep: null arguments");
+  return run_keep({*args}, "fsp_paged_keep", stream);
+}
+
+extern "C" int fsp_paged_keep_counted(const fsp_paged_keep_args* args, const int32_t* first_piece, int32_t* counts,
+                                      void* stream) {
+  if (!args) return set_error(FSP_EINVAL, "fsp_paged_keep_counted: null arguments");
+  if (!args->other) return set_error(FSP_EINVAL, "fsp_paged_keep_counted: in place nothing is counted");
+  if (args->cache.batch > 0 && (!first_piece || !counts))
+    return set_error(FSP_EINVAL, "fsp_paged_keep_counted: null pointer");
+  return run_keep({*args, first_piece, counts}, "fsp_paged_keep_counted", stream);
 }
 
 extern "C" int fsp_paged_copy(const fsp_paged_cache* cache, const int32_t* sources, const int32_t* targets,

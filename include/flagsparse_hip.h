@@ -754,6 +754,11 @@ struct fsp_paged_keep_args {
   int32_t* kept;
 };
 int fsp_paged_keep(const struct fsp_paged_keep_args* args, void* stream);
+/* The same into other pages for long texts, whose marks are counted by pieces first (what fsp_paged_keep counts grows
+ * with the square of a sequence's marks): first_piece [batch] as for fsp_attention_paged, counts [n_pieces + batch]
+ * int32, in any state. */
+int fsp_paged_keep_counted(const struct fsp_paged_keep_args* args, const int32_t* first_piece, int32_t* counts,
+                           void* stream);
 
 /*
  * Copies page sources[i] of k_pages and of v_pages to page targets[i], i in [0, n); nothing where either is

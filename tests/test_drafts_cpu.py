@@ -194,3 +194,13 @@ def test_partial_sums_by_tokens():
         assert L.fsp_attention_tree_by_tokens(base._cache() + _tree(), most, None) == -1
     assert L.fsp_attention_tree_by_tokens(None, 1, None) == -1
     assert L.fsp_attention_tree_by_tokens(base._cache() + _tree(q=0), 2, None) == -1
+
+
+def test_counted_keep_refusals_of_the_library():
+    L, c = _abi.lib(), base._cache()
+    call = L.fsp_paged_keep_counted
+    assert call(None, 16, 16, None) == -1 and call(c + c + _keep(other=0), 16, 16, None) == -1
+    for first, counts in ((None, 16), (16, None)):
+        assert call(c + c + _keep(other=1), first, counts, None) == -1
+    for kw in ({"tokens": -1}, {"keep": 0}, {"lengths": 0}, {"kept": 0}, {"pieces": 0}, {"n_pieces": 1}, {"piece": 200}):
+        assert call(c + c + _keep(**({"other": 1} | kw)), 16, 16, None) == -1

@@ -478,3 +478,81 @@ def test_drafting_is_the_text_read_at_once(dev, window, sinks):
         ref.check("q", q[at], tuple(x[at] for x in turned))
         want = ref.packed(q, k, v, [n], [n], True, window, d**-0.5, sinks=sinks)["out"]
         ref.check("out", torch.stack([x for _, _, x in seen[b]]), tuple(x[at] for x in want))
+
+
+@pytest.mark.parametrize("share", [0.0, 0.5, 1.0])
+def test_keep_into_other_pages_of_long_texts(dev, share):
+    # so many marks that they are counted by pieces first: ragged texts, marks of all and of some of a text
+    lengths, new = [40000, 0, 17, 20000, 3001, 33000], [39000, 0, 17, 20000, 1, 5]
+    kv, k, v = _cache(dev, lengths, 16, 1, 8, BF, room=1)
+    to, _, _ = _cache(dev, [40000, 0, 17, 15000, 3001, 33000], 24, 1, 8, BF, seed=5, room=1)
+    before = to.k_pages.clone(), to.v_pages.clone()
+    marks = _marks(new, share, 2)
+    n = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    keep = torch.cat([torch.ones(3, dtype=torch.bool), *marks]).to(dev)[3:]
+    want = [a - b + int(m.sum()) for a, b, m in zip(lengths, new, marks)]
+    for _ in range(2):
+        got = fs.flagsparse_paged_keep(keep, n, _indptr(new, dev), prepared=kv, into=to)
+        assert got.tolist() == [-1 if b == 3 and share == 1.0 else m for b, m in enumerate(want)]  # no room for all
+    changed = torch.zeros(to.n_pages, 24, dtype=torch.bool, device=dev)
+    for b in range(len(lengths)):
+        here = _slots(to, b, range(max(0, int(got[b]))))
+        if int(got[b]) >= 0:
+            for pages, rows in ((to.k_pages, k[b]), (to.v_pages, v[b])):
+                assert torch.equal(pages[here].cpu(), _kept_rows(rows, new[b], marks[b]))
+        changed[here] = True
+    for now, then in zip((to.k_pages, to.v_pages), before):
+        assert torch.equal(_bits(now[~changed]), _bits(then[~changed]))
+    for bad in ([-1, 1, 16, 40000, 0, 4], [2**40, 17, 4000, 19999, -2**40, 2**31 - 1]):
+        got = fs.flagsparse_paged_keep(keep, torch.tensor(bad, device=dev), _indptr(new, dev), prepared=kv, into=to)
+        assert got[0] == got[2] == got[4] == got[5] == -1 and got[3] == -1
+    for bad in ([0, 2**30, 17, 20000, 59018, 59023], [-5, 39000, 0, 39017, 0, 59018, 2**31 - 1]):
+        fs.flagsparse_paged_keep(keep, n, torch.tensor((bad + [59023])[:7], device=dev), prepared=kv, into=to)
+    torch.cuda.synchronize()
+
+
+def test_keep_of_long_texts_in_a_graph(dev):
+    lengths = [30000, 900]
+    kv, k, _ = _cache(dev, lengths, 16, 2, 64, BF)
+    to, _, _ = _cache(dev, lengths, 16, 2, 64, BF, seed=5)
+    keep, tokens = torch.cat(_marks(lengths, 0.5, 1)).to(dev), _indptr(lengths, dev)
+    n = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    graph = torch.cuda.CUDAGraph()
+    fs.flagsparse_paged_keep(keep, n, tokens, prepared=kv, into=to)
+    with torch.cuda.graph(graph):
+        got = fs.flagsparse_paged_keep(keep, n, tokens, prepared=kv, into=to)
+    for seed in range(3):
+        marks = _marks(lengths, 0.1 + 0.4 * seed, seed)
+        keep.copy_(torch.cat(marks))
+        eager = fs.flagsparse_paged_keep(keep, n, tokens, prepared=kv, into=to)
+        to.k_pages.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(eager, got)
+        for b in range(2):
+            here = _slots(to, b, range(int(got[b])))
+            assert torch.equal(to.k_pages[here].cpu(), _kept_rows(k[b], lengths[b], marks[b]))
+
+
+def test_keep_into_other_pages_takes_time_by_the_tokens(dev):
+    # eight times the tokens of a text: eight times the time and not its square, 64 times
+    def time_of(tokens):
+        k, v, k2, v2 = (torch.zeros(tokens // 64, 64, 1, 8, dtype=BF, device=dev) for _ in range(4))
+        table = torch.arange(tokens // 64, dtype=torch.int32, device=dev)
+        ends = torch.tensor([0, tokens // 64], device=dev)
+        kv, to = fs.prepare_paged_kv(k, v, ends, table), fs.prepare_paged_kv(k2, v2, ends, table)
+        keep = torch.arange(tokens, device=dev) % 2 == 0
+        n = torch.tensor([tokens], dtype=torch.int32, device=dev)
+        best = float("inf")
+        for _ in range(5):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(5):
+                got = fs.flagsparse_paged_keep(keep, n, prepared=kv, into=to)
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        assert got.tolist() == [tokens // 2]
+        return best
+
+    assert time_of(1 << 21) <= 24 * time_of(1 << 18)
