@@ -21,6 +21,8 @@ As with the sparse products, ``prepare_*`` checks index arrays once (the host wa
 the calls with ``prepared=`` neither check them again nor wait: they can be captured in a graph.
 """
 
+import functools
+import math
 import struct
 
 import numpy as np
@@ -251,7 +253,7 @@ class PreparedPagedKV:
 
     __slots__ = ("k_pages", "v_pages", "dtype", "device", "indptr", "indices", "batch", "n_pages",
                  "page_size", "kv_heads", "dim", "room", "_piece", "_pieces", "_first", "_most", "_streams",
-                 "_calls", "_counts", "_held", "_lists")
+                 "_calls", "_counts", "_held", "_lists", "_sizes")
 
     def __init__(self, k_pages, v_pages, indptr, indices, pages):
         self.k_pages = k_pages
@@ -265,7 +267,7 @@ class PreparedPagedKV:
         rooms = pages * self.page_size
         self.room = int(rooms.max()) if len(rooms) else 0
         self._held = pages  # of each sequence, on the host
-        self._lists = {}  # pieces of other sizes, or under a window: see _list
+        self._lists, self._sizes = {}, {}  # pieces of other sizes, or under a window: see _list
         # the pieces that attention is cut into
         self._piece = int(_abi.lib().fsp_attention_paged_piece(int(rooms.sum()), self.kv_heads))
         self._pieces, self._first, self._most = _on_device(
@@ -292,23 +294,38 @@ class PreparedPagedKV:
             self._streams.mark(stream, self.device, (self.indptr, self.indices, self._pieces))
         return stream
 
-    def _list(self, sight, each, slots, most, rows):
+    def _list(self, sight, slots, most, ways, way):
         """(tokens of a piece, pieces, first pieces, most of one sequence, streams that they are marked on):
         pieces of at most ``most`` tokens, of each sequence no more than ``sight`` tokens in a row can
-        touch (0: all of its room), that go to ``each`` workgroups of ``rows`` rows, of which ``slots`` run
-        at a time; made when first asked for and kept."""
-        key = (sight, each, slots, most, rows)
-        kept = self._lists.get(key)
-        if kept is None:
+        touch (0: all of its room), that go to ``way[0]`` workgroups of ``way[1]`` rows, of which ``slots`` run
+        at a time.  The first call makes those of all ``ways`` that calls of its kind may go, and they are kept."""
+        key = (sight, slots, most, ways)
+        sizes = self._sizes.get(key)
+        if sizes is None:
             if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("a call's first run with these sizes builds its work list, which "
-                                   "cannot be captured: make one such call before the capture")
-            piece = _piece_of(self._held * self.page_size, *key)
-            table = _on_device(*_pieces(self._held, self.page_size, piece, sight), piece, self.device)
+                raise RuntimeError("a call's first run with this window and these heads builds its work lists, "
+                                   "which cannot be captured: make one such call before the capture")
+            sizes = {w: _piece_of(self._held * self.page_size, sight, w[0], slots, most, w[1]) for w in ways}
+            for piece in sorted(set(sizes.values())):
+                if (sight, piece) not in self._lists:
+                    table = _on_device(*_pieces(self._held, self.page_size, piece, sight), piece, self.device)
+                    # for good: captured graphs read it
+                    self._lists.setdefault((sight, piece), (piece, *table, _Streams()))
             torch.cuda.current_stream(self.device).synchronize()  # calls may come from other streams
-            kept = (piece, *table, _Streams())
-            kept = self._lists.setdefault(key, kept)  # for good: captured graphs read it
-        return kept
+            self._sizes[key] = sizes
+        return self._lists[sight, sizes[way]]
+
+
+@functools.lru_cache(maxsize=64)
+def _tree_ways(kv_heads, group):
+    """How the pieces of a tree call may be gone through, whatever its numbers of drafted tokens: (workgroups of a
+    piece, rows of each), tiles by powers of two."""
+    L = _abi.lib()
+    tiles = {}
+    for longest in range(1, int(L.fsp_attention_tree_drafts()) + 1):
+        rows = int(L.fsp_attention_tree_rows(group, longest))
+        tiles[rows] = max(tiles.get(rows, 1), -(-group * longest // rows))
+    return tuple((kv_heads << i, rows) for rows, n in sorted(tiles.items()) for i in range((n - 1).bit_length() + 1))
 
 
 def _piece_of(rooms, sight, each, slots, most, rows):
@@ -708,8 +725,8 @@ def flagsparse_attention_paged(q, lengths, *, prepared=None, k_pages=None, v_pag
 
     ``q``: [sequences, heads, dim]; ``lengths[b]``: the tokens that sequence b holds, the query's
     own among them (0: the sequence is empty, and its output is zeros).  ``window``: only the last
-    ``window`` tokens are seen, and with ``sinks`` the first ``sinks`` too (the first call with such sizes
-    builds a work list and cannot be captured).  ``scale``: dim ** -0.5 by default.  Returns [sequences, heads, dim],
+    ``window`` tokens are seen, and with ``sinks`` the first ``sinks`` too (the first call with such a window
+    and as many heads builds a work list and cannot be captured).  ``scale``: dim ** -0.5 by default.  Returns [sequences, heads, dim],
     with the float32 log-sum-exp [sequences, heads] if ``return_lse``; neither is differentiable, nor
     is what flagsparse_paged_append gives.  With ``prepared`` nothing is
     waited for, so lengths are not checked: one that its sequence's pages cannot hold gives NaN."""
@@ -738,8 +755,8 @@ def flagsparse_attention_paged(q, lengths, *, prepared=None, k_pages=None, v_pag
     table, firsts, piece, most, marked = kv._pieces, kv._first, kv._piece, kv._most, None
     if first:
         tiles = -(-heads // kv.kv_heads // 16)
-        piece, table, firsts, most, marked = kv._list(min(past + first, _TOKENS_CAP), kv.kv_heads * tiles,
-                                                      768, 1024, 16)
+        way = (kv.kv_heads * tiles, 16)
+        piece, table, firsts, most, marked = kv._list(min(past + first, _TOKENS_CAP), 768, 1024, (way,), way)
     pieces, need, room = table.shape[0], 0, None
     if pieces > kv.batch:
         need = int(_abi.lib().fsp_attention_paged_counts(pieces, most, kv.batch, heads, kv.kv_heads))
@@ -816,8 +833,8 @@ def flagsparse_attention_paged_tree(q, lengths, token_indptr=None, *, parents=No
     sequence with more drafted tokens than ``longest``, or a length that its pages cannot hold or less than
     its drafted tokens, rows whose parents do not come earlier, and rows of no sequence are NaN.  What
     is not finite in a hidden drafted token's value may reach other rows of its sequence (its weight is zero,
-    and zero times it is NaN), in its key it does not.  The first call of its sizes builds a work list
-    and cannot be captured."""
+    and zero times it is NaN), in its key it does not.  The first call with its window, sinks and number
+    of heads builds work lists and cannot be captured; others, whatever their numbers of tokens, use them."""
     key = None
     if out is None and type(prepared) is PreparedPagedKV and type(scale) in _PLAIN and \
             type(window) in _PLAIN and type(sinks) in _PLAIN and type(longest) in _PLAIN:
@@ -863,13 +880,15 @@ def flagsparse_attention_paged_tree(q, lengths, token_indptr=None, *, parents=No
         if return_lse:
             lse.fill_(float("nan"))
     else:
-        # the same for all calls of a program, whatever numbers of tokens they have
+        # the same for all calls of a program, whatever numbers of tokens they have, and so are the lists
         sight = min(past + first + most, _TOKENS_CAP) if past else 0
         group = heads // kv.kv_heads
         of = int(_abi.lib().fsp_attention_tree_rows(group, longest))
-        # tiles of an average sequence: those of the longest trees are few
+        # tiles of an average sequence, as those of the longest trees are few, to a power of two
         tiles = min(-(-group * longest // of), 1 + group * tokens // (kv.batch * of))
-        piece, pieces, firsts, longest_list, marked = kv._list(sight, kv.kv_heads * tiles, 512, 8192, of)
+        way = (kv.kv_heads << round(math.log2(tiles)), of)
+        piece, pieces, firsts, longest_list, marked = kv._list(
+            sight, 512, 8192, _tree_ways(kv.kv_heads, group), way)
         n_pieces, need, room, by_tokens = pieces.shape[0], 0, None, 0
         if n_pieces > kv.batch:
             need = int(_abi.lib().fsp_attention_tree_counts(n_pieces, longest_list, kv.batch, kv.kv_heads,

@@ -1,6 +1,8 @@
 """Drafted trees, kept tokens and copied pages without a GPU: work lists, argument structs, the refusals of the
 library, and which drafted tokens the tests' reference lets a row see."""
 
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -204,3 +206,17 @@ def test_counted_keep_refusals_of_the_library():
         assert call(c + c + _keep(other=1), first, counts, None) == -1
     for kw in ({"tokens": -1}, {"keep": 0}, {"lengths": 0}, {"kept": 0}, {"pieces": 0}, {"n_pieces": 1}, {"piece": 200}):
         assert call(c + c + _keep(**({"other": 1} | kw)), 16, 16, None) == -1
+
+
+@pytest.mark.parametrize("kv_heads,group", [(1, 1), (2, 3), (8, 4), (1, 23), (1, 64), (3, 128)])
+def test_ways_of_all_numbers_of_drafts(kv_heads, group):
+    # what a call may look up, for any longest tree and any number of tokens, is among the ways
+    L = _abi.lib()
+    ways = attention._tree_ways(kv_heads, group)
+    assert len(set(ways)) == len(ways) <= 3 + (2 * group - 1).bit_length()
+    for longest in (1, 2, 4, 5, 8, 9, 31, 100, 255, 256):
+        rows = L.fsp_attention_tree_rows(group, longest)
+        for tiles in range(1, -(-group * longest // rows) + 1):
+            assert any(way == (kv_heads << i, rows) and abs(2**i - tiles) <= tiles / 2
+                       for way in ways for i in range(20)), (longest, tiles)
+            assert (kv_heads << round(math.log2(tiles)), rows) in ways

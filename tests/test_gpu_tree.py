@@ -461,3 +461,33 @@ def test_partial_sums_of_ragged_trees(dev, heads, kv_heads, dim):
     trees = [_tree(n, s) for s, n in enumerate(new)]
     _check(dev, past, trees, 64, heads, kv_heads, dim, BF, longest=4)
     _check(dev, past, trees, 64, heads, kv_heads, dim, HF, room=60)
+
+
+@pytest.mark.parametrize("heads,window,sinks", [(4, None, 0), (12, 700, 5)])
+def test_other_numbers_of_drafts_use_the_same_lists(dev, heads, window, sinks):
+    # after the first call of a program others build nothing: they can be captured whatever they draft
+    kv = _long_cache(dev, 4, 100, 2, 64, BF)
+    n = torch.full((4,), 6000, dtype=torch.int32, device=dev)
+
+    def call(new, longest=None):
+        q = _normal(sum(new), sum(new), heads, 64, dtype=BF).to(dev)
+        tokens, parents = _indptr(new, dev), torch.full((sum(new),), -1, dtype=torch.int32, device=dev)
+
+        def run():
+            return fs.flagsparse_attention_paged_tree(q, n, tokens, parents=parents, longest=longest, prepared=kv,
+                                                      window=window, sinks=sinks)
+        return run
+
+    call([1, 0, 2, 1])()
+    lists, streams = list(kv._lists), torch.cuda.Stream(dev)
+    for new, longest in (([3, 3, 3, 3], 3), ([20, 1, 0, 7], None), ([256, 256, 256, 256], None), ([40, 1, 2, 3], 64)):
+        run, graph = call(new, longest), torch.cuda.CUDAGraph()
+        streams.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.graph(graph, stream=streams):
+            got = run()
+        for _ in range(2):
+            got.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, run())
+    assert list(kv._lists) == lists
