@@ -121,6 +121,7 @@ SIGNATURES = {
     "fsp_attention_dim_cap": (_i64, []),
     "fsp_paged_append": (_i32, [_p, _p]),
     "fsp_paged_append_drafts": (_i32, [_p, _p, _p]),
+    "fsp_paged_append_at": (_i32, [_p, _p, _p, _p]),
     "fsp_paged_keep": (_i32, [_p, _p]),
     "fsp_paged_keep_counted": (_i32, [_p, _p, _p, _p]),
     "fsp_paged_copy": (_i32, [_p, _p, _p, _i64, _p]),

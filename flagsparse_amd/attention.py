@@ -475,7 +475,7 @@ def _paged_of(prepared, k_pages, v_pages, indptr, indices, lengths):
 
 def flagsparse_paged_append(k, v, lengths, token_indptr=None, *, prepared=None, k_pages=None,
                             v_pages=None, indptr=None, indices=None, q=None, cos=None, sin=None,
-                            interleaved=False, parents=None, out=None):
+                            interleaved=False, parents=None, text_lengths=None, out=None):
     """Write new keys and values into a paged cache, rotated by their positions on the way.
 
     ``k``, ``v``: [tokens, kv_heads, dim], the new tokens of each sequence one after the other:
@@ -487,6 +487,9 @@ def flagsparse_paged_append(k, v, lengths, token_indptr=None, *, prepared=None, 
     ``parents``: the new tokens are drafted ones, at most 256 a sequence, that form trees
     (flagsparse_attention_paged_tree): each is stored in its turn, but rotated by the position of its sequence's
     first new token plus the tokens before it on its way up the tree.
+    ``text_lengths``: what the sequences' texts count with the new tokens, where that is more than the cache holds of
+    them because some were given up (flagsparse_paged_keep leaves the others rotated as they are): new tokens are
+    stored behind what is left, by ``lengths``, and rotated by their positions in the texts.
 
     Returns the rotated ``q`` [tokens, heads, dim] (written to ``out`` where given, which may be ``q``),
     or None without ``q``.  The pages that new tokens go to belong to one sequence each, and ``k``,
@@ -496,14 +499,14 @@ def flagsparse_paged_append(k, v, lengths, token_indptr=None, *, prepared=None, 
     ``q`` comes back as NaN."""
     key = None
     if out is None and type(prepared) is PreparedPagedKV:
-        key = _layouts(k, v, q, cos, sin, lengths, token_indptr, parents) + (
+        key = _layouts(k, v, q, cos, sin, lengths, token_indptr, parents, text_lengths) + (
             bool(interleaved), prepared.k_pages.data_ptr(), prepared.v_pages.data_ptr())
         kept = prepared._calls.get(key)
         if kept is not None and not (k.data_ptr() | v.data_ptr()) % 16 and (
                 q is None or q.data_ptr() % 16 == 0):
             head, like = kept
             res = None if q is None else torch.empty_like(like, memory_format=_CONTIGUOUS)
-            _append(prepared, head, k, v, q, res, cos, sin, token_indptr, lengths, parents)
+            _append(prepared, head, k, v, q, res, cos, sin, token_indptr, lengths, parents, text_lengths)
             return res
     kv, n = _paged_of(prepared, k_pages, v_pages, indptr, indices, lengths)
     dev, dt = kv.device, kv.dtype
@@ -512,7 +515,7 @@ def flagsparse_paged_append(k, v, lengths, token_indptr=None, *, prepared=None, 
     tokens = k.shape[0]
     if v.shape[0] != tokens:
         raise ValueError(f"v must have {tokens} tokens, got {v.shape[0]}")
-    given = (k, v, q, cos, sin, lengths, token_indptr, parents)
+    given = (k, v, q, cos, sin, lengths, token_indptr, parents, text_lengths)
     if token_indptr is None:
         if tokens != kv.batch:
             raise ValueError(f"k must have one token for each of {kv.batch} sequences, got "
@@ -524,6 +527,8 @@ def flagsparse_paged_append(k, v, lengths, token_indptr=None, *, prepared=None, 
         if prepared is None:
             _check_drafts(kv, n, token_indptr, parents, tokens, 1 if token_indptr is None else
                           int(_abi.lib().fsp_attention_tree_drafts()))
+    if text_lengths is not None:
+        text_lengths = _int32(text_lengths, "text_lengths", kv.batch, dev)
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin come together")
     half = rows = 0
@@ -556,9 +561,9 @@ def flagsparse_paged_append(k, v, lengths, token_indptr=None, *, prepared=None, 
         steps = (*_steps(q), *_steps(res)) if heads else (0, 0, 0, 0)
         head = kv._packed() + _APPEND.pack(tokens, heads, half, rows, bool(interleaved),
                                            *_steps(k), *_steps(v), *steps)
-        _append(kv, head, k, v, q, res, cos, sin, token_indptr, n, parents)
+        _append(kv, head, k, v, q, res, cos, sin, token_indptr, n, parents, text_lengths)
         if key is not None and all(x is y for x, y in zip(
-                (k, v, q, cos, sin, n, token_indptr, parents), given)):
+                (k, v, q, cos, sin, n, token_indptr, parents, text_lengths), given)):
             _keep(kv._calls, key, (head, None if q is None else _like(q.shape, dt, dev)))
     elif res is not None:  # tokens of no sequence
         res.fill_(float("nan"))
@@ -572,10 +577,12 @@ def _at(t):
     return 0 if t is None else t.data_ptr()
 
 
-def _append(kv, head, k, v, q, res, cos, sin, token_indptr, lengths, parents):
+def _append(kv, head, k, v, q, res, cos, sin, token_indptr, lengths, parents, text_lengths):
     args = head + _APPEND_AT.pack(k.data_ptr(), v.data_ptr(), _at(q), _at(res), _at(cos), _at(sin),
                                   _at(token_indptr), lengths.data_ptr())
-    if parents is None:
+    if text_lengths is not None:
+        status = _abi.lib_on(kv.device).fsp_paged_append_at(args, _at(parents), text_lengths.data_ptr(), kv._on())
+    elif parents is None:
         status = _abi.lib_on(kv.device).fsp_paged_append(args, kv._on())
     else:
         status = _abi.lib_on(kv.device).fsp_paged_append_drafts(args, parents.data_ptr(), kv._on())
@@ -593,7 +600,9 @@ def flagsparse_paged_keep(keep, lengths, token_indptr=None, *, prepared=None, k_
     ``lengths[b]`` is what sequence b holds.  The marked ones stay, in their order, and close up behind the
     tokens before them: in place, where the pages they move in belong to one sequence each, or in the pages of
     ``into``, another PreparedPagedKV with as many sequences, heads and dims, to which the tokens before them are
-    copied too (pages that the call does not read; several may lie in the same arrays).
+    copied too (pages that the call does not read; several may lie in the same arrays).  Keys stay rotated as they
+    are: after a text whose tokens were given up go others by flagsparse_paged_append with ``text_lengths``.  A
+    window of the attention, and its first tokens, go by places in the cache.
 
     Returns the new lengths, int32.  With ``prepared`` nothing is waited for, so lengths are not checked: where
     one is more than its pages hold or less than its marked tokens, or ``into`` has no room for

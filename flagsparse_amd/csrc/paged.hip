@@ -93,7 +93,7 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(
     const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ q,
     T* __restrict__ q_out, const float* __restrict__ cos, const float* __restrict__ sin,
     const int32_t* __restrict__ tokens, const int32_t* __restrict__ lengths,
-    const int32_t* __restrict__ parents) {
+    const int32_t* __restrict__ parents, const int32_t* __restrict__ text) {
   const int lane = threadIdx.x & 63;
   const int64_t unit = (int64_t)blockIdx.x * (kAppendThreads / kWave) +
                        __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -112,14 +112,16 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(
     b = __builtin_amdgcn_readfirstlane(max(b, 0));
     const int begin = tokens[b], end = tokens[b + 1];
     mine = begin <= t && t < end;
-    pos = turn = (int64_t)lengths[b] - end + t;
+    pos = (int64_t)lengths[b] - end + t;
+    turn = (int64_t)text[b] - end + t;
     if (parents && mine && (begin < 0 || end > s.n_tokens)) mine = false;  // its parents are not there
     if (parents && mine) {
       depth = __builtin_amdgcn_readfirstlane(depth_of(parents + begin, (int)(t - begin), end - begin));
-      turn = (int64_t)lengths[b] - (end - begin) + depth;
+      turn = (int64_t)text[b] - (end - begin) + depth;
     }
   } else {
-    pos = turn = (int64_t)lengths[b] - 1;
+    pos = (int64_t)lengths[b] - 1;
+    turn = (int64_t)text[b] - 1;
     if (parents) depth = parents[t] == -1 ? 0 : -1;
   }
   const int first = c.indptr[b], last = c.indptr[b + 1];
@@ -554,6 +556,7 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(
 
 struct AppendCall : fsp_paged_append_args {
   const int32_t* parents;
+  const int32_t* text;  // what the positions go by
 };
 
 template <typename T, int MODE>
@@ -571,7 +574,7 @@ int launch_append(const AppendCall& a, hipStream_t st) {
                      static_cast<T*>(a.cache.k_pages), static_cast<T*>(a.cache.v_pages),
                      static_cast<const T*>(a.k), static_cast<const T*>(a.v),
                      static_cast<const T*>(a.q), static_cast<T*>(a.q_out), a.cos, a.sin,
-                     a.token_indptr, a.lengths, a.parents);
+                     a.token_indptr, a.lengths, a.parents, MODE == kStill ? a.lengths : a.text);
   return check_hip(hipGetLastError(), "paged_append_kernel launch");
 }
 
@@ -667,14 +670,21 @@ int run_append(const AppendCall& a, const std::string& who, void* stream) {
 
 extern "C" int fsp_paged_append(const fsp_paged_append_args* args, void* stream) {
   if (!args) return set_error(FSP_EINVAL, "fsp_paged_append: null arguments");
-  return run_append({*args, nullptr}, "fsp_paged_append", stream);
+  return run_append({*args, nullptr, args->lengths}, "fsp_paged_append", stream);
 }
 
 extern "C" int fsp_paged_append_drafts(const fsp_paged_append_args* args, const int32_t* parents,
                                        void* stream) {
   if (!args) return set_error(FSP_EINVAL, "fsp_paged_append_drafts: null arguments");
   if (!parents && args->n_tokens > 0) return set_error(FSP_EINVAL, "fsp_paged_append_drafts: null pointer");
-  return run_append({*args, parents}, "fsp_paged_append_drafts", stream);
+  return run_append({*args, parents, args->lengths}, "fsp_paged_append_drafts", stream);
+}
+
+extern "C" int fsp_paged_append_at(const fsp_paged_append_args* args, const int32_t* parents,
+                                   const int32_t* text_lengths, void* stream) {
+  if (!args) return set_error(FSP_EINVAL, "fsp_paged_append_at: null arguments");
+  if (!text_lengths && args->n_tokens > 0) return set_error(FSP_EINVAL, "fsp_paged_append_at: null pointer");
+  return run_append({*args, parents, text_lengths}, "fsp_paged_append_at", stream);
 }
 
 extern "C" int64_t fsp_attention_paged_piece(int64_t tokens, int64_t kv_heads) {

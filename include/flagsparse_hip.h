@@ -734,6 +734,11 @@ int fsp_paged_append(const struct fsp_paged_append_args* args, void* stream);
  */
 int fsp_paged_append_drafts(const struct fsp_paged_append_args* args, const int32_t* parents,
                             void* stream);
+/* Either of them (parents may be NULL) where tokens were taken from the texts (fsp_paged_keep): sequence b's new
+ * tokens are stored behind what the cache holds of it, by lengths[b], but rotated by their positions in a text of
+ * text_lengths[b] tokens, the new ones among them. */
+int fsp_paged_append_at(const struct fsp_paged_append_args* args, const int32_t* parents,
+                        const int32_t* text_lengths, void* stream);
 
 /*
  * Of the last tokens of each sequence (token_indptr[b + 1] - token_indptr[b]; NULL: `each`, n_tokens / batch)

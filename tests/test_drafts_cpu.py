@@ -220,3 +220,10 @@ def test_ways_of_all_numbers_of_drafts(kv_heads, group):
             assert any(way == (kv_heads << i, rows) and abs(2**i - tiles) <= tiles / 2
                        for way in ways for i in range(20)), (longest, tiles)
             assert (kv_heads << round(math.log2(tiles)), rows) in ways
+
+
+def test_append_at_refusals_of_the_library():
+    L, c = _abi.lib(), base._cache()
+    for args in ((c + base._append(), None, None), (None, None, 16), (c + base._append(half=33), 16, 16),
+                 (c + base._append(k=0), None, 16)):
+        assert L.fsp_paged_append_at(*args, None) == -1

@@ -556,3 +556,80 @@ def test_keep_into_other_pages_takes_time_by_the_tokens(dev):
         return best
 
     assert time_of(1 << 21) <= 24 * time_of(1 << 18)
+
+
+@pytest.mark.parametrize("dtype,half,interleaved", [(BF, 32, False), (HF, 32, True), (HF, 20, False), (BF, 17, True)])
+def test_a_text_goes_on_after_tokens_were_given_up(dev, dtype, half, interleaved):
+    # its kept keys stay where they stood in the text, and so do those that come after them
+    dim, g, h, text, new = 64, 2, 4, [300, 41, 128], [3, 1, 5]
+    cos, sin = _table(400, half)
+    kw = {"cos": cos.to(dev), "sin": sin.to(dev), "interleaved": interleaved}
+    kv, _, _ = _cache(dev, text, 16, g, dim, dtype, room=1)
+    to, _, _ = _cache(dev, text, 16, g, dim, dtype, seed=5, room=1)
+    k, v = (_normal(s, sum(text), g, dim, dtype=dtype) for s in (1, 2))
+    n = torch.tensor(text, dtype=torch.int32, device=dev)
+    fs.flagsparse_paged_append(k.to(dev), v.to(dev), n, _indptr(text, dev), prepared=kv, **kw)
+    marks = _marks(text, 0.4, 3)
+    left = fs.flagsparse_paged_keep(torch.cat(marks).to(dev), n, _indptr(text, dev), prepared=kv, into=to)
+    pos = [m.nonzero().flatten() for m in marks]
+
+    def check(cache, lengths, turns, key, value):
+        at = 0
+        for b, turn in enumerate(turns):
+            here = _slots(cache, b, range(int(lengths[b]) - len(turn), int(lengths[b])))
+            ref.check("k", cache.k_pages[here],
+                      tuple(t for t in _turned(key[at:at + len(turn)], turn, cos, sin, interleaved)))
+            assert torch.equal(cache.v_pages[here].cpu(), value[at:at + len(turn)])
+            at += len(turn)
+
+    check(to, left, pos, torch.cat([x[m] for x, m in zip(k.split(text), marks)]),
+          torch.cat([x[m] for x, m in zip(v.split(text), marks)]))
+    # one token each, several, and drafted ones
+    for lengths, tree in ((None, None), (new, None), (new, [_tree(m, s) for s, m in enumerate(new)])):
+        counts = lengths or [1] * 3
+        depths = [[len(w) - 1 for w in _ways(t)] for t in tree] if tree else [list(range(m)) for m in counts]
+        turns = [torch.tensor(d) + m for d, m in zip(depths, text)]
+        kn, vn, q = (_normal(s, sum(counts), m, dim, dtype=dtype) for s, m in ((7, g), (8, g), (9, h)))
+        more = torch.tensor(counts, device=dev)
+        for cast in (torch.int32, torch.int64):
+            got = fs.flagsparse_paged_append(
+                kn.to(dev), vn.to(dev), (left + more).to(cast), lengths and _indptr(lengths, dev), prepared=to,
+                q=q.to(dev), parents=torch.tensor(sum(tree, []), device=dev) if tree else None,
+                text_lengths=(n + more).to(cast), **kw)
+            ref.check("q", got, _turned(q, torch.cat(turns), cos, sin, interleaved))
+            check(to, left + more, turns, kn, vn)
+    # a position that the table does not hold, or before the text: not stored, and NaN
+    before = _bits(to.k_pages).clone()
+    for bad in (0, -7, 401, 2**40):
+        wrong = torch.full((3,), bad, device=dev)
+        q = _normal(9, 3, h, dim, dtype=dtype).to(dev)
+        got = fs.flagsparse_paged_append(q[:, :g], q[:, :g], left + 1, prepared=to, q=q, text_lengths=wrong, **kw)
+        assert torch.isnan(got).all() and torch.equal(_bits(to.k_pages), before)
+    # without a rotation there is nothing to go by
+    fs.flagsparse_paged_append(q[:, :g], q[:, :g], left + 1, prepared=to, text_lengths=wrong)
+    here = _slots(to, 1, [int(left[1])])
+    assert torch.equal(to.k_pages[here], q[1:2, :g])
+    for bad in (n[:2], n.cpu(), n[None]):
+        with pytest.raises(ValueError):
+            fs.flagsparse_paged_append(q[:, :g], q[:, :g], left + 1, prepared=to, text_lengths=bad, **kw)
+    with pytest.raises(TypeError):
+        fs.flagsparse_paged_append(q[:, :g], q[:, :g], left + 1, prepared=to, text_lengths=n.float(), **kw)
+
+
+def test_texts_as_long_as_the_cache_holds_are_the_call_without(dev):
+    lengths = [70, 20]
+    kv, _, _ = _cache(dev, lengths, 16, 2, 64, BF)
+    cos, sin = (t.to(dev) for t in _table(80, 32))
+    k, v, q = (_normal(s, 7, m, 64, dtype=BF).to(dev) for s, m in ((1, 2), (2, 2), (3, 4)))
+    n, tokens = torch.tensor(lengths, dtype=torch.int32, device=dev), torch.tensor([0, 4, 7], device=dev)
+    kw = {"prepared": kv, "q": q, "cos": cos, "sin": sin}
+    for parents in (None, torch.tensor([-1, 0, 0, 1, -1, 0, 1], device=dev)):
+        want = fs.flagsparse_paged_append(k, v, n, tokens, parents=parents, **kw)
+        kept = _bits(kv.k_pages).clone()
+        kv.k_pages.zero_()
+        fs.flagsparse_paged_append(k, v, n, tokens, parents=parents, **kw)
+        now = _bits(kv.k_pages).clone()
+        kv.k_pages.zero_()
+        got = fs.flagsparse_paged_append(k, v, n, tokens, parents=parents, text_lengths=n, **kw)
+        assert torch.equal(got, want) and torch.equal(_bits(kv.k_pages), now)
+        kv.k_pages.view(torch.int16).copy_(kept)
