@@ -1077,16 +1077,16 @@ def prepare_attention_packed(indptr, k_indptr=None):
 
 
 def _packed_inputs(q, k, v, indptr, k_indptr, prepared, causal, window, sinks):
-    """(prepared, causal, window, sinks) of a call whose arrays are checked against each other."""
+    """(prepared, causal, window, sinks) of a call whose arrays are checked against each other; no window and
+    sinks where together they show all keys."""
     _check_tensor(q, "q")
     _check_tensor(k, "k", q.dtype, q.device, None, q.shape[2])
     _check_tensor(v, "v", q.dtype, q.device, k.shape[1], q.shape[2])
     _check_heads(q.shape[1], k.shape[1])
     _check_dim(q.shape[2])
-    window = _window_of(window)
-    if window and not causal:
+    if _window_of(window) and not causal:
         raise ValueError("window needs causal=True")
-    sinks = _sinks_of(sinks, window)
+    _sinks_of(sinks, _window_of(window))
     if prepared is None:
         if indptr is None:
             raise ValueError("indptr is required when prepared is not provided")
@@ -1100,7 +1100,7 @@ def _packed_inputs(q, k, v, indptr, k_indptr, prepared, causal, window, sinks):
     if k.shape[0] != prepared.k_tokens or v.shape[0] != prepared.k_tokens:
         raise ValueError(f"k and v must have {prepared.k_tokens} tokens, got {k.shape[0]} and "
                          f"{v.shape[0]}")
-    return prepared, bool(causal), window, sinks
+    return prepared, bool(causal), *_sight_of(window, sinks, prepared._longest[1])
 
 
 def _pack(prepared, q, k, v, causal, window, scale, out, grads=(), sinks=0):
@@ -1196,8 +1196,8 @@ def flagsparse_attention_packed(q, k, v, indptr=None, k_indptr=None, *, prepared
     by ``indptr`` / ``k_indptr`` (checked by this call, which waits for them) or by ``prepared``
     (prepare_attention_packed).  With ``causal`` query i of nq sees key j of nk if
     j <= i + nk - nq, the last query all of them; ``window``: only the last ``window`` of those, and with
-    ``sinks`` the sequence's first ``sinks`` keys too (the first call with sinks builds a work list and cannot be
-    captured).
+    ``sinks`` the sequence's first ``sinks`` keys too (the first call with sinks that hide anything, and as many heads,
+    builds a work list and cannot be captured).
     ``scale``: dim ** -0.5 by default.  Returns [tokens, heads, dim], with the float32 log-sum-exp
     [tokens, heads] if ``return_lse``.  The output is differentiable with respect to q, k and v where
     they require a gradient (the log-sum-exp is not); forward-mode tangents raise NotImplementedError.

@@ -403,3 +403,29 @@ def test_short_sequences_beside_those_with_jobs(dev, heads, kv_heads):
         _both(dev, lengths, lengths, heads, kv_heads, 64, BF, 30, 6)
     _both(dev, [40, 600, 0, 90], [300, 650, 70, 9], heads, kv_heads, 96, HF, 25, 100)
     _both(dev, [300] * 9, [300] * 9, heads, kv_heads, 128, HF, 200, 130)
+
+
+def test_first_keys_that_reach_the_window_are_the_causal_call(dev):
+    # to the bit, without lists of their own: also as a graph's first call
+    lengths = [300, 20, 0, 513]
+    q, k, v, g = _inputs(dev, lengths, [n + 30 for n in lengths], 6, 2, 64, BF)
+    p = fs.prepare_attention_packed(_indptr(lengths, dev), _indptr([n + 30 for n in lengths], dev))
+
+    def both(**kw):
+        out, lse = fs.flagsparse_attention_packed(q, k, v, prepared=p, return_lse=True, **kw)
+        return (out, lse, *fs.flagsparse_attention_packed_backward(g, q, k, v, out, lse, prepared=p, **kw))
+
+    want, side = both(), torch.cuda.Stream(dev)
+    for window, sinks in ((500, 43), (1, 542), (542, 1), (2**40, 7)):
+        graph = torch.cuda.CUDAGraph()
+        side.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.graph(graph, stream=side):
+            got = both(window=window, sinks=sinks)
+        for _ in range(2):
+            for t in got:
+                t.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(want, got))
+    hidden = both(window=500, sinks=42)  # one key of one query
+    assert not torch.equal(hidden[0][832], want[0][832])
