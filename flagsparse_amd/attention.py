@@ -305,7 +305,7 @@ class PreparedPagedKV:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("a call's first run with this window and these heads builds its work lists, "
                                    "which cannot be captured: make one such call before the capture")
-            sizes = {w: _piece_of(self._held * self.page_size, sight, w[0], slots, most, w[1]) for w in ways}
+            sizes = dict(zip(ways, _pieces_of(self._held * self.page_size, sight, ways, slots, most)))
             for piece in sorted(set(sizes.values())):
                 if (sight, piece) not in self._lists:
                     table = _on_device(*_pieces(self._held, self.page_size, piece, sight), piece, self.device)
@@ -329,9 +329,13 @@ def _tree_ways(kv_heads, group):
 
 
 def _piece_of(rooms, sight, each, slots, most, rows):
-    """The tokens of a piece, from 256 to ``most``, by which the pieces of all sequences end soonest.  A
-    workgroup takes as long as its tokens, and 100 + 2 * rows for what it does before and after them
-    (its sums are written and read again); all of them take something between their sum over the
+    return _pieces_of(rooms, sight, ((each, rows),), slots, most)[0]
+
+
+def _pieces_of(rooms, sight, ways, slots, most):
+    """For each of the ``ways``, (workgroups of a piece, rows of each), the tokens of a piece, from 256 to ``most``, by
+    which the pieces of all sequences end soonest.  A workgroup takes as long as its tokens, and 100 + 2 * rows for
+    what it does before and after them (its sums are written and read again); all of them take something between their sum over the
     ``slots`` and rounds of ``slots`` that wait for each other.  Mostly that gives whole rounds of even pieces: 8
     sequences of 30064, 8 key heads, 256 rows beside each (16 workgroups a piece), pieces of 2048 / 3840 /
     4096 / 5120 / 7552 (one round) / 10112 tokens 391 / 368 / 373 / 379 / 361 / 398 us; 96 ragged ones of up to
@@ -339,26 +343,27 @@ def _piece_of(rooms, sight, each, slots, most, rows):
     142; 33 ragged ones under a window of 2047, 23 heads of 80, up to 26 tokens, of 128 / 256 / 512 / 1024
     35 / 28 / 32 / 40."""
     seen = np.minimum(rooms, sight) if sight else rooms
-    around = 100 + 2 * rows
-    longest = int(seen.max(initial=0))
-    best = (float("inf"), 256)
+    longest, tokens = int(seen.max(initial=0)), int(seen.sum())
+    best = [(float("inf"), 256)] * len(ways)
     n = max(1, -(-longest // most))
     while True:
         piece = max(256, -(-longest // n // 128) * 128)
         whole = seen // piece
-        rest = np.sort(seen - whole * piece)[::-1]
-        rest = rest[rest > 0]
-        count = int(whole.sum()) * each
-        starts = np.arange(0, max(1, count + each * len(rest)), slots)
-        firsts = np.full(len(starts), piece)
-        if len(rest):
-            after = np.maximum(starts - count, 0) // each
-            firsts = np.where(starts < count, piece, rest[np.minimum(after, len(rest) - 1)])
-        total = each * (int(seen.sum()) + around * (int(whole.sum()) + len(rest)))
-        rounds = float((firsts + around).sum())
-        best = min(best, (rounds + max(total / slots, float(firsts[0] + around)), piece))
+        rest = seen - whole * piece
+        rest = np.sort(rest[rest > 0])[::-1]
+        wholes, rests = int(whole.sum()), len(rest)
+        for i, (each, rows) in enumerate(ways):
+            around, count = 100 + 2 * rows, wholes * each
+            starts = max(1, -(-(count + each * rests) // slots))  # rounds, and those that start with whole pieces
+            full = min(starts, -(-count // slots)) if rests else starts
+            first = piece if full else int(rest[0])
+            rounds = full * piece + starts * around
+            if full < starts:
+                rounds += int(rest[(np.arange(full, starts) * slots - count) // each].sum())
+            total = each * (tokens + around * (wholes + rests))
+            best[i] = min(best[i], (rounds + max(total / slots, float(first + around)), piece))
         if piece == 256:
-            return best[1]
+            return [size for _, size in best]
         n += 1 + n // 8
 
 
@@ -897,7 +902,7 @@ def flagsparse_attention_paged_tree(q, lengths, token_indptr=None, *, parents=No
         tiles = min(-(-group * longest // of), 1 + group * tokens // (kv.batch * of))
         way = (kv.kv_heads << round(math.log2(tiles)), of)
         piece, pieces, firsts, longest_list, marked = kv._list(
-            sight, 512, 8192, _tree_ways(kv.kv_heads, group), way)
+            sight, 512, 8192, (way,) if prepared is None else _tree_ways(kv.kv_heads, group), way)
         n_pieces, need, room, by_tokens = pieces.shape[0], 0, None, 0
         if n_pieces > kv.batch:
             need = int(_abi.lib().fsp_attention_tree_counts(n_pieces, longest_list, kv.batch, kv.kv_heads,

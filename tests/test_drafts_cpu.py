@@ -227,3 +227,19 @@ def test_append_at_refusals_of_the_library():
     for args in ((c + base._append(), None, None), (None, None, 16), (c + base._append(half=33), 16, 16),
                  (c + base._append(k=0), None, 16)):
         assert L.fsp_paged_append_at(*args, None) == -1
+
+
+def test_sizes_of_pieces_of_several_ways():
+    # those of each way alone, the soonest end by the rule written out
+    rooms, slots, most = np.array([30064, 700, 0, 16, 9000, 4096], dtype=np.int64), 512, 8192
+    ways = attention._tree_ways(4, 3) + ((600, 32),)
+
+    def end_of(piece, each, rows):
+        held = sorted((min(piece, n - at) for n in rooms for at in range(0, n, piece)), key=lambda n: (n < piece, -n))
+        work = [n + 100 + 2 * rows for n in held for _ in range(each)]
+        return sum(work[::slots]) + max(sum(work) / slots, work[0])
+
+    sizes = attention._pieces_of(rooms, 0, ways, slots, most)
+    for (each, rows), size in zip(ways, sizes):
+        assert size == attention._piece_of(rooms, 0, each, slots, most, rows)
+        assert all(end_of(size, each, rows) <= end_of(piece, each, rows) for piece in (256, 1024, 7552, 8192))
