@@ -271,7 +271,7 @@ class PreparedPagedKV:
         # the pieces that attention is cut into
         self._piece = int(_abi.lib().fsp_attention_paged_piece(int(rooms.sum()), self.kv_heads))
         self._pieces, self._first, self._most = _on_device(
-            *_pieces(pages, self.page_size, self._piece), self._piece, k_pages.device)
+            [(*_pieces(pages, self.page_size, self._piece), self._piece)], k_pages.device)[0]
         self._counts = _abi.Calls()  # the pieces' counts of arrivals, by stream and number
         self._streams = _Streams()
         self._calls = _abi.Calls()
@@ -306,11 +306,11 @@ class PreparedPagedKV:
                 raise RuntimeError("a call's first run with this window and these heads builds its work lists, "
                                    "which cannot be captured: make one such call before the capture")
             sizes = dict(zip(ways, _pieces_of(self._held * self.page_size, sight, ways, slots, most)))
-            for piece in sorted(set(sizes.values())):
-                if (sight, piece) not in self._lists:
-                    table = _on_device(*_pieces(self._held, self.page_size, piece, sight), piece, self.device)
-                    # for good: captured graphs read it
-                    self._lists.setdefault((sight, piece), (piece, *table, _Streams()))
+            new = [piece for piece in sorted(set(sizes.values())) if (sight, piece) not in self._lists]
+            tables = _on_device([(*_pieces(self._held, self.page_size, piece, sight), piece) for piece in new],
+                                self.device)
+            for piece, table in zip(new, tables):  # for good: captured graphs read it
+                self._lists.setdefault((sight, piece), (piece, *table, _Streams()))
             torch.cuda.current_stream(self.device).synchronize()  # calls may come from other streams
             self._sizes[key] = sizes
         return self._lists[sight, sizes[way]]
@@ -367,13 +367,17 @@ def _pieces_of(rooms, sight, ways, slots, most):
         n += 1 + n // 8
 
 
-def _on_device(table, first, most, piece, device):
-    """The lists of _pieces on the device.  Long pieces first, for short ones to even out the end: 96 ragged
-    sequences of up to 4096 tokens, 8 heads of 128: 51 us, 55 in the sequences' order."""
-    held = np.minimum(piece, table[:, 4] - table[:, 1])
-    table = table[np.argsort(-held, kind="stable")]
-    both = torch.from_numpy(np.concatenate([table.ravel(), first])).to(device)
-    return both[:table.size].view(-1, 8), both[table.size:], most
+def _on_device(lists, device):
+    """Lists of _pieces and the tokens of a piece each, [(table, first pieces, most, piece)], on the device, in one
+    array.  Long pieces first, for short ones to even out the end: 96 ragged sequences of up to 4096 tokens, 8
+    heads of 128: 51 us, 55 in the sequences' order."""
+    tables = [table[np.argsort(-np.minimum(piece, table[:, 4] - table[:, 1]), kind="stable")].ravel()
+              for table, _, _, piece in lists]
+    parts = tables + [first for _, first, _, _ in lists]
+    if not parts:
+        return []
+    parts = torch.from_numpy(np.concatenate(parts)).to(device).split([len(part) for part in parts])
+    return [(parts[i].view(-1, 8), parts[len(lists) + i], most) for i, (_, _, most, _) in enumerate(lists)]
 
 
 def _pieces(pages, page_size, piece, sight=0):
