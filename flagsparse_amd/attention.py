@@ -691,8 +691,8 @@ def flagsparse_paged_copy(sources, targets, *, prepared=None, k_pages=None, v_pa
 
     A sequence that branches shares the pages that both only read by its page table, and has its last one
     copied.  ``sources``, ``targets``: [n], int32 or int64, numbers of the cache's pages; no page is the target
-    of two, and none that is a target is another's source.  The cache is given by ``prepared`` or by its
-    pages; with ``prepared`` nothing is waited for, so numbers are not checked: a pair with one outside the
+    of two, and none that is a target is another's source.  The cache is given by ``prepared``, for which any
+    table of these pages does (it is not read, so that one prepared cache serves all branches), or by its pages; with ``prepared`` nothing is waited for, so numbers are not checked: a pair with one outside the
     cache copies nothing."""
     key = None
     if prepared is not None:
@@ -850,8 +850,9 @@ def flagsparse_attention_paged_tree(q, lengths, token_indptr=None, *, parents=No
     differentiable.  With ``prepared`` nothing is waited for, so indices are not checked: rows of a
     sequence with more drafted tokens than ``longest``, or a length that its pages cannot hold or less than
     its drafted tokens, rows whose parents do not come earlier, and rows of no sequence are NaN.  What
-    is not finite in a hidden drafted token's value may reach other rows of its sequence (its weight is zero,
-    and zero times it is NaN), in its key it does not.  The first call with its window, sinks and number
+    is not finite in a value that a row does not see, but another row of its sequence does, may reach it (a drafted
+    token's off its way, or a token's of the text that only the windows of rows less deep hold: its weight is zero,
+    and zero times it is NaN); in a key it does not.  The first call with its window, sinks and number
     of heads builds work lists and cannot be captured; others, whatever their numbers of tokens, use them."""
     key = None
     if out is None and type(prepared) is PreparedPagedKV and type(scale) in _PLAIN and \

@@ -491,3 +491,62 @@ def test_other_numbers_of_drafts_use_the_same_lists(dev, heads, window, sinks):
             torch.cuda.synchronize()
             assert torch.equal(got, run())
     assert list(kv._lists) == lists
+
+
+def test_what_is_not_finite_between_the_windows_of_rows(dev):
+    # text that the windows of less deep rows hold and those of deeper rows do not
+    past, trees, window = [500, 40], [[-1, 0, 1, 2, 3, 4, 5], [-1, -1]], 100
+    kv, k, v = _cache(dev, [507, 42], 16, 2, 64, HF)
+    q, n = _normal(5, 9, 4, 64, dtype=HF).to(dev), torch.tensor([507, 42], device=dev)
+    parents, tokens = torch.tensor(sum(trees, []), device=dev), _indptr([7, 2], dev)
+
+    def call(**kw):
+        return fs.flagsparse_attention_paged_tree(q, n, tokens, parents=parents, prepared=kv, window=window, **kw)
+
+    def at(place):
+        return kv.indices[place // 16].long(), place % 16
+
+    clean = call()
+    for place, sees in ((400, 0), (401, 1), (403, 3), (407, 7)):  # position 500 + depth sees what is past 400 + depth
+        kv.k_pages[at(place)] = float("nan")
+        dirty = call()
+        assert torch.isnan(dirty[:sees]).all() and torch.equal(dirty[sees:], clean[sees:])
+        kv.k_pages[at(place)] = k[0][place].to(dev)
+        for bad in (float("nan"), float("inf")):
+            kv.v_pages[at(place)] = bad
+            dirty = call()
+            assert not torch.isfinite(dirty[:sees]).any() and torch.equal(dirty[7:], clean[7:])
+            if sees == 0:  # before all windows: not read
+                assert torch.equal(dirty, clean)
+        kv.v_pages[at(place)] = v[0][place].to(dev)
+    assert torch.equal(call(), clean)
+
+
+def test_the_ends_of_as_many_tokens_as_a_table_may_hold_count_once(dev):
+    # keys of score 0 in one page for all places but the first, one in the middle and the last, each of whose pages has
+    # one key that weighs as much as all others or more, at its first, an inner and its last place
+    page, times = 1 << 20, 2047
+    k, v = (torch.zeros(4, page, 1, 8, dtype=BF, device=dev) for _ in range(2))
+    v[0] = 1
+    table = torch.zeros(times, dtype=torch.int32, device=dev)
+    heavy = ((0, 1, 0, 8.0), (1000, 2, 777777, -8.0), (times - 1, 3, page - 1, 8.0))
+    for entry, which, slot, value in heavy:
+        table[entry] = which
+        v[which] = 1
+        k[which, slot], v[which, slot] = 2, value
+    kv = fs.prepare_paged_kv(k, v, torch.tensor([0, times], device=dev), table)
+    q = torch.full((1, 2, 8), 4.0, dtype=BF, device=dev)
+    q[0, 1] = 3.875
+    n = torch.tensor([page * times], dtype=torch.int32, device=dev)
+    out, lse = fs.flagsparse_attention_paged_tree(q, n, prepared=kv, return_lse=True)
+    others = page * times - 3
+    for head, x in enumerate((4.0, 3.875)):
+        w = math.exp(8 * 2 * x * 8**-0.5)
+        total = others + 3 * w
+        want = (others + w * sum(value for _, _, _, value in heavy)) / total
+        # sums in 32 bits of 2^18 pieces in turn, (2^18 + 2^15) 2^-24 and 2^-15 in a piece, less than 2^-5 of the sum,
+        # above and below; weights and the result are rounded to 8 bits.  A heavy key twice or
+        # not at all is off by twice as much
+        bound = (2 * 2.0**-5 + 2 * 2.0**-8) * (others + 24 * w) / total
+        assert float((out[0, head].double() - want).abs().max()) <= bound, (head, out[0, head], want, bound)
+        assert abs(float(lse[0, head]) - math.log(total)) <= 2.0**-5
