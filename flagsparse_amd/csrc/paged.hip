@@ -86,8 +86,10 @@ struct AppendShape {
 // there are few tokens.  Bound by memory for prompts (a read and a write of every element: 24 of up to 2000
 // tokens, 16 query and 16 key heads of 64, 111 MB in 20.8 us, 5.3 TB/s, part of it still in the
 // last-level cache) and by the chain token -> sequence -> page -> row for single tokens (16 tokens, 32
-// query and 8 key heads of 128: 3.8 us).  An element a thread took 48 us for those prompts.
-template <typename T, int MODE>
+// query and 8 key heads of 128: 3.8 us).  An element a thread took 48 us for those prompts.  AWAY: a token's position
+// may not be its place: it has a parent, or its text is longer than what the cache holds.  Looked for in all calls
+// that made the prompts 25.1 us a call instead of 23.4.
+template <typename T, int MODE, bool AWAY>
 __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(
     Cache c, AppendShape s, T* __restrict__ k_pages, T* __restrict__ v_pages,
     const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ q,
@@ -112,20 +114,24 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(
     b = __builtin_amdgcn_readfirstlane(max(b, 0));
     const int begin = tokens[b], end = tokens[b + 1];
     mine = begin <= t && t < end;
-    pos = (int64_t)lengths[b] - end + t;
-    turn = (int64_t)text[b] - end + t;
-    if (parents && mine && (begin < 0 || end > s.n_tokens)) mine = false;  // its parents are not there
-    if (parents && mine) {
-      depth = __builtin_amdgcn_readfirstlane(depth_of(parents + begin, (int)(t - begin), end - begin));
-      turn = (int64_t)text[b] - (end - begin) + depth;
+    pos = turn = (int64_t)lengths[b] - end + t;
+    if constexpr (AWAY) {
+      turn = (int64_t)text[b] - end + t;
+      if (parents && mine && (begin < 0 || end > s.n_tokens)) mine = false;  // its parents are not there
+      if (parents && mine) {
+        depth = __builtin_amdgcn_readfirstlane(depth_of(parents + begin, (int)(t - begin), end - begin));
+        turn = (int64_t)text[b] - (end - begin) + depth;
+      }
     }
   } else {
-    pos = (int64_t)lengths[b] - 1;
-    turn = (int64_t)text[b] - 1;
-    if (parents) depth = parents[t] == -1 ? 0 : -1;
+    pos = turn = (int64_t)lengths[b] - 1;
+    if constexpr (AWAY) {
+      turn = (int64_t)text[b] - 1;
+      if (parents) depth = parents[t] == -1 ? 0 : -1;
+    }
   }
   const int first = c.indptr[b], last = c.indptr[b + 1];
-  const bool ok = mine && depth >= 0 && pos >= 0 && turn >= 0 &&
+  const bool ok = mine && pos >= 0 && (!AWAY || (depth >= 0 && turn >= 0)) &&
                   pos < (int64_t)(last - first) * c.page_size && (MODE == kStill || turn < s.table_rows);
   int64_t page = 0, slot = 0;
   if (ok) {
@@ -568,13 +574,15 @@ int launch_append(const AppendCall& a, hipStream_t st) {
                       a.q_head,   a.q_out_token, a.q_out_head, (int)a.heads, (int)a.half, (int)a.table_rows,
                       a.interleaved != 0, (int)parts};
   constexpr int kWaves = kAppendThreads / kWave;
-  hipLaunchKernelGGL((paged_append_kernel<T, MODE>),
+  const int32_t* text = MODE == kStill ? a.lengths : a.text;
+  hipLaunchKernelGGL((a.parents || text != a.lengths ? paged_append_kernel<T, MODE, true>
+                                                     : paged_append_kernel<T, MODE, false>),
                      dim3((unsigned)((a.n_tokens * parts + kWaves - 1) / kWaves)),
                      dim3(kAppendThreads), 0, st, cache_of(a.cache), s,
                      static_cast<T*>(a.cache.k_pages), static_cast<T*>(a.cache.v_pages),
                      static_cast<const T*>(a.k), static_cast<const T*>(a.v),
                      static_cast<const T*>(a.q), static_cast<T*>(a.q_out), a.cos, a.sin,
-                     a.token_indptr, a.lengths, a.parents, MODE == kStill ? a.lengths : a.text);
+                     a.token_indptr, a.lengths, a.parents, text);
   return check_hip(hipGetLastError(), "paged_append_kernel launch");
 }
 
