@@ -207,12 +207,16 @@ struct PagedShape {
 // first ones that stay visible lay right before the others, so that it sees the places [first, last), and
 // place e is token e from ``old`` on and e - first before it.  So a window with first tokens costs what a window
 // that much longer does: 64 sequences of up to 60000 tokens, window 4096 and 64 first tokens, 8 heads of 128, 32
-// queries, 331 MB in 66 us, 5.0 TB/s of the 7.0 of a plain read (ragged: 2 rounds of workgroups).
+// queries, 331 MB in 66 us, 5.0 TB/s of the 7.0 of a plain read (ragged: 2 rounds of workgroups).  Without SINKS a
+// place is its token's: looked up in all calls the kernel took 9.8 us for 9.4 under a window of 1000.
+template <bool SINKS>
 struct Seen {
   int first, old;
   __device__ Seen(const PagedShape& s, int last)
-      : first(s.window ? (int)max((int64_t)last - s.window - s.sinks, (int64_t)0) : 0),
+      : first(!s.window ? 0 : SINKS ? (int)max((int64_t)last - s.window - s.sinks, (int64_t)0)
+                                    : max(last - s.window, 0)),
         old(s.window ? max(last - s.window, 0) : 0) {}
+  __device__ int token(int e) const { return SINKS && e < old ? e - first : e; }
 };
 
 // The next step's keys are asked for once this step's scores are made, its values once this step's
@@ -225,7 +229,7 @@ struct Seen {
 // 532 us, 6.1 TB/s of the 7.0 of a plain read, as for 256 of 4096, 32 queries; 96 ragged ones of up to
 // 4096, 200 MB, 44 us, 4.6 TB/s: less than two rounds of workgroups, each with the chain piece -> length
 // -> page -> keys before it.  For 1000 tokens that chain, the join and the launch are all of its 7.8 us.
-template <typename T, int DP, bool EXACT, bool NT>
+template <typename T, int DP, bool EXACT, bool NT, bool SINKS>
 __global__ __launch_bounds__(256, 3) void attention_paged_kernel(
     Cache c, PagedShape s, const Piece* __restrict__ pieces, const T* __restrict__ k_pages,
     const T* __restrict__ v_pages, const T* __restrict__ q, int64_t q_token, int64_t q_head,
@@ -254,11 +258,11 @@ __global__ __launch_bounds__(256, 3) void attention_paged_kernel(
   const bool ok = length >= 0 && length <= pc.room;
   // the query sees tokens [first, last); the sequence's pieces in use, and whether this is one
   const int last = ok ? length : 0;
-  const Seen seen(s, last);
+  const Seen<SINKS> seen(s, last);
   const int first = seen.first;
   const int p0 = first / s.piece, p1 = max(p0 + 1, (last + s.piece - 1) / s.piece);
   // under a window with first tokens the list counts from the first piece in use, and is as long as a window
-  const int skip = s.sinks ? p0 : 0, mine = pc.begin / s.piece + skip;
+  const int skip = SINKS ? p0 : 0, mine = pc.begin / s.piece + skip;
   if (mine < p0 || mine >= p1) return;
   const int begin = max(first, mine * s.piece);
   const int n = (int)min((int64_t)last, ((int64_t)mine + 1) * s.piece) - begin;
@@ -279,7 +283,7 @@ __global__ __launch_bounds__(256, 3) void attention_paged_kernel(
   const int padded = (n + 127) & ~127;
   for (int i = threadIdx.x; i < padded; i += 256) {
     const int e = begin + (i < n ? i : 0);
-    const uint32_t j = e < seen.old ? e - first : e;
+    const uint32_t j = seen.token(e);
     const uint32_t at = j / (uint32_t)c.page_size;
     const int64_t page = n > 0 ? c.indices[pc.page + at] : 0, slot = j - at * c.page_size;
     s_k[i] = page * c.k_page + slot * c.k_slot;
@@ -499,7 +503,7 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(
   const int length = lengths[b], room = (c.indptr[b + 1] - c.indptr[b]) * c.page_size;
   const int slot = first_piece[b];
   const int last = length >= 0 && length <= room ? length : 0;
-  const int first = Seen(s, last).first;
+  const int first = Seen<true>(s, last).first;
   const int p0 = first / s.piece, p1 = max(p0 + 1, (last + s.piece - 1) / s.piece), n = p1 - p0;
   if (n < 2) return;
   const int64_t at = (int64_t)(slot + (s.sinks ? 0 : p0)) * s.heads + h;
@@ -604,13 +608,13 @@ int64_t paged_workgroups(const fsp_attention_paged_args& a) {
   return a.n_pieces * a.cache.kv_heads * ((group + kHeadTile - 1) / kHeadTile);
 }
 
-template <typename T, int DP, bool EXACT, bool NT>
+template <typename T, int DP, bool EXACT, bool NT, bool SINKS>
 int launch_paged(const PagedCall& a, hipStream_t st) {
   const PagedShape s{(int)a.heads,    (int)a.window,  (int)a.piece,
                      (int)a.n_pieces, (float)a.scale, (int)a.sinks};
   float* part_o = static_cast<float*>(a.workspace);
   float* part_ml = part_o + a.n_pieces * a.heads * a.cache.dim;
-  hipLaunchKernelGGL((attention_paged_kernel<T, DP, EXACT, NT>), dim3((unsigned)paged_workgroups(a)),
+  hipLaunchKernelGGL((attention_paged_kernel<T, DP, EXACT, NT, SINKS>), dim3((unsigned)paged_workgroups(a)),
                      dim3(256), 0, st, cache_of(a.cache), s,
                      reinterpret_cast<const Piece*>(a.pieces),
                      static_cast<const T*>(a.cache.k_pages),
@@ -632,9 +636,10 @@ int launch_paged(const PagedCall& a, hipStream_t st) {
 template <typename T, int DP, bool EXACT>
 int launch_paged_nt(const PagedCall& a, hipStream_t st) {
   const int64_t bytes = a.cache.table_len * a.cache.page_size * a.cache.kv_heads * a.cache.dim * 4;
-  return bytes > (256 << 20) && a.heads / a.cache.kv_heads <= kHeadTile
-             ? launch_paged<T, DP, EXACT, true>(a, st)
-             : launch_paged<T, DP, EXACT, false>(a, st);
+  const bool nt = bytes > (256 << 20) && a.heads / a.cache.kv_heads <= kHeadTile;
+  if (a.sinks)
+    return nt ? launch_paged<T, DP, EXACT, true, true>(a, st) : launch_paged<T, DP, EXACT, false, true>(a, st);
+  return nt ? launch_paged<T, DP, EXACT, true, false>(a, st) : launch_paged<T, DP, EXACT, false, false>(a, st);
 }
 
 template <typename T>
