@@ -615,6 +615,22 @@ struct Jobs {
   __device__ int first_slot(int q_begin, int b) const {
     return (int)(((uint32_t)q_begin << (twice ? 1 : 0)) / (uint32_t)chunk) + (twice ? 0 : b);
   }
+  // Whether a sequence's first keys go to jobs.  Those that need no sums do too where they have a slot: they are more
+  // work than most tiles of the list, and so start before them (6 sequences up to 1501, 4 key heads of 96: 24.0 / 23.9 us).
+  __device__ bool takes(const Tile& t) const { return t.nq > chunk || (slots > 0 && !twice && t.nq > 0); }
+  // The last sequence whose slots start at or before this one, the same in a wave: 64 of those it may be at a look.
+  __device__ int sequence_of(int slot) const {
+    const int lane = threadIdx.x & 63;
+    int b = 0;
+    for (int n = batch; n > 1;) {  // it is one of n from b on
+      const int step = (n + kWave - 1) / kWave, of = b + min(lane * step, n - 1);
+      const bool in = lane * step < n && first_slot(sequences[of].q_begin, of) <= slot;
+      const int count = max(__popcll(__ballot(in)), 1);  // b itself starts no later
+      b += (count - 1) * step;
+      n = min(step, n - (count - 1) * step);
+    }
+    return __builtin_amdgcn_readfirstlane(b);
+  }
 };
 
 template <int ROWS>
@@ -631,25 +647,18 @@ __device__ __forceinline__ bool job_of(const Jobs& jobs, const Shape& s, int spl
   g = n % per;
   n /= per;
   slot = n % jobs.slots;
-  const int at = n / jobs.slots * ROWS, lane = threadIdx.x & 63;
+  const int at = n / jobs.slots * ROWS;
   if (at / ROWS >= jobs.tiles) return false;
-  int b = 0;  // the last sequence whose slots start at or before this one, 64 at a look
-  for (int i = 0; i < jobs.batch; i += kWave) {
-    const int of = min(i + lane, jobs.batch - 1);
-    const bool in = i + lane < jobs.batch && jobs.first_slot(jobs.sequences[of].q_begin, of) <= slot;
-    const int count = __popcll(__ballot(in));
-    b += count;
-    if (count < kWave) break;
-  }
-  b = __builtin_amdgcn_readfirstlane(b - 1);
+  const int b = jobs.sequence_of(slot);
   t = jobs.sequences[b];
   const int64_t begin = (int64_t)(slot - jobs.first_slot(t.q_begin, b)) * jobs.chunk;
   t.first = t.k_begin + at;
   t.at = at;
   t.rows = min(ROWS, t.nk - at);
-  if (t.nq <= jobs.chunk || begin >= t.nq || at >= min(t.nk, s.sinks)) return false;
+  if (begin >= t.nq || at >= min(t.nk, s.sinks) || !jobs.takes(t)) return false;
   from = (int)begin;
   to = (int)min(begin + jobs.chunk, (int64_t)t.nq);
+  if (t.nq <= jobs.chunk) slot = -1;  // nothing to add: as a tile of the list
   return true;
 }
 
@@ -681,7 +690,7 @@ __global__ __launch_bounds__(64 * BLOCKS * PARTS, 2) void attention_grad_kv_kern
   } else {
     tile_and_head(blockIdx.x - (SINKS ? jobs.blocks : 0), n_tiles, s.kv_heads * split, tile, g);
     t = tiles[tile];
-    if (SINKS && t.at < s.sinks && t.nq > jobs.chunk) return;
+    if (SINKS && t.at < s.sinks && jobs.takes(t)) return;
   }
   const int share = g % split;  // of the group's heads
   g /= split;
@@ -943,9 +952,11 @@ __global__ __launch_bounds__(256) void attention_grad_sinks_sum_kernel(
   }
   const int quads = s.dim / 4, per = 2 * jobs.tiles * ROWS * quads, blocks = (per + 255) / 256;
   const int i = (blockIdx.x % blocks) * 256 + threadIdx.x;
-  const int g = blockIdx.x / blocks % s.kv_heads, b = blockIdx.x / blocks / s.kv_heads;
-  if (i >= per) return;
+  const int g = blockIdx.x / blocks % s.kv_heads, of_all = blockIdx.x / blocks / s.kv_heads;
+  const int b = jobs.twice ? jobs.sequence_of(of_all) : of_all;  // of few slots beside sequences, or of sequences
   const Tile t = jobs.sequences[b];
+  const int first = jobs.first_slot(t.q_begin, b);
+  if (i >= per || (jobs.twice && first != of_all)) return;
   const int d = i % quads * 4, of = i / quads;
   const bool keys = of >= jobs.tiles * ROWS;
   const int row = keys ? of - jobs.tiles * ROWS : of;
@@ -954,7 +965,6 @@ __global__ __launch_bounds__(256) void attention_grad_sinks_sum_kernel(
   int lot, hit;
   seen_of(s, t, row / ROWS * ROWS, lot, hit);
   f32x4 y{};
-  const int first = jobs.first_slot(t.q_begin, b);
   const int from = (uint32_t)lot / (uint32_t)jobs.chunk, last = (uint32_t)(t.nq - 1) / (uint32_t)jobs.chunk;
   if (lot < t.nq)
     for (int c = from; c <= last; ++c)
@@ -1155,7 +1165,8 @@ int launch_grad_kv(const Call& a, int split, hipStream_t st) {
   if (int rc = check_hip(hipGetLastError(), "attention_grad_kv_kernel launch")) return rc;
   const int64_t quads = split > 1 ? a.kv_heads * a.k_tokens * a.dim / 2 : 0;
   if (SINKS && jobs.slots > 0) {
-    const int64_t of_jobs = (2 * jobs.tiles * 32 * BLOCKS * (a.dim / 4) + 255) / 256 * a.kv_heads * a.batch;
+    const int64_t of_jobs = (2 * jobs.tiles * 32 * BLOCKS * (a.dim / 4) + 255) / 256 * a.kv_heads *
+                            (jobs.twice ? jobs.slots : a.batch);
     hipLaunchKernelGGL((attention_grad_sinks_sum_kernel<T, 32 * BLOCKS>),
                        dim3((unsigned)(of_jobs + (quads + 255) / 256)), dim3(256), 0, st, shape_of(a), split,
                        jobs, (int)of_jobs, sums, a.k_tokens, static_cast<T*>(a.grad_k), a.grad_k_token,
@@ -1272,6 +1283,21 @@ int run_forward(const Call& a, const std::string& who, void* stream) {
 
 int run_backward(const Call& a, const std::string& who, void* stream) {
   if (int rc = check_packed(a, who)) return rc;
+  if (a.sinks && a.n_k_tiles > 0) {
+    if (a.batch < 1 || !a.sequences) return set_error(FSP_EINVAL, who + ": sequences");
+    // tiles of 32 keys, the most jobs
+    const int64_t firsts = first_keys(a.sinks, a.k_longest), tiles = (firsts + kRows / 2 - 1) / (kRows / 2);
+    const int64_t all = kMaxBlocks / a.heads - a.n_k_halves - 8;
+    const int64_t batch = has_jobs(a) ? a.batch : 1, chunk = chunk_of(a.window, firsts);
+    const int64_t slots = job_slots(a.q_tokens, batch, chunk);
+    // the vectors of a sequence's sums, which are counted in 32 bits, and the workgroups that add or look at them;
+    // those that add the shares of other keys are few, as shares are made where tiles are
+    const int64_t vectors = 2 * ((firsts + kRows - 1) / kRows * kRows) * (a.dim / 4);
+    const int64_t sums = slots_twice(a.q_tokens, batch, chunk) ? slots : batch;
+    if (a.batch > 0x7fffffffLL || (tiles > 0 && slots > all / tiles) || vectors > (1 << 30) ||
+        sums > (kMaxBlocks - (1 << 16)) / a.kv_heads / (vectors / 256 + 1))
+      return set_error(FSP_EINVAL, who + ": sinks of so many sequences");
+  }
   // without queries, and with one share of the heads, there is nothing to keep
   const bool work = a.n_k_tiles > 0 && (has_jobs(a) || fsp_attention_packed_workspace(
       a.n_k_tiles, a.heads, a.kv_heads, a.dim, a.q_tokens, a.k_tokens, a.causal && !a.window) > 0);
@@ -1285,16 +1311,6 @@ int run_backward(const Call& a, const std::string& who, void* stream) {
       !aligned16(a.grad_k, a.grad_k_token, a.grad_k_head) ||
       !aligned16(a.grad_v, a.grad_v_token, a.grad_v_head))
     return set_error(FSP_EINVAL, who + ": rows must be 16-byte aligned");
-  if (a.sinks && a.n_k_tiles > 0) {
-    if (a.batch < 1 || !a.sequences) return set_error(FSP_EINVAL, who + ": sequences");
-    // tiles of 32 keys, the most jobs
-    const int64_t firsts = first_keys(a.sinks, a.k_longest), tiles = (firsts + kRows / 2 - 1) / (kRows / 2);
-    const int64_t all = kMaxBlocks / a.heads - a.n_k_halves - 8, batch = has_jobs(a) ? a.batch : 1;
-    if (a.batch > 0x7fffffffLL ||
-        (tiles > 0 && job_slots(a.q_tokens, batch, chunk_of(a.window, firsts)) > all / tiles) ||
-        batch > kMaxBlocks / 4 / a.kv_heads / (tiles * (kRows / 2) * (a.dim / 4) / 128 + 1))  // and of 2^31 vectors
-      return set_error(FSP_EINVAL, who + ": sinks of so many sequences");
-  }
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (a.sinks)
     return a.dtype == FSP_BF16 ? launch_backward_dim<bf16, true>(a, st) : launch_backward_dim<f16, true>(a, st);

@@ -429,3 +429,14 @@ def test_first_keys_that_reach_the_window_are_the_causal_call(dev):
             assert all(torch.equal(a, b) for a, b in zip(want, got))
     hidden = both(window=500, sinks=42)  # one key of one query
     assert not torch.equal(hidden[0][832], want[0][832])
+
+
+@pytest.mark.parametrize("batch", [70, 5000])
+def test_jobs_among_very_many_sequences(dev, batch):
+    # their sequences are searched for, 64 at a look, and again where there are more
+    lengths = [1 + i % 3 for i in range(batch)]
+    for at, n in ((0, 700), (batch // 2, 1100), (batch - 1, 513)):
+        lengths[at] = n
+    _both(dev, lengths, lengths, 2, 1, 64, BF, 2, 1)
+    lengths = [0] * (batch // 2) + [900] + [0] * batch + [2, 600, 0]
+    _both(dev, lengths, lengths, 2, 1, 64, HF, 30, 40)

@@ -162,3 +162,32 @@ def test_workspace_of_short_sequences():
                 go=0)
     assert L.fsp_attention_packed_sinks_backward(base._packed(**args), 4, 64, 10**6, None) == -1
     assert b"null pointer" in L.fsp_last_error()
+
+
+@pytest.mark.parametrize("batch,q_longest", [(10**6, 64), (10**6, 5000), (200_000, 5000)])
+def test_as_many_sequences_as_there_are(batch, q_longest):
+    # with jobs and without: what is launched for the first keys' sums goes by the queries
+    args = dict(window=32, heads=32, kv_heads=8, dim=128, q_tokens=2 * 10**7, k_tokens=2 * 10**7, go=0,
+                q_longest=q_longest, k_longest=q_longest)
+    assert _abi.lib().fsp_attention_packed_sinks_backward(base._packed(**args), 4, 64, batch, None) == -1
+    assert b"null pointer" in _abi.lib().fsp_last_error()
+
+
+@pytest.mark.parametrize("batch", [1, 2, 63, 64, 65, 130, 4096, 4097, 9000])
+def test_search_for_the_sequence_of_a_slot(batch):
+    # 64 at a look of the first slots, as the kernels do it
+    rng = np.random.default_rng(batch)
+    for twice in (False, True):
+        q_len = rng.integers(0, 3, batch) * rng.integers(0, 900, batch)
+        begin = np.cumsum(q_len) - q_len
+        first = 2 * begin // 512 if twice else begin // 512 + np.arange(batch)
+        for slot in {0, int(first[-1]), int(first[-1]) + 3, *rng.integers(0, first[-1] + 2, 40).tolist()}:
+            b, n = 0, batch
+            while n > 1:
+                step = -(-n // 64)
+                looks = [b + lane * step for lane in range(64) if lane * step < n]
+                seen = [bool(first[i] <= slot) for i in looks]
+                count = sum(seen)
+                assert count >= 1 and all(seen[:count])
+                b, n = b + (count - 1) * step, min(step, n - (count - 1) * step)
+            assert b == int(np.nonzero(first <= slot)[0][-1])
