@@ -348,12 +348,17 @@ template <typename T>
 int launch_copy(const fsp_paged_cache& c, const int32_t* sources, const int32_t* targets, int64_t n,
                 hipStream_t st) {
   const int64_t steps = (c.page_size * c.kv_heads * (c.dim / 8) + kThreads - 1) / kThreads;
-  int64_t parts = (4096 + 2 * n - 1) / (2 * n);
-  if (parts > steps) parts = steps;
-  hipLaunchKernelGGL((paged_copy_kernel<T>), dim3((unsigned)(2 * n * parts)), dim3(kThreads), 0, st,
-                     cache_of(c), (int)c.n_pages, static_cast<T*>(c.k_pages), static_cast<T*>(c.v_pages),
-                     sources, targets, (int)parts);
-  return check_hip(hipGetLastError(), "paged_copy_kernel launch");
+  constexpr int64_t kMost = kMaxBlocks / 4;  // pages of a launch
+  for (; n > 0; n -= kMost, sources += kMost, targets += kMost) {
+    const int64_t here = n < kMost ? n : kMost;
+    int64_t parts = (4096 + 2 * here - 1) / (2 * here);
+    if (parts > steps) parts = steps;
+    hipLaunchKernelGGL((paged_copy_kernel<T>), dim3((unsigned)(2 * here * parts)), dim3(kThreads), 0, st,
+                       cache_of(c), (int)c.n_pages, static_cast<T*>(c.k_pages), static_cast<T*>(c.v_pages),
+                       sources, targets, (int)parts);
+    if (int rc = check_hip(hipGetLastError(), "paged_copy_kernel launch")) return rc;
+  }
+  return FSP_OK;
 }
 
 }  // namespace
@@ -408,7 +413,7 @@ extern "C" int fsp_paged_copy(const fsp_paged_cache* cache, const int32_t* sourc
                               int64_t n, void* stream) {
   if (!cache) return set_error(FSP_EINVAL, "fsp_paged_copy: null arguments");
   if (int rc = check_cache(*cache, "fsp_paged_copy")) return rc;
-  if (n < 0 || n > kMaxBlocks / 4 || cache->page_size * cache->kv_heads > (1 << 30) / (cache->dim / 8))
+  if (n < 0 || n > 0x7fffffffLL || cache->page_size * cache->kv_heads > (1 << 30) / (cache->dim / 8))
     return set_error(FSP_EINVAL, "fsp_paged_copy: size out of range");
   if (n == 0) return FSP_OK;
   if (!sources || !targets || (cache->n_pages > 0 && (!cache->k_pages || !cache->v_pages)))

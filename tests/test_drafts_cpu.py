@@ -243,3 +243,9 @@ def test_sizes_of_pieces_of_several_ways():
     for (each, rows), size in zip(ways, sizes):
         assert size == attention._piece_of(rooms, 0, each, slots, most, rows)
         assert all(end_of(size, each, rows) <= end_of(piece, each, rows) for piece in (256, 1024, 7552, 8192))
+
+
+def test_copies_of_as_many_pages_as_there_are():
+    L, c = _abi.lib(), base._cache(page_size=1, n_pages=2**31 - 1)
+    assert L.fsp_paged_copy(c, None, 16, 2**31 - 1, None) == -1 and b"null pointer" in L.fsp_last_error()
+    assert L.fsp_paged_copy(c, None, 16, 2**31, None) == -1 and b"out of range" in L.fsp_last_error()

@@ -633,3 +633,16 @@ def test_texts_as_long_as_the_cache_holds_are_the_call_without(dev):
         got = fs.flagsparse_paged_append(k, v, n, tokens, parents=parents, text_lengths=n, **kw)
         assert torch.equal(got, want) and torch.equal(_bits(kv.k_pages), now)
         kv.k_pages.view(torch.int16).copy_(kept)
+
+
+def test_copies_of_more_pages_than_one_launch_has(dev):
+    n = 4_500_000
+    x = torch.arange(2 * n, dtype=torch.int32, device=dev).view(torch.bfloat16).view(2 * n, 1, 1, 2)
+    k = torch.cat([x] * 4, -1)
+    v = k.view(torch.int16).bitwise_not().view(torch.bfloat16)
+    want = [t.view(torch.int16)[n:].flip(0).clone() for t in (k, v)]
+    at = torch.arange(n, dtype=torch.int32, device=dev)
+    kv = fs.prepare_paged_kv(k, v, torch.zeros(1, dtype=torch.int32, device=dev), at[:0])
+    fs.flagsparse_paged_copy(2 * n - 1 - at, at, prepared=kv)
+    for t, w in zip((k, v), want):
+        assert torch.equal(t.view(torch.int16)[:n], w) and torch.equal(t.view(torch.int16)[n:], w.flip(0))
