@@ -172,17 +172,17 @@ constexpr int kSpan = kWave;
 
 template <typename T, bool COUNTED>
 __global__ __launch_bounds__(kThreads) void paged_keep_into_kernel(
-    Cache c, KeepShape s, const Piece* __restrict__ pieces, int piece_size, const T* __restrict__ k_pages,
-    const T* __restrict__ v_pages, T* __restrict__ to_k, T* __restrict__ to_v,
+    Cache c, KeepShape s, int first_block, const Piece* __restrict__ pieces, int piece_size,
+    const T* __restrict__ k_pages, const T* __restrict__ v_pages, T* __restrict__ to_k, T* __restrict__ to_v,
     const uint8_t* __restrict__ keep, const int32_t* __restrict__ tokens,
     const int32_t* __restrict__ lengths, int32_t* __restrict__ kept, const int32_t* __restrict__ counts,
     const int32_t* __restrict__ totals) {
   constexpr int U = 8;
   __shared__ int64_t s_from[2][kSpan], s_to[2][kSpan];  // where keys and values lie, and go
   __shared__ int s_before[4], s_all[4], s_n;
-  const int parts = piece_size / kSpan;
-  const Piece pc = pieces[blockIdx.x / parts];
-  const int b = pc.seq, at = pc.begin + (int)(blockIdx.x % parts) * kSpan;
+  const int parts = piece_size / kSpan, block = first_block + (int)blockIdx.x;
+  const Piece pc = pieces[block / parts];
+  const int b = pc.seq, at = pc.begin + block % parts * kSpan;
   const Marked m(tokens, s.each, s.n_tokens, b, lengths[b], pc.room);
   const int length = m.past + m.count;
   if (at >= length && at > 0) return;
@@ -336,12 +336,17 @@ int launch_keep(const KeepCall& a, hipStream_t st) {
                        cache_of(a.cache), (int)a.piece, a.first_piece, a.lengths, a.counts, totals);
     if (int rc = check_hip(hipGetLastError(), "paged_keep_before_kernel launch")) return rc;
   }
-  hipLaunchKernelGGL((a.counts ? paged_keep_into_kernel<T, true> : paged_keep_into_kernel<T, false>),
-                     dim3((unsigned)(a.n_pieces * (a.piece / kSpan))), dim3(kThreads), 0, st, cache_of(a.cache),
-                     s, pieces, (int)a.piece, static_cast<const T*>(a.cache.k_pages),
-                     static_cast<const T*>(a.cache.v_pages), static_cast<T*>(to.k_pages),
-                     static_cast<T*>(to.v_pages), a.keep, a.token_indptr, a.lengths, a.kept, a.counts, totals);
-  return check_hip(hipGetLastError(), "paged_keep_into_kernel launch");
+  const int64_t blocks = a.n_pieces * (a.piece / kSpan);
+  for (int64_t first = 0; first < blocks; first += kMaxBlocks) {  // one launch, but for tables of more than 2^30 tokens
+    const int64_t n = blocks - first < kMaxBlocks ? blocks - first : kMaxBlocks;
+    hipLaunchKernelGGL((a.counts ? paged_keep_into_kernel<T, true> : paged_keep_into_kernel<T, false>),
+                       dim3((unsigned)n), dim3(kThreads), 0, st, cache_of(a.cache), s, (int)first, pieces,
+                       (int)a.piece, static_cast<const T*>(a.cache.k_pages),
+                       static_cast<const T*>(a.cache.v_pages), static_cast<T*>(to.k_pages),
+                       static_cast<T*>(to.v_pages), a.keep, a.token_indptr, a.lengths, a.kept, a.counts, totals);
+    if (int rc = check_hip(hipGetLastError(), "paged_keep_into_kernel launch")) return rc;
+  }
+  return FSP_OK;
 }
 
 template <typename T>
@@ -384,7 +389,7 @@ int run_keep(const KeepCall& a, const std::string& who, void* stream) {
         a.into.batch != a.cache.batch)
       return set_error(FSP_EINVAL, who + ": the caches differ in type, heads, dim or sequences");
     if (a.piece < 128 || a.piece > kList || a.piece % 128 || a.n_pieces < a.cache.batch || !a.pieces ||
-        a.n_pieces > kMaxBlocks / (a.piece / kSpan) ||
+        a.n_pieces > kMaxBlocks || a.n_pieces > 0x7fffffff / (a.piece / kSpan) ||
         a.cache.kv_heads * (a.cache.dim / 8) > 0x7fffffff / kSpan)
       return set_error(FSP_EINVAL, who + ": pieces");
   }

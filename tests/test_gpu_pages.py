@@ -646,3 +646,18 @@ def test_copies_of_more_pages_than_one_launch_has(dev):
     fs.flagsparse_paged_copy(2 * n - 1 - at, at, prepared=kv)
     for t, w in zip((k, v), want):
         assert torch.equal(t.view(torch.int16)[:n], w) and torch.equal(t.view(torch.int16)[n:], w.flip(0))
+
+
+def test_keep_of_more_tokens_than_one_launch_has(dev):
+    # the same page for all places, here and there: as long as none but the last is dropped, places do not change
+    page, times = 1 << 20, 1100
+    kp, vp = (_normal(s, 1, page, 1, 8, dtype=BF).to(dev) for s in (1, 2))
+    table = torch.zeros(times, dtype=torch.int32, device=dev)
+    ends = torch.tensor([0, times], device=dev)
+    kv = fs.prepare_paged_kv(kp, vp, ends, table)
+    k2, v2 = torch.zeros_like(kp), torch.zeros_like(vp)
+    to = fs.prepare_paged_kv(k2, v2, ends, table)
+    n = torch.tensor([page * times], dtype=torch.int32, device=dev)
+    got = fs.flagsparse_paged_keep(torch.tensor([True, True, False], device=dev), n, prepared=kv, into=to)
+    assert got.tolist() == [page * times - 1]
+    assert torch.equal(k2, kp) and torch.equal(v2, vp)
