@@ -50,10 +50,10 @@ _PACKED, _PACKED_AT = struct.Struct("10qd24q"), struct.Struct("10q")
 _KEEP, _KEEP_AT = struct.Struct("5q"), struct.Struct("5q")
 _TREE, _TREE_AT = struct.Struct("6qd7q"), struct.Struct("8q")
 
-# Where a text may have more marks than so many, they are counted by pieces before it is kept into other pages, by two
-# more launches.  Without and with that, half of the tokens kept, us: 16 texts of 8192, 8 heads of 128 120 / 124, 16 of
-# 16384 224 / 226, 8 of 32768 236 / 226, 4 of 131072 600 / 430; one head of 64, a text of 16384 12 / 19, of 32768 15 / 19,
-# 8 of 16384 26 / 21, one of 131072 79 / 22, of 2^20 3482 / 112.
+# Where a text may have more marks than so many, they are counted by pieces before it is kept into other pages, by
+# two more launches.  Without and with that, half of the tokens kept, us: 16 texts of 8192, 8 heads of 128 120 / 124,
+# 16 of 16384 224 / 226, 8 of 32768 236 / 226, 4 of 131072 600 / 430; one head of 64, a text of 16384 12 / 19, of
+# 32768 15 / 19, 8 of 16384 26 / 21, one of 131072 79 / 22, of 2^20 3482 / 112.
 _COUNTED_FROM = 16384
 
 # A prepared object keeps the first part for each layout of arrays that it has checked, so that the
@@ -333,15 +333,15 @@ def _piece_of(rooms, sight, each, slots, most, rows):
 
 
 def _pieces_of(rooms, sight, ways, slots, most):
-    """For each of the ``ways``, (workgroups of a piece, rows of each), the tokens of a piece, from 256 to ``most``, by
-    which the pieces of all sequences end soonest.  A workgroup takes as long as its tokens, and 100 + 2 * rows for
-    what it does before and after them (its sums are written and read again); all of them take something between their sum over the
-    ``slots`` and rounds of ``slots`` that wait for each other.  Mostly that gives whole rounds of even pieces: 8
-    sequences of 30064, 8 key heads, 256 rows beside each (16 workgroups a piece), pieces of 2048 / 3840 /
-    4096 / 5120 / 7552 (one round) / 10112 tokens 391 / 368 / 373 / 379 / 361 / 398 us; 96 ragged ones of up to
-    8000, 32 rows, of 256 / 512 / 1024 / 2048 / 4096 111 / 98 / 90 / 87 / 89 us, 128 rows 152 / 131 / 116 / 112 /
-    142; 33 ragged ones under a window of 2047, 23 heads of 80, up to 26 tokens, of 128 / 256 / 512 / 1024
-    35 / 28 / 32 / 40."""
+    """For each of the ``ways``, (workgroups of a piece, rows of each), the tokens of a piece, from 256 to ``most``,
+    by which the pieces of all sequences end soonest.  A workgroup takes as long as its tokens, and 100 + 2 * rows
+    for what it does before and after them (its sums are written and read again); all of them take something
+    between their sum over the ``slots`` and rounds of ``slots`` that wait for each other.  Mostly that gives whole
+    rounds of even pieces: 8 sequences of 30064, 8 key heads, 256 rows beside each (16 workgroups a piece), pieces
+    of 2048 / 3840 / 4096 / 5120 / 7552 (one round) / 10112 tokens 391 / 368 / 373 / 379 / 361 / 398 us; 96 ragged
+    ones of up to 8000, 32 rows, of 256 / 512 / 1024 / 2048 / 4096 111 / 98 / 90 / 87 / 89 us, 128 rows 152 / 131 /
+    116 / 112 / 142; 33 ragged ones under a window of 2047, 23 heads of 80, up to 26 tokens, of 128 / 256 / 512 /
+    1024 35 / 28 / 32 / 40."""
     seen = np.minimum(rooms, sight) if sight else rooms
     longest, tokens = int(seen.max(initial=0)), int(seen.sum())
     best = [(float("inf"), 256)] * len(ways)
@@ -607,11 +607,12 @@ def flagsparse_paged_keep(keep, lengths, token_indptr=None, *, prepared=None, k_
     ``keep``: [tokens], bool, the marks of the last tokens of each sequence one after the other: sequence
     b's are ``token_indptr[b]`` to ``token_indptr[b + 1]`` (None: as many for each), as many as it may have;
     ``lengths[b]`` is what sequence b holds.  The marked ones stay, in their order, and close up behind the
-    tokens before them: in place, where the pages they move in belong to one sequence each, or in the pages of
-    ``into``, another PreparedPagedKV with as many sequences, heads and dims, to which the tokens before them are
-    copied too (pages that the call does not read; several may lie in the same arrays).  Keys stay rotated as they
-    are: after a text whose tokens were given up go others by flagsparse_paged_append with ``text_lengths``.  A
-    window of the attention, and its first tokens, go by places in the cache.
+    tokens before them: in place, where the pages they move in belong to one sequence each (a chain of steps, made for
+    drafted tokens: of a long text ``into`` takes a small part of the time), or in the pages of ``into``, another
+    PreparedPagedKV with as many sequences, heads and dims, to which the tokens before them are copied too (pages
+    that the call does not read; several may lie in the same arrays).  Keys stay rotated as they are: after a text
+    whose tokens were given up go others by flagsparse_paged_append with ``text_lengths``.  A window of the
+    attention, and its first tokens, go by places in the cache.
 
     Returns the new lengths, int32.  With ``prepared`` nothing is waited for, so lengths are not checked: where
     one is more than its pages hold or less than its marked tokens, or ``into`` has no room for
@@ -692,8 +693,9 @@ def flagsparse_paged_copy(sources, targets, *, prepared=None, k_pages=None, v_pa
     A sequence that branches shares the pages that both only read by its page table, and has its last one
     copied.  ``sources``, ``targets``: [n], int32 or int64, numbers of the cache's pages; no page is the target
     of two, and none that is a target is another's source.  The cache is given by ``prepared``, for which any
-    table of these pages does (it is not read, so that one prepared cache serves all branches), or by its pages; with ``prepared`` nothing is waited for, so numbers are not checked: a pair with one outside the
-    cache copies nothing."""
+    table of these pages does (it is not read, so that one prepared cache serves all branches), or by its pages;
+    with ``prepared`` nothing is waited for, so numbers are not checked: a pair with one outside the cache copies
+    nothing."""
     key = None
     if prepared is not None:
         if not isinstance(prepared, PreparedPagedKV):
@@ -744,10 +746,10 @@ def flagsparse_attention_paged(q, lengths, *, prepared=None, k_pages=None, v_pag
     ``q``: [sequences, heads, dim]; ``lengths[b]``: the tokens that sequence b holds, the query's
     own among them (0: the sequence is empty, and its output is zeros).  ``window``: only the last
     ``window`` tokens are seen, and with ``sinks`` the first ``sinks`` too (the first call with such a window
-    and as many heads builds a work list and cannot be captured).  ``scale``: dim ** -0.5 by default.  Returns [sequences, heads, dim],
-    with the float32 log-sum-exp [sequences, heads] if ``return_lse``; neither is differentiable, nor
-    is what flagsparse_paged_append gives.  With ``prepared`` nothing is
-    waited for, so lengths are not checked: one that its sequence's pages cannot hold gives NaN."""
+    and as many heads builds a work list and cannot be captured).  ``scale``: dim ** -0.5 by default.  Returns
+    [sequences, heads, dim], with the float32 log-sum-exp [sequences, heads] if ``return_lse``; neither is
+    differentiable, nor is what flagsparse_paged_append gives.  With ``prepared`` nothing is waited for, so lengths
+    are not checked: one that its sequence's pages cannot hold gives NaN."""
     key = None
     if out is None and type(prepared) is PreparedPagedKV and type(scale) in _PLAIN and \
             type(window) in _PLAIN and type(sinks) in _PLAIN:

@@ -377,9 +377,14 @@ __device__ __forceinline__ int lower(f32x16& y, f32x16 (&acc)[NT]) {
 constexpr int kFewKeys = 128;
 // Under a window with first tokens, where no query may come to see many, the rule is finer: by what a tile's first
 // query sees, and by the dim, as what the output's rounding does to delta against what one rounding does to
-// the gradient falls with its root.  The same ratio without and with delta made anew, 2000 tokens, 264 keys a
-// query: dim 40 1.53 / 1.45, 64 1.50 / 1.45, 96 1.47 / 1.43; dim 64, 404 and 1204 keys: 1.50, 1.47 without.  It takes
-// about a third of this kernel's time: 6 sequences up to 1501, 270 keys, 12 heads of 96 21 / 29 us.
+// the gradient falls with its root.  The same ratio without it, of rows that see 140 / 300 / 500 / 700 / 1200 / 1600
+// keys, the mean of both types: dim 48 1.53 / 1.50 / 1.51 / 1.50 / 1.50 / 1.51, 64 1.51 / 1.51 / 1.50 / 1.49 / 1.49 /
+// 1.49, 72 1.51 / 1.51 / 1.48 / 1.48 / 1.48 / 1.47, 80 1.50 / 1.48 / 1.47 / 1.49 / 1.48 / 1.47, 96 1.50 / 1.48 / 1.48 /
+// 1.46 / 1.47 / 1.46, 128 1.49 / 1.47 / 1.47 / 1.45 / 1.46 / 1.45, some 0.02 up or down from case to case; with it
+// 1.42 to 1.47 everywhere.  There is no step in that: it is made anew up to the power of two from which on the mean is
+// below 1.50 without (dims below 64 never get there).  This kernel with delta made anew by no tile / by this rule / by
+// all: four sequences of 4096, 16 heads of 64, 528 keys a query 72.5 / 81.7 / 114.5 us; 6 up to 1501, 12 heads of 96,
+// 270 keys, where the longest tile is all of it, 18.9 / 27.8 / 27.6.
 __device__ __forceinline__ bool delta_anew(int dim, int seen) {
   return seen <= 256 || dim < 64 || (dim < 80 && seen <= 512);
 }
@@ -616,7 +621,8 @@ struct Jobs {
     return (int)(((uint32_t)q_begin << (twice ? 1 : 0)) / (uint32_t)chunk) + (twice ? 0 : b);
   }
   // Whether a sequence's first keys go to jobs.  Those that need no sums do too where they have a slot: they are more
-  // work than most tiles of the list, and so start before them (6 sequences up to 1501, 4 key heads of 96: 24.0 / 23.9 us).
+  // work than most tiles of the list, and so start before them (6 sequences up to 1501, 4 key heads of 96: 24.0 /
+  // 23.9 us).
   __device__ bool takes(const Tile& t) const { return t.nq > chunk || (slots > 0 && !twice && t.nq > 0); }
   // The last sequence whose slots start at or before this one, the same in a wave: 64 of those it may be at a look.
   __device__ int sequence_of(int slot) const {

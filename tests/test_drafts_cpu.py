@@ -191,7 +191,8 @@ def test_partial_sums_by_tokens():
     assert L.fsp_attention_tree_by_tokens_workspace(16, 512, 32, 128) == 16 * 512 * 32 * 130 * 4
     assert L.fsp_attention_tree_workspace(1024, 32, 128, 256) == 32 * 16 * 512 * 32 * 130 * 4
     assert L.fsp_attention_tree_by_tokens_workspace(-1, 512, 32, 128) == 0
-    assert L.fsp_attention_tree_by_tokens_workspace(2000, 2**31 - 1024, 64, 128) == 2000 * (2**31 - 1024) * 64 * 520
+    most = 2**31 - 1024
+    assert L.fsp_attention_tree_by_tokens_workspace(2000, most, 64, 128) == 2000 * most * 64 * 520
     for most in (0, -1, 4):
         assert L.fsp_attention_tree_by_tokens(base._cache() + _tree(), most, None) == -1
     assert L.fsp_attention_tree_by_tokens(None, 1, None) == -1
@@ -204,7 +205,8 @@ def test_counted_keep_refusals_of_the_library():
     assert call(None, 16, 16, None) == -1 and call(c + c + _keep(other=0), 16, 16, None) == -1
     for first, counts in ((None, 16), (16, None)):
         assert call(c + c + _keep(other=1), first, counts, None) == -1
-    for kw in ({"tokens": -1}, {"keep": 0}, {"lengths": 0}, {"kept": 0}, {"pieces": 0}, {"n_pieces": 1}, {"piece": 200}):
+    for kw in ({"tokens": -1}, {"keep": 0}, {"lengths": 0}, {"kept": 0}, {"pieces": 0}, {"n_pieces": 1},
+               {"piece": 200}):
         assert call(c + c + _keep(**({"other": 1} | kw)), 16, 16, None) == -1
 
 
