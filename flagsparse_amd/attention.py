@@ -329,6 +329,7 @@ def _tree_ways(kv_heads, group):
 
 
 def _piece_of(rooms, sight, each, slots, most, rows):
+    """The size of a piece for one way: see _pieces_of."""
     return _pieces_of(rooms, sight, ((each, rows),), slots, most)[0]
 
 

@@ -106,7 +106,8 @@ __global__ __launch_bounds__(kThreads) void paged_keep_kernel(
   if (which == 0 && threadIdx.x == 0) kept[b] = m.ok ? m.past + stay : -1;
 }
 
-// How many marks of a sequence's places [from, to), which are not all marked ones, stay: the same in all threads.
+// How many of a sequence's places [from, to) stay, the ``past`` before the marked ones among them: the same in all
+// threads.
 __device__ __forceinline__ int kept_in(const uint8_t* marks, int past, int from, int to) {
   __shared__ int s_count[kThreads / kWave];
   int count = 0;
@@ -118,7 +119,7 @@ __device__ __forceinline__ int kept_in(const uint8_t* marks, int past, int from,
   return s_count[0] + s_count[1] + s_count[2] + s_count[3];
 }
 
-// How many tokens of each piece stay: counts[the piece's place among those of its sequence, after the ones before].
+// How many tokens of each piece stay, by the slot of its sequence's first one and its place in the sequence.
 __global__ __launch_bounds__(kThreads) void paged_keep_count_kernel(
     KeepShape s, const Piece* __restrict__ pieces, int piece_size, const uint8_t* __restrict__ keep,
     const int32_t* __restrict__ tokens, const int32_t* __restrict__ lengths, int32_t* __restrict__ counts) {
@@ -165,7 +166,7 @@ __global__ __launch_bounds__(kThreads) void paged_keep_before_kernel(
 // Into other pages: a workgroup takes kSpan of a sequence's tokens, all heads of their keys and values.  How many
 // tokens stay before them, and of all, it counts itself, four marks to a word; or, COUNTED, has two launches before
 // it count by pieces, as what all workgroups count grows with the square of the marks.  Bound by memory where heads
-// are large: half of 16 sequences of 8192, 8 heads of 128, 537 MB in 110 to 124 us, 4.3 to 4.9 TB/s, of 4 of 131072
+// are large: half of 16 sequences of 8192, 8 heads of 128, 537 MB in 110 to 125 us, 4.3 to 4.9 TB/s, of 4 of 131072
 // 2147 MB in 430 us, 5.0 TB/s, where a plain copy has 4.7 to 4.9; one of 2^20 tokens, one head of 64, 268 MB in 112 us:
 // a workgroup moves 16 KB after its chain of loads.  A workgroup to a head of 1024 tokens, whose rows of 256 bytes
 // lie apart, took 155 us for the first.
