@@ -22,7 +22,6 @@ the calls with ``prepared=`` neither check them again nor wait: they can be capt
 """
 
 import functools
-import math
 import struct
 
 import numpy as np
@@ -319,13 +318,21 @@ class PreparedPagedKV:
 @functools.lru_cache(maxsize=64)
 def _tree_ways(kv_heads, group):
     """How the pieces of a tree call may be gone through, whatever its numbers of drafted tokens: (workgroups of a
-    piece, rows of each), tiles by powers of two."""
+    piece, rows of each)."""
     L = _abi.lib()
     tiles = {}
     for longest in range(1, int(L.fsp_attention_tree_drafts()) + 1):
         rows = int(L.fsp_attention_tree_rows(group, longest))
         tiles[rows] = max(tiles.get(rows, 1), -(-group * longest // rows))
-    return tuple((kv_heads << i, rows) for rows, n in sorted(tiles.items()) for i in range((n - 1).bit_length() + 1))
+    return tuple((kv_heads * n, rows) for rows, most in sorted(tiles.items())
+                 for n in sorted({_near(n) for n in range(1, most + 1)}))
+
+
+def _near(n):
+    """A number of tiles or one close to it, by quarters of powers of two from 8 on.  By powers of two alone five tiles
+    are sized as four: 4 sequences of 30000, 100 drafted tokens, 6 heads of 128 over 1 71 us, 58 so."""
+    step = 1 << max(0, n.bit_length() - 3)
+    return (n + step // 2) // step * step
 
 
 def _piece_of(rooms, sight, each, slots, most, rows):
@@ -352,14 +359,16 @@ def _pieces_of(rooms, sight, ways, slots, most):
         whole = seen // piece
         rest = seen - whole * piece
         rest = np.sort(rest[rest > 0])[::-1]
-        wholes, rests = int(whole.sum()), len(rest)
+        wholes, rests, few = int(whole.sum()), len(rest), rest.tolist()
         for i, (each, rows) in enumerate(ways):
             around, count = 100 + 2 * rows, wholes * each
             starts = max(1, -(-(count + each * rests) // slots))  # rounds, and those that start with whole pieces
             full = min(starts, -(-count // slots)) if rests else starts
-            first = piece if full else int(rest[0])
+            first = piece if full else few[0]
             rounds = full * piece + starts * around
-            if full < starts:
+            if starts - full < 32:
+                rounds += sum([few[(i * slots - count) // each] for i in range(full, starts)])
+            else:
                 rounds += int(rest[(np.arange(full, starts) * slots - count) // each].sum())
             total = each * (tokens + around * (wholes + rests))
             best[i] = min(best[i], (rounds + max(total / slots, float(first + around)), piece))
@@ -906,9 +915,9 @@ def flagsparse_attention_paged_tree(q, lengths, token_indptr=None, *, parents=No
         sight = min(past + first + most, _TOKENS_CAP) if past else 0
         group = heads // kv.kv_heads
         of = int(_abi.lib().fsp_attention_tree_rows(group, longest))
-        # tiles of an average sequence, as those of the longest trees are few, to a power of two
+        # tiles of an average sequence, as those of the longest trees are few
         tiles = min(-(-group * longest // of), 1 + group * tokens // (kv.batch * of))
-        way = (kv.kv_heads << round(math.log2(tiles)), of)
+        way = (kv.kv_heads * _near(tiles), of)
         piece, pieces, firsts, longest_list, marked = kv._list(
             sight, 512, 8192, (way,) if prepared is None else _tree_ways(kv.kv_heads, group), way)
         n_pieces, need, room, by_tokens = pieces.shape[0], 0, None, 0
