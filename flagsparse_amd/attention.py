@@ -926,7 +926,7 @@ def flagsparse_attention_paged_tree(q, lengths, token_indptr=None, *, parents=No
                                                             group, longest))
             size = int(_abi.lib().fsp_attention_tree_workspace(n_pieces, heads, kv.dim, longest))
             less = int(_abi.lib().fsp_attention_tree_by_tokens_workspace(longest_list, tokens, heads, kv.dim))
-            if less < size:
+            if 2 * less < size:
                 by_tokens, size = longest_list, less
             room = _like((size,), torch.uint8, dev)
         head = kv._packed() + _TREE.pack(

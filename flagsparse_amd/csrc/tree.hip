@@ -20,7 +20,8 @@ constexpr int kTableKeys = 1024;  // keys whose places LDS holds at a time
 struct TreeShape {
   int heads, window, sinks, piece, n_pieces, n_tokens, longest, tiles;
   float scale;
-  int by_tokens;  // how partial sums lie: see Sums
+  int by_tokens;  // how partial sums lie, and how far the rows of a piece behind those of the one before: see Sums
+  int64_t step;
 };
 
 // A sequence's drafted tokens and what of its keys any of them sees: the places [first, last), where
@@ -42,18 +43,15 @@ struct Drafted {
   __device__ int pieces_end(int piece) const { return last / piece + (last % piece > 0); }
 };
 
-// Where the partial sums of a sequence's rows for one key head start, and how many rows one piece's lie behind those
-// of the piece before.  By pieces, ``longest`` tokens' rows each, or by tokens, all rows of the call for each piece
-// that a sequence has at most: the caller takes the smaller.  Where most sequences have fewer drafted tokens than
-// ``longest``, or no bound is given, that is the second: 64 sequences with room for 131072 tokens and 8 drafted
-// ones each, 32 heads of 128, 136 MB instead of 4.4 GB (pieces of 8192).
-struct Sums {
-  int64_t first, step;
-  __device__ Sums(const TreeShape& s, const Drafted& t, int slot, int g, int group)
-      : first(s.by_tokens ? (int64_t)t.begin * s.heads + (int64_t)g * t.count * group
-                          : (int64_t)slot * s.longest * s.heads + (int64_t)g * s.longest * group),
-        step((int64_t)(s.by_tokens ? s.n_tokens : s.longest) * s.heads) {}
-};
+// Where the partial sums of a sequence's rows for one key head start.  By pieces, ``longest`` tokens' rows each, or by
+// tokens, all rows of the call for each piece that a sequence has at most: the caller takes that where it is less than
+// half as much.  It is where most sequences have fewer drafted tokens than ``longest``, or no bound is given: 64
+// sequences with room for 131072 tokens and 8 drafted ones each, 32 heads of 128, 136 MB instead of 4.4 GB (pieces of
+// 8192).
+__device__ __forceinline__ int64_t sums_at(const TreeShape& s, const Drafted& t, int slot, int g, int group) {
+  const int64_t token = s.by_tokens ? t.begin : (int64_t)slot * s.longest;
+  return token * s.heads + g * ((s.by_tokens ? t.count : s.longest) * group);
+}
 
 // Rows of NaN for the tokens [from, to), those of one key head's queries.
 template <typename T>
@@ -381,8 +379,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attention_tree_kernel(
 
   // join the waves, 16 rows at a time
   const bool split = p1 - p0 > 1;
-  const Sums sums(s, t, pc.slot, g, group);
-  const int64_t slot = sums.first + (mine - p0) * sums.step;
+  const int64_t first = sums_at(s, t, pc.slot, g, group), slot = first + (mine - p0) * s.step;
   auto to_out = [&](int r, int d, f32x4 y, float most, float total) {
     const int64_t token = t.begin + (r0 + r) / group;
     const int head = head0 + (r0 + r) % group;
@@ -435,7 +432,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attention_tree_kernel(
   if constexpr (RT > 1) return;
   if (!split || !arrived) return;  // without counts, another launch joins them
   if (last_to_arrive(arrived + ((int64_t)b * c.kv_heads + g) * s.tiles + tile, p1 - p0))
-    join_tile<T, DP>(part_o, part_ml, sums.first + r0, sums.step, p1 - p0, min(ROWS, rows - r0), c.dim, to_out);
+    join_tile<T, DP>(part_o, part_ml, first + r0, s.step, p1 - p0, min(ROWS, rows - r0), c.dim, to_out);
 }
 
 // Rows past a head's dim are read from here.
@@ -639,8 +636,7 @@ __global__ __launch_bounds__(256, 2) void attention_tree_wide_kernel(
     store_rows<T, NT>(out + token * out_token + head * out_head, o, sum == 0 ? 0.0f : 1.0f / sum, c.dim, half);
     return;
   }
-  const Sums sums(s, t, pc.slot, g, group);
-  const int64_t at = sums.first + (mine - p0) * sums.step + row;
+  const int64_t at = sums_at(s, t, pc.slot, g, group) + (mine - p0) * s.step + row;
   store_rows<float, NT>(part_o + at * c.dim, o, 1.0f, c.dim, half);
   if (half == 0)
     *reinterpret_cast<f32x2*>(part_ml + 2 * at) = f32x2{top == -INFINITY ? -INFINITY : top * cs, sum};
@@ -663,8 +659,7 @@ __global__ __launch_bounds__(256) void attention_tree_join_kernel(
   const Drafted t(s, tokens, b, lengths[b], (c.indptr[b + 1] - c.indptr[b]) * c.page_size);
   const int p0 = t.first / s.piece, n = t.pieces_end(s.piece) - p0;
   if (n < 2 || g >= c.kv_heads || r >= t.count * group) return;
-  const Sums sums(s, t, first_piece[b], g, group);
-  const int64_t step = sums.step, at = sums.first + r;
+  const int64_t step = s.step, at = sums_at(s, t, first_piece[b], g, group) + r;
   const f32x2* ml = part_ml + at;
   const float* o = part_o + at * c.dim + (d < c.dim ? d : 0);
   float most = -INFINITY, total = 0;
@@ -732,7 +727,7 @@ int launch_tree(const TreeCall& a, Kernel kernel, hipStream_t st, More... more) 
   const int64_t tiles = tiles_of(a.longest, a.heads / a.cache.kv_heads);
   const TreeShape s{(int)a.heads,    (int)a.window,  (int)a.sinks, (int)a.piece,  (int)a.n_pieces,
                     (int)a.n_tokens, (int)a.longest, (int)tiles,   (float)a.scale,
-                    a.most > 0};
+                    a.most > 0,      (a.most ? a.n_tokens : a.longest) * a.heads};
   float* part_o = static_cast<float*>(a.workspace);
   float* part_ml = part_o + (a.most ? a.most * a.n_tokens : a.n_pieces * a.longest) * a.heads * a.cache.dim;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(a.n_pieces * a.cache.kv_heads * tiles)), dim3(256), 0, st,
